@@ -1,0 +1,312 @@
+"""Rows of activations in 8 bits, and matrix products over 8-bit and 4-bit weights.
+
+A row in 8 bits is e4m3 numbers q [K] with one float32 scale s; it stands for q * s.  `add_rmsnorm8`
+and `glu8` make such rows (s: the row's largest magnitude over 448), `linear8` multiplies them by
+weights that are kept the same way, a scale per output feature (`Weights8`).
+
+`linear4` multiplies float32 or bfloat16 rows by 4-bit weights (`Weights4`): (code - 8) * group scale *
+feature scale, codes 0..15, the group scales e4m3, the feature scales float32.  (code - 8) times an
+e4m3 number has at most seven significant bits, so the tensor cores take the weights as they are, in
+bfloat16 without a rounding; float32 rows go through them as three bfloat16 parts that add up to the row
+exactly.  Sums are float32 in every product, and only the result is rounded.
+
+Everything here launches on torch's current stream of the tensors' device, keeps no buffer between
+calls and may be captured into a CUDA graph (a call that has to bring rows into another layout first
+allocates from torch's pool, as any captured torch operation does).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import KernelError, _check, _code, _need_cuda, _ptr, _stream, build
+
+for _name in ("rows8", "linear_quantized_few"):
+    build.register_module(_name, ["common.cuh"])
+
+E4M3 = torch.float8_e4m3fn
+TOP = 448.0                      # the largest e4m3 number
+LEAST = 1e-30                    # a row's largest magnitude counts as this much at least
+_FOUR_BF16, _FOUR_F32, _EIGHT = 0, 1, 2
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+class _Device:
+    """Makes the tensors' device the current one for a launch, where it is not."""
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.device.index
+        self.before = None
+
+    def __enter__(self):
+        now = torch._C._cuda_getDevice()
+        if now != self.index:
+            self.before = now
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
+def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"the tensors lie on {first.device} and {t.device}")
+
+
+def _rows(t: torch.Tensor, what: str, dtypes, shape=None) -> None:
+    """Rows that a kernel walks: 2-D, of a dtype it takes, each row's elements side by side."""
+    if t.dim() != 2 or t.dtype not in dtypes or (shape is not None and tuple(t.shape) != shape):
+        names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+        want = f" {list(shape)}" if shape is not None else ""
+        raise KernelError(f"{what}: {names} rows{want} are taken, got {t.dtype} {list(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise KernelError(f"{what}: rows must be contiguous")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise KernelError(f"{what}: rows must not overlap")
+
+
+def _vector(t: torch.Tensor, what: str, size: int) -> None:
+    if t.dtype != torch.float32 or tuple(t.shape) != (size,) or (size > 1 and t.stride(0) != 1):
+        raise KernelError(f"{what}: a contiguous float32 vector [{size}] is taken, got {t.dtype} {list(t.shape)}")
+
+
+def new_rows8(rows: int, width: int, device) -> torch.Tensor:
+    """Uninitialised e4m3 rows [rows, width] that begin a multiple of 16 bytes apart, as `linear8` takes
+    them without a copy."""
+    return torch.empty(rows, (width + 15) // 16 * 16, dtype=torch.uint8, device=device).view(E4M3)[:, :width]
+
+
+# ---------------------------------------------------------------------------
+# rows in 8 bits
+# ---------------------------------------------------------------------------
+
+def add_rmsnorm8(x: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.Tensor, eps: float, out: torch.Tensor,
+                 scales: torch.Tensor, sum_out: Optional[torch.Tensor] = None) -> None:
+    """x + delta, its RMS norm, and that in 8 bits: y = sum / sqrt(mean(sum^2) + eps) * gain goes to `out`
+    (e4m3 [T, W]) and `scales` (float32 [T]).  `x`: the float32 residual; `delta`: float32 or bfloat16 rows
+    to add to it, or None.  The sum goes to `sum_out`, which is `x` itself if a delta is given and
+    nothing else is said (without either, `x` is only read)."""
+    _rows(x, "add_rmsnorm8 input", (torch.float32,))
+    rows, width = x.shape
+    if delta is not None:
+        _rows(delta, "add_rmsnorm8 delta", _FLOATS, (rows, width))
+        if sum_out is None:
+            sum_out = x
+    if sum_out is not None:
+        _rows(sum_out, "add_rmsnorm8 sum", (torch.float32,), (rows, width))
+    _vector(gain, "add_rmsnorm8 gain", width)
+    _rows(out, "add_rmsnorm8 output", (E4M3,), (rows, width))
+    _vector(scales, "add_rmsnorm8 scales", rows)
+    _need_cuda(x, delta, gain, out, scales, sum_out)
+    _one_device(x, delta, gain, out, scales, sum_out)
+    lib = build.load("rows8")
+    with _Device(x):
+        code = lib.cb_norm8(_ptr(x), x.stride(0), _ptr(delta), _code(delta.dtype) if delta is not None else 0,
+                            delta.stride(0) if delta is not None else 0, _ptr(gain), eps, _ptr(sum_out),
+                            sum_out.stride(0) if sum_out is not None else 0, _ptr(out), out.stride(0), _ptr(scales),
+                            rows, width, _stream())
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"add_rmsnorm8 takes rows of 1 to {lib.cb_rows8_widest()} features, got {width}")
+    _check(code, "add_rmsnorm8")
+
+
+def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Optional[float] = None,
+         alpha: float = 1.0, offset: float = 0.0) -> None:
+    """The gated pair of rows [g: F | u: F] in 8 bits: `out` (e4m3 [T, F]) and `scales` (float32 [T]).
+    `limit` None: silu(g) * u.  A number: the capped pair of `ops.glu`, g' sigmoid(alpha g') (u' + offset)
+    with g' = min(g, limit), u' = clamp(u, -limit, limit)."""
+    _rows(both, "glu8 input", _FLOATS)
+    rows, width = both.shape[0], both.shape[1] // 2
+    if both.shape[1] % 2:
+        raise KernelError(f"glu8 takes rows [g | u] of an even width, got {both.shape[1]}")
+    if limit is not None and not limit > 0:
+        raise KernelError("glu8: the limit must be positive")
+    _rows(out, "glu8 output", (E4M3,), (rows, width))
+    _vector(scales, "glu8 scales", rows)
+    _need_cuda(both, out, scales)
+    _one_device(both, out, scales)
+    lib = build.load("rows8")
+    with _Device(both):
+        code = lib.cb_glu8(_ptr(both), _code(both.dtype), both.stride(0), _ptr(out), out.stride(0), _ptr(scales),
+                           rows, width, limit if limit is not None else 0.0, alpha, offset, _stream())
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"glu8 takes 1 to {lib.cb_rows8_widest()} features, got {width}")
+    _check(code, "glu8")
+
+
+# ---------------------------------------------------------------------------
+# weights
+# ---------------------------------------------------------------------------
+
+def _aligned16(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0)
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements between rows (one row: as many as would do)."""
+    per = 16 // t.element_size()
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + per - 1) // per * per
+
+
+def _in_aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """The same values in rows that begin on multiples of 16 bytes."""
+    per = 16 // t.element_size()
+    wide = torch.empty(t.shape[0], (t.shape[1] + per - 1) // per * per, dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+    wide.copy_(t)
+    return wide
+
+
+class Weights8:
+    """A matrix [N, K] in 8 bits: e4m3 `values` [N, K], float32 `scales` [N]; weight (n, k) is
+    values[n, k] * scales[n].  Values whose rows do not begin on multiples of 16 bytes are copied into rows
+    that do, once, here."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        _rows(values, "8-bit weights", (E4M3,))
+        if values.shape[0] == 0 or values.shape[1] == 0:
+            raise KernelError(f"8-bit weights: an empty matrix {list(values.shape)}")
+        _vector(scales, "8-bit weights' scales", values.shape[0])
+        _one_device(values, scales)
+        self.values = values if _aligned16(values) else _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
+        self.scales = scales
+        self.shape = values.shape
+
+    @classmethod
+    def pack(cls, w: torch.Tensor) -> "Weights8":
+        """From a matrix of floating numbers: each row's largest magnitude becomes 448."""
+        w = _finite(w)
+        scales = w.abs().amax(dim=1).clamp_min(LEAST) / TOP
+        return cls((w / scales[:, None]).clamp(-TOP, TOP).to(E4M3), scales)
+
+    def dense(self) -> torch.Tensor:
+        """The float32 matrix that these weights stand for."""
+        return self.values.float() * self.scales[:, None]
+
+
+def _finite(w: torch.Tensor) -> torch.Tensor:
+    if w.dim() != 2 or not w.is_floating_point() or w.numel() == 0:
+        raise KernelError(f"weights are packed from a matrix of floating numbers, got {w.dtype} {list(w.shape)}")
+    w = w.float()
+    if not bool(torch.isfinite(w).all()):
+        raise KernelError("weights are packed from finite numbers")
+    return w
+
+
+# Code i of eight neighbouring k lies at this bit of their int32: even k in the low half, odd k in the high
+# half, so that masking one nibble of both halves gives the codes of two neighbouring k.
+CODE_SHIFTS = tuple(4 * (i // 2) + 16 * (i % 2) for i in range(8))
+
+
+class Weights4:
+    """A matrix [N, K] in 4 bits: weight (n, k) is (code - 8) * group_scales[n, k // group] * scales[n].
+    `codes`: int32 [N, K / 8], eight codes of neighbouring k a word at the bits `CODE_SHIFTS`;
+    `group_scales`: e4m3 [N, K / group] (`group` is read off the shapes: a multiple of 32 that divides K);
+    `scales`: float32 [N]."""
+
+    def __init__(self, codes: torch.Tensor, group_scales: torch.Tensor, scales: torch.Tensor):
+        _rows(codes, "4-bit weights' codes", (torch.int32,))
+        n, k = codes.shape[0], codes.shape[1] * 8
+        if n == 0 or k == 0:
+            raise KernelError(f"4-bit weights: an empty matrix [{n}, {k}]")
+        _rows(group_scales, "4-bit weights' group scales", (E4M3,))
+        groups = group_scales.shape[1]
+        if group_scales.shape[0] != n or groups == 0 or k % groups or (k // groups) % 32:
+            raise KernelError(f"4-bit weights: group scales [{n}, K / group] are taken, the group a multiple of 32 "
+                              f"that divides K = {k}, got {list(group_scales.shape)}")
+        _vector(scales, "4-bit weights' scales", n)
+        _one_device(codes, group_scales, scales)
+        self.codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
+            memory_format=torch.contiguous_format)
+        self.group_scales = group_scales.contiguous()
+        self.scales = scales
+        self.group = k // groups
+        self.shape = torch.Size((n, k))
+
+    @classmethod
+    def pack(cls, w: torch.Tensor, group: int = 64) -> "Weights4":
+        """From a matrix of floating numbers [N, K]: a group's largest magnitude becomes code 1 or 15 (before
+        its scale is rounded to e4m3; the codes are then the nearest for the scales as they are)."""
+        w = _finite(w)
+        n, k = w.shape
+        if group <= 0 or group % 32 or k % group:
+            raise KernelError(f"4-bit weights: a group is a multiple of 32 that divides K = {k}, got {group}")
+        parts = w.view(n, k // group, group)
+        want = parts.abs().amax(dim=2) / 7
+        scales = want.amax(dim=1).clamp_min(LEAST) / TOP
+        # (no group's scale may round to zero: the smallest number above it is 2^-9)
+        group_scales = (want / scales[:, None]).clamp(2.0 ** -9, TOP).to(E4M3)
+        step = group_scales.float() * scales[:, None]
+        codes = (torch.round(parts / step[:, :, None]).clamp(-8, 7) + 8).to(torch.int32).view(n, k // 8, 8)
+        words = torch.zeros(n, k // 8, dtype=torch.int32, device=w.device)
+        for i, shift in enumerate(CODE_SHIFTS):
+            words |= codes[:, :, i] << shift
+        return cls(words, group_scales, scales)
+
+    def dense(self) -> torch.Tensor:
+        """The float32 matrix that these weights stand for."""
+        n, k = self.shape
+        shifts = torch.tensor(CODE_SHIFTS, dtype=torch.int32, device=self.codes.device)
+        codes = ((self.codes[:, :, None] >> shifts) & 15) - 8
+        grouped = codes.float().view(n, -1, self.group) * self.group_scales.float()[:, :, None]
+        return grouped.view(n, k) * self.scales[:, None]
+
+
+# ---------------------------------------------------------------------------
+# products: out[M, N] = rows[M, K] . W[N, K]^T (+ add)
+# ---------------------------------------------------------------------------
+
+def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) -> None:
+    _rows(out, f"{what} output", _FLOATS, shape)
+    if add is not None:
+        _rows(add, f"{what} add", (torch.float32,), shape)
+
+
+def _product(kind: int, rows, row_scales, values, ldw: int, group_scales, w, group: int, out, add, what: str) -> None:
+    m, (n, k) = rows.shape[0], w.shape
+    if m == 0:
+        return
+    lib = build.load("linear_quantized_few")
+    with _Device(rows):
+        code = lib.cb_linear_quantized_few(
+            kind, _ptr(rows), _pitch(rows), _ptr(row_scales), _ptr(values), ldw, _ptr(group_scales), _ptr(w.scales),
+            _ptr(add), add.stride(0) if add is not None else 0, _ptr(out), _code(out.dtype), out.stride(0), m, n, k,
+            group, _stream())
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"{what}: sizes out of range: rows {list(rows.shape)}, weights {list(w.shape)}")
+    _check(code, what)
+
+
+def linear8(rows: torch.Tensor, row_scales: torch.Tensor, w: Weights8, out: torch.Tensor,
+            add: Optional[torch.Tensor] = None) -> None:
+    """out = (rows * row_scales) . W^T (+ add): e4m3 `rows` [M, K], float32 `row_scales` [M]; `out`: float32
+    or bfloat16 [M, N]; `add`: float32 [M, N], which may be `out`."""
+    if not isinstance(w, Weights8):
+        raise KernelError(f"linear8 takes Weights8, got {type(w).__name__}")
+    n, k = w.shape
+    _rows(rows, "linear8 rows", (E4M3,), (rows.shape[0], k))
+    _vector(row_scales, "linear8 row scales", rows.shape[0])
+    _out_rows(out, add, (rows.shape[0], n), "linear8")
+    _need_cuda(rows, row_scales, w.values, out, add)
+    _one_device(rows, row_scales, w.values, out, add)
+    if not _aligned16(rows):
+        rows = _in_aligned_rows(rows.view(torch.uint8)).view(E4M3)
+    _product(_EIGHT, rows, row_scales, w.values, _pitch(w.values), None, w, 0, out, add, "linear (8-bit weights)")
+
+
+def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch.Tensor] = None) -> None:
+    """out = a . W^T (+ add): float32 or bfloat16 rows `a` [M, K]; `out`: float32 or bfloat16 [M, N]; `add`:
+    float32 [M, N], which may be `out`."""
+    if not isinstance(w, Weights4):
+        raise KernelError(f"linear4 takes Weights4, got {type(w).__name__}")
+    n, k = w.shape
+    _rows(a, "linear4 rows", _FLOATS, (a.shape[0], k))
+    _out_rows(out, add, (a.shape[0], n), "linear4")
+    _need_cuda(a, w.codes, out, add)
+    _one_device(a, w.codes, out, add)
+    if not _aligned16(a):
+        a = _in_aligned_rows(a)
+    _product(_FOUR_F32 if a.dtype == torch.float32 else _FOUR_BF16, a, None, w.codes, k // 2, w.group_scales, w,
+             w.group, out, add, "linear (4-bit weights)")

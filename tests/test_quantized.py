@@ -1,0 +1,115 @@
+"""The quantised operators' host side: packed weights and what is refused (no kernel runs)."""
+import pytest
+import torch
+
+from crucible_b200.ops import KernelError, quantized
+from quantized_cases import E4M3, dense4, dense8, random_rows8, random_weights4, random_weights8
+
+
+def _gen():
+    return torch.Generator().manual_seed(7)
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (5, 96, 32), (7, 192, 96), (16, 256, 64), (3, 1024, 128), (4, 160, 160)])
+def test_pack4_keeps_weights_within_half_a_step(n, k, group):
+    w = torch.randn(n, k, generator=_gen()) * 0.02
+    w[0, :group] = 0.0                                 # a group of zeros
+    p = quantized.Weights4.pack(w, group)
+    assert p.shape == (n, k) and p.group == group
+    assert torch.equal(p.dense().double(), dense4(p).float().double()) or \
+        torch.allclose(p.dense().double(), dense4(p), rtol=2.0 ** -22, atol=0)
+    step = p.group_scales.double().repeat_interleave(group, 1) * p.scales.double()[:, None]
+    # 7 steps reach the largest; its scale may round down by half a step of e4m3, 2^-4: 7.47 steps, code 15
+    assert ((w.double() - dense4(p)).abs() <= step * (0.5 + 1e-5)).all()
+    assert (dense4(p)[0, :group] == 0).all()
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 17), (16, 256)])
+def test_pack8_rounds_to_nearest(n, k):
+    w = torch.randn(n, k, generator=_gen()) * 0.02
+    w[n // 2] = 0.0
+    p = quantized.Weights8.pack(w)
+    assert p.values.stride(0) % 16 == 0 or n == 1
+    assert ((w.double() - dense8(p)).abs() <= w.double().abs() * (2.0 ** -4 + 1e-6) + p.scales.double()[:, None] * 2.0 ** -10).all()
+    assert torch.allclose(p.dense().double(), dense8(p), rtol=2.0 ** -23, atol=0)
+
+
+def test_codes_lie_where_they_are_said_to():
+    w = torch.arange(-8, 0).float().repeat(4)[None]     # codes 0..7, four times
+    p = quantized.Weights4(torch.tensor([[0, 0, 0, 0]], dtype=torch.int32), torch.ones(1, 1).to(E4M3), torch.ones(1))
+    assert (p.dense() == -8).all()
+    word = sum(i << s for i, s in enumerate(quantized.CODE_SHIFTS))
+    p = quantized.Weights4(torch.tensor([[word] * 4], dtype=torch.int32), torch.ones(1, 1).to(E4M3), torch.ones(1))
+    assert torch.equal(p.dense(), w)
+
+
+def test_rows_of_new_rows8_begin_on_16_bytes():
+    for width in (1, 15, 16, 17, 100):
+        q = quantized.new_rows8(3, width, "cpu")
+        assert q.shape == (3, width) and q.dtype == E4M3 and q.stride(0) % 16 == 0
+
+
+def _refused(match, fn, *args, **kw):
+    with pytest.raises(KernelError, match=match):
+        fn(*args, **kw)
+
+
+def test_weights_that_are_refused():
+    ok = torch.zeros(4, 8, dtype=torch.int32)
+    one = torch.ones(4)
+    for groups in (3, 5, 64):
+        _refused("group", quantized.Weights4, ok, torch.ones(4, groups).to(E4M3), one)
+    _refused("group scales", quantized.Weights4, ok, torch.ones(4, 2), one)
+    _refused("codes", quantized.Weights4, ok.long(), torch.ones(4, 2).to(E4M3), one)
+    _refused("float32 vector", quantized.Weights4, ok, torch.ones(4, 2).to(E4M3), one.double())
+    _refused("float32 vector", quantized.Weights4, ok, torch.ones(4, 2).to(E4M3), torch.ones(5))
+    _refused("empty", quantized.Weights4, ok[:0], torch.ones(0, 2).to(E4M3), one[:0])
+    _refused("empty", quantized.Weights8, torch.zeros(4, 0).to(E4M3), one)
+    _refused("8-bit weights", quantized.Weights8, torch.zeros(4, 8, dtype=torch.uint8), one)
+    _refused("finite", quantized.Weights8.pack, torch.tensor([[1.0, float("nan")]]))
+    _refused("finite", quantized.Weights4.pack, torch.full((2, 32), float("inf")), 32)
+    for group in (0, 16, 48, 33, 64):
+        _refused("group", quantized.Weights4.pack, torch.ones(2, 96), group)
+
+
+def test_calls_that_are_refused():
+    g = _gen()
+    x, q, s = torch.zeros(3, 20), quantized.new_rows8(3, 20, "cpu"), torch.zeros(3)
+    gain = torch.ones(20)
+    norm = quantized.add_rmsnorm8
+    _refused("CUDA device", norm, x, None, gain, 1e-5, q, s)               # all is well but the device
+    _refused("input", norm, x.bfloat16(), None, gain, 1e-5, q, s)
+    _refused("delta", norm, x, torch.zeros(3, 19), gain, 1e-5, q, s)
+    _refused("delta", norm, x, torch.zeros(3, 20).half(), gain, 1e-5, q, s)
+    _refused("overlap", norm, x, torch.zeros(1, 20).expand(3, 20), gain, 1e-5, q, s)
+    _refused("gain", norm, x, None, torch.ones(21), 1e-5, q, s)
+    _refused("output", norm, x, None, gain, 1e-5, q[:2], s)
+    _refused("output", norm, x, None, gain, 1e-5, torch.zeros(3, 20), s)
+    _refused("scales", norm, x, None, gain, 1e-5, q, s[:2])
+    _refused("sum", norm, x, None, gain, 1e-5, q, s, sum_out=x.bfloat16())
+    _refused("contiguous", norm, torch.zeros(20, 3).t(), None, gain, 1e-5, q, s)
+    both = torch.zeros(3, 40)
+    _refused("CUDA device", quantized.glu8, both, q, s)
+    _refused("even", quantized.glu8, torch.zeros(3, 41), q, s)
+    _refused("limit", quantized.glu8, both, q, s, 0.0)
+    _refused("limit", quantized.glu8, both, q, s, float("nan"))
+    _refused("output", quantized.glu8, torch.zeros(3, 42), q, s)
+
+    w8, w4 = random_weights8(6, 64, "cpu", g), random_weights4(6, 64, 32, "cpu", g)
+    rows, scales = random_rows8(3, 64, "cpu", g)
+    out = torch.zeros(3, 6)
+    _refused("CUDA device", quantized.linear8, rows, scales, w8, out)
+    _refused("Weights8", quantized.linear8, rows, scales, w4, out)
+    _refused("rows", quantized.linear8, rows[:, :63], scales, w8, out)
+    _refused("rows", quantized.linear8, torch.zeros(3, 64), scales, w8, out)
+    _refused("row scales", quantized.linear8, rows, scales[:2], w8, out)
+    _refused("output", quantized.linear8, rows, scales, w8, torch.zeros(3, 7))
+    _refused("output", quantized.linear8, rows, scales, w8, out.half())
+    _refused("overlap", quantized.linear8, rows, scales, w8, torch.zeros(6).expand(3, 6))
+    _refused("add", quantized.linear8, rows, scales, w8, out, add=out.bfloat16())
+    a = torch.zeros(3, 64)
+    _refused("CUDA device", quantized.linear4, a, w4, out)
+    _refused("Weights4", quantized.linear4, a, w8, out)
+    _refused("rows", quantized.linear4, a.half(), w4, out)
+    _refused("rows", quantized.linear4, torch.zeros(3, 32), w4, out)
+    _refused("add", quantized.linear4, a, w4, out, add=torch.zeros(2, 6))
