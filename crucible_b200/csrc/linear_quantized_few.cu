@@ -11,39 +11,16 @@
 // product does not see the order of k, so a thread takes 16 neighbouring bytes of a feature's
 // weights and the same k of its row of the step, whatever k the instruction calls them.
 //
-// Four bits.  (code - 8) * scale has at most 3 + 4 significant bits, so it is a bf16 number and the
-// tensor cores multiply the weights themselves: code bits put into the mantissa of 16 are 16 + code,
-// and one fused multiply-add, (16 + code) scale - 24 scale, is exact (24 scale has 2 + 4 significant bits).
-// fp32 rows are the sum of three bf16 numbers exactly (the 24 bits of the mantissa, 8 by 8), each
-// of which meets the weights: the products are exact and only fp32 sums are rounded.
-//
 // A block owns 16 features and 8 rows; its warps take segments of K in turn and their sums are added
 // in the warps' order, so the order of a dot product's sum depends on K alone.
-#include "common.cuh"
+#include "quantized.cuh"
 
 namespace {
-
-enum Kind { FOUR_BF16 = 0, FOUR_F32 = 1, EIGHT = 2 };
 
 constexpr int WARPS = 8;
 constexpr int FEATURES = 16;            // a block
 constexpr int ROWS = 8;
 constexpr int BATCH = 2;                // segments of weights a warp has in flight
-
-struct Args {
-    const void* rows;                   // bf16, fp32 or e4m3 [M, ldr elements]
-    long long ldr;
-    const float* row_scale;             // EIGHT: [M]
-    const void* w;                      // int32 [N, K / 8], or e4m3 [N, ldw]
-    long long ldw;
-    const uint8_t* group_scale;         // e4m3 [N, K / group]
-    const float* feature_scale;         // [N]
-    const float* add;                   // fp32 [M, lda] or null
-    long long lda;
-    void* out;                          // [M, ldo]
-    long long ldo;
-    int M, N, K, group, out_bf16;
-};
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -59,48 +36,8 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// An e4m3 scale as a pair of equal bf16 numbers, and -24 times it: both exact.
-__device__ __forceinline__ void scale_pairs(uint8_t e4m3, uint32_t& s2, uint32_t& c2) {
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)e4m3));
-    float s;
-    asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.f32.f16 %0, lo;\n\t}" : "=f"(s) : "r"(h2));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s2) : "f"(s));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(c2) : "f"(-24.f * s));
-}
-
-// Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.
-__device__ __forceinline__ uint32_t weight_pair(uint32_t word, int i, uint32_t s2, uint32_t c2) {
-    const uint32_t put = i == 0 ? word << 3 : word >> (4 * i - 3);
-    const uint32_t magic = (put & 0x00780078u) | 0x41804180u;       // 16 + code, twice
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(magic), "r"(s2), "r"(c2));
-    return r;
-}
-
-// Two fp32 numbers as three pairs of bf16 whose sum they are.  (Cut, not rounded: 8 bits at a time, and what
-// is left is exact.  An infinity or a NaN stands in the first pair alone.)
-__device__ __forceinline__ void three_parts(float x, float y, uint32_t (&p)[3]) {
-    float v[2] = {x, y};
-    uint32_t part[2][3];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t bits = __float_as_uint(v[i]);
-        const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
-        const float first = __uint_as_float(bits & 0xFFFF0000u);
-        const float rest = finite ? v[i] - first : 0.f;
-        const float second = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
-        const float third = rest - second;
-        part[i][0] = finite || (bits & 0x007FFFFFu) == 0 ? bits >> 16 : 0x7FC0u;
-        part[i][1] = __float_as_uint(second) >> 16;
-        part[i][2] = __float_as_uint(third) >> 16;
-    }
-#pragma unroll
-    for (int j = 0; j < 3; ++j) p[j] = part[0][j] | (part[1][j] << 16);
-}
-
 template <int KIND>
-__global__ void __launch_bounds__(WARPS * 32) linear_few_kernel(const Args p) {
+__global__ void __launch_bounds__(WARPS * 32) linear_few_kernel(const QuantizedArgs p) {
     constexpr int SEG = KIND == EIGHT ? 64 : 128;       // k of a segment: 64 bytes of a feature's weights
     constexpr int MINE = SEG / 4;                       // k of a thread: 16 bytes
     __shared__ float sums[WARPS][FEATURES][ROWS + 1];
@@ -119,7 +56,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear_few_kernel(const Args p) {
     const int groups = KIND == EIGHT ? 0 : K / p.group;
     const uint8_t* s0 = p.group_scale + (long long)f0 * groups;
     const uint8_t* s1 = p.group_scale + (long long)f1 * groups;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
     const int segments = (K + SEG - 1) / SEG;
 
     // 16 e4m3 numbers from `at`; zeros beyond K, where a row may end inside them
@@ -196,12 +133,16 @@ __global__ void __launch_bounds__(WARPS * 32) linear_few_kernel(const Args p) {
                             three_parts(r.x, r.y, b0);
                             three_parts(r.z, r.w, b1);
 #pragma unroll
-                            for (int i = 2; i >= 0; --i) mma_bf16(acc, a[h], b0[i], b1[i]);
+                            for (int i = 0; i < 3; ++i) mma_bf16(i == 0 ? acc : rest, a[h], b0[i], b1[i]);
                         }
                     }
                 }
             }
         }
+    }
+    if constexpr (KIND == FOUR_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += rest[i];
     }
     sums[warp][g][2 * t] = acc[0], sums[warp][g][2 * t + 1] = acc[1];
     sums[warp][g + 8][2 * t] = acc[2], sums[warp][g + 8][2 * t + 1] = acc[3];
@@ -211,12 +152,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear_few_kernel(const Args p) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) v += sums[w][f][m];
-    v *= __ldg(p.feature_scale + n0 + f);
-    if (KIND == EIGHT) v *= __ldg(p.row_scale + m0 + m);
-    if (p.add != nullptr) v += p.add[(long long)(m0 + m) * p.lda + n0 + f];
-    const long long at = (long long)(m0 + m) * p.ldo + n0 + f;
-    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    else static_cast<float*>(p.out)[at] = v;
+    finish(p, v, KIND == EIGHT ? __ldg(p.row_scale + m0 + m) : 1.f, __ldg(p.feature_scale + n0 + f), m0 + m, n0 + f);
 }
 
 }  // namespace
@@ -232,7 +168,7 @@ CB_EXPORT int cb_linear_quantized_few(int kind, const void* rows, long long ldr,
     if (K <= 0 || (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
         (M + ROWS - 1) / ROWS > 65535 || (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;
-    const Args p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
+    const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
                     M, N, K, group, out_dtype == CB_BF16};
     const dim3 grid((N + FEATURES - 1) / FEATURES, (M + ROWS - 1) / ROWS), block(WARPS * 32);
     cudaStream_t s = (cudaStream_t)stream;

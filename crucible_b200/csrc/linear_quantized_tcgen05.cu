@@ -1,0 +1,447 @@
+// out[M,N] = rows[M,K] . W[N,K]^T over quantised weights on the 5th-generation tensor cores, for
+// more than a few rows.  128 features of W are the M side of the MMA (lanes of tensor memory) and up
+// to 256 rows its N side.
+//
+//   EIGHT      both operands e4m3, brought by TMA (128 k a stage), tcgen05.mma kind::f8f6f4
+//   FOUR_BF16  the codes come in by TMA, 256 k of 128 features a stage; four warps make bf16 weights
+//              of them (exact, see quantized.cuh), 64 k a stage of the MMA's ring, a feature a thread
+//   FOUR_F32   the same with three bf16 parts of every row side by side on the MMA's N side, which a
+//              kernel before this one has split: their sums lie in tensor memory apart and meet
+//              in the epilogue
+//
+// Few tiles: the blocks (x, y, 0..S-1) form a cluster that splits K.  Each leaves its sums in its own
+// shared memory, and each adds up a share of the rows from all of them, in the order of the
+// shares: no scratch memory, no atomics, the same sum every time.
+//
+// Roles: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor memory and
+// issues the MMAs, warps 2-5 make weights of codes and then run the epilogue, warp 6 sends the
+// copies of codes.
+#include "quantized.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+constexpr int FEATURES = 128;
+constexpr int THREADS = 224;
+constexpr int PACKED_K = 256;           // k of a stage of codes: 128 bytes a feature
+
+template <int KIND, int TOK> struct Sizes {
+    static constexpr int PARTS = KIND == FOUR_F32 ? 3 : 1;
+    static constexpr int BK = KIND == EIGHT ? 128 : 64;              // 128 bytes a row of either operand
+    static constexpr int A_BYTES = FEATURES * 128;
+    static constexpr int B_BYTES = PARTS * TOK * 128;
+    static constexpr int PACKED = KIND == EIGHT ? 0 : 2;             // stages of codes
+    // a block of up to 64 rows shares its SM with another; one of more has it to itself
+    static constexpr int ROOM = (TOK <= 64 && PARTS == 1) || TOK <= 32 ? 110 * 1024 : 220 * 1024;
+    static constexpr int FIT = (ROOM - PACKED * A_BYTES) / (A_BYTES + B_BYTES);
+    static constexpr int STAGES = FIT > 6 ? 6 : FIT;
+    static constexpr int N = PARTS * TOK;
+    static constexpr int TMEM = N <= 32 ? 32 : (N <= 64 ? 64 : (N <= 128 ? 128 : 256));
+};
+
+template <int KIND, int TOK> struct Storage {
+    using S = Sizes<KIND, TOK>;
+    alignas(1024) uint8_t a[S::STAGES][S::A_BYTES];
+    alignas(1024) uint8_t b[S::STAGES][S::B_BYTES];
+    alignas(1024) uint8_t codes[S::PACKED == 0 ? 1 : S::PACKED][S::PACKED == 0 ? 16 : S::A_BYTES];
+    alignas(8) uint64_t full[S::STAGES], empty[S::STAGES], codes_full[2], codes_empty[2], done;
+    uint32_t tmem;
+    int abort_flag;
+};
+
+__device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// kind::f8f6f4 with e4m3 A and B (format 0), K-major, fp32 sums
+__device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
+}
+
+template <int KIND, int TOK>
+__global__ void __launch_bounds__(THREADS)
+linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
+                      const QuantizedArgs p, int tok, int splits, int* __restrict__ status) {
+    using S = Sizes<KIND, TOK>;
+    extern __shared__ uint8_t smem_raw[];
+    Storage<KIND, TOK>& s = *reinterpret_cast<Storage<KIND, TOK>*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    cb_pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n0 = blockIdx.x * FEATURES, m0 = blockIdx.y * tok;
+    const uint32_t rank = splits > 1 ? tc::cluster_rank() : 0u;
+    // this block's share of K, in units of what comes in at once; the launcher keeps it from being empty
+    constexpr int UNIT = KIND == EIGHT ? S::BK : PACKED_K;
+    const int units = (p.K + UNIT - 1) / UNIT, per = (units + splits - 1) / splits;
+    const int k_begin = (int)rank * per * UNIT, k_end = min(p.K, k_begin + per * UNIT);
+    const int n_kb = (k_end - k_begin + S::BK - 1) / S::BK;
+    volatile int* abort_flag = &s.abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            tc::mbar_init(&s.full[i], KIND == EIGHT ? 1 : 5);        // (the copy, and four warps' weights)
+            tc::mbar_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < S::PACKED; ++i) {
+            tc::mbar_init(&s.codes_full[i], 1);
+            tc::mbar_init(&s.codes_empty[i], 4);
+        }
+        tc::mbar_init(&s.done, 1);
+        s.abort_flag = 0;
+        tc::fence_barrier_init();
+        tc::prefetch_tensormap(&map_rows);
+        tc::prefetch_tensormap(&map_w);
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(&s.tmem, S::TMEM);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (tc::elect_one()) {
+            int st = 0, sent = 0;
+            uint32_t parity = 1;
+            const uint32_t bytes = (KIND == EIGHT ? S::A_BYTES : 0) + S::PARTS * tok * 128;
+            for (int kb = 0; kb < n_kb; ++kb) {
+                if (kb >= S::STAGES && !tc::mbar_wait(&s.empty[st], parity, abort_flag)) {
+                    tc::give_up(abort_flag, status, tc::ST_PRODUCER_TIMEOUT);
+                    break;
+                }
+                tc::mbar_expect_tx(&s.full[st], bytes);
+                const int k = k_begin + kb * S::BK;
+                if constexpr (KIND == EIGHT) tc::tma_load_2d(s.a[st], &map_w, &s.full[st], k, n0);
+                if constexpr (KIND == FOUR_F32) tc::tma_load_3d(s.b[st], &map_rows, &s.full[st], k, m0, 0);
+                else tc::tma_load_2d(s.b[st], &map_rows, &s.full[st], k, m0);
+                sent = kb + 1;
+                if (++st == S::STAGES) st = 0, parity ^= 1;
+            }
+            if (*abort_flag) {
+                // our own copies land before the block's shared memory goes away.  (A stage's barrier may
+                // lack the arrivals of warps that gave up, so the bound is what ends this wait.)
+                for (int kb = max(0, sent - S::STAGES); kb < sent; ++kb)
+                    for (uint32_t i = 0; i < tc::WAIT_LIMIT; ++i)
+                        if (tc::mbar_try_wait(&s.full[kb % S::STAGES], (kb / S::STAGES) & 1)) break;
+            }
+        }
+    } else if (warp == 1) {
+        if (tc::elect_one()) {
+            const uint32_t idesc = KIND == EIGHT ? instr_desc_e4m3(tok) : tc::instr_desc_bf16(FEATURES, S::PARTS * tok);
+            constexpr uint32_t A_STEP = S::A_BYTES >> 4, B_STEP = S::B_BYTES >> 4;
+            const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
+            const uint32_t desc_hi = (uint32_t)(desc0 >> 32), a_lo = (uint32_t)desc0;
+            const uint32_t b_lo = (uint32_t)tc::smem_desc_sw128(tc::smem_u32(s.b[0]));
+            const uint32_t full0 = tc::smem_u32(&s.full[0]), empty0 = tc::smem_u32(&s.empty[0]);
+            bool ok = true;
+            uint32_t phase = 0;
+            for (int kb0 = 0; kb0 < n_kb && ok; kb0 += S::STAGES, phase ^= 1) {
+#pragma unroll
+                for (int st = 0; st < S::STAGES; ++st) {
+                    if (kb0 + st >= n_kb) break;
+                    if (!tc::mbar_wait_at(full0 + 8 * st, phase, abort_flag)) {
+                        tc::give_up(abort_flag, status, tc::ST_MMA_TIMEOUT);
+                        ok = false;
+                        break;
+                    }
+                    tc::tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {           // 32 bytes of K an instruction: two descriptor units
+                        const uint64_t a = tc::desc_of(a_lo + st * A_STEP + 2 * k, desc_hi);
+                        const uint64_t b = tc::desc_of(b_lo + st * B_STEP + 2 * k, desc_hi);
+                        const uint32_t more = kb0 > 0 || st > 0 || k > 0 ? 1u : 0u;
+                        if constexpr (KIND == EIGHT) umma_e4m3(tmem, a, b, idesc, more);
+                        else tc::umma_bf16(tmem, a, b, idesc, more);
+                    }
+                    tc::umma_commit_at(empty0 + 8 * st);
+                }
+            }
+            if (ok) tc::umma_commit(&s.done);
+        }
+    } else if (warp == 6) {
+        if constexpr (KIND != EIGHT) if (tc::elect_one()) {
+            int st = 0, sent = 0;
+            uint32_t parity = 1;
+            const int n_pk = (k_end - k_begin + PACKED_K - 1) / PACKED_K;
+            for (int i = 0; i < n_pk; ++i) {
+                if (i >= S::PACKED && !tc::mbar_wait(&s.codes_empty[st], parity, abort_flag)) {
+                    tc::give_up(abort_flag, status, tc::ST_PRODUCER_TIMEOUT);
+                    break;
+                }
+                tc::mbar_expect_tx(&s.codes_full[st], S::A_BYTES);
+                tc::tma_load_2d(s.codes[st], &map_w, &s.codes_full[st], (k_begin + i * PACKED_K) / 2, n0);
+                sent = i + 1;
+                if (++st == S::PACKED) st = 0, parity ^= 1;
+            }
+            if (*abort_flag)
+                for (int i = max(0, sent - S::PACKED); i < sent; ++i)
+                    for (uint32_t j = 0; j < tc::WAIT_LIMIT; ++j)
+                        if (tc::mbar_try_wait(&s.codes_full[i % S::PACKED], (i / S::PACKED) & 1)) break;
+        }
+    } else {
+        const int r = (warp & 3) * 32 + lane;               // the feature: a lane of tensor memory
+        const int n = n0 + r;
+        bool ok = true;
+        if constexpr (KIND != EIGHT) {
+            const int sub = p.group / 32;                   // runs of 32 k that share a scale
+            const int groups = p.K / p.group;
+            const uint8_t* my_scales = p.group_scale + (long long)min(n, p.N - 1) * groups;
+            int at = k_begin / p.group, in = k_begin / 32 % sub;
+            // the scales of 256 k, asked for a stage of codes ahead
+            auto load_scales = [&](uint8_t (&sc)[8], int k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sc[i] = k + 32 * i < k_end ? __ldg(my_scales + at) : (uint8_t)0;
+                    if (++in == sub) in = 0, ++at;
+                }
+            };
+            uint8_t sc[8], next[8];
+            load_scales(next, k_begin);
+            int slot = 0, pk = 0;
+            uint32_t slot_parity = 1, pk_parity = 0;
+            for (int kb = 0; kb < n_kb && ok; kb += 4) {
+                ok = tc::mbar_wait(&s.codes_full[pk], pk_parity, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) {
+                    tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sc[i] = next[i];
+                load_scales(next, k_begin + (kb + 4) * 64);
+                const uint8_t* packed = s.codes[pk] + r * 128;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (kb + j >= n_kb) break;
+                    const uint4 c0 = *reinterpret_cast<const uint4*>(packed + (((2 * j) ^ (r & 7)) << 4));
+                    const uint4 c1 = *reinterpret_cast<const uint4*>(packed + (((2 * j + 1) ^ (r & 7)) << 4));
+                    if (kb + j >= S::STAGES) {
+                        ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+                            break;
+                        }
+                    }
+                    const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+                    uint32_t s2[2], c2[2];
+                    scale_pairs(sc[2 * j], s2[0], c2[0]);
+                    scale_pairs(sc[2 * j + 1], s2[1], c2[1]);
+                    uint8_t* mine = s.a[slot] + r * 128;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
+                        *reinterpret_cast<uint4*>(mine + ((c ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.full[slot]);
+                    if (++slot == S::STAGES) slot = 0, slot_parity ^= 1;
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&s.codes_empty[pk]);
+                if (++pk == S::PACKED) pk = 0, pk_parity ^= 1;
+            }
+        }
+        // ---- epilogue
+        if (ok) {
+            ok = tc::mbar_wait(&s.done, 0, abort_flag);
+            if (!ok && !*abort_flag) tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        tc::tc_fence_after_sync();
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const float fs = n < p.N ? __ldg(p.feature_scale + n) : 0.f;
+        // 16 rows' sums of this feature
+        auto load16 = [&](int c, float (&v)[16]) {
+            uint32_t u[S::PARTS][16];
+#pragma unroll
+            for (int i = 0; i < S::PARTS; ++i) tc::tmem_ld_32x16(mine + i * tok + c, u[i]);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] = __uint_as_float(u[S::PARTS - 1][i]);
+#pragma unroll
+                for (int j = S::PARTS - 2; j >= 0; --j) v[i] += __uint_as_float(u[j][i]);
+            }
+        };
+        auto store16 = [&](int c, const float (&v)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int m = m0 + c + i;
+                if (n < p.N && c + i < tok && m < p.M)
+                    finish(p, v[i], KIND == EIGHT ? __ldg(p.row_scale + m) : 1.f, fs, m, n);
+            }
+        };
+        if (splits == 1) {
+            if (ok) {
+#pragma unroll 1
+                for (int c = 0; c < tok; c += 16) {
+                    float v[16];
+                    load16(c, v);
+                    store16(c, v);
+                }
+            }
+        } else {
+            float* left = reinterpret_cast<float*>(s.a[0]);           // [row][feature]; the ring is free by now
+            if (ok) {
+#pragma unroll 1
+                for (int c = 0; c < tok; c += 16) {
+                    float v[16];
+                    load16(c, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) left[(c + i) * FEATURES + r] = v[i];
+                }
+            }
+            tc::cluster_sync_all();
+            // this block's share of the rows, 8 at a time
+            const int share = (tok / 8 + splits - 1) / splits * 8;
+            const uint32_t base = tc::smem_u32(left) + 4 * r;
+            const int c_end = min(tok, (int)(rank + 1) * share);
+            if (ok && !*abort_flag) {
+#pragma unroll 1
+                for (int c = (int)rank * share; c < c_end; c += 8) {
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+                    for (int q = 0; q < splits; ++q) {
+                        const uint32_t theirs = tc::cluster_map(base + c * FEATURES * 4, (uint32_t)q);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float x;
+                            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(theirs + i * FEATURES * 4) : "memory");
+                            v[i] += x;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int m = m0 + c + i;
+                        if (n < p.N && m < p.M) finish(p, v[i], KIND == EIGHT ? __ldg(p.row_scale + m) : 1.f, fs, m, n);
+                    }
+                }
+            }
+        }
+        tc::tc_fence_before_sync();
+    }
+    __syncwarp();
+    if (splits > 1) {
+        // the other warps' part of the barrier between leaving and reading; then nobody goes while his
+        // shared memory is read
+        if (warp < 2 || warp == 6) tc::cluster_sync_all();
+        tc::cluster_sync_all();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after_sync();
+        tc::tmem_dealloc(tmem, S::TMEM);
+    }
+}
+
+// fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ rows, long long ldr,
+                                                         __nv_bfloat16* __restrict__ parts, int M, int K) {
+    cb_pdl_wait();
+    const long long total = (long long)M * (K / 4);
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long m = i / (K / 4), k = i % (K / 4) * 4;
+        const float4 v = __ldg(reinterpret_cast<const float4*>(rows + m * ldr + k));
+        uint32_t a[3], b[3];
+        three_parts(v.x, v.y, a);
+        three_parts(v.z, v.w, b);
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            *reinterpret_cast<uint2*>(parts + ((long long)j * M + m) * K + k) = make_uint2(a[j], b[j]);
+    }
+}
+
+// A matrix read in boxes of 128 bytes by `box_rows` rows with the 128-byte swizzle; beyond it zeros.  `parts` > 1: so
+// many matrices one behind the other, all of them in a box.
+bool make_map(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t row_bytes,
+              uint32_t box_rows, uint32_t parts) {
+    tc::EncodeTiledFn fn = tc::encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {cols, rows, parts};
+    cuuint64_t strides[2] = {row_bytes, row_bytes * rows};
+    cuuint32_t box[3] = {bf16 ? 64u : 128u, box_rows, parts};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, parts > 1 ? 3 : 2,
+              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KIND, int TOK>
+int launch(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
+           cudaStream_t stream) {
+    constexpr int SMEM = (int)sizeof(Storage<KIND, TOK>) + 1024;
+    static_assert(SMEM <= 232448, "a block's shared memory");
+    static_assert(TOK * FEATURES * 4 <= (int)(sizeof(Storage<KIND, TOK>::a) + sizeof(Storage<KIND, TOK>::b)),
+                  "the sums that a block leaves for its cluster must fit in the ring");
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    static bool configured[64] = {};
+    if (dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(linear_tcgen05_kernel<KIND, TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) configured[dev] = true;
+    }
+    cb_launch_cluster(linear_tcgen05_kernel<KIND, TOK>,
+                      dim3((p.N + FEATURES - 1) / FEATURES, (p.M + tok - 1) / tok, splits), dim3(THREADS), SMEM, stream,
+                      splits, rows, w, p, tok, splits, status);
+    return cb_last_error();
+}
+
+template <int KIND>
+int launch_tok(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
+               cudaStream_t stream) {
+    if (tok <= 32) return launch<KIND, 32>(p, rows, w, tok, splits, status, stream);
+    if (tok <= 64) return launch<KIND, 64>(p, rows, w, tok, splits, status, stream);
+    if constexpr (KIND != FOUR_F32) {
+        if (tok <= 128) return launch<KIND, 128>(p, rows, w, tok, splits, status, stream);
+        if (tok <= 256) return launch<KIND, 256>(p, rows, w, tok, splits, status, stream);
+    }
+    return CB_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+// `tok`: rows a tile, a multiple of 16 up to 256 (fp32 rows: 64); `splits`: shares of K, 1 to 8 (as many as leave
+// none empty); `parts`: bf16 [3, M, K], where fp32 rows are split to.
+CB_EXPORT int cb_linear_quantized_tcgen05(int kind, const void* rows, long long ldr, const float* row_scale,
+                                          const void* w, long long ldw, const void* group_scale,
+                                          const float* feature_scale, const float* add, long long lda, void* out,
+                                          int out_dtype, long long ldo, int M, int N, int K, int group, int tok,
+                                          int splits, void* parts, int* status, void* stream) {
+    if (M <= 0 || N <= 0) return 0;
+    const int size = kind == EIGHT ? 1 : (kind == FOUR_F32 ? 4 : 2);
+    if (K <= 0 || tok < 16 || tok % 16 || tok > (kind == FOUR_F32 ? 64 : 256) || splits < 1 || splits > 8 ||
+        (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
+        (M + tok - 1) / tok > 65535 || (kind != EIGHT && (group <= 0 || group % 32 || K % group)) ||
+        (kind == FOUR_F32 && (parts == nullptr || ((uintptr_t)parts & 15))))
+        return CB_ERR_UNSUPPORTED;
+    const int unit = kind == EIGHT ? 128 : PACKED_K, units = (K + unit - 1) / unit;
+    if (splits > units) splits = units;
+    while (splits > 1 && (splits - 1) * ((units + splits - 1) / splits) >= units) --splits;
+    const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
+                             M, N, K, group, out_dtype == CB_BF16};
+    cudaStream_t st = (cudaStream_t)stream;
+    CUtensorMap mr, mw;
+    bool ok = make_map(&mw, w, false, (uint64_t)N, kind == EIGHT ? (uint64_t)K : (uint64_t)K / 2, (uint64_t)ldw, FEATURES, 1);
+    if (kind == FOUR_F32) ok = ok && make_map(&mr, parts, true, (uint64_t)M, (uint64_t)K, (uint64_t)K * 2, tok, 3);
+    else ok = ok && make_map(&mr, rows, kind == FOUR_BF16, (uint64_t)M, (uint64_t)K, (uint64_t)ldr * size, tok, 1);
+    if (!ok) return CB_ERR_UNSUPPORTED;
+    if (kind == FOUR_F32) {
+        const long long quads = (long long)M * (K / 4);
+        const int blocks = (int)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8);
+        cb_launch(split_rows_kernel, dim3(blocks), dim3(256), 0, st, (const float*)rows, ldr, (__nv_bfloat16*)parts, M, K);
+        return launch_tok<FOUR_F32>(p, mr, mw, tok, splits, status, st);
+    }
+    if (kind == FOUR_BF16) return launch_tok<FOUR_BF16>(p, mr, mw, tok, splits, status, st);
+    if (kind == EIGHT) return launch_tok<EIGHT>(p, mr, mw, tok, splits, status, st);
+    return CB_ERR_UNSUPPORTED;
+}

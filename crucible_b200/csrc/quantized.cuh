@@ -1,0 +1,79 @@
+// What the products over quantised weights share: how a code becomes a bf16 weight, and how a fp32
+// row becomes three bf16 ones.
+//
+// (code - 8) * scale has at most 3 + 4 significant bits for an e4m3 scale, so it is a bf16 number and
+// the tensor cores multiply the weights themselves.  Code bits put into the mantissa of 16 are
+// 16 + code, and one fused multiply-add, (16 + code) scale - 24 scale, is exact (24 scale has 2 + 4
+// significant bits).
+//
+// A fp32 row is the sum of three bf16 rows exactly: the 24 bits of the mantissa, 8 by 8.  Their
+// products with the weights are exact too, and only fp32 sums are rounded.  The first part has a sum of
+// its own: the numbers of the others are 2^-8 of it and less, and a sum that held the first would
+// cut off their last bits at every addition (rows of 8,192: 2.4e-6 off with one sum).
+#pragma once
+#include "common.cuh"
+
+enum QuantizedKind { FOUR_BF16 = 0, FOUR_F32 = 1, EIGHT = 2 };
+
+struct QuantizedArgs {
+    const void* rows;                   // bf16, fp32 or e4m3 [M, ldr elements]
+    long long ldr;
+    const float* row_scale;             // EIGHT: [M]
+    const void* w;                      // codes int32 [N, K / 8], or e4m3 [N, ldw]
+    long long ldw;                      // bytes
+    const uint8_t* group_scale;         // e4m3 [N, K / group]
+    const float* feature_scale;         // [N]
+    const float* add;                   // fp32 [M, lda] or null
+    long long lda;
+    void* out;                          // [M, ldo]
+    long long ldo;
+    int M, N, K, group, out_bf16;
+};
+
+// An e4m3 scale as a pair of equal bf16 numbers, and -24 times it: both exact.
+__device__ __forceinline__ void scale_pairs(uint32_t e4m3, uint32_t& s2, uint32_t& c2) {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)e4m3));
+    float s;
+    asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.f32.f16 %0, lo;\n\t}" : "=f"(s) : "r"(h2));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s2) : "f"(s));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(c2) : "f"(-24.f * s));
+}
+
+// Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.
+__device__ __forceinline__ uint32_t weight_pair(uint32_t word, int i, uint32_t s2, uint32_t c2) {
+    const uint32_t put = i == 0 ? word << 3 : word >> (4 * i - 3);
+    const uint32_t magic = (put & 0x00780078u) | 0x41804180u;       // 16 + code, twice
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(magic), "r"(s2), "r"(c2));
+    return r;
+}
+
+// Two fp32 numbers as three pairs of bf16 whose sum they are.  (Cut, not rounded: what is left is
+// exact.  An infinity or a NaN stands in the first pair alone.)
+__device__ __forceinline__ void three_parts(float x, float y, uint32_t (&p)[3]) {
+    const float v[2] = {x, y};
+    uint32_t part[2][3];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t bits = __float_as_uint(v[i]);
+        const bool finite = (bits & 0x7F800000u) != 0x7F800000u;
+        const float rest = finite ? v[i] - __uint_as_float(bits & 0xFFFF0000u) : 0.f;
+        const float second = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
+        part[i][0] = finite || (bits & 0x007FFFFFu) == 0 ? bits >> 16 : 0x7FC0u;
+        part[i][1] = __float_as_uint(second) >> 16;
+        part[i][2] = __float_as_uint(rest - second) >> 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) p[j] = part[0][j] | (part[1][j] << 16);
+}
+
+// A sum's way out: its scales, the addition, the rounding.
+__device__ __forceinline__ void finish(const QuantizedArgs& p, float v, float row_scale, float feature_scale, int m, int n) {
+    v *= feature_scale;
+    v *= row_scale;
+    if (p.add != nullptr) v += p.add[(long long)m * p.lda + n];
+    const long long at = (long long)m * p.ldo + n;
+    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    else static_cast<float*>(p.out)[at] = v;
+}

@@ -633,4 +633,4 @@ def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Te
     _check(code, "sample_rows")
 
 
-from . import quantized, small_batch, tensor_core  # noqa: E402  (they take what stands above)
+from . import small_batch, tensor_core, quantized  # noqa: E402  (they take what stands above)

@@ -20,10 +20,11 @@ from typing import Optional
 
 import torch
 
-from . import KernelError, _check, _code, _need_cuda, _ptr, _stream, build
+from . import LAUNCHES, KernelError, _check, _code, _need_cuda, _ptr, _stream, build, tensor_core
 
-for _name in ("rows8", "linear_quantized_few"):
-    build.register_module(_name, ["common.cuh"])
+build.register_module("rows8", ["common.cuh"])
+build.register_module("linear_quantized_few", ["common.cuh", "quantized.cuh"])
+build.register_module("linear_quantized_tcgen05", ["common.cuh", "quantized.cuh", "tc_common.cuh"])
 
 E4M3 = torch.float8_e4m3fn
 TOP = 448.0                      # the largest e4m3 number
@@ -264,16 +265,36 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
         _rows(add, f"{what} add", (torch.float32,), shape)
 
 
+FEW_ROWS = 16                    # products of up to so many rows run on mma.sync
+
+
+def tile_of(kind: int, m: int, n: int, k: int):
+    """(rows a tile, shares of K) of the tcgen05 product."""
+    most = 64 if kind == _FOUR_F32 else 256
+    tok = -(-m // -(-m // most))
+    tok = (tok + 15) // 16 * 16
+    tiles = -(-n // 128) * -(-m // tok)
+    slots = 148 * (2 if tok <= (32 if kind == _FOUR_F32 else 64) else 1)
+    units = -(-k // (128 if kind == _EIGHT else 256))
+    return tok, max(1, min(8, slots // tiles, units // 2))
+
+
 def _product(kind: int, rows, row_scales, values, ldw: int, group_scales, w, group: int, out, add, what: str) -> None:
     m, (n, k) = rows.shape[0], w.shape
     if m == 0:
         return
-    lib = build.load("linear_quantized_few")
     with _Device(rows):
-        code = lib.cb_linear_quantized_few(
-            kind, _ptr(rows), _pitch(rows), _ptr(row_scales), _ptr(values), ldw, _ptr(group_scales), _ptr(w.scales),
-            _ptr(add), add.stride(0) if add is not None else 0, _ptr(out), _code(out.dtype), out.stride(0), m, n, k,
-            group, _stream())
+        common = (kind, _ptr(rows), _pitch(rows), _ptr(row_scales), _ptr(values), ldw, _ptr(group_scales),
+                  _ptr(w.scales), _ptr(add), add.stride(0) if add is not None else 0, _ptr(out), _code(out.dtype),
+                  out.stride(0), m, n, k, group)
+        if m <= FEW_ROWS:
+            code = build.load("linear_quantized_few").cb_linear_quantized_few(*common, _stream())
+        else:
+            parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device) if kind == _FOUR_F32 else None
+            code = build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05(
+                *common, *tile_of(kind, m, n, k), _ptr(parts), _ptr(tensor_core.status_word(rows.device)), _stream())
+            if kind == _FOUR_F32 and code == 0:
+                LAUNCHES[0] += 1                       # (the rows' parts)
     if code == build.UNSUPPORTED:
         raise KernelError(f"{what}: sizes out of range: rows {list(rows.shape)}, weights {list(w.shape)}")
     _check(code, what)
