@@ -16,8 +16,7 @@
 // Roles: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor memory and
 // issues the MMAs, warps 2-5 make weights of codes and then run the epilogue, warp 6 sends the
 // copies of codes.
-#include "quantized.cuh"
-#include "tc_common.cuh"
+#include "quantized_tc.cuh"
 
 namespace {
 
@@ -55,12 +54,7 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// kind::f8f6f4 with e4m3 A and B (format 0), K-major, fp32 sums
-__device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {
-    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(FEATURES >> 4) << 24);
-}
-
-template <int KIND, int TOK>
+template <int KIND, int TOK, bool BF16>
 __global__ void __launch_bounds__(THREADS)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
                       const QuantizedArgs p, int tok, int splits, int* __restrict__ status) {
@@ -131,7 +125,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         }
     } else if (warp == 1) {
         if (tc::elect_one()) {
-            const uint32_t idesc = KIND == EIGHT ? instr_desc_e4m3(tok) : tc::instr_desc_bf16(FEATURES, S::PARTS * tok);
+            const uint32_t idesc = KIND == EIGHT ? instr_desc_e4m3(FEATURES, tok) : tc::instr_desc_bf16(FEATURES, S::PARTS * tok);
             constexpr uint32_t A_STEP = S::A_BYTES >> 4, B_STEP = S::B_BYTES >> 4;
             const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
             const uint32_t desc_hi = (uint32_t)(desc0 >> 32), a_lo = (uint32_t)desc0;
@@ -187,20 +181,9 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         const int n = n0 + r;
         bool ok = true;
         if constexpr (KIND != EIGHT) {
-            const int sub = p.group / 32;                   // runs of 32 k that share a scale
-            const int groups = p.K / p.group;
-            const uint8_t* my_scales = p.group_scale + (long long)min(n, p.N - 1) * groups;
-            int at = k_begin / p.group, in = k_begin / 32 % sub;
-            // the scales of 256 k, asked for a stage of codes ahead
-            auto load_scales = [&](uint8_t (&sc)[8], int k) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sc[i] = k + 32 * i < k_end ? __ldg(my_scales + at) : (uint8_t)0;
-                    if (++in == sub) in = 0, ++at;
-                }
-            };
-            uint8_t sc[8], next[8];
-            load_scales(next, k_begin);
+            ScaleWalk walk(p, n, k_begin);
+            uint8_t sc[8], next[8];                         // of 256 k, asked for a stage of codes ahead
+            walk.next(next, k_begin, k_end);
             int slot = 0, pk = 0;
             uint32_t slot_parity = 1, pk_parity = 0;
             for (int kb = 0; kb < n_kb && ok; kb += 4) {
@@ -212,13 +195,11 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sc[i] = next[i];
-                load_scales(next, k_begin + (kb + 4) * 64);
+                walk.next(next, k_begin + (kb + 4) * 64, k_end);
                 const uint8_t* packed = s.codes[pk] + r * 128;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (kb + j >= n_kb) break;
-                    const uint4 c0 = *reinterpret_cast<const uint4*>(packed + (((2 * j) ^ (r & 7)) << 4));
-                    const uint4 c1 = *reinterpret_cast<const uint4*>(packed + (((2 * j + 1) ^ (r & 7)) << 4));
                     if (kb + j >= S::STAGES) {
                         ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
                         ok = __all_sync(0xffffffffu, ok);
@@ -227,18 +208,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                             break;
                         }
                     }
-                    const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-                    uint32_t s2[2], c2[2];
-                    scale_pairs(sc[2 * j], s2[0], c2[0]);
-                    scale_pairs(sc[2 * j + 1], s2[1], c2[1]);
-                    uint8_t* mine = s.a[slot] + r * 128;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
-                        *reinterpret_cast<uint4*>(mine + ((c ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
+                    make_weights(packed, j, r, sc[2 * j], sc[2 * j + 1], s.a[slot] + r * 128);
                     tc::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[slot]);
@@ -258,45 +228,41 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         tc::tc_fence_after_sync();
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float fs = n < p.N ? __ldg(p.feature_scale + n) : 0.f;
-        // 16 rows' sums of this feature
-        auto load16 = [&](int c, float (&v)[16]) {
-            uint32_t u[S::PARTS][16];
-#pragma unroll
-            for (int i = 0; i < S::PARTS; ++i) tc::tmem_ld_32x16(mine + i * tok + c, u[i]);
+        const int m_end = min(p.M, m0 + tok);
+        // 32 rows' sums of this feature (a last 16 beside something that nobody uses)
+        auto load_rows = [&](int c, float (&v)[32]) {
+            uint32_t u[32];
+            tc::tmem_ld_32x32(mine + (S::PARTS - 1) * tok + c, u);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                v[i] = __uint_as_float(u[S::PARTS - 1][i]);
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
 #pragma unroll
-                for (int j = S::PARTS - 2; j >= 0; --j) v[i] += __uint_as_float(u[j][i]);
-            }
-        };
-        auto store16 = [&](int c, const float (&v)[16]) {
+            for (int j = S::PARTS - 2; j >= 0; --j) {
+                tc::tmem_ld_32x32(mine + j * tok + c, u);
+                tc::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int m = m0 + c + i;
-                if (n < p.N && c + i < tok && m < p.M)
-                    finish(p, v[i], KIND == EIGHT ? __ldg(p.row_scale + m) : 1.f, fs, m, n);
+                for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(u[i]);
             }
         };
         if (splits == 1) {
             if (ok) {
 #pragma unroll 1
-                for (int c = 0; c < tok; c += 16) {
-                    float v[16];
-                    load16(c, v);
-                    store16(c, v);
+                for (int c = 0; c < tok; c += 32) {
+                    float v[32];
+                    load_rows(c, v);
+                    store_rows<KIND, BF16>(p, v, fs, n, m0 + c, m_end, p.add, p.lda);
                 }
             }
         } else {
             float* left = reinterpret_cast<float*>(s.a[0]);           // [row][feature]; the ring is free by now
             if (ok) {
 #pragma unroll 1
-                for (int c = 0; c < tok; c += 16) {
-                    float v[16];
-                    load16(c, v);
+                for (int c = 0; c < tok; c += 32) {
+                    float v[32];
+                    load_rows(c, v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) left[(c + i) * FEATURES + r] = v[i];
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i < tok) left[(c + i) * FEATURES + r] = v[i];
                 }
             }
             tc::cluster_sync_all();
@@ -359,53 +325,39 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict
     }
 }
 
-// A matrix read in boxes of 128 bytes by `box_rows` rows with the 128-byte swizzle; beyond it zeros.  `parts` > 1: so
-// many matrices one behind the other, all of them in a box.
-bool make_map(CUtensorMap* map, const void* base, bool bf16, uint64_t rows, uint64_t cols, uint64_t row_bytes,
-              uint32_t box_rows, uint32_t parts) {
-    tc::EncodeTiledFn fn = tc::encode_fn();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {cols, rows, parts};
-    cuuint64_t strides[2] = {row_bytes, row_bytes * rows};
-    cuuint32_t box[3] = {bf16 ? 64u : 128u, box_rows, parts};
-    cuuint32_t estr[3] = {1, 1, 1};
-    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, parts > 1 ? 3 : 2,
-              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <int KIND, int TOK>
+template <int KIND, int TOK, bool BF16>
 int launch(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
            cudaStream_t stream) {
     constexpr int SMEM = (int)sizeof(Storage<KIND, TOK>) + 1024;
     static_assert(SMEM <= 232448, "a block's shared memory");
     static_assert(TOK * FEATURES * 4 <= (int)(sizeof(Storage<KIND, TOK>::a) + sizeof(Storage<KIND, TOK>::b)),
                   "the sums that a block leaves for its cluster must fit in the ring");
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
     static bool configured[64] = {};
-    if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(linear_tcgen05_kernel<KIND, TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-        if (e != cudaSuccess) return (int)e;
-        if (dev < 64) configured[dev] = true;
-    }
-    cb_launch_cluster(linear_tcgen05_kernel<KIND, TOK>,
-                      dim3((p.N + FEATURES - 1) / FEATURES, (p.M + tok - 1) / tok, splits), dim3(THREADS), SMEM, stream,
+    auto kernel = linear_tcgen05_kernel<KIND, TOK, BF16>;
+    const int rc = allow_shared(kernel, SMEM, configured);
+    if (rc != 0) return rc;
+    cb_launch_cluster(kernel, dim3((p.N + FEATURES - 1) / FEATURES, (p.M + tok - 1) / tok, splits), dim3(THREADS), SMEM, stream,
                       splits, rows, w, p, tok, splits, status);
     return cb_last_error();
 }
 
-template <int KIND>
+template <int KIND, bool BF16>
 int launch_tok(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
                cudaStream_t stream) {
-    if (tok <= 32) return launch<KIND, 32>(p, rows, w, tok, splits, status, stream);
-    if (tok <= 64) return launch<KIND, 64>(p, rows, w, tok, splits, status, stream);
+    if (tok <= 32) return launch<KIND, 32, BF16>(p, rows, w, tok, splits, status, stream);
+    if (tok <= 64) return launch<KIND, 64, BF16>(p, rows, w, tok, splits, status, stream);
     if constexpr (KIND != FOUR_F32) {
-        if (tok <= 128) return launch<KIND, 128>(p, rows, w, tok, splits, status, stream);
-        if (tok <= 256) return launch<KIND, 256>(p, rows, w, tok, splits, status, stream);
+        if (tok <= 128) return launch<KIND, 128, BF16>(p, rows, w, tok, splits, status, stream);
+        if (tok <= 256) return launch<KIND, 256, BF16>(p, rows, w, tok, splits, status, stream);
     }
     return CB_ERR_UNSUPPORTED;
+}
+
+template <int KIND>
+int launch_out(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
+               cudaStream_t stream) {
+    return p.out_bf16 ? launch_tok<KIND, true>(p, rows, w, tok, splits, status, stream)
+                      : launch_tok<KIND, false>(p, rows, w, tok, splits, status, stream);
 }
 
 }  // namespace
@@ -431,17 +383,17 @@ CB_EXPORT int cb_linear_quantized_tcgen05(int kind, const void* rows, long long 
                              M, N, K, group, out_dtype == CB_BF16};
     cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap mr, mw;
-    bool ok = make_map(&mw, w, false, (uint64_t)N, kind == EIGHT ? (uint64_t)K : (uint64_t)K / 2, (uint64_t)ldw, FEATURES, 1);
-    if (kind == FOUR_F32) ok = ok && make_map(&mr, parts, true, (uint64_t)M, (uint64_t)K, (uint64_t)K * 2, tok, 3);
-    else ok = ok && make_map(&mr, rows, kind == FOUR_BF16, (uint64_t)M, (uint64_t)K, (uint64_t)ldr * size, tok, 1);
+    bool ok = quantized_map(&mw, w, false, (uint64_t)N, kind == EIGHT ? (uint64_t)K : (uint64_t)K / 2, (uint64_t)ldw, FEATURES, 1);
+    if (kind == FOUR_F32) ok = ok && quantized_map(&mr, parts, true, (uint64_t)M, (uint64_t)K, (uint64_t)K * 2, tok, 3);
+    else ok = ok && quantized_map(&mr, rows, kind == FOUR_BF16, (uint64_t)M, (uint64_t)K, (uint64_t)ldr * size, tok, 1);
     if (!ok) return CB_ERR_UNSUPPORTED;
     if (kind == FOUR_F32) {
         const long long quads = (long long)M * (K / 4);
         const int blocks = (int)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8);
         cb_launch(split_rows_kernel, dim3(blocks), dim3(256), 0, st, (const float*)rows, ldr, (__nv_bfloat16*)parts, M, K);
-        return launch_tok<FOUR_F32>(p, mr, mw, tok, splits, status, st);
+        return launch_out<FOUR_F32>(p, mr, mw, tok, splits, status, st);
     }
-    if (kind == FOUR_BF16) return launch_tok<FOUR_BF16>(p, mr, mw, tok, splits, status, st);
-    if (kind == EIGHT) return launch_tok<EIGHT>(p, mr, mw, tok, splits, status, st);
+    if (kind == FOUR_BF16) return launch_out<FOUR_BF16>(p, mr, mw, tok, splits, status, st);
+    if (kind == EIGHT) return launch_out<EIGHT>(p, mr, mw, tok, splits, status, st);
     return CB_ERR_UNSUPPORTED;
 }

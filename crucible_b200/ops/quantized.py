@@ -24,7 +24,8 @@ from . import LAUNCHES, KernelError, _check, _code, _need_cuda, _ptr, _stream, b
 
 build.register_module("rows8", ["common.cuh"])
 build.register_module("linear_quantized_few", ["common.cuh", "quantized.cuh"])
-build.register_module("linear_quantized_tcgen05", ["common.cuh", "quantized.cuh", "tc_common.cuh"])
+for _name in ("linear_quantized_tcgen05", "linear_quantized_pairs_tcgen05"):
+    build.register_module(_name, ["common.cuh", "quantized.cuh", "quantized_tc.cuh", "tc_common.cuh"])
 
 E4M3 = torch.float8_e4m3fn
 TOP = 448.0                      # the largest e4m3 number
@@ -266,33 +267,49 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 
 
 FEW_ROWS = 16                    # products of up to so many rows run on mma.sync
+FORM = None                      # tests name one of the forms, "few", "tiles" or "pairs", to reach it at any size
 
 
-def tile_of(kind: int, m: int, n: int, k: int):
-    """(rows a tile, shares of K) of the tcgen05 product."""
+def _up(x: int, to: int) -> int:
+    return (x + to - 1) // to * to
+
+
+def form_of(kind: int, m: int, n: int, k: int):
+    """Which kernel takes the product, and how: ("few",), ("tiles", rows a tile, shares of K) or ("pairs", rows a
+    tile, pairs of SMs)."""
+    form = FORM
+    if form is None or (form == "pairs" and kind == _FOUR_F32):
+        form = "few" if m <= FEW_ROWS else "tiles" if kind == _FOUR_F32 or m <= 256 else "pairs"
+    if form == "few":
+        return ("few",)
     most = 64 if kind == _FOUR_F32 else 256
-    tok = -(-m // -(-m // most))
-    tok = (tok + 15) // 16 * 16
+    tok = _up(-(-m // -(-m // most)), 16)
+    if form == "pairs":
+        return "pairs", tok, 74
     tiles = -(-n // 128) * -(-m // tok)
     slots = 148 * (2 if tok <= (32 if kind == _FOUR_F32 else 64) else 1)
     units = -(-k // (128 if kind == _EIGHT else 256))
-    return tok, max(1, min(8, slots // tiles, units // 2))
+    return "tiles", tok, max(1, min(8, slots // tiles, units // 2))
 
 
 def _product(kind: int, rows, row_scales, values, ldw: int, group_scales, w, group: int, out, add, what: str) -> None:
     m, (n, k) = rows.shape[0], w.shape
     if m == 0:
         return
+    form, *how = form_of(kind, m, n, k)
     with _Device(rows):
         common = (kind, _ptr(rows), _pitch(rows), _ptr(row_scales), _ptr(values), ldw, _ptr(group_scales),
                   _ptr(w.scales), _ptr(add), add.stride(0) if add is not None else 0, _ptr(out), _code(out.dtype),
                   out.stride(0), m, n, k, group)
-        if m <= FEW_ROWS:
+        if form == "few":
             code = build.load("linear_quantized_few").cb_linear_quantized_few(*common, _stream())
+        elif form == "pairs":
+            code = build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs(
+                *common, *how, _ptr(tensor_core.status_word(rows.device)), _stream())
         else:
             parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device) if kind == _FOUR_F32 else None
             code = build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05(
-                *common, *tile_of(kind, m, n, k), _ptr(parts), _ptr(tensor_core.status_word(rows.device)), _stream())
+                *common, *how, _ptr(parts), _ptr(tensor_core.status_word(rows.device)), _stream())
             if kind == _FOUR_F32 and code == 0:
                 LAUNCHES[0] += 1                       # (the rows' parts)
     if code == build.UNSUPPORTED:

@@ -148,6 +148,26 @@ def test_linear8_prompts(rows, n, k):
     _check8(rows, n, k, torch.float32, True)
 
 
+@pytest.mark.parametrize("form", ["few", "tiles", "pairs"])
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (3, 130, 100), (16, 257, 129), (17, 128, 128), (40, 255, 600), (129, 300, 1000),
+                                      (250, 513, 256), (257, 700, 2049), (300, 256, 6000), (513, 40000, 64)])
+def test_linear8_by_every_form(form, rows, n, k, monkeypatch):
+    monkeypatch.setattr(quantized, "FORM", form)
+    for out, add in ((torch.float32, True), (torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)):
+        _check8(rows, n, k, out, add)
+
+
+@pytest.mark.parametrize("form", ["few", "tiles", "pairs"])
+@pytest.mark.parametrize("rows,n,k,group", [(1, 1, 32, 32), (3, 130, 96, 96), (16, 257, 160, 32), (17, 128, 256, 64),
+                                            (40, 255, 608, 32), (129, 300, 1024, 128), (250, 513, 288, 96),
+                                            (257, 700, 2080, 32), (300, 256, 6144, 6144), (513, 40000, 64, 64)])
+def test_linear4_by_every_form(form, rows, n, k, group, monkeypatch):
+    monkeypatch.setattr(quantized, "FORM", form)
+    for dtype in (torch.bfloat16, torch.float32):
+        for out, add in ((torch.float32, True), (torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)):
+            _check4(rows, n, k, group, dtype, out, add)
+
+
 def _check4(rows, n, k, group, dtype, out_dtype, add, seed=0):
     gen = _gen(seed + rows * 7919 + n * 31 + k)
     w = random_weights4(n, k, group, DEV, gen)
