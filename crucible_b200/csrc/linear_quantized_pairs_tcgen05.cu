@@ -6,7 +6,7 @@
 // their SMs and walk the tiles; while the sums of one leave tensor memory, the other half takes the next.
 //
 //   EIGHT      both operands e4m3 by TMA, 128 k a stage, kind::f8f6f4
-//   FOUR_BF16  the codes by TMA, 256 k a stage; four warps of each block make bf16 weights of them
+//   FOUR_BF16  the codes by TMA, 256 k a stage; eight warps of each block make bf16 weights of them
 //              (exact, see quantized.cuh), 64 k a stage of the MMA's ring, a feature a thread
 //
 // fp32 results.  The tensor cores cut off what an addition leaves below the sum's last bit, always towards
@@ -15,8 +15,9 @@
 // pair does this under the MMAs of the next chunk.
 //
 // Roles in each block: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor
-// memory (the first block's issues the MMAs), warps 2-5 take the sums out, warp 6 sends the copies of
-// codes, warps 7-10 make weights of them.
+// memory (the first block's issues the MMAs), warps 2-9 take the sums out (two to a quarter of the lanes, 32
+// rows in turn), warp 10 sends the copies of codes, warps 11-18 make weights of them (two sets of four, 64
+// k in turn: between a warp's reading codes and its weights being there lie as long as two stages' MMAs).
 #include "quantized_tc.cuh"
 
 namespace {
@@ -30,7 +31,7 @@ constexpr int CHUNK = 2048;             // K of one sum, fp32 results
 template <int KIND> struct Sizes {
     static constexpr int BK = KIND == EIGHT ? 128 : 64;
     static constexpr int STAGES = KIND == EIGHT ? 6 : 5;
-    static constexpr int THREADS = KIND == EIGHT ? 192 : 352;
+    static constexpr int THREADS = KIND == EIGHT ? 320 : 608;
 };
 
 template <int KIND> struct Storage {
@@ -110,11 +111,11 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
         }
         for (int i = 0; i < PACKED; ++i) {
             tc::mbar_init(&s.codes_full[i], 1);
-            tc::mbar_init(&s.codes_empty[i], 4);
+            tc::mbar_init(&s.codes_empty[i], 8);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s.done[i], 1);
-            tc::mbar_init(&s.taken[i], 8);                           // (four warps of each block)
+            tc::mbar_init(&s.taken[i], 16);                          // (eight warps of each block)
         }
         s.abort_flag = 0;
         tc::fence_barrier_init();
@@ -202,7 +203,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
                 if (ok) pair_commit(&s.done[half]);
             }
         }
-    } else if (warp < 6) {
+    } else if (warp < 10) {
         const int r = (warp & 3) * 32 + lane;
         int at = 0;
         for (; u.more(); u.advance(), ++at) {
@@ -222,7 +223,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
             const long long lda = first ? p.lda : p.ldo;
             const uint32_t mine = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll 1
-            for (int c = 0; c < m_end - m0; c += 32) {
+            for (int c = 32 * ((warp - 2) >> 2); c < m_end - m0; c += 64) {
                 uint32_t x[32];
                 float v[32];
                 tc::tmem_ld_32x32(mine + c, x);
@@ -235,7 +236,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
             __syncwarp();
             if (lane == 0) arrive_at(tc::cluster_map(tc::smem_u32(&s.taken[half]), 0));
         }
-    } else if (warp == 6) {
+    } else if (warp == 10) {
         if constexpr (KIND != EIGHT) if (tc::elect_one()) {
             int st = 0;
             long long sent = 0;
@@ -262,35 +263,37 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
         }
     } else {
         if constexpr (KIND != EIGHT) {
-            const int r = (warp - 7) * 32 + lane;
+            const int r = (warp + 1 & 3) * 32 + lane, set = (warp - 11) >> 2;
+            // (the ring's slots and the stages of codes go on from one unit to the next, and so do the turns)
             int slot = 0, pk = 0;
             long long made = 0;
             uint32_t slot_parity = 1, pk_parity = 0;
             bool ok = true;
             for (; u.more() && ok; u.advance()) {
                 const int n = (u.n_tile() * 2 + (int)rank) * MINE + r, k_end = u.k_end();
-                ScaleWalk walk(p, n, u.k_begin());
-                uint8_t sc[8], next[8];
-                walk.next(next, u.k_begin(), k_end);
+                const Scales scales(p, n);
+                uint2 sc, next = scales.load(u.k_begin(), k_end);
                 for (int k = u.k_begin(); k < k_end && ok; k += PACKED_K) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sc[i] = next[i];
-                    walk.next(next, k + PACKED_K, k_end);
+                    sc = next;
+                    next = scales.load(k + PACKED_K, k_end);
                     ok = tc::mbar_wait(&s.codes_full[pk], pk_parity, abort_flag);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (k + 64 * j >= k_end) break;
-                        if (made >= STAGES) {
-                            ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
-                            ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) break;
+                        if ((made & 1) == set) {
+                            if (made >= STAGES) {
+                                ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
+                                ok = __all_sync(0xffffffffu, ok);
+                                if (!ok) break;
+                            }
+                            make_weights(s.codes[pk] + r * 128, j, r, Scales::of(sc, 2 * j), Scales::of(sc, 2 * j + 1),
+                                         s.a[slot] + r * 128);
+                            tc::fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) arrive_at(tc::cluster_map(tc::smem_u32(&s.full[slot]), 0));
                         }
-                        make_weights(s.codes[pk] + r * 128, j, r, sc[2 * j], sc[2 * j + 1], s.a[slot] + r * 128);
-                        tc::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) arrive_at(tc::cluster_map(tc::smem_u32(&s.full[slot]), 0));
                         ++made;
                         if (++slot == STAGES) slot = 0, slot_parity ^= 1;
                     }
@@ -335,7 +338,7 @@ CB_EXPORT int cb_linear_quantized_pairs(int kind, const void* rows, long long ld
                                         int N, int K, int group, int tok, int pairs, int* status, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     const int size = kind == EIGHT ? 1 : 2;
-    if ((kind != EIGHT && kind != FOUR_BF16) || K <= 0 || tok < 16 || tok % 16 || tok > 256 || pairs < 1 ||
+    if ((kind != EIGHT && kind != FOUR_BF16) || K <= 0 || K > MOST_K || tok < 16 || tok % 16 || tok > 256 || pairs < 1 ||
         (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
         (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;

@@ -181,9 +181,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         const int n = n0 + r;
         bool ok = true;
         if constexpr (KIND != EIGHT) {
-            ScaleWalk walk(p, n, k_begin);
-            uint8_t sc[8], next[8];                         // of 256 k, asked for a stage of codes ahead
-            walk.next(next, k_begin, k_end);
+            const Scales scales(p, n);
+            uint2 sc, next = scales.load(k_begin, k_end);
             int slot = 0, pk = 0;
             uint32_t slot_parity = 1, pk_parity = 0;
             for (int kb = 0; kb < n_kb && ok; kb += 4) {
@@ -193,9 +192,8 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                     tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
                     break;
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sc[i] = next[i];
-                walk.next(next, k_begin + (kb + 4) * 64, k_end);
+                sc = next;
+                next = scales.load(k_begin + (kb + 4) * 64, k_end);
                 const uint8_t* packed = s.codes[pk] + r * 128;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -208,7 +206,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                             break;
                         }
                     }
-                    make_weights(packed, j, r, sc[2 * j], sc[2 * j + 1], s.a[slot] + r * 128);
+                    make_weights(packed, j, r, Scales::of(sc, 2 * j), Scales::of(sc, 2 * j + 1), s.a[slot] + r * 128);
                     tc::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[slot]);
@@ -371,7 +369,7 @@ CB_EXPORT int cb_linear_quantized_tcgen05(int kind, const void* rows, long long 
                                           int splits, void* parts, int* status, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     const int size = kind == EIGHT ? 1 : (kind == FOUR_F32 ? 4 : 2);
-    if (K <= 0 || tok < 16 || tok % 16 || tok > (kind == FOUR_F32 ? 64 : 256) || splits < 1 || splits > 8 ||
+    if (K <= 0 || K > MOST_K || tok < 16 || tok % 16 || tok > (kind == FOUR_F32 ? 64 : 256) || splits < 1 || splits > 8 ||
         (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
         (M + tok - 1) / tok > 65535 || (kind != EIGHT && (group <= 0 || group % 32 || K % group)) ||
         (kind == FOUR_F32 && (parts == nullptr || ((uintptr_t)parts & 15))))

@@ -13,6 +13,9 @@
 #pragma once
 #include "common.cuh"
 
+// K of a product at the most: indices along K, and the products that stand for divisions of them, are 32-bit
+constexpr int MOST_K = 1 << 20;
+
 enum QuantizedKind { FOUR_BF16 = 0, FOUR_F32 = 1, EIGHT = 2 };
 
 struct QuantizedArgs {

@@ -3,6 +3,7 @@
 #pragma once
 #include "quantized.cuh"
 #include "tc_common.cuh"
+#include <type_traits>
 
 // kind::f8f6f4 with e4m3 A and B (format 0), K-major, fp32 sums
 __device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {
@@ -28,55 +29,91 @@ __device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, in
     }
 }
 
-// Walks the group scales of one feature, 256 k at a time.
-struct ScaleWalk {
-    const uint8_t* scales;
-    int sub, at, in;                    // runs of 32 k that share a scale; the present scale; runs it has had
-    __device__ ScaleWalk(const QuantizedArgs& p, int n, int k)
-        : scales(p.group_scale + (long long)min(n, p.N - 1) * (p.K / p.group)), sub(p.group / 32), at(k / p.group),
-          in(k / 32 % (p.group / 32)) {}
-    // (`k_end`: zeros from there on)
-    __device__ __forceinline__ void next(uint8_t (&sc)[8], int k, int k_end) {
+// The group scales of one feature, 256 k (eight runs of 32) at a time, asked for a stage of codes ahead.  Where 256 k
+// are whole groups and a feature's scales begin on a multiple of 8, 4 or 2 bytes, as those 256 k have, one load
+// brings them (a load of a byte is 32 lines of memory for a warp, and eight of them for 256 k take the load unit
+// as long as the MMAs take); else one of a byte each.
+struct Scales {
+    const uint8_t* from;
+    int sub, groups;                    // runs of 32 k that share a scale; scales of a feature
+    bool together;
+    __device__ Scales(const QuantizedArgs& p, int n) : sub(p.group / 32), groups(p.K / p.group) {
+        from = p.group_scale + (long long)min(n, p.N - 1) * groups;
+        const int per = 8 / sub;        // scales of 256 k
+        together = (sub == 1 || sub == 2 || sub == 4) && groups % per == 0 && ((uintptr_t)p.group_scale & (per - 1)) == 0;
+    }
+    // run i of 256 k from k: byte i (a multiple of 256; zeros from k_end on)
+    __device__ __forceinline__ uint2 load(int k, int k_end) const {
+        if (k >= k_end) return make_uint2(0u, 0u);
+        if (together) {
+            // (k_end is a multiple of 256, or of the whole K: no scale is read that is not there)
+            const int at = k / 32 / sub;
+            if (sub == 1) return __ldg(reinterpret_cast<const uint2*>(from + at));
+            if (sub == 2) {
+                const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(from + at));
+                return make_uint2(__byte_perm(x, 0, 0x1100), __byte_perm(x, 0, 0x3322));
+            }
+            const uint32_t x = __ldg(reinterpret_cast<const uint16_t*>(from + at));
+            return make_uint2(__byte_perm(x, 0, 0x0000), __byte_perm(x, 0, 0x1111));
+        }
+        uint32_t w[2] = {0u, 0u};
+        int at = k / 32 / sub, in = k / 32 % sub;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            sc[i] = k + 32 * i < k_end ? __ldg(scales + at) : (uint8_t)0;
+            if (k + 32 * i < k_end) w[i >> 2] |= (uint32_t)__ldg(from + at) << (8 * (i & 3));
             if (++in == sub) in = 0, ++at;
         }
+        return make_uint2(w[0], w[1]);
     }
+    static __device__ __forceinline__ uint32_t of(uint2 w, int i) { return ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u; }
 };
 
 // 32 rows' sums of feature n, rows m to m + 31 (those below m_end are stored): scales, addition, rounding, store.
 // Neighbouring lanes hold neighbouring features, so a row's store is 64 or 128 neighbouring bytes a warp.  Loads go
 // out together before anything is stored.  `add`: fp32 with `lda` between rows, or null; it may be the output.
+// (WHOLE: nothing to ask per row.  With a question a row, this took 24 instructions a number, which a lone
+// warp issues one in five cycles.)
+template <int KIND, bool BF16, bool ADD, bool WHOLE>
+__device__ __forceinline__ void store_rows_as(const QuantizedArgs& p, const float (&v)[32], float fs, float rs, int n, int m,
+                                              int m_end, const float* add, long long lda) {
+    const bool here = WHOLE || n < p.N;
+    using Out = typename std::conditional<BF16, __nv_bfloat16, float>::type;
+    const float* from = ADD ? add + (long long)m * lda + n : nullptr;
+    Out* to = static_cast<Out*>(p.out) + ((long long)m * p.ldo + n);
+#pragma unroll
+    for (int half = 0; half < 32; half += 16) {         // (16 loads on their way; 32 would cost other warps their registers)
+        float a[16];
+        if (ADD) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                a[i] = WHOLE || (here && m + half + i < m_end) ? __ldcg(from) : 0.f;
+                from += lda;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float x = v[half + i] * fs;
+            if (KIND == EIGHT) x *= __shfl_sync(0xffffffffu, rs, half + i);
+            if (ADD) x += a[i];
+            if (WHOLE || (here && m + half + i < m_end)) *to = cb_from_float<Out>(x);
+            to += p.ldo;
+        }
+    }
+}
+
 template <int KIND, bool BF16>
 __device__ __forceinline__ void store_rows(const QuantizedArgs& p, const float (&v)[32], float fs, int n, int m, int m_end,
                                            const float* add, long long lda) {
     const int lane = threadIdx.x & 31;
     float rs = 1.f;
     if (KIND == EIGHT) rs = __ldg(p.row_scale + min(m + lane, p.M - 1));
-    const bool here = n < p.N;
-    const bool whole = m + 32 <= m_end;                 // (the same for all threads)
-    float a[32];
+    const bool whole = m + 32 <= m_end && n - lane + 32 <= p.N;
     if (add != nullptr) {
-        const float* from = add + (long long)m * lda + n;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) a[i] = here && (whole || m + i < m_end) ? __ldcg(from + (long long)i * lda) : 0.f;
+        if (whole) store_rows_as<KIND, BF16, true, true>(p, v, fs, rs, n, m, m_end, add, lda);
+        else store_rows_as<KIND, BF16, true, false>(p, v, fs, rs, n, m, m_end, add, lda);
     } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) a[i] = 0.f;
-    }
-    const long long at = (long long)m * p.ldo + n;
-    float* f32 = static_cast<float*>(p.out) + at;
-    __nv_bfloat16* bf16 = static_cast<__nv_bfloat16*>(p.out) + at;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        float x = v[i] * fs;
-        if (KIND == EIGHT) x *= __shfl_sync(0xffffffffu, rs, i);
-        x += a[i];
-        if (here && (whole || m + i < m_end)) {
-            if (BF16) bf16[(long long)i * p.ldo] = __float2bfloat16_rn(x);
-            else f32[(long long)i * p.ldo] = x;
-        }
+        if (whole) store_rows_as<KIND, BF16, false, true>(p, v, fs, rs, n, m, m_end, add, lda);
+        else store_rows_as<KIND, BF16, false, false>(p, v, fs, rs, n, m, m_end, add, lda);
     }
 }
 
