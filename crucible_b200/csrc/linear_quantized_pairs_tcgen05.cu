@@ -51,8 +51,12 @@ __device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, uin
                  ::"r"(tc::smem_u32(dst)), "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
+// An arrival at a barrier of either block.  What it announces lies in this block's shared or tensor memory, where
+// the MMAs of the pair read and write it through the async proxy, and a proxy or tcgen05 fence stands ahead of
+// the arrival.  So its release has the block as its scope: one of the cluster's waits for every write
+// the thread ever made, 1,050 cycles here (a stage's MMAs take 512).
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 // One arrival at this barrier of both blocks when the MMAs issued so far have finished.
@@ -288,7 +292,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
                                 ok = __all_sync(0xffffffffu, ok);
                                 if (!ok) break;
                             }
-                            make_weights(s.codes[pk] + r * 128, j, r, Scales::of(sc, 2 * j), Scales::of(sc, 2 * j + 1),
+                            make_weights(s.codes[pk] + r * 128, j, r, scales.of(sc, 2 * j), scales.of(sc, 2 * j + 1),
                                          s.a[slot] + r * 128);
                             tc::fence_proxy_async();
                             __syncwarp();

@@ -206,7 +206,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                             break;
                         }
                     }
-                    make_weights(packed, j, r, Scales::of(sc, 2 * j), Scales::of(sc, 2 * j + 1), s.a[slot] + r * 128);
+                    make_weights(packed, j, r, scales.of(sc, 2 * j), scales.of(sc, 2 * j + 1), s.a[slot] + r * 128);
                     tc::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[slot]);

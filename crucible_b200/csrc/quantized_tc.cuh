@@ -35,26 +35,23 @@ __device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, in
 // as long as the MMAs take); else one of a byte each.
 struct Scales {
     const uint8_t* from;
-    int sub, groups;                    // runs of 32 k that share a scale; scales of a feature
+    int sub, lg;                        // runs of 32 k that share a scale, and its logarithm where they come together
     bool together;
-    __device__ Scales(const QuantizedArgs& p, int n) : sub(p.group / 32), groups(p.K / p.group) {
+    __device__ Scales(const QuantizedArgs& p, int n) : sub(p.group / 32) {
+        const int groups = p.K / p.group, per = 8 / sub;
         from = p.group_scale + (long long)min(n, p.N - 1) * groups;
-        const int per = 8 / sub;        // scales of 256 k
         together = (sub == 1 || sub == 2 || sub == 4) && groups % per == 0 && ((uintptr_t)p.group_scale & (per - 1)) == 0;
+        lg = together ? sub >> 1 : 0;
     }
-    // run i of 256 k from k: byte i (a multiple of 256; zeros from k_end on)
+    // The scales of 256 k from k (a multiple of 256; zeros from k_end on), as `of` reads them: nothing here waits for
+    // the one load.  (k_end is a multiple of 256, or the whole K, which then is one: all of them are there.)
     __device__ __forceinline__ uint2 load(int k, int k_end) const {
         if (k >= k_end) return make_uint2(0u, 0u);
         if (together) {
-            // (k_end is a multiple of 256, or of the whole K: no scale is read that is not there)
-            const int at = k / 32 / sub;
-            if (sub == 1) return __ldg(reinterpret_cast<const uint2*>(from + at));
-            if (sub == 2) {
-                const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(from + at));
-                return make_uint2(__byte_perm(x, 0, 0x1100), __byte_perm(x, 0, 0x3322));
-            }
-            const uint32_t x = __ldg(reinterpret_cast<const uint16_t*>(from + at));
-            return make_uint2(__byte_perm(x, 0, 0x0000), __byte_perm(x, 0, 0x1111));
+            const uint8_t* at = from + (k >> 5 >> lg);
+            if (lg == 0) return __ldg(reinterpret_cast<const uint2*>(at));
+            if (lg == 1) return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(at)), 0u);
+            return make_uint2(__ldg(reinterpret_cast<const uint16_t*>(at)), 0u);
         }
         uint32_t w[2] = {0u, 0u};
         int at = k / 32 / sub, in = k / 32 % sub;
@@ -65,7 +62,11 @@ struct Scales {
         }
         return make_uint2(w[0], w[1]);
     }
-    static __device__ __forceinline__ uint32_t of(uint2 w, int i) { return ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u; }
+    // the scale of run i
+    __device__ __forceinline__ uint32_t of(uint2 w, int i) const {
+        const int b = i >> lg;
+        return ((b < 4 ? w.x : w.y) >> (8 * (b & 3))) & 255u;
+    }
 };
 
 // 32 rows' sums of feature n, rows m to m + 31 (those below m_end are stored): scales, addition, rounding, store.
