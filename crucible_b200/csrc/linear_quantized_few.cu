@@ -18,9 +18,9 @@
 
 namespace {
 
-constexpr int WARPS = 8;
 constexpr int PAIRS = 2;                // 16 features each: a block's
 constexpr int FEATURES = 16 * PAIRS;
+constexpr int BATCH = 2;                // segments of weights that a warp asks for together
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -36,42 +36,45 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// What a thread holds of a segment's weights: 16 bytes of each of its features, and their scales.
-template <int KIND> struct Held {
+// What a thread holds of a segment's weights: 16 bytes of each of its features, and their scales (of features
+// g and g + 8 in two bytes).
+struct Held {
     uint4 w[PAIRS][2];
-    uint8_t scale[PAIRS][2];
+    uint32_t scale[PAIRS];
 };
 
-// NT: groups of 8 rows.  BATCH: segments of weights a warp has in flight.
-template <int KIND, int NT, int BATCH>
-__global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
+// NT: groups of 8 rows.  WARPS share K.
+template <int KIND, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (KIND == FOUR_F32 ? 8 : 16) / WARPS)
+linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
     constexpr int SEG = KIND == EIGHT ? 64 : 128;       // k of a segment: 64 bytes of a feature's weights
     constexpr int MINE = SEG / 4;                       // k of a thread: 16 bytes
+    constexpr int SIZE = KIND == EIGHT ? 1 : (KIND == FOUR_F32 ? 4 : 2);
     constexpr int ROWS = 8 * NT;
     __shared__ float sums[WARPS][FEATURES][ROWS + 1];
     cb_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * FEATURES, m0 = blockIdx.y * ROWS;
-    const int K = p.K, segments = (K + SEG - 1) / SEG;
-    const int groups = KIND == EIGHT ? 0 : K / p.group;
+    const int K = p.K, whole = K / SEG;                 // (segments that do not end in K's tail)
     // the thread's features (beyond the last: the last, whose sums nobody stores) and rows
-    const uint8_t *w[PAIRS][2], *scales[PAIRS][2];
+    const uint8_t* w[PAIRS][2];
+    uint32_t scales[PAIRS][2];                          // offsets, in a matrix of group scales
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const long long f = min(n0 + 16 * i + 8 * h + g, p.N - 1);
-            w[i][h] = static_cast<const uint8_t*>(p.w) + f * p.ldw;
-            scales[i][h] = p.group_scale + f * groups;
+            const int f = min(n0 + 16 * i + 8 * h + g, p.N - 1);
+            w[i][h] = static_cast<const uint8_t*>(p.w) + f * p.ldw + 16 * t;
+            scales[i][h] = KIND == EIGHT ? 0 : (uint32_t)(f - n0) * (uint32_t)p.groups;
         }
-    constexpr int SIZE = KIND == EIGHT ? 1 : (KIND == FOUR_F32 ? 4 : 2);
+    const uint8_t* const block_scales = KIND == EIGHT ? nullptr : p.group_scale + (long long)n0 * p.groups;
     const uint8_t* rows[NT];
     bool has_row[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         has_row[i] = m0 + 8 * i + g < p.M;
-        rows[i] = static_cast<const uint8_t*>(p.rows) + (has_row[i] ? m0 + 8 * i + g : 0) * p.ldr * SIZE;
+        rows[i] = static_cast<const uint8_t*>(p.rows) + (has_row[i] ? m0 + 8 * i + g : 0) * p.ldr * SIZE + t * MINE * SIZE;
     }
     float acc[PAIRS][NT][4], rest[KIND == FOUR_F32 ? PAIRS : 1][NT][4];
 #pragma unroll
@@ -90,34 +93,36 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
             if (i < left) word[i >> 2] |= (uint32_t)at[i] << (8 * (i & 3));
         return make_uint4(word[0], word[1], word[2], word[3]);
     };
-    auto fetch = [&](Held<KIND>& h, int seg) {
+    // TAIL: the segment in which K ends; a thread whose k lie beyond it has zeros
+    auto fetch = [&](Held& h, int seg, bool tail) {
         const int k = seg * SEG + t * MINE;
-        // the run of 32 k's scale: k / 32 over the runs that share one, by its reciprocal (0: one run)
-        const uint32_t at = KIND == EIGHT ? 0 : (run_magic ? __umulhi((uint32_t)k >> 5, run_magic) : (uint32_t)k >> 5);
+        if (tail && k >= K) {
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i)
+            for (int i = 0; i < PAIRS; ++i) h.w[i][0] = h.w[i][1] = make_uint4(0, 0, 0, 0), h.scale[i] = 0;
+            return;
+        }
+        // the scale of a run of 32 k: 2 (k / 32) over the runs that share one, by half their reciprocal
+        const uint32_t at = KIND == EIGHT ? 0 : __umulhi((uint32_t)k >> 4, run_magic);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                h.w[i][j] = make_uint4(0, 0, 0, 0);
-                h.scale[i][j] = 0;
-                if (k < K) {
-                    if constexpr (KIND == EIGHT) {
-                        h.w[i][j] = load16(w[i][j] + k, K - k);
-                    } else {
-                        h.w[i][j] = __ldg(reinterpret_cast<const uint4*>(w[i][j] + (k >> 1)));
-                        h.scale[i][j] = __ldg(scales[i][j] + at);
-                    }
-                }
+                const uint8_t* from = w[i][j] + seg * 64;
+                h.w[i][j] = KIND == EIGHT && tail ? load16(from, K - k) : __ldg(reinterpret_cast<const uint4*>(from));
             }
+            if (KIND != EIGHT)
+                h.scale[i] = (uint32_t)__ldg(block_scales + (scales[i][0] + at)) |
+                             (uint32_t)__ldg(block_scales + (scales[i][1] + at)) << 8;
+        }
     };
-    auto multiply = [&](const Held<KIND>& h, int seg) {
+    auto multiply = [&](const Held& h, int seg, bool tail) {
         const int k = seg * SEG + t * MINE;
         if constexpr (KIND == EIGHT) {
             uint4 r[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 r[j] = make_uint4(0, 0, 0, 0);
-                if (has_row[j] && k < K) r[j] = load16(rows[j] + k, K - k);
+                if (has_row[j] && (!tail || k < K)) r[j] = load16(rows[j] + seg * SEG, tail ? K - k : 16);
             }
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i) {
@@ -130,11 +135,6 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
                 }
             }
         } else {
-            uint32_t s2[PAIRS][2], c2[PAIRS][2];
-#pragma unroll
-            for (int i = 0; i < PAIRS; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) scale_pairs(h.scale[i][j], s2[i][j], c2[i][j]);
             uint4 b16[KIND == FOUR_BF16 ? NT : 1][4];
             if constexpr (KIND == FOUR_BF16) {
 #pragma unroll
@@ -142,9 +142,13 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         b16[j][c] = make_uint4(0, 0, 0, 0);
-                        if (has_row[j] && k < K) b16[j][c] = __ldg(reinterpret_cast<const uint4*>(rows[j] + 2 * k) + c);
+                        if (has_row[j] && (!tail || k < K))
+                            b16[j][c] = __ldg(reinterpret_cast<const uint4*>(rows[j] + seg * SEG * SIZE) + c);
                     }
             }
+            uint32_t s2[PAIRS][2], c2[PAIRS][2];
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) scale_pairs(h.scale[i], s2[i], c2[i]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {               // eight k at a time
                 uint32_t b[NT][3][4];                   // [rows][part][pairs of k]
@@ -154,7 +158,8 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (has_row[j] && k < K) r = __ldg(reinterpret_cast<const float4*>(rows[j] + 4 * k) + 2 * c + q);
+                            if (has_row[j] && (!tail || k < K))
+                                r = __ldg(reinterpret_cast<const float4*>(rows[j] + seg * SEG * SIZE) + 2 * c + q);
                             uint32_t one[3], two[3];
                             three_parts(r.x, r.y, one);
                             three_parts(r.z, r.w, two);
@@ -189,16 +194,38 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
         }
     };
 
-    Held<KIND> now[BATCH], then[BATCH];
+    // Two batches take turns: one is on its way while the other is multiplied.
+    Held x[BATCH], y[BATCH];
+    int seg = warp;
+    auto more = [&]() { return seg + (BATCH - 1) * WARPS < whole; };
+    auto ask = [&](Held (&h)[BATCH]) {
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) fetch(now[b], warp + b * WARPS);
-    for (int seg = warp; seg < segments; seg += WARPS * BATCH) {
+        for (int b = 0; b < BATCH; ++b) fetch(h[b], seg + b * WARPS, false);
+    };
+    auto take = [&](const Held (&h)[BATCH], int from) {
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) fetch(then[b], seg + (BATCH + b) * WARPS);
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) multiply(now[b], seg + b * WARPS);
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) now[b] = then[b];
+        for (int b = 0; b < BATCH; ++b) multiply(h[b], from + b * WARPS, false);
+    };
+    bool have = more();
+    if (have) ask(x);
+#pragma unroll 1
+    while (have) {
+        int from = seg;
+        seg += WARPS * BATCH;
+        have = more();
+        if (have) ask(y);
+        take(x, from);
+        if (!have) break;
+        from = seg;
+        seg += WARPS * BATCH;
+        have = more();
+        if (have) ask(x);
+        take(y, from);
+    }
+#pragma unroll 1
+    for (; seg * SEG < K; seg += WARPS) {
+        fetch(x[0], seg, true);
+        multiply(x[0], seg, true);
     }
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i)
@@ -211,7 +238,7 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
                 sums[warp][16 * i + 8 * (e >> 1) + g][8 * j + 2 * t + (e & 1)] = v;
             }
     __syncthreads();
-#pragma unroll
+#pragma unroll 1
     for (int at = threadIdx.x; at < FEATURES * ROWS; at += WARPS * 32) {
         const int f = at % FEATURES, m = at / FEATURES;
         if (n0 + f >= p.N || m0 + m >= p.M) continue;
@@ -222,11 +249,17 @@ __global__ void __launch_bounds__(WARPS * 32, KIND == FOUR_F32 ? 1 : 2) linear_f
     }
 }
 
-template <int KIND>
+template <int KIND, int NT>
 void launch(const QuantizedArgs& p, uint32_t run_magic, cudaStream_t s) {
-    const unsigned tiles = (p.N + FEATURES - 1) / FEATURES;
-    if (p.M <= 8) cb_launch(linear_few_kernel<KIND, 1, 2>, dim3(tiles), dim3(WARPS * 32), 0, s, p, run_magic);
-    else cb_launch(linear_few_kernel<KIND, 2, 1>, dim3(tiles, (p.M + 15) / 16), dim3(WARPS * 32), 0, s, p, run_magic);
+    const dim3 grid((p.N + FEATURES - 1) / FEATURES, (p.M + 8 * NT - 1) / (8 * NT));
+    if (p.K <= 6144) cb_launch(linear_few_kernel<KIND, NT, 4>, grid, dim3(128), 0, s, p, run_magic);
+    else cb_launch(linear_few_kernel<KIND, NT, 8>, grid, dim3(256), 0, s, p, run_magic);
+}
+
+template <int KIND>
+void launch_rows(const QuantizedArgs& p, uint32_t run_magic, cudaStream_t s) {
+    if (p.M <= 8) launch<KIND, 1>(p, run_magic, s);
+    else launch<KIND, 2>(p, run_magic, s);
 }
 
 }  // namespace
@@ -243,13 +276,15 @@ CB_EXPORT int cb_linear_quantized_few(int kind, const void* rows, long long ldr,
         (M + 15) / 16 > 65535 || (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;
     const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
-                             M, N, K, group, out_dtype == CB_BF16};
-    const uint32_t sub = (uint32_t)group / 32;          // ceil(2^32 / sub): exact while K / 32 * sub < 2^32
-    const uint32_t run_magic = sub > 1 ? (uint32_t)(((1ull << 32) + sub - 1) / sub) : 0;
+                             M, N, K, group, out_dtype == CB_BF16, group > 0 ? K / group : 0};
+    // half the reciprocal of the runs that share a scale, ceil(2^31 / runs): its products with 2 (k / 32) are exact
+    // while K / 32 * runs < 2^31
+    const uint32_t runs = (uint32_t)group / 32;
+    const uint32_t run_magic = runs > 0 ? (uint32_t)(((1ull << 31) + runs - 1) / runs) : 0;
     cudaStream_t s = (cudaStream_t)stream;
-    if (kind == FOUR_BF16) launch<FOUR_BF16>(p, run_magic, s);
-    else if (kind == FOUR_F32) launch<FOUR_F32>(p, run_magic, s);
-    else if (kind == EIGHT) launch<EIGHT>(p, run_magic, s);
+    if (kind == FOUR_BF16) launch_rows<FOUR_BF16>(p, run_magic, s);
+    else if (kind == FOUR_F32) launch_rows<FOUR_F32>(p, run_magic, s);
+    else if (kind == EIGHT) launch_rows<EIGHT>(p, run_magic, s);
     else return CB_ERR_UNSUPPORTED;
     return cb_last_error();
 }

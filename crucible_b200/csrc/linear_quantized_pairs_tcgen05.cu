@@ -292,7 +292,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
                                 ok = __all_sync(0xffffffffu, ok);
                                 if (!ok) break;
                             }
-                            make_weights(s.codes[pk] + r * 128, j, r, scales.of(sc, 2 * j), scales.of(sc, 2 * j + 1),
+                            make_weights(s.codes[pk] + r * 128, j, r, scales.of(sc, 2 * j),
                                          s.a[slot] + r * 128);
                             tc::fence_proxy_async();
                             __syncwarp();
@@ -347,7 +347,7 @@ CB_EXPORT int cb_linear_quantized_pairs(int kind, const void* rows, long long ld
         (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;
     const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
-                             M, N, K, group, out_dtype == CB_BF16};
+                             M, N, K, group, out_dtype == CB_BF16, group > 0 ? K / group : 0};
     const int tiles = (M + tok - 1) / tok * ((N + 2 * MINE - 1) / (2 * MINE));
     if (pairs > tiles) pairs = tiles;
     CUtensorMap mr, mw;

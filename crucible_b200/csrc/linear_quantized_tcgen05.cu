@@ -206,7 +206,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                             break;
                         }
                     }
-                    make_weights(packed, j, r, scales.of(sc, 2 * j), scales.of(sc, 2 * j + 1), s.a[slot] + r * 128);
+                    make_weights(packed, j, r, scales.of(sc, 2 * j), s.a[slot] + r * 128);
                     tc::fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.full[slot]);
@@ -378,7 +378,7 @@ CB_EXPORT int cb_linear_quantized_tcgen05(int kind, const void* rows, long long 
     if (splits > units) splits = units;
     while (splits > 1 && (splits - 1) * ((units + splits - 1) / splits) >= units) --splits;
     const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
-                             M, N, K, group, out_dtype == CB_BF16};
+                             M, N, K, group, out_dtype == CB_BF16, group > 0 ? K / group : 0};
     cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap mr, mw;
     bool ok = quantized_map(&mw, w, false, (uint64_t)N, kind == EIGHT ? (uint64_t)K : (uint64_t)K / 2, (uint64_t)ldw, FEATURES, 1);

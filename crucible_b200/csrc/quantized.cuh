@@ -30,17 +30,21 @@ struct QuantizedArgs {
     long long lda;
     void* out;                          // [M, ldo]
     long long ldo;
-    int M, N, K, group, out_bf16;
+    int M, N, K, group, out_bf16, groups;           // groups: K / group
 };
 
-// An e4m3 scale as a pair of equal bf16 numbers, and -24 times it: both exact.
-__device__ __forceinline__ void scale_pairs(uint32_t e4m3, uint32_t& s2, uint32_t& c2) {
+// Two e4m3 scales (the lower two bytes), each as a pair of equal bf16 numbers and as -24 times that: all exact.
+__device__ __forceinline__ void scale_pairs(uint32_t e4m3x2, uint32_t (&s2)[2], uint32_t (&c2)[2]) {
     uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)e4m3));
-    float s;
-    asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.f32.f16 %0, lo;\n\t}" : "=f"(s) : "r"(h2));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s2) : "f"(s));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(c2) : "f"(-24.f * s));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)e4m3x2));
+    float s[2];
+    asm("{\n\t.reg .f16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+        : "=f"(s[0]), "=f"(s[1]) : "r"(h2));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s2[i]) : "f"(s[i]));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(c2[i]) : "r"(s2[i]), "r"(0xC1C0C1C0u));       // -24
+    }
 }
 
 // Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.

@@ -12,14 +12,13 @@ __device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {
 
 // 64 codes of one feature (two runs of 32 k, a scale each) as bf16 weights in row `r` of a K-major tile of 128-byte
 // rows in the 128-byte swizzle; the codes lie in chunks 2j and 2j + 1 of row `r` of such a tile of codes.
-__device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, int r, uint32_t scale0, uint32_t scale1,
+__device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, int r, uint32_t two_scales,
                                              uint8_t* weights_row) {
     const uint4 c0 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j) ^ (r & 7)) << 4));
     const uint4 c1 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j + 1) ^ (r & 7)) << 4));
     const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
     uint32_t s2[2], c2[2];
-    scale_pairs(scale0, s2[0], c2[0]);
-    scale_pairs(scale1, s2[1], c2[1]);
+    scale_pairs(two_scales, s2, c2);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
         uint32_t v[4];
@@ -38,7 +37,7 @@ struct Scales {
     int sub, lg;                        // runs of 32 k that share a scale, and its logarithm where they come together
     bool together;
     __device__ Scales(const QuantizedArgs& p, int n) : sub(p.group / 32) {
-        const int groups = p.K / p.group, per = 8 / sub;
+        const int groups = p.groups, per = 8 / sub;
         from = p.group_scale + (long long)min(n, p.N - 1) * groups;
         together = (sub == 1 || sub == 2 || sub == 4) && groups % per == 0 && ((uintptr_t)p.group_scale & (per - 1)) == 0;
         lg = together ? sub >> 1 : 0;
@@ -62,10 +61,11 @@ struct Scales {
         }
         return make_uint2(w[0], w[1]);
     }
-    // the scale of run i
+    // the scales of runs i and i + 1 (i even): the lower two bytes
     __device__ __forceinline__ uint32_t of(uint2 w, int i) const {
         const int b = i >> lg;
-        return ((b < 4 ? w.x : w.y) >> (8 * (b & 3))) & 255u;
+        const uint32_t x = (b < 4 ? w.x : w.y) >> (8 * (b & 3));
+        return lg == 0 ? x : __byte_perm(x, 0, 0x0000);
     }
 };
 
