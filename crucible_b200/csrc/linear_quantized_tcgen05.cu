@@ -3,7 +3,7 @@
 // to 256 rows its N side.
 //
 //   EIGHT      both operands e4m3, brought by TMA (128 k a stage), tcgen05.mma kind::f8f6f4
-//   FOUR_BF16  the codes come in by TMA, 256 k of 128 features a stage; four warps make bf16 weights
+//   FOUR_BF16  the codes come in by TMA, 256 k of 128 features a stage; eight warps make bf16 weights
 //              of them (exact, see quantized.cuh), 64 k a stage of the MMA's ring, a feature a thread
 //   FOUR_F32   the same with three bf16 parts of every row side by side on the MMA's N side, which a
 //              kernel before this one has split: their sums lie in tensor memory apart and meet
@@ -14,14 +14,14 @@
 // shares: no scratch memory, no atomics, the same sum every time.
 //
 // Roles: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor memory and
-// issues the MMAs, warps 2-5 make weights of codes and then run the epilogue, warp 6 sends the
-// copies of codes.
+// issues the MMAs, warps 2-9 make weights of codes (two sets of four, 64 k in turn) and then take the sums
+// out (two to a quarter of the lanes, 32 rows in turn), warp 10 sends the copies of codes.
 #include "quantized_tc.cuh"
 
 namespace {
 
 constexpr int FEATURES = 128;
-constexpr int THREADS = 224;
+constexpr int THREADS = 352;
 constexpr int PACKED_K = 256;           // k of a stage of codes: 128 bytes a feature
 
 template <int KIND, int TOK> struct Sizes {
@@ -31,7 +31,8 @@ template <int KIND, int TOK> struct Sizes {
     static constexpr int B_BYTES = PARTS * TOK * 128;
     static constexpr int PACKED = KIND == EIGHT ? 0 : 2;             // stages of codes
     // a block of up to 64 rows shares its SM with another; one of more has it to itself
-    static constexpr int ROOM = (TOK <= 64 && PARTS == 1) || TOK <= 32 ? 110 * 1024 : 220 * 1024;
+    static constexpr int BLOCKS = (TOK <= 64 && PARTS == 1) || TOK <= 32 ? 2 : 1;
+    static constexpr int ROOM = BLOCKS == 2 ? 110 * 1024 : 220 * 1024;
     static constexpr int FIT = (ROOM - PACKED * A_BYTES) / (A_BYTES + B_BYTES);
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int N = PARTS * TOK;
@@ -55,7 +56,7 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
 }
 
 template <int KIND, int TOK, bool BF16>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, Sizes<KIND, TOK>::BLOCKS)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
                       const QuantizedArgs p, int tok, int splits, int* __restrict__ status) {
     using S = Sizes<KIND, TOK>;
@@ -75,12 +76,12 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
-            tc::mbar_init(&s.full[i], KIND == EIGHT ? 1 : 5);        // (the copy, and four warps' weights)
+            tc::mbar_init(&s.full[i], KIND == EIGHT ? 1 : 5);        // (the copy, and a set of four warps)
             tc::mbar_init(&s.empty[i], 1);
         }
         for (int i = 0; i < S::PACKED; ++i) {
             tc::mbar_init(&s.codes_full[i], 1);
-            tc::mbar_init(&s.codes_empty[i], 4);
+            tc::mbar_init(&s.codes_empty[i], 8);
         }
         tc::mbar_init(&s.done, 1);
         s.abort_flag = 0;
@@ -156,7 +157,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
             }
             if (ok) tc::umma_commit(&s.done);
         }
-    } else if (warp == 6) {
+    } else if (warp == 10) {
         if constexpr (KIND != EIGHT) if (tc::elect_one()) {
             int st = 0, sent = 0;
             uint32_t parity = 1;
@@ -177,7 +178,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                         if (tc::mbar_try_wait(&s.codes_full[i % S::PACKED], (i / S::PACKED) & 1)) break;
         }
     } else {
-        const int r = (warp & 3) * 32 + lane;               // the feature: a lane of tensor memory
+        const int r = (warp & 3) * 32 + lane, set = (warp - 2) >> 2;     // the feature: a lane of tensor memory
         const int n = n0 + r;
         bool ok = true;
         if constexpr (KIND != EIGHT) {
@@ -198,18 +199,20 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (kb + j >= n_kb) break;
-                    if (kb + j >= S::STAGES) {
-                        ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) {
-                            tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
-                            break;
+                    if ((j & 1) == set) {
+                        if (kb + j >= S::STAGES) {
+                            ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) {
+                                tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+                                break;
+                            }
                         }
+                        make_weights(packed, j, r, scales.of(sc, 2 * j), s.a[slot] + r * 128);
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&s.full[slot]);
                     }
-                    make_weights(packed, j, r, scales.of(sc, 2 * j), s.a[slot] + r * 128);
-                    tc::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&s.full[slot]);
                     if (++slot == S::STAGES) slot = 0, slot_parity ^= 1;
                 }
                 __syncwarp();
@@ -245,7 +248,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         if (splits == 1) {
             if (ok) {
 #pragma unroll 1
-                for (int c = 0; c < tok; c += 32) {
+                for (int c = 32 * set; c < tok; c += 64) {
                     float v[32];
                     load_rows(c, v);
                     store_rows<KIND, BF16>(p, v, fs, n, m0 + c, m_end, p.add, p.lda);
@@ -255,7 +258,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
             float* left = reinterpret_cast<float*>(s.a[0]);           // [row][feature]; the ring is free by now
             if (ok) {
 #pragma unroll 1
-                for (int c = 0; c < tok; c += 32) {
+                for (int c = 32 * set; c < tok; c += 64) {
                     float v[32];
                     load_rows(c, v);
 #pragma unroll
@@ -264,28 +267,40 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                 }
             }
             tc::cluster_sync_all();
-            // this block's share of the rows, 8 at a time
-            const int share = (tok / 8 + splits - 1) / splits * 8;
+            // this block's share of the rows, 4 at a time by the two sets in turn; what they are added to is asked
+            // for ahead of the others' sums
+            const int share = (tok / 4 + splits - 1) / splits * 4;
             const uint32_t base = tc::smem_u32(left) + 4 * r;
-            const int c_end = min(tok, (int)(rank + 1) * share);
+            const int c_end = min(min(tok, (int)(rank + 1) * share), p.M - m0);
             if (ok && !*abort_flag) {
 #pragma unroll 1
-                for (int c = (int)rank * share; c < c_end; c += 8) {
-                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+                for (int c = (int)rank * share + 4 * set; c < c_end; c += 8) {
+                    float a[4], v[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (p.add != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            a[i] = n < p.N && c + i < c_end ? __ldcg(p.add + (long long)(m0 + c + i) * p.lda + n) : 0.f;
+                    }
+#pragma unroll 4
                     for (int q = 0; q < splits; ++q) {
                         const uint32_t theirs = tc::cluster_map(base + c * FEATURES * 4, (uint32_t)q);
+                        float x[4];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float x;
-                            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(theirs + i * FEATURES * 4) : "memory");
-                            v[i] += x;
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[i]) : "r"(theirs + i * FEATURES * 4) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] += x[i];
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < 4; ++i) {
                         const int m = m0 + c + i;
-                        if (n < p.N && m < p.M) finish(p, v[i], KIND == EIGHT ? __ldg(p.row_scale + m) : 1.f, fs, m, n);
+                        if (n >= p.N || c + i >= c_end) continue;
+                        float y = v[i] * fs;
+                        if (KIND == EIGHT) y *= __ldg(p.row_scale + m);
+                        if (p.add != nullptr) y += a[i];
+                        const long long at = (long long)m * p.ldo + n;
+                        if (BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+                        else static_cast<float*>(p.out)[at] = y;
                     }
                 }
             }
@@ -296,7 +311,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     if (splits > 1) {
         // the other warps' part of the barrier between leaving and reading; then nobody goes while his
         // shared memory is read
-        if (warp < 2 || warp == 6) tc::cluster_sync_all();
+        if (warp < 2 || warp == 10) tc::cluster_sync_all();
         tc::cluster_sync_all();
     }
     __syncthreads();

@@ -47,11 +47,13 @@ __device__ __forceinline__ void scale_pairs(uint32_t e4m3x2, uint32_t (&s2)[2], 
     }
 }
 
-// Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.
+// Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.  (The mask and the 16s come as registers: with
+// both as constants the compiler takes two instructions for them, and the unit that runs them is what a product of a few rows
+// waits for.)
 __device__ __forceinline__ uint32_t weight_pair(uint32_t word, int i, uint32_t s2, uint32_t c2) {
     const uint32_t put = i == 0 ? word << 3 : word >> (4 * i - 3);
-    const uint32_t magic = (put & 0x00780078u) | 0x41804180u;       // 16 + code, twice
-    uint32_t r;
+    uint32_t magic, r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(magic) : "r"(put), "r"(0x00780078u), "r"(0x41804180u));   // 16 + code, twice
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(magic), "r"(s2), "r"(c2));
     return r;
 }
