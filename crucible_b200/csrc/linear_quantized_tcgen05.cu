@@ -4,7 +4,8 @@
 //
 //   EIGHT      both operands e4m3, brought by TMA (128 k a stage), tcgen05.mma kind::f8f6f4
 //   FOUR_BF16  the codes come in by TMA, 256 k of 128 features a stage; eight warps make bf16 weights
-//              of them (exact, see quantized.cuh), 64 k a stage of the MMA's ring, a feature a thread
+//              of them (exact, see quantized.cuh), 64 k a stage, a feature a thread, and put them into
+//              tensor memory, where the MMA takes them from
 //   FOUR_F32   the same with three bf16 parts of every row side by side on the MMA's N side, which a
 //              kernel before this one has split: their sums lie in tensor memory apart and meet
 //              in the epilogue
@@ -27,24 +28,28 @@ constexpr int PACKED_K = 256;           // k of a stage of codes: 128 bytes a fe
 template <int KIND, int TOK> struct Sizes {
     static constexpr int PARTS = KIND == FOUR_F32 ? 3 : 1;
     static constexpr int BK = KIND == EIGHT ? 128 : 64;              // 128 bytes a row of either operand
-    static constexpr int A_BYTES = FEATURES * 128;
+    static constexpr int CODES_BYTES = FEATURES * 128;
+    static constexpr int A_BYTES = KIND == EIGHT ? FEATURES * 128 : 0;
     static constexpr int B_BYTES = PARTS * TOK * 128;
-    static constexpr int PACKED = KIND == EIGHT ? 0 : 2;             // stages of codes
-    // a block of up to 64 rows shares its SM with another; one of more has it to itself
-    static constexpr int BLOCKS = (TOK <= 64 && PARTS == 1) || TOK <= 32 ? 2 : 1;
-    static constexpr int ROOM = BLOCKS == 2 ? 110 * 1024 : 220 * 1024;
-    static constexpr int FIT = (ROOM - PACKED * A_BYTES) / (A_BYTES + B_BYTES);
-    static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int N = PARTS * TOK;
-    static constexpr int TMEM = N <= 32 ? 32 : (N <= 64 ? 64 : (N <= 128 ? 128 : 256));
+    static constexpr int USED = N + (KIND == EIGHT ? 0 : WEIGHT_STAGES * WEIGHT_COLS);
+    static constexpr int TMEM = USED <= 32 ? 32 : (USED <= 64 ? 64 : (USED <= 128 ? 128 : (USED <= 256 ? 256 : 512)));
+    // a block of few rows shares its SM with another; one of more has it to itself
+    static constexpr int BLOCKS = N <= 96 ? 2 : 1;
+    static constexpr int ROOM = BLOCKS == 2 ? 110 * 1024 : 220 * 1024;
+    static constexpr int PACKED = KIND == EIGHT ? 0 : (BLOCKS == 2 ? 3 : 4);         // stages of codes
+    static constexpr int FIT = (ROOM - PACKED * CODES_BYTES) / (A_BYTES + B_BYTES);
+    static constexpr int STAGES = FIT > 8 ? 8 : FIT;
 };
 
 template <int KIND, int TOK> struct Storage {
     using S = Sizes<KIND, TOK>;
-    alignas(1024) uint8_t a[S::STAGES][S::A_BYTES];
     alignas(1024) uint8_t b[S::STAGES][S::B_BYTES];
-    alignas(1024) uint8_t codes[S::PACKED == 0 ? 1 : S::PACKED][S::PACKED == 0 ? 16 : S::A_BYTES];
-    alignas(8) uint64_t full[S::STAGES], empty[S::STAGES], codes_full[2], codes_empty[2], done;
+    alignas(1024) uint8_t a[KIND == EIGHT ? S::STAGES : 1][KIND == EIGHT ? S::A_BYTES : 16];
+    alignas(1024) uint8_t codes[S::PACKED == 0 ? 1 : S::PACKED][S::PACKED == 0 ? 16 : S::CODES_BYTES];
+    alignas(8) uint64_t full[S::STAGES], empty[S::STAGES];            // the copies' ring
+    uint64_t made[WEIGHT_STAGES], used[WEIGHT_STAGES];               // the weights' ring in tensor memory
+    uint64_t codes_full[4], codes_empty[4], done;
     uint32_t tmem;
     int abort_flag;
 };
@@ -76,8 +81,12 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
-            tc::mbar_init(&s.full[i], KIND == EIGHT ? 1 : 5);        // (the copy, and a set of four warps)
+            tc::mbar_init(&s.full[i], 1);
             tc::mbar_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < WEIGHT_STAGES; ++i) {
+            tc::mbar_init(&s.made[i], 4);                            // (a set of four warps)
+            tc::mbar_init(&s.used[i], 1);
         }
         for (int i = 0; i < S::PACKED; ++i) {
             tc::mbar_init(&s.codes_full[i], 1);
@@ -96,7 +105,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     tc::tc_fence_before_sync();
     __syncthreads();
     tc::tc_fence_after_sync();
-    const uint32_t tmem = s.tmem;
+    const uint32_t tmem = s.tmem, weights = tmem + S::TMEM - WEIGHT_STAGES * WEIGHT_COLS;
 
     if (warp == 0) {
         if (tc::elect_one()) {
@@ -117,8 +126,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                 if (++st == S::STAGES) st = 0, parity ^= 1;
             }
             if (*abort_flag) {
-                // our own copies land before the block's shared memory goes away.  (A stage's barrier may
-                // lack the arrivals of warps that gave up, so the bound is what ends this wait.)
+                // our own copies land before the block's shared memory goes away
                 for (int kb = max(0, sent - S::STAGES); kb < sent; ++kb)
                     for (uint32_t i = 0; i < tc::WAIT_LIMIT; ++i)
                         if (tc::mbar_try_wait(&s.full[kb % S::STAGES], (kb / S::STAGES) & 1)) break;
@@ -128,31 +136,34 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         if (tc::elect_one()) {
             const uint32_t idesc = KIND == EIGHT ? instr_desc_e4m3(FEATURES, tok) : tc::instr_desc_bf16(FEATURES, S::PARTS * tok);
             constexpr uint32_t A_STEP = S::A_BYTES >> 4, B_STEP = S::B_BYTES >> 4;
-            const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
-            const uint32_t desc_hi = (uint32_t)(desc0 >> 32), a_lo = (uint32_t)desc0;
-            const uint32_t b_lo = (uint32_t)tc::smem_desc_sw128(tc::smem_u32(s.b[0]));
-            const uint32_t full0 = tc::smem_u32(&s.full[0]), empty0 = tc::smem_u32(&s.empty[0]);
+            const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.b[0]));
+            const uint32_t desc_hi = (uint32_t)(desc0 >> 32), b_lo = (uint32_t)desc0;
+            const uint32_t a_lo = (uint32_t)tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
+            int st = 0, ws = 0;
+            uint32_t parity = 0, made_parity = 0, more = 0;
             bool ok = true;
-            uint32_t phase = 0;
-            for (int kb0 = 0; kb0 < n_kb && ok; kb0 += S::STAGES, phase ^= 1) {
+            for (int kb = 0; kb < n_kb; ++kb) {
+                ok = tc::mbar_wait(&s.full[st], parity, abort_flag);
+                if (KIND != EIGHT) ok = ok && tc::mbar_wait(&s.made[ws], made_parity, abort_flag);
+                if (!ok) {
+                    tc::give_up(abort_flag, status, tc::ST_MMA_TIMEOUT);
+                    break;
+                }
+                tc::tc_fence_after_sync();
 #pragma unroll
-                for (int st = 0; st < S::STAGES; ++st) {
-                    if (kb0 + st >= n_kb) break;
-                    if (!tc::mbar_wait_at(full0 + 8 * st, phase, abort_flag)) {
-                        tc::give_up(abort_flag, status, tc::ST_MMA_TIMEOUT);
-                        ok = false;
-                        break;
-                    }
-                    tc::tc_fence_after_sync();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {           // 32 bytes of K an instruction: two descriptor units
-                        const uint64_t a = tc::desc_of(a_lo + st * A_STEP + 2 * k, desc_hi);
-                        const uint64_t b = tc::desc_of(b_lo + st * B_STEP + 2 * k, desc_hi);
-                        const uint32_t more = kb0 > 0 || st > 0 || k > 0 ? 1u : 0u;
-                        if constexpr (KIND == EIGHT) umma_e4m3(tmem, a, b, idesc, more);
-                        else tc::umma_bf16(tmem, a, b, idesc, more);
-                    }
-                    tc::umma_commit_at(empty0 + 8 * st);
+                for (int k = 0; k < 4; ++k) {               // 32 bytes of K an instruction: two descriptor units
+                    const uint64_t b = tc::desc_of(b_lo + st * B_STEP + 2 * k, desc_hi);
+                    if constexpr (KIND == EIGHT)
+                        umma_e4m3(tmem, tc::desc_of(a_lo + st * A_STEP + 2 * k, desc_hi), b, idesc, more);
+                    else
+                        tc::umma_bf16_ts(tmem, weights + ws * WEIGHT_COLS + 8 * k, b, idesc, more);
+                    more = 1;
+                }
+                tc::umma_commit(&s.empty[st]);
+                if (++st == S::STAGES) st = 0, parity ^= 1;
+                if (KIND != EIGHT) {
+                    tc::umma_commit(&s.used[ws]);
+                    if (++ws == WEIGHT_STAGES) ws = 0, made_parity ^= 1;
                 }
             }
             if (ok) tc::umma_commit(&s.done);
@@ -167,7 +178,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                     tc::give_up(abort_flag, status, tc::ST_PRODUCER_TIMEOUT);
                     break;
                 }
-                tc::mbar_expect_tx(&s.codes_full[st], S::A_BYTES);
+                tc::mbar_expect_tx(&s.codes_full[st], S::CODES_BYTES);
                 tc::tma_load_2d(s.codes[st], &map_w, &s.codes_full[st], (k_begin + i * PACKED_K) / 2, n0);
                 sent = i + 1;
                 if (++st == S::PACKED) st = 0, parity ^= 1;
@@ -184,9 +195,10 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
         if constexpr (KIND != EIGHT) {
             const Scales scales(p, n);
             uint2 sc, next = scales.load(k_begin, k_end);
-            int slot = 0, pk = 0;
-            uint32_t slot_parity = 1, pk_parity = 0;
-            for (int kb = 0; kb < n_kb && ok; kb += 4) {
+            const uint32_t my_weights = weights + ((uint32_t)((warp & 3) * 32) << 16);
+            int pk = 0;
+            uint32_t pk_parity = 0, used_parity = 1;
+            for (int kb = 0; kb < n_kb && ok; kb += 4, used_parity ^= 1) {
                 ok = tc::mbar_wait(&s.codes_full[pk], pk_parity, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
@@ -199,21 +211,24 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (kb + j >= n_kb) break;
-                    if ((j & 1) == set) {
-                        if (kb + j >= S::STAGES) {
-                            ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
-                            ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) {
-                                tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
-                                break;
-                            }
+                    if ((j & 1) != set) continue;
+                    static_assert(WEIGHT_STAGES == 4, "a stage of codes goes once around the weights' ring");
+                    uint32_t v[32];
+                    make_weights(packed, j, r, scales.of(sc, 2 * j), v);
+                    if (kb > 0) {
+                        ok = tc::mbar_wait(&s.used[j], used_parity, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+                            break;
                         }
-                        make_weights(packed, j, r, scales.of(sc, 2 * j), s.a[slot] + r * 128);
-                        tc::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&s.full[slot]);
+                        tc::tc_fence_after_sync();
                     }
-                    if (++slot == S::STAGES) slot = 0, slot_parity ^= 1;
+                    tc::tmem_st_32x32(my_weights + j * WEIGHT_COLS, v);
+                    tc::tmem_st_wait();
+                    tc::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&s.made[j]);
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.codes_empty[pk]);
@@ -255,7 +270,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                 }
             }
         } else {
-            float* left = reinterpret_cast<float*>(s.a[0]);           // [row][feature]; the ring is free by now
+            float* left = reinterpret_cast<float*>(s.b[0]);           // [row][feature]; the ring is free by now
             if (ok) {
 #pragma unroll 1
                 for (int c = 32 * set; c < tok; c += 64) {
@@ -343,7 +358,7 @@ int launch(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w
            cudaStream_t stream) {
     constexpr int SMEM = (int)sizeof(Storage<KIND, TOK>) + 1024;
     static_assert(SMEM <= 232448, "a block's shared memory");
-    static_assert(TOK * FEATURES * 4 <= (int)(sizeof(Storage<KIND, TOK>::a) + sizeof(Storage<KIND, TOK>::b)),
+    static_assert(TOK * FEATURES * 4 <= (int)(sizeof(Storage<KIND, TOK>::a) * (KIND == EIGHT) + sizeof(Storage<KIND, TOK>::b)),
                   "the sums that a block leaves for its cluster must fit in the ring");
     static bool configured[64] = {};
     auto kernel = linear_tcgen05_kernel<KIND, TOK, BF16>;

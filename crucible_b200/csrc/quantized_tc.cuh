@@ -10,23 +10,24 @@ __device__ __forceinline__ uint32_t instr_desc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 64 codes of one feature (two runs of 32 k, a scale each) as bf16 weights in row `r` of a K-major tile of 128-byte
-// rows in the 128-byte swizzle; the codes lie in chunks 2j and 2j + 1 of row `r` of such a tile of codes.
-__device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, int r, uint32_t two_scales,
-                                             uint8_t* weights_row) {
+// 64 codes of one feature (two runs of 32 k, a scale each) as bf16 weights, two of neighbouring k a register; the codes
+// lie in chunks 2j and 2j + 1 of row `r` of a tile of 128-byte rows in the 128-byte swizzle.
+__device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, int r, uint32_t two_scales, uint32_t (&v)[32]) {
     const uint4 c0 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j) ^ (r & 7)) << 4));
     const uint4 c1 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j + 1) ^ (r & 7)) << 4));
     const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
     uint32_t s2[2], c2[2];
     scale_pairs(two_scales, s2, c2);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        uint32_t v[4];
+    for (int c = 0; c < 8; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
-        *reinterpret_cast<uint4*>(weights_row + ((c ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-    }
+        for (int i = 0; i < 4; ++i) v[4 * c + i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
 }
+
+// The weights' place is tensor memory, as the MMA's A operand: lane = feature, a column = two neighbouring k, 32 columns
+// a stage of 64 k.  (In shared memory they were 16 KB written and 16 KB read a stage beside the rows' and codes' own
+// bytes: 570 of the 656 cycles that a stage took with 256 rows, 600 with 16.)
+constexpr int WEIGHT_STAGES = 4, WEIGHT_COLS = 32;
 
 // The group scales of one feature, 256 k (eight runs of 32) at a time, asked for a stage of codes ahead.  Where 256 k
 // are whole groups and a feature's scales begin on a multiple of 8, 4 or 2 bytes, as those 256 k have, one load

@@ -282,7 +282,7 @@ def form_of(kind: int, m: int, n: int, k: int):
         form = "few" if m <= FEW_ROWS else "tiles" if kind == _FOUR_F32 or m <= 256 else "pairs"
     if form == "few":
         return ("few",)
-    most = 64 if kind == _FOUR_F32 else 256
+    most = 64 if kind == _FOUR_F32 else 192 if form == "pairs" and kind == _FOUR_BF16 else 256
     tok = _up(-(-m // -(-m // most)), 16)
     if form == "pairs":
         return "pairs", tok, 74
