@@ -25,34 +25,46 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// 4 consecutive elements from `at` of a row of `width`; zeros beyond it.
-template <typename T, bool VEC>
-__device__ __forceinline__ float4 load4(const T* __restrict__ row, int at, int width) {
-    float v[4];
-    if (VEC) {
-        if constexpr (sizeof(T) == 4) {
-            return *reinterpret_cast<const float4*>(row + at);
-        } else {
-            const uint2 raw = *reinterpret_cast<const uint2*>(row + at);
-            return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xFFFF0000u),
-                               __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xFFFF0000u));
-        }
-    }
+// E consecutive elements from `at` of a row of `width`; zeros beyond it.
+template <typename T, int E, bool VEC>
+__device__ __forceinline__ void load_chunk(const T* __restrict__ row, int at, int width, float (&v)[E]) {
+    if constexpr (VEC && sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = at + i < width ? cb_to_float(row[at + i]) : 0.f;
-    return make_float4(v[0], v[1], v[2], v[3]);
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ row, int at, int width, float4 v, float inv) {
-    const uint32_t lo = e4m3x2(v.x * inv, v.y * inv), hi = e4m3x2(v.z * inv, v.w * inv);
-    const uint32_t word = lo | (hi << 16);
-    if (VEC) {
-        *reinterpret_cast<uint32_t*>(row + at) = word;
+        for (int i = 0; i < E; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(row + at + i);
+            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+        }
+    } else if constexpr (VEC) {
+        uint32_t w[E / 2];
+        if constexpr (E == 8) {
+            const uint4 x = *reinterpret_cast<const uint4*>(row + at);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(row + at);
+            w[0] = x.x, w[1] = x.y;
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at + i < width) row[at + i] = (uint8_t)(word >> (8 * i));
+        for (int i = 0; i < E; ++i) v[i] = at + i < width ? cb_to_float(row[at + i]) : 0.f;
+    }
+}
+
+template <int E, bool VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ row, int at, int width, const float (&v)[E], float inv) {
+    uint32_t word[E / 4];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+        word[i] = e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) | (e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16);
+    if constexpr (VEC && E == 8) {
+        *reinterpret_cast<uint2*>(row + at) = make_uint2(word[0], word[1]);
+    } else if constexpr (VEC) {
+        *reinterpret_cast<uint32_t*>(row + at) = word[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (at + i < width) row[at + i] = (uint8_t)(word[i >> 2] >> (8 * (i & 3)));
     }
 }
 
@@ -76,59 +88,63 @@ __device__ __forceinline__ float row_max(uint32_t v, uint32_t* scratch) {
     return __uint_as_float(v);
 }
 
-__device__ __forceinline__ uint32_t magnitude(float4 v) {
-    const uint32_t m = 0x7FFFFFFFu;
-    return max(max(__float_as_uint(v.x) & m, __float_as_uint(v.y) & m),
-               max(__float_as_uint(v.z) & m, __float_as_uint(v.w) & m));
+template <int E> __device__ __forceinline__ uint32_t magnitude(const float (&v)[E]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
 }
 
 // max(v, LEAST) that keeps a NaN
 __device__ __forceinline__ float at_least(float v) { return v < LEAST ? LEAST : v; }
 
-// CH: chunks of 4 a thread.  WARP: a warp a row (blockDim.y rows a block), else a block a row.
+// CH: chunks a thread.  WARP: a warp a row (blockDim.y rows a block), else a block a row.
 template <typename D, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long long ldd,
-                             const float* __restrict__ gain, float eps, float* sum_out, long long lds,
-                             uint8_t* __restrict__ q, long long ldq, float* __restrict__ scales, int rows, int width) {
+__global__ void __launch_bounds__(WARP ? 128 : (CH < 8 ? 512 : 1024))
+norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long long ldd, const float* __restrict__ gain,
+             float eps, float* sum_out, long long lds, uint8_t* __restrict__ q, long long ldq,
+             float* __restrict__ scales, int rows, int width) {
+    constexpr int E = 4;
     __shared__ float scratch[32];
     cb_pdl_wait();
     const long long row = (long long)blockIdx.x * (WARP ? blockDim.y : 1) + (WARP ? threadIdx.y : 0);
     if (row >= rows) return;                           // (a whole warp at a time: only with WARP)
-    const int step = 4 * (WARP ? 32 : blockDim.x), at0 = 4 * threadIdx.x;
+    const int step = E * (WARP ? 32 : blockDim.x), at0 = E * threadIdx.x;
     const float* xr = x + row * ldx;
-    float4 v[CH];
+    float v[CH][E];
     float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
-        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < width) v[c] = load4<float, VEC>(xr, at, width);
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[c][i] = 0.f;
+        if (at < width) load_chunk<float, E, VEC>(xr, at, width, v[c]);
     }
     if (delta != nullptr) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = at0 + c * step;
             if (at < width) {
-                const float4 d = load4<D, VEC>(delta + row * ldd, at, width);
-                v[c].x += d.x, v[c].y += d.y, v[c].z += d.z, v[c].w += d.w;
+                float d[E];
+                load_chunk<D, E, VEC>(delta + row * ldd, at, width, d);
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[c][i] += d[i];
             }
         }
     }
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-        ss += (v[c].x * v[c].x + v[c].y * v[c].y) + (v[c].z * v[c].z + v[c].w * v[c].w);
+    for (int c = 0; c < CH; ++c) ss += (v[c][0] * v[c][0] + v[c][1] * v[c][1]) + (v[c][2] * v[c][2] + v[c][3] * v[c][3]);
     if (sum_out != nullptr) {
         float* sr = sum_out + row * lds;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = at0 + c * step;
             if (VEC) {
-                if (at < width) *reinterpret_cast<float4*>(sr + at) = v[c];
+                if (at < width) *reinterpret_cast<float4*>(sr + at) = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
             } else {
-                const float e[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at + i < width) sr[at + i] = e[i];
+                for (int i = 0; i < E; ++i)
+                    if (at + i < width) sr[at + i] = v[c][i];
             }
         }
     }
@@ -139,9 +155,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm8_kernel(const float* x
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
         if (at < width) {
-            const float4 w = load4<float, VEC>(gain, at, width);
-            v[c].x = v[c].x * r * w.x, v[c].y = v[c].y * r * w.y;
-            v[c].z = v[c].z * r * w.z, v[c].w = v[c].w * r * w.w;
+            float w[E];
+            load_chunk<float, E, VEC>(gain, at, width, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[c][i] = v[c][i] * r * w[i];
             top = max(top, magnitude(v[c]));
         }
     }
@@ -150,45 +167,49 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm8_kernel(const float* x
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
-        if (at < width) store_e4m3<VEC>(q + row * ldq, at, width, v[c], inv);
+        if (at < width) store_e4m3<E, VEC>(q + row * ldq, at, width, v[c], inv);
     }
     if (threadIdx.x == 0) scales[row] = most / E4M3_TOP;
 }
 
+// The exponential and the quotient of the hardware's unit: e^-g is off by 2^-22 + |g| 2^-24 relative to it, the quotient
+// by 2^-22; a row's numbers are then rounded to 2^-4.  With expf and the exact division 2,048 rows of 14,336 bf16
+// pairs took 77 us, which is what those instructions take.
 __device__ __forceinline__ float pair8(float g, float u, float limit, float alpha, float offset) {
     if (limit > 0.f) {
         // (written so that a NaN stays one)
         g = g > limit ? limit : g;
         u = (u > limit ? limit : (u < -limit ? -limit : u)) + offset;
-        return g / (1.0f + expf(-alpha * g)) * u;
+        return __fdividef(g, 1.0f + __expf(-alpha * g)) * u;
     }
-    return g / (1.0f + expf(-g)) * u;
+    return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
 template <typename T, int CH, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, long long ldq,
-                            float* __restrict__ scales, int rows, int width, float limit, float alpha, float offset) {
+__global__ void __launch_bounds__(WARP ? 128 : 1024)
+glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, long long ldq,
+            float* __restrict__ scales, int rows, int width, float limit, float alpha, float offset) {
+    constexpr int E = 16 / sizeof(T);
     __shared__ uint32_t scratch[32];
     cb_pdl_wait();
     const long long row = (long long)blockIdx.x * (WARP ? blockDim.y : 1) + (WARP ? threadIdx.y : 0);
     if (row >= rows) return;
-    const int step = 4 * (WARP ? 32 : blockDim.x), at0 = 4 * threadIdx.x;
+    const int step = E * (WARP ? 32 : blockDim.x), at0 = E * threadIdx.x;
     const T* gr = both + row * ldb;
     const T* ur = gr + width;
-    float4 v[CH];
+    float v[CH][E];
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
-        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (at < width) {
-            const float4 g = load4<T, VEC>(gr, at, width), u = load4<T, VEC>(ur, at, width);
-            v[c].x = pair8(g.x, u.x, limit, alpha, offset), v[c].y = pair8(g.y, u.y, limit, alpha, offset);
-            v[c].z = pair8(g.z, u.z, limit, alpha, offset), v[c].w = pair8(g.w, u.w, limit, alpha, offset);
-            if (!VEC) {                                // (an offset makes something of the zeros beyond the row)
-                if (at + 1 >= width) v[c].y = 0.f;
-                if (at + 2 >= width) v[c].z = 0.f;
-                if (at + 3 >= width) v[c].w = 0.f;
+            float g[E], u[E];
+            load_chunk<T, E, VEC>(gr, at, width, g);
+            load_chunk<T, E, VEC>(ur, at, width, u);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                v[c][i] = pair8(g[i], u[i], limit, alpha, offset);
+                if (!VEC && at + i >= width) v[c][i] = 0.f;        // (an offset makes something of the zeros beyond the row)
             }
             top = max(top, magnitude(v[c]));
         }
@@ -198,33 +219,41 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) glu8_kernel(const T* __rest
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
-        if (at < width) store_e4m3<VEC>(q + row * ldq, at, width, v[c], inv);
+        if (at < width) store_e4m3<E, VEC>(q + row * ldq, at, width, v[c], inv);
     }
     if (threadIdx.x == 0) scales[row] = most / E4M3_TOP;
 }
 
 constexpr int WARP_ROW = 512;           // widths up to here: a warp a row, 4 rows a block
 constexpr int WIDEST = 32768;
+constexpr int MANY_ROWS = 296;          // two for every SM
 
 struct Shape {
-    int chunks;                         // of 4 a thread: 1, 2, 4 or 8
+    int chunks;                         // a thread: 1, 2, 4 or 8
     bool warp;
     dim3 grid, block;
 };
 
-// A block a row: as few threads as hold it with 4 chunks each (8 beyond 16,384 numbers).
-inline Shape shape_of(int rows, int width) {
+// A block a row, of at most `most` threads (twice that where a row needs it).  Many rows: as many chunks of `e` a thread
+// as leave a block `least` threads, so that several blocks are on an SM and one's loads run beside another's sums; few
+// rows: as few chunks as there are threads for, since then the chain of one row is all there is.  us, 2,048 rows: norms
+// of 4,096 with 256 and 512 threads 17.9 and 18.1, of 2,048 8.0 and 11.3; pairs of 14,336 bf16 with 448 and 896 39.8
+// and 32.3, of 8,192 with 256 and 512 22.5 and 17.7.
+inline Shape shape_of(int rows, int width, int e, int least, int most) {
     Shape s;
-    const int quads = (width + 3) / 4;
+    const int all = (width + e - 1) / e;
     s.warp = width <= WARP_ROW;
     if (s.warp) {
-        s.chunks = quads <= 32 ? 1 : (quads <= 64 ? 2 : 4);
+        s.chunks = all <= 32 ? 1 : (all <= 64 ? 2 : 4);
         s.block = dim3(32, 4);
         s.grid = dim3((rows + 3) / 4);
         return s;
     }
-    s.chunks = quads <= 4096 ? 4 : 8;
-    s.block = dim3(((quads + s.chunks - 1) / s.chunks + 31) / 32 * 32);
+    s.chunks = 32 / e;
+    if (s.chunks == 8 && all <= 4 * most) s.chunks = 4;
+    if (rows < MANY_ROWS) least = most;
+    while (s.chunks > 1 && (all + s.chunks - 1) / s.chunks < least && (all + s.chunks / 2 - 1) / (s.chunks / 2) <= most) s.chunks /= 2;
+    s.block = dim3(((all + s.chunks - 1) / s.chunks + 31) / 32 * 32);
     s.grid = dim3(rows);
     return s;
 }
@@ -241,7 +270,7 @@ void launch_norm8(const Shape& s, const float* x, long long ldx, const D* delta,
     if (s.warp)
         s.chunks == 1 ? CB_NORM8(1, true) : (s.chunks == 2 ? CB_NORM8(2, true) : CB_NORM8(4, true));
     else
-        s.chunks == 4 ? CB_NORM8(4, false) : CB_NORM8(8, false);
+        s.chunks == 1 ? CB_NORM8(1, false) : (s.chunks == 2 ? CB_NORM8(2, false) : (s.chunks == 4 ? CB_NORM8(4, false) : CB_NORM8(8, false)));
 #undef CB_NORM8
 }
 
@@ -251,10 +280,11 @@ void launch_glu8(const Shape& s, const T* both, long long ldb, uint8_t* q, long 
 #define CB_GLU8(CH, WARP)                                                                                        \
     cb_launch(glu8_kernel<T, CH, WARP, VEC>, s.grid, s.block, 0, stream, both, ldb, q, ldq, scales, rows, width, \
               limit, alpha, offset)
+    constexpr bool F32 = sizeof(T) == 4;               // (bf16 chunks are 8 long: no row has more than 4 a thread)
     if (s.warp)
         s.chunks == 1 ? CB_GLU8(1, true) : (s.chunks == 2 ? CB_GLU8(2, true) : CB_GLU8(4, true));
     else
-        s.chunks == 4 ? CB_GLU8(4, false) : CB_GLU8(8, false);
+        s.chunks == 1 ? CB_GLU8(1, false) : (s.chunks == 2 ? CB_GLU8(2, false) : (s.chunks == 4 ? CB_GLU8(4, false) : CB_GLU8((F32 ? 8 : 4), false)));
 #undef CB_GLU8
 }
 
@@ -268,7 +298,7 @@ CB_EXPORT int cb_norm8(const float* x, long long ldx, const void* delta, int del
                        float* scales, int rows, int width, void* stream) {
     if (rows <= 0) return 0;
     if (width <= 0 || width > WIDEST) return CB_ERR_UNSUPPORTED;
-    const Shape s = shape_of(rows, width);
+    const Shape s = shape_of(rows, width, 4, 256, 512);
     const int dsize = delta_dtype == CB_BF16 ? 2 : 4;
     const bool vec = width % 4 == 0 && ldx % 4 == 0 && ldq % 4 == 0 && aligned(x, 16) && aligned(gain, 16) &&
                      aligned(q, 4) && (!sum_out || (lds % 4 == 0 && aligned(sum_out, 16))) &&
@@ -291,9 +321,9 @@ CB_EXPORT int cb_glu8(const void* both, int dtype, long long ldb, void* q, long 
                       int width, float limit, float alpha, float offset, void* stream) {
     if (rows <= 0) return 0;
     if (width <= 0 || width > WIDEST) return CB_ERR_UNSUPPORTED;
-    const Shape s = shape_of(rows, width);
-    const int size = dtype == CB_BF16 ? 2 : 4;
-    const bool vec = width % 4 == 0 && ldb % 4 == 0 && ldq % 4 == 0 && aligned(both, 4 * size) && aligned(q, 4);
+    const int e = dtype == CB_BF16 ? 8 : 4;            // 16 bytes
+    const Shape s = shape_of(rows, width, e, 512, 1024);
+    const bool vec = width % e == 0 && ldb % e == 0 && ldq % e == 0 && aligned(both, 16) && aligned(q, e);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == CB_BF16) {
         const __nv_bfloat16* b = (const __nv_bfloat16*)both;

@@ -16,11 +16,12 @@ allocates from torch's pool, as any captured torch operation does).
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
-from . import LAUNCHES, KernelError, _check, _code, _need_cuda, _ptr, _stream, build, tensor_core
+from . import LAUNCHES, KernelError, _check, _need_cuda, _ptr, _stream, build, tensor_core
 
 build.register_module("rows8", ["common.cuh"])
 build.register_module("linear_quantized_few", ["common.cuh", "quantized.cuh"])
@@ -34,22 +35,25 @@ _FOUR_BF16, _FOUR_F32, _EIGHT = 0, 1, 2
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
-class _Device:
-    """Makes the tensors' device the current one for a launch, where it is not."""
+# Every function asks first whether all is as it usually is, in one expression over plain attributes; only where it is
+# not are the tensors looked over one by one, for what is refused and for what is unusual but taken (a row of any
+# stride where there is one row, say).  Looked over one by one they took 6 to 11 us of host time a call, which
+# for a few rows is more than the kernel takes; the one expression takes 2 to 3.
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-        self.before = None
+_F32 = torch.float32
+_device_now = torch._C._cuda_getDevice
 
-    def __enter__(self):
-        now = torch._C._cuda_getDevice()
-        if now != self.index:
-            self.before = now
-            torch.cuda.set_device(self.index)
 
-    def __exit__(self, *_):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def _at(dev: int, call, *args) -> int:
+    """call(*args, stream) with device `dev` the current one."""
+    now = _device_now()
+    if now == dev:
+        return call(*args, _stream())
+    torch.cuda.set_device(dev)
+    try:
+        return call(*args, _stream())
+    finally:
+        torch.cuda.set_device(now)
 
 
 def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
@@ -91,12 +95,34 @@ def add_rmsnorm8(x: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.Ten
     (e4m3 [T, W]) and `scales` (float32 [T]).  `x`: the float32 residual; `delta`: float32 or bfloat16 rows
     to add to it, or None.  The sum goes to `sum_out`, which is `x` itself if a delta is given and
     nothing else is said (without either, `x` is only read)."""
+    if sum_out is None and delta is not None:
+        sum_out = x
+    dev, shape, xs, os = x.get_device(), x.shape, x.stride(), out.stride()
+    ss = xs if sum_out is None or sum_out is x else sum_out.stride()
+    ds = xs if delta is None else delta.stride()
+    if not (dev >= 0 and len(shape) == 2 and x.dtype is _F32 and out.dtype is E4M3 and scales.dtype is _F32
+            and gain.dtype is _F32 and out.shape == shape and xs[1] == 1 == os[1] and xs[0] >= shape[1] <= os[0]
+            and gain.shape == (shape[1],) and scales.shape == (shape[0],) and gain.is_contiguous() and scales.is_contiguous()
+            and out.get_device() == dev == gain.get_device() and scales.get_device() == dev
+            and (delta is None or (delta.shape == shape and delta.dtype in _FLOATS and ds[1] == 1
+                                   and ds[0] >= shape[1] and delta.get_device() == dev))
+            and (ss is xs or (sum_out.shape == shape and sum_out.dtype is _F32 and ss[1] == 1
+                              and ss[0] >= shape[1] and sum_out.get_device() == dev))):
+        _look_over_norm8(x, delta, gain, out, scales, sum_out)
+    lib = build.load("rows8")
+    code = _at(dev, lib.cb_norm8, x.data_ptr(), xs[0], _ptr(delta), 1 if delta is not None and delta.dtype is not _F32 else 0,
+               ds[0], gain.data_ptr(), eps, _ptr(sum_out), ss[0], out.data_ptr(), os[0], scales.data_ptr(),
+               shape[0], shape[1])
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"add_rmsnorm8 takes rows of 1 to {lib.cb_rows8_widest()} features, got {shape[1]}")
+    _check(code, "add_rmsnorm8")
+
+
+def _look_over_norm8(x, delta, gain, out, scales, sum_out) -> None:
     _rows(x, "add_rmsnorm8 input", (torch.float32,))
     rows, width = x.shape
     if delta is not None:
         _rows(delta, "add_rmsnorm8 delta", _FLOATS, (rows, width))
-        if sum_out is None:
-            sum_out = x
     if sum_out is not None:
         _rows(sum_out, "add_rmsnorm8 sum", (torch.float32,), (rows, width))
     _vector(gain, "add_rmsnorm8 gain", width)
@@ -104,15 +130,6 @@ def add_rmsnorm8(x: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.Ten
     _vector(scales, "add_rmsnorm8 scales", rows)
     _need_cuda(x, delta, gain, out, scales, sum_out)
     _one_device(x, delta, gain, out, scales, sum_out)
-    lib = build.load("rows8")
-    with _Device(x):
-        code = lib.cb_norm8(_ptr(x), x.stride(0), _ptr(delta), _code(delta.dtype) if delta is not None else 0,
-                            delta.stride(0) if delta is not None else 0, _ptr(gain), eps, _ptr(sum_out),
-                            sum_out.stride(0) if sum_out is not None else 0, _ptr(out), out.stride(0), _ptr(scales),
-                            rows, width, _stream())
-    if code == build.UNSUPPORTED:
-        raise KernelError(f"add_rmsnorm8 takes rows of 1 to {lib.cb_rows8_widest()} features, got {width}")
-    _check(code, "add_rmsnorm8")
 
 
 def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Optional[float] = None,
@@ -120,23 +137,30 @@ def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Opt
     """The gated pair of rows [g: F | u: F] in 8 bits: `out` (e4m3 [T, F]) and `scales` (float32 [T]).
     `limit` None: silu(g) * u.  A number: the capped pair of `ops.glu`, g' sigmoid(alpha g') (u' + offset)
     with g' = min(g, limit), u' = clamp(u, -limit, limit)."""
+    dev, shape, bs, os = both.get_device(), out.shape, both.stride(), out.stride()
+    if not (dev >= 0 and len(shape) == 2 and both.dtype in _FLOATS and out.dtype is E4M3 and scales.dtype is _F32
+            and both.shape == (shape[0], 2 * shape[1]) and bs[1] == 1 == os[1] and bs[0] >= 2 * shape[1]
+            and os[0] >= shape[1] and scales.shape == (shape[0],) and scales.is_contiguous()
+            and out.get_device() == dev == scales.get_device() and (limit is None or limit > 0)):
+        _look_over_glu8(both, out, scales, limit)
+    lib = build.load("rows8")
+    code = _at(dev, lib.cb_glu8, both.data_ptr(), 0 if both.dtype is _F32 else 1, bs[0], out.data_ptr(), os[0],
+               scales.data_ptr(), shape[0], shape[1], limit if limit is not None else 0.0, alpha, offset)
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"glu8 takes 1 to {lib.cb_rows8_widest()} features, got {shape[1]}")
+    _check(code, "glu8")
+
+
+def _look_over_glu8(both, out, scales, limit) -> None:
     _rows(both, "glu8 input", _FLOATS)
-    rows, width = both.shape[0], both.shape[1] // 2
     if both.shape[1] % 2:
         raise KernelError(f"glu8 takes rows [g | u] of an even width, got {both.shape[1]}")
     if limit is not None and not limit > 0:
         raise KernelError("glu8: the limit must be positive")
-    _rows(out, "glu8 output", (E4M3,), (rows, width))
-    _vector(scales, "glu8 scales", rows)
+    _rows(out, "glu8 output", (E4M3,), (both.shape[0], both.shape[1] // 2))
+    _vector(scales, "glu8 scales", both.shape[0])
     _need_cuda(both, out, scales)
     _one_device(both, out, scales)
-    lib = build.load("rows8")
-    with _Device(both):
-        code = lib.cb_glu8(_ptr(both), _code(both.dtype), both.stride(0), _ptr(out), out.stride(0), _ptr(scales),
-                           rows, width, limit if limit is not None else 0.0, alpha, offset, _stream())
-    if code == build.UNSUPPORTED:
-        raise KernelError(f"glu8 takes 1 to {lib.cb_rows8_widest()} features, got {width}")
-    _check(code, "glu8")
 
 
 # ---------------------------------------------------------------------------
@@ -167,14 +191,20 @@ class Weights8:
     that do, once, here."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        _rows(values, "8-bit weights", (E4M3,))
-        if values.shape[0] == 0 or values.shape[1] == 0:
-            raise KernelError(f"8-bit weights: an empty matrix {list(values.shape)}")
-        _vector(scales, "8-bit weights' scales", values.shape[0])
-        _one_device(values, scales)
+        shape = values.shape
+        if not (len(shape) == 2 and values.dtype is E4M3 and scales.dtype is _F32 and values.is_contiguous()
+                and scales.shape == (shape[0],) and scales.is_contiguous() and shape[0] and shape[1]
+                and values.get_device() == scales.get_device()):
+            _rows(values, "8-bit weights", (E4M3,))
+            if values.shape[0] == 0 or values.shape[1] == 0:
+                raise KernelError(f"8-bit weights: an empty matrix {list(values.shape)}")
+            _vector(scales, "8-bit weights' scales", values.shape[0])
+            _one_device(values, scales)
         self.values = values if _aligned16(values) else _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
         self.scales = scales
-        self.shape = values.shape
+        self.shape = shape
+        self.pitch = _pitch(self.values)
+        self.device = values.get_device()
 
     @classmethod
     def pack(cls, w: torch.Tensor) -> "Weights8":
@@ -209,6 +239,17 @@ class Weights4:
     `scales`: float32 [N]."""
 
     def __init__(self, codes: torch.Tensor, group_scales: torch.Tensor, scales: torch.Tensor):
+        shape, groups = codes.shape, group_scales.shape
+        if (len(shape) == 2 == len(groups) and codes.dtype is torch.int32 and group_scales.dtype is E4M3
+                and scales.dtype is _F32 and groups[0] == shape[0] and scales.shape == (shape[0],) and shape[0] > 0
+                and groups[1] > 0 and shape[1] % (4 * groups[1]) == 0 and shape[1] > 0 and scales.is_contiguous()
+                and codes.is_contiguous() and group_scales.is_contiguous() and codes.data_ptr() % 16 == 0
+                and codes.get_device() == group_scales.get_device() == scales.get_device()):
+            self.codes, self.group_scales, self.scales = codes, group_scales, scales
+            self.group = shape[1] * 8 // groups[1]
+            self.shape = torch.Size((shape[0], shape[1] * 8))
+            self.device = codes.get_device()
+            return
         _rows(codes, "4-bit weights' codes", (torch.int32,))
         n, k = codes.shape[0], codes.shape[1] * 8
         if n == 0 or k == 0:
@@ -226,6 +267,7 @@ class Weights4:
         self.scales = scales
         self.group = k // groups
         self.shape = torch.Size((n, k))
+        self.device = codes.get_device()
 
     @classmethod
     def pack(cls, w: torch.Tensor, group: int = 64) -> "Weights4":
@@ -274,10 +316,11 @@ def _up(x: int, to: int) -> int:
     return (x + to - 1) // to * to
 
 
-def form_of(kind: int, m: int, n: int, k: int):
-    """Which kernel takes the product, and how: ("few",), ("tiles", rows a tile, shares of K) or ("pairs", rows a
+@functools.lru_cache(maxsize=4096)
+def _rule(forced, kind: int, m: int, n: int, k: int):
+    """Which kernel takes a product, and how: ("few",), ("tiles", rows a tile, shares of K) or ("pairs", rows a
     tile, pairs of SMs)."""
-    form = FORM
+    form = forced
     if form is None or (form == "pairs" and kind == _FOUR_F32):
         form = "few" if m <= FEW_ROWS else "tiles" if kind == _FOUR_F32 or m <= 256 else "pairs"
     if form == "few":
@@ -292,28 +335,36 @@ def form_of(kind: int, m: int, n: int, k: int):
     return "tiles", tok, max(1, min(8, slots // tiles, units // 2))
 
 
-def _product(kind: int, rows, row_scales, values, ldw: int, group_scales, w, group: int, out, add, what: str) -> None:
-    m, (n, k) = rows.shape[0], w.shape
+def form_of(kind: int, m: int, n: int, k: int):
+    return _rule(FORM, kind, m, n, k)
+
+
+def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ldw: int, group_scales, w, group: int, out,
+             ldo: int, add, what: str) -> None:
     if m == 0:
         return
-    form, *how = form_of(kind, m, n, k)
-    with _Device(rows):
-        common = (kind, _ptr(rows), _pitch(rows), _ptr(row_scales), _ptr(values), ldw, _ptr(group_scales),
-                  _ptr(w.scales), _ptr(add), add.stride(0) if add is not None else 0, _ptr(out), _code(out.dtype),
-                  out.stride(0), m, n, k, group)
-        if form == "few":
-            code = build.load("linear_quantized_few").cb_linear_quantized_few(*common, _stream())
-        elif form == "pairs":
-            code = build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs(
-                *common, *how, _ptr(tensor_core.status_word(rows.device)), _stream())
+    n, k = w.shape
+    form = form_of(kind, m, n, k)
+    common = (kind, rows.data_ptr(), ldr, row_scales, values.data_ptr(), ldw, group_scales, w.scales.data_ptr(),
+              _ptr(add), add.stride(0) if add is not None else 0, out.data_ptr(), 0 if out.dtype is _F32 else 1, ldo, m, n, k,
+              group)
+    if form[0] == "few":
+        code = _at(dev, build.load("linear_quantized_few").cb_linear_quantized_few, *common)
+    else:
+        status = tensor_core._status.get(dev)
+        if status is None:
+            status = tensor_core.status_word(rows.device)
+        if form[0] == "pairs":
+            code = _at(dev, build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs, *common, form[1],
+                       form[2], status.data_ptr())
         else:
             parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device) if kind == _FOUR_F32 else None
-            code = build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05(
-                *common, *how, _ptr(parts), _ptr(tensor_core.status_word(rows.device)), _stream())
+            code = _at(dev, build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05, *common, form[1], form[2],
+                       _ptr(parts), status.data_ptr())
             if kind == _FOUR_F32 and code == 0:
                 LAUNCHES[0] += 1                       # (the rows' parts)
     if code == build.UNSUPPORTED:
-        raise KernelError(f"{what}: sizes out of range: rows {list(rows.shape)}, weights {list(w.shape)}")
+        raise KernelError(f"{what}: sizes out of range: rows [{m}, {k}], weights [{n}, {k}]")
     _check(code, what)
 
 
@@ -323,15 +374,24 @@ def linear8(rows: torch.Tensor, row_scales: torch.Tensor, w: Weights8, out: torc
     or bfloat16 [M, N]; `add`: float32 [M, N], which may be `out`."""
     if not isinstance(w, Weights8):
         raise KernelError(f"linear8 takes Weights8, got {type(w).__name__}")
+    dev, shape, rs, os = rows.get_device(), rows.shape, rows.stride(), out.stride()
     n, k = w.shape
-    _rows(rows, "linear8 rows", (E4M3,), (rows.shape[0], k))
-    _vector(row_scales, "linear8 row scales", rows.shape[0])
-    _out_rows(out, add, (rows.shape[0], n), "linear8")
-    _need_cuda(rows, row_scales, w.values, out, add)
-    _one_device(rows, row_scales, w.values, out, add)
-    if not _aligned16(rows):
-        rows = _in_aligned_rows(rows.view(torch.uint8)).view(E4M3)
-    _product(_EIGHT, rows, row_scales, w.values, _pitch(w.values), None, w, 0, out, add, "linear (8-bit weights)")
+    if not (dev == w.device >= 0 and len(shape) == 2 and shape[1] == k and rows.dtype is E4M3 and row_scales.dtype is _F32
+            and row_scales.shape == (shape[0],) and row_scales.is_contiguous() and out.dtype in _FLOATS
+            and out.shape == (shape[0], n) and rs[1] == 1 == os[1] and rs[0] >= k and os[0] >= n
+            and out.get_device() == dev == row_scales.get_device() and rs[0] % 16 == 0 and rows.data_ptr() % 16 == 0
+            and (add is None or (add.dtype is _F32 and add.shape == out.shape and add.is_contiguous()
+                                 and add.get_device() == dev))):
+        _rows(rows, "linear8 rows", (E4M3,), (rows.shape[0], k))
+        _vector(row_scales, "linear8 row scales", rows.shape[0])
+        _out_rows(out, add, (rows.shape[0], n), "linear8")
+        _need_cuda(rows, row_scales, w.values, out, add)
+        _one_device(rows, row_scales, w.values, out, add)
+        if not _aligned16(rows):
+            rows = _in_aligned_rows(rows.view(torch.uint8)).view(E4M3)
+        rs = (_pitch(rows),)
+    _product(_EIGHT, dev, rows, shape[0], rs[0], row_scales.data_ptr(), w.values, w.pitch, None, w, 0, out, os[0],
+             add, "linear (8-bit weights)")
 
 
 def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch.Tensor] = None) -> None:
@@ -339,12 +399,20 @@ def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch
     float32 [M, N], which may be `out`."""
     if not isinstance(w, Weights4):
         raise KernelError(f"linear4 takes Weights4, got {type(w).__name__}")
+    dev, shape, rs, os = a.get_device(), a.shape, a.stride(), out.stride()
     n, k = w.shape
-    _rows(a, "linear4 rows", _FLOATS, (a.shape[0], k))
-    _out_rows(out, add, (a.shape[0], n), "linear4")
-    _need_cuda(a, w.codes, out, add)
-    _one_device(a, w.codes, out, add)
-    if not _aligned16(a):
-        a = _in_aligned_rows(a)
-    _product(_FOUR_F32 if a.dtype == torch.float32 else _FOUR_BF16, a, None, w.codes, k // 2, w.group_scales, w,
-             w.group, out, add, "linear (4-bit weights)")
+    f32 = a.dtype is _F32
+    if not (dev == w.device >= 0 and len(shape) == 2 and shape[1] == k and a.dtype in _FLOATS and out.dtype in _FLOATS
+            and out.shape == (shape[0], n) and rs[1] == 1 == os[1] and rs[0] >= k and os[0] >= n
+            and out.get_device() == dev and rs[0] % 8 == 0 and a.data_ptr() % 16 == 0
+            and (add is None or (add.dtype is _F32 and add.shape == out.shape and add.is_contiguous()
+                                 and add.get_device() == dev))):
+        _rows(a, "linear4 rows", _FLOATS, (a.shape[0], k))
+        _out_rows(out, add, (a.shape[0], n), "linear4")
+        _need_cuda(a, w.codes, out, add)
+        _one_device(a, w.codes, out, add)
+        if not _aligned16(a):
+            a = _in_aligned_rows(a)
+        rs = (_pitch(a),)
+    _product(_FOUR_F32 if f32 else _FOUR_BF16, dev, a, shape[0], rs[0], None, w.codes, k // 2, w.group_scales.data_ptr(),
+             w, w.group, out, os[0], add, "linear (4-bit weights)")
