@@ -272,7 +272,7 @@ CB_EXPORT int cb_linear_quantized_few(int kind, const void* rows, long long ldr,
                                       int N, int K, int group, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     const int size = kind == EIGHT ? 1 : (kind == FOUR_F32 ? 4 : 2);
-    if (K <= 0 || K > MOST_K || (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
+    if (K <= 0 || K > MOST_K || ldw > MOST_PITCH || (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
         (M + 15) / 16 > 65535 || (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;
     const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,

@@ -1,14 +1,15 @@
 // out[M,N] = rows[M,K] . W[N,K]^T over quantised weights for many rows (prompts): two SMs on one tile.
 //
-// A pair of blocks multiplies 256 features by up to 256 rows (192 over 4-bit weights) (tcgen05.mma cta_group::2): each block
+// A pair of blocks multiplies 256 features by up to 256 rows (tcgen05.mma cta_group::2): each block
 // brings 128 of the features and half of the rows, so a block fetches as many bytes for its 128 x 256 sums as
 // a lone one would for 256 x 256, and both halves of tensor memory are free to take turns.  Pairs stay on
 // their SMs and walk the tiles; while the sums of one leave tensor memory, the other half takes the next.
 //
 //   EIGHT      both operands e4m3 by TMA, 128 k a stage, kind::f8f6f4
 //   FOUR_BF16  the codes by TMA, 256 k a stage; eight warps of each block make bf16 weights of them
-//              (exact, see quantized.cuh), 64 k a stage, a feature a thread, and put them into tensor
-//              memory, where the MMA takes them from: four stages of them leave room for twice 192 rows
+//              (exact, see quantized.cuh), 64 k a stage of the MMA's ring, a feature a thread.  (In tensor memory,
+//              where lone blocks keep them, they leave room for 192 rows twice, not 256, and what a stage takes
+//              is the making: 557 cycles a stage of 192 rows against 656 of 256.)
 //
 // fp32 results.  The tensor cores cut off what an addition leaves below the sum's last bit, always towards
 // zero, and over a long K that adds up (K = 14,336 in one sum: 4.2e-6 of the result's norm).  So a
@@ -25,27 +26,21 @@ namespace {
 
 constexpr int MINE = 128;               // features of a block
 constexpr int PACKED_K = 256;
-constexpr int PACKED = 4;
+constexpr int PACKED = 2;                // (more stages of codes change nothing)
 constexpr int TILE_BYTES = MINE * 128;
 constexpr int CHUNK = 2048;             // K of one sum, fp32 results
 
 template <int KIND> struct Sizes {
     static constexpr int BK = KIND == EIGHT ? 128 : 64;
-    static constexpr int STAGES = KIND == EIGHT ? 6 : 8;
-    static constexpr int MOST_ROWS = KIND == EIGHT ? 256 : 192;
-    static constexpr int B_BYTES = MOST_ROWS / 2 * 128;
-    static constexpr int HALF = KIND == EIGHT ? 256 : 192;           // columns from one half of tensor memory to the other
+    static constexpr int STAGES = KIND == EIGHT ? 6 : 5;
     static constexpr int THREADS = KIND == EIGHT ? 320 : 608;
 };
 
 template <int KIND> struct Storage {
-    using S = Sizes<KIND>;
-    alignas(1024) uint8_t b[S::STAGES][S::B_BYTES];
-    alignas(1024) uint8_t a[KIND == EIGHT ? S::STAGES : 1][KIND == EIGHT ? TILE_BYTES : 16];
+    alignas(1024) uint8_t a[Sizes<KIND>::STAGES][TILE_BYTES];
+    alignas(1024) uint8_t b[Sizes<KIND>::STAGES][TILE_BYTES];
     alignas(1024) uint8_t codes[KIND == EIGHT ? 1 : PACKED][KIND == EIGHT ? 16 : TILE_BYTES];
-    alignas(8) uint64_t full[S::STAGES], empty[S::STAGES];           // the copies' ring
-    uint64_t made[WEIGHT_STAGES], used[WEIGHT_STAGES];              // the weights' ring in tensor memory
-    uint64_t codes_full[PACKED], codes_empty[PACKED];
+    alignas(8) uint64_t full[Sizes<KIND>::STAGES], empty[Sizes<KIND>::STAGES], codes_full[PACKED], codes_empty[PACKED];
     uint64_t done[2], taken[2];         // a half of tensor memory: its sums are whole; they are out of it
     uint32_t tmem;
     int abort_flag;
@@ -72,17 +67,16 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
                  ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-__device__ __forceinline__ void pair_mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-// A in tensor memory: each block's own 128 rows
-__device__ __forceinline__ void pair_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+template <int KIND>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (KIND == EIGHT)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
 // The tiles of a pair in the order in which every role walks them: the rows' tiles of one run of
@@ -118,12 +112,8 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            tc::mbar_init(&s.full[i], 1);
+            tc::mbar_init(&s.full[i], KIND == EIGHT ? 1 : 9);        // (the copies, and four warps of each block)
             tc::mbar_init(&s.empty[i], 1);
-        }
-        for (int i = 0; i < WEIGHT_STAGES; ++i) {
-            tc::mbar_init(&s.made[i], 8);                            // (a set of four warps of each block)
-            tc::mbar_init(&s.used[i], 1);
         }
         for (int i = 0; i < PACKED; ++i) {
             tc::mbar_init(&s.codes_full[i], 1);
@@ -146,7 +136,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
     __syncthreads();
     tc::cluster_sync_all();             // the other block's barriers are ready too
     tc::tc_fence_after_sync();
-    const uint32_t tmem = s.tmem, weights = tmem + 512 - WEIGHT_STAGES * WEIGHT_COLS;
+    const uint32_t tmem = s.tmem;
     Units u(p, tok, blockIdx.x >> 1, gridDim.x >> 1, chunk_k);
 
     if (warp == 0) {
@@ -173,8 +163,9 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
                 }
             }
             if (*abort_flag && rank == 0) {
-                // both blocks' copies land before their shared memory goes away (the barrier of the cluster is
-                // behind this)
+                // both blocks' copies land before their shared memory goes away (the barrier of the
+                // cluster is behind this).  A stage's barrier may lack arrivals of warps that gave
+                // up, so the bound is what ends this wait.
                 for (long long i = sent > STAGES ? sent - STAGES : 0; i < sent; ++i)
                     for (uint32_t j = 0; j < tc::WAIT_LIMIT; ++j)
                         if (tc::mbar_try_wait(&s.full[i % STAGES], (uint32_t)(i / STAGES) & 1)) break;
@@ -183,12 +174,12 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
     } else if (warp == 1) {
         if (rank == 0 && tc::elect_one()) {
             const uint32_t idesc = KIND == EIGHT ? instr_desc_e4m3(2 * MINE, tok) : tc::instr_desc_bf16(2 * MINE, tok);
-            constexpr uint32_t A_STEP = TILE_BYTES >> 4, B_STEP = Sizes<KIND>::B_BYTES >> 4;
-            const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.b[0]));
-            const uint32_t desc_hi = (uint32_t)(desc0 >> 32), b_lo = (uint32_t)desc0;
-            const uint32_t a_lo = (uint32_t)tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
-            int st = 0, at = 0, ws = 0;
-            uint32_t parity = 0, made_parity = 0;
+            constexpr uint32_t STEP = TILE_BYTES >> 4;
+            const uint64_t desc0 = tc::smem_desc_sw128(tc::smem_u32(s.a[0]));
+            const uint32_t desc_hi = (uint32_t)(desc0 >> 32), a_lo = (uint32_t)desc0;
+            const uint32_t b_lo = (uint32_t)tc::smem_desc_sw128(tc::smem_u32(s.b[0]));
+            int st = 0, at = 0;
+            uint32_t parity = 0;
             bool ok = true;
             for (; u.more() && ok; u.advance(), ++at) {
                 const int half = at & 1;
@@ -197,31 +188,23 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
                     break;
                 }
                 tc::tc_fence_after_sync();
-                const uint32_t d = tmem + half * Sizes<KIND>::HALF;
+                const uint32_t d = tmem + half * 256;
                 uint32_t more = 0;
                 for (int k = u.k_begin(), k_end = u.k_end(); k < k_end; k += BK) {
-                    ok = tc::mbar_wait(&s.full[st], parity, abort_flag);
-                    if (KIND != EIGHT) ok = ok && tc::mbar_wait(&s.made[ws], made_parity, abort_flag);
-                    if (!ok) {
+                    if (!tc::mbar_wait(&s.full[st], parity, abort_flag)) {
                         tc::give_up(abort_flag, status, tc::ST_MMA_TIMEOUT);
+                        ok = false;
                         break;
                     }
                     tc::tc_fence_after_sync();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint64_t b = tc::desc_of(b_lo + st * B_STEP + 2 * i, desc_hi);
-                        if constexpr (KIND == EIGHT)
-                            pair_mma_e4m3(d, tc::desc_of(a_lo + st * A_STEP + 2 * i, desc_hi), b, idesc, more);
-                        else
-                            pair_mma_bf16_ts(d, weights + ws * WEIGHT_COLS + 8 * i, b, idesc, more);
+                        pair_mma<KIND>(d, tc::desc_of(a_lo + st * STEP + 2 * i, desc_hi),
+                                       tc::desc_of(b_lo + st * STEP + 2 * i, desc_hi), idesc, more);
                         more = 1;
                     }
                     pair_commit(&s.empty[st]);
                     if (++st == STAGES) st = 0, parity ^= 1;
-                    if (KIND != EIGHT) {
-                        pair_commit(&s.used[ws]);
-                        if (++ws == WEIGHT_STAGES) ws = 0, made_parity ^= 1;
-                    }
                 }
                 if (ok) pair_commit(&s.done[half]);
             }
@@ -244,7 +227,7 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
             const bool first = u.chunk == 0;
             const float* add = first ? p.add : static_cast<const float*>(p.out);
             const long long lda = first ? p.lda : p.ldo;
-            const uint32_t mine = tmem + half * Sizes<KIND>::HALF + ((uint32_t)((warp & 3) * 32) << 16);
+            const uint32_t mine = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll 1
             for (int c = 32 * ((warp - 2) >> 2); c < m_end - m0; c += 64) {
                 uint32_t x[32];
@@ -288,11 +271,9 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
         if constexpr (KIND != EIGHT) {
             const int r = (warp & 3) * 32 + lane, set = (warp - 11) >> 2;
             // (the ring's slots and the stages of codes go on from one unit to the next, and so do the turns)
-            const uint32_t my_weights = weights + ((uint32_t)((warp & 3) * 32) << 16);
-            // (the rings go on from one unit to the next, and so do the turns)
-            int ws = 0, pk = 0;
-            bool around = false;
-            uint32_t used_parity = 1, pk_parity = 0;
+            int slot = 0, pk = 0;
+            long long made = 0;
+            uint32_t slot_parity = 1, pk_parity = 0;
             bool ok = true;
             for (; u.more() && ok; u.advance()) {
                 const int n = (u.n_tile() * 2 + (int)rank) * MINE + r, k_end = u.k_end();
@@ -307,22 +288,25 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (k + 64 * j >= k_end) break;
-                        if ((ws & 1) == set) {
+                        if ((made & 1) == set) {
                             uint32_t v[32];
                             make_weights(s.codes[pk] + r * 128, j, r, scales.of(sc, 2 * j), v);
-                            if (around) {
-                                ok = tc::mbar_wait(&s.used[ws], used_parity, abort_flag);
+                            if (made >= STAGES) {
+                                ok = tc::mbar_wait(&s.empty[slot], slot_parity, abort_flag);
                                 ok = __all_sync(0xffffffffu, ok);
                                 if (!ok) break;
-                                tc::tc_fence_after_sync();
                             }
-                            tc::tmem_st_32x32(my_weights + ws * WEIGHT_COLS, v);
-                            tc::tmem_st_wait();
-                            tc::tc_fence_before_sync();
+                            uint8_t* to = s.a[slot] + r * 128;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) =
+                                    make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                            tc::fence_proxy_async();
                             __syncwarp();
-                            if (lane == 0) arrive_at(tc::cluster_map(tc::smem_u32(&s.made[ws]), 0));
+                            if (lane == 0) arrive_at(tc::cluster_map(tc::smem_u32(&s.full[slot]), 0));
                         }
-                        if (++ws == WEIGHT_STAGES) ws = 0, used_parity ^= 1, around = true;
+                        ++made;
+                        if (++slot == STAGES) slot = 0, slot_parity ^= 1;
                     }
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&s.codes_empty[pk]);
@@ -358,14 +342,14 @@ int launch(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w
 
 }  // namespace
 
-// `tok`: rows a tile, a multiple of 16 up to 256 (4-bit weights: 192); `pairs`: pairs of SMs to run on.
+// `tok`: rows a tile, a multiple of 16 up to 256; `pairs`: pairs of SMs to run on.
 CB_EXPORT int cb_linear_quantized_pairs(int kind, const void* rows, long long ldr, const float* row_scale, const void* w,
                                         long long ldw, const void* group_scale, const float* feature_scale,
                                         const float* add, long long lda, void* out, int out_dtype, long long ldo, int M,
                                         int N, int K, int group, int tok, int pairs, int* status, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     const int size = kind == EIGHT ? 1 : 2;
-    if ((kind != EIGHT && kind != FOUR_BF16) || K <= 0 || K > MOST_K || tok < 16 || tok % 16 || tok > (kind == EIGHT ? 256 : 192) || pairs < 1 ||
+    if ((kind != EIGHT && kind != FOUR_BF16) || K <= 0 || K > MOST_K || tok < 16 || tok % 16 || tok > 256 || pairs < 1 ||
         (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) ||
         (kind != EIGHT && (group <= 0 || group % 32 || K % group)))
         return CB_ERR_UNSUPPORTED;

@@ -25,6 +25,11 @@ constexpr int FEATURES = 128;
 constexpr int THREADS = 352;
 constexpr int PACKED_K = 256;           // k of a stage of codes: 128 bytes a feature
 
+// The weights' place is tensor memory, as the MMA's A operand: lane = feature, a column = two neighbouring k, 32 columns
+// a stage of 64 k.  (In shared memory they were 16 KB written and 16 KB read a stage beside the rows' and codes' own
+// bytes: 64 rows of 4,096 by 28,672 took 41 us, 31 like this.)
+constexpr int WEIGHT_STAGES = 4, WEIGHT_COLS = 32;
+
 template <int KIND, int TOK> struct Sizes {
     static constexpr int PARTS = KIND == FOUR_F32 ? 3 : 1;
     static constexpr int BK = KIND == EIGHT ? 128 : 64;              // 128 bytes a row of either operand

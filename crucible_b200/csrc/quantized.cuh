@@ -15,6 +15,7 @@
 
 // K of a product at the most: indices along K, and the products that stand for divisions of them, are 32-bit
 constexpr int MOST_K = 1 << 20;
+constexpr int MOST_PITCH = 1 << 24;     // bytes from one feature's weights to the next: a block's offsets are 32-bit
 
 enum QuantizedKind { FOUR_BF16 = 0, FOUR_F32 = 1, EIGHT = 2 };
 
@@ -85,4 +86,16 @@ __device__ __forceinline__ void finish(const QuantizedArgs& p, float v, float ro
     const long long at = (long long)m * p.ldo + n;
     if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
     else static_cast<float*>(p.out)[at] = v;
+}
+
+// Shared memory beyond the default, asked for once a kernel and device.
+template <typename Kernel>
+static inline int allow_shared(Kernel kernel, int bytes, bool (&configured)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 64 && configured[dev]) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) configured[dev] = true;
+    return (int)e;
 }

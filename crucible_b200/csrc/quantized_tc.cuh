@@ -24,11 +24,6 @@ __device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, in
         for (int i = 0; i < 4; ++i) v[4 * c + i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
 }
 
-// The weights' place is tensor memory, as the MMA's A operand: lane = feature, a column = two neighbouring k, 32 columns
-// a stage of 64 k.  (In shared memory they were 16 KB written and 16 KB read a stage beside the rows' and codes' own
-// bytes: 570 of the 656 cycles that a stage took with 256 rows, 600 with 16.)
-constexpr int WEIGHT_STAGES = 4, WEIGHT_COLS = 32;
-
 // The group scales of one feature, 256 k (eight runs of 32) at a time, asked for a stage of codes ahead.  Where 256 k
 // are whole groups and a feature's scales begin on a multiple of 8, 4 or 2 bytes, as those 256 k have, one load
 // brings them (a load of a byte is 32 lines of memory for a warp, and eight of them for 256 k take the load unit
@@ -132,16 +127,4 @@ static inline bool quantized_map(CUtensorMap* map, const void* base, bool bf16, 
     return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, parts > 1 ? 3 : 2,
               const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Shared memory beyond the default, asked for once a kernel and device.
-template <typename Kernel>
-static inline int allow_shared(Kernel kernel, int bytes, bool (&configured)[64]) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    if (dev < 64 && configured[dev]) return 0;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) configured[dev] = true;
-    return (int)e;
 }

@@ -25,6 +25,7 @@ from . import LAUNCHES, KernelError, _check, _need_cuda, _ptr, _stream, build, t
 
 build.register_module("rows8", ["common.cuh"])
 build.register_module("linear_quantized_few", ["common.cuh", "quantized.cuh"])
+build.register_module("linear_quantized_ring", ["common.cuh", "quantized.cuh", "tc_common.cuh"])
 for _name in ("linear_quantized_tcgen05", "linear_quantized_pairs_tcgen05"):
     build.register_module(_name, ["common.cuh", "quantized.cuh", "quantized_tc.cuh", "tc_common.cuh"])
 
@@ -32,6 +33,7 @@ E4M3 = torch.float8_e4m3fn
 TOP = 448.0                      # the largest e4m3 number
 LEAST = 1e-30                    # a row's largest magnitude counts as this much at least
 _FOUR_BF16, _FOUR_F32, _EIGHT = 0, 1, 2
+_MOST_PITCH = 1 << 24            # bytes between rows of weights (`csrc/quantized.cuh`)
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
@@ -200,7 +202,9 @@ class Weights8:
                 raise KernelError(f"8-bit weights: an empty matrix {list(values.shape)}")
             _vector(scales, "8-bit weights' scales", values.shape[0])
             _one_device(values, scales)
-        self.values = values if _aligned16(values) else _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
+        if not _aligned16(values) or (shape[0] > 1 and values.stride(0) > _MOST_PITCH):
+            values = _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
+        self.values = values
         self.scales = scales
         self.shape = shape
         self.pitch = _pitch(self.values)
@@ -309,7 +313,7 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 
 
 FEW_ROWS = 16                    # products of up to so many rows run on mma.sync
-FORM = None                      # tests name one of the forms, "few", "tiles" or "pairs", to reach it at any size
+FORM = None                      # tests name one of the forms, "few", "ring", "tiles" or "pairs", to reach it at any size
 
 
 def _up(x: int, to: int) -> int:
@@ -319,13 +323,17 @@ def _up(x: int, to: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _rule(forced, kind: int, m: int, n: int, k: int):
     """Which kernel takes a product, and how: ("few",), ("tiles", rows a tile, shares of K) or ("pairs", rows a
-    tile, pairs of SMs)."""
+    tile, pairs of SMs), or ("ring", groups of warps)."""
     form = forced
     if form is None or (form == "pairs" and kind == _FOUR_F32):
         form = "few" if m <= FEW_ROWS else "tiles" if kind == _FOUR_F32 or m <= 256 else "pairs"
+    if form == "ring" and (kind != _FOUR_BF16 or k % 256):
+        form = "few"
     if form == "few":
         return ("few",)
-    most = 64 if kind == _FOUR_F32 else 192 if form == "pairs" and kind == _FOUR_BF16 else 256
+    if form == "ring":
+        return "ring", 4 if n >= 296 * 128 else 2 if n >= 296 * 64 else 1
+    most = 64 if kind == _FOUR_F32 else 256
     tok = _up(-(-m // -(-m // most)), 16)
     if form == "pairs":
         return "pairs", tok, 74
@@ -354,7 +362,9 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
         status = tensor_core._status.get(dev)
         if status is None:
             status = tensor_core.status_word(rows.device)
-        if form[0] == "pairs":
+        if form[0] == "ring":
+            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, form[1], status.data_ptr())
+        elif form[0] == "pairs":
             code = _at(dev, build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs, *common, form[1],
                        form[2], status.data_ptr())
         else:

@@ -157,7 +157,7 @@ def test_linear8_by_every_form(form, rows, n, k, monkeypatch):
         _check8(rows, n, k, out, add)
 
 
-@pytest.mark.parametrize("form", ["few", "tiles", "pairs"])
+@pytest.mark.parametrize("form", ["few", "ring", "tiles", "pairs"])
 @pytest.mark.parametrize("rows,n,k,group", [(1, 1, 32, 32), (3, 130, 96, 96), (16, 257, 160, 32), (17, 128, 256, 64),
                                             (40, 255, 608, 32), (129, 300, 1024, 128), (250, 513, 288, 96),
                                             (257, 700, 2080, 32), (300, 256, 6144, 6144), (513, 40000, 64, 64)])
@@ -166,6 +166,16 @@ def test_linear4_by_every_form(form, rows, n, k, group, monkeypatch):
     for dtype in (torch.bfloat16, torch.float32):
         for out, add in ((torch.float32, True), (torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)):
             _check4(rows, n, k, group, dtype, out, add)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 8, 9, 16, 17])
+@pytest.mark.parametrize("n,k,group", [(1, 256, 32), (33, 256, 256), (64, 512, 64), (100, 1024, 32), (129, 1280, 160), (300, 1536, 96),
+                                       (18944, 768, 128), (20000, 256, 64), (40000, 512, 32), (31, 4096, 2048)])
+def test_linear4_by_the_ring(rows, n, k, group, monkeypatch):
+    """Every number of groups, K of one stage and of several, scales that begin inside a segment."""
+    monkeypatch.setattr(quantized, "FORM", "ring")
+    _check4(rows, n, k, group, torch.bfloat16, torch.float32, True)
+    _check4(rows, n, k, group, torch.bfloat16, torch.bfloat16, False)
 
 
 def _check4(rows, n, k, group, dtype, out_dtype, add, seed=0):
