@@ -17,7 +17,7 @@ allocates from torch's pool, as any captured torch operation does).
 from __future__ import annotations
 
 import functools
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -312,35 +312,125 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
         _rows(add, f"{what} add", (torch.float32,), shape)
 
 
-FEW_ROWS = 16                    # products of up to so many rows run on mma.sync
+# Which kernel, and how.  What follows was measured on B200 for the three kinds of product at 11 sizes of weights, 1,280 by
+# 768 to 28,672 by 4,096 (and 50,304 by 768, 4,096 by 14,336), and 1 to 2,048 rows, in every form: the rules below took
+# 1.0 to 1.3% longer than the best form on the average.
+#
+#   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
+#            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
+#   "ring"   the same arithmetic behind a ring of stages: 4-bit weights and bfloat16 rows, K a multiple of 256.  8 rows of
+#            4,096 by 4,096, ring / few / tiles: 5.8 / 7.5 / 9.5; 16 rows by 14,336 15.4 / 22.0 / 18.4; 32 rows by 2,048 (K of
+#            8,192) 11.1 / 14.5 / 12.9, by 6,144 (K of 4,096) 14.4 / 18.3 / 12.8.  More groups of warps a block read the
+#            rows less often, as long as every SM still has two blocks: 1 / 2 / 4 groups by 14,336 13.3 / 12.7 / 14.1, by
+#            50,304 (K of 768) 14.0 / 12.3 / 10.4.
+#   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K.
+#   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
+#
+# Between the last two, and for the rows a tile and the shares of K, a model of what a launch takes decides: a block's
+# fixed part, its steps along K (longer where two blocks are on an SM, and never shorter than the memory
+# allows), what a cluster costs, and how many blocks follow one another on an SM.  us, in `_COSTS`.
 FORM = None                      # tests name one of the forms, "few", "ring", "tiles" or "pairs", to reach it at any size
+N_SMS = 148
+_SMALL, _SMALL_8_ROWS = 1_600_000, 4_200_000           # weights of a matrix that "few" ends first: up to 64 rows, up to 8
+
+
+class _Costs(NamedTuple):
+    base: float                  # a launch of tiles
+    block: float                 # a block of it, and per row
+    block_row: float
+    step: float                  # 128 bytes of a row along K (128 k in 8 bits, 64 k else), and per column of sums
+    step_col: float
+    two: float                   # times that, with two blocks on an SM
+    step_bytes: float            # at least, for all blocks on an SM
+    share: float                 # a cluster, per row, per block of it
+    share_row: float
+    share_block: float
+    pair_base: float             # a launch of pairs
+    pair_step: float             # a step of theirs, and per row
+    pair_step_row: float
+    pair_out: float              # a tile's way out, per row
+
+
+_COSTS = {
+    _EIGHT: _Costs(0.88, 2.80, 0.0086, 0.150, 0.0010, 2.44, 0.214, 0.87, 0.0252, 0.10, 7.2, 0.160, 0.0008, 0.0052),
+    _FOUR_BF16: _Costs(3.58, 1.32, 0.0097, 0.1545, 0.0007, 1.90, 0.192, 1.17, 0.0111, 0.12, 10.1, 0.131, 0.0009, 0.0089),
+    _FOUR_F32: _Costs(3.97, 1.69, 0.0136, 0.179, 0.0004, 1.77, 0.022, 0.0, 0.0051, 0.73, 0.0, 0.0, 0.0, 0.0),
+}
 
 
 def _up(x: int, to: int) -> int:
     return (x + to - 1) // to * to
 
 
+def _tiles_us(kind: int, m: int, n: int, k: int, tok: int, shares: int) -> float:
+    c, parts = _COSTS[kind], 3 if kind == _FOUR_F32 else 1
+    steps = -(-k // (128 if kind == _EIGHT else 64)) / shares
+    per_sm = _blocks_an_sm(kind, tok)
+    left, us = -(-n // 128) * -(-m // tok) * shares, c.base
+    fixed = c.block + c.block_row * tok
+    if shares > 1:
+        fixed += c.share + c.share_row * tok + c.share_block * shares
+    alone = c.step + c.step_col * parts * tok
+    while left > 0:
+        now = min(left, N_SMS * per_sm)
+        left -= now
+        us += fixed + steps * max(alone * (c.two if now > N_SMS else 1.0), c.step_bytes * now / N_SMS)
+    return us
+
+
+def _blocks_an_sm(kind: int, tok: int) -> int:
+    return 2 if tok <= (32 if kind == _FOUR_F32 else 64) else 1
+
+
+def _pairs_us(kind: int, m: int, n: int, k: int, tok: int) -> float:
+    c = _COSTS[kind]
+    steps = -(-k // (128 if kind == _EIGHT else 64))
+    waves = -(-(-(-n // 256) * -(-m // tok)) // (N_SMS // 2))
+    out = c.pair_out * tok
+    return c.pair_base + waves * max(steps * (c.pair_step + c.pair_step_row * tok), out) + out
+
+
+def _even(m: int, most: int) -> int:
+    """Rows a tile, at most `most`, that cut m into equal tiles."""
+    return _up(-(-m // -(-m // most)), 16)
+
+
 @functools.lru_cache(maxsize=4096)
 def _rule(forced, kind: int, m: int, n: int, k: int):
-    """Which kernel takes a product, and how: ("few",), ("tiles", rows a tile, shares of K) or ("pairs", rows a
-    tile, pairs of SMs), or ("ring", groups of warps)."""
+    """("few",), ("ring", groups of warps), ("tiles", rows a tile, shares of K) or ("pairs", rows a tile, pairs of SMs)."""
     form = forced
-    if form is None or (form == "pairs" and kind == _FOUR_F32):
-        form = "few" if m <= FEW_ROWS else "tiles" if kind == _FOUR_F32 or m <= 256 else "pairs"
-    if form == "ring" and (kind != _FOUR_BF16 or k % 256):
+    if form is None:
+        small = n * k <= _SMALL and m <= 64
+        if kind == _FOUR_BF16:
+            form = "ring" if m <= 16 or (m <= 32 and n <= 2048) else "few" if small else None
+        elif small or (n * k <= _SMALL_8_ROWS and m <= 8):
+            form = "few"
+    if (form == "ring" and (kind != _FOUR_BF16 or k % 256)):
         form = "few"
     if form == "few":
         return ("few",)
     if form == "ring":
-        return "ring", 4 if n >= 296 * 128 else 2 if n >= 296 * 64 else 1
-    most = 64 if kind == _FOUR_F32 else 256
-    tok = _up(-(-m // -(-m // most)), 16)
-    if form == "pairs":
-        return "pairs", tok, 74
-    tiles = -(-n // 128) * -(-m // tok)
-    slots = 148 * (2 if tok <= (32 if kind == _FOUR_F32 else 64) else 1)
+        return "ring", 4 if n >= 37888 else 2 if n >= 9472 else 1
     units = -(-k // (128 if kind == _EIGHT else 256))
-    return "tiles", tok, max(1, min(8, slots // tiles, units // 2))
+    best = None
+    if form != "pairs" or kind == _FOUR_F32:
+        for most in (32, 64) if kind == _FOUR_F32 else (32, 64, 128, 256):
+            tok = _even(m, most)
+            if -(-m // tok) > 65535:
+                continue
+            tiles, per_sm = -(-n // 128) * -(-m // tok), _blocks_an_sm(kind, tok)
+            for shares in (1, 2, 4, 8) if per_sm == 2 else (1, 2, 4):
+                if shares == 1 or (shares <= units and tiles * shares <= 320):
+                    us = _tiles_us(kind, m, n, k, tok, shares)
+                    if best is None or us < best[0]:
+                        best = us, ("tiles", tok, shares)
+    if kind != _FOUR_F32 and (form == "pairs" or (form is None and m >= 48)):
+        for most in (64, 96, 128, 160, 192, 224, 256):
+            tok = _even(m, most)
+            us = _pairs_us(kind, m, n, k, tok)
+            if best is None or us < best[0]:
+                best = us, ("pairs", tok, N_SMS // 2)
+    return best[1]
 
 
 def form_of(kind: int, m: int, n: int, k: int):

@@ -113,3 +113,23 @@ def test_calls_that_are_refused():
     _refused("rows", quantized.linear4, a.half(), w4, out)
     _refused("rows", quantized.linear4, torch.zeros(3, 32), w4, out)
     _refused("add", quantized.linear4, a, w4, out, add=torch.zeros(2, 6))
+
+
+def test_the_rule_names_a_form_that_takes_the_product():
+    for kind in (quantized._EIGHT, quantized._FOUR_BF16, quantized._FOUR_F32):
+        for forced in (None, "few", "ring", "tiles", "pairs"):
+            for m in (1, 8, 9, 16, 17, 33, 64, 65, 100, 129, 256, 257, 1000, 2049, 30000, 1 << 20):
+                for n, k in ((1, 32), (127, 256), (129, 96), (768, 2048), (4096, 14336), (28672, 4096), (300000, 64)):
+                    form, *how = quantized._rule(forced, kind, m, n, k)
+                    if form == "few":
+                        assert forced in (None, "few", "ring")
+                    elif form == "ring":
+                        assert kind == quantized._FOUR_BF16 and k % 256 == 0 and how[0] in (1, 2, 4)
+                    else:
+                        rows, more = how
+                        assert rows % 16 == 0 and 16 <= rows <= (64 if kind == quantized._FOUR_F32 else 256)
+                        if form == "tiles":
+                            assert more in (1, 2, 4, 8) and more <= -(-k // (128 if kind == quantized._EIGHT else 256))
+                            assert -(-m // rows) <= 65535
+                        else:
+                            assert form == "pairs" and kind != quantized._FOUR_F32 and more == 74
