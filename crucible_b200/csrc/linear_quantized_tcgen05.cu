@@ -14,6 +14,12 @@
 // shared memory, and each adds up a share of the rows from all of them, in the order of the
 // shares: no scratch memory, no atomics, the same sum every time.
 //
+// fp32 results over 4-bit weights.  The tensor cores cut off what an addition leaves below the sum's last bit, always
+// towards zero, and over a long K that adds up (K = 14,336 in one sum: 4.2e-6 of the result's norm; e4m3 products have
+// 8 bits and lose nothing to speak of).  So every CHUNK of K the sums come out of tensor memory and are added, rounded, to
+// those before them, which stand in the threads' registers and, of 256 rows, half of them in tensor memory beside the
+// weights.
+//
 // Roles: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor memory and
 // issues the MMAs, warps 2-9 make weights of codes (two sets of four, 64 k in turn) and then take the sums
 // out (two to a quarter of the lanes, 32 rows in turn), warp 10 sends the copies of codes.
@@ -29,6 +35,8 @@ constexpr int PACKED_K = 256;           // k of a stage of codes: 128 bytes a fe
 // a stage of 64 k.  (In shared memory they were 16 KB written and 16 KB read a stage beside the rows' and codes' own
 // bytes: 64 rows of 4,096 by 28,672 took 41 us, 31 like this.)
 constexpr int WEIGHT_STAGES = 4, WEIGHT_COLS = 32;
+
+constexpr int CHUNK = 2048;             // K of one sum where sums are long: a multiple of what a stage of codes holds
 
 template <int KIND, int TOK> struct Sizes {
     static constexpr int PARTS = KIND == FOUR_F32 ? 3 : 1;
@@ -54,7 +62,7 @@ template <int KIND, int TOK> struct Storage {
     alignas(1024) uint8_t codes[S::PACKED == 0 ? 1 : S::PACKED][S::PACKED == 0 ? 16 : S::CODES_BYTES];
     alignas(8) uint64_t full[S::STAGES], empty[S::STAGES];            // the copies' ring
     uint64_t made[WEIGHT_STAGES], used[WEIGHT_STAGES];               // the weights' ring in tensor memory
-    uint64_t codes_full[4], codes_empty[4], done;
+    uint64_t codes_full[4], codes_empty[4], done, drained;
     uint32_t tmem;
     int abort_flag;
 };
@@ -70,6 +78,8 @@ __global__ void __launch_bounds__(THREADS, Sizes<KIND, TOK>::BLOCKS)
 linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
                       const QuantizedArgs p, int tok, int splits, int* __restrict__ status) {
     using S = Sizes<KIND, TOK>;
+    constexpr bool CHUNKED = KIND != EIGHT && !BF16;
+    constexpr int CHUNK_STEPS = CHUNK / 64;
     extern __shared__ uint8_t smem_raw[];
     Storage<KIND, TOK>& s = *reinterpret_cast<Storage<KIND, TOK>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -98,6 +108,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
             tc::mbar_init(&s.codes_empty[i], 8);
         }
         tc::mbar_init(&s.done, 1);
+        tc::mbar_init(&s.drained, 8);
         s.abort_flag = 0;
         tc::fence_barrier_init();
         tc::prefetch_tensormap(&map_rows);
@@ -147,8 +158,15 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
             int st = 0, ws = 0;
             uint32_t parity = 0, made_parity = 0, more = 0;
             bool ok = true;
+            uint32_t drained_parity = 0;
             for (int kb = 0; kb < n_kb; ++kb) {
-                ok = tc::mbar_wait(&s.full[st], parity, abort_flag);
+                ok = true;
+                if (CHUNKED && kb > 0 && kb % CHUNK_STEPS == 0) {
+                    tc::umma_commit(&s.done);
+                    ok = tc::mbar_wait(&s.drained, drained_parity, abort_flag);
+                    drained_parity ^= 1, more = 0;
+                }
+                ok = ok && tc::mbar_wait(&s.full[st], parity, abort_flag);
                 if (KIND != EIGHT) ok = ok && tc::mbar_wait(&s.made[ws], made_parity, abort_flag);
                 if (!ok) {
                     tc::give_up(abort_flag, status, tc::ST_MMA_TIMEOUT);
@@ -196,7 +214,42 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     } else {
         const int r = (warp & 3) * 32 + lane, set = (warp - 2) >> 2;     // the feature: a lane of tensor memory
         const int n = n0 + r;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         bool ok = true;
+        // 32 rows' sums of this feature (a last 16 beside something that nobody uses)
+        auto load_rows = [&](int c, float (&v)[32]) {
+            uint32_t u[32];
+            tc::tmem_ld_32x32(mine + (S::PARTS - 1) * tok + c, u);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
+#pragma unroll
+            for (int j = S::PARTS - 2; j >= 0; --j) {
+                tc::tmem_ld_32x32(mine + j * tok + c, u);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(u[i]);
+            }
+        };
+        // the sums of the chunks before the last: 32 rows in turn by the two sets
+        constexpr int OWN = CHUNKED ? (TOK + 63) / 64 : 1, HELD = OWN < 2 ? OWN : 2;
+        static_assert(OWN <= HELD || S::N + (OWN - HELD) * 64 + WEIGHT_STAGES * WEIGHT_COLS <= S::TMEM, "the rest fit in tensor memory");
+        float before[HELD][32];
+        const uint32_t kept = mine + S::N + set * 32 * (OWN > HELD ? OWN - HELD : 0);
+        auto add_before = [&](int o, float (&v)[32]) {
+            if (o < HELD) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += before[o < HELD ? o : 0][i];
+            } else {
+                uint32_t u[32];
+                tc::tmem_ld_32x32(kept + (o - HELD) * 32, u);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(u[i]);
+            }
+        };
+        uint32_t done_parity = 0;
+        bool chunks = false;
         if constexpr (KIND != EIGHT) {
             const Scales scales(p, n);
             uint2 sc, next = scales.load(k_begin, k_end);
@@ -238,49 +291,78 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&s.codes_empty[pk]);
                 if (++pk == S::PACKED) pk = 0, pk_parity ^= 1;
+                if constexpr (CHUNKED) {
+                    static_assert(CHUNK_STEPS % 4 == 0, "a chunk is whole stages of codes");
+                    if (ok && (kb + 4) % CHUNK_STEPS == 0 && kb + 4 < n_kb) {
+                        ok = tc::mbar_wait(&s.done, done_parity, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
+                            break;
+                        }
+                        tc::tc_fence_after_sync();
+#pragma unroll
+                        for (int o = 0; o < OWN; ++o) {
+                            if (32 * set + 64 * o >= tok) break;
+                            float v[32];
+                            load_rows(32 * set + 64 * o, v);
+                            if (chunks) add_before(o, v);
+                            if (o < HELD) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) before[o < HELD ? o : 0][i] = v[i];
+                            } else {
+                                uint32_t u[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i]);
+                                tc::tmem_st_32x32(kept + (o - HELD) * 32, u);
+                            }
+                        }
+                        if (OWN > HELD) tc::tmem_st_wait();
+                        tc::tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&s.drained);
+                        done_parity ^= 1, chunks = true;
+                    }
+                }
             }
         }
         // ---- epilogue
         if (ok) {
-            ok = tc::mbar_wait(&s.done, 0, abort_flag);
+            ok = tc::mbar_wait(&s.done, done_parity, abort_flag);
             if (!ok && !*abort_flag) tc::give_up(abort_flag, status, tc::ST_EPILOGUE_TIMEOUT);
             ok = __all_sync(0xffffffffu, ok);
         }
         tc::tc_fence_after_sync();
-        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float fs = n < p.N ? __ldg(p.feature_scale + n) : 0.f;
         const int m_end = min(p.M, m0 + tok);
-        // 32 rows' sums of this feature (a last 16 beside something that nobody uses)
-        auto load_rows = [&](int c, float (&v)[32]) {
-            uint32_t u[32];
-            tc::tmem_ld_32x32(mine + (S::PARTS - 1) * tok + c, u);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
-#pragma unroll
-            for (int j = S::PARTS - 2; j >= 0; --j) {
-                tc::tmem_ld_32x32(mine + j * tok + c, u);
-                tc::tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] += __uint_as_float(u[i]);
-            }
+        auto whole_rows = [&](int c, int o, float (&v)[32]) {
+            load_rows(c, v);
+            if (CHUNKED && chunks) add_before(o, v);
         };
         if (splits == 1) {
             if (ok) {
-#pragma unroll 1
-                for (int c = 32 * set; c < tok; c += 64) {
+                constexpr int TURNS = CHUNKED ? OWN : 1;            // (registers are indexed by constants)
+                for (int c0 = 0; c0 < tok; c0 += 64 * TURNS)
+#pragma unroll
+                for (int o = 0; o < TURNS; ++o) {
+                    const int c = c0 + 64 * o + 32 * set;
+                    if (c >= tok) break;
                     float v[32];
-                    load_rows(c, v);
+                    whole_rows(c, o, v);
                     store_rows<KIND, BF16>(p, v, fs, n, m0 + c, m_end, p.add, p.lda);
                 }
             }
         } else {
             float* left = reinterpret_cast<float*>(s.b[0]);           // [row][feature]; the ring is free by now
             if (ok) {
-#pragma unroll 1
-                for (int c = 32 * set; c < tok; c += 64) {
+                constexpr int TURNS = CHUNKED ? OWN : 1;
+                for (int c0 = 0; c0 < tok; c0 += 64 * TURNS)
+#pragma unroll
+                for (int o = 0; o < TURNS; ++o) {
+                    const int c = c0 + 64 * o + 32 * set;
+                    if (c >= tok) break;
                     float v[32];
-                    load_rows(c, v);
+                    whole_rows(c, o, v);
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (c + i < tok) left[(c + i) * FEATURES + r] = v[i];

@@ -150,6 +150,8 @@ norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long lo
     }
     ss = row_sum<WARP>(ss, scratch);
     const float r = 1.0f / sqrtf(ss / (float)width + eps);
+    // y = v r with v = sum * gain: the row's factor r is in its largest number as well, so 448 / max |v| takes v to e4m3 with
+    // three roundings, whatever r was rounded to
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -158,31 +160,46 @@ norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long lo
             float w[E];
             load_chunk<float, E, VEC>(gain, at, width, w);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[c][i] = v[c][i] * r * w[i];
+            for (int i = 0; i < E; ++i) v[c][i] *= w[i];
             top = max(top, magnitude(v[c]));
         }
     }
-    const float most = at_least(row_max<WARP>(top, reinterpret_cast<uint32_t*>(scratch)));
-    const float inv = E4M3_TOP / most;
+    const float top_v = row_max<WARP>(top, reinterpret_cast<uint32_t*>(scratch)), top_y = top_v * r;
+    const float most = at_least(top_y);
+    const float factor = top_y >= LEAST ? E4M3_TOP / top_v : (top_y < LEAST ? r * (E4M3_TOP / LEAST) : top_y);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
-        if (at < width) store_e4m3<E, VEC>(q + row * ldq, at, width, v[c], inv);
+        if (at < width) store_e4m3<E, VEC>(q + row * ldq, at, width, v[c], factor);
     }
     if (threadIdx.x == 0) scales[row] = most / E4M3_TOP;
 }
 
-// The exponential and the quotient of the hardware's unit: e^-g is off by 2^-22 + |g| 2^-24 relative to it, the quotient
-// by 2^-22; a row's numbers are then rounded to 2^-4.  With expf and the exact division 2,048 rows of 14,336 bf16
-// pairs took 77 us, which is what those instructions take.
+// z / (1 + e^-a z) by the hardware's unit, 2^-22 each for the power of two and the reciprocal, and a few products:
+// t = -a z log2 e loses 2^-24 of itself, up to 2^-18 of the power, unless its rest, which one fused multiply-add gives, goes
+// back into it; and a step of Newton's takes the reciprocal to 2^-24.  (With expf and the exact division 2,048 rows
+// of 14,336 bf16 pairs took 77 us, which is what those instructions take.)
+__device__ __forceinline__ float gated(float z, float alpha) {
+    const float x = -alpha * z, log2e = 1.44269504f;
+    const float t = x * log2e;
+    const float rest = fmaf(x, log2e, -t) + x * 1.92596299e-8f;       // log2 e has more digits, too
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    e = fmaf(e, rest * 0.693147182f, e);
+    const float d = fminf(1.0f + e, 1e38f);                           // (no infinity in what follows; a NaN is in z as well)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    return z * r;
+}
+
 __device__ __forceinline__ float pair8(float g, float u, float limit, float alpha, float offset) {
     if (limit > 0.f) {
         // (written so that a NaN stays one)
         g = g > limit ? limit : g;
         u = (u > limit ? limit : (u < -limit ? -limit : u)) + offset;
-        return __fdividef(g, 1.0f + __expf(-alpha * g)) * u;
+        return gated(g, alpha) * u;
     }
-    return __fdividef(g, 1.0f + __expf(-g)) * u;
+    return gated(g, 1.0f) * u;
 }
 
 template <typename T, int CH, bool WARP, bool VEC>
