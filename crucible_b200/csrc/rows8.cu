@@ -175,20 +175,18 @@ norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long lo
     if (threadIdx.x == 0) scales[row] = most / E4M3_TOP;
 }
 
-// z / (1 + e^-a z) by the hardware's unit, 2^-22 each for the power of two and the reciprocal, and a few products:
-// t = -a z log2 e loses 2^-24 of itself, up to 2^-18 of the power, unless its rest, which one fused multiply-add gives, goes
-// back into it; and a step of Newton's takes the reciprocal to 2^-24.  (With expf and the exact division 2,048 rows
-// of 14,336 bf16 pairs took 77 us, which is what those instructions take.)
+// z / (1 + e^-a z) by the hardware's unit, 2^-22 and 2^-23 for the power of two and the reciprocal.  t = -a z log2 e loses
+// 2^-24 of itself, up to 2^-18 of the power, unless its rest, which one fused multiply-add gives, goes back into it.
+// (With expf and the exact division 2,048 rows of 14,336 bf16 pairs took 77 us, which is what those instructions take.)
 __device__ __forceinline__ float gated(float z, float alpha) {
-    const float x = -alpha * z, log2e = 1.44269504f;
+    // (beyond e^88 there is nothing of z left, below e^-88 all of it; a NaN is in z as well)
+    const float x = fmaxf(fminf(-alpha * z, 88.f), -88.f), log2e = 1.44269504f;
     const float t = x * log2e;
     const float rest = fmaf(x, log2e, -t) + x * 1.92596299e-8f;       // log2 e has more digits, too
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     e = fmaf(e, rest * 0.693147182f, e);
-    const float d = fminf(1.0f + e, 1e38f);                           // (no infinity in what follows; a NaN is in z as well)
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return z * r;
 }
 

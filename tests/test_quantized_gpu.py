@@ -106,6 +106,21 @@ def test_rows8_of_zeros_and_of_what_is_no_number(width):
     assert torch.isinf(s[2]) and torch.isnan(v[2, 0]) and (v[2, 1:] == 0).all()
 
 
+@pytest.mark.parametrize("pair", [(None, 1.0, 0.0), (7.0, 1.702, 1.0), (1e30, 1.0, 0.0)])
+def test_glu8_far_from_zero(pair):
+    """Gates whose exponential is nothing, or more than 32 bits hold."""
+    g = torch.tensor([0.0, 1e-30, -1e-30, 20.0, -20.0, 60.0, -60.0, 87.0, -87.0, 100.0, -100.0, 1e6, -1e6, 3e38, -3e38, 0.5], device=DEV)
+    rows = []
+    for i in range(16):                                # each gate beside small ones, so that none of them hides it
+        r = torch.full((16,), 0.25, device=DEV)
+        r[i] = g[i]
+        rows.append(torch.cat([r, torch.ones(16, device=DEV)]))
+    both = torch.stack(rows)
+    q, s = quantized.new_rows8(16, 16, DEV), torch.empty(16, device=DEV)
+    quantized.glu8(both, q, s, *pair)
+    check_rows8(q, s, exact_glu(both, *pair))
+
+
 def test_rows8_refuse_what_no_block_holds():
     x, q, s = torch.zeros(1, 32769, device=DEV), quantized.new_rows8(1, 32769, DEV), torch.zeros(1, device=DEV)
     with pytest.raises(KernelError, match="32768"):
