@@ -101,7 +101,7 @@ __device__ __forceinline__ float at_least(float v) { return v < LEAST ? LEAST : 
 // CH: chunks a thread.  WARP: a warp a row (blockDim.y rows a block), else a block a row.
 template <typename D, int CH, bool WARP, bool VEC>
 __global__ void __launch_bounds__(WARP ? 128 : (CH < 8 ? 512 : 1024))
-norm8_kernel(const float* x, long long ldx, const D* __restrict__ delta, long long ldd, const float* __restrict__ gain,
+norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const float* __restrict__ gain,
              float eps, float* sum_out, long long lds, uint8_t* __restrict__ q, long long ldq,
              float* __restrict__ scales, int rows, int width) {
     constexpr int E = 4;
@@ -307,7 +307,7 @@ void launch_glu8(const Shape& s, const T* both, long long ldb, uint8_t* q, long 
 
 CB_EXPORT int cb_rows8_widest() { return WIDEST; }
 
-// Strides in elements.  `delta` and `sum_out` may be null; `sum_out` may be `x`.
+// Strides in elements.  `delta` and `sum_out` may be null; `sum_out` may be `x` or `delta`.
 CB_EXPORT int cb_norm8(const float* x, long long ldx, const void* delta, int delta_dtype, long long ldd,
                        const float* gain, float eps, float* sum_out, long long lds, void* q, long long ldq,
                        float* scales, int rows, int width, void* stream) {

@@ -8,6 +8,9 @@ spelling of the same network (`scripts/export_hf.py:83-103`) with the names of
 identical layers of pre-RMSNorm, grouped-query attention with half-split RoPE
 and a SwiGLU feed-forward, run once each in order.
 
+`feed_forward_weight_group` in either spelling: the feed-forwards' matrices are kept in 4 bits with a scale for
+so many weights (`parts/swiglu.py::SwiGLU4`); the checkpoint stays as it is.
+
 Like the reference's GPU loader (`engine/src/gpu_model.rs:506-520`) anything
 other than rope / rmsnorm / pre / swiglu is refused, loudly.
 """
@@ -40,7 +43,15 @@ def _dense_decoder(*, architecture: str, raw: Mapping[str, Any], vocab: int, hid
                       head_dim=head_dim, softmax_scale=1.0 / math.sqrt(head_dim),
                       window=None, position=position)
     norm = NormSpec(kind="rmsnorm", width=hidden, eps=eps)
-    ffn = FeedForwardSpec(kind="swiglu", width=hidden, intermediate=intermediate)
+    r = KeyReader(raw)
+    if r.has("feed_forward_weight_group"):
+        group = r.integer("feed_forward_weight_group")
+        if group % 32 or hidden % group or intermediate % group:
+            raise ConfigError(f"config.json: 'feed_forward_weight_group' must be a multiple of 32 that divides "
+                              f"{hidden} and {intermediate}, got {group}")
+        ffn = FeedForwardSpec(kind="swiglu_4bit", width=hidden, intermediate=intermediate, extra=(("group", group),))
+    else:
+        ffn = FeedForwardSpec(kind="swiglu", width=hidden, intermediate=intermediate)
     layer = pre_norm_layer(mixer, norm, ffn, norm)
     return ModelConfig(
         architecture=architecture, vocab_size=vocab, hidden_size=hidden,
@@ -105,6 +116,11 @@ def _parse_crucible(raw: Mapping[str, Any]) -> ModelConfig:
         names=CRUCIBLE_NAMES)
 
 
+def _weight_group(cfg: ModelConfig) -> dict:
+    ffn = cfg.layers[0].feed_forward
+    return {"feed_forward_weight_group": ffn.option("group")} if ffn.kind == "swiglu_4bit" else {}
+
+
 def _describe_crucible(cfg: ModelConfig) -> dict:
     layer = cfg.layers[0]
     m = layer.mixer
@@ -118,7 +134,7 @@ def _describe_crucible(cfg: ModelConfig) -> dict:
         "attention": label, "pos_encoding": "rope", "activation": "swiglu",
         "norm": "rmsnorm", "norm_placement": "pre",
         "rope_theta": m.position.theta, "rms_norm_eps": layer.mixer_norm.eps,
-        "tie_word_embeddings": cfg.tie_word_embeddings,
+        "tie_word_embeddings": cfg.tie_word_embeddings, **_weight_group(cfg),
     }
 
 
@@ -181,7 +197,7 @@ def _describe_llama(cfg: ModelConfig) -> dict:
         "max_position_embeddings": cfg.max_context, "hidden_act": "silu",
         "rope_theta": m.position.theta, "rms_norm_eps": layer.mixer_norm.eps,
         "tie_word_embeddings": cfg.tie_word_embeddings,
-        "attention_bias": False, "mlp_bias": False,
+        "attention_bias": False, "mlp_bias": False, **_weight_group(cfg),
     }
 
 

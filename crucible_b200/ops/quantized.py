@@ -209,12 +209,14 @@ class Weights8:
         self.shape = shape
         self.pitch = _pitch(self.values)
         self.device = values.get_device()
+        if self.device >= 0:
+            _status(self.device)
 
     @classmethod
     def pack(cls, w: torch.Tensor) -> "Weights8":
         """From a matrix of floating numbers: each row's largest magnitude becomes 448."""
         w = _finite(w)
-        scales = w.abs().amax(dim=1).clamp_min(LEAST) / TOP
+        scales = w.abs().amax(dim=1).clamp_min(LEAST) * (1 / TOP)
         return cls((w / scales[:, None]).clamp(-TOP, TOP).to(E4M3), scales)
 
     def dense(self) -> torch.Tensor:
@@ -253,6 +255,8 @@ class Weights4:
             self.group = shape[1] * 8 // groups[1]
             self.shape = torch.Size((shape[0], shape[1] * 8))
             self.device = codes.get_device()
+            if self.device >= 0:
+                _status(self.device)
             return
         _rows(codes, "4-bit weights' codes", (torch.int32,))
         n, k = codes.shape[0], codes.shape[1] * 8
@@ -272,6 +276,8 @@ class Weights4:
         self.group = k // groups
         self.shape = torch.Size((n, k))
         self.device = codes.get_device()
+        if self.device >= 0:
+            _status(self.device)
 
     @classmethod
     def pack(cls, w: torch.Tensor, group: int = 64) -> "Weights4":
@@ -282,8 +288,10 @@ class Weights4:
         if group <= 0 or group % 32 or k % group:
             raise KernelError(f"4-bit weights: a group is a multiple of 32 that divides K = {k}, got {group}")
         parts = w.view(n, k // group, group)
-        want = parts.abs().amax(dim=2) / 7
-        scales = want.amax(dim=1).clamp_min(LEAST) / TOP
+        # (products with reciprocals, and quotients of tensors alone: a quotient by a number is rounded otherwise on
+        # another device, and a scale that falls on the other side of a border is 2^-3 off)
+        want = parts.abs().amax(dim=2) * (1 / 7)
+        scales = want.amax(dim=1).clamp_min(LEAST) * (1 / TOP)
         # (no group's scale may round to zero: the smallest number above it is 2^-9)
         group_scales = (want / scales[:, None]).clamp(2.0 ** -9, TOP).to(E4M3)
         step = group_scales.float() * scales[:, None]
@@ -433,6 +441,18 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
     return best[1]
 
 
+def _status(dev: int) -> int:
+    """The address of the word that a kernel writes if one of its bounded waits runs out (`tensor_core.check_status`
+    raises then).  None yet, and a graph is being captured: null, since the word's zero would be written by the
+    graph's replays and not now."""
+    word = tensor_core._status.get(dev)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        word = tensor_core.status_word(torch.device("cuda", dev))
+    return word.data_ptr()
+
+
 def form_of(kind: int, m: int, n: int, k: int):
     return _rule(FORM, kind, m, n, k)
 
@@ -449,18 +469,16 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
     if form[0] == "few":
         code = _at(dev, build.load("linear_quantized_few").cb_linear_quantized_few, *common)
     else:
-        status = tensor_core._status.get(dev)
-        if status is None:
-            status = tensor_core.status_word(rows.device)
+        status = _status(dev)
         if form[0] == "ring":
-            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, form[1], status.data_ptr())
+            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, form[1], status)
         elif form[0] == "pairs":
             code = _at(dev, build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs, *common, form[1],
-                       form[2], status.data_ptr())
+                       form[2], status)
         else:
             parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device) if kind == _FOUR_F32 else None
             code = _at(dev, build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05, *common, form[1], form[2],
-                       _ptr(parts), status.data_ptr())
+                       _ptr(parts), status)
             if kind == _FOUR_F32 and code == 0:
                 LAUNCHES[0] += 1                       # (the rows' parts)
     if code == build.UNSUPPORTED:

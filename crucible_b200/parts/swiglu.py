@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 
 from .. import ops
-from ..config.model_config import FeedForwardSpec
+from ..config.model_config import ConfigError, FeedForwardSpec
+from ..ops import quantized, small_batch
 from .base import FEED_FORWARDS, FeedForward, TensorDecl
 
 
@@ -41,4 +42,32 @@ class SwiGLU(FeedForward):
         ops.linear(act, self.down, residual, accumulate=True, closes=ctx)
 
 
+class SwiGLU4(SwiGLU):
+    """The same with its matrices in 4 bits (`quantized.Weights4`): the checkpoint's are packed once, at load,
+    with an e4m3 scale for every `group` weights of a feature (option, 64) and a float32 one a feature.  Rows, sums
+    and the gated pair are those of the engine's dtype."""
+
+    def __init__(self, spec: FeedForwardSpec):
+        super().__init__(spec)
+        self.group = int(spec.option("group", 64))
+        if self.group <= 0 or self.group % 32 or spec.width % self.group or spec.intermediate % self.group:
+            raise ConfigError(f"4-bit feed-forward: a group is a multiple of 32 that divides the widths "
+                              f"{spec.width} and {spec.intermediate}, got {self.group}")
+
+    def bind(self, tensors, dtype, device):
+        both = torch.cat([tensors["gate"], tensors["up"]], dim=0)
+        self.gate_up = quantized.Weights4.pack(both, self.group)
+        self.down = quantized.Weights4.pack(tensors["down"], self.group)
+        self.dtype = dtype
+
+    def forward(self, ctx, h, residual):
+        t, i = h.shape[0], self.spec.intermediate
+        both = ctx.scratch("ffn.gate_up", (t, 2 * i), self.dtype)
+        act = ctx.scratch("ffn.act", (t, i), self.dtype)
+        quantized.linear4(small_batch.as_tensor(h), self.gate_up, both)
+        ops.swiglu(both, act)
+        quantized.linear4(act, self.down, residual, add=residual)
+
+
 FEED_FORWARDS.register("swiglu", SwiGLU)
+FEED_FORWARDS.register("swiglu_4bit", SwiGLU4)

@@ -133,3 +133,25 @@ def test_the_rule_names_a_form_that_takes_the_product():
                             assert -(-m // rows) <= 65535
                         else:
                             assert form == "pairs" and kind != quantized._FOUR_F32 and more == 74
+
+
+def test_a_config_names_4_bit_feed_forwards():
+    from crucible_b200.config import ConfigError, parse_config, shape
+    raw = shape("120m")
+    assert parse_config(raw).layers[0].feed_forward.kind == "swiglu"
+    for group in (32, 128, 256):
+        cfg = parse_config({**raw, "feed_forward_weight_group": group})
+        assert cfg.layers[0].feed_forward.kind == "swiglu_4bit" and cfg.layers[0].feed_forward.option("group") == group
+    for group in (16, 48, 100, 512, 0, -32, "64"):
+        with pytest.raises(ConfigError):
+            parse_config({**raw, "feed_forward_weight_group": group})
+
+
+def test_a_described_config_keeps_the_group():
+    from crucible_b200.config import get_architecture, parse_config, shape
+    for name in ("120m", "llama-1b"):
+        for extra in ({}, {"feed_forward_weight_group": 64}):
+            cfg = parse_config({**shape(name), **extra})
+            again = get_architecture(cfg.architecture).describe(cfg)
+            assert again.get("feed_forward_weight_group") == extra.get("feed_forward_weight_group")
+            assert parse_config(again).layers == cfg.layers

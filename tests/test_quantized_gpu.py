@@ -328,6 +328,19 @@ def test_a_row_does_not_depend_on_the_others():
         assert torch.equal(y4[1], z4[1]) and torch.equal(y8[1], z8[1])
 
 
+def test_packing_is_the_same_on_every_device():
+    gen = torch.Generator().manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        w = (torch.randn(300, 1024, generator=gen) * 0.05).to(dtype)
+        for group in (32, 128):
+            here, there = quantized.Weights4.pack(w, group), quantized.Weights4.pack(w.to(DEV), group)
+            assert torch.equal(here.codes, there.codes.cpu()) and torch.equal(here.scales, there.scales.cpu())
+            assert torch.equal(here.group_scales.view(torch.uint8), there.group_scales.view(torch.uint8).cpu())
+        here, there = quantized.Weights8.pack(w), quantized.Weights8.pack(w.to(DEV))
+        assert torch.equal(here.values.view(torch.uint8), there.values.view(torch.uint8).cpu())
+        assert torch.equal(here.scales, there.scales.cpu())
+
+
 def _layer8(x, delta, gain, up, down, bufs):
     quantized.add_rmsnorm8(x, delta, gain, 1e-5, bufs["q"], bufs["s"])
     quantized.linear8(bufs["q"], bufs["s"], up, bufs["both"])
@@ -473,3 +486,40 @@ def test_float32_results_of_a_long_k_are_not_cut_off(rows, form, dtype, monkeypa
     want = a.double() @ dense4(w).t()
     assert float((out.double() - want).norm() / want.norm()) <= 1e-6
     check_product(out, a.double(), dense4(w), None, 3 if dtype == "f32" else 1)
+
+
+def test_every_form_on_streams_of_its_own():
+    """Products of all forms side by side, eagerly, again and again: each gives what it gives alone."""
+    gen = _gen()
+    jobs = []
+    for rows, n, k, dtype in ((1, 3000, 1024, "bf16"), (8, 9500, 512, "bf16"), (40, 2000, 2048, "bf16"), (300, 5000, 768, "bf16"),
+                              (3, 900, 640, "f32"), (50, 1500, 4096, "f32"), (700, 1280, 512, "bf16")):
+        w = random_weights4(n, k, 64, DEV, gen)
+        a = _randn(gen, rows, k).to(DTYPES[dtype])
+        out = torch.empty(rows, n, device=DEV)
+        jobs.append((lambda a=a, w=w, out=out: quantized.linear4(a, w, out), out))
+    for rows, n, k in ((1, 700, 768), (20, 4000, 2048), (64, 2048, 4096), (500, 3000, 1024)):
+        w, (q, s) = random_weights8(n, k, DEV, gen), random_rows8(rows, k, DEV, gen)
+        out = torch.empty(rows, n, device=DEV)
+        jobs.append((lambda q=q, s=s, w=w, out=out: quantized.linear8(q, s, w, out), out))
+    for call, _out in jobs:
+        call()
+    want = [out.clone() for _call, out in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _, out in jobs:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (call, _out) in zip(streams, jobs):
+            with torch.cuda.stream(stream):
+                call()
+    torch.cuda.synchronize()
+    for (_call, out), right in zip(jobs, want):
+        assert torch.equal(out, right)
+
+
+def test_no_kernel_gave_up():
+    """Runs last here: no bounded wait of the kernels above ran out."""
+    from crucible_b200.ops import tensor_core
+    tensor_core.check_status(DEV)
