@@ -69,7 +69,7 @@ __device__ __forceinline__ void store_e4m3(uint8_t* __restrict__ row, int at, in
 }
 
 // Over the threads of one row (a warp, or the whole block): the sum in a fixed order, or the largest of
-// non-negative floats by their bits, by which a NaN is larger than every number.
+// non-negative floats by their bits, by which a (positive) NaN is larger than every number.
 template <bool WARP>
 __device__ __forceinline__ float row_sum(float v, float* scratch) {
     if (WARP) return cb_warp_sum(v);
@@ -77,8 +77,8 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
 }
 
 template <bool WARP>
-__device__ __forceinline__ float row_max(uint32_t v, uint32_t* scratch) {
-    v = __reduce_max_sync(0xffffffffu, v);
+__device__ __forceinline__ float row_max(float m, uint32_t* scratch) {
+    uint32_t v = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7FFFFFFFu);
     if (!WARP) {
         __syncthreads();
         if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
@@ -88,10 +88,10 @@ __device__ __forceinline__ float row_max(uint32_t v, uint32_t* scratch) {
     return __uint_as_float(v);
 }
 
-template <int E> __device__ __forceinline__ uint32_t magnitude(const float (&v)[E]) {
-    uint32_t m = 0;
+// The larger of m and every |v|; a NaN is larger than all.
+template <int E> __device__ __forceinline__ float magnitude(float m, const float (&v)[E]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[i])));
     return m;
 }
 
@@ -152,7 +152,7 @@ norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const
     const float r = 1.0f / sqrtf(ss / (float)width + eps);
     // y = v r with v = sum * gain: the row's factor r is in its largest number as well, so 448 / max |v| takes v to e4m3 with
     // three roundings, whatever r was rounded to
-    uint32_t top = 0;
+    float top = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
@@ -161,7 +161,7 @@ norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const
             load_chunk<float, E, VEC>(gain, at, width, w);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[c][i] *= w[i];
-            top = max(top, magnitude(v[c]));
+            top = magnitude(top, v[c]);
         }
     }
     const float top_v = row_max<WARP>(top, reinterpret_cast<uint32_t*>(scratch)), top_y = top_v * r;
@@ -190,8 +190,9 @@ __device__ __forceinline__ float gated(float z, float alpha) {
     return z * r;
 }
 
+template <bool CAPPED>
 __device__ __forceinline__ float pair8(float g, float u, float limit, float alpha, float offset) {
-    if (limit > 0.f) {
+    if (CAPPED) {
         // (written so that a NaN stays one)
         g = g > limit ? limit : g;
         u = (u > limit ? limit : (u < -limit ? -limit : u)) + offset;
@@ -200,7 +201,7 @@ __device__ __forceinline__ float pair8(float g, float u, float limit, float alph
     return gated(g, 1.0f) * u;
 }
 
-template <typename T, int CH, bool WARP, bool VEC>
+template <typename T, int CH, bool WARP, bool VEC, bool CAPPED>
 __global__ void __launch_bounds__(WARP ? 128 : 1024)
 glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, long long ldq,
             float* __restrict__ scales, int rows, int width, float limit, float alpha, float offset) {
@@ -213,7 +214,7 @@ glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, 
     const T* gr = both + row * ldb;
     const T* ur = gr + width;
     float v[CH][E];
-    uint32_t top = 0;
+    float top = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int at = at0 + c * step;
@@ -223,10 +224,10 @@ glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, 
             load_chunk<T, E, VEC>(ur, at, width, u);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                v[c][i] = pair8(g[i], u[i], limit, alpha, offset);
+                v[c][i] = pair8<CAPPED>(g[i], u[i], limit, alpha, offset);
                 if (!VEC && at + i >= width) v[c][i] = 0.f;        // (an offset makes something of the zeros beyond the row)
             }
-            top = max(top, magnitude(v[c]));
+            top = magnitude(top, v[c]);
         }
     }
     const float most = at_least(row_max<WARP>(top, scratch));
@@ -289,11 +290,11 @@ void launch_norm8(const Shape& s, const float* x, long long ldx, const D* delta,
 #undef CB_NORM8
 }
 
-template <typename T, bool VEC>
-void launch_glu8(const Shape& s, const T* both, long long ldb, uint8_t* q, long long ldq, float* scales, int rows,
+template <typename T, bool VEC, bool CAPPED>
+void launch_glu8_as(const Shape& s, const T* both, long long ldb, uint8_t* q, long long ldq, float* scales, int rows,
                  int width, float limit, float alpha, float offset, cudaStream_t stream) {
 #define CB_GLU8(CH, WARP)                                                                                        \
-    cb_launch(glu8_kernel<T, CH, WARP, VEC>, s.grid, s.block, 0, stream, both, ldb, q, ldq, scales, rows, width, \
+    cb_launch(glu8_kernel<T, CH, WARP, VEC, CAPPED>, s.grid, s.block, 0, stream, both, ldb, q, ldq, scales, rows, width, \
               limit, alpha, offset)
     constexpr bool F32 = sizeof(T) == 4;               // (bf16 chunks are 8 long: no row has more than 4 a thread)
     if (s.warp)
@@ -301,6 +302,13 @@ void launch_glu8(const Shape& s, const T* both, long long ldb, uint8_t* q, long 
     else
         s.chunks == 1 ? CB_GLU8(1, false) : (s.chunks == 2 ? CB_GLU8(2, false) : (s.chunks == 4 ? CB_GLU8(4, false) : CB_GLU8((F32 ? 8 : 4), false)));
 #undef CB_GLU8
+}
+
+template <typename T, bool VEC>
+void launch_glu8(const Shape& s, const T* both, long long ldb, uint8_t* q, long long ldq, float* scales, int rows,
+                 int width, float limit, float alpha, float offset, cudaStream_t stream) {
+    if (limit > 0.f) launch_glu8_as<T, VEC, true>(s, both, ldb, q, ldq, scales, rows, width, limit, alpha, offset, stream);
+    else launch_glu8_as<T, VEC, false>(s, both, ldb, q, ldq, scales, rows, width, limit, alpha, offset, stream);
 }
 
 }  // namespace
