@@ -6,7 +6,8 @@
 // 16 + code, and one fused multiply-add, (16 + code) scale - 24 scale, is exact (24 scale has 2 + 4
 // significant bits).
 //
-// A fp32 row is the sum of three bf16 rows exactly: the 24 bits of the mantissa, 8 by 8.  Their
+// A fp32 row is the sum of three bf16 rows exactly: the 24 bits of the mantissa, 8 by 8 (of numbers below 2^-110
+// what lies below 2^-133, the last bit that bf16 has, is lost).  Their
 // products with the weights are exact too, and only fp32 sums are rounded.  The first part has a sum of
 // its own: the numbers of the others are 2^-8 of it and less, and a sum that held the first would
 // cut off their last bits at every addition (rows of 8,192: 2.4e-6 off with one sum).

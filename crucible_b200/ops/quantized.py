@@ -8,11 +8,13 @@ weights that are kept the same way, a scale per output feature (`Weights8`).
 feature scale, codes 0..15, the group scales e4m3, the feature scales float32.  (code - 8) times an
 e4m3 number has at most seven significant bits, so the tensor cores take the weights as they are, in
 bfloat16 without a rounding; float32 rows go through them as three bfloat16 parts that add up to the row
-exactly.  Sums are float32 in every product, and only the result is rounded.
+exactly (but for what lies below 2^-133).  Sums are float32 in every product, and only the result is rounded.  Which
+kernel runs, and with it the order of a sum, goes by the sizes, the number of rows among them.
 
 Everything here launches on torch's current stream of the tensors' device, keeps no buffer between
 calls and may be captured into a CUDA graph (a call that has to bring rows into another layout first
-allocates from torch's pool, as any captured torch operation does).
+allocates from torch's pool, as any captured torch operation does).  Outputs may not overlap inputs, but where
+a function says so.  The waits inside the products are bounded; `tensor_core.check_status` raises if one ran out.
 """
 from __future__ import annotations
 
@@ -193,24 +195,23 @@ class Weights8:
     that do, once, here."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        shape = values.shape
-        if not (len(shape) == 2 and values.dtype is E4M3 and scales.dtype is _F32 and values.is_contiguous()
-                and scales.shape == (shape[0],) and scales.is_contiguous() and shape[0] and shape[1]
-                and values.get_device() == scales.get_device()):
+        shape, dev = values.shape, values.get_device()
+        if (len(shape) == 2 and values.dtype is E4M3 and scales.dtype is _F32 and values.is_contiguous()
+                and scales.shape == (shape[0],) and scales.is_contiguous() and shape[0] > 0 and shape[1] > 0
+                and scales.get_device() == dev and shape[1] % 16 == 0 and values.data_ptr() % 16 == 0):
+            self.values, self.pitch = values, shape[1]
+        else:
             _rows(values, "8-bit weights", (E4M3,))
-            if values.shape[0] == 0 or values.shape[1] == 0:
-                raise KernelError(f"8-bit weights: an empty matrix {list(values.shape)}")
-            _vector(scales, "8-bit weights' scales", values.shape[0])
+            if shape[0] == 0 or shape[1] == 0:
+                raise KernelError(f"8-bit weights: an empty matrix {list(shape)}")
+            _vector(scales, "8-bit weights' scales", shape[0])
             _one_device(values, scales)
-        if not _aligned16(values) or (shape[0] > 1 and values.stride(0) > _MOST_PITCH):
-            values = _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
-        self.values = values
-        self.scales = scales
-        self.shape = shape
-        self.pitch = _pitch(self.values)
-        self.device = values.get_device()
-        if self.device >= 0:
-            _status(self.device)
+            if not _aligned16(values) or (shape[0] > 1 and values.stride(0) > _MOST_PITCH):
+                values = _in_aligned_rows(values.view(torch.uint8)).view(E4M3)
+            self.values, self.pitch = values, _pitch(values)
+        self.scales, self.shape, self.device = scales, shape, dev
+        if dev >= 0 and dev not in tensor_core._status:
+            _status(dev)
 
     @classmethod
     def pack(cls, w: torch.Tensor) -> "Weights8":
@@ -255,7 +256,7 @@ class Weights4:
             self.group = shape[1] * 8 // groups[1]
             self.shape = torch.Size((shape[0], shape[1] * 8))
             self.device = codes.get_device()
-            if self.device >= 0:
+            if self.device >= 0 and self.device not in tensor_core._status:
                 _status(self.device)
             return
         _rows(codes, "4-bit weights' codes", (torch.int32,))
@@ -374,16 +375,15 @@ def _tiles_us(kind: int, m: int, n: int, k: int, tok: int, shares: int) -> float
     c, parts = _COSTS[kind], 3 if kind == _FOUR_F32 else 1
     steps = -(-k // (128 if kind == _EIGHT else 64)) / shares
     per_sm = _blocks_an_sm(kind, tok)
-    left, us = -(-n // 128) * -(-m // tok) * shares, c.base
     fixed = c.block + c.block_row * tok
     if shares > 1:
         fixed += c.share + c.share_row * tok + c.share_block * shares
     alone = c.step + c.step_col * parts * tok
-    while left > 0:
-        now = min(left, N_SMS * per_sm)
-        left -= now
-        us += fixed + steps * max(alone * (c.two if now > N_SMS else 1.0), c.step_bytes * now / N_SMS)
-    return us
+
+    def round_of(blocks: int) -> float:
+        return fixed + steps * max(alone * (c.two if blocks > N_SMS else 1.0), c.step_bytes * blocks / N_SMS)
+    full, rest = divmod(-(-n // 128) * -(-m // tok) * shares, N_SMS * per_sm)
+    return c.base + full * round_of(N_SMS * per_sm) + (round_of(rest) if rest else 0.0)
 
 
 def _blocks_an_sm(kind: int, tok: int) -> int:
@@ -489,7 +489,8 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
 def linear8(rows: torch.Tensor, row_scales: torch.Tensor, w: Weights8, out: torch.Tensor,
             add: Optional[torch.Tensor] = None) -> None:
     """out = (rows * row_scales) . W^T (+ add): e4m3 `rows` [M, K], float32 `row_scales` [M]; `out`: float32
-    or bfloat16 [M, N]; `add`: float32 [M, N], which may be `out`."""
+    or bfloat16 [M, N]; `add`: float32 [M, N], which may be `out`.  K up to 2^20.  Rows that do not begin on
+    multiples of 16 bytes (`new_rows8` makes such that do) are brought into ones that do, at every call."""
     if not isinstance(w, Weights8):
         raise KernelError(f"linear8 takes Weights8, got {type(w).__name__}")
     dev, shape, rs, os = rows.get_device(), rows.shape, rows.stride(), out.stride()
@@ -514,7 +515,8 @@ def linear8(rows: torch.Tensor, row_scales: torch.Tensor, w: Weights8, out: torc
 
 def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch.Tensor] = None) -> None:
     """out = a . W^T (+ add): float32 or bfloat16 rows `a` [M, K]; `out`: float32 or bfloat16 [M, N]; `add`:
-    float32 [M, N], which may be `out`."""
+    float32 [M, N], which may be `out`.  K up to 2^20.  Rows that do not begin on multiples of 16 bytes are brought
+    into ones that do, at every call."""
     if not isinstance(w, Weights4):
         raise KernelError(f"linear4 takes Weights4, got {type(w).__name__}")
     dev, shape, rs, os = a.get_device(), a.shape, a.stride(), out.stride()
