@@ -14,6 +14,7 @@
 // A block owns 32 features and 8 or 16 rows; its warps take segments of K in turn and their sums are added
 // in the warps' order, so the order of a dot product's sum depends on K alone.  A warp asks for its next
 // segments' weights before it multiplies the present ones.
+#define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 
 namespace {
@@ -53,6 +54,7 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
     constexpr int ROWS = 8 * NT;
     __shared__ float sums[WARPS][FEATURES][ROWS + 1];
     cb_pdl_wait();
+    cb_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * FEATURES, m0 = blockIdx.y * ROWS;

@@ -20,6 +20,7 @@
 // memory (the first block's issues the MMAs), warps 2-9 take the sums out (two to a quarter of the lanes, 32
 // rows in turn), warp 10 sends the copies of codes, warps 11-18 make weights of them (two sets of four, 64
 // k in turn: between a warp's reading codes and its weights being there lie as long as two stages' MMAs).
+#define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized_tc.cuh"
 
 namespace {
@@ -105,7 +106,6 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
     constexpr int BK = Sizes<KIND>::BK, STAGES = Sizes<KIND>::STAGES;
     extern __shared__ uint8_t smem_raw[];
     Storage<KIND>& s = *reinterpret_cast<Storage<KIND>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    cb_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     volatile int* abort_flag = &s.abort_flag;
@@ -136,6 +136,9 @@ linear_pairs_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_c
     __syncthreads();
     tc::cluster_sync_all();             // the other block's barriers are ready too
     tc::tc_fence_after_sync();
+    // barriers and tensor memory are ready; what earlier kernels wrote is read from here on
+    cb_pdl_wait();
+    cb_pdl_trigger();
     const uint32_t tmem = s.tmem;
     Units u(p, tok, blockIdx.x >> 1, gridDim.x >> 1, chunk_k);
 

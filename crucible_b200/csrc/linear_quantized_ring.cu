@@ -9,6 +9,7 @@
 // A block's warps form groups: each owns 32 features, and the warps of a group take segments of 128 k in
 // turn, one of every stage.  Their sums are added in the warps' order, so the order of a dot product's sum depends on
 // the sizes alone.  A thread takes 16 neighbouring bytes of a feature's codes, 32 k, and the same k of its row.
+#define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 #include "tc_common.cuh"
 
@@ -51,7 +52,6 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
     extern __shared__ uint8_t smem_raw[];
     Storage<NT, GROUPS, SHARE>& s = *reinterpret_cast<Storage<NT, GROUPS, SHARE>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    cb_pdl_wait();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * S::FEATURES, m0 = blockIdx.y * S::ROWS;
     const int segments = (p.K + SEG - 1) / SEG, n_st = (segments + SHARE - 1) / SHARE;
@@ -65,6 +65,8 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
         tc::fence_barrier_init();
     }
     __syncthreads();
+    cb_pdl_wait();                      // (the barriers are ready; what earlier kernels wrote is read from here on)
+    cb_pdl_trigger();
     float acc[PAIRS][NT][4];
     const int group = warp / SHARE, turn = warp % SHARE;
     const int g = lane >> 2, t = lane & 3;

@@ -23,6 +23,7 @@
 // Roles: warp 0 sends the copies of the rows (and of 8-bit weights), warp 1 owns tensor memory and
 // issues the MMAs, warps 2-9 make weights of codes (two sets of four, 64 k in turn) and then take the sums
 // out (two to a quarter of the lanes, 32 rows in turn), warp 10 sends the copies of codes.
+#define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized_tc.cuh"
 
 namespace {
@@ -83,7 +84,6 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     extern __shared__ uint8_t smem_raw[];
     Storage<KIND, TOK>& s = *reinterpret_cast<Storage<KIND, TOK>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    cb_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * FEATURES, m0 = blockIdx.y * tok;
     const uint32_t rank = splits > 1 ? tc::cluster_rank() : 0u;
@@ -121,6 +121,9 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     tc::tc_fence_before_sync();
     __syncthreads();
     tc::tc_fence_after_sync();
+    // barriers and tensor memory are ready; what earlier kernels wrote is read from here on
+    cb_pdl_wait();
+    cb_pdl_trigger();
     const uint32_t tmem = s.tmem, weights = tmem + S::TMEM - WEIGHT_STAGES * WEIGHT_COLS;
 
     if (warp == 0) {
@@ -427,6 +430,7 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ rows, long long ldr,
                                                          __nv_bfloat16* __restrict__ parts, int M, int K) {
     cb_pdl_wait();
+    cb_pdl_trigger();
     const long long total = (long long)M * (K / 4);
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
         const long long m = i / (K / 4), k = i % (K / 4) * 4;

@@ -11,6 +11,7 @@
 // Memory bounds both: one pass over the data, a row's numbers stay in the registers of the threads
 // that fetched them (4 consecutive ones a chunk) while the row's sum of squares and largest
 // magnitude are taken.
+#define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "common.cuh"
 
 namespace {
@@ -107,6 +108,7 @@ norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const
     constexpr int E = 4;
     __shared__ float scratch[32];
     cb_pdl_wait();
+    cb_pdl_trigger();
     const long long row = (long long)blockIdx.x * (WARP ? blockDim.y : 1) + (WARP ? threadIdx.y : 0);
     if (row >= rows) return;                           // (a whole warp at a time: only with WARP)
     const int step = E * (WARP ? 32 : blockDim.x), at0 = E * threadIdx.x;
@@ -208,6 +210,7 @@ glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, 
     constexpr int E = 16 / sizeof(T);
     __shared__ uint32_t scratch[32];
     cb_pdl_wait();
+    cb_pdl_trigger();
     const long long row = (long long)blockIdx.x * (WARP ? blockDim.y : 1) + (WARP ? threadIdx.y : 0);
     if (row >= rows) return;
     const int step = E * (WARP ? 32 : blockDim.x), at0 = E * threadIdx.x;
