@@ -323,7 +323,7 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 
 # Which kernel, and how.  What follows was measured on B200 for the three kinds of product at 11 sizes of weights, 1,280 by
 # 768 to 28,672 by 4,096 (and 50,304 by 768, 4,096 by 14,336), and 1 to 2,048 rows, in every form: the rules below took
-# 1.0 to 1.3% longer than the best form on the average.
+# 0.8% longer than the best form on the average.
 #
 #   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
@@ -340,7 +340,7 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 # allows), what a cluster costs, and how many blocks follow one another on an SM.  us, in `_COSTS`.
 FORM = None                      # tests name one of the forms, "few", "ring", "tiles" or "pairs", to reach it at any size
 N_SMS = 148
-_SMALL, _SMALL_8_ROWS = 1_600_000, 4_200_000           # weights of a matrix that "few" ends first: up to 64 rows, up to 8
+_SMALL, _SMALL_8_ROWS = 1_200_000, 4_200_000           # weights of a matrix that "few" ends first: up to 64 rows, up to 8
 
 
 class _Costs(NamedTuple):
@@ -361,9 +361,9 @@ class _Costs(NamedTuple):
 
 
 _COSTS = {
-    _EIGHT: _Costs(0.88, 2.80, 0.0086, 0.150, 0.0010, 2.44, 0.214, 0.87, 0.0252, 0.10, 7.2, 0.160, 0.0008, 0.0052),
+    _EIGHT: _Costs(1.77, 0.80, 0.0116, 0.1705, 0.0011, 3.26, 0.232, 1.21, 0.0206, 0.13, 6.39, 0.152, 0.0007, 0.008),
     _FOUR_BF16: _Costs(3.58, 1.32, 0.0097, 0.1545, 0.0007, 1.90, 0.192, 1.17, 0.0111, 0.12, 10.1, 0.131, 0.0009, 0.0089),
-    _FOUR_F32: _Costs(3.97, 1.69, 0.0136, 0.179, 0.0004, 1.77, 0.022, 0.0, 0.0051, 0.73, 0.0, 0.0, 0.0, 0.0),
+    _FOUR_F32: _Costs(4.02, 1.16, 0.0190, 0.1736, 0.0005, 1.76, 0.237, 0.40, 0.0209, 0.21, 0.0, 0.0, 0.0, 0.0),
 }
 
 
