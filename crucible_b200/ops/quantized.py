@@ -37,6 +37,9 @@ LEAST = 1e-30                    # a row's largest magnitude counts as this much
 _FOUR_BF16, _FOUR_F32, _EIGHT = 0, 1, 2
 _MOST_PITCH = 1 << 24            # bytes between rows of weights (`csrc/quantized.cuh`)
 _FLOATS = (torch.float32, torch.bfloat16)
+_MOST_ROWS = (1 << 31) - 1024    # the kernels count rows and features in 32 bits
+_SLAB = 1 << 16                  # float32 rows over 4-bit weights at a time: three bfloat16 copies of them are needed
+_LEAST_LIMIT = 2.0 ** -126       # (a smaller limit could be zero in float32)
 
 
 # Every function asks first whether all is as it usually is, in one expression over plain attributes; only where it is
@@ -76,6 +79,12 @@ def _rows(t: torch.Tensor, what: str, dtypes, shape=None) -> None:
         raise KernelError(f"{what}: rows must be contiguous")
     if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         raise KernelError(f"{what}: rows must not overlap")
+    _count(t.shape[0], what)
+
+
+def _count(rows: int, what: str) -> None:
+    if rows > _MOST_ROWS:
+        raise KernelError(f"{what}: up to {_MOST_ROWS} rows are taken, got {rows}")
 
 
 def _vector(t: torch.Tensor, what: str, size: int) -> None:
@@ -106,7 +115,8 @@ def add_rmsnorm8(x: torch.Tensor, delta: Optional[torch.Tensor], gain: torch.Ten
     ds = xs if delta is None else delta.stride()
     if not (dev >= 0 and len(shape) == 2 and x.dtype is _F32 and out.dtype is E4M3 and scales.dtype is _F32
             and gain.dtype is _F32 and out.shape == shape and xs[1] == 1 == os[1] and xs[0] >= shape[1] <= os[0]
-            and gain.shape == (shape[1],) and scales.shape == (shape[0],) and gain.is_contiguous() and scales.is_contiguous()
+            and shape[0] <= _MOST_ROWS and gain.shape == (shape[1],) and gain.is_contiguous()
+            and scales.shape == (shape[0],) and scales.is_contiguous()
             and out.get_device() == dev == gain.get_device() and scales.get_device() == dev
             and (delta is None or (delta.shape == shape and delta.dtype in _FLOATS and ds[1] == 1
                                    and ds[0] >= shape[1] and delta.get_device() == dev))
@@ -145,7 +155,8 @@ def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Opt
     if not (dev >= 0 and len(shape) == 2 and both.dtype in _FLOATS and out.dtype is E4M3 and scales.dtype is _F32
             and both.shape == (shape[0], 2 * shape[1]) and bs[1] == 1 == os[1] and bs[0] >= 2 * shape[1]
             and os[0] >= shape[1] and scales.shape == (shape[0],) and scales.is_contiguous()
-            and out.get_device() == dev == scales.get_device() and (limit is None or limit > 0)):
+            and out.get_device() == dev == scales.get_device() and shape[0] <= _MOST_ROWS
+            and (limit is None or limit >= _LEAST_LIMIT)):
         _look_over_glu8(both, out, scales, limit)
     lib = build.load("rows8")
     code = _at(dev, lib.cb_glu8, both.data_ptr(), 0 if both.dtype is _F32 else 1, bs[0], out.data_ptr(), os[0],
@@ -159,8 +170,8 @@ def _look_over_glu8(both, out, scales, limit) -> None:
     _rows(both, "glu8 input", _FLOATS)
     if both.shape[1] % 2:
         raise KernelError(f"glu8 takes rows [g | u] of an even width, got {both.shape[1]}")
-    if limit is not None and not limit > 0:
-        raise KernelError("glu8: the limit must be positive")
+    if limit is not None and not limit >= _LEAST_LIMIT:
+        raise KernelError(f"glu8: the limit must be positive, {_LEAST_LIMIT:.3g} or more, got {limit}")
     _rows(out, "glu8 output", (E4M3,), (both.shape[0], both.shape[1] // 2))
     _vector(scales, "glu8 scales", both.shape[0])
     _need_cuda(both, out, scales)
@@ -462,6 +473,7 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
     if m == 0:
         return
     n, k = w.shape
+    _count(max(m, n), what)
     form = form_of(kind, m, n, k)
     common = (kind, rows.data_ptr(), ldr, row_scales, values.data_ptr(), ldw, group_scales, w.scales.data_ptr(),
               _ptr(add), add.stride(0) if add is not None else 0, out.data_ptr(), 0 if out.dtype is _F32 else 1, ldo, m, n, k,
@@ -534,5 +546,10 @@ def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch
         if not _aligned16(a):
             a = _in_aligned_rows(a)
         rs = (_pitch(a),)
+    if f32 and shape[0] > _SLAB:
+        for at in range(0, shape[0], _SLAB):
+            to = at + _SLAB
+            linear4(a[at:to], w, out[at:to], add=None if add is None else add[at:to])
+        return
     _product(_FOUR_F32 if f32 else _FOUR_BF16, dev, a, shape[0], rs[0], None, w.codes, k // 2, w.group_scales.data_ptr(),
              w, w.group, out, os[0], add, "linear (4-bit weights)")

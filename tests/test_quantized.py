@@ -155,3 +155,21 @@ def test_a_described_config_keeps_the_group():
             again = get_architecture(cfg.architecture).describe(cfg)
             assert again.get("feed_forward_weight_group") == extra.get("feed_forward_weight_group")
             assert parse_config(again).layers == cfg.layers
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    many = 1 << 31
+    x, out, scales = (torch.empty(many, 1, device="meta"), torch.empty(many, 1, dtype=E4M3, device="meta"),
+                      torch.empty(many, device="meta"))
+    _refused("up to 2147482624 rows", quantized.add_rmsnorm8, x, None, torch.ones(1), 1e-5, out, scales)
+    _refused("up to 2147482624 rows", quantized.glu8, torch.empty(many, 2, device="meta"), out, scales)
+    w8, w4 = random_weights8(1, 1, "cpu", _gen()), random_weights4(1, 32, 32, "cpu", _gen())
+    _refused("up to 2147482624 rows", quantized.linear8, out, scales, w8, x)
+    _refused("up to 2147482624 rows", quantized.linear4, torch.empty(many, 32, device="meta"), w4, x)
+
+
+def test_a_limit_that_float32_may_have_as_zero_is_refused():
+    both, q, s = torch.zeros(3, 40), quantized.new_rows8(3, 20, "cpu"), torch.zeros(3)
+    for limit in (1e-50, 2.0 ** -127, -1.0):
+        _refused("limit", quantized.glu8, both, q, s, limit)
+    _refused("CUDA device", quantized.glu8, both, q, s, 2.0 ** -126)

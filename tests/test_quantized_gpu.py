@@ -228,6 +228,18 @@ def test_linear4_prompts(rows, n, k, group, dtype):
     _check4(rows, n, k, group, DTYPES[dtype], torch.float32, True)
 
 
+@pytest.mark.parametrize("rows", [128, 129, 300])
+def test_float32_rows_a_slab_at_a_time(rows, monkeypatch):
+    monkeypatch.setattr(quantized, "_SLAB", 128)
+    _check4(rows, 200, 256, 64, torch.float32, torch.float32, True)
+    _check4(rows, 200, 256, 64, torch.float32, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear4_millions_of_rows(dtype):
+    _check4(4_200_000, 3, 32, 32, DTYPES[dtype], torch.float32, False)
+
+
 @pytest.mark.parametrize("rows", [1, 8, 40, 300])
 def test_products_add_into_their_output(rows):
     gen = _gen(rows)
