@@ -148,9 +148,9 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
                             b16[j][c] = __ldg(reinterpret_cast<const uint4*>(rows[j] + seg * SEG * SIZE) + c);
                     }
             }
-            uint32_t s2[PAIRS][2], c2[PAIRS][2];
+            ScalePair s[PAIRS][2];
 #pragma unroll
-            for (int i = 0; i < PAIRS; ++i) scale_pairs(h.scale[i], s2[i], c2[i]);
+            for (int i = 0; i < PAIRS; ++i) scale_pairs(h.scale[i], s[i]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {               // eight k at a time
                 uint32_t b[NT][3][4];                   // [rows][part][pairs of k]
@@ -180,8 +180,8 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
                     const uint32_t yw = c == 0 ? y.x : (c == 1 ? y.y : (c == 2 ? y.z : y.w));
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        const uint32_t a[4] = {weight_pair(xw, 2 * q, s2[i][0], c2[i][0]), weight_pair(yw, 2 * q, s2[i][1], c2[i][1]),
-                                               weight_pair(xw, 2 * q + 1, s2[i][0], c2[i][0]), weight_pair(yw, 2 * q + 1, s2[i][1], c2[i][1])};
+                        const uint32_t a[4] = {weight_pair(xw, 2 * q, s[i][0]), weight_pair(yw, 2 * q, s[i][1]),
+                                               weight_pair(xw, 2 * q + 1, s[i][0]), weight_pair(yw, 2 * q + 1, s[i][1])};
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
                             mma_bf16(acc[i][j], a, b[j][0][2 * q], b[j][0][2 * q + 1]);

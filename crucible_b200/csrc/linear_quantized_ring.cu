@@ -7,8 +7,12 @@
 // of 4,096 by 28,672).
 //
 // A block's warps form groups: each owns 32 features, and the warps of a group take segments of 128 k in
-// turn, one of every stage.  Their sums are added in the warps' order, so the order of a dot product's sum depends on
-// the sizes alone.  A thread takes 16 neighbouring bytes of a feature's codes, 32 k, and the same k of its row.
+// turn, one of every stage.  Few features: the blocks (x, y, 0..S-1) form a cluster that splits K.  The warps' and the
+// blocks' sums are added in their order, so the order of a dot product's sum depends on the sizes alone.  A thread takes
+// 16 neighbouring bytes of a feature's codes, 32 k, and the same k of its row.
+//
+// What it takes is instructions (issue slots 59%, the units of shifts and of bf16 arithmetic about half of the time):
+// more warps an SM, fewer waits, group scales through shared memory and blocks that stay and share the features evenly changed nothing.
 #define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 #include "tc_common.cuh"
@@ -21,8 +25,8 @@ constexpr int PAIRS = 2;                // 16 features each: a group's
 template <int NT, int GROUPS, int SHARE> struct Sizes {
     static constexpr int WARPS = GROUPS * SHARE, FEATURES = GROUPS * 16 * PAIRS, ROWS = 8 * NT;
     static constexpr int CODES_BYTES = FEATURES * 64 * SHARE, ROWS_BYTES = ROWS * 256 * SHARE;
-    static constexpr int BLOCKS = WARPS > 8 ? 1 : 2;
-    static constexpr int FIT = (BLOCKS == 2 ? 108 * 1024 : 200 * 1024) / (CODES_BYTES + ROWS_BYTES);
+    static constexpr int BLOCKS = 16 / WARPS;
+    static constexpr int FIT = 216 * 1024 / BLOCKS / (CODES_BYTES + ROWS_BYTES);
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static_assert(STAGES >= 2, "a ring");
 };
@@ -47,14 +51,16 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int c) { return c ==
 template <int NT, int GROUPS, int SHARE>
 __global__ void __launch_bounds__(GROUPS * SHARE * 32 + 32, Sizes<NT, GROUPS, SHARE>::BLOCKS)
 linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
-                   const QuantizedArgs p, uint32_t run_magic, int* __restrict__ status) {
+                   const QuantizedArgs p, uint32_t run_magic, int splits, int* __restrict__ status) {
     using S = Sizes<NT, GROUPS, SHARE>;
     extern __shared__ uint8_t smem_raw[];
     Storage<NT, GROUPS, SHARE>& s = *reinterpret_cast<Storage<NT, GROUPS, SHARE>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * S::FEATURES, m0 = blockIdx.y * S::ROWS;
-    const int segments = (p.K + SEG - 1) / SEG, n_st = (segments + SHARE - 1) / SHARE;
+    const int segments = (p.K + SEG - 1) / SEG, stages = (segments + SHARE - 1) / SHARE;
+    // this block's share of K; the launcher keeps it from being empty
+    const int per = (stages + splits - 1) / splits, begin = (int)blockIdx.z * per, end = min(stages, begin + per);
     volatile int* abort_flag = &s.abort_flag;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
@@ -78,14 +84,14 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
         if (tc::elect_one()) {
             int st = 0, sent = 0;
             uint32_t parity = 1;
-            for (int i = 0; i < n_st; ++i) {
+            for (int i = 0; i < end - begin; ++i) {
                 if (i >= S::STAGES && !tc::mbar_wait(&s.empty[st], parity, abort_flag)) {
                     tc::give_up(abort_flag, status, tc::ST_PRODUCER_TIMEOUT);
                     break;
                 }
                 tc::mbar_expect_tx(&s.full[st], S::CODES_BYTES + S::ROWS_BYTES);
-                tc::tma_load_3d(s.codes[st], &map_w, &s.full[st], 0, n0, i * (SHARE / 2));
-                tc::tma_load_3d(s.rows[st], &map_rows, &s.full[st], 0, m0, i * (SHARE * 2));
+                tc::tma_load_3d(s.codes[st], &map_w, &s.full[st], 0, n0, (begin + i) * (SHARE / 2));
+                tc::tma_load_3d(s.rows[st], &map_rows, &s.full[st], 0, m0, (begin + i) * (SHARE * 2));
                 sent = i + 1;
                 if (++st == S::STAGES) st = 0, parity ^= 1;
             }
@@ -127,11 +133,11 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
         const int rows_at = (turn * 2 + (t >> 1)) * (S::ROWS * 128) + g * 128;
         const int piece0 = (t & 1) * 4;
         uint32_t scale[PAIRS], next[PAIRS];
-        ask(next, turn);
+        ask(next, begin * SHARE + turn);
         int st = 0;
         uint32_t parity = 0;
 #pragma unroll 1
-        for (int i = 0; i < n_st; ++i) {
+        for (int i = begin; i < end; ++i) {
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) scale[q] = next[q];
             const int seg = i * SHARE + turn;
@@ -146,12 +152,12 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
                 const uint8_t* codes = s.codes[st] + codes_at;
                 const uint8_t* rows = s.rows[st] + rows_at;
                 uint4 x[PAIRS], y[PAIRS];
-                uint32_t s2[PAIRS][2], c2[PAIRS][2];
+                ScalePair both[PAIRS][2];
 #pragma unroll
                 for (int q = 0; q < PAIRS; ++q) {
                     x[q] = *reinterpret_cast<const uint4*>(codes + q * 2048);
                     y[q] = *reinterpret_cast<const uint4*>(codes + q * 2048 + 1024);
-                    scale_pairs(scale[q], s2[q], c2[q]);
+                    scale_pairs(scale[q], both[q]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {               // eight k at a time
@@ -163,8 +169,8 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
                         const uint32_t xw = word_of(x[q], c), yw = word_of(y[q], c);
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint32_t a[4] = {weight_pair(xw, 2 * e, s2[q][0], c2[q][0]), weight_pair(yw, 2 * e, s2[q][1], c2[q][1]),
-                                                   weight_pair(xw, 2 * e + 1, s2[q][0], c2[q][0]), weight_pair(yw, 2 * e + 1, s2[q][1], c2[q][1])};
+                            const uint32_t a[4] = {weight_pair(xw, 2 * e, both[q][0]), weight_pair(yw, 2 * e, both[q][1]),
+                                                   weight_pair(xw, 2 * e + 1, both[q][0]), weight_pair(yw, 2 * e + 1, both[q][1])};
 #pragma unroll
                             for (int j = 0; j < NT; ++j) mma_bf16(acc[q][j], a, e ? b[j].z : b[j].x, e ? b[j].w : b[j].y);
                         }
@@ -191,17 +197,47 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
                     sums[(turn * S::FEATURES + 32 * group + 16 * i + 8 * (e >> 1) + mine) * (S::ROWS + 1) + 8 * j + 2 * t + (e & 1)] = acc[i][j][e];
     }
     __syncthreads();
-    if (!whole) return;
+    auto each = [&](int first, int step, auto sum_of) {
 #pragma unroll 1
-    for (int at = threadIdx.x; at < S::FEATURES * S::ROWS; at += S::WARPS * 32 + 32) {
-        const int f = at % S::FEATURES, m = at / S::FEATURES;
-        if (m0 + m >= p.M) break;
-        if (n0 + f >= p.N) continue;
+        for (int at = first; at < S::FEATURES * S::ROWS; at += step) {
+            const int f = at % S::FEATURES, m = at / S::FEATURES;
+            if (m0 + m >= p.M) break;
+            if (n0 + f >= p.N) continue;
+            finish(p, sum_of(at, f, m), 1.f, __ldg(p.feature_scale + n0 + f), m0 + m, n0 + f);
+        }
+    };
+    auto warps_sum = [&](int at, int f, int m) {
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) v += sums[(i * S::FEATURES + f) * (S::ROWS + 1) + m];
-        finish(p, v, 1.f, __ldg(p.feature_scale + n0 + f), m0 + m, n0 + f);
+        return v;
+    };
+    constexpr int THREADS = S::WARPS * 32 + 32;
+    if (splits == 1) {
+        if (whole) each(threadIdx.x, THREADS, warps_sum);
+        return;
     }
+    // The blocks of a cluster split K: each leaves its sums in its shared memory, and each adds up a share of the numbers from all
+    // of them, in their order.
+    float* const mine_of_k = sums + SHARE * S::FEATURES * (S::ROWS + 1);            // [ROWS][FEATURES]
+    static_assert((SHARE * (S::ROWS + 1) + S::ROWS) * S::FEATURES * 4 <= (int)(sizeof(s.codes) + sizeof(s.rows)), "the sums fit in the ring");
+    for (int at = threadIdx.x; at < S::FEATURES * S::ROWS; at += THREADS) mine_of_k[at] = warps_sum(at, at % S::FEATURES, at / S::FEATURES);
+    __syncwarp();
+    tc::cluster_sync_all();
+    const uint32_t theirs = tc::smem_u32(mine_of_k);
+    if (whole)
+        each((int)blockIdx.z * THREADS + threadIdx.x, splits * THREADS, [&](int at, int, int) {
+            float v = 0.f;
+#pragma unroll 4
+            for (int q = 0; q < splits; ++q) {
+                float x;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_map(theirs + 4 * at, (uint32_t)q)) : "memory");
+                v += x;
+            }
+            return v;
+        });
+    __syncwarp();
+    tc::cluster_sync_all();             // nobody goes while his shared memory is read
 }
 
 // A matrix of rows of `row_bytes` bytes (a multiple of 128) as [128 bytes of a row][row][128 bytes], read in boxes of `depth`
@@ -219,7 +255,7 @@ bool ring_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_by
 }
 
 template <int NT, int GROUPS, int SHARE>
-int launch(const QuantizedArgs& p, uint32_t run_magic, int* status, cudaStream_t stream) {
+int launch(const QuantizedArgs& p, uint32_t run_magic, int splits, int* status, cudaStream_t stream) {
     using S = Sizes<NT, GROUPS, SHARE>;
     constexpr int SMEM = (int)sizeof(Storage<NT, GROUPS, SHARE>) + 1024;
     CUtensorMap mr, mw;
@@ -230,33 +266,39 @@ int launch(const QuantizedArgs& p, uint32_t run_magic, int* status, cudaStream_t
     auto kernel = linear_ring_kernel<NT, GROUPS, SHARE>;
     const int rc = allow_shared(kernel, SMEM, configured);
     if (rc != 0) return rc;
-    cb_launch(kernel, dim3((p.N + S::FEATURES - 1) / S::FEATURES, (p.M + S::ROWS - 1) / S::ROWS), dim3(S::WARPS * 32 + 32), SMEM,
-              stream, mr, mw, p, run_magic, status);
+    const int stages = (p.K + SHARE * SEG - 1) / (SHARE * SEG);
+    if (splits > stages) splits = stages;
+    while (splits > 1 && (splits - 1) * ((stages + splits - 1) / splits) >= stages) --splits;
+    cb_launch_cluster(kernel, dim3((p.N + S::FEATURES - 1) / S::FEATURES, (p.M + S::ROWS - 1) / S::ROWS, splits),
+                      dim3(S::WARPS * 32 + 32), SMEM, stream, splits, mr, mw, p, run_magic, splits, status);
     return cb_last_error();
 }
 
 template <int NT>
-int launch_groups(const QuantizedArgs& p, int groups, uint32_t run_magic, int* status, cudaStream_t stream) {
-    if (groups == 4) return launch<NT, 4, 2>(p, run_magic, status, stream);
-    if (groups == 2) return launch<NT, 2, 4>(p, run_magic, status, stream);
-    return launch<NT, 1, 8>(p, run_magic, status, stream);
+int launch_as(const QuantizedArgs& p, int groups, int share, int splits, uint32_t run_magic, int* status, cudaStream_t stream) {
+    if (groups == 1 && share == 8) return launch<NT, 1, 8>(p, run_magic, splits, status, stream);
+    if (groups == 1 && share == 4) return launch<NT, 1, 4>(p, run_magic, splits, status, stream);
+    if (groups == 2 && share == 4) return launch<NT, 2, 4>(p, run_magic, splits, status, stream);
+    if (groups == 2 && share == 2) return launch<NT, 2, 2>(p, run_magic, splits, status, stream);
+    return CB_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
-// `groups` of warps a block: 1, 2 or 4, of 32 features each.  K a multiple of 256; rows bf16.
+// `groups` of `share` warps a block, of 32 features a group: 1 x 8, 2 x 4, 1 x 4 or 2 x 2; `splits`:
+// shares of K, 1 to 8 (as many as leave none empty).  K a multiple of 256; rows bf16.
 CB_EXPORT int cb_linear_quantized_ring(int kind, const void* rows, long long ldr, const float* row_scale, const void* w,
                                        long long ldw, const void* group_scale, const float* feature_scale,
                                        const float* add, long long lda, void* out, int out_dtype, long long ldo, int M,
-                                       int N, int K, int group, int groups, int* status, void* stream) {
+                                       int N, int K, int group, int groups, int share, int splits, int* status, void* stream) {
     if (M <= 0 || N <= 0) return 0;
     if (kind != FOUR_BF16 || K <= 0 || K % 256 || K > MOST_K || (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * 2) | (uintptr_t)ldw) & 15) ||
-        (M + 7) / 8 > 65535 || group <= 0 || group % 32 || K % group || (groups != 1 && groups != 2 && groups != 4))
+        (M + 7) / 8 > 65535 || group <= 0 || group % 32 || K % group || splits < 1 || splits > 8)
         return CB_ERR_UNSUPPORTED;
     const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
                              M, N, K, group, out_dtype == CB_BF16, K / group};
     const uint32_t runs = (uint32_t)group / 32;
     const uint32_t run_magic = (uint32_t)(((1ull << 31) + runs - 1) / runs);
     cudaStream_t s = (cudaStream_t)stream;
-    return M <= 8 ? launch_groups<1>(p, groups, run_magic, status, s) : launch_groups<2>(p, groups, run_magic, status, s);
+    return M <= 8 ? launch_as<1>(p, groups, share, splits, run_magic, status, s) : launch_as<2>(p, groups, share, splits, run_magic, status, s);
 }

@@ -35,8 +35,13 @@ struct QuantizedArgs {
     int M, N, K, group, out_bf16, groups;           // groups: K / group
 };
 
-// Two e4m3 scales (the lower two bytes), each as a pair of equal bf16 numbers and as -24 times that: all exact.
-__device__ __forceinline__ void scale_pairs(uint32_t e4m3x2, uint32_t (&s2)[2], uint32_t (&c2)[2]) {
+// An e4m3 scale as a pair of equal bf16 numbers, and -24 and -136 times that: all exact.
+struct ScalePair {
+    uint32_t s, c24, c136;
+};
+
+// Two e4m3 scales (the lower two bytes).
+__device__ __forceinline__ void scale_pairs(uint32_t e4m3x2, ScalePair (&scale)[2]) {
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)e4m3x2));
     float s[2];
@@ -44,19 +49,20 @@ __device__ __forceinline__ void scale_pairs(uint32_t e4m3x2, uint32_t (&s2)[2], 
         : "=f"(s[0]), "=f"(s[1]) : "r"(h2));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s2[i]) : "f"(s[i]));
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(c2[i]) : "r"(s2[i]), "r"(0xC1C0C1C0u));       // -24
+        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(scale[i].s) : "f"(s[i]));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(scale[i].c24) : "r"(scale[i].s), "r"(0xC1C0C1C0u));       // -24
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(scale[i].c136) : "r"(scale[i].s), "r"(0xC308C308u));      // -136
     }
 }
 
 // Pair i (k = 2i, 2i + 1) of a word of eight codes as two bf16 weights.  (The mask and the 16s come as registers: with
 // both as constants the compiler takes two instructions for them, and the unit that runs them is what a product of a few rows
 // waits for.)
-__device__ __forceinline__ uint32_t weight_pair(uint32_t word, int i, uint32_t s2, uint32_t c2) {
-    const uint32_t put = i == 0 ? word << 3 : word >> (4 * i - 3);
+__device__ __forceinline__ uint32_t weight_pair(uint32_t word, int i, const ScalePair& scale) {
     uint32_t magic, r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(magic) : "r"(put), "r"(0x00780078u), "r"(0x41804180u));   // 16 + code, twice
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(magic), "r"(s2), "r"(c2));
+    if (i == 0) asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(magic) : "r"(word), "r"(0x000F000Fu), "r"(0x43004300u));      // 128 + code, twice
+    else asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(magic) : "r"(word >> (4 * i - 3)), "r"(0x00780078u), "r"(0x41804180u));   // 16 + code
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(magic), "r"(scale.s), "r"(i == 0 ? scale.c136 : scale.c24));
     return r;
 }
 

@@ -16,12 +16,12 @@ __device__ __forceinline__ void make_weights(const uint8_t* codes_row, int j, in
     const uint4 c0 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j) ^ (r & 7)) << 4));
     const uint4 c1 = *reinterpret_cast<const uint4*>(codes_row + (((2 * j + 1) ^ (r & 7)) << 4));
     const uint32_t word[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    uint32_t s2[2], c2[2];
-    scale_pairs(two_scales, s2, c2);
+    ScalePair s[2];
+    scale_pairs(two_scales, s);
 #pragma unroll
     for (int c = 0; c < 8; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * c + i] = weight_pair(word[c], i, s2[c >> 2], c2[c >> 2]);
+        for (int i = 0; i < 4; ++i) v[4 * c + i] = weight_pair(word[c], i, s[c >> 2]);
 }
 
 // The group scales of one feature, 256 k (eight runs of 32) at a time, asked for a stage of codes ahead.  Where 256 k

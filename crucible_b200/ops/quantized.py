@@ -339,10 +339,14 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
 #   "ring"   the same arithmetic behind a ring of stages: 4-bit weights and bfloat16 rows, K a multiple of 256.  8 rows of
-#            4,096 by 4,096, ring / few / tiles: 5.8 / 7.5 / 9.5; 16 rows by 14,336 15.4 / 22.0 / 18.4; 32 rows by 2,048 (K of
-#            8,192) 11.1 / 14.5 / 12.9, by 6,144 (K of 4,096) 14.4 / 18.3 / 12.8.  More groups of warps a block read the
-#            rows less often, as long as every SM still has two blocks: 1 / 2 / 4 groups by 14,336 13.3 / 12.7 / 14.1, by
-#            50,304 (K of 768) 14.0 / 12.3 / 10.4.
+#            4,096 by 4,096, ring / few / tiles: 5.3 / 7.5 / 9.5; 16 rows by 14,336 14.9 / 22.0 / 18.4; 32 rows by 2,048 (K of
+#            8,192) 11.1 / 14.5 / 12.9, by 6,144 (K of 4,096) 14.4 / 18.3 / 12.8.  A block is so many groups of warps by
+#            warps that share a group's K: 1 x 8 while the SMs have two blocks or fewer at once, 1 x 4 beyond (8 rows by
+#            28,672, 1 x 8 / 1 x 4 / 2 x 4: 23.4 / 20.2 / 23.0; by 4,096 5.3 / 6.0 / 7.6), 2 x 2 where K is short beside
+#            the features and the rows are best read less often (by 50,304, K of 768, 1 x 4 / 2 x 2: 9.7 / 8.8), 2 x 4 for
+#            16 rows, whose stages are larger (by 14,336, 1 x 4 / 2 x 4: 16.9 / 14.9).  Few features and a long K: blocks of
+#            a cluster share K (8 rows by 2,048, K of 14,336, one share / four: 12.6 / 8.6; K of 8,192 8.3 / 6.1; by
+#            4,096, K of 4,096, one / two: 5.3 / 5.9).
 #   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K.
 #   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
 #
@@ -414,9 +418,22 @@ def _even(m: int, most: int) -> int:
     return _up(-(-m // -(-m // most)), 16)
 
 
+def _ring(m: int, n: int, k: int):
+    """Groups of warps a block, warps a group, blocks that share K."""
+    if n >= (9472 if k <= 1024 else 12000):
+        if n >= (16 if m <= 8 else 24) * k:
+            return 2, 2, 1
+        return (1, 4, 1) if m <= 8 or k <= 1024 else (2, 4, 1)
+    blocks, stages, shares = -(-n // 32) * -(-m // (8 if m <= 8 else 16)), -(-k // 1024), 1
+    while shares < 8 and 2 * shares <= stages and 2 * shares * blocks <= 2 * N_SMS:
+        shares *= 2
+    return 1, 8, shares if shares >= 4 or stages >= 12 else 1
+
+
 @functools.lru_cache(maxsize=4096)
 def _rule(forced, kind: int, m: int, n: int, k: int):
-    """("few",), ("ring", groups of warps), ("tiles", rows a tile, shares of K) or ("pairs", rows a tile, pairs of SMs)."""
+    """("few",), ("ring", groups of warps, warps a group, shares of K), ("tiles", rows a tile, shares of K) or
+    ("pairs", rows a tile, pairs of SMs)."""
     form = forced
     if form is None:
         small = n * k <= _SMALL and m <= 64
@@ -429,7 +446,7 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
     if form == "few":
         return ("few",)
     if form == "ring":
-        return "ring", 4 if n >= 37888 else 2 if n >= 9472 else 1
+        return ("ring",) + _ring(m, n, k)
     units = -(-k // (128 if kind == _EIGHT else 256))
     best = None
     if form != "pairs" or kind == _FOUR_F32:
@@ -483,7 +500,7 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
     else:
         status = _status(dev)
         if form[0] == "ring":
-            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, form[1], status)
+            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, *form[1:], status)
         elif form[0] == "pairs":
             code = _at(dev, build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs, *common, form[1],
                        form[2], status)

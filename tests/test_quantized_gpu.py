@@ -193,6 +193,20 @@ def test_linear4_by_the_ring(rows, n, k, group, monkeypatch):
     _check4(rows, n, k, group, torch.bfloat16, torch.bfloat16, False)
 
 
+@pytest.mark.parametrize("block", [(1, 8), (1, 4), (2, 4), (2, 2)])
+@pytest.mark.parametrize("shares", [1, 2, 3, 4, 8])
+def test_linear4_by_rings_that_share_k(block, shares, monkeypatch):
+    monkeypatch.setattr(quantized, "_rule", lambda *sizes: ("ring", *block, shares))
+    for rows, n, k, group in ((1, 33, 256, 32), (8, 100, 2304, 64), (9, 64, 4096, 4096), (20, 129, 1280, 160), (3, 31, 8448, 96)):
+        _check4(rows, n, k, group, torch.bfloat16, torch.float32, True)
+        _check4(rows, n, k, group, torch.bfloat16, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("rows,n,k,group", [(1, 2048, 8192, 64), (8, 500, 14336, 128), (16, 1280, 4096, 64), (20, 512, 8192, 32)])
+def test_linear4_of_few_features(rows, n, k, group):
+    _check4(rows, n, k, group, torch.bfloat16, torch.float32, True)
+
+
 def _check4(rows, n, k, group, dtype, out_dtype, add, seed=0):
     gen = _gen(seed + rows * 7919 + n * 31 + k)
     w = random_weights4(n, k, group, DEV, gen)
