@@ -1,4 +1,5 @@
-// out[M,N] = rows[M,K] . W[N,K]^T for few bf16 rows (decoded tokens) and 4-bit weights whose K is a multiple of 256.
+// out[M,N] = rows[M,K] . W[N,K]^T for few rows (decoded tokens) and 4-bit weights whose K is a multiple of 256.  Rows are
+// bf16; up to five fp32 ones are made three bf16 ones each by a kernel before this one, whose sums meet at the way out.
 //
 // The arithmetic of linear_quantized_few: codes become bf16 weights, exactly (see quantized.cuh), in the registers
 // that hold mma.sync's operands.  Here codes and rows come through a ring of stages in shared memory that one
@@ -51,7 +52,7 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int c) { return c ==
 template <int NT, int GROUPS, int SHARE>
 __global__ void __launch_bounds__(GROUPS * SHARE * 32 + 32, Sizes<NT, GROUPS, SHARE>::BLOCKS)
 linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
-                   const QuantizedArgs p, uint32_t run_magic, int splits, int* __restrict__ status) {
+                   const QuantizedArgs p, uint32_t run_magic, int parts, int splits, int* __restrict__ status) {
     using S = Sizes<NT, GROUPS, SHARE>;
     extern __shared__ uint8_t smem_raw[];
     Storage<NT, GROUPS, SHARE>& s = *reinterpret_cast<Storage<NT, GROUPS, SHARE>*>(
@@ -203,10 +204,12 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
             const int f = at % S::FEATURES, m = at / S::FEATURES;
             if (m0 + m >= p.M) break;
             if (n0 + f >= p.N) continue;
-            finish(p, sum_of(at, f, m), 1.f, __ldg(p.feature_scale + n0 + f), m0 + m, n0 + f);
+            float v = sum_of(f, m);
+            if (parts == 3) v += sum_of(f, p.M + m) + sum_of(f, 2 * p.M + m);
+            finish(p, v, 1.f, __ldg(p.feature_scale + n0 + f), m0 + m, n0 + f);
         }
     };
-    auto warps_sum = [&](int at, int f, int m) {
+    auto warps_sum = [&](int f, int m) {
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) v += sums[(i * S::FEATURES + f) * (S::ROWS + 1) + m];
@@ -221,17 +224,17 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
     // of them, in their order.
     float* const mine_of_k = sums + SHARE * S::FEATURES * (S::ROWS + 1);            // [ROWS][FEATURES]
     static_assert((SHARE * (S::ROWS + 1) + S::ROWS) * S::FEATURES * 4 <= (int)(sizeof(s.codes) + sizeof(s.rows)), "the sums fit in the ring");
-    for (int at = threadIdx.x; at < S::FEATURES * S::ROWS; at += THREADS) mine_of_k[at] = warps_sum(at, at % S::FEATURES, at / S::FEATURES);
+    for (int at = threadIdx.x; at < S::FEATURES * S::ROWS; at += THREADS) mine_of_k[at] = warps_sum(at % S::FEATURES, at / S::FEATURES);
     __syncwarp();
     tc::cluster_sync_all();
     const uint32_t theirs = tc::smem_u32(mine_of_k);
     if (whole)
-        each((int)blockIdx.z * THREADS + threadIdx.x, splits * THREADS, [&](int at, int, int) {
+        each((int)blockIdx.z * THREADS + threadIdx.x, splits * THREADS, [&](int f, int m) {
             float v = 0.f;
 #pragma unroll 4
             for (int q = 0; q < splits; ++q) {
                 float x;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_map(theirs + 4 * at, (uint32_t)q)) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_map(theirs + 4 * (m * S::FEATURES + f), (uint32_t)q)) : "memory");
                 v += x;
             }
             return v;
@@ -255,12 +258,12 @@ bool ring_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_by
 }
 
 template <int NT, int GROUPS, int SHARE>
-int launch(const QuantizedArgs& p, uint32_t run_magic, int splits, int* status, cudaStream_t stream) {
+int launch(const QuantizedArgs& p, uint32_t run_magic, int parts, int splits, int* status, cudaStream_t stream) {
     using S = Sizes<NT, GROUPS, SHARE>;
     constexpr int SMEM = (int)sizeof(Storage<NT, GROUPS, SHARE>) + 1024;
     CUtensorMap mr, mw;
     if (!ring_map(&mw, p.w, (uint64_t)p.N, (uint64_t)p.K / 2, (uint64_t)p.ldw, S::FEATURES, SHARE / 2) ||
-        !ring_map(&mr, p.rows, (uint64_t)p.M, (uint64_t)p.K * 2, (uint64_t)p.ldr * 2, S::ROWS, SHARE * 2))
+        !ring_map(&mr, p.rows, (uint64_t)p.M * parts, (uint64_t)p.K * 2, (uint64_t)p.ldr * 2, S::ROWS, SHARE * 2))
         return CB_ERR_UNSUPPORTED;
     static bool configured[64] = {};
     auto kernel = linear_ring_kernel<NT, GROUPS, SHARE>;
@@ -270,35 +273,45 @@ int launch(const QuantizedArgs& p, uint32_t run_magic, int splits, int* status, 
     if (splits > stages) splits = stages;
     while (splits > 1 && (splits - 1) * ((stages + splits - 1) / splits) >= stages) --splits;
     cb_launch_cluster(kernel, dim3((p.N + S::FEATURES - 1) / S::FEATURES, (p.M + S::ROWS - 1) / S::ROWS, splits),
-                      dim3(S::WARPS * 32 + 32), SMEM, stream, splits, mr, mw, p, run_magic, splits, status);
+                      dim3(S::WARPS * 32 + 32), SMEM, stream, splits, mr, mw, p, run_magic, parts, splits, status);
     return cb_last_error();
 }
 
 template <int NT>
-int launch_as(const QuantizedArgs& p, int groups, int share, int splits, uint32_t run_magic, int* status, cudaStream_t stream) {
-    if (groups == 1 && share == 8) return launch<NT, 1, 8>(p, run_magic, splits, status, stream);
-    if (groups == 1 && share == 4) return launch<NT, 1, 4>(p, run_magic, splits, status, stream);
-    if (groups == 2 && share == 4) return launch<NT, 2, 4>(p, run_magic, splits, status, stream);
-    if (groups == 2 && share == 2) return launch<NT, 2, 2>(p, run_magic, splits, status, stream);
+int launch_as(const QuantizedArgs& p, int groups, int share, int splits, uint32_t run_magic, int parts, int* status, cudaStream_t stream) {
+    if (groups == 1 && share == 8) return launch<NT, 1, 8>(p, run_magic, parts, splits, status, stream);
+    if (groups == 1 && share == 4) return launch<NT, 1, 4>(p, run_magic, parts, splits, status, stream);
+    if (groups == 2 && share == 4) return launch<NT, 2, 4>(p, run_magic, parts, splits, status, stream);
+    if (groups == 2 && share == 2) return launch<NT, 2, 2>(p, run_magic, parts, splits, status, stream);
     return CB_ERR_UNSUPPORTED;
 }
 
 }  // namespace
 
 // `groups` of `share` warps a block, of 32 features a group: 1 x 8, 2 x 4, 1 x 4 or 2 x 2; `splits`:
-// shares of K, 1 to 8 (as many as leave none empty).  K a multiple of 256; rows bf16.
+// shares of K, 1 to 8 (as many as leave none empty).  K a multiple of 256;
+// rows bf16, or up to five of fp32 and `parts`, bf16 [3, M, K], where they are split to.
 CB_EXPORT int cb_linear_quantized_ring(int kind, const void* rows, long long ldr, const float* row_scale, const void* w,
                                        long long ldw, const void* group_scale, const float* feature_scale,
                                        const float* add, long long lda, void* out, int out_dtype, long long ldo, int M,
-                                       int N, int K, int group, int groups, int share, int splits, int* status, void* stream) {
+                                       int N, int K, int group, int groups, int share, int splits, void* parts,
+                                       int* status, void* stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (kind != FOUR_BF16 || K <= 0 || K % 256 || K > MOST_K || (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * 2) | (uintptr_t)ldw) & 15) ||
-        (M + 7) / 8 > 65535 || group <= 0 || group % 32 || K % group || splits < 1 || splits > 8)
+    const int size = kind == FOUR_F32 ? 4 : 2;
+    if ((kind != FOUR_BF16 && kind != FOUR_F32) || K <= 0 || K % 256 || K > MOST_K ||
+        (((uintptr_t)rows | (uintptr_t)w | (uintptr_t)(ldr * size) | (uintptr_t)ldw) & 15) || (M + 7) / 8 > 65535 ||
+        (kind == FOUR_F32 && (M > 5 || parts == nullptr || ((uintptr_t)parts & 15))) || group <= 0 || group % 32 || K % group || splits < 1 || splits > 8)
         return CB_ERR_UNSUPPORTED;
-    const QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
+    QuantizedArgs p = {rows, ldr, row_scale, w, ldw, (const uint8_t*)group_scale, feature_scale, add, lda, out, ldo,
                              M, N, K, group, out_dtype == CB_BF16, K / group};
     const uint32_t runs = (uint32_t)group / 32;
     const uint32_t run_magic = (uint32_t)(((1ull << 31) + runs - 1) / runs);
     cudaStream_t s = (cudaStream_t)stream;
-    return M <= 8 ? launch_as<1>(p, groups, share, splits, run_magic, status, s) : launch_as<2>(p, groups, share, splits, run_magic, status, s);
+    int n_parts = 1;
+    if (kind == FOUR_F32) {
+        split_rows((const float*)rows, ldr, (__nv_bfloat16*)parts, M, K, s);
+        p.rows = parts, p.ldr = K, n_parts = 3;
+    }
+    return M * n_parts <= 8 ? launch_as<1>(p, groups, share, splits, run_magic, n_parts, status, s)
+                            : launch_as<2>(p, groups, share, splits, run_magic, n_parts, status, s);
 }

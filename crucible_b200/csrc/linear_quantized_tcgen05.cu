@@ -426,24 +426,6 @@ linear_tcgen05_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid
     }
 }
 
-// fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ rows, long long ldr,
-                                                         __nv_bfloat16* __restrict__ parts, int M, int K) {
-    cb_pdl_wait();
-    cb_pdl_trigger();
-    const long long total = (long long)M * (K / 4);
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const long long m = i / (K / 4), k = i % (K / 4) * 4;
-        const float4 v = __ldg(reinterpret_cast<const float4*>(rows + m * ldr + k));
-        uint32_t a[3], b[3];
-        three_parts(v.x, v.y, a);
-        three_parts(v.z, v.w, b);
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-            *reinterpret_cast<uint2*>(parts + ((long long)j * M + m) * K + k) = make_uint2(a[j], b[j]);
-    }
-}
-
 template <int KIND, int TOK, bool BF16>
 int launch(const QuantizedArgs& p, const CUtensorMap& rows, const CUtensorMap& w, int tok, int splits, int* status,
            cudaStream_t stream) {
@@ -507,9 +489,7 @@ CB_EXPORT int cb_linear_quantized_tcgen05(int kind, const void* rows, long long 
     else ok = ok && quantized_map(&mr, rows, kind == FOUR_BF16, (uint64_t)M, (uint64_t)K, (uint64_t)ldr * size, tok, 1);
     if (!ok) return CB_ERR_UNSUPPORTED;
     if (kind == FOUR_F32) {
-        const long long quads = (long long)M * (K / 4);
-        const int blocks = (int)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8);
-        cb_launch(split_rows_kernel, dim3(blocks), dim3(256), 0, st, (const float*)rows, ldr, (__nv_bfloat16*)parts, M, K);
+        split_rows((const float*)rows, ldr, (__nv_bfloat16*)parts, M, K, st);
         return launch_out<FOUR_F32>(p, mr, mw, tok, splits, status, st);
     }
     if (kind == FOUR_BF16) return launch_out<FOUR_BF16>(p, mr, mw, tok, splits, status, st);

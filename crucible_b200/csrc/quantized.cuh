@@ -85,6 +85,30 @@ __device__ __forceinline__ void three_parts(float x, float y, uint32_t (&p)[3]) 
     for (int j = 0; j < 3; ++j) p[j] = part[0][j] | (part[1][j] << 16);
 }
 
+// fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.
+static __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ rows, long long ldr,
+                                                         __nv_bfloat16* __restrict__ parts, int M, int K) {
+    cb_pdl_wait();
+    cb_pdl_trigger();
+    const long long total = (long long)M * (K / 4);
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long m = i / (K / 4), k = i % (K / 4) * 4;
+        const float4 v = __ldg(reinterpret_cast<const float4*>(rows + m * ldr + k));
+        uint32_t a[3], b[3];
+        three_parts(v.x, v.y, a);
+        three_parts(v.z, v.w, b);
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            *reinterpret_cast<uint2*>(parts + ((long long)j * M + m) * K + k) = make_uint2(a[j], b[j]);
+    }
+}
+
+static inline void split_rows(const float* rows, long long ldr, __nv_bfloat16* parts, int M, int K, cudaStream_t stream) {
+    const long long quads = (long long)M * (K / 4);
+    const int blocks = (int)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8);
+    cb_launch(split_rows_kernel, dim3(blocks), dim3(256), 0, stream, rows, ldr, parts, M, K);
+}
+
 // A sum's way out: its scales, the addition, the rounding.
 __device__ __forceinline__ void finish(const QuantizedArgs& p, float v, float row_scale, float feature_scale, int m, int n) {
     v *= feature_scale;

@@ -338,7 +338,7 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #
 #   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
-#   "ring"   the same arithmetic behind a ring of stages: 4-bit weights and bfloat16 rows, K a multiple of 256.  8 rows of
+#   "ring"   the same arithmetic behind a ring of stages: 4-bit weights, K a multiple of 256, bfloat16 rows.  8 rows of
 #            4,096 by 4,096, ring / few / tiles: 5.3 / 7.5 / 9.5; 16 rows by 14,336 14.9 / 22.0 / 18.4; 32 rows by 2,048 (K of
 #            8,192) 11.1 / 14.5 / 12.9, by 6,144 (K of 4,096) 14.4 / 18.3 / 12.8.  A block is so many groups of warps by
 #            warps that share a group's K: 1 x 8 while the SMs have two blocks or fewer at once, 1 x 4 beyond (8 rows by
@@ -347,6 +347,8 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #            16 rows, whose stages are larger (by 14,336, 1 x 4 / 2 x 4: 16.9 / 14.9).  Few features and a long K: blocks of
 #            a cluster share K (8 rows by 2,048, K of 14,336, one share / four: 12.6 / 8.6; K of 8,192 8.3 / 6.1; by
 #            4,096, K of 4,096, one / two: 5.3 / 5.9).
+#            Up to five float32 rows are up to 15 bfloat16 ones here (1 and 5 rows by 28,672, ring / tiles: 21.4 / 40.9 and
+#            29.8 / 41.2; by 2,048, K of 8,192, 7.5 / 13.8 and 9.1 / 14.2; of 768 by 1,280, ring / few: 3.6 / 3.7 and 3.9 / 3.8).
 #   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K.
 #   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
 #
@@ -355,6 +357,7 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 # allows), what a cluster costs, and how many blocks follow one another on an SM.  us, in `_COSTS`.
 FORM = None                      # tests name one of the forms, "few", "ring", "tiles" or "pairs", to reach it at any size
 N_SMS = 148
+_RING_F32_ROWS = 5               # (three bfloat16 rows each, and the ring takes 16)
 _SMALL, _SMALL_8_ROWS = 1_200_000, 4_200_000           # weights of a matrix that "few" ends first: up to 64 rows, up to 8
 
 
@@ -419,7 +422,7 @@ def _even(m: int, most: int) -> int:
 
 
 def _ring(m: int, n: int, k: int):
-    """Groups of warps a block, warps a group, blocks that share K."""
+    """Groups of warps a block, warps a group, blocks that share K, for m bfloat16 rows."""
     if n >= (9472 if k <= 1024 else 12000):
         if n >= (16 if m <= 8 else 24) * k:
             return 2, 2, 1
@@ -439,14 +442,16 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
         small = n * k <= _SMALL and m <= 64
         if kind == _FOUR_BF16:
             form = "ring" if m <= 16 or (m <= 32 and n <= 2048) else "few" if small else None
+        elif kind == _FOUR_F32 and m <= _RING_F32_ROWS and k % 256 == 0:
+            form = "ring"
         elif small or (n * k <= _SMALL_8_ROWS and m <= 8):
             form = "few"
-    if (form == "ring" and (kind != _FOUR_BF16 or k % 256)):
+    if form == "ring" and (kind == _EIGHT or k % 256 or (kind == _FOUR_F32 and m > _RING_F32_ROWS)):
         form = "few"
     if form == "few":
         return ("few",)
     if form == "ring":
-        return ("ring",) + _ring(m, n, k)
+        return ("ring",) + _ring(3 * m if kind == _FOUR_F32 else m, n, k)
     units = -(-k // (128 if kind == _EIGHT else 256))
     best = None
     if form != "pairs" or kind == _FOUR_F32:
@@ -499,17 +504,19 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
         code = _at(dev, build.load("linear_quantized_few").cb_linear_quantized_few, *common)
     else:
         status = _status(dev)
+        parts = None
+        if kind == _FOUR_F32:
+            parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device)
         if form[0] == "ring":
-            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, *form[1:], status)
+            code = _at(dev, build.load("linear_quantized_ring").cb_linear_quantized_ring, *common, *form[1:], _ptr(parts), status)
         elif form[0] == "pairs":
             code = _at(dev, build.load("linear_quantized_pairs_tcgen05").cb_linear_quantized_pairs, *common, form[1],
                        form[2], status)
         else:
-            parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device) if kind == _FOUR_F32 else None
             code = _at(dev, build.load("linear_quantized_tcgen05").cb_linear_quantized_tcgen05, *common, form[1], form[2],
                        _ptr(parts), status)
-            if kind == _FOUR_F32 and code == 0:
-                LAUNCHES[0] += 1                       # (the rows' parts)
+        if kind == _FOUR_F32 and code == 0:
+            LAUNCHES[0] += 1                           # (the rows' parts)
     if code == build.UNSUPPORTED:
         raise KernelError(f"{what}: sizes out of range: rows [{m}, {k}], weights [{n}, {k}]")
     _check(code, what)

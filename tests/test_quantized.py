@@ -118,13 +118,15 @@ def test_calls_that_are_refused():
 def test_the_rule_names_a_form_that_takes_the_product():
     for kind in (quantized._EIGHT, quantized._FOUR_BF16, quantized._FOUR_F32):
         for forced in (None, "few", "ring", "tiles", "pairs"):
-            for m in (1, 8, 9, 16, 17, 33, 64, 65, 100, 129, 256, 257, 1000, 2049, 30000, 1 << 20):
-                for n, k in ((1, 32), (127, 256), (129, 96), (768, 2048), (4096, 14336), (28672, 4096), (300000, 64)):
+            for m in (1, 5, 6, 8, 9, 16, 17, 33, 64, 65, 100, 129, 256, 257, 1000, 2049, 30000, 1 << 20):
+                for n, k in ((1, 32), (127, 256), (129, 96), (768, 2048), (4096, 14336), (28672, 4096), (300000, 64),
+                             (512, 8192), (60000, 1024)):
                     form, *how = quantized._rule(forced, kind, m, n, k)
                     if form == "few":
                         assert forced in (None, "few", "ring")
                     elif form == "ring":
-                        assert kind == quantized._FOUR_BF16 and k % 256 == 0 and how[0] in (1, 2, 4)
+                        assert k % 256 == 0 and tuple(how[:2]) in ((1, 8), (1, 4), (2, 4), (2, 2)) and how[2] in (1, 2, 4, 8)
+                        assert kind == quantized._FOUR_BF16 or (kind == quantized._FOUR_F32 and m <= 5)
                     else:
                         rows, more = how
                         assert rows % 16 == 0 and 16 <= rows <= (64 if kind == quantized._FOUR_F32 else 256)

@@ -200,6 +200,23 @@ def test_linear4_by_rings_that_share_k(block, shares, monkeypatch):
     for rows, n, k, group in ((1, 33, 256, 32), (8, 100, 2304, 64), (9, 64, 4096, 4096), (20, 129, 1280, 160), (3, 31, 8448, 96)):
         _check4(rows, n, k, group, torch.bfloat16, torch.float32, True)
         _check4(rows, n, k, group, torch.bfloat16, torch.bfloat16, False)
+    for rows, n, k, group in ((1, 33, 256, 32), (2, 100, 2304, 64), (3, 64, 4096, 4096), (5, 129, 1280, 160)):
+        _check4(rows, n, k, group, torch.float32, torch.float32, True)
+        _check4(rows, n, k, group, torch.float32, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 6])
+def test_few_float32_rows(rows):
+    """Those that the ring takes as three rows each, and one more."""
+    for n, k, group in ((1000, 768, 64), (2048, 8192, 128), (300, 4096, 32), (12000, 256, 256)):
+        _check4(rows, n, k, group, torch.float32, torch.float32, rows % 2 == 0)
+
+
+def test_six_float32_rows_are_too_many_for_the_ring(monkeypatch):
+    monkeypatch.setattr(quantized, "_rule", lambda *sizes: ("ring", 1, 8, 1))
+    gen = _gen()
+    with pytest.raises(KernelError, match="sizes out of range"):
+        quantized.linear4(_randn(gen, 6, 256), random_weights4(32, 256, 32, DEV, gen), torch.empty(6, 32, device=DEV))
 
 
 @pytest.mark.parametrize("rows,n,k,group", [(1, 2048, 8192, 64), (8, 500, 14336, 128), (16, 1280, 4096, 64), (20, 512, 8192, 32)])
