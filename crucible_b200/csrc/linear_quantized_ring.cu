@@ -109,38 +109,35 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
         const uint8_t* const scales = p.group_scale + (long long)n0 * p.groups;
-        const uint32_t runs = (uint32_t)p.group >> 5;
-        const bool regular = runs <= 2 || runs % 4 == 0;              // a segment's four runs begin a scale, or lie in one
         uint32_t s_off[PAIRS][2];
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int f = min(n0 + 32 * group + 16 * i + 8 * h + mine, p.N - 1) - n0;
-                s_off[i][h] = (uint32_t)f * (uint32_t)p.groups + (regular ? (runs == 1 ? t : (runs == 2 ? t >> 1 : 0)) : 0);
-            }
-        const uint32_t s_add = regular ? 0 : 2 * t;
-        auto ask = [&](uint32_t (&scale)[PAIRS], int seg) {
+            for (int h = 0; h < 2; ++h)
+                s_off[i][h] = (uint32_t)(min(n0 + 32 * group + 16 * i + 8 * h + mine, p.N - 1) - n0) * (uint32_t)p.groups;
+        // The scales of a segment's codes, asked for a stage ahead.  (The bytes stay apart until they are needed: put together
+        // here they would be waited for here, which took 6% of the time.)
+        auto ask = [&](uint32_t (&scale)[PAIRS][2], int seg) {
             if (seg >= segments) return;
-            // the scale of the first run of 32 k (or of the thread's): 2 (k / 32) over the runs that share one, by half
-            // their reciprocal
-            const uint32_t at = __umulhi((uint32_t)(8 * seg) + s_add, run_magic);
+            // the scale of a run of 32 k: 2 (k / 32) over the runs that share one, by half their reciprocal
+            const uint32_t at = __umulhi((uint32_t)(8 * seg + 2 * t), run_magic);
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i)
-                scale[i] = (uint32_t)__ldg(scales + (s_off[i][0] + at)) + 256u * (uint32_t)__ldg(scales + (s_off[i][1] + at));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) scale[i][h] = __ldg(scales + (s_off[i][h] + at));
         };
         // where the thread's codes and rows lie in a stage
         const int codes_at = (turn >> 1) * (S::FEATURES * 128) + (32 * group + mine) * 128 + ((((turn & 1) * 4 + t) ^ mine) << 4);
         const int rows_at = (turn * 2 + (t >> 1)) * (S::ROWS * 128) + g * 128;
         const int piece0 = (t & 1) * 4;
-        uint32_t scale[PAIRS], next[PAIRS];
+        uint32_t scale[PAIRS][2], next[PAIRS][2];
         ask(next, begin * SHARE + turn);
         int st = 0;
         uint32_t parity = 0;
 #pragma unroll 1
         for (int i = begin; i < end; ++i) {
 #pragma unroll
-            for (int q = 0; q < PAIRS; ++q) scale[q] = next[q];
+            for (int q = 0; q < PAIRS; ++q) scale[q][0] = next[q][0], scale[q][1] = next[q][1];
             const int seg = i * SHARE + turn;
             ask(next, seg + SHARE);
             ok = tc::mbar_wait(&s.full[st], parity, abort_flag);
@@ -158,7 +155,7 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
                 for (int q = 0; q < PAIRS; ++q) {
                     x[q] = *reinterpret_cast<const uint4*>(codes + q * 2048);
                     y[q] = *reinterpret_cast<const uint4*>(codes + q * 2048 + 1024);
-                    scale_pairs(scale[q], both[q]);
+                    scale_pairs(__byte_perm(scale[q][0], scale[q][1], 0x0040), both[q]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {               // eight k at a time

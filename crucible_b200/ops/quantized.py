@@ -339,16 +339,16 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
 #   "ring"   the same arithmetic behind a ring of stages: 4-bit weights, K a multiple of 256, bfloat16 rows.  8 rows of
-#            4,096 by 4,096, ring / few / tiles: 5.3 / 7.5 / 9.5; 16 rows by 14,336 14.9 / 22.0 / 18.4; 32 rows by 2,048 (K of
-#            8,192) 11.1 / 14.5 / 12.9, by 6,144 (K of 4,096) 14.4 / 18.3 / 12.8.  A block is so many groups of warps by
+#            4,096 by 4,096, ring / few / tiles: 4.8 / 7.0 / 8.1; 16 rows by 14,336 14.6 / 20.6 / 16.5; 32 rows by 2,048 (K of
+#            8,192) 9.7 / 12.7 / 11.2, by 6,144 (K of 4,096) 13.0 / 19.8 / 11.5.  A block is so many groups of warps by
 #            warps that share a group's K: 1 x 8 while the SMs have two blocks or fewer at once, 1 x 4 beyond (8 rows by
-#            28,672, 1 x 8 / 1 x 4 / 2 x 4: 23.4 / 20.2 / 23.0; by 4,096 5.3 / 6.0 / 7.6), 2 x 2 where K is short beside
-#            the features and the rows are best read less often (by 50,304, K of 768, 1 x 4 / 2 x 2: 9.7 / 8.8), 2 x 4 for
-#            16 rows, whose stages are larger (by 14,336, 1 x 4 / 2 x 4: 16.9 / 14.9).  Few features and a long K: blocks of
-#            a cluster share K (8 rows by 2,048, K of 14,336, one share / four: 12.6 / 8.6; K of 8,192 8.3 / 6.1; by
-#            4,096, K of 4,096, one / two: 5.3 / 5.9).
-#            Up to five float32 rows are up to 15 bfloat16 ones here (1 and 5 rows by 28,672, ring / tiles: 21.4 / 40.9 and
-#            29.8 / 41.2; by 2,048, K of 8,192, 7.5 / 13.8 and 9.1 / 14.2; of 768 by 1,280, ring / few: 3.6 / 3.7 and 3.9 / 3.8).
+#            28,672, 1 x 8 / 1 x 4 / 2 x 4: 22.5 / 19.8 / 22.7; by 4,096 4.8 / 5.4 / 7.1), 2 x 2 where K is short beside
+#            the features and the rows are best read less often (by 50,304, K of 768, 1 x 4 / 2 x 2: 9.5 / 8.4), 2 x 4 for
+#            16 rows, whose stages are larger (by 14,336, 1 x 4 / 2 x 4: 15.4 / 14.6).  Few features and a long K: blocks of
+#            a cluster share K (8 rows by 2,048, K of 14,336, one share / four: 10.9 / 8.0; K of 8,192 7.2 / 5.5; by
+#            4,096, K of 4,096, one / two: 4.8 / 5.4).
+#            Up to five float32 rows are up to 15 bfloat16 ones here (1 and 5 rows by 28,672, ring / tiles: 20.7 / 40.8 and
+#            29.5 / 41.2; by 2,048, K of 8,192, 7.0 / 13.8 and 8.6 / 14.1; of 768 by 1,280, ring / few: 3.7 / 3.4 and 4.0 / 3.6).
 #   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K.
 #   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
 #
@@ -441,8 +441,9 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
     if form is None:
         small = n * k <= _SMALL and m <= 64
         if kind == _FOUR_BF16:
-            form = "ring" if m <= 16 or (m <= 32 and n <= 2048) else "few" if small else None
-        elif kind == _FOUR_F32 and m <= _RING_F32_ROWS and k % 256 == 0:
+            narrow = (n <= 2048 and (n >= 1536 or k <= 4096)) or (n <= 4096 and k <= 2048)
+            form = "ring" if m <= 16 or (m <= 32 and narrow) else "few" if small else None
+        elif kind == _FOUR_F32 and m <= _RING_F32_ROWS and k % 256 == 0 and not (small and k <= 1024):
             form = "ring"
         elif small or (n * k <= _SMALL_8_ROWS and m <= 8):
             form = "few"
