@@ -12,8 +12,9 @@
 // blocks' sums are added in their order, so the order of a dot product's sum depends on the sizes alone.  A thread takes
 // 16 neighbouring bytes of a feature's codes, 32 k, and the same k of its row.
 //
-// What it takes is instructions (issue slots 59%, the units of shifts and of bf16 arithmetic about half of the time):
-// more warps an SM, fewer waits, group scales through shared memory and blocks that stay and share the features evenly changed nothing.
+// What it takes is instructions (8 rows of 4,096 by 128,256, 69 us: issue slots 58%, the unit of shifts and masks 53%,
+// memory 45%): more warps an SM, fewer waits, group scales through shared memory and blocks that stay and share the
+// features evenly changed nothing.
 #define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 #include "tc_common.cuh"
@@ -116,7 +117,7 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
             for (int h = 0; h < 2; ++h)
                 s_off[i][h] = (uint32_t)(min(n0 + 32 * group + 16 * i + 8 * h + mine, p.N - 1) - n0) * (uint32_t)p.groups;
         // The scales of a segment's codes, asked for a stage ahead.  (The bytes stay apart until they are needed: put together
-        // here they would be waited for here, which took 6% of the time.)
+        // here they would be waited for here, which took 2 to 8% of the time.)
         auto ask = [&](uint32_t (&scale)[PAIRS][2], int seg) {
             if (seg >= segments) return;
             // the scale of a run of 32 k: 2 (k / 32) over the runs that share one, by half their reciprocal
