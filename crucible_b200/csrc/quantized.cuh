@@ -86,7 +86,7 @@ __device__ __forceinline__ void three_parts(float x, float y, uint32_t (&p)[3]) 
 }
 
 // fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.
-static __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ rows, long long ldr,
+template <int THREADS> __global__ void __launch_bounds__(THREADS) split_rows_kernel(const float* __restrict__ rows, long long ldr,
                                                          __nv_bfloat16* __restrict__ parts, int M, int K) {
     cb_pdl_wait();
     cb_pdl_trigger();
@@ -103,10 +103,10 @@ static __global__ void __launch_bounds__(256) split_rows_kernel(const float* __r
     }
 }
 
-static inline void split_rows(const float* rows, long long ldr, __nv_bfloat16* parts, int M, int K, cudaStream_t stream) {
+template <int THREADS = 256> void split_rows(const float* rows, long long ldr, __nv_bfloat16* parts, int M, int K, cudaStream_t stream) {
     const long long quads = (long long)M * (K / 4);
-    const int blocks = (int)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8);
-    cb_launch(split_rows_kernel, dim3(blocks), dim3(256), 0, stream, rows, ldr, parts, M, K);
+    const int blocks = (int)(quads / THREADS + 1 < 148 * 8 ? quads / THREADS + 1 : 148 * 8);
+    cb_launch(split_rows_kernel<THREADS>, dim3(blocks), dim3(THREADS), 0, stream, rows, ldr, parts, M, K);
 }
 
 // A sum's way out: its scales, the addition, the rounding.

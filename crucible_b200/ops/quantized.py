@@ -25,7 +25,7 @@ import torch
 
 from . import LAUNCHES, KernelError, _check, _need_cuda, _ptr, _stream, build, tensor_core
 
-build.register_module("rows8", ["common.cuh"])
+build.register_module("rows8", ["common.cuh", "quantized.cuh", "tc_common.cuh"])
 build.register_module("linear_quantized_few", ["common.cuh", "quantized.cuh"])
 build.register_module("linear_quantized_ring", ["common.cuh", "quantized.cuh", "tc_common.cuh"])
 for _name in ("linear_quantized_tcgen05", "linear_quantized_pairs_tcgen05"):
@@ -160,7 +160,8 @@ def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Opt
         _look_over_glu8(both, out, scales, limit)
     lib = build.load("rows8")
     code = _at(dev, lib.cb_glu8, both.data_ptr(), 0 if both.dtype is _F32 else 1, bs[0], out.data_ptr(), os[0],
-               scales.data_ptr(), shape[0], shape[1], limit if limit is not None else 0.0, alpha, offset)
+               scales.data_ptr(), shape[0], shape[1], limit if limit is not None else 0.0, alpha, offset,
+               _status(dev) if shape[0] >= 1024 else 0)
     if code == build.UNSUPPORTED:
         raise KernelError(f"glu8 takes 1 to {lib.cb_rows8_widest()} features, got {shape[1]}")
     _check(code, "glu8")

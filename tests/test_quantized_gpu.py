@@ -76,6 +76,26 @@ def test_glu8(width, dtype, pair):
         _frame_kept(q, frame, left, 3.0)
 
 
+@pytest.mark.parametrize("dtype,width", [("bf16", 8192), ("bf16", 8200), ("bf16", 14336), ("bf16", 14344), ("bf16", 28800), ("bf16", 28808),
+                                         ("bf16", 9001), ("f32", 4100), ("f32", 7168), ("f32", 7172), ("f32", 14400), ("f32", 14404)])
+@pytest.mark.parametrize("rows", [1023, 1024, 1337])
+def test_glu8_of_many_long_rows(dtype, width, rows):
+    """Around the sizes from which rows come through shared memory, by blocks of either size, to which they do."""
+    gen = _gen(width + rows)
+    wide = (2 * _randn(gen, rows, 2 * width + 8)).to(DTYPES[dtype])
+    both = wide[:, :2 * width]
+    both[rows - 1, 5], both[7, width + 1] = float("nan"), float("inf")
+    both[8] = 0.0
+    for limit, alpha, offset in ((None, 1.0, 0.0), (2.0, 1.25, 0.75)):
+        out, scales = quantized.new_rows8(rows, width, DEV), torch.full((rows + 1,), -1.0, device=DEV)
+        quantized.glu8(both, out, scales[:rows], limit, alpha, offset)
+        y = exact_glu(both, limit, alpha, offset)
+        fine = torch.isfinite(y).all(dim=1)
+        assert int(fine.sum()) == (rows - 2 if limit is None else rows - 1) and scales[rows] == -1.0
+        check_rows8(out[fine], scales[:rows][fine], y[fine], f"{dtype} {rows} x {width} {limit}")
+        assert not torch.isfinite(scales[:rows][~fine]).any()
+
+
 @pytest.mark.parametrize("width", [5, 64, 768, 4096, 20000])
 def test_rows8_of_zeros_and_of_what_is_no_number(width):
     nan, inf = float("nan"), float("inf")
