@@ -350,7 +350,9 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #            4,096, K of 4,096, one / two: 4.8 / 5.4).
 #            Up to five float32 rows are up to 15 bfloat16 ones here (1 and 5 rows by 28,672, ring / tiles: 20.7 / 40.8 and
 #            29.5 / 41.2; by 2,048, K of 8,192, 7.0 / 13.8 and 8.6 / 14.1; of 768 by 1,280, ring / few: 3.7 / 3.4 and 4.0 / 3.6).
-#   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K.
+#   "tiles"  tcgen05, a block a tile of 128 features by up to 256 rows, up to 8 blocks sharing K (33 float32 rows by 2,048, K of
+#            8,192, shared by 4 / 6 / 8: 15.7 / 13.9 / 19.9; a cluster of eight that fill their SMs needs eight free ones
+#            side by side).
 #   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
 #
 # Between the last two, and for the rows a tile and the shares of K, a model of what a launch takes decides: a block's
@@ -392,7 +394,9 @@ def _up(x: int, to: int) -> int:
 
 def _tiles_us(kind: int, m: int, n: int, k: int, tok: int, shares: int) -> float:
     c, parts = _COSTS[kind], 3 if kind == _FOUR_F32 else 1
-    steps = -(-k // (128 if kind == _EIGHT else 64)) / shares
+    unit = 128 if kind == _EIGHT else 256              # K is shared in such units, of one step or four
+    units = -(-k // unit)
+    steps = -(-units // shares) * (1 if kind == _EIGHT else 4)
     per_sm = _blocks_an_sm(kind, tok)
     fixed = c.block + c.block_row * tok
     if shares > 1:
@@ -462,7 +466,7 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
             if -(-m // tok) > 65535:
                 continue
             tiles, per_sm = -(-n // 128) * -(-m // tok), _blocks_an_sm(kind, tok)
-            for shares in (1, 2, 4, 8) if per_sm == 2 else (1, 2, 4):
+            for shares in (1, 2, 4, 6, 8) if per_sm == 2 else (1, 2, 4, 6):
                 if shares == 1 or (shares <= units and tiles * shares <= 320):
                     us = _tiles_us(kind, m, n, k, tok, shares)
                     if best is None or us < best[0]:

@@ -131,7 +131,7 @@ def test_the_rule_names_a_form_that_takes_the_product():
                         rows, more = how
                         assert rows % 16 == 0 and 16 <= rows <= (64 if kind == quantized._FOUR_F32 else 256)
                         if form == "tiles":
-                            assert more in (1, 2, 4, 8) and more <= -(-k // (128 if kind == quantized._EIGHT else 256))
+                            assert more in (1, 2, 4, 6, 8) and more <= -(-k // (128 if kind == quantized._EIGHT else 256))
                             assert -(-m // rows) <= 65535
                         else:
                             assert form == "pairs" and kind != quantized._FOUR_F32 and more == 74
