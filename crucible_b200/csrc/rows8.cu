@@ -435,7 +435,10 @@ void launch_glu8_as(const Shape& s, const T* both, long long ldb, uint8_t* q, lo
 // Shared memory of a block of the ring, and its rows: two blocks of 512 threads an SM, or one of 1,024.
 constexpr int ring_room(int threads) { return (threads == 512 ? 112 : 225) * 1024; }
 
-inline int ring_threads(int rows, int width, int size) {
+// Threads of a block of the ring, or 0: a block a row.  (The ring waits for its copies, and a wait that runs out has to be told:
+// without a place for that, null, a block a row, which waits for nothing.)
+inline int ring_threads(int rows, int width, int size, const int* status) {
+    if (status == nullptr) return 0;
     const int bytes = 2 * width * size;
     if (bytes <= RING_BYTES || 2 * bytes > ring_room(1024)) return 0;
     const int threads = 2 * bytes <= ring_room(512) ? 512 : 1024;
@@ -502,6 +505,15 @@ CB_EXPORT int cb_norm8(const float* x, long long ldx, const void* delta, int del
     return cb_last_error();
 }
 
+// The fewest rows that are brought by copies which a kernel waits for, whatever their width.
+CB_EXPORT int cb_glu8_waits_from() { return MANY_ROWS < RING_MANY ? MANY_ROWS : RING_MANY; }
+
+// Whether so many pairs of rows that begin on 16 bytes are brought by such copies, with a place to tell of waits that run out
+// (`status`) or without.
+CB_EXPORT int cb_glu8_waits(int dtype, int rows, int width, const int* status) {
+    return ring_threads(rows, width, dtype == CB_BF16 ? 2 : 4, status) != 0;
+}
+
 // limit <= 0: silu(g) * u; else the capped pair.  `status` (may be null): where a wait for memory that runs out is told.
 CB_EXPORT int cb_glu8(const void* both, int dtype, long long ldb, void* q, long long ldq, float* scales, int rows,
                       int width, float limit, float alpha, float offset, int* status, void* stream) {
@@ -511,7 +523,7 @@ CB_EXPORT int cb_glu8(const void* both, int dtype, long long ldb, void* q, long 
     const Shape s = shape_of(rows, width, e, 1024, 160, 1024);
     const bool vec = width % e == 0 && ldb % e == 0 && ldq % e == 0 && aligned(both, 16) && aligned(q, e);
     cudaStream_t st = (cudaStream_t)stream;
-    const int ring = vec ? ring_threads(rows, width, 16 / e) : 0;
+    const int ring = vec ? ring_threads(rows, width, 16 / e, status) : 0;
     if (ring != 0)
         return dtype == CB_BF16 ? launch_glu8_ring(ring, (const __nv_bfloat16*)both, ldb, (uint8_t*)q, ldq, scales, rows, width, limit, alpha, offset, status, st)
                                 : launch_glu8_ring(ring, (const float*)both, ldb, (uint8_t*)q, ldq, scales, rows, width, limit, alpha, offset, status, st);

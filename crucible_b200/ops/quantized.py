@@ -14,7 +14,8 @@ kernel runs, and with it the order of a sum, goes by the sizes, the number of ro
 Everything here launches on torch's current stream of the tensors' device, keeps no buffer between
 calls and may be captured into a CUDA graph (a call that has to bring rows into another layout first
 allocates from torch's pool, as any captured torch operation does).  Outputs may not overlap inputs, but where
-a function says so.  The waits inside the products are bounded; `tensor_core.check_status` raises if one ran out.
+a function says so.  The waits inside the products, and inside `glu8` of many long rows, are bounded;
+`tensor_core.check_status` raises if one ran out.
 """
 from __future__ import annotations
 
@@ -40,6 +41,7 @@ _FLOATS = (torch.float32, torch.bfloat16)
 _MOST_ROWS = (1 << 31) - 1024    # the kernels count rows and features in 32 bits
 _SLAB = 1 << 16                  # float32 rows over 4-bit weights at a time: three bfloat16 copies of them are needed
 _LEAST_LIMIT = 2.0 ** -126       # (a smaller limit could be zero in float32)
+_WAITS_FROM = 296                # rows of `glu8` from which its kernel may wait for copies (`cb_glu8_waits_from`)
 
 
 # Every function asks first whether all is as it usually is, in one expression over plain attributes; only where it is
@@ -161,7 +163,7 @@ def glu8(both: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, limit: Opt
     lib = build.load("rows8")
     code = _at(dev, lib.cb_glu8, both.data_ptr(), 0 if both.dtype is _F32 else 1, bs[0], out.data_ptr(), os[0],
                scales.data_ptr(), shape[0], shape[1], limit if limit is not None else 0.0, alpha, offset,
-               _status(dev) if shape[0] >= 1024 else 0)
+               _status(dev) if shape[0] >= _WAITS_FROM else 0)
     if code == build.UNSUPPORTED:
         raise KernelError(f"glu8 takes 1 to {lib.cb_rows8_widest()} features, got {shape[1]}")
     _check(code, "glu8")

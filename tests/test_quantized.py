@@ -175,3 +175,36 @@ def test_a_limit_that_float32_may_have_as_zero_is_refused():
     for limit in (1e-50, 2.0 ** -127, -1.0):
         _refused("limit", quantized.glu8, both, q, s, limit)
     _refused("CUDA device", quantized.glu8, both, q, s, 2.0 ** -126)
+
+
+def test_a_wait_of_glu8_that_runs_out_is_told(monkeypatch):
+    """Wherever the kernel would wait for copies it is handed a place to say that a wait ran out; where there is none
+    (nothing was called yet and a graph is being captured) it does not wait."""
+    from crucible_b200.ops import build
+    lib = build.load("rows8")
+    assert lib.cb_glu8_waits_from() == quantized._WAITS_FROM
+    told = {}
+
+    class Recorder:
+        cb_rows8_widest = lib.cb_rows8_widest
+
+        @staticmethod
+        def cb_glu8(both, dtype, ldb, q, ldq, scales, rows, width, limit, alpha, offset, status):
+            told[dtype, rows, width] = status
+            return 0
+    monkeypatch.setattr(build, "load", lambda name: Recorder)
+    monkeypatch.setattr(quantized, "_at", lambda dev, call, *args: call(*args))
+    monkeypatch.setattr(quantized, "_look_over_glu8", lambda *args: None)       # (tensors without memory, on no GPU)
+    monkeypatch.setattr(quantized, "_status", lambda dev: 1 << 20)
+    waiting = 0
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        for rows in (1, 8, 295, 296, 297, 512, 1023, 1024, 1025, 4096):
+            for width in (8, 4096, 7168, 7176, 8192, 14336, 14344, 14400, 14408, 20000, 28800, 28808, 32768):
+                both, out = torch.empty(rows, 2 * width, dtype=dtype, device="meta"), torch.empty(rows, width, dtype=E4M3, device="meta")
+                quantized.glu8(both, out, torch.empty(rows, device="meta"))
+                status = told.pop((code, rows, width))
+                assert not lib.cb_glu8_waits(code, rows, width, 0)
+                waits = lib.cb_glu8_waits(code, rows, width, 1 << 20)
+                waiting += waits
+                assert status or not waits, f"{dtype} {rows} x {width}"
+    assert waiting > 20
