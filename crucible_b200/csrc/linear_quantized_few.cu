@@ -14,6 +14,9 @@
 // A block owns 32 features and 8 or 16 rows; its warps take segments of K in turn and their sums are added
 // in the warps' order, so the order of a dot product's sum depends on K alone.  A warp asks for its next
 // segments' weights before it multiplies the present ones.
+//
+// LONG: fp32 results over 4-bit weights where a warp's share of K is above MMA_CHUNK: so many k a sum, and the sums are added
+// with rounding.
 #define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 
@@ -46,7 +49,7 @@ struct Held {
 };
 
 // NT: groups of 8 rows.  WARPS share K.
-template <int KIND, int NT, int WARPS>
+template <int KIND, int NT, int WARPS, bool LONG>
 __global__ void __launch_bounds__(WARPS * 32, (KIND == FOUR_F32 ? 8 : 16) / WARPS)
 linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
     constexpr int SEG = KIND == EIGHT ? 64 : 128;       // k of a segment: 64 bytes of a feature's weights
@@ -208,8 +211,20 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) multiply(h[b], from + b * WARPS, false);
     };
+    constexpr int SUMS = PAIRS * NT * 4;
+    float room[LONG ? SUMS : 1];
+    float* const aside = LONG ? set_aside(room) : nullptr;
+    auto end_of_chunk = [&]() {
+#pragma unroll
+        for (int q = 0; q < SUMS; ++q) {
+            float &v = acc[q / (NT * 4)][q / 4 % NT][q % 4], &r = rest[KIND == FOUR_F32 ? q / (NT * 4) : 0][q / 4 % NT][q % 4];
+            aside[q] += KIND == FOUR_F32 ? v + r : v;
+            v = r = 0.f;
+        }
+    };
     bool have = more();
     if (have) ask(x);
+    int left = MMA_CHUNK / (2 * BATCH * SEG);
 #pragma unroll 1
     while (have) {
         int from = seg;
@@ -223,7 +238,12 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
         have = more();
         if (have) ask(x);
         take(y, from);
+        if (LONG && --left == 0) {
+            left = MMA_CHUNK / (2 * BATCH * SEG);
+            end_of_chunk();
+        }
     }
+    if (LONG) end_of_chunk();
 #pragma unroll 1
     for (; seg * SEG < K; seg += WARPS) {
         fetch(x[0], seg, true);
@@ -237,6 +257,7 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
             for (int e = 0; e < 4; ++e) {
                 float v = acc[i][j][e];
                 if constexpr (KIND == FOUR_F32) v += rest[i][j][e];
+                if (LONG) v += aside[(i * NT + j) * 4 + e];
                 sums[warp][16 * i + 8 * (e >> 1) + g][8 * j + 2 * t + (e & 1)] = v;
             }
     __syncthreads();
@@ -254,8 +275,20 @@ linear_few_kernel(const QuantizedArgs p, uint32_t run_magic) {
 template <int KIND, int NT>
 void launch(const QuantizedArgs& p, uint32_t run_magic, cudaStream_t s) {
     const dim3 grid((p.N + FEATURES - 1) / FEATURES, (p.M + 8 * NT - 1) / (8 * NT));
-    if (p.K <= 6144) cb_launch(linear_few_kernel<KIND, NT, 4>, grid, dim3(128), 0, s, p, run_magic);
-    else cb_launch(linear_few_kernel<KIND, NT, 8>, grid, dim3(256), 0, s, p, run_magic);
+    constexpr int SHORT_K = 6144;
+    static_assert(SHORT_K / 4 <= MMA_CHUNK, "four warps' sums are never long");
+    if (p.K <= SHORT_K) {
+        cb_launch(linear_few_kernel<KIND, NT, 4, false>, grid, dim3(128), 0, s, p, run_magic);
+        return;
+    }
+    // (e4m3 products have 8 bits, and their sums lose nothing to speak of: 2.9e-7 of the norm for a K of 262,144)
+    if constexpr (KIND != EIGHT) {
+        if (!p.out_bf16 && p.K > 8 * MMA_CHUNK) {
+            cb_launch(linear_few_kernel<KIND, NT, 8, true>, grid, dim3(256), 0, s, p, run_magic);
+            return;
+        }
+    }
+    cb_launch(linear_few_kernel<KIND, NT, 8, false>, grid, dim3(256), 0, s, p, run_magic);
 }
 
 template <int KIND>

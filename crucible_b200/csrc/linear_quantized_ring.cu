@@ -12,6 +12,8 @@
 // blocks' sums are added in their order, so the order of a dot product's sum depends on the sizes alone.  A thread takes
 // 16 neighbouring bytes of a feature's codes, 32 k, and the same k of its row.
 //
+// LONG: fp32 results where a warp's share of K is above MMA_CHUNK: so many k a sum, and the sums are added with rounding.
+//
 // What it takes is instructions (8 rows of 4,096 by 128,256, 69 us: issue slots 58%, the unit of shifts and masks 53%,
 // memory 45%): more warps an SM, fewer waits, group scales through shared memory and blocks that stay and share the
 // features evenly changed nothing.
@@ -50,7 +52,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int c) { return c == 0 ? v.x : (c == 1 ? v.y : (c == 2 ? v.z : v.w)); }
 
-template <int NT, int GROUPS, int SHARE>
+template <int NT, int GROUPS, int SHARE, bool LONG>
 __global__ void __launch_bounds__(GROUPS * SHARE * 32 + 32, Sizes<NT, GROUPS, SHARE>::BLOCKS)
 linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_w,
                    const QuantizedArgs p, uint32_t run_magic, int parts, int splits, int* __restrict__ status) {
@@ -133,7 +135,10 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
         const int piece0 = (t & 1) * 4;
         uint32_t scale[PAIRS][2], next[PAIRS][2];
         ask(next, begin * SHARE + turn);
-        int st = 0;
+        constexpr int SUMS = PAIRS * NT * 4;
+        float room[LONG ? SUMS : 1];
+        float* const aside = LONG ? set_aside(room) : nullptr;
+        int st = 0, left = MMA_CHUNK / SEG;
         uint32_t parity = 0;
 #pragma unroll 1
         for (int i = begin; i < end; ++i) {
@@ -179,6 +184,18 @@ linear_ring_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_co
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&s.empty[st]);
             if (++st == S::STAGES) st = 0, parity ^= 1;
+            if (LONG && --left == 0) {
+                left = MMA_CHUNK / SEG;
+#pragma unroll
+                for (int q = 0; q < SUMS; ++q) {
+                    float& v = acc[q / (NT * 4)][q / 4 % NT][q % 4];
+                    aside[q] += v, v = 0.f;
+                }
+            }
+        }
+        if (LONG) {
+#pragma unroll
+            for (int q = 0; q < SUMS; ++q) acc[q / (NT * 4)][q / 4 % NT][q % 4] += aside[q];
         }
     }
     __syncthreads();
@@ -255,8 +272,8 @@ bool ring_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_by
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, int GROUPS, int SHARE>
-int launch(const QuantizedArgs& p, uint32_t run_magic, int parts, int splits, int* status, cudaStream_t stream) {
+template <int NT, int GROUPS, int SHARE, bool LONG>
+int launch_as(const QuantizedArgs& p, uint32_t run_magic, int parts, int splits, int* status, cudaStream_t stream) {
     using S = Sizes<NT, GROUPS, SHARE>;
     constexpr int SMEM = (int)sizeof(Storage<NT, GROUPS, SHARE>) + 1024;
     CUtensorMap mr, mw;
@@ -264,19 +281,26 @@ int launch(const QuantizedArgs& p, uint32_t run_magic, int parts, int splits, in
         !ring_map(&mr, p.rows, (uint64_t)p.M * parts, (uint64_t)p.K * 2, (uint64_t)p.ldr * 2, S::ROWS, SHARE * 2))
         return CB_ERR_UNSUPPORTED;
     static bool configured[64] = {};
-    auto kernel = linear_ring_kernel<NT, GROUPS, SHARE>;
+    auto kernel = linear_ring_kernel<NT, GROUPS, SHARE, LONG>;
     const int rc = allow_shared(kernel, SMEM, configured);
     if (rc != 0) return rc;
-    const int stages = (p.K + SHARE * SEG - 1) / (SHARE * SEG);
-    if (splits > stages) splits = stages;
-    while (splits > 1 && (splits - 1) * ((stages + splits - 1) / splits) >= stages) --splits;
     cb_launch_cluster(kernel, dim3((p.N + S::FEATURES - 1) / S::FEATURES, (p.M + S::ROWS - 1) / S::ROWS, splits),
                       dim3(S::WARPS * 32 + 32), SMEM, stream, splits, mr, mw, p, run_magic, parts, splits, status);
     return cb_last_error();
 }
 
+template <int NT, int GROUPS, int SHARE>
+int launch(const QuantizedArgs& p, uint32_t run_magic, int parts, int splits, int* status, cudaStream_t stream) {
+    const int stages = (p.K + SHARE * SEG - 1) / (SHARE * SEG);
+    if (splits > stages) splits = stages;
+    while (splits > 1 && (splits - 1) * ((stages + splits - 1) / splits) >= stages) --splits;
+    const bool one_sum = p.out_bf16 || (stages + splits - 1) / splits * SEG <= MMA_CHUNK;
+    return one_sum ? launch_as<NT, GROUPS, SHARE, false>(p, run_magic, parts, splits, status, stream)
+                   : launch_as<NT, GROUPS, SHARE, true>(p, run_magic, parts, splits, status, stream);
+}
+
 template <int NT>
-int launch_as(const QuantizedArgs& p, int groups, int share, int splits, uint32_t run_magic, int parts, int* status, cudaStream_t stream) {
+int launch_block(const QuantizedArgs& p, int groups, int share, int splits, uint32_t run_magic, int parts, int* status, cudaStream_t stream) {
     if (groups == 1 && share == 8) return launch<NT, 1, 8>(p, run_magic, parts, splits, status, stream);
     if (groups == 1 && share == 4) return launch<NT, 1, 4>(p, run_magic, parts, splits, status, stream);
     if (groups == 2 && share == 4) return launch<NT, 2, 4>(p, run_magic, parts, splits, status, stream);
@@ -310,6 +334,6 @@ CB_EXPORT int cb_linear_quantized_ring(int kind, const void* rows, long long ldr
         split_rows((const float*)rows, ldr, (__nv_bfloat16*)parts, M, K, s);
         p.rows = parts, p.ldr = K, n_parts = 3;
     }
-    return M * n_parts <= 8 ? launch_as<1>(p, groups, share, splits, run_magic, n_parts, status, s)
-                            : launch_as<2>(p, groups, share, splits, run_magic, n_parts, status, s);
+    return M * n_parts <= 8 ? launch_block<1>(p, groups, share, splits, run_magic, n_parts, status, s)
+                            : launch_block<2>(p, groups, share, splits, run_magic, n_parts, status, s);
 }
