@@ -357,11 +357,18 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #            side by side).
 #   "pairs"  tcgen05, two SMs a tile of 256 features by up to 256 rows, tile after tile.
 #
+# The tiles add up a block's share of K in one sum, from which the tensor cores cut off a little at every addition.  Over 4-bit
+# weights the kernel takes float32 results 2,048 of K at a time; of e4m3 products, which have 8 bits, sums of 4,096 are off by
+# 2.3e-7 of the norm, of 8,192 by 4.9e-7, of 12,288 by 8.4e-7 and of 16,384 by 1.2e-6, so there a share is 12,288 at most.
+# Where K has no such shares the pairs take it, 2,048 at a time (33 rows of 14,336 by 28,672 75.2 us, in one sum 68.5; by
+# 20,000 two blocks share K: 65.6).
+#
 # Between the last two, and for the rows a tile and the shares of K, a model of what a launch takes decides: a block's
 # fixed part, its steps along K (longer where two blocks are on an SM, and never shorter than the memory
 # allows), what a cluster costs, and how many blocks follow one another on an SM.  us, in `_COSTS`.
 FORM = None                      # tests name one of the forms, "few", "ring", "tiles" or "pairs", to reach it at any size
 N_SMS = 148
+_LONG_8 = 12288                  # K of one sum of e4m3 products, float32 results
 _RING_F32_ROWS = 5               # (three bfloat16 rows each, and the ring takes 16)
 _SMALL, _SMALL_8_ROWS = 1_200_000, 4_200_000           # weights of a matrix that "few" ends first: up to 64 rows, up to 8
 
@@ -441,9 +448,9 @@ def _ring(m: int, n: int, k: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def _rule(forced, kind: int, m: int, n: int, k: int):
+def _rule(forced, kind: int, m: int, n: int, k: int, f32: bool = False):
     """("few",), ("ring", groups of warps, warps a group, shares of K), ("tiles", rows a tile, shares of K) or
-    ("pairs", rows a tile, pairs of SMs)."""
+    ("pairs", rows a tile, pairs of SMs).  `f32`: float32 results."""
     form = forced
     if form is None:
         small = n * k <= _SMALL and m <= 64
@@ -469,11 +476,13 @@ def _rule(forced, kind: int, m: int, n: int, k: int):
                 continue
             tiles, per_sm = -(-n // 128) * -(-m // tok), _blocks_an_sm(kind, tok)
             for shares in (1, 2, 4, 6, 8) if per_sm == 2 else (1, 2, 4, 6):
-                if shares == 1 or (shares <= units and tiles * shares <= 320):
+                if shares > 1 and (shares > units or tiles * shares > 320):
+                    continue
+                if not (f32 and kind == _EIGHT and form is None and -(-units // shares) * 128 > _LONG_8):
                     us = _tiles_us(kind, m, n, k, tok, shares)
                     if best is None or us < best[0]:
                         best = us, ("tiles", tok, shares)
-    if kind != _FOUR_F32 and (form == "pairs" or (form is None and m >= 48)):
+    if kind != _FOUR_F32 and (form == "pairs" or (form is None and (m >= 48 or best is None))):
         for most in (64, 96, 128, 160, 192, 224, 256):
             tok = _even(m, most)
             us = _pairs_us(kind, m, n, k, tok)
@@ -494,8 +503,8 @@ def _status(dev: int) -> int:
     return word.data_ptr()
 
 
-def form_of(kind: int, m: int, n: int, k: int):
-    return _rule(FORM, kind, m, n, k)
+def form_of(kind: int, m: int, n: int, k: int, f32: bool = False):
+    return _rule(FORM, kind, m, n, k, f32)
 
 
 def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ldw: int, group_scales, w, group: int, out,
@@ -504,7 +513,7 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
         return
     n, k = w.shape
     _count(max(m, n), what)
-    form = form_of(kind, m, n, k)
+    form = form_of(kind, m, n, k, out.dtype is _F32)
     common = (kind, rows.data_ptr(), ldr, row_scales, values.data_ptr(), ldw, group_scales, w.scales.data_ptr(),
               _ptr(add), add.stride(0) if add is not None else 0, out.data_ptr(), 0 if out.dtype is _F32 else 1, ldo, m, n, k,
               group)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from crucible_b200.ops import quantized
-from quantized_cases import check_product, dense4
+from quantized_cases import E4M3, TOP, check_product, dense4, dense8
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -52,6 +52,24 @@ def test_from_registers(k, rows, dtype, monkeypatch):
     want = a.double() @ dense4(w).t()
     assert float((out.double() - want).norm() / want.norm()) <= 1e-6
     check_product(out, a.double(), dense4(w), None, 3 if dtype == "f32" else 1)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 33, 100])
+@pytest.mark.parametrize("n,k", [(200, 262144), (20000, 24576), (20000, 32768), (600, 73728)])
+def test_8_bit_rows(rows, n, k):
+    """e4m3 products have 8 bits, and sums of them of 12,288 of K stay below the bound."""
+    gen = torch.Generator(device=DEV).manual_seed(rows + k)
+    x = torch.randn(rows, k, generator=gen, device=DEV)
+    s = x.abs().amax(dim=1) / TOP
+    q = (x / s[:, None]).clamp(-TOP, TOP).to(E4M3)
+    w = quantized.Weights8.pack(torch.randn(n, k, generator=gen, device=DEV) * 0.02)
+    out = torch.empty(rows, n, device=DEV)
+    quantized.linear8(q, s, w, out)
+    w = quantized.Weights8(w.values[-200:], w.scales[-200:])
+    exact = q.double() * s.double()[:, None]
+    want = exact @ dense8(w).t()
+    assert float((out[:, -200:].double() - want).norm() / want.norm()) <= 1e-6
+    check_product(out[:, -200:], exact, dense8(w), None)
 
 
 def test_no_kernel_gave_up():

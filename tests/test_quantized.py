@@ -208,3 +208,14 @@ def test_a_wait_of_glu8_that_runs_out_is_told(monkeypatch):
                 waiting += waits
                 assert status or not waits, f"{dtype} {rows} x {width}"
     assert waiting > 20
+
+
+def test_shares_of_a_long_k_in_8_bits():
+    """float32 results of e4m3 products: no sum of more than 12,288 of K but in the pairs, which take 2,048 at a time, and from
+    registers, whose sums keep more."""
+    for m in (9, 33, 100, 1000):
+        for n in (200, 2048, 28672):
+            for k in (8192, 12288, 12289, 14336, 16384, 65536, 262144, 1 << 20):
+                form, *how = quantized._rule(None, quantized._EIGHT, m, n, k, True)
+                assert form in ("few", "pairs") or -(-(-(-k // 128)) // how[1]) * 128 <= 12288, (m, n, k, form, how)
+                assert quantized._rule(None, quantized._EIGHT, m, n, k)[0] != "ring"
