@@ -12,7 +12,7 @@ import torch
 
 from .. import ops
 from ..config.model_config import ConfigError, FeedForwardSpec
-from ..ops import quantized, small_batch
+from ..ops import quantized
 from .base import FEED_FORWARDS, FeedForward, TensorDecl
 
 
@@ -46,6 +46,7 @@ class SwiGLU4(SwiGLU):
     """The same with its matrices in 4 bits (`quantized.Weights4`): the checkpoint's are packed once, at load,
     with an e4m3 scale for every `group` weights of a feature (option, 64) and a float32 one a feature.  Rows, sums
     and the gated pair are those of the engine's dtype."""
+    fuses_norm = False         # its first product takes normalised rows: nobody is asked to leave others for it
 
     def __init__(self, spec: FeedForwardSpec):
         super().__init__(spec)
@@ -64,7 +65,7 @@ class SwiGLU4(SwiGLU):
         t, i = h.shape[0], self.spec.intermediate
         both = ctx.scratch("ffn.gate_up", (t, 2 * i), self.dtype)
         act = ctx.scratch("ffn.act", (t, i), self.dtype)
-        quantized.linear4(small_batch.as_tensor(h), self.gate_up, both)
+        quantized.linear4(h, self.gate_up, both)
         ops.swiglu(both, act)
         quantized.linear4(act, self.down, residual, add=residual)
 

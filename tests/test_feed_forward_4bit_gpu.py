@@ -75,3 +75,44 @@ def test_generation_in_bfloat16_follows_the_plain_model(tmp_path, name):
             band = TOLERANCE["bfloat16"] * float(logits.abs().max())
             assert float(logits.max() - logits[tok]) <= 2 * band, "token outside the rounding band"
             seq.append(tok)
+
+
+WIDE = {**CONFIGS["llama"], "num_hidden_layers": 2, "hidden_size": 1024, "num_attention_heads": 8, "num_key_value_heads": 4,
+        "head_dim": 128, "intermediate_size": 8192, "max_position_embeddings": 1024, "feed_forward_weight_group": 64}
+
+
+def test_a_wide_model_in_bfloat16_takes_prompts_by_every_form(tmp_path, monkeypatch):
+    """Prompts of some hundred rows go through the tiles and the pairs inside a step, a few rows through the ring; in none of
+    them does a product leave rows for a norm that does not read them."""
+    from crucible_b200 import LLM, SamplingParams, ops
+    from crucible_b200.ops import quantized
+    from crucible_b200.weights import write_random_model
+    monkeypatch.setitem(CONFIGS, "wide", WIDE)
+    folder = write_random_model(WIDE, os.path.join(str(tmp_path), "wide"), 3, std=helpers.TEST_STD)
+    forms, asked = set(), []
+    form_of, emit_of = quantized.form_of, ops._norm_emit
+    monkeypatch.setattr(quantized, "form_of", lambda *sizes: (forms.add(form_of(*sizes)[0]), form_of(*sizes))[1])
+
+    def emit(ctx, rows, tensor_core):
+        left = emit_of(ctx, rows, tensor_core)
+        asked.append(left.norm if left is not None else None)
+        return left
+    monkeypatch.setattr(ops, "_norm_emit", emit)
+    prompts = [helpers.random_tokens(WIDE["vocab_size"], n, 90 + i) for i, n in enumerate((40, 600))]
+    cfg, w = _plain(folder, "wide")
+    for prompt in prompts:
+        # (a prompt of 600 whole, and in portions of 128 rows)
+        for budget in (640, 128):
+            llm = LLM(folder, dtype="bfloat16", max_batch=2, prefill_token_budget=budget)
+            ahead = {id(layer.norms["feed_forward_norm"]) for layer in llm.engine.model.layers}
+            asked.clear()
+            out = llm.generate([prompt], SamplingParams(max_tokens=3))[0]
+            assert not any(id(norm) in ahead for norm in asked)
+            seq = list(prompt)
+            for tok in out:
+                logits = pm.plain_forward(cfg, w, seq)[-1]
+                band = TOLERANCE["bfloat16"] * float(logits.abs().max())
+                assert float(logits.max() - logits[tok]) <= 2 * band, "token outside the rounding band"
+                seq.append(tok)
+            del llm
+    assert {"ring", "tiles", "pairs"} <= forms, forms

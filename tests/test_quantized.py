@@ -219,3 +219,30 @@ def test_shares_of_a_long_k_in_8_bits():
                 form, *how = quantized._rule(None, quantized._EIGHT, m, n, k, True)
                 assert form in ("few", "pairs") or -(-(-(-k // 128)) // how[1]) * 128 <= 12288, (m, n, k, form, how)
                 assert quantized._rule(None, quantized._EIGHT, m, n, k)[0] != "ring"
+
+
+def test_4_bit_feed_forwards_take_normalised_rows():
+    """The block neither asks the attention's last product to leave rows ahead of the norm, which nobody would read, nor hands
+    over rows that are not normalised yet."""
+    from crucible_b200.config.model_config import FeedForwardSpec
+    from crucible_b200.parts.base import FEED_FORWARDS
+    from crucible_b200.parts.block import PreNormBlock
+    calls = []
+
+    class Norm:
+        supports_ahead = supports_lazy = True
+
+        def forward(self, ctx, x, lazy=False):
+            calls.append(("norm", lazy))
+            return "rows"
+
+    class Ctx:
+        def announce_norm(self, norm, rows):
+            calls.append(("announced", norm))
+    norm, rows = Norm(), torch.zeros(2, 64)
+    for kind, takes in (("swiglu", True), ("swiglu_4bit", False)):
+        part = FEED_FORWARDS.build(kind, FeedForwardSpec(kind=kind, width=64, intermediate=128, extra=(("group", 32),) * (kind != "swiglu")))
+        calls.clear()
+        PreNormBlock._announce(Ctx(), (norm, part), rows)
+        assert PreNormBlock._norm(Ctx(), norm, part, rows) == "rows"
+        assert calls == [("announced", norm if takes else None), ("norm", takes)]
