@@ -39,7 +39,8 @@ _FOUR_BF16, _FOUR_F32, _EIGHT = 0, 1, 2
 _MOST_PITCH = 1 << 24            # bytes between rows of weights (`csrc/quantized.cuh`)
 _FLOATS = (torch.float32, torch.bfloat16)
 _MOST_ROWS = (1 << 31) - 1024    # the kernels count rows and features in 32 bits
-_SLAB = 1 << 16                  # float32 rows over 4-bit weights at a time: three bfloat16 copies of them are needed
+_SLAB = 1 << 16                  # float32 rows over 4-bit weights at a time, at most
+_SCRATCH = 512 << 20             # and at most so many bytes of their three bfloat16 parts, 6 a number
 _LEAST_LIMIT = 2.0 ** -126       # (a smaller limit could be zero in float32)
 _WAITS_FROM = 296                # rows of `glu8` from which its kernel may wait for copies (`cb_glu8_waits_from`)
 
@@ -566,10 +567,17 @@ def linear8(rows: torch.Tensor, row_scales: torch.Tensor, w: Weights8, out: torc
              add, "linear (8-bit weights)")
 
 
+def _slab(m: int, k: int) -> int:
+    """Rows at a time, of m float32 rows over 4-bit weights: equal slabs, in tiles of 64."""
+    most = max(64, min(_SLAB, _SCRATCH // (6 * k)) // 64 * 64)
+    return min(most, _up(-(-m // -(-m // most)), 64))
+
+
 def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch.Tensor] = None) -> None:
     """out = a . W^T (+ add): float32 or bfloat16 rows `a` [M, K]; `out`: float32 or bfloat16 [M, N]; `add`:
     float32 [M, N], which may be `out`.  K up to 2^20.  Rows that do not begin on multiples of 16 bytes are brought
-    into ones that do, at every call."""
+    into ones that do, at every call.  float32 rows take scratch memory from torch's pool for the call: 6 bytes a number for their
+    bfloat16 parts, 512 MB at most (more rows than that holds are taken a part at a time)."""
     if not isinstance(w, Weights4):
         raise KernelError(f"linear4 takes Weights4, got {type(w).__name__}")
     dev, shape, rs, os = a.get_device(), a.shape, a.stride(), out.stride()
@@ -587,9 +595,10 @@ def linear4(a: torch.Tensor, w: Weights4, out: torch.Tensor, add: Optional[torch
         if not _aligned16(a):
             a = _in_aligned_rows(a)
         rs = (_pitch(a),)
-    if f32 and shape[0] > _SLAB:
-        for at in range(0, shape[0], _SLAB):
-            to = at + _SLAB
+    if f32 and shape[0] > 64 and (shape[0] > _SLAB or 6 * k * shape[0] > _SCRATCH):
+        rows = _slab(shape[0], k)
+        for at in range(0, shape[0], rows):
+            to = at + rows
             linear4(a[at:to], w, out[at:to], add=None if add is None else add[at:to])
         return
     _product(_FOUR_F32 if f32 else _FOUR_BF16, dev, a, shape[0], rs[0], None, w.codes, k // 2, w.group_scales.data_ptr(),

@@ -246,3 +246,13 @@ def test_4_bit_feed_forwards_take_normalised_rows():
         PreNormBlock._announce(Ctx(), (norm, part), rows)
         assert PreNormBlock._norm(Ctx(), norm, part, rows) == "rows"
         assert calls == [("announced", norm if takes else None), ("norm", takes)]
+
+
+def test_scratch_of_float32_rows_is_bounded():
+    """Slabs of float32 rows: whole tiles, equal but for the last, at most 512 MB of parts, and no more of them than that takes."""
+    for k in (32, 256, 4096, 14336, 16384, 100000 // 32 * 32, 1 << 20):
+        for m in (65, 2048, 4096, 65536, 65537, 1 << 20, 4_200_000):
+            rows = quantized._slab(m, k)
+            assert rows % 64 == 0 and 64 <= rows <= quantized._SLAB and 6 * k * rows <= 512 << 20
+            least = max(-(-m // quantized._SLAB), -(-6 * k * m // (512 << 20)))
+            assert -(-m // rows) <= least + 1 + least // 4 or rows <= 640        # (a slab of few tiles wastes more of the room)
