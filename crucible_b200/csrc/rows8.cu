@@ -19,6 +19,7 @@ namespace {
 
 constexpr float E4M3_TOP = 448.f;
 constexpr float LEAST = 1e-30f;
+constexpr float BIG_R = 262144.f;       // a factor r up to here: neither r * (448 / LEAST) nor 448 / max |v| of a max |v| r from LEAST on overflows
 
 // two fp32 to two e4m3 (the lower byte is `lo`): to nearest even, beyond 448 to 448, NaN stays NaN
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -152,7 +153,7 @@ norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const
         }
     }
     ss = row_sum<WARP>(ss, scratch);
-    const float r = 1.0f / sqrtf(ss / (float)width + eps);
+    float r = 1.0f / sqrtf(ss / (float)width + eps);
     // y = v r with v = sum * gain: the row's factor r is in its largest number as well, so 448 / max |v| takes v to e4m3 with
     // three roundings, whatever r was rounded to
     float top = 0.f;
@@ -167,7 +168,15 @@ norm8_kernel(const float* x, long long ldx, const D* delta, long long ldd, const
             top = magnitude(top, v[c]);
         }
     }
-    const float top_v = row_max<WARP>(top, reinterpret_cast<uint32_t*>(scratch)), top_y = top_v * r;
+    float top_v = row_max<WARP>(top, reinterpret_cast<uint32_t*>(scratch));
+    const float top_y = top_v * r;
+    if (r > BIG_R) {                                   // (eps below 1.5e-11 and a row of next to nothing)
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[c][i] *= r;
+        top_v = top_y, r = 1.f;
+    }
     const float most = at_least(top_y);
     const float factor = top_y >= LEAST ? E4M3_TOP / top_v : (top_y < LEAST ? r * (E4M3_TOP / LEAST) : top_y);
 #pragma unroll
