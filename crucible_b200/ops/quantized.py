@@ -243,7 +243,7 @@ class Weights8:
 def _finite(w: torch.Tensor) -> torch.Tensor:
     if w.dim() != 2 or not w.is_floating_point() or w.numel() == 0:
         raise KernelError(f"weights are packed from a matrix of floating numbers, got {w.dtype} {list(w.shape)}")
-    w = w.float()
+    w = w.float().contiguous()
     if not bool(torch.isfinite(w).all()):
         raise KernelError("weights are packed from finite numbers")
     return w

@@ -256,3 +256,12 @@ def test_scratch_of_float32_rows_is_bounded():
             assert rows % 64 == 0 and 64 <= rows <= quantized._SLAB and 6 * k * rows <= 512 << 20
             least = max(-(-m // quantized._SLAB), -(-6 * k * m // (512 << 20)))
             assert -(-m // rows) <= least + 1 + least // 4 or rows <= 640        # (a slab of few tiles wastes more of the room)
+
+
+def test_a_transposed_matrix_is_packed():
+    w = torch.randn(64, 96, generator=_gen())
+    for view in (w.t(), w.t()[:, ::2], w[::2].t(), w.t().double(), w.t().bfloat16(), w.flip(0)):
+        rows = view.contiguous()
+        for cls, group in ((quantized.Weights8, ()), (quantized.Weights4, (32,))):
+            here, there = cls.pack(view, *group), cls.pack(rows, *group)
+            assert here.shape == view.shape and torch.equal(here.dense(), there.dense())
