@@ -344,7 +344,9 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
 #   "ring"   the same arithmetic behind a ring of stages: 4-bit weights, K a multiple of 256, bfloat16 rows.  8 rows of
 #            4,096 by 4,096, ring / few / tiles: 4.8 / 7.0 / 8.1; 16 rows by 14,336 14.6 / 20.6 / 16.5; 32 rows by 2,048 (K of
-#            8,192) 9.7 / 12.7 / 11.2, by 6,144 (K of 4,096) 13.0 / 19.8 / 11.5.  A block is so many groups of warps by
+#            8,192) 9.7 / 12.7 / 11.2, by 6,144 (K of 4,096) 13.0 / 19.8 / 11.5.  17 to 32 rows by few features, ring / tiles: by
+#            1,920 (tiles of which six share a long K) K of 5,120 7.3 / 8.1, of 6,144 8.2 / 8.2, of 8,192 10.3 / 9.3, of 16,384
+#            16.6 / 13.3; by 1,984 (four share it) 7.3 / 9.3, 8.2 / 9.7, 10.3 / 11.3, 16.6 / 17.2.  A block is so many groups of warps by
 #            warps that share a group's K: 1 x 8 while the SMs have two blocks or fewer at once, 1 x 4 beyond (8 rows by
 #            28,672, 1 x 8 / 1 x 4 / 2 x 4: 22.5 / 19.8 / 22.7; by 4,096 4.8 / 5.4 / 7.1), 2 x 2 where K is short beside
 #            the features and the rows are best read less often (by 50,304, K of 768, 1 x 4 / 2 x 2: 9.5 / 8.4), 2 x 4 for
@@ -456,7 +458,7 @@ def _rule(forced, kind: int, m: int, n: int, k: int, f32: bool = False):
     if form is None:
         small = n * k <= _SMALL and m <= 64
         if kind == _FOUR_BF16:
-            narrow = (n <= 2048 and (n >= 1536 or k <= 4096)) or (n <= 4096 and k <= 2048)
+            narrow = (n <= 2048 and (n > 1920 or k <= 5120)) or (n <= 4096 and k <= 2048)
             form = "ring" if m <= 16 or (m <= 32 and narrow) else "few" if small else None
         elif kind == _FOUR_F32 and m <= _RING_F32_ROWS and k % 256 == 0 and not (small and k <= 1024):
             form = "ring"

@@ -265,3 +265,11 @@ def test_a_transposed_matrix_is_packed():
         for cls, group in ((quantized.Weights8, ()), (quantized.Weights4, (32,))):
             here, there = cls.pack(view, *group), cls.pack(rows, *group)
             assert here.shape == view.shape and torch.equal(here.dense(), there.dense())
+
+
+def test_few_rows_by_few_features_of_a_long_k():
+    """17 to 32 rows: the ring up to 5,120 of K, and beyond it only where no six tiles share K (measured both sides)."""
+    for m in (17, 32):
+        for n, k, form in ((1536, 5120, "ring"), (1536, 8192, "tiles"), (1920, 16384, "tiles"), (1984, 16384, "ring"),
+                           (2048, 8192, "ring"), (1408, 5120, "ring"), (4096, 2048, "ring"), (4096, 4096, "tiles")):
+            assert quantized._rule(None, quantized._FOUR_BF16, m, n, k)[0] == form, (m, n, k)
