@@ -497,7 +497,8 @@ def _rule(forced, kind: int, m: int, n: int, k: int, f32: bool = False):
 def _status(dev: int) -> int:
     """The address of the word that a kernel writes if one of its bounded waits runs out (`tensor_core.check_status`
     raises then).  None yet, and a graph is being captured: null, since the word's zero would be written by the
-    graph's replays and not now."""
+    graph's replays and not now.  (`glu8` then takes the kernel that does not wait, a product is refused; whoever made
+    his weights before the capture has the word.)"""
     word = tensor_core._status.get(dev)
     if word is None:
         if torch.cuda.is_current_stream_capturing():
@@ -524,6 +525,9 @@ def _product(kind: int, dev: int, rows, m: int, ldr: int, row_scales, values, ld
         code = _at(dev, build.load("linear_quantized_few").cb_linear_quantized_few, *common)
     else:
         status = _status(dev)
+        if not status:
+            raise KernelError(f"{what}: the first use on a device cannot be inside a graph's capture: its kernels have no place yet "
+                              f"to say that a wait ran out")
         parts = None
         if kind == _FOUR_F32:
             parts = torch.empty(3 * m * k, dtype=torch.bfloat16, device=rows.device)

@@ -273,3 +273,21 @@ def test_few_rows_by_few_features_of_a_long_k():
         for n, k, form in ((1536, 5120, "ring"), (1536, 8192, "tiles"), (1920, 16384, "tiles"), (1984, 16384, "ring"),
                            (2048, 8192, "ring"), (1408, 5120, "ring"), (4096, 2048, "ring"), (4096, 4096, "tiles")):
             assert quantized._rule(None, quantized._FOUR_BF16, m, n, k)[0] == form, (m, n, k)
+
+
+def test_a_product_that_could_not_tell_of_a_wait_is_refused(monkeypatch):
+    """Inside a capture on a device that has no status word yet."""
+    from crucible_b200.ops import tensor_core
+    monkeypatch.setattr(tensor_core, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    launched = []
+    monkeypatch.setattr(quantized, "_at", lambda dev, call, *args: launched.append(call) or 0)
+    w = random_weights4(300, 256, 64, "cpu", _gen())
+    for rows, dtype in ((1, torch.bfloat16), (100, torch.bfloat16), (100, torch.float32)):
+        a, out = torch.zeros(rows, 256, dtype=dtype), torch.zeros(rows, 300)
+        kind = quantized._FOUR_F32 if dtype == torch.float32 else quantized._FOUR_BF16
+        monkeypatch.setattr(quantized, "FORM", None if rows == 1 else "tiles")
+        form = quantized.form_of(kind, rows, 300, 256)[0]
+        call = (kind, 0, a, rows, 256, None, w.codes, 128, w.group_scales.data_ptr(), w, 64, out, 300, None, "linear (4-bit weights)")
+        assert form in ("ring", "tiles") and not launched
+        _refused("inside a graph's capture", quantized._product, *call)
