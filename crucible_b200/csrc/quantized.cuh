@@ -85,7 +85,8 @@ __device__ __forceinline__ void three_parts(float x, float y, uint32_t (&p)[3]) 
     for (int j = 0; j < 3; ++j) p[j] = part[0][j] | (part[1][j] << 16);
 }
 
-// fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.
+// fp32 rows as three bf16 ones: parts [3, M, K].  Four numbers a thread.  (A template, so that only the sources that launch it
+// carry it.)
 template <int THREADS> __global__ void __launch_bounds__(THREADS) split_rows_kernel(const float* __restrict__ rows, long long ldr,
                                                          __nv_bfloat16* __restrict__ parts, int M, int K) {
     cb_pdl_wait();

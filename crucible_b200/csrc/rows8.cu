@@ -10,7 +10,8 @@
 //
 // Memory bounds both: one pass over the data, a row's numbers stay in the registers of the threads
 // that fetched them (16 bytes a chunk) while the row's sum of squares and largest magnitude are taken.
-// (2,048 rows of 4,096 with a bf16 delta 17.0 us, 5.4 TB/s; 2,048 of 14,336 bf16 pairs 27.2, 5.4 TB/s.)
+// (In a chain over inputs that are not in L2: 2,048 rows of 4,096 with a bf16 delta 17.0 us, 5.4 TB/s; 2,048 of 14,336 bf16
+// pairs 27.2, 5.4 TB/s.)
 #define CB_PDL_BIT 6      // this file's bit in CRUCIBLE_PDL
 #include "quantized.cuh"
 #include "tc_common.cuh"
@@ -292,7 +293,7 @@ glu8_kernel(const T* __restrict__ both, long long ldb, uint8_t* __restrict__ q, 
 
 // The same for many long rows: a block stays on its SM and walks rows, which one thread brings into shared memory, as
 // many ahead as fit.  (A block a row has nothing on its way while it computes and takes the row's maximum.  us, 2,048 rows,
-// this / a block a row: 14,336 bf16 pairs 27.1 / 31.9, 11,008 22.0 / 27.5, 10,240 20.7 / 21.8, 8,192 17.8 / 17.4; 7,168 fp32
+// this / a block a row: 14,336 bf16 pairs 27.2 / 31.9, 11,008 22.0 / 27.5, 10,240 20.7 / 21.8, 8,192 17.8 / 17.4; 7,168 fp32
 // pairs 24.5 / 27.8, 4,096 15.6 / 15.5.)
 constexpr int RING_ROWS = 8;            // stages at most
 constexpr int RING_BYTES = 32768;       // rows of more than this

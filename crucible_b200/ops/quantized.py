@@ -337,8 +337,8 @@ def _out_rows(out: torch.Tensor, add: Optional[torch.Tensor], shape, what: str) 
 
 
 # Which kernel, and how.  What follows was measured on B200 for the three kinds of product at 11 sizes of weights, 1,280 by
-# 768 to 28,672 by 4,096 (and 50,304 by 768, 4,096 by 14,336), and 1 to 2,048 rows, in every form: the rules below took
-# 0.8% longer than the best form on the average.
+# 768 to 28,672 by 4,096 (and 50,304 by 768, 4,096 by 14,336), and 1 to 2,048 rows, in every form: the rules below, fitted to
+# these, took 0.8% longer than the best form on the average.
 #
 #   "few"    mma.sync from registers.  Nothing stands between a load and its use, so small matrices end first: us at 64
 #            rows of 768 by 1,280, few / tiles: 4.8 / 5.2 (8 bits), 5.2 / 6.8 (4 bits); 8 rows of 2,048 by 2,048 5.2 / 5.9.
