@@ -1,0 +1,865 @@
+// Attention over the paged cache in 4 bits (`cache4.cuh`): scores s_j = q . k_j over the keys that a row sees,
+// softmax, o = sum_j p_j v_j, in one pass over the keys with a running maximum.
+//
+// The codes go to the tensor cores as they are.  With k = step c + low in every group,
+//     q . k   = sum_groups step (sum_f q_f c_f) + low (sum_f q_f)
+//     o_f     = sum_j (p_j step_j) c_jf + sum_j p_j low_j
+// so a tile of 16 keys is two products over codes; steps and lows meet the sums in float32.  A code in the low
+// four bits of a half word IS the float16 number code * 2^-24 (a subnormal, which the tensor cores multiply like any
+// other), in the next four bits code * 2^-20: taking codes apart is a mask for every two of them and a shift for
+// every eight, and 2^-24 and 16 are put right in the scales.  Queries and p step are float16 then: the queries
+// of a row are scaled by a power of two so that the largest lies in [2^13, 2^14), which holds bfloat16 numbers
+// exactly down to 2^-30 of it; p step is scaled by a power of two that follows the largest step seen, and rounded
+// to 11 bits.  float32 rows take two float16 parts of either (22 bits), their sums over keys leave the
+// tensor cores tile by tile (these cut off what float32 additions would round), and their codes are made
+// normal numbers, code | 1024 less 1032: the tensor cores line the products of subnormals up as if they were
+// normal and lose up to ten bits of the sum, which float32 rows showed (3e-5 to 7e-5 off) and bfloat16 ones do not.
+//
+// Keys are the rows of a tile and queries its columns: eight rows (heads of a group, tokens of a portion) a column
+// tile, one or two of them a block, so that no more than that is multiplied for a single token.  S^T comes out with
+// keys over lanes; `movmatrix` turns it for the second product, which takes P^T, again eight columns.
+//
+// A block of four warps takes the row tile's share of the keys, a warp every fourth tile of 16, each with a
+// ring of its own in shared memory that cp.async fills a few tiles ahead: nothing is waited for but copies of the
+// warp itself.  The warps' results meet in shared memory, those of up to eight blocks of a cluster in each
+// other's; more shares than that go through memory and a second kernel.
+#pragma once
+#include "cache4.cuh"
+
+#include <type_traits>
+
+namespace {
+
+constexpr float A4_LOG2E = 1.4426950408889634f;
+constexpr int A4_WARPS = 4;
+
+struct Attn4Params {
+    const void* q;
+    long long q_stride;
+    void* out;
+    long long out_stride;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    int n_pages, page_tokens, kv_heads, n_rep;
+    const int* row_start;      // requests of consecutive rows ...
+    const int* first_pos;
+    const int* table;
+    int table_stride;
+    int requests;
+    const int* picks;          // ... or, with picks, every row by itself: [rows][kv heads][count]
+    int pick_count;
+    const int* row_request;
+    const int* positions;
+    int rows;
+    int page_tiles;            // tiles of 16 keys a page (0: a tile may lie in two) ...
+    uint32_t page_tiles_inverse;      // ... and 2^32 over them, rounded up (0: one tile a page)
+    int window;                // 0: all earlier keys
+    float scale_log2;
+    int row_tiles;
+    int chunk_tiles;           // tiles of 16 keys a share where shares go through memory, else 0
+    int n_chunks;
+    float* partial;            // [x][chunk][8 NT][D + 2]
+};
+
+__device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void a4_copy16(uint32_t dst, const void* src, bool there) {
+    const int bytes = there ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void a4_copy4(uint32_t dst, const void* src, bool there) {
+    const int bytes = there ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t a4_turned(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float a4_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t a4_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float a4_power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Two codes a register: from the low four bits of each half (HIGH: from the next four, and 16 times as large).
+// In units of 2^-24; or (F32) in units of 1 and less 8, which goes to the lows: terms of both signs, smaller sums.
+template <bool F32, bool HIGH>
+__device__ __forceinline__ uint32_t a4_codes(uint32_t w) {
+    const uint32_t c = w & (HIGH ? 0x00f000f0u : 0x000f000fu);
+    if constexpr (!F32) return c;
+    const uint32_t m = c | 0x64006400u, k = HIGH ? 0x64806480u : 0x64086408u;       // 1024 + code, 1024 + 8 (or 16 times that)
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&k));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// The NG pairs of a key.
+template <int NG>
+__device__ __forceinline__ void a4_pairs(uint32_t (&out)[NG], const uint8_t* at) {
+    if constexpr (NG == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        out[0] = v.x; out[1] = v.y;
+    } else if constexpr (NG % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < NG / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(at)[i];
+            out[4 * i] = v.x; out[4 * i + 1] = v.y; out[4 * i + 2] = v.z; out[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) out[i] = reinterpret_cast<const uint32_t*>(at)[i];
+    }
+}
+
+template <bool F32>
+__device__ __forceinline__ float a4_low(uint32_t pair) {
+    return F32 ? fmaf(8.f, c4_step(pair), c4_low(pair)) : c4_low(pair);
+}
+
+// Largest over the eight lanes that hold the keys of one column.
+__device__ __forceinline__ float a4_over_keys_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float a4_over_keys_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// Shared memory of a block of D features, NG groups, NT column tiles, PARTS float16 parts of a query.
+template <int D, int NG, int NT, int PARTS>
+struct A4Layout {
+    static constexpr int SIDE = 16 * D / 2;                    // codes of a tile's keys, or values
+    static constexpr int SCALES = 16 * NG * 4;
+    static constexpr int STAGE = 2 * SIDE + 2 * SCALES;
+    static constexpr int STAGES = D <= 64 ? 6 : D <= 128 ? 4 : 3;
+    static constexpr int PITCH = D + 4;                        // floats of a row of results (lanes of four rows meet other banks)
+    static constexpr int RESULT = 8 * NT * PITCH * 4;          // a warp's result takes its ring's place
+    static constexpr int RING = STAGE * STAGES > RESULT ? STAGE * STAGES : RESULT;
+    static constexpr int Q = (D / 16) * PARTS * NT * 32 * 8;   // queries as the products take them
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int AT_Q = A4_WARPS * RING;
+    static constexpr int AT_SUMS = AT_Q + Q;                   // [ROWS][NG] sums of a row's scaled queries
+    static constexpr int AT_FACTOR = AT_SUMS + ROWS * NG * 4;  // [ROWS] what raw scores are multiplied by
+    static constexpr int AT_STATE = AT_FACTOR + ROWS * 4;      // [WARPS + 1][ROWS][2]: reference and sum
+    static constexpr int TOTAL = AT_STATE + (A4_WARPS + 1) * ROWS * 8;
+};
+
+// 16-byte units of a tile's rows change places so that lanes that read rows 2t meet other banks.
+template <int D>
+__device__ __forceinline__ int a4_place(int r, int unit) {
+    constexpr int UNITS = D / 32;
+    if constexpr (D == 64) {
+        const int u = (r & 3) * 2 + unit;
+        return (r >> 2) * 128 + ((u ^ (2 * ((r >> 2) & 1))) << 4);
+    } else if constexpr (D == 128) {
+        const int u = (r & 1) * 4 + unit;
+        return (r >> 1) * 128 + ((u ^ (2 * ((r >> 1) & 3))) << 4);
+    } else if constexpr (D == 256) {
+        return r * 128 + ((unit ^ (2 * ((r >> 1) & 3)) ^ (r & 1)) << 4);
+    } else {
+        return (r * UNITS + unit) << 4;
+    }
+}
+
+template <int D, int NG, int NT, bool F32>
+__global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) attention4_kernel(const Attn4Params p) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    constexpr int PARTS = F32 ? 2 : 1;
+    using L = A4Layout<D, NG, NT, PARTS>;
+    constexpr int GROUP = D / NG, W = D / 64, KS = D / 16, MT = D / 16;
+    constexpr float CODE = F32 ? 1.f : 16777216.f;      // 1 over the unit of the codes
+    using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+
+    // which rows, which keys
+    int x = blockIdx.x;
+    const int row_tile = x % p.row_tiles;
+    x /= p.row_tiles;
+    const int kv = x % p.kv_heads;
+    x /= p.kv_heads;
+    int row0, n_rows, first, request;
+    if (p.picks != nullptr) {
+        row0 = x;
+        request = p.row_request[x];
+        first = p.positions[x];
+        n_rows = (request >= 0 && request < p.requests && first >= 0) ? p.n_rep : 0;
+    } else {
+        request = x;
+        row0 = p.row_start[x];
+        n_rows = min(p.row_start[x + 1], p.rows) - row0;
+        n_rows = (row0 < 0 ? 0 : n_rows) * p.n_rep;
+        first = p.first_pos[x];
+    }
+    const int base = row_tile * L::ROWS;
+    if (base >= n_rows) return;                 // (all blocks of a cluster together)
+    const int* table = p.table + (size_t)request * p.table_stride;
+    const int last_row = min(n_rows, base + L::ROWS) - 1;
+    const int min_pos = first + base / p.n_rep, max_pos = first + last_row / p.n_rep;
+    int tile_lo = 0, tile_hi;
+    const int* picks = nullptr;
+    if (p.picks != nullptr) {
+        picks = p.picks + ((size_t)row0 * p.kv_heads + kv) * p.pick_count;
+        tile_hi = p.pick_count * p.page_tiles;
+    } else {
+        if (p.window > 0) tile_lo = max(0, min_pos - p.window + 1) >> 4;
+        tile_hi = (max_pos >> 4) + 1;
+    }
+    const int lowest = p.window > 0 ? max_pos - p.window : -1;         // a tile that begins here or before needs a look
+    int n_chunks = 1;
+    if (p.chunk_tiles > 0) {
+        n_chunks = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
+        if ((int)blockIdx.z >= max(n_chunks, 1)) return;
+        tile_lo += blockIdx.z * p.chunk_tiles;
+        if ((int)blockIdx.z + 1 < n_chunks) tile_hi = tile_lo + p.chunk_tiles;       // (the last takes what is left)
+    } else if (gridDim.z > 1) {
+        const int share = (tile_hi - tile_lo + gridDim.z - 1) / gridDim.z;
+        tile_lo += blockIdx.z * share;
+        tile_hi = min(tile_hi, tile_lo + share);
+    }
+
+    // ---- the warp's ring ----------------------------------------------------
+    const uint32_t ring = a4_smem(smem) + warp * L::RING;
+    const bool whole = p.page_tiles > 0;                 // a tile lies in one page
+    const size_t side_rows = (size_t)p.n_pages * p.kv_heads * p.page_tokens;
+    const size_t head_row = (size_t)kv * p.page_tokens;
+    const uint8_t* const code_src[2] = {p.codes + head_row * (D / 2) + lane * 16,
+                                        p.codes + (side_rows + head_row) * (D / 2) + lane * 16};
+    // (scales: lanes of both sides side by side)
+    const uint8_t* const scale_src = p.scales + (head_row + (lane >= 4 * NG ? side_rows : 0)) * (NG * 4) + (lane % (4 * NG)) * 16;
+    uint32_t place[D / 64];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) place[j] = a4_place<D>((lane + 32 * j) / (D / 32), (lane + 32 * j) % (D / 32));
+    // The row of tile i's first key (whole) for head 0, or -1 where its page is none; its position goes to `key`.
+    auto look = [&](int i, int& key) -> long long {
+        key = i * 16;
+        if (i >= tile_hi || !whole) return -1;
+        int index = p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse);
+        if (index * p.page_tiles > i) --index;           // (rounded up, the inverse is at most one too much)
+        const int slot = (i - index * p.page_tiles) * 16;
+        if (picks != nullptr) {
+            index = picks[index];
+            key = index * p.page_tokens + slot;
+        }
+        if ((unsigned)index >= (unsigned)p.table_stride) return -1;
+        const int page = table[index];
+        if ((unsigned)page >= (unsigned)p.n_pages) return -1;
+        return (long long)page * (p.kv_heads * p.page_tokens) + slot;
+    };
+    auto fetch = [&](int i, int stage, int key, long long at) {
+        if (i < tile_hi) {
+            const uint32_t to = ring + stage * L::STAGE;
+            if (whole) {
+                // (a tile whose page is none is filled with zeros, and masked)
+                const bool there = at >= 0;
+                const long long row = there ? at : 0;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint8_t* src = code_src[s] + row * (D / 2);
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) a4_copy16(to + s * L::SIDE + place[j], src + j * 512, there);
+                }
+                if constexpr (8 * NG <= 32) {
+                    if (lane < 8 * NG) a4_copy16(to + 2 * L::SIDE + lane * 16, scale_src + row * (NG * 4), there);
+                } else {
+#pragma unroll
+                    for (int c = lane; c < 8 * NG; c += 32) {
+                        const int side = c / (4 * NG), u = c % (4 * NG);
+                        a4_copy16(to + 2 * L::SIDE + c * 16,
+                                  p.scales + (head_row + row + side * side_rows) * (NG * 4) + u * 16, there);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int c = lane; c < 16 * (D / 32); c += 32) {
+                    const int r = c / (D / 32), u = c % (D / 32);
+                    const long long one = key + r <= max_pos
+                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
+                    const size_t row = one >= 0 ? (size_t)one + head_row : 0;
+                    const uint8_t* src = p.codes + row * (D / 2) + u * 16;
+                    a4_copy16(to + a4_place<D>(r, u), src, one >= 0);
+                    a4_copy16(to + L::SIDE + a4_place<D>(r, u), src + side_rows * (D / 2), one >= 0);
+                }
+#pragma unroll 1
+                for (int c = lane; c < 16 * NG; c += 32) {
+                    const int r = c / NG, u = c % NG;
+                    const long long one = key + r <= max_pos
+                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
+                    const size_t row = one >= 0 ? (size_t)one + head_row : 0;
+                    const uint8_t* src = p.scales + (row * NG + u) * 4;
+                    a4_copy4(to + 2 * L::SIDE + c * 4, src, one >= 0);
+                    a4_copy4(to + 2 * L::SIDE + L::SCALES + c * 4, src + side_rows * (NG * 4), one >= 0);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int ahead = tile_lo + warp;            // the next tile to fetch
+    int key_of[L::STAGES];                 // first keys of the tiles in flight; -1: of no page
+#pragma unroll
+    for (int s = 0; s < L::STAGES - 1; ++s) {
+        int key;
+        const long long at = look(ahead, key);
+        fetch(ahead, s, key, at);
+        key_of[s] = whole && at < 0 ? -1 : key;
+        ahead += A4_WARPS;
+    }
+    int next_key;
+    long long next_at = look(ahead, next_key);
+
+    // ---- the queries, as columns of the first product --------------------------
+    {
+        __half* qs = reinterpret_cast<__half*>(smem + L::AT_Q);
+        float* sums = reinterpret_cast<float*>(smem + L::AT_SUMS);
+        float* factor = reinterpret_cast<float*>(smem + L::AT_FACTOR);
+#pragma unroll 1
+        for (int r = warp; r < L::ROWS; r += A4_WARPS) {
+            float v[D / 32];
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
+            if (base + r < n_rows) {
+                const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
+                const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(row0 + tok) * p.q_stride + (size_t)head * D;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) v[i] = cb_to_float(src[lane + 32 * i]);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) most = fmaxf(most, fabsf(v[i]));
+            most = cb_warp_max(most);
+            // (100: the factor 2^-e stays far from float32's ends)
+            const int e = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+            const float up = a4_power(e);
+            if (lane == 0) factor[r] = p.scale_log2 * a4_power(-e);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                v[i] *= up;
+                const int f = lane + 32 * i, w = f >> 6, k = (f >> 3) & 7, c8 = f & 7;
+                // step (w, k / 4, c8 & 1) of the product, lane (r & 7, c8 / 2), number (0, 2, 1, 3)[k & 3]
+                const int ks = (w * 2 + (k >> 2)) * 2 + (c8 & 1), n = ((k & 1) << 1) | ((k >> 1) & 1);
+                float y = (k & 1) ? v[i] * 0.0625f : v[i];        // its codes come 16 times too large
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    const __half h = __float2half_rn(y);
+                    y -= __half2float(h);
+                    qs[(((ks * PARTS + part) * NT + (r >> 3)) * 32 + (r & 7) * 4 + (c8 >> 1)) * 4 + n] = h;
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < GROUP / 32; ++i) s += v[gr * (GROUP / 32) + i];
+                s = cb_warp_sum(s);
+                if (lane == 0) sums[r * NG + gr] = s;
+            }
+        }
+        __syncthreads();
+    }
+    const uint2* qf = reinterpret_cast<const uint2*>(smem + L::AT_Q) + lane;
+    constexpr bool Q_IN_REGS = KS * PARTS * NT <= 8;
+    uint2 qr[Q_IN_REGS ? KS * PARTS * NT : 1];
+    if constexpr (Q_IN_REGS) {
+#pragma unroll
+        for (int i = 0; i < KS * PARTS * NT; ++i) qr[i] = qf[i * 32];
+    }
+    float qsum[NT][NG][2], factor[NT][2];
+    int pos[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = n * 8 + 2 * t + c;
+            factor[n][c] = reinterpret_cast<const float*>(smem + L::AT_FACTOR)[r];
+            pos[n][c] = first + min(base + r, n_rows - 1) / p.n_rep;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) qsum[n][gr][c] = reinterpret_cast<const float*>(smem + L::AT_SUMS)[r * NG + gr];
+        }
+
+    // Sums of a column are kept relative to 2^off, off = m - eps: m the reference of its scores (log2), at most 8 below the
+    // largest, and 2^eps the scale of p step in float16; `bound` is the step from which eps is too much.
+    float off[NT][2], eps[NT][2], bound[NT][2], sum[NT][2], lows[NT][NG][2], o[MT][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            off[n][c] = -3.0e38f;
+            eps[n][c] = 101.f;
+            bound[n][c] = a4_power(-95);
+            sum[n][c] = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) lows[n][gr][c] = 0.f;
+        }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
+
+    // ---- over the keys -----------------------------------------------------------
+    // One tile.  EDGE: some row may not see some key of it.
+    auto tile = [&](auto edge, const uint8_t* at, int key0) {
+        constexpr bool EDGE = decltype(edge)::value;
+        // S^T = K Q^T, by groups
+        float s[NT][4];
+        uint32_t kw[2][2 * W];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h;
+            if constexpr (D == 64) {
+                const uint2 v = *reinterpret_cast<const uint2*>(at + a4_place<D>(r, t >> 1) + (t & 1) * 8);
+                kw[h][0] = v.x; kw[h][1] = v.y;
+            } else if constexpr (D == 192) {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + r * 96 + t * 24 + j * 8);
+                    kw[h][2 * j] = v.x; kw[h][2 * j + 1] = v.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < D / 128; ++j) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(at + a4_place<D>(r, t * (D / 128) + j));
+                    kw[h][4 * j] = v.x; kw[h][4 * j + 1] = v.y; kw[h][4 * j + 2] = v.z; kw[h][4 * j + 3] = v.w;
+                }
+            }
+        }
+        uint32_t ksc[2][NG], vsc[2][NG];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            a4_pairs<NG>(ksc[h], at + 2 * L::SIDE + (g + 8 * h) * (NG * 4));
+            a4_pairs<NG>(vsc[h], at + 2 * L::SIDE + L::SCALES + (g + 8 * h) * (NG * 4));
+        }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+            for (int b = gr * (GROUP / 32); b < (gr + 1) * (GROUP / 32); ++b) {         // 32 features
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int ks = b * 2 + c, wi = c * W + (b >> 1);
+                    const uint32_t wa = (b & 1) ? kw[0][wi] >> 8 : kw[0][wi], wb = (b & 1) ? kw[1][wi] >> 8 : kw[1][wi];
+                    const uint32_t a0 = a4_codes<F32, false>(wa), a1 = a4_codes<F32, false>(wb);
+                    const uint32_t a2 = a4_codes<F32, true>(wa), a3 = a4_codes<F32, true>(wb);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            uint2 q;
+                            if constexpr (Q_IN_REGS) q = qr[(ks * PARTS + part) * NT + n];
+                            else q = qf[((ks * PARTS + part) * NT + n) * 32];
+                            a4_mma(acc[n], a0, a1, a2, a3, q.x, q.y);
+                        }
+                }
+            }
+            const float sa = c4_step(ksc[0][gr]) * CODE, la = a4_low<F32>(ksc[0][gr]);
+            const float sb = c4_step(ksc[1][gr]) * CODE, lb = a4_low<F32>(ksc[1][gr]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float wa = gr == 0 ? la * qsum[n][gr][c] : fmaf(la, qsum[n][gr][c], s[n][c]);
+                    const float wb = gr == 0 ? lb * qsum[n][gr][c] : fmaf(lb, qsum[n][gr][c], s[n][2 + c]);
+                    s[n][c] = fmaf(acc[n][c], sa, wa);
+                    s[n][2 + c] = fmaf(acc[n][2 + c], sb, wb);
+                }
+            }
+        }
+
+        // what a row does not see: bits 4 n + 2 h + c
+        uint32_t hidden = 0;
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int key = key0 + g + 8 * h;
+                        bool out = key0 < 0 || key > pos[n][c] || (p.window > 0 && key <= pos[n][c] - p.window);
+                        if (!whole && !out)
+                            out = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) < 0;
+                        if (out) {
+                            s[n][2 * h + c] = -INFINITY;
+                            hidden |= 1u << (4 * n + 2 * h + c);
+                        }
+                    }
+        }
+
+        // the references move only when they have to.  (The pair's bits less its sign: steps are not negative, and a larger
+        // step has the larger bits.)
+        float most_step[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            most_step[h] = c4_step(vsc[h][0]);
+#pragma unroll
+            for (int gr = 1; gr < NG; ++gr) most_step[h] = fmaxf(most_step[h], c4_step(vsc[h][gr]));
+        }
+        bool move = false;
+        float top[NT][2], step_top[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                top[n][c] = fmaxf(s[n][c], s[n][2 + c]);
+                if constexpr (EDGE)
+                    step_top[n][c] = fmaxf((hidden >> (4 * n + c)) & 1 ? 0.f : most_step[0],
+                                           (hidden >> (4 * n + 2 + c)) & 1 ? 0.f : most_step[1]);
+                else step_top[n][c] = fmaxf(most_step[0], most_step[1]);
+                move = move || fmaf(top[n][c], factor[n][c], -off[n][c]) > eps[n][c] + 8.f || step_top[n][c] >= bound[n][c];
+            }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float m = fmaxf(off[n][c] + eps[n][c], a4_over_keys_max(top[n][c] * factor[n][c]));
+                    const float st = a4_over_keys_max(step_top[n][c]);
+                    const int e = min(max((int)(__float_as_uint(fmaxf(st, bound[n][c] * 0.5f)) >> 23) - 127, -96), 126);
+                    const float e5 = 5.f - (float)e, to = m - e5;
+                    const float r = a4_exp2(off[n][c] - to);
+                    off[n][c] = to;
+                    eps[n][c] = e5;
+                    bound[n][c] = a4_power(e + 1);
+                    sum[n][c] *= r;
+#pragma unroll
+                    for (int gr = 0; gr < NG; ++gr) lows[n][gr][c] *= r;
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        o[j][n][c] *= r;
+                        o[j][n][2 + c] *= r;
+                    }
+                }
+        }
+
+        // p, and P^T step as columns of the second product
+        uint32_t b[NG][PARTS][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float pr[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                pr[j] = a4_exp2(fmaf(s[n][j], factor[n][j & 1], -off[n][j & 1]));
+                sum[n][j & 1] += pr[j];
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                float w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = pr[j] * c4_step(vsc[j >> 1][gr]);
+                    float low = a4_low<F32>(vsc[j >> 1][gr]);
+                    if constexpr (EDGE)
+                        if ((hidden >> (4 * n + j)) & 1) w[j] = low = 0.f;       // (what nobody wrote may be no number)
+                    lows[n][gr][j & 1] = fmaf(pr[j], low, lows[n][gr][j & 1]);
+                }
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                    const uint32_t h0 = a4_half2(w[0], w[1]), h1 = a4_half2(w[2], w[3]);
+                    if constexpr (PARTS == 2) {
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                        w[0] -= f0.x; w[1] -= f0.y; w[2] -= f1.x; w[3] -= f1.y;
+                    }
+                    b[gr][part][n][0] = a4_turned(h0);
+                    b[gr][part][n][1] = a4_turned(h1);
+                }
+            }
+        }
+
+        // O^T += V^T P^T
+        const uint8_t* values = at + L::SIDE;
+        uint32_t vw[4][W];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = 2 * t + (j & 1) + 8 * (j >> 1);
+            if constexpr (D == 64) {
+                vw[j][0] = *reinterpret_cast<const uint32_t*>(values + a4_place<D>(r, g >> 2) + (g & 3) * 4);
+            } else if constexpr (D == 128) {
+                const uint2 v = *reinterpret_cast<const uint2*>(values + a4_place<D>(r, g >> 1) + (g & 1) * 8);
+                vw[j][0] = v.x; vw[j][1] = v.y;
+            } else if constexpr (D == 256) {
+                const uint4 v = *reinterpret_cast<const uint4*>(values + a4_place<D>(r, g));
+                vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
+            } else {
+#pragma unroll
+                for (int w = 0; w < W; ++w) vw[j][w] = *reinterpret_cast<const uint32_t*>(values + r * 96 + g * 12 + w * 4);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                // half words of two keys side by side: features of tiles 4w + half and 4w + 2 + half
+                uint32_t z0 = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
+                uint32_t z1 = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int m = 4 * w + 2 * u + half, gr = m * 16 / GROUP;
+                    if (u == 1) { z0 >>= 8; z1 >>= 8; }
+                    const uint32_t a0 = a4_codes<F32, false>(z0), a1 = a4_codes<F32, true>(z0);
+                    const uint32_t a2 = a4_codes<F32, false>(z1), a3 = a4_codes<F32, true>(z1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if constexpr (F32) {
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                            a4_mma(part, a0, a1, a2, a3, b[gr][1][n][0], b[gr][1][n][1]);
+                            a4_mma(part, a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) o[m][n][j] += part[j];
+                        } else {
+                            a4_mma(o[m][n], a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
+                        }
+                    }
+                }
+            }
+    };
+    int stage = 0;
+    for (int i = tile_lo + warp; i < tile_hi; i += A4_WARPS) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
+        __syncwarp();
+        const int key0 = key_of[0];
+        // the stage that was read last takes the tile after those in flight
+        fetch(ahead, stage == 0 ? L::STAGES - 1 : stage - 1, next_key, next_at);
+#pragma unroll
+        for (int s = 0; s + 2 < L::STAGES; ++s) key_of[s] = key_of[s + 1];
+        key_of[L::STAGES - 2] = whole && next_at < 0 ? -1 : next_key;
+        ahead += A4_WARPS;
+        next_at = look(ahead, next_key);
+        const uint8_t* at = smem + warp * L::RING + stage * L::STAGE;
+        stage = stage + 1 == L::STAGES ? 0 : stage + 1;
+        if (key0 < 0 || key0 + 15 > min_pos || key0 <= lowest || !whole) tile(std::true_type{}, at, key0);
+        else tile(std::false_type{}, at, key0);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the warps' results ------------------------------------------------------
+    // A column's result is o over the codes' unit (and over 16 of it where they come 16 times too large) plus its lows,
+    // relative to 2^off.
+    __syncthreads();
+    float* mine = reinterpret_cast<float*>(smem + warp * L::RING);
+    float* state = reinterpret_cast<float*>(smem + L::AT_STATE);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float l = a4_over_keys_sum(sum[n][c]);
+            float low[NG];
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) low[gr] = a4_over_keys_sum(lows[n][gr][c]);
+            const int r = n * 8 + 2 * t + c;
+            if (g == 0) {
+                state[(warp * L::ROWS + r) * 2] = off[n][c];
+                state[(warp * L::ROWS + r) * 2 + 1] = l;
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                mine[r * L::PITCH + m * 16 + g] = fmaf(o[m][n][c], CODE, low[m * 16 / GROUP]);
+                mine[r * L::PITCH + m * 16 + 8 + g] = fmaf(o[m][n][2 + c], CODE / 16.f, low[m * 16 / GROUP]);
+            }
+        }
+    __syncthreads();
+    // every row's weights of the warps, and what the block has of it
+    float* block_state = state + A4_WARPS * L::ROWS * 2;
+    if (threadIdx.x < L::ROWS) {
+        const int r = threadIdx.x;
+        float top = -3.4e38f, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) top = fmaxf(top, state[(w * L::ROWS + r) * 2]);
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) {
+            const float weight = a4_exp2(state[(w * L::ROWS + r) * 2] - top);
+            l = fmaf(state[(w * L::ROWS + r) * 2 + 1], weight, l);
+            state[(w * L::ROWS + r) * 2] = weight;
+        }
+        block_state[r * 2] = top;
+        block_state[r * 2 + 1] = l;
+    }
+    __syncthreads();
+    const int live = min(L::ROWS, n_rows - base);
+    auto of_block = [&](int i) {
+        const int r = i / D;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w)
+            v = fmaf(reinterpret_cast<const float*>(smem + w * L::RING)[i + r * (L::PITCH - D)], state[(w * L::ROWS + r) * 2], v);
+        return v;
+    };
+    auto store = [&](int i, float v) {
+        const int r = i / D, tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
+        reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + (i - r * D)] = cb_from_float<T>(v);
+    };
+    if (p.chunk_tiles > 0 && n_chunks > 1) {
+        float* to = p.partial + ((size_t)blockIdx.x * p.n_chunks + blockIdx.z) * (L::ROWS * (D + 2));
+        for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32) to[2 * L::ROWS + i] = of_block(i);
+        if (threadIdx.x < 2 * live) to[threadIdx.x] = block_state[threadIdx.x];
+        return;
+    }
+    if (p.chunk_tiles > 0 || gridDim.z == 1) {
+        for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32) {
+            const float l = block_state[(i / D) * 2 + 1];
+            store(i, l == 0.f ? 0.f : of_block(i) / l);          // (a row that sees no key: zeros)
+        }
+        return;
+    }
+    // blocks of a cluster: each takes its share of the numbers from all
+    for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32)
+        reinterpret_cast<float*>(smem)[i + i / D * (L::PITCH - D)] = of_block(i);      // (over warp 0's, which this thread alone reads)
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const uint32_t result = a4_smem(smem), states = a4_smem(block_state);
+    const int shares = gridDim.z;
+    const int per = (live * D + shares - 1) / shares;
+    for (int i = blockIdx.z * per + threadIdx.x; i < min(live * D, (int)(blockIdx.z + 1) * per); i += A4_WARPS * 32) {
+        float top = -3.4e38f, refs[8], ls[8], vals[8];
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+            refs[z] = -3.4e38f;
+            ls[z] = vals[z] = 0.f;
+            if (z < shares) {
+                uint32_t there, state_there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(result + (i + i / D * (L::PITCH - D)) * 4), "r"(z));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(state_there) : "r"(states + (i / D) * 8), "r"(z));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(vals[z]) : "r"(there));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(refs[z]), "=f"(ls[z]) : "r"(state_there));
+                top = fmaxf(top, refs[z]);
+            }
+        }
+        float v = 0.f, l = 0.f;
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+            const float weight = a4_exp2(refs[z] - top);
+            v = fmaf(vals[z], weight, v);
+            l = fmaf(ls[z], weight, l);
+        }
+        store(i, l == 0.f ? 0.f : v / l);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Shares that went through memory: one block a row tile.
+template <int D, int NT, bool F32>
+__global__ void __launch_bounds__(128) attention4_merge_kernel(const Attn4Params p) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    constexpr int ROWS = 8 * NT;
+    using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    int x = blockIdx.x;
+    const int row_tile = x % p.row_tiles;
+    x /= p.row_tiles;
+    const int kv = x % p.kv_heads;
+    x /= p.kv_heads;
+    int row0, n_rows, first, tile_lo = 0, tile_hi;
+    const int base = row_tile * ROWS;
+    if (p.picks != nullptr) {
+        row0 = x;
+        const int request = p.row_request[x];
+        first = p.positions[x];
+        n_rows = (request >= 0 && request < p.requests && first >= 0) ? p.n_rep : 0;
+        tile_hi = p.pick_count * p.page_tiles;
+    } else {
+        row0 = p.row_start[x];
+        n_rows = (row0 < 0 ? 0 : min(p.row_start[x + 1], p.rows) - row0) * p.n_rep;
+        first = p.first_pos[x];
+        if (p.window > 0) tile_lo = max(0, first + base / p.n_rep - p.window + 1) >> 4;
+        tile_hi = ((first + (min(n_rows, base + ROWS) - 1) / p.n_rep) >> 4) + 1;
+    }
+    if (base >= n_rows) return;
+    const int n = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
+    if (n <= 1) return;                          // (its block has written the rows)
+    const float* from = p.partial + (size_t)blockIdx.x * p.n_chunks * (ROWS * (D + 2));
+    const int live = min(ROWS, n_rows - base);
+    for (int i = blockIdx.y * 128 + threadIdx.x; i < live * D; i += gridDim.y * 128) {
+        const int r = i / D;
+        float top = -3.4e38f, v = 0.f, l = 0.f;
+        for (int z = 0; z < n; ++z) top = fmaxf(top, from[(size_t)z * (ROWS * (D + 2)) + 2 * r]);
+#pragma unroll 4
+        for (int z = 0; z < n; ++z) {
+            const float* one = from + (size_t)z * (ROWS * (D + 2));
+            const float weight = a4_exp2(one[2 * r] - top);
+            v = fmaf(one[2 * ROWS + i], weight, v);
+            l = fmaf(one[2 * r + 1], weight, l);
+        }
+        const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
+        reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + (i - r * D)] =
+            cb_from_float<T>(l == 0.f ? 0.f : v / l);
+    }
+}
+
+template <int D, int NG, int NT, bool F32>
+int attention4_launch(const Attn4Params& p, long long blocks, int shares, cudaStream_t stream) {
+    using L = A4Layout<D, NG, NT, F32 ? 2 : 1>;
+    static bool ready[64] = {};          // (per device; setting it twice does no harm)
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        const int rc = (int)cudaFuncSetAttribute(attention4_kernel<D, NG, NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 L::TOTAL);
+        if (rc != 0) return rc;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    const bool through_memory = p.chunk_tiles > 0;
+    const dim3 grid((unsigned)blocks, 1, (unsigned)(through_memory ? p.n_chunks : shares));
+    int rc = cb_launch_cluster(attention4_kernel<D, NG, NT, F32>, grid, dim3(A4_WARPS * 32), L::TOTAL, stream,
+                               through_memory ? 1 : shares, p);
+    if (rc == 0 && through_memory)
+        rc = cb_launch(attention4_merge_kernel<D, NT, F32>, dim3((unsigned)blocks, (8 * NT * D + 511) / 512), dim3(128), 0, stream, p);
+    return rc;
+}
+
+template <int D, int NG>
+int attention4_of(const Attn4Params& p, int dtype, int column_tiles, long long blocks, int shares, cudaStream_t stream) {
+    if (dtype == CB_F32) return attention4_launch<D, NG, 1, true>(p, blocks, shares, stream);
+    if (column_tiles == 1) return attention4_launch<D, NG, 1, false>(p, blocks, shares, stream);
+    return attention4_launch<D, NG, 2, false>(p, blocks, shares, stream);
+}
+
+}  // namespace
+
+// One file a head size (D) is built, so that a model compiles only its own.
+#define ATTENTION4_ENTRY(D)                                                                                             \
+    {                                                                                                                   \
+        if (group != 32 && group != 64 && group != 128) return CB_ERR_UNSUPPORTED;                                       \
+        if (D % group != 0 || column_tiles < 1 || column_tiles > 2 || shares < 1 || shares > 8) return CB_ERR_UNSUPPORTED; \
+        const int rows_a_tile = 8 * column_tiles;                                                                        \
+        const int row_tiles = (most_rows * n_rep + rows_a_tile - 1) / rows_a_tile;                                       \
+        const long long blocks = (long long)(picks != nullptr ? rows : requests) * kv_heads * row_tiles;                 \
+        if (blocks <= 0) return 0;                                                                                       \
+        if (blocks >= (1LL << 31) || n_chunks > 65535) return CB_ERR_UNSUPPORTED;                                        \
+        const Attn4Params p = {q, q_stride, out, out_stride, reinterpret_cast<const uint8_t*>(codes),                    \
+                               reinterpret_cast<const uint8_t*>(scales), n_pages, page_tokens, kv_heads, n_rep,          \
+                               row_start, first_pos, table, table_stride, requests, picks, pick_count, row_request,      \
+                               positions, rows, page_tokens % 16 ? 0 : page_tokens / 16,                                 \
+                               page_tokens % 16 || page_tokens == 16 ? 0u : (uint32_t)((1ull << 32) / (page_tokens / 16)) + 1u, window, scale * A4_LOG2E, row_tiles, chunk_tiles, n_chunks, partial};    \
+        const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);                                                   \
+        int rc = CB_ERR_UNSUPPORTED;                                                                                     \
+        if (group == 32) rc = attention4_of<D, D / 32>(p, dtype, column_tiles, blocks, shares, s);                       \
+        else if (group == 64) rc = attention4_of<D, D / 64>(p, dtype, column_tiles, blocks, shares, s);                  \
+        else if constexpr (D % 128 == 0) rc = attention4_of<D, D / 128>(p, dtype, column_tiles, blocks, shares, s);      \
+        if (rc == CB_ERR_UNSUPPORTED) return rc;                                                                         \
+        const int last = cb_last_error();                                                                                \
+        return rc != 0 ? rc : last;                                                                                      \
+    }

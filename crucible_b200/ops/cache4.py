@@ -1,0 +1,338 @@
+"""A paged key/value cache in 4 bits: writing it, attention over it, and picking the pages to attend to.
+
+A key or value row (one token, one kv head) is held by groups of `group` features as codes 0..15 with a bfloat16
+pair (step, low) and stands for code * step + low.  low is the group's least number rounded down to bfloat16, step
+is (largest - low) * (1 / 15) rounded to bfloat16 (0 if it is under 1e-30), the code is (x - low) * (1 / step)
+rounded to the nearest, ties to even, and held within 0..15; every operation is float32's, rounded once.  A group
+that holds a number that is not finite, or numbers further apart than float32 reaches, stands for NaN.  A number is off by at most half a
+step (and 3 % of one where the rounding of the step cuts the largest off).
+
+`rope_append4` rotates q and k of packed rows by their positions and writes k and v to the rows' places;
+`attention4` is causal grouped-query attention over what the pages hold, for single tokens, portions and whole
+prompts; `pick_pages4` chooses for every row and kv head the pages whose bounds allow the largest logits, for
+`attention4(..., picks=)` to read alone.  Pages that are to be picked keep bounds (`Pages4.new(..., bounds=True)`):
+`rope_append4` brings those of every page that it writes up to date.
+
+Everything launches on torch's current stream of the tensors' device and may be captured into a CUDA graph; what is
+allocated on the way (partial results of very long contexts, pages laid out anew for long portions) comes from
+torch's pool.  Outputs may not overlap inputs, but where a function says so.  Sums and softmax statistics are
+float32.  Page ids, positions and row numbers on the device are looked over by the kernels: a key whose table entry names no
+page of the pool is not seen, a row of a request that is none is left as it is.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from . import KernelError, _check, _code, _need_cuda, build, tensor_core
+from .quantized import _at, _one_device
+
+build.register_module("append4", ["common.cuh", "cache4.cuh"])
+build.register_module("pick4", ["common.cuh", "cache4.cuh"])
+HEAD_DIMS = (64, 128, 192, 256)
+for _dim in HEAD_DIMS:
+    build.register_module(f"attention4_{_dim}", ["common.cuh", "cache4.cuh", "attention4.cuh"])
+
+GROUPS = (32, 64, 128)
+_F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
+_FLOATS = (_F32, _BF16)
+
+
+class Pages4:
+    """A pool of pages in 4 bits: `codes` uint8 [2, pages, kv heads, page tokens, dim / 2] (keys, values), `scales`
+    bfloat16 [2, pages, kv heads, page tokens, dim / group, 2] (step, low); head sizes are multiples of 64 up to 256,
+    groups 32, 64 or 128 features that divide them.  Bytes of a row are int32 words; word (dim / 64) g + w, g < 8,
+    holds the codes of the features 64 w + 8 k + g, its bits 4n.. 4n + 3 that of k = (0, 1, 4, 5, 2, 3, 6, 7)[n].
+    `bounds`: int8 [pages, kv heads, 2, dim] (largest, least key of each feature over the tokens that a page holds)
+    with float32 `bound_scales` [pages, kv heads], or neither.  The tensors are kept, not copied."""
+
+    __slots__ = ("codes", "scales", "bounds", "bound_scales", "n_pages", "kv_heads", "page_tokens", "head_dim", "group", "device")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, bounds: Optional[torch.Tensor] = None,
+                 bound_scales: Optional[torch.Tensor] = None):
+        cs, ss = codes.shape, scales.shape
+        if len(cs) != 5 or cs[0] != 2 or codes.dtype != torch.uint8 or 2 * cs[4] not in HEAD_DIMS or not codes.is_contiguous():
+            raise KernelError("a pool's codes are contiguous uint8 [2, pages, kv heads, page tokens, dim / 2] with dim in "
+                              f"{HEAD_DIMS}, got {codes.dtype} {list(cs)}")
+        dim = 2 * cs[4]
+        if (len(ss) != 6 or ss[:4] != cs[:4] or ss[5] != 2 or scales.dtype != _BF16 or not scales.is_contiguous()
+                or ss[4] < 1 or dim % ss[4] or dim // ss[4] not in GROUPS):
+            raise KernelError("a pool's scales are contiguous bfloat16 [2, pages, kv heads, page tokens, dim / group, 2] with "
+                              f"groups of {GROUPS}, got {scales.dtype} {list(ss)} for codes {list(cs)}")
+        if min(cs) < 1:
+            raise KernelError(f"a pool has pages, kv heads and tokens, got {list(cs)}")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise KernelError("a pool's codes and scales begin on multiples of 16 bytes")
+        if (bounds is None) != (bound_scales is None):
+            raise KernelError("bounds come with their scales")
+        if bounds is not None and not (
+                bounds.dtype == torch.int8 and tuple(bounds.shape) == (cs[1], cs[2], 2, dim) and bounds.is_contiguous()
+                and bounds.data_ptr() % 16 == 0 and bound_scales.dtype == _F32
+                and tuple(bound_scales.shape) == (cs[1], cs[2]) and bound_scales.is_contiguous()):
+            raise KernelError(f"bounds are contiguous int8 [{cs[1]}, {cs[2]}, 2, {dim}] with float32 scales [{cs[1]}, {cs[2]}], "
+                              f"got {bounds.dtype} {list(bounds.shape)} and {bound_scales.dtype} {list(bound_scales.shape)}")
+        _one_device(codes, scales, bounds, bound_scales)
+        self.codes, self.scales, self.bounds, self.bound_scales = codes, scales, bounds, bound_scales
+        self.n_pages, self.kv_heads, self.page_tokens, self.head_dim = cs[1], cs[2], cs[3], dim
+        self.group, self.device = dim // ss[4], codes.get_device()
+
+    @classmethod
+    def new(cls, n_pages: int, page_tokens: int, kv_heads: int, head_dim: int, group: int = 64, bounds: bool = False,
+            device="cuda:0") -> "Pages4":
+        """Pages of zeros (every key and value stands for 0)."""
+        if head_dim not in HEAD_DIMS or group not in GROUPS or head_dim % group:
+            raise KernelError(f"pages in 4 bits take heads of {HEAD_DIMS} features in groups of {GROUPS} that divide them, "
+                              f"got {head_dim} and {group}")
+        if min(n_pages, page_tokens, kv_heads) < 1:
+            raise KernelError("a pool has pages, kv heads and tokens")
+        shape = (2, n_pages, kv_heads, page_tokens)
+        kept = (torch.zeros(n_pages, kv_heads, 2, head_dim, dtype=torch.int8, device=device),
+                torch.zeros(n_pages, kv_heads, device=device)) if bounds else ()
+        return cls(torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(*shape, head_dim // group, 2, dtype=_BF16, device=device), *kept)
+
+    def values(self, dtype: torch.dtype = _F32):
+        """What the pool stands for: (keys, values), each [pages, kv heads, page tokens, dim]."""
+        if dtype not in _FLOATS:
+            raise KernelError(f"pages are read back as float32 or bfloat16, not {dtype}")
+        _need_cuda(self.codes)
+        out = torch.empty(2, self.n_pages, self.kv_heads, self.page_tokens, self.head_dim, dtype=dtype, device=self.codes.device)
+        lib = build.load("append4")
+        _check(_at(self.device, lib.cb_values4, self.codes.data_ptr(), self.scales.data_ptr(), self.group,
+                   2 * self.n_pages * self.kv_heads * self.page_tokens, self.head_dim, out.data_ptr(), _code(dtype)),
+               "values in 4 bits")
+        return out[0], out[1]
+
+    def bound_values(self) -> torch.Tensor:
+        """What the bounds stand for: float32 [pages, kv heads, 2, dim]."""
+        if self.bounds is None:
+            raise KernelError("these pages keep no bounds")
+        return self.bounds.float() * self.bound_scales[..., None, None]
+
+
+class Batch:
+    """The packed rows of a step.  On the device, int32: `positions` [rows] and `row_request` [rows] (a row's position in
+    its request, its request's number), `row_start` [requests + 1] and `first_pos` [requests] (where a request's
+    rows begin, and the position of the first), `table` [requests, pages] (which page of the pool holds a
+    request's tokens i * page_tokens onwards).  On the host: how many tokens of every request are
+    `new_tokens`, its rows in this step, and `held_tokens`, before them.  A request's rows are consecutive and
+    so are their positions.  Rows behind the last request's are left alone.
+
+    A call that is captured into a graph may be replayed with other numbers on the device, as long as no request brings more rows
+    than the most that the host was told of and the same leading requests bring one; the kernels are shaped by the host's
+    numbers, the results follow the device's."""
+
+    __slots__ = ("positions", "row_request", "row_start", "first_pos", "table", "new_tokens", "held_tokens", "requests",
+                 "most_new", "reach", "lead", "device", "checked")
+
+    def __init__(self, positions, row_request, row_start, first_pos, table, new_tokens: Sequence[int],
+                 held_tokens: Sequence[int], reach: Optional[int] = None):
+        self.positions, self.row_request, self.row_start = positions, row_request, row_start
+        self.first_pos, self.table = first_pos, table
+        self.new_tokens, self.held_tokens = new_tokens, held_tokens
+        self.requests = requests = len(new_tokens)
+        dev = positions.get_device()
+        self.device = dev
+        ts, rows = table.shape, positions.shape
+        if not (requests > 0 and len(held_tokens) == requests and len(ts) == 2 and ts[0] == requests and ts[1] > 0
+                and len(rows) == 1 and row_request.shape == rows and row_start.shape == (requests + 1,)
+                and first_pos.shape == (requests,)
+                and positions.dtype is _I32 and row_request.dtype is _I32 and row_start.dtype is _I32
+                and first_pos.dtype is _I32 and table.dtype is _I32
+                and positions.is_contiguous() and row_request.is_contiguous() and row_start.is_contiguous()
+                and first_pos.is_contiguous() and table.is_contiguous()
+                and dev == row_request.get_device() == row_start.get_device() == first_pos.get_device() == table.get_device()):
+            self._refuse()
+        self.most_new = max(new_tokens)
+        if self.most_new < 1 or min(new_tokens) < 1 or min(held_tokens) < 0:
+            raise KernelError("a batch's requests bring at least one token each, and hold none or more")
+        self.reach = max(map(int.__add__, new_tokens, held_tokens)) if reach is None else reach
+        lead = 0
+        for n in new_tokens:
+            if n != 1:
+                break
+            lead += 1
+        self.lead = lead
+
+    def _refuse(self):
+        t = {"positions": self.positions, "row_request": self.row_request, "row_start": self.row_start,
+             "first_pos": self.first_pos, "table": self.table}
+        _one_device(*t.values())
+        raise KernelError("a batch takes contiguous int32 tensors positions [rows], row_request [rows], row_start [requests + 1], "
+                          "first_pos [requests] and table [requests, pages], and two host lists with a number a request; got "
+                          + ", ".join(f"{n} {v.dtype} {list(v.shape)}" for n, v in t.items())
+                          + f", {len(self.new_tokens)} and {len(self.held_tokens)} numbers")
+
+    @classmethod
+    def of(cls, ctx, group: int) -> "Batch":
+        """The step of a `StepContext`, over the pages of one of its cache groups."""
+        made = ctx.__dict__.setdefault("_batches4", {})
+        batch = made.get(group)
+        if batch is None:
+            host = ctx.host
+            batch = made[group] = cls(ctx.positions, ctx.row_request, ctx.req_row_start, ctx.req_first_pos,
+                                      ctx.block_table(group), host.new_tokens, host.first_pos, host.context_bucket)
+        return batch
+
+
+def _rows_of(t: torch.Tensor, what: str, width: int, dtype=None) -> None:
+    if t.dim() != 2 or t.shape[1] != width or t.dtype not in _FLOATS or (dtype is not None and t.dtype != dtype):
+        names = "float32 or bfloat16" if dtype is None else str(dtype).replace("torch.", "")
+        raise KernelError(f"{what}: {names} rows [T, {width}] are taken, got {t.dtype} {list(t.shape)}")
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        raise KernelError(f"{what}: rows must be contiguous and not overlap")
+
+
+def _step_checks(what: str, rows: int, batch: Batch, pages: Pages4, *tensors) -> None:
+    if rows < batch.positions.shape[0]:
+        raise KernelError(f"{what}: the batch has {batch.positions.shape[0]} rows, the tensors {rows}")
+    _need_cuda(*tensors, batch.positions, pages.codes)
+    _one_device(pages.codes, batch.positions, *tensors)
+
+
+def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                 batch: Batch, pages: Pages4, neighbours: bool = False) -> None:
+    """Rows [q : n_heads | k : kv heads | v : kv heads] of heads side by side: q rotated by the rows' positions goes to `q`
+    (which may be the first columns of `qkv` themselves), k rotated and v as it is go to the rows' places in the
+    pages, in 4 bits.  `cos`, `sin`: float32 [positions, r / 2], the angles of every position; the first r
+    features of a head turn, (a, b) -> (a cos - b sin, a sin + b cos), feature i with i + r / 2 or (`neighbours`)
+    2 i with 2 i + 1.  None: nothing turns.  Rows whose position is beyond the tables are left out.  No two rows are of one place."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    width = (n_heads + 2 * kv) * dim
+    if n_heads < 1:
+        raise KernelError("rope_append4: a positive number of query heads is needed")
+    _rows_of(qkv, "rope_append4 rows", width)
+    _rows_of(q, "rope_append4 queries", n_heads * dim, qkv.dtype)
+    if (cos is None) != (sin is None):
+        raise KernelError("rope_append4: cos and sin come together")
+    rotary = 0
+    if cos is not None:
+        rotary = 2 * cos.shape[-1]
+        if (cos.dim() != 2 or cos.dtype != _F32 or sin.dtype != _F32 or sin.shape != cos.shape or not cos.is_contiguous()
+                or not sin.is_contiguous() or rotary > dim):
+            raise KernelError(f"rope_append4: the tables are contiguous float32 [positions, r / 2] with r at most {dim}, got "
+                              f"{cos.dtype} {list(cos.shape)} and {sin.dtype} {list(sin.shape)}")
+    _step_checks("rope_append4", min(qkv.shape[0], q.shape[0]), batch, pages, qkv, q, cos, sin)
+    lib = build.load("append4")
+    code = _at(pages.device, lib.cb_append4, qkv.data_ptr(), _code(qkv.dtype), qkv.stride(0), q.data_ptr(), q.stride(0),
+               cos.data_ptr() if rotary else 0, sin.data_ptr() if rotary else 0, rotary, cos.shape[0] if rotary else 0,
+               1 if neighbours else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
+               batch.table.shape[1], batch.requests, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
+               pages.page_tokens, n_heads, kv, dim, pages.group, batch.positions.shape[0],
+               pages.bounds.data_ptr() if pages.bounds is not None else 0,
+               pages.bound_scales.data_ptr() if pages.bounds is not None else 0)
+    _check(code, "rope_append4")
+
+
+def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, picks: torch.Tensor, first: int = 1,
+                last: int = 2) -> None:
+    """For every row and kv head `picks.shape[2]` of the request's pages up to the row's own, by their place in the table
+    and in ascending order, -1 behind them where there are fewer: the `first` first and `last` last always, the others
+    by the largest bound on a logit that a head of the group has in them, of equal ones the first.  `picks`: int32
+    [rows, kv heads, count].  A query is rounded to 8 bits for it (largest magnitude 127), as the bounds are."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    _rows_of(q, "pick_pages4 queries", n_heads * dim)
+    if n_heads < 1 or n_heads % kv:
+        raise KernelError(f"pick_pages4: {n_heads} query heads do not share {kv} kv heads evenly")
+    if pages.bounds is None:
+        raise KernelError("pick_pages4: these pages keep no bounds")
+    rows = batch.positions.shape[0]
+    _picks_ok("pick_pages4", picks, rows, kv)
+    if first < 0 or last < 1 or first + last > picks.shape[2]:
+        raise KernelError(f"pick_pages4: of {picks.shape[2]} pages the first {first} and the last {last} cannot always be "
+                          "among them (the row's own page has to be)")
+    _step_checks("pick_pages4", q.shape[0], batch, pages, q, picks)
+    # scores are held for as many pages as the longest context may have
+    most = min(batch.table.shape[1], -(-batch.reach // pages.page_tokens))
+    lib = build.load("pick4")
+    code = _at(pages.device, lib.cb_pick4, q.data_ptr(), _code(q.dtype), q.stride(0), batch.positions.data_ptr(),
+               batch.row_request.data_ptr(), batch.table.data_ptr(), batch.table.shape[1], batch.requests,
+               pages.bounds.data_ptr(), pages.bound_scales.data_ptr(), pages.n_pages, pages.page_tokens, n_heads // kv, kv,
+               dim, rows, picks.data_ptr(), picks.shape[2], first, last, most, _pick_shares(rows * kv, most))
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"pick_pages4 takes tables of up to {(lib.cb_pick4_room() - n_heads // kv * (2 * dim + 4)) // 4} pages "
+                          f"a request here, got {most}; longer pages make shorter tables")
+    _check(code, "pick_pages4")
+
+
+def _pick_shares(blocks: int, pages: int) -> int:
+    """Blocks of a cluster that score a row's pages: as many as fill the SMs, none with fewer than 128 pages."""
+    shares = 1
+    while shares < 8 and blocks * shares * 2 <= 2 * tensor_core.N_SMS and pages >= 256 * shares:
+        shares *= 2
+    return shares
+
+
+def _picks_ok(what: str, picks: torch.Tensor, rows: int, kv_heads: int) -> None:
+    if (picks.dim() != 3 or picks.dtype != _I32 or not picks.is_contiguous() or picks.shape[0] < rows
+            or picks.shape[1] != kv_heads or picks.shape[2] < 1):
+        raise KernelError(f"{what}: the picks are contiguous int32 [{rows}, {kv_heads}, count], got {picks.dtype} {list(picks.shape)}")
+
+
+def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, batch: Batch, pages: Pages4,
+               window: Optional[int] = None, picks: Optional[torch.Tensor] = None) -> None:
+    """out = softmax(scale q . k) v: every row over the keys of its request up to its own position (the last `window` of
+    them), heads of a group over the same kv head (head h over h // (n_heads / kv heads)).  `q`, `out`: rows [T,
+    n_heads * dim] of one type.  A row that sees no key is zero.  `picks` (int32 [rows, kv heads, count], as
+    `pick_pages4` leaves them): the pages of the table that a row attends to, each named once, -1 for none; every row is then
+    walked by itself, so that this is for a few rows a request; page sizes are multiples of 16, and there is no window."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    _rows_of(q, "attention4 queries", n_heads * dim)
+    _rows_of(out, "attention4 output", n_heads * dim, q.dtype)
+    if n_heads < 1 or n_heads % kv:
+        raise KernelError(f"attention4: {n_heads} query heads do not share {kv} kv heads evenly")
+    if window is not None and window < 1:
+        raise KernelError(f"attention4: a window is positive, got {window}")
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"attention4: the scale is a positive number, got {scale}")
+    rows = batch.positions.shape[0]
+    if picks is not None:
+        _picks_ok("attention4", picks, rows, kv)
+        if window is not None or pages.page_tokens % 16:
+            raise KernelError("attention4: picks go with pages of a multiple of 16 tokens and without a window")
+    _step_checks("attention4", min(q.shape[0], out.shape[0]), batch, pages, q, out, picks)
+    _walk(q, out, n_heads, scale, batch, pages, window, picks, batch.requests, batch.most_new, 0)
+
+
+_RESIDENT = 4 * tensor_core.N_SMS     # blocks of one column tile that the SMs hold at once
+
+
+def _shares(blocks: int, tiles: int) -> tuple:
+    """(blocks of a cluster, tiles a share through memory or 0, shares): how the keys of a row tile are dealt, by the
+    launch's blocks and the most tiles of 16 keys that a row sees."""
+    want = max(1, min(_RESIDENT // max(1, blocks), tiles // 8))
+    if want <= 8:
+        return 1 << (want.bit_length() - 1), 0, 1
+    chunk = -(-tiles // want)
+    return 1, chunk, -(-tiles // chunk)
+
+
+def _walk(q, out, n_heads, scale, batch, pages, window, picks, requests, most_new, first) -> None:
+    """The kernel that walks the cache as it lies, for `requests` of the batch's requests from `first` on."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    n_rep, f32 = n_heads // kv, q.dtype is _F32
+    most_rows = 1 if picks is not None else most_new
+    columns = 1 if f32 or most_rows * n_rep <= 8 else 2
+    row_tiles = -(-most_rows * n_rep // (8 * columns))
+    rows = batch.positions.shape[0]
+    blocks = (rows if picks is not None else requests) * kv * row_tiles
+    if picks is not None:
+        tiles = picks.shape[2] * pages.page_tokens // 16
+    else:
+        tiles = -(-(batch.reach if window is None else min(batch.reach, window + most_new)) // 16) + 1
+    shares, chunk, chunks = _shares(blocks, tiles)
+    partial = None
+    if chunk:
+        partial = torch.empty(blocks * chunks * 8 * columns * (dim + 2), dtype=_F32, device=q.device)
+    lib = build.load(f"attention4_{dim}")
+    code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),
+               pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv, n_rep, pages.group,
+               batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first,
+               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1], requests,
+               picks.data_ptr() if picks is not None else 0, picks.shape[2] if picks is not None else 0,
+               batch.row_request.data_ptr(), batch.positions.data_ptr(), rows, most_rows, window or 0, scale, columns,
+               shares, chunk, chunks, partial.data_ptr() if partial is not None else 0)
+    if code == build.UNSUPPORTED:
+        raise KernelError(f"attention4: {blocks} blocks of rows are more than a launch takes")
+    _check(code, "attention4")
