@@ -34,7 +34,7 @@ struct AppendParams {
     long long q_stride;
     const float* cos_t;
     const float* sin_t;
-    int rotary, n_positions, neighbours;
+    int rotary, n_positions, neighbours, write;
     const int* positions;
     const int* row_request;
     const int* table;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) append4_kernel(const AppendParams p) {
     cb_pdl_wait();
     constexpr int NI = D / 32, W = D / 64, NG = D / GROUP;
     const int lane = threadIdx.x & 31;
-    const int heads = p.n_heads + 2 * p.kv_heads;
+    const int heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0);
     const long long items = (long long)p.rows * heads;
     for (long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * 8) {
         const int row = (int)(item / heads), head = (int)(item - (long long)row * heads);
@@ -318,7 +318,7 @@ int append_of(const AppendParams& p, int dtype, cudaStream_t stream) {
     int rc;
     if (dtype == CB_F32) rc = cb_launch(append4_kernel<D, GROUP, float>, grid, dim3(256), 0, stream, p);
     else rc = cb_launch(append4_kernel<D, GROUP, __nv_bfloat16>, grid, dim3(256), 0, stream, p);
-    if (rc == 0 && p.bounds != nullptr)
+    if (rc == 0 && p.write && p.bounds != nullptr)
         rc = cb_launch(bounds4_kernel<D>, dim3((unsigned)p.rows * p.kv_heads), dim3(4 * D), 0, stream, p, GROUP);
     return rc;
 }
@@ -335,12 +335,12 @@ int append_dim(const AppendParams& p, int group, int dtype, cudaStream_t stream)
 }  // namespace
 
 CB_EXPORT int cb_append4(const void* qkv, int dtype, long long qkv_stride, void* q, long long q_stride, const float* cos_t,
-                         const float* sin_t, int rotary, int n_positions, int neighbours, const int* positions,
+                         const float* sin_t, int rotary, int n_positions, int neighbours, int write, const int* positions,
                          const int* row_request, const int* table, int table_stride, int n_requests, void* codes,
                          void* scales, int n_pages, int page_tokens, int n_heads, int kv_heads, int head_dim, int group,
                          int rows, void* bounds, float* bound_scales, void* stream) {
     if (rows <= 0) return 0;
-    AppendParams p = {qkv, qkv_stride, q, q_stride, cos_t, sin_t, rotary, n_positions, neighbours, positions, row_request,
+    AppendParams p = {qkv, qkv_stride, q, q_stride, cos_t, sin_t, rotary, n_positions, neighbours, write, positions, row_request,
                       table, table_stride, n_requests, reinterpret_cast<uint32_t*>(codes), reinterpret_cast<uint32_t*>(scales),
                       n_pages, page_tokens, n_heads, kv_heads, rows, reinterpret_cast<int8_t*>(bounds), bound_scales};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -37,6 +37,10 @@ def _add_engine_options(p):
     p.add_argument("--kv-pages", type=int, default=None,
                    help="KV pages; default: enough for max-batch full-context sequences")
     p.add_argument("--page-tokens", type=int, default=16, help="tokens per KV page")
+    p.add_argument("--cache-group", type=int, default=None, choices=[32, 64, 128],
+                   help="keep keys and values in 4 bits, by groups of so many features")
+    p.add_argument("--attend-pages", type=int, default=None,
+                   help="with --cache-group: decoded tokens attend to so many pages of their context")
     p.add_argument("--prefill-chunk-tokens", type=int, default=None,
                    help="cap on one request's prompt tokens per scheduler step")
     p.add_argument("--prefill-token-budget", type=int, default=1024,
@@ -51,7 +55,7 @@ def cmd_generate(args) -> int:
               page_tokens=args.page_tokens, prefill_token_budget=args.prefill_token_budget,
               prefill_chunk_tokens=args.prefill_chunk_tokens,
               max_prefill_requests=args.max_prefill_requests, graph=args.graph,
-              profile=args.profile)
+              profile=args.profile, cache_group=args.cache_group, attend_pages=args.attend_pages)
     vocab = llm.config.vocab_size
     if args.prompt_ids is not None:
         prompts = [_ids(p) for p in args.prompt_ids]

@@ -53,6 +53,8 @@ class CacheStorage:
     Inside a page each KV head's tokens are contiguous (page_tokens * head_dim
     elements in a row), so a head's keys are read in long runs."""
 
+    in_4_bits = False
+
     def __init__(self, n_slots: int, n_pages: int, page_tokens: int, kv_heads: int,
                  head_dim: int, dtype: torch.dtype, device, value_dim: Optional[int] = None,
                  values_are_keys: bool = False):
@@ -92,6 +94,26 @@ class CacheStorage:
 
     def values(self, slot: int) -> torch.Tensor:
         return self._slot(slot)[1]
+
+
+class CacheStorage4:
+    """Device pages of one cache group in 4 bits (`ops.cache4`): a pool a slot, keys and values of one size.
+    `attend_pages`: how many pages a request that brings a single token attends to (None: all)."""
+
+    in_4_bits = True
+
+    def __init__(self, n_slots: int, n_pages: int, page_tokens: int, kv_heads: int, head_dim: int, group: int, device,
+                 attend_pages: Optional[int] = None):
+        from ..ops import cache4
+        self.page_tokens, self.n_pages, self.kv_heads = page_tokens, n_pages, kv_heads
+        self.head_dim = self.value_dim = head_dim
+        self.values_are_keys = False
+        self.attend_pages = attend_pages
+        self._slots = [cache4.Pages4.new(n_pages, page_tokens, kv_heads, head_dim, group, bounds=attend_pages is not None,
+                                         device=device) for _ in range(n_slots)]
+
+    def pages(self, slot: int):
+        return self._slots[slot]
 
 
 class Scratch:

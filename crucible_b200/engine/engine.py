@@ -25,7 +25,7 @@ from ..cache import pages as cache_codes
 from ..config.registry import load_config
 from ..models.decoder import DecoderModel
 from ..weights.loader import load_weights
-from .context import CacheStorage, HostStep, Scratch, StepContext, StepLayout
+from .context import CacheStorage, CacheStorage4, HostStep, Scratch, StepContext, StepLayout
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
            "float32": torch.float32, "fp32": torch.float32, "f32": torch.float32}
@@ -97,6 +97,10 @@ class EngineOptions:
     profile: bool = False                 # CUDA events around every part's forward; steps run eagerly
     max_context: Optional[int] = None     # most tokens of a request; default: the model's limit, or,
                                           # for a design that names none, what the page pool holds
+    cache_group: Optional[int] = None     # keys and values in 4 bits, by groups of so many features (32, 64
+                                          # or 128); None: in the engine's dtype
+    attend_pages: Optional[int] = None    # with cache_group: a request that brings one token attends to so
+                                          # many of its pages, the first, the last two and the others by a bound on their logits
 
 
 class Engine:
@@ -140,10 +144,7 @@ class Engine:
         # A table entry whose page the window has passed and given back names it, so a
         # kernel that loads whole tiles of keys reads zeros there (every such key is masked)
         # and never another request's data.
-        self.storages = [CacheStorage(len(g.layers), n_pages + 1, o.page_tokens, g.need.kv_heads,
-                                      g.need.head_dim, self.dtype, self.device,
-                                      value_dim=g.need.value_dim,
-                                      values_are_keys=g.need.values_are_keys) for g in groups]
+        self.storages = [self._storage(g, n_pages + 1) for g in groups]
         self.null_page = n_pages
         self.table_strides = tuple(ctx_pages for _ in groups)
         # The manager keeps every live request's table in the form that goes to the device
@@ -175,6 +176,27 @@ class Engine:
         self._failures_seen = tensor_core.FAILURES[0]
         self._shapes_seen = {}
         self._packer = _Packer(self.table_strides)
+
+    def _storage(self, group, n_pages: int):
+        o, need = self.options, group.need
+        if o.cache_group is None:
+            if o.attend_pages is not None:
+                raise ValueError("attend_pages goes with cache_group: only pages in 4 bits keep the bounds that pages are picked by")
+            return CacheStorage(len(group.layers), n_pages, o.page_tokens, need.kv_heads, need.head_dim, self.dtype, self.device,
+                                value_dim=need.value_dim, values_are_keys=need.values_are_keys)
+        mixers = [self.model.layers[i].mixer for i in group.layers]
+        for mixer in mixers:
+            why = mixer.refuses_cache4(o.cache_group)
+            if why is not None:
+                raise ValueError(f"cache_group: {why}")
+        if o.attend_pages is not None and (o.attend_pages < 3 or o.page_tokens % 16 or need.window is not None):
+            raise ValueError("attend_pages takes 3 pages or more, of a multiple of 16 tokens, and attention without a window; got "
+                             f"{o.attend_pages} pages of {o.page_tokens} and a window of {need.window}")
+        for mixer in mixers:
+            # (long portions are attended to over pages laid out anew, whose size follows the contexts)
+            mixer.graph_safe_prompt_steps = False
+        return CacheStorage4(len(group.layers), n_pages, o.page_tokens, need.kv_heads, need.head_dim, o.cache_group, self.device,
+                             attend_pages=o.attend_pages)
 
     META_RING = 4
 

@@ -5,6 +5,8 @@ contract).  Option names and meanings follow the reference's command line where
 it has them (`engine/src/main.rs:130-160`, `:476-497`): `max_batch`, `kv_pages`,
 `prefill_chunk_tokens`, `prefill_token_budget`, `max_prefill_requests`, `graph`;
 `profile=True` attributes device time to the model's parts (`engine/profile.py`).
+`cache_group=64` keeps keys and values in 4 bits, `attend_pages=N` with it lets a request that brings one token attend
+to N of its pages (`engine/engine.py`).
 """
 from __future__ import annotations
 
@@ -21,10 +23,11 @@ class LLM:
                  max_batch: int = 16, kv_pages: Optional[int] = None, page_tokens: int = 16,
                  prefill_token_budget: int = 1024, prefill_chunk_tokens: Optional[int] = None,
                  max_prefill_requests: Optional[int] = None, graph: bool = True,
-                 profile: bool = False):
+                 profile: bool = False, cache_group: Optional[int] = None, attend_pages: Optional[int] = None):
         self.engine = Engine(model, EngineOptions(dtype=dtype, page_tokens=page_tokens,
                                                   n_pages=kv_pages, max_requests=max_batch,
-                                                  device=device, graph=graph, profile=profile))
+                                                  device=device, graph=graph, profile=profile,
+                                                  cache_group=cache_group, attend_pages=attend_pages))
         self.scheduler_options = SchedulerOptions(
             max_batch=max_batch, prefill_token_budget=prefill_token_budget,
             prefill_chunk_tokens=prefill_chunk_tokens, max_prefill_requests=max_prefill_requests)

@@ -192,12 +192,13 @@ def _step_checks(what: str, rows: int, batch: Batch, pages: Pages4, *tensors) ->
 
 
 def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
-                 batch: Batch, pages: Pages4, neighbours: bool = False) -> None:
+                 batch: Batch, pages: Pages4, neighbours: bool = False, write: bool = True) -> None:
     """Rows [q : n_heads | k : kv heads | v : kv heads] of heads side by side: q rotated by the rows' positions goes to `q`
     (which may be the first columns of `qkv` themselves), k rotated and v as it is go to the rows' places in the
     pages, in 4 bits.  `cos`, `sin`: float32 [positions, r / 2], the angles of every position; the first r
     features of a head turn, (a, b) -> (a cos - b sin, a sin + b cos), feature i with i + r / 2 or (`neighbours`)
-    2 i with 2 i + 1.  None: nothing turns.  Rows whose position is beyond the tables are left out.  No two rows are of one place."""
+    2 i with 2 i + 1.  None: nothing turns.  Rows whose position is beyond the tables are left out.  No two rows are of one place.
+    `write` False: q alone (the pages hold the rows already)."""
     dim, kv = pages.head_dim, pages.kv_heads
     width = (n_heads + 2 * kv) * dim
     if n_heads < 1:
@@ -217,7 +218,7 @@ def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional
     lib = build.load("append4")
     code = _at(pages.device, lib.cb_append4, qkv.data_ptr(), _code(qkv.dtype), qkv.stride(0), q.data_ptr(), q.stride(0),
                cos.data_ptr() if rotary else 0, sin.data_ptr() if rotary else 0, rotary, cos.shape[0] if rotary else 0,
-               1 if neighbours else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
+               1 if neighbours else 0, 1 if write else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
                batch.table.shape[1], batch.requests, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, n_heads, kv, dim, pages.group, batch.positions.shape[0],
                pages.bounds.data_ptr() if pages.bounds is not None else 0,
@@ -230,15 +231,16 @@ def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, pick
     """For every row and kv head `picks.shape[2]` of the request's pages up to the row's own, by their place in the table
     and in ascending order, -1 behind them where there are fewer: the `first` first and `last` last always, the others
     by the largest bound on a logit that a head of the group has in them, of equal ones the first.  `picks`: int32
-    [rows, kv heads, count].  A query is rounded to 8 bits for it (largest magnitude 127), as the bounds are."""
+    [rows, kv heads, count], or [n, ..] for the first n rows alone.  A query is rounded to 8 bits for it (largest magnitude
+    127), as the bounds are."""
     dim, kv = pages.head_dim, pages.kv_heads
     _rows_of(q, "pick_pages4 queries", n_heads * dim)
     if n_heads < 1 or n_heads % kv:
         raise KernelError(f"pick_pages4: {n_heads} query heads do not share {kv} kv heads evenly")
     if pages.bounds is None:
         raise KernelError("pick_pages4: these pages keep no bounds")
-    rows = batch.positions.shape[0]
-    _picks_ok("pick_pages4", picks, rows, kv)
+    _picks_ok("pick_pages4", picks, kv)
+    rows = min(picks.shape[0], batch.positions.shape[0])
     if first < 0 or last < 1 or first + last > picks.shape[2]:
         raise KernelError(f"pick_pages4: of {picks.shape[2]} pages the first {first} and the last {last} cannot always be "
                           "among them (the row's own page has to be)")
@@ -264,10 +266,10 @@ def _pick_shares(blocks: int, pages: int) -> int:
     return shares
 
 
-def _picks_ok(what: str, picks: torch.Tensor, rows: int, kv_heads: int) -> None:
-    if (picks.dim() != 3 or picks.dtype != _I32 or not picks.is_contiguous() or picks.shape[0] < rows
-            or picks.shape[1] != kv_heads or picks.shape[2] < 1):
-        raise KernelError(f"{what}: the picks are contiguous int32 [{rows}, {kv_heads}, count], got {picks.dtype} {list(picks.shape)}")
+def _picks_ok(what: str, picks: torch.Tensor, kv_heads: int) -> None:
+    if (picks.dim() != 3 or picks.dtype != _I32 or not picks.is_contiguous() or picks.shape[1] != kv_heads
+            or min(picks.shape) < 1):
+        raise KernelError(f"{what}: the picks are contiguous int32 [rows, {kv_heads}, count], got {picks.dtype} {list(picks.shape)}")
 
 
 def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, batch: Batch, pages: Pages4,
@@ -276,7 +278,8 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     them), heads of a group over the same kv head (head h over h // (n_heads / kv heads)).  `q`, `out`: rows [T,
     n_heads * dim] of one type.  A row that sees no key is zero.  `picks` (int32 [rows, kv heads, count], as
     `pick_pages4` leaves them): the pages of the table that a row attends to, each named once, -1 for none; every row is then
-    walked by itself, so that this is for a few rows a request; page sizes are multiples of 16, and there is no window."""
+    walked by itself, so that this is for a few rows a request; page sizes are multiples of 16, and there is no window.
+    Picks of the first n rows alone are for the first n requests, which bring one row each; the others attend to all."""
     dim, kv = pages.head_dim, pages.kv_heads
     _rows_of(q, "attention4 queries", n_heads * dim)
     _rows_of(out, "attention4 output", n_heads * dim, q.dtype)
@@ -287,12 +290,19 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention4: the scale is a positive number, got {scale}")
     rows = batch.positions.shape[0]
+    behind = 0
     if picks is not None:
-        _picks_ok("attention4", picks, rows, kv)
+        _picks_ok("attention4", picks, kv)
         if window is not None or pages.page_tokens % 16:
             raise KernelError("attention4: picks go with pages of a multiple of 16 tokens and without a window")
+        behind = picks.shape[0]
+        if behind < rows and behind > batch.lead:
+            raise KernelError(f"attention4: picks of {behind} of {rows} rows, but only the first {batch.lead} requests bring one row")
     _step_checks("attention4", min(q.shape[0], out.shape[0]), batch, pages, q, out, picks)
-    _walk(q, out, n_heads, scale, batch, pages, window, picks, batch.requests, batch.most_new, 0)
+    if picks is not None:
+        _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
+    if behind < rows:
+        _walk(q, out, n_heads, scale, batch, pages, window, None, behind, batch.requests)
 
 
 _RESIDENT = 4 * tensor_core.N_SMS     # blocks of one column tile that the SMs hold at once
@@ -308,19 +318,21 @@ def _shares(blocks: int, tiles: int) -> tuple:
     return 1, chunk, -(-tiles // chunk)
 
 
-def _walk(q, out, n_heads, scale, batch, pages, window, picks, requests, most_new, first) -> None:
-    """The kernel that walks the cache as it lies, for `requests` of the batch's requests from `first` on."""
+def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
+    """The kernel that walks the cache as it lies: for the requests first .. last - 1 of the batch, or for the rows that
+    have picks."""
     dim, kv = pages.head_dim, pages.kv_heads
     n_rep, f32 = n_heads // kv, q.dtype is _F32
-    most_rows = 1 if picks is not None else most_new
-    columns = 1 if f32 or most_rows * n_rep <= 8 else 2
-    row_tiles = -(-most_rows * n_rep // (8 * columns))
     rows = batch.positions.shape[0]
-    blocks = (rows if picks is not None else requests) * kv * row_tiles
     if picks is not None:
+        most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
     else:
-        tiles = -(-(batch.reach if window is None else min(batch.reach, window + most_new)) // 16) + 1
+        most_rows, blocks = max(batch.new_tokens[first:last]), last - first
+        reach = batch.reach if window is None else min(batch.reach, window + most_rows)
+        tiles = -(-reach // 16) + (window is not None)
+    columns = 1 if f32 or most_rows * n_rep <= 8 else 2
+    blocks *= kv * -(-most_rows * n_rep // (8 * columns))
     shares, chunk, chunks = _shares(blocks, tiles)
     partial = None
     if chunk:
@@ -329,9 +341,11 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, requests, most_ne
     code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),
                pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv, n_rep, pages.group,
                batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first,
-               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1], requests,
+               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1],
+               batch.requests if picks is not None else last - first,
                picks.data_ptr() if picks is not None else 0, picks.shape[2] if picks is not None else 0,
-               batch.row_request.data_ptr(), batch.positions.data_ptr(), rows, most_rows, window or 0, scale, columns,
+               batch.row_request.data_ptr(), batch.positions.data_ptr(),
+               rows if picks is None else min(rows, picks.shape[0]), most_rows, window or 0, scale, columns,
                shares, chunk, chunks, partial.data_ptr() if partial is not None else 0)
     if code == build.UNSUPPORTED:
         raise KernelError(f"attention4: {blocks} blocks of rows are more than a launch takes")

@@ -17,6 +17,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from ..ops import cache4
 from ..config.model_config import MixerSpec
 from .base import MIXERS, POSITIONS, CacheNeed, Mixer, TensorDecl
 
@@ -69,6 +70,10 @@ class PagedAttention(Mixer):
         t = h.shape[0]
         qkv = ctx.scratch("attn.qkv", (t, self.q_width + 2 * self.kv_width), self.dtype)
         cache = ctx.cache(binding.group)
+        if cache.in_4_bits:
+            out = self._forward4(ctx, h, qkv, cache, binding)
+            ops.linear(out, self.wo, residual, accumulate=True, closes=ctx)
+            return
         rot = self.position.rotation() if self.position is not None else None
         if rot is not None or self.position is None:
             cos, sin, rotary_dim = rot if rot is not None else (None, None, 0)
@@ -87,6 +92,37 @@ class PagedAttention(Mixer):
         ops.paged_attention(qkv, out, s.n_heads, s.n_kv_heads, s.head_dim, s.softmax_scale,
                             s.window, ctx, cache, binding)
         ops.linear(out, self.wo, residual, accumulate=True, closes=ctx)
+
+    def refuses_cache4(self, group):
+        s = self.spec
+        if s.head_dim in cache4.HEAD_DIMS and group in cache4.GROUPS and s.head_dim % group == 0:
+            return None
+        return (f"a cache in 4 bits takes heads of {cache4.HEAD_DIMS} features in groups of {cache4.GROUPS} that divide them, "
+                f"not {s.head_dim} in groups of {group}")
+
+    def _forward4(self, ctx, h, qkv, cache, binding):
+        """The same over pages in 4 bits; requests that bring one token may attend to some of their pages alone."""
+        s = self.spec
+        t = qkv.shape[0]
+        pages, batch = cache.pages(binding.slot), cache4.Batch.of(ctx, binding.group)
+        ops.linear(h, self.wqkv, qkv)
+        q = qkv[:, :self.q_width]
+        cos = sin = None
+        if self.position is not None:
+            rot = self.position.rotation()
+            if rot is not None:
+                cos, sin, _ = rot
+            else:
+                k = qkv[:, self.q_width:self.q_width + self.kv_width]
+                self.position.apply(ctx, q.view(t, s.n_heads, s.head_dim), k.view(t, s.n_kv_heads, s.head_dim))
+        cache4.rope_append4(qkv, q, s.n_heads, cos, sin, batch, pages, write=binding.write)
+        out = ctx.scratch("attn.out", (t, self.q_width), self.dtype)
+        picks = None
+        if cache.attend_pages is not None and batch.lead:
+            picks = ctx.scratch("attn.picks", (batch.lead, s.n_kv_heads, cache.attend_pages), torch.int32)
+            cache4.pick_pages4(q, s.n_heads, batch, pages, picks)
+        cache4.attention4(q, out, s.n_heads, s.softmax_scale, batch, pages, window=s.window, picks=picks)
+        return out
 
 
 MIXERS.register("attention", PagedAttention)

@@ -125,6 +125,10 @@ class Mixer(Part):
     def state_bytes(self) -> int:
         return 0
 
+    def refuses_cache4(self, group: int) -> Optional[str]:
+        """Why the mixer cannot keep its keys and values in 4 bits by groups of `group` features (None: it can)."""
+        return f"{type(self).__name__} keeps its cache in the engine's dtype only"
+
     def forward(self, ctx, h: torch.Tensor, residual: torch.Tensor,
                 binding: LayerBinding) -> None:
         raise NotImplementedError
