@@ -1,11 +1,13 @@
 // Writing the cache in 4 bits, and reading it back as it stands.
 //
 //   append4   a row's q and k are rotated by its position, k and v go to the row's place in the pages.
-//             One warp a (row, head): lane L holds the features L + 32 i, so that a group's least and
-//             largest number are warp reductions, and a word of codes is put together from four lanes.
+//             D/8 lanes a (row, head), eight neighbouring features a lane: 16 bytes a load where rows are
+//             aligned.  Lane l of eight takes the features whose codes lie at bits 4l.. 4l + 3 of their words, so that
+//             eight lanes' codes are turned into eight words by a transposition of 8 x 8 nibbles, three
+//             shuffles; a group's least and largest number take two to four shuffles each.
 //   bounds4   of every page that the step wrote: each feature's largest and least key over the tokens that
-//             the page now holds, in 8 bits with one scale.  A block a (row, kv head); only the last row of
-//             each page's run does anything.
+//             the page now holds, in 8 bits with one scale.  A block a (row, kv head), a thread a word of codes and
+//             every 16th token; only the last row of each page's run does anything.
 //   values4   the whole pool as float32 or bfloat16 rows.
 //   expand4   the pages of some requests as rows of float32 or bfloat16 in pages of 64 tokens, for attention
 //             over many rows.
@@ -16,14 +18,15 @@
 
 namespace {
 
-__device__ __forceinline__ float warp_least(float v) {
+// (fminf and fmaxf would lose a NaN)
+__device__ __forceinline__ float least_of(float a, float b) {
     float r;
-    asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float warp_largest(float v) {
+__device__ __forceinline__ float largest_of(float a, float b) {
     float r;
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
@@ -76,105 +79,158 @@ __device__ __forceinline__ uint32_t code_of(float x, const Coding& c) {
     return (uint32_t)fminf(fmaxf(v, 0.f), 15.f);
 }
 
-template <int D, int GROUP, typename T>
-__global__ void __launch_bounds__(256) append4_kernel(const AppendParams p) {
-    cb_pdl_trigger();
-    cb_pdl_wait();
-    constexpr int NI = D / 32, W = D / 64, NG = D / GROUP;
-    const int lane = threadIdx.x & 31;
-    const int heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0);
-    const long long items = (long long)p.rows * heads;
-    for (long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * 8) {
-        const int row = (int)(item / heads), head = (int)(item - (long long)row * heads);
-        const int request = p.row_request[row], pos = p.positions[row];
-        if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) continue;
-        const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)row * p.qkv_stride + (size_t)head * D;
-        float x[NI];
+// Eight neighbouring numbers (VEC: aligned to 16 bytes).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_eight(const T* src, float (&v)[8]) {
+    if constexpr (!VEC) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) x[i] = cb_to_float(src[lane + 32 * i]);
-        if (head < p.n_heads + p.kv_heads && p.rotary > 0) {
-            const int half = p.rotary >> 1;
-            const float* cs = p.cos_t + (size_t)pos * half;
-            const float* sn = p.sin_t + (size_t)pos * half;
+        for (int e = 0; e < 8; ++e) v[e] = cb_to_float(src[e]);
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(src);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int f = lane + 32 * i;
-                if (f < p.rotary) {
-                    const bool first = p.neighbours ? (f & 1) == 0 : f < half;
-                    const int at = p.neighbours ? f >> 1 : first ? f : f - half;
-                    const int other = p.neighbours ? f ^ 1 : first ? f + half : f - half;
-                    const float y = cb_to_float(src[other]);
-                    const float own = __fmul_rn(x[i], cs[at]), cross = __fmul_rn(y, sn[at]);
-                    x[i] = first ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
-                }
-            }
-        }
-        if (head < p.n_heads) {
-            __syncwarp();                     // q may take its own place: every lane has read what it turns
-            T* dst = reinterpret_cast<T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * D;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) dst[lane + 32 * i] = cb_from_float<T>(x[i]);
-            continue;
-        }
-        const int side = head >= p.n_heads + p.kv_heads;
-        const int kv = head - p.n_heads - side * p.kv_heads;
-        long long at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-        if (at < 0) continue;
-        at += (long long)kv * p.page_tokens + (long long)side * p.n_pages * p.kv_heads * p.page_tokens;
-        constexpr int PER = GROUP / 32;
-        uint32_t code[NI], pair = 0;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float least = x[g * PER], largest = x[g * PER];
-#pragma unroll
-            for (int i = 1; i < PER; ++i) {
-                // (a NaN has to stay one)
-                const float v = x[g * PER + i];
-                least = least <= v ? least : v != v ? v : least != least ? least : v;
-                largest = largest >= v ? largest : v != v ? v : largest != largest ? largest : v;
-            }
-            const Coding c = coding_of(warp_least(least), warp_largest(largest));
-#pragma unroll
-            for (int i = 0; i < PER; ++i) code[g * PER + i] = code_of(x[g * PER + i], c);
-            if (lane == g) pair = c.pair;
-        }
-        if (lane < NG) p.scales[at * NG + lane] = pair;
-        const int shift = c4_shift(lane >> 3);             // of feature k = lane / 8; k + 4 lies 8 bits higher
-        uint32_t word[W];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            word[w] = (code[2 * w] << shift) | (code[2 * w + 1] << (shift + 8));
-            word[w] |= __shfl_xor_sync(0xffffffffu, word[w], 8);
-            word[w] |= __shfl_xor_sync(0xffffffffu, word[w], 16);
-        }
-        if (lane < 8) {
-            uint32_t* dst = p.codes + at * (D / 8) + lane * W;
-            if constexpr (W == 1) dst[0] = word[0];
-            else if constexpr (W == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
-            else if constexpr (W == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
-            else {
-#pragma unroll
-                for (int w = 0; w < W; ++w) dst[w] = word[w];
-            }
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = __uint_as_float(w[e] << 16);
+            v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
         }
     }
 }
 
-// The value of feature f of the row `at`.
-template <int D>
-__device__ __forceinline__ float value_of(const uint32_t* codes, const uint32_t* scales, long long at, int group, int f) {
-    const uint32_t word = codes[at * (D / 8) + (f & 7) * (D / 64) + (f >> 6)];
-    const uint32_t pair = scales[at * (D / group) + f / group];
-    return fmaf((float)((word >> c4_shift((f >> 3) & 7)) & 15u), c4_step(pair), c4_low(pair));
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_eight(T* dst, const float (&v)[8]) {
+    if constexpr (!VEC) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = cb_from_float<T>(v[e]);
+    } else if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        __nv_bfloat162 b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(b);
+    }
 }
 
-// A block of D threads a feature each, four threads a feature over the tokens.
-template <int D>
-__global__ void __launch_bounds__(4 * D) bounds4_kernel(const AppendParams p, int group) {
+// VEC: rows are aligned to 16 bytes, and half of the rotated features is a multiple of eight.
+template <int D, int GROUP, typename T, bool VEC>
+__global__ void __launch_bounds__(256) append4_kernel(const AppendParams p) {
     cb_pdl_trigger();
     cb_pdl_wait();
-    __shared__ float part[2][4][D];
-    __shared__ float largest[8];
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, W = D / 64, NG = D / GROUP;
+    const int lane = threadIdx.x & 31, within = lane % LANES;
+    const int w = within >> 3, l = within & 7;
+    const int k = (l & 1) | ((l & 2) << 1) | ((l & 4) >> 1);            // (0, 1, 4, 5, 2, 3, 6, 7)[l]
+    const int f = 64 * w + 8 * k;
+    const int heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0);
+    const long long items = (long long)p.rows * heads;
+    const long long stride = (long long)gridDim.x * 8 * PER_WARP;
+    const long long begin = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP;
+    for (long long at_item = begin; at_item < items; at_item += stride) {         // (whole warps: shuffles)
+        const long long item = at_item + lane / LANES;
+        const bool mine = item < items && lane < LANES * PER_WARP;
+        const int row = mine ? (int)(item / heads) : 0, head = mine ? (int)(item - (long long)row * heads) : 0;
+        const int request = p.row_request[row], pos = p.positions[row];
+        const bool live = mine && request >= 0 && request < p.n_requests && pos >= 0 && !(p.rotary > 0 && pos >= p.n_positions);
+        const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)row * p.qkv_stride + (size_t)head * D;
+        long long at = -1;
+        const int side = head >= p.n_heads + p.kv_heads;
+        if (live && head >= p.n_heads) {
+            at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+            if (at >= 0) at += (long long)(head - p.n_heads - side * p.kv_heads) * p.page_tokens
+                             + (long long)side * p.n_pages * p.kv_heads * p.page_tokens;
+        }
+        float x[8];
+        if (live) {
+            load_eight<T, VEC>(src + f, x);
+            if (f < p.rotary && head < p.n_heads + p.kv_heads) {
+                const int half = p.rotary >> 1;
+                const float* cs = p.cos_t + (size_t)pos * half;
+                const float* sn = p.sin_t + (size_t)pos * half;
+                if (VEC && !p.neighbours) {
+                    const bool first = f < half;
+                    float y[8], c[8], s[8];
+                    const int j = first ? f : f - half;
+                    load_eight<T, VEC>(src + (first ? f + half : j), y);
+                    load_eight<float, VEC>(cs + j, c);
+                    load_eight<float, VEC>(sn + j, s);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float own = __fmul_rn(x[e], c[e]), cross = __fmul_rn(y[e], s[e]);
+                        x[e] = first ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
+                    }
+                } else if (p.neighbours) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (f + 2 * e >= p.rotary) break;
+                        const float a = x[2 * e], b = x[2 * e + 1], c = cs[(f >> 1) + e], s = sn[(f >> 1) + e];
+                        x[2 * e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+                        x[2 * e + 1] = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (f + e >= p.rotary) break;
+                        const bool first = f + e < half;
+                        const int j = first ? f + e : f + e - half;
+                        const float y = cb_to_float(src[first ? j + half : j]);
+                        const float own = __fmul_rn(x[e], cs[j]), cross = __fmul_rn(y, sn[j]);
+                        x[e] = first ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        }
+        __syncwarp();                     // q may take its own place: every lane has read what it turns
+        if (live && head < p.n_heads)
+            store_eight<T, VEC>(reinterpret_cast<T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * D + f, x);
+        if (!__any_sync(0xffffffffu, at >= 0)) continue;
+        // groups of 32 are the lanes of equal l & 2, of 64 all eight, of 128 two eights
+        float least = x[0], largest = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) {
+            least = least_of(least, x[e]);
+            largest = largest_of(largest, x[e]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            if (o == 2 && GROUP < 64) continue;
+            if (o == 8 && GROUP < 128) continue;
+            least = least_of(least, __shfl_xor_sync(0xffffffffu, least, o));
+            largest = largest_of(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        }
+        const Coding c = coding_of(least, largest);
+        uint32_t m = 0;                   // the lane's codes, feature g at nibble g
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m |= code_of(x[e], c) << (4 * e);
+        // transposed over eight lanes: nibble n of lane g is nibble g of lane n
+        uint32_t other = __shfl_xor_sync(0xffffffffu, m, 4);
+        m = (l & 4) ? __byte_perm(other, m, 0x7632) : __byte_perm(m, other, 0x5410);
+        other = __shfl_xor_sync(0xffffffffu, m, 2);
+        m = (l & 2) ? __byte_perm(other, m, 0x7351) : __byte_perm(m, other, 0x6240);
+        other = __shfl_xor_sync(0xffffffffu, m, 1);
+        m = (l & 1) ? ((other >> 4) & 0x0f0f0f0fu) | (m & 0xf0f0f0f0u) : (m & 0x0f0f0f0fu) | ((other << 4) & 0xf0f0f0f0u);
+        if (at >= 0) {
+            p.codes[at * (D / 8) + l * W + w] = m;
+            // (the first lane of a group)
+            const bool one = GROUP == 32 ? (l & ~2) == 0 : GROUP == 64 ? l == 0 : (within & 15) == 0;
+            if (one) p.scales[at * NG + f / GROUP] = c.pair;
+        }
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, int group) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    constexpr int WORDS = D / 8, W = D / 64;                 // 16 threads a word, two words a warp
+    __shared__ float largest[2 * D / 32];
+    __shared__ __align__(16) int8_t rounded[2][D];
     const int row = blockIdx.x / p.kv_heads, kv = blockIdx.x - row * p.kv_heads;
     const int request = p.row_request[row], pos = p.positions[row];
     if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) return;
@@ -185,37 +241,56 @@ __global__ void __launch_bounds__(4 * D) bounds4_kernel(const AppendParams p, in
     const int held = pos - index * p.page_tokens + 1;
     const long long page = (at - (held - 1)) / ((long long)p.kv_heads * p.page_tokens);
     at += (long long)kv * p.page_tokens - (held - 1);
-    const int f = threadIdx.x % D, q = threadIdx.x / D;
-    float hi = -INFINITY, lo = INFINITY;
-    for (int i = q; i < held; i += 4) {
-        const float v = value_of<D>(p.codes, p.scales, at + i, group, f);
-        hi = fmaxf(hi, v);
-        lo = fminf(lo, v);
-    }
-    part[0][q][f] = hi;
-    part[1][q][f] = lo;
-    __syncthreads();
-    if (q == 0) {
+    const int tid = threadIdx.x, lane = tid & 31, word = tid >> 4, t = tid & 15;
+    const int g = word / W, w = word - g * W, f = 64 * w + g;         // features f + 8 k
+    const uint32_t* codes = p.codes + at * WORDS + word;
+    const uint32_t* scales = p.scales + at * (D / group);
+    const int g0 = f / group, g1 = (f + 32) / group;                  // k < 4, k >= 4
+    float hi[8], lo[8];
 #pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            hi = fmaxf(hi, part[0][i][f]);
-            lo = fminf(lo, part[1][i][f]);
+    for (int k = 0; k < 8; ++k) hi[k] = -INFINITY, lo[k] = INFINITY;
+#pragma unroll 4
+    for (int i = t; i < held; i += 16) {
+        const uint32_t c = codes[(size_t)i * WORDS];
+        const uint32_t a = scales[(size_t)i * (D / group) + g0], b = scales[(size_t)i * (D / group) + g1];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t pair = k < 4 ? a : b;
+            const float v = fmaf((float)((c >> c4_shift(k)) & 15u), c4_step(pair), c4_low(pair));
+            hi[k] = fmaxf(hi[k], v);
+            lo[k] = fminf(lo[k], v);
         }
-        if (!(lo <= hi)) hi = lo = 0.f;          // (a feature of which no token's key is a number)
-        const float most = cb_warp_max(fmaxf(fabsf(hi), fabsf(lo)));
-        if ((f & 31) == 0) largest[f >> 5] = most;
     }
-    __syncthreads();
-    if (q != 0) return;
     float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) most = fmaxf(most, largest[i]);
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
+            lo[k] = fminf(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], o));
+        }
+        if (!(lo[k] <= hi[k])) hi[k] = lo[k] = 0.f;          // (a feature of which no token's key is a number)
+        most = fmaxf(most, fmaxf(fabsf(hi[k]), fabsf(lo[k])));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+    if (lane == 0) largest[tid >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * D / 32; ++i) most = fmaxf(most, largest[i]);
     const float scale = __fmul_rn(most, 1.0f / 127.0f);
     const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        // lane t of a word writes feature t & 7, its largest or least
+        if ((t & 7) == k)
+            rounded[t >> 3][f + 8 * k] =
+                (int8_t)(int)fminf(fmaxf(rintf(__fmul_rn(t < 8 ? hi[k] : lo[k], inverse)), -127.f), 127.f);
+    }
+    __syncthreads();
     const long long to = page * p.kv_heads + kv;
-    p.bounds[(to * 2) * D + f] = (int8_t)(int)fminf(fmaxf(rintf(__fmul_rn(hi, inverse)), -127.f), 127.f);
-    p.bounds[(to * 2 + 1) * D + f] = (int8_t)(int)fminf(fmaxf(rintf(__fmul_rn(lo, inverse)), -127.f), 127.f);
-    if (f == 0) p.bound_scales[to] = scale;
+    if (tid < 2 * D / 16)
+        reinterpret_cast<int4*>(p.bounds + to * 2 * D)[tid] = reinterpret_cast<const int4*>(rounded)[tid];
+    if (tid == 0) p.bound_scales[to] = scale;
 }
 
 // Eight neighbouring features of a row.
@@ -230,19 +305,6 @@ __device__ __forceinline__ void eight_values(const uint32_t* codes, const uint32
     for (int g = 0; g < 8; ++g) v[g] = fmaf((float)((words[g * (D / 64)] >> shift) & 15u), step, low);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_eight(T* dst, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        __nv_bfloat162 b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(b);
-    }
-}
-
 template <int D, typename T>
 __global__ void __launch_bounds__(256) values4_kernel(const uint32_t* codes, const uint32_t* scales, int group, long long rows,
                                                       T* out) {
@@ -254,7 +316,7 @@ __global__ void __launch_bounds__(256) values4_kernel(const uint32_t* codes, con
         const int f = (int)(i - at * (D / 8)) * 8;
         float v[8];
         eight_values<D>(codes, scales, at, group, f, v);
-        store_eight(out + at * D + f, v);
+        store_eight<T, true>(out + at * D + f, v);
     }
 }
 
@@ -269,57 +331,98 @@ struct ExpandParams {
     int window;
     void* keys;              // [blocks of 64 tokens][kv heads][64][D]
     void* values;
-    int* blocks;             // [requests][block_stride]: where each request's blocks of 64 tokens lie
+    int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
 };
 
-// A block of threads a block of 64 tokens and kv head.  Which request the block of tokens is of follows from how many
-// blocks the requests before it have; tokens that no row of the step sees are left out, as zeros.
+// A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
+// last token.  Which request a block is of follows from how many blocks the requests before it have; tokens that no row of
+// the step sees are left out, as zeros.  A value that is no number becomes its key's: attention by tiles multiplies the
+// values of masked keys by zero, but does not take their scores.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     cb_pdl_trigger();
     cb_pdl_wait();
-    int request = 0, before = 0, count = 0, held = 0, first = 0;
+    __shared__ uint32_t bad[64];
     const int block = blockIdx.x;
+    if (block == 0 && blockIdx.y == 0) {
+        int before = 0;
+        for (int r = 0; r < p.n_requests; ++r) {
+            const int count = (p.first_pos[r] + p.row_start[r + 1] - p.row_start[r] + 63) >> 6;
+            for (int i = threadIdx.x; i < p.block_stride; i += 256)
+                p.blocks[(size_t)r * p.block_stride + i] = i < count && before + i < p.n_blocks ? before + i : p.n_blocks;
+            before += count;
+        }
+    }
+    int request = 0, before = 0, held = 0, first = 0;
     for (; request < p.n_requests; ++request) {
         first = p.first_pos[request];
         held = first + p.row_start[request + 1] - p.row_start[request];
-        count = (held + 63) >> 6;
+        const int count = (held + 63) >> 6;
         if (block < before + count) break;
         before += count;
     }
-    if (request == p.n_requests) return;
     const int index = block - before;
-    if (index >= p.block_stride) return;
-    if (blockIdx.y == 0 && threadIdx.x == 0) p.blocks[(size_t)request * p.block_stride + index] = block;
+    const bool some = block < p.n_blocks && request < p.n_requests;
     const int lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
-    for (int i = threadIdx.x; i < 64 * (D / 8); i += 256) {
-        const int t = i / (D / 8), f = (i - t * (D / 8)) * 8, pos = index * 64 + t;
-        const long long to = (((long long)block * p.kv_heads + blockIdx.y) * 64 + t) * D + f;
-        float k[8] = {0.f}, v[8] = {0.f};
-        if (pos < held && pos >= lo) {
-            long long at = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-            if (at >= 0) {
-                at += (long long)blockIdx.y * p.page_tokens;
-                eight_values<D>(p.codes, p.scales, at, p.group, f, k);
-                eight_values<D>(p.codes, p.scales, at + (long long)p.n_pages * p.kv_heads * p.page_tokens, p.group, f, v);
+    if (threadIdx.x < 64) bad[threadIdx.x] = 0;
+    __syncthreads();
+    constexpr float MOST = sizeof(T) == 2 ? 3.3895314e38f : 3.4028235e38f;
+    constexpr int ITEMS = 64 * (D / 8) / 256;
+    float v[ITEMS][8];
+    long long at[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        const int i = threadIdx.x + 256 * j, t = i / (D / 8), f = (i - t * (D / 8)) * 8, pos = index * 64 + t;
+        at[j] = -1;
+        if (some && pos < held && pos >= lo)
+            at[j] = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+        if (at[j] >= 0) {
+            at[j] += (long long)blockIdx.y * p.page_tokens;
+            eight_values<D>(p.codes, p.scales, at[j] + (long long)p.n_pages * p.kv_heads * p.page_tokens, p.group, f, v[j]);
+            if (!(v[j][0] == v[j][0])) {                    // (a group's numbers are all none or all some)
+                bad[t] = 1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
             }
         }
-        store_eight(reinterpret_cast<T*>(p.keys) + to, k);
-        store_eight(reinterpret_cast<T*>(p.values) + to, v);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        const int i = threadIdx.x + 256 * j, t = i / (D / 8), f = (i - t * (D / 8)) * 8;
+        const long long to = (((long long)block * p.kv_heads + blockIdx.y) * 64 + t) * D + f;
+        float k[8] = {0.f};
+        if (at[j] >= 0) eight_values<D>(p.codes, p.scales, at[j], p.group, f, k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (bad[t]) k[e] = __int_as_float(0x7fffffff);
+            else if (k[e] == k[e]) k[e] = fminf(fmaxf(k[e], -MOST), MOST);
+            v[j][e] = fminf(fmaxf(v[j][e], -MOST), MOST);
+        }
+        store_eight<T, true>(reinterpret_cast<T*>(p.keys) + to, k);
+        store_eight<T, true>(reinterpret_cast<T*>(p.values) + to, v[j]);
     }
 }
 
 template <int D, int GROUP>
 int append_of(const AppendParams& p, int dtype, cudaStream_t stream) {
-    const long long items = (long long)p.rows * (p.n_heads + 2 * p.kv_heads);
-    const dim3 grid((unsigned)min((items + 7) / 8, 148LL * 8));
+    const int size = dtype == CB_F32 ? 4 : 2;
+    const long long per_block = 8 * (32 / (D / 8));
+    const long long items = (long long)p.rows * (p.n_heads + (p.write ? 2 * p.kv_heads : 0));
+    const dim3 grid((unsigned)min((items + per_block - 1) / per_block, 148LL * 32));
+    const bool vec = ((uintptr_t)p.qkv | (uintptr_t)p.q | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16 == 0
+        && p.qkv_stride * size % 16 == 0 && p.q_stride * size % 16 == 0 && (p.rotary / 2) % 8 == 0;
     int rc;
-    if (dtype == CB_F32) rc = cb_launch(append4_kernel<D, GROUP, float>, grid, dim3(256), 0, stream, p);
-    else rc = cb_launch(append4_kernel<D, GROUP, __nv_bfloat16>, grid, dim3(256), 0, stream, p);
+    if (dtype == CB_F32) rc = cb_launch(vec ? append4_kernel<D, GROUP, float, true> : append4_kernel<D, GROUP, float, false>,
+                                        grid, dim3(256), 0, stream, p);
+    else rc = cb_launch(vec ? append4_kernel<D, GROUP, __nv_bfloat16, true> : append4_kernel<D, GROUP, __nv_bfloat16, false>,
+                        grid, dim3(256), 0, stream, p);
     if (rc == 0 && p.write && p.bounds != nullptr)
-        rc = cb_launch(bounds4_kernel<D>, dim3((unsigned)p.rows * p.kv_heads), dim3(4 * D), 0, stream, p, GROUP);
+        rc = cb_launch(bounds4_kernel<D>, dim3((unsigned)p.rows * p.kv_heads), dim3(2 * D), 0, stream, p, GROUP);
     return rc;
 }
 
@@ -380,7 +483,7 @@ CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
                             keys, values, blocks, block_stride, n_blocks};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)n_blocks, (unsigned)kv_heads);
+    const dim3 grid((unsigned)n_blocks + 1, (unsigned)kv_heads);
 #define EXPAND(D)                                                                              \
     if (head_dim == D) {                                                                       \
         if (dtype == CB_F32) cb_launch(expand4_kernel<D, float>, grid, dim3(256), 0, s, p);    \

@@ -760,13 +760,18 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Shares that went through memory: one block a row tile.
+// Shares that went through memory: one block a row, D / 4 threads a share side by side.
+constexpr int A4_MOST_CHUNKS = 1024;
+
 template <int D, int NT, bool F32>
-__global__ void __launch_bounds__(128) attention4_merge_kernel(const Attn4Params p) {
+__global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params p) {
     cb_pdl_trigger();
-    cb_pdl_wait();
-    constexpr int ROWS = 8 * NT;
+    constexpr int ROWS = 8 * NT, LANES = D / 4, SETS = 256 / LANES;
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+    __shared__ float weights[A4_MOST_CHUNKS], part[8];
+    __shared__ float4 sums[SETS][LANES];
+    cb_pdl_wait();
+    const int r = blockIdx.y;
     int x = blockIdx.x;
     const int row_tile = x % p.row_tiles;
     x /= p.row_tiles;
@@ -787,24 +792,57 @@ __global__ void __launch_bounds__(128) attention4_merge_kernel(const Attn4Params
         if (p.window > 0) tile_lo = max(0, first + base / p.n_rep - p.window + 1) >> 4;
         tile_hi = ((first + (min(n_rows, base + ROWS) - 1) / p.n_rep) >> 4) + 1;
     }
-    if (base >= n_rows) return;
+    if (base + r >= n_rows) return;
     const int n = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
-    if (n <= 1) return;                          // (its block has written the rows)
-    const float* from = p.partial + (size_t)blockIdx.x * p.n_chunks * (ROWS * (D + 2));
-    const int live = min(ROWS, n_rows - base);
-    for (int i = blockIdx.y * 128 + threadIdx.x; i < live * D; i += gridDim.y * 128) {
-        const int r = i / D;
-        float top = -3.4e38f, v = 0.f, l = 0.f;
-        for (int z = 0; z < n; ++z) top = fmaxf(top, from[(size_t)z * (ROWS * (D + 2)) + 2 * r]);
+    if (n <= 1) return;                          // (its block has written the row)
+    constexpr int ONE = ROWS * (D + 2);
+    const float* from = p.partial + (size_t)blockIdx.x * p.n_chunks * ONE;
+    const int tid = threadIdx.x, set = tid / LANES, lane = tid % LANES;
+    // weights of the shares
+    float top = -3.4e38f;
+    for (int z = tid; z < n; z += 256) {
+        weights[z] = from[(size_t)z * ONE + 2 * r];
+        top = fmaxf(top, weights[z]);
+    }
+    top = cb_warp_max(top);
+    if ((tid & 31) == 0) part[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, part[i]);
+    float l = 0.f;
+    for (int z = tid; z < n; z += 256) {
+        const float w = a4_exp2(weights[z] - top);
+        weights[z] = w;
+        l = fmaf(from[(size_t)z * ONE + 2 * r + 1], w, l);
+    }
+    l = cb_warp_sum(l);
+    __syncthreads();
+    if ((tid & 31) == 0) part[tid >> 5] = l;
+    __syncthreads();
+    if (set < SETS) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* mine = from + 2 * ROWS + r * D + lane * 4;
 #pragma unroll 4
-        for (int z = 0; z < n; ++z) {
-            const float* one = from + (size_t)z * (ROWS * (D + 2));
-            const float weight = a4_exp2(one[2 * r] - top);
-            v = fmaf(one[2 * ROWS + i], weight, v);
-            l = fmaf(one[2 * r + 1], weight, l);
+        for (int z = set; z < n; z += SETS) {
+            const float4 one = *reinterpret_cast<const float4*>(mine + (size_t)z * ONE);
+            const float w = weights[z];
+            v.x = fmaf(one.x, w, v.x);
+            v.y = fmaf(one.y, w, v.y);
+            v.z = fmaf(one.z, w, v.z);
+            v.w = fmaf(one.w, w, v.w);
         }
+        sums[set][lane] = v;
+    }
+    __syncthreads();
+    if (tid < D) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) v += reinterpret_cast<const float*>(sums[i])[tid];
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l += part[i];
         const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
-        reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + (i - r * D)] =
+        reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + tid] =
             cb_from_float<T>(l == 0.f ? 0.f : v / l);
     }
 }
@@ -826,7 +864,7 @@ int attention4_launch(const Attn4Params& p, long long blocks, int shares, cudaSt
     int rc = cb_launch_cluster(attention4_kernel<D, NG, NT, F32>, grid, dim3(A4_WARPS * 32), L::TOTAL, stream,
                                through_memory ? 1 : shares, p);
     if (rc == 0 && through_memory)
-        rc = cb_launch(attention4_merge_kernel<D, NT, F32>, dim3((unsigned)blocks, (8 * NT * D + 511) / 512), dim3(128), 0, stream, p);
+        rc = cb_launch(attention4_merge_kernel<D, NT, F32>, dim3((unsigned)blocks, 8 * NT), dim3(256), 0, stream, p);
     return rc;
 }
 
@@ -848,7 +886,7 @@ int attention4_of(const Attn4Params& p, int dtype, int column_tiles, long long b
         const int row_tiles = (most_rows * n_rep + rows_a_tile - 1) / rows_a_tile;                                       \
         const long long blocks = (long long)(picks != nullptr ? rows : requests) * kv_heads * row_tiles;                 \
         if (blocks <= 0) return 0;                                                                                       \
-        if (blocks >= (1LL << 31) || n_chunks > 65535) return CB_ERR_UNSUPPORTED;                                        \
+        if (blocks >= (1LL << 31) || n_chunks > A4_MOST_CHUNKS) return CB_ERR_UNSUPPORTED;                                        \
         const Attn4Params p = {q, q_stride, out, out_stride, reinterpret_cast<const uint8_t*>(codes),                    \
                                reinterpret_cast<const uint8_t*>(scales), n_pages, page_tokens, kv_heads, n_rep,          \
                                row_start, first_pos, table, table_stride, requests, picks, pick_count, row_request,      \

@@ -6,9 +6,11 @@
 // two products of whole numbers (below 2^24, so float32 holds them), and a page scores (float) dot * (b a), the
 // largest over the heads of the group: every operation is rounded once, so that which pages are picked is defined.
 //
-// Up to eight blocks of a cluster score a row's pages (four lanes a page, 16 bytes a load, the queries in shared
-// memory) into the first one's shared memory.  That one finds the count-th largest score by its bits, eight at a
-// time, and writes the pages out in ascending order, of equal scores those that come first.
+// Up to eight blocks of a cluster score a row's pages (four lanes a page, 16 bytes a load, two pages at a time, the
+// queries in shared memory) into the first one's shared memory.  That one finds the count-th largest score by its
+// bits, eight at a time below the first in which the largest and the least differ (so that the histogram's bins are hit
+// evenly; as a rule the second or third decides), and writes the pages out in ascending order, of equal scores
+// those that come first.
 #define CB_PDL_BIT 6      // with the other quantised operators
 #include "cache4.cuh"
 
@@ -46,6 +48,7 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
     int4* q8 = reinterpret_cast<int4*>(smem + (size_t)p.most_pages * 4);                // [n_rep][2][D / 16]
     float* q_scale = reinterpret_cast<float*>(q8 + (size_t)p.n_rep * 2 * (D / 16));     // [n_rep]
     __shared__ int histogram[256], found[4], warp_counts[PICK_THREADS / 32];
+    __shared__ uint32_t ends[2][PICK_THREADS / 32];
     const int row = blockIdx.x / p.kv_heads, kv = blockIdx.x - row * p.kv_heads;
     const int request = p.row_request[row], pos = p.positions[row];
     if (request < 0 || request >= p.n_requests || pos < 0) return;                      // (all blocks of a cluster)
@@ -87,46 +90,66 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
     const int stride = gridDim.z * (PICK_THREADS / 4);
     uint32_t there = (uint32_t)__cvta_generic_to_shared(score);
     if (gridDim.z > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(there));
-    for (int at = blockIdx.z * (PICK_THREADS / 4); at < pages; at += stride) {       // (whole warps: shuffles)
-        const int index = at + (tid >> 2);
-        const int page = index < pages ? table[index] : -1;
-        const bool known = page >= 0 && page < p.n_pages;
-        int4 hi[D / 64], lo[D / 64];
-        float a = 0.f;
-        if (known) {
-            const size_t to = (size_t)page * p.kv_heads + kv;
-            const int4* b = reinterpret_cast<const int4*>(p.bounds + to * 2 * D);
+    constexpr int WIDE = 2;
+    for (int at = blockIdx.z * (PICK_THREADS / 4); at < pages; at += WIDE * stride) {       // (whole warps: shuffles)
+        int4 hi[WIDE][D / 64], lo[WIDE][D / 64];
+        float a[WIDE];
+        int page[WIDE];
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-                hi[j] = b[quarter + 4 * j];
-                lo[j] = b[D / 16 + quarter + 4 * j];
-            }
-            a = p.bound_scales[to];
-        } else {
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) hi[j] = lo[j] = make_int4(0, 0, 0, 0);
+        for (int n = 0; n < WIDE; ++n) {
+            const int index = at + n * stride + (tid >> 2);
+            page[n] = index < pages ? table[index] : -1;
         }
-        float best = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n) {
+            a[n] = 0.f;
+            if ((unsigned)page[n] < (unsigned)p.n_pages) {
+                const size_t to = (size_t)page[n] * p.kv_heads + kv;
+                const int4* b = reinterpret_cast<const int4*>(p.bounds + to * 2 * D);
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) {
+                    hi[n][j] = b[quarter + 4 * j];
+                    lo[n][j] = b[D / 16 + quarter + 4 * j];
+                }
+                a[n] = p.bound_scales[to];
+            } else {
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) hi[n][j] = lo[n][j] = make_int4(0, 0, 0, 0);
+            }
+        }
+        float best[WIDE];
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n) best[n] = -INFINITY;
         for (int h = 0; h < p.n_rep; ++h) {
             const int4* up = q8 + (size_t)h * 2 * (D / 16);
-            int dot = 0;
+            int dot[WIDE] = {};
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
                 const int4 u = up[quarter + 4 * j], d = up[D / 16 + quarter + 4 * j];
-                dot = __dp4a(u.x, hi[j].x, dot); dot = __dp4a(u.y, hi[j].y, dot);
-                dot = __dp4a(u.z, hi[j].z, dot); dot = __dp4a(u.w, hi[j].w, dot);
-                dot = __dp4a(d.x, lo[j].x, dot); dot = __dp4a(d.y, lo[j].y, dot);
-                dot = __dp4a(d.z, lo[j].z, dot); dot = __dp4a(d.w, lo[j].w, dot);
+#pragma unroll
+                for (int n = 0; n < WIDE; ++n) {
+                    dot[n] = __dp4a(u.x, hi[n][j].x, dot[n]); dot[n] = __dp4a(u.y, hi[n][j].y, dot[n]);
+                    dot[n] = __dp4a(u.z, hi[n][j].z, dot[n]); dot[n] = __dp4a(u.w, hi[n][j].w, dot[n]);
+                    dot[n] = __dp4a(d.x, lo[n][j].x, dot[n]); dot[n] = __dp4a(d.y, lo[n][j].y, dot[n]);
+                    dot[n] = __dp4a(d.z, lo[n][j].z, dot[n]); dot[n] = __dp4a(d.w, lo[n][j].w, dot[n]);
+                }
             }
-            dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-            dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-            best = fmaxf(best, __fmul_rn((float)dot, __fmul_rn(q_scale[h], a)));
+            const float unit = q_scale[h];
+#pragma unroll
+            for (int n = 0; n < WIDE; ++n) {
+                dot[n] += __shfl_xor_sync(0xffffffffu, dot[n], 1);
+                dot[n] += __shfl_xor_sync(0xffffffffu, dot[n], 2);
+                best[n] = fmaxf(best[n], __fmul_rn((float)dot[n], __fmul_rn(unit, a[n])));
+            }
         }
-        if (quarter == 0 && index < pages) {
-            uint32_t s = known ? max(order_of(best), 1u) : 0u;
-            if (index < p.first || index > own - p.last) s = 0xffffffffu;
-            if (gridDim.z > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there + index * 4), "r"(s) : "memory");
-            else score[index] = s;
+#pragma unroll
+        for (int n = 0; n < WIDE; ++n) {
+            const int index = at + n * stride + (tid >> 2);
+            if (quarter == 0 && index < pages) {
+                const uint32_t s = (unsigned)page[n] < (unsigned)p.n_pages ? max(order_of(best[n]), 1u) : 0u;
+                if (gridDim.z > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there + index * 4), "r"(s) : "memory");
+                else score[index] = s;
+            }
         }
     }
     if (gridDim.z > 1) {
@@ -135,46 +158,74 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
         if (blockIdx.z != 0) return;
     }
     __syncthreads();
-    // the count-th largest score, and how many of those equal to it are wanted
-    uint32_t prefix = 0, mask = 0;
-    int wanted = p.count;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) histogram[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < pages; i += PICK_THREADS)
-            if ((score[i] & mask) == prefix) atomicAdd(&histogram[(score[i] >> shift) & 255], 1);
-        __syncthreads();
-        if (warp == 0) {
-            // lane L sums the bins 8 L .. 8 L + 7; the wanted one is in the first lane from the top that reaches it
-            int mine = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mine += histogram[8 * lane + j];
-            int above = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_down_sync(0xffffffffu, above, o);
-                if (lane + o < 32) above += v;
-            }
-            above -= mine;                              // scores in higher lanes' bins
-            if (above < wanted && above + mine >= wanted) {
-                int b = 7;
-                while (above + histogram[8 * lane + b] < wanted) above += histogram[8 * lane + b--];
-                found[0] = 8 * lane + b;
-                found[1] = wanted - above;
-            }
+    // Pages from `free_lo` to `free_hi` are chosen among; those before and behind them are taken always.
+    const int free_lo = p.first, free_hi = own - p.last;
+    int wanted = p.count - p.first - p.last;              // (pages > count: there are more than that)
+    uint32_t prefix = 0xffffffffu, mask = 0;
+    if (wanted > 0) {
+        // the ends of the scores: above `shift` + 8 bits they do not differ
+        uint32_t least = 0xffffffffu, most = 0;
+        for (int i = free_lo + tid; i <= free_hi; i += PICK_THREADS) {
+            least = min(least, score[i]);
+            most = max(most, score[i]);
         }
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) ends[0][warp] = least, ends[1][warp] = most;
         __syncthreads();
-        prefix |= (uint32_t)found[0] << shift;
-        mask |= 255u << shift;
-        wanted = found[1];
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PICK_THREADS / 32; ++i) {
+            least = min(least, ends[0][i]);
+            most = max(most, ends[1][i]);
+        }
+        const int differ = 32 - __clz(least ^ most);      // bits from the lowest on that are not all alike
+        mask = differ >= 32 ? 0u : 0xffffffffu << differ;
+        prefix = most & mask;
+        for (int top = differ; top > 0;) {
+            const int shift = max(top - 8, 0);
+            const uint32_t bins = (1u << (top - shift)) - 1u;
+            if (tid < 256) histogram[tid] = 0;
+            __syncthreads();
+            for (int i = free_lo + tid; i <= free_hi; i += PICK_THREADS)
+                if ((score[i] & mask) == prefix) atomicAdd(&histogram[(score[i] >> shift) & bins], 1);
+            __syncthreads();
+            if (warp == 0) {
+                // lane L sums the bins 8 L .. 8 L + 7; the wanted one is in the first lane from the top that reaches it
+                int mine = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mine += histogram[8 * lane + j];
+                int above = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_down_sync(0xffffffffu, above, o);
+                    if (lane + o < 32) above += v;
+                }
+                above -= mine;                              // scores in higher lanes' bins
+                if (above < wanted && above + mine >= wanted) {
+                    int b = 7;
+                    while (above + histogram[8 * lane + b] < wanted) above += histogram[8 * lane + b--];
+                    found[0] = 8 * lane + b;
+                    found[1] = wanted - above;
+                    found[2] = histogram[8 * lane + b];
+                }
+            }
+            __syncthreads();
+            prefix |= (uint32_t)found[0] << shift;
+            mask |= bins << shift;
+            wanted = found[1];
+            if (found[2] == wanted) break;                  // all of the bin: what its lower bits are does not matter
+            top = shift;
+            __syncthreads();
+        }
     }
     // out in ascending order: larger ones, and the first `wanted` equal ones
     int done = 0, equal_done = 0;
     for (int at = 0; at < pages; at += PICK_THREADS) {
         const int i = at + tid;
-        const uint32_t s = i < pages ? score[i] : 0;
-        const bool equal = i < pages && s == prefix, larger = i < pages && s > prefix;
+        const uint32_t s = i < pages ? score[i] & mask : 0;
+        const bool always = i < pages && (i < free_lo || i > free_hi);
+        const bool equal = i < pages && !always && wanted > 0 && s == prefix;
+        const bool larger = always || (i < pages && wanted > 0 && s > prefix);
         const uint32_t equals = __ballot_sync(0xffffffffu, equal), largers = __ballot_sync(0xffffffffu, larger);
         if (lane == 0) warp_counts[warp] = __popc(equals) | (__popc(largers) << 16);
         __syncthreads();

@@ -302,6 +302,13 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     if picks is not None:
         _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
     if behind < rows:
+        n_rep, lead = n_heads // kv, max(behind, batch.lead)
+        if lead < batch.requests and _laid_out(q, out, batch, n_rep, pages, window, lead):
+            if behind < lead:
+                _walk(q, out, n_heads, scale, batch, pages, window, None, behind, lead)
+            if _tiles(q, out, n_heads, scale, batch, pages, window, lead):
+                return
+            behind = lead
         _walk(q, out, n_heads, scale, batch, pages, window, None, behind, batch.requests)
 
 
@@ -350,3 +357,41 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     if code == build.UNSUPPORTED:
         raise KernelError(f"attention4: {blocks} blocks of rows are more than a launch takes")
     _check(code, "attention4")
+
+
+LAID_OUT_ROWS = 64          # rows of a kv head from which a portion's keys are laid out anew
+
+
+def _laid_out(q, out, batch, n_rep, pages, window, first) -> bool:
+    return (q.dtype is _BF16 and max(batch.new_tokens[first:]) * n_rep >= LAID_OUT_ROWS
+            and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16))
+
+
+class _Step:
+    """What the attention kernels over 16-bit pages read of a step: its requests from some on, in blocks of 64 tokens."""
+
+    page_tokens = 64
+    __slots__ = ("positions", "req_row_start", "req_first_pos")
+
+    def __init__(self, batch, first):
+        self.positions = batch.positions
+        self.req_row_start, self.req_first_pos = batch.row_start[first:], batch.first_pos[first:]
+
+
+def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
+    """bfloat16 portions of many rows: the keys and values of the requests from `first` on are laid out in bfloat16 once
+    (not again for every tile of rows), and attention runs over these by the kernels of the 16-bit cache."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    counts = [-(-(h + n) // 64) for h, n in zip(batch.held_tokens[first:], batch.new_tokens[first:])]
+    n_blocks, stride, requests = sum(counts), max(counts), len(counts)
+    both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=_BF16, device=q.device)
+    blocks = torch.empty(requests, stride, dtype=_I32, device=q.device)
+    lib = build.load("append4")
+    step = _Step(batch, first)
+    _check(_at(pages.device, lib.cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv,
+               dim, pages.group, step.req_row_start.data_ptr(), step.req_first_pos.data_ptr(),
+               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1], requests, window or 0,
+               both[0].data_ptr(), both[1].data_ptr(), 1, blocks.data_ptr(), stride, n_blocks), "pages laid out")
+    new = batch.new_tokens[first:]
+    reqs = tensor_core._Requests(step, blocks, 0, requests, max(new), 64 * stride, batch.positions.shape[0])
+    return tensor_core._attend(q, out, both[0], both[1], reqs, n_heads, kv, dim, scale, window, step, step)
