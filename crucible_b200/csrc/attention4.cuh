@@ -32,6 +32,9 @@ namespace {
 
 constexpr float A4_LOG2E = 1.4426950408889634f;
 constexpr int A4_WARPS = 4;
+#ifndef A4_BLOCKS
+#define A4_BLOCKS 4
+#endif
 
 struct Attn4Params {
     const void* q;
@@ -63,13 +66,11 @@ struct Attn4Params {
 
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ void a4_copy16(uint32_t dst, const void* src, bool there) {
-    const int bytes = there ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void a4_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void a4_copy4(uint32_t dst, const void* src, bool there) {
-    const int bytes = there ? 4 : 0;
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void a4_copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -182,7 +183,7 @@ __device__ __forceinline__ int a4_place(int r, int unit) {
 }
 
 template <int D, int NG, int NT, bool F32>
-__global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) attention4_kernel(const Attn4Params p) {
+__global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOCKS : 2) attention4_kernel(const Attn4Params p) {
     cb_pdl_trigger();
     cb_pdl_wait();
     constexpr int PARTS = F32 ? 2 : 1;
@@ -191,7 +192,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
     constexpr float CODE = F32 ? 1.f : 16777216.f;      // 1 over the unit of the codes
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    // (the warp's number by way of a shuffle: known to be the same in all lanes, what follows from it lives in uniform registers)
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
     // which rows, which keys
     int x = blockIdx.x;
@@ -225,6 +227,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
     } else {
         if (p.window > 0) tile_lo = max(0, min_pos - p.window + 1) >> 4;
         tile_hi = (max_pos >> 4) + 1;
+        // (what lies beyond the table is not there)
+        if (p.page_tiles > 0) tile_hi = (int)min((long long)tile_hi, (long long)p.table_stride * p.page_tiles);
     }
     const int lowest = p.window > 0 ? max_pos - p.window : -1;         // a tile that begins here or before needs a look
     int n_chunks = 1;
@@ -248,49 +252,67 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                                         p.codes + (side_rows + head_row) * (D / 2) + lane * 16};
     // (scales: lanes of both sides side by side)
     const uint8_t* const scale_src = p.scales + (head_row + (lane >= 4 * NG ? side_rows : 0)) * (NG * 4) + (lane % (4 * NG)) * 16;
+    // Where the lane's shares of a stage lie; of keys g (and g + 8), of values 2t and 2t + 1 (and 8 behind these).
+    // (kept, not worked out anew for every tile: what the compiler cannot see through it does not take apart again)
+    constexpr int EIGHT = 8 * D / 2;                        // eight rows further
+    uint32_t k_at = a4_place<D>(g, (t * D / 8) >> 4) + ((t * D / 8) & 15), v_at[2], s_at = 2 * L::SIDE + g * (NG * 4);
+    v_at[0] = L::SIDE + a4_place<D>(2 * t, (g * D / 16) >> 4) + ((g * D / 16) & 15);
+    v_at[1] = L::SIDE + a4_place<D>(2 * t + 1, (g * D / 16) >> 4) + ((g * D / 16) & 15);
+    asm volatile("" : "+r"(k_at), "+r"(v_at[0]), "+r"(v_at[1]), "+r"(s_at));
     uint32_t place[D / 64];
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) place[j] = a4_place<D>((lane + 32 * j) / (D / 32), (lane + 32 * j) % (D / 32));
-    // The row of tile i's first key (whole) for head 0, or -1 where its page is none; its position goes to `key`.
-    auto look = [&](int i, int& key) -> long long {
-        key = i * 16;
-        if (i >= tile_hi || !whole) return -1;
-        int index = p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse);
+    // The first key of tile i, and (whole) which page that is: -1 where there is none.
+    auto key_of = [&](int i, int& page) {
+        int index = whole ? (p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse)) : 0;
         if (index * p.page_tiles > i) --index;           // (rounded up, the inverse is at most one too much)
         const int slot = (i - index * p.page_tiles) * 16;
-        if (picks != nullptr) {
-            index = picks[index];
-            key = index * p.page_tokens + slot;
-        }
-        if ((unsigned)index >= (unsigned)p.table_stride) return -1;
-        const int page = table[index];
-        if ((unsigned)page >= (unsigned)p.n_pages) return -1;
-        return (long long)page * (p.kv_heads * p.page_tokens) + slot;
+        if (picks != nullptr) index = picks[index];
+        page = !whole ? 0 : (unsigned)index < (unsigned)p.table_stride ? table[index] : -1;
+        if ((unsigned)page >= (unsigned)p.n_pages) page = -1;
+        return picks != nullptr ? index * p.page_tokens + slot : i * 16;
     };
-    auto fetch = [&](int i, int stage, int key, long long at) {
-        if (i < tile_hi) {
+    // The tiles to fetch, one after the other; 32 of them are looked up at a time, a lane each: the row (for head 0) of
+    // each, and whether some row of the block may not see some key of it.  A tile whose page is none is masked whole;
+    // what is fetched for it (the pool's first rows) is of no account, as is what lies behind a request's last token.
+    int ahead = tile_lo + warp, looked = 0;
+    uint32_t rows_of = 0, edges_of = 0xffffffffu;
+    const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_tokens;
+    auto look = [&]() {
+        const int i = ahead + A4_WARPS * lane;
+        int page, key = 0;
+        bool there = false;
+        if (i < tile_hi && whole) {
+            key = key_of(i, page);
+            there = page >= 0;
+        }
+        rows_of = there ? (uint32_t)page * page_rows + (uint32_t)(key % p.page_tokens) : 0u;
+        edges_of = __ballot_sync(0xffffffffu, !there || key + 15 > min_pos || key <= lowest);
+    };
+    uint32_t edges = 0;                    // of the tiles in flight, the next to be taken in the lowest bit
+    auto fetch = [&](int stage) {
+        if (ahead < tile_hi) {
             const uint32_t to = ring + stage * L::STAGE;
             if (whole) {
-                // (a tile whose page is none is filled with zeros, and masked)
-                const bool there = at >= 0;
-                const long long row = there ? at : 0;
+                const uint32_t row = __shfl_sync(0xffffffffu, rows_of, looked);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const uint8_t* src = code_src[s] + row * (D / 2);
+                    const uint8_t* src = code_src[s] + (size_t)row * (D / 2);
 #pragma unroll
-                    for (int j = 0; j < D / 64; ++j) a4_copy16(to + s * L::SIDE + place[j], src + j * 512, there);
+                    for (int j = 0; j < D / 64; ++j) a4_copy16(to + s * L::SIDE + place[j], src + j * 512);
                 }
                 if constexpr (8 * NG <= 32) {
-                    if (lane < 8 * NG) a4_copy16(to + 2 * L::SIDE + lane * 16, scale_src + row * (NG * 4), there);
+                    if (lane < 8 * NG) a4_copy16(to + 2 * L::SIDE + lane * 16, scale_src + (size_t)row * (NG * 4));
                 } else {
 #pragma unroll
                     for (int c = lane; c < 8 * NG; c += 32) {
                         const int side = c / (4 * NG), u = c % (4 * NG);
                         a4_copy16(to + 2 * L::SIDE + c * 16,
-                                  p.scales + (head_row + row + side * side_rows) * (NG * 4) + u * 16, there);
+                                  p.scales + (head_row + row + side * side_rows) * (NG * 4) + u * 16);
                     }
                 }
             } else {
+                const int key = ahead * 16;
 #pragma unroll 1
                 for (int c = lane; c < 16 * (D / 32); c += 32) {
                     const int r = c / (D / 32), u = c % (D / 32);
@@ -298,8 +320,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                         ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
                     const size_t row = one >= 0 ? (size_t)one + head_row : 0;
                     const uint8_t* src = p.codes + row * (D / 2) + u * 16;
-                    a4_copy16(to + a4_place<D>(r, u), src, one >= 0);
-                    a4_copy16(to + L::SIDE + a4_place<D>(r, u), src + side_rows * (D / 2), one >= 0);
+                    a4_copy16(to + a4_place<D>(r, u), src);
+                    a4_copy16(to + L::SIDE + a4_place<D>(r, u), src + side_rows * (D / 2));
                 }
 #pragma unroll 1
                 for (int c = lane; c < 16 * NG; c += 32) {
@@ -308,25 +330,23 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                         ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
                     const size_t row = one >= 0 ? (size_t)one + head_row : 0;
                     const uint8_t* src = p.scales + (row * NG + u) * 4;
-                    a4_copy4(to + 2 * L::SIDE + c * 4, src, one >= 0);
-                    a4_copy4(to + 2 * L::SIDE + L::SCALES + c * 4, src + side_rows * (NG * 4), one >= 0);
+                    a4_copy4(to + 2 * L::SIDE + c * 4, src);
+                    a4_copy4(to + 2 * L::SIDE + L::SCALES + c * 4, src + side_rows * (NG * 4));
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    int ahead = tile_lo + warp;            // the next tile to fetch
-    int key_of[L::STAGES];                 // first keys of the tiles in flight; -1: of no page
-#pragma unroll
-    for (int s = 0; s < L::STAGES - 1; ++s) {
-        int key;
-        const long long at = look(ahead, key);
-        fetch(ahead, s, key, at);
-        key_of[s] = whole && at < 0 ? -1 : key;
+        edges = (edges >> 1) | (edges_of & 1u) << (L::STAGES - 2);
+        edges_of >>= 1;
         ahead += A4_WARPS;
-    }
-    int next_key;
-    long long next_at = look(ahead, next_key);
+        if (++looked == 32) {
+            looked = 0;
+            look();
+        }
+    };
+    look();
+#pragma unroll 1
+    for (int s = 0; s < L::STAGES - 1; ++s) fetch(s);
 
     // ---- the queries, as columns of the first product --------------------------
     {
@@ -398,14 +418,14 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
         }
 
     // Sums of a column are kept relative to 2^off, off = m - eps: m the reference of its scores (log2), at most 8 below the
-    // largest, and 2^eps the scale of p step in float16; `bound` is the step from which eps is too much.
-    float off[NT][2], eps[NT][2], bound[NT][2], sum[NT][2], lows[NT][NG][2], o[MT][NT][4];
+    // largest, and 2^eps the scale of p step in float16 (`limit` is eps + 8); `bound` is the step from which eps is too much.
+    float off[NT][2], limit[NT][2], bound[NT][2], sum[NT][2], lows[NT][NG][2], o[MT][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             off[n][c] = -3.0e38f;
-            eps[n][c] = 101.f;
+            limit[n][c] = 109.f;
             bound[n][c] = a4_power(-95);
             sum[n][c] = 0.f;
 #pragma unroll
@@ -427,20 +447,17 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
         uint32_t kw[2][2 * W];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int r = g + 8 * h;
-            if constexpr (D == 64) {
-                const uint2 v = *reinterpret_cast<const uint2*>(at + a4_place<D>(r, t >> 1) + (t & 1) * 8);
-                kw[h][0] = v.x; kw[h][1] = v.y;
-            } else if constexpr (D == 192) {
+            if constexpr (D == 64 || D == 192) {
 #pragma unroll
-                for (int j = 0; j < 3; ++j) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at + r * 96 + t * 24 + j * 8);
+                for (int j = 0; j < D / 64; ++j) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at + k_at + h * EIGHT + j * 8);
                     kw[h][2 * j] = v.x; kw[h][2 * j + 1] = v.y;
                 }
             } else {
+                // (256: the lane's second unit is the first's neighbour, which the places exchange but do not part)
 #pragma unroll
                 for (int j = 0; j < D / 128; ++j) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at + a4_place<D>(r, t * (D / 128) + j));
+                    const uint4 v = *reinterpret_cast<const uint4*>(at + (j == 0 ? k_at : k_at ^ 16) + h * EIGHT);
                     kw[h][4 * j] = v.x; kw[h][4 * j + 1] = v.y; kw[h][4 * j + 2] = v.z; kw[h][4 * j + 3] = v.w;
                 }
             }
@@ -448,8 +465,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
         uint32_t ksc[2][NG], vsc[2][NG];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            a4_pairs<NG>(ksc[h], at + 2 * L::SIDE + (g + 8 * h) * (NG * 4));
-            a4_pairs<NG>(vsc[h], at + 2 * L::SIDE + L::SCALES + (g + 8 * h) * (NG * 4));
+            a4_pairs<NG>(ksc[h], at + s_at + 8 * h * (NG * 4));
+            a4_pairs<NG>(vsc[h], at + s_at + L::SCALES + 8 * h * (NG * 4));
         }
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
@@ -509,8 +526,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                     }
         }
 
-        // the references move only when they have to.  (The pair's bits less its sign: steps are not negative, and a larger
-        // step has the larger bits.)
+        // the references move only when they have to
         float most_step[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -529,20 +545,20 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                     step_top[n][c] = fmaxf((hidden >> (4 * n + c)) & 1 ? 0.f : most_step[0],
                                            (hidden >> (4 * n + 2 + c)) & 1 ? 0.f : most_step[1]);
                 else step_top[n][c] = fmaxf(most_step[0], most_step[1]);
-                move = move || fmaf(top[n][c], factor[n][c], -off[n][c]) > eps[n][c] + 8.f || step_top[n][c] >= bound[n][c];
+                move = move || fmaf(top[n][c], factor[n][c], -off[n][c]) > limit[n][c] || step_top[n][c] >= bound[n][c];
             }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float m = fmaxf(off[n][c] + eps[n][c], a4_over_keys_max(top[n][c] * factor[n][c]));
+                    const float m = fmaxf(off[n][c] + (limit[n][c] - 8.f), a4_over_keys_max(top[n][c] * factor[n][c]));
                     const float st = a4_over_keys_max(step_top[n][c]);
                     const int e = min(max((int)(__float_as_uint(fmaxf(st, bound[n][c] * 0.5f)) >> 23) - 127, -96), 126);
                     const float e5 = 5.f - (float)e, to = m - e5;
                     const float r = a4_exp2(off[n][c] - to);
                     off[n][c] = to;
-                    eps[n][c] = e5;
+                    limit[n][c] = e5 + 8.f;
                     bound[n][c] = a4_power(e + 1);
                     sum[n][c] *= r;
 #pragma unroll
@@ -591,22 +607,19 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
         }
 
         // O^T += V^T P^T
-        const uint8_t* values = at + L::SIDE;
         uint32_t vw[4][W];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int r = 2 * t + (j & 1) + 8 * (j >> 1);
-            if constexpr (D == 64) {
-                vw[j][0] = *reinterpret_cast<const uint32_t*>(values + a4_place<D>(r, g >> 2) + (g & 3) * 4);
-            } else if constexpr (D == 128) {
-                const uint2 v = *reinterpret_cast<const uint2*>(values + a4_place<D>(r, g >> 1) + (g & 1) * 8);
+            const uint8_t* from = at + v_at[j & 1] + (j >> 1) * EIGHT;
+            if constexpr (D == 128) {
+                const uint2 v = *reinterpret_cast<const uint2*>(from);
                 vw[j][0] = v.x; vw[j][1] = v.y;
             } else if constexpr (D == 256) {
-                const uint4 v = *reinterpret_cast<const uint4*>(values + a4_place<D>(r, g));
+                const uint4 v = *reinterpret_cast<const uint4*>(from);
                 vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
             } else {
 #pragma unroll
-                for (int w = 0; w < W; ++w) vw[j][w] = *reinterpret_cast<const uint32_t*>(values + r * 96 + g * 12 + w * 4);
+                for (int w = 0; w < W; ++w) vw[j][w] = reinterpret_cast<const uint32_t*>(from)[w];
             }
         }
 #pragma unroll
@@ -637,22 +650,26 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? 4 : 2) 
                 }
             }
     };
-    int stage = 0;
-    for (int i = tile_lo + warp; i < tile_hi; i += A4_WARPS) {
+    int into = L::STAGES - 1;              // the stage that was read last, to be filled; the next one is to be read
+    auto next = [&]() -> const uint8_t* {
         asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
         __syncwarp();
-        const int key0 = key_of[0];
-        // the stage that was read last takes the tile after those in flight
-        fetch(ahead, stage == 0 ? L::STAGES - 1 : stage - 1, next_key, next_at);
-#pragma unroll
-        for (int s = 0; s + 2 < L::STAGES; ++s) key_of[s] = key_of[s + 1];
-        key_of[L::STAGES - 2] = whole && next_at < 0 ? -1 : next_key;
-        ahead += A4_WARPS;
-        next_at = look(ahead, next_key);
-        const uint8_t* at = smem + warp * L::RING + stage * L::STAGE;
-        stage = stage + 1 == L::STAGES ? 0 : stage + 1;
-        if (key0 < 0 || key0 + 15 > min_pos || key0 <= lowest || !whole) tile(std::true_type{}, at, key0);
-        else tile(std::false_type{}, at, key0);
+        fetch(into);
+        into = into + 1 == L::STAGES ? 0 : into + 1;
+        return smem + warp * L::RING + into * L::STAGE;
+    };
+    // (two loops, so that the one over whole tiles is nothing else: one loop that chose between the two forms moved
+    // registers about at every turn)
+    for (int i = tile_lo + warp; i < tile_hi; i += A4_WARPS) {
+        while (!(edges & 1)) {
+            tile(std::false_type{}, next(), 0);
+            i += A4_WARPS;
+            if (i >= tile_hi) break;
+        }
+        if (i >= tile_hi) break;
+        int page;
+        const int key0 = key_of(i, page);
+        tile(std::true_type{}, next(), page < 0 ? -1 : key0);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -791,6 +808,7 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
         first = p.first_pos[x];
         if (p.window > 0) tile_lo = max(0, first + base / p.n_rep - p.window + 1) >> 4;
         tile_hi = ((first + (min(n_rows, base + ROWS) - 1) / p.n_rep) >> 4) + 1;
+        if (p.page_tiles > 0) tile_hi = (int)min((long long)tile_hi, (long long)p.table_stride * p.page_tiles);
     }
     if (base + r >= n_rows) return;
     const int n = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
