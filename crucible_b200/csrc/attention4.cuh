@@ -19,10 +19,14 @@
 // tile, one or two of them a block, so that no more than that is multiplied for a single token.  S^T comes out with
 // keys over lanes; `movmatrix` turns it for the second product, which takes P^T, again eight columns.
 //
-// A block of four warps takes the row tile's share of the keys, a warp every fourth tile of 16, each with a
-// ring of its own in shared memory that cp.async fills a few tiles ahead: nothing is waited for but copies of the
-// warp itself.  The warps' results meet in shared memory, those of up to eight blocks of a cluster in each
-// other's; more shares than that go through memory and a second kernel.
+// A block of four warps takes a row tile's share of the keys, a warp every fourth pair of tiles of 16, each with a
+// ring of its own in shared memory that cp.async fills a pair ahead: nothing is waited for but copies of the
+// warp itself.  How keys are dealt to blocks:
+//   shares   up to eight blocks of a cluster take equal shares of a row tile's keys and put their results together
+//            in each other's shared memory;
+//   stream   as many blocks as the SMs hold take equal shares of ALL tiles of the launch, wherever one row tile's
+//            end and the next one's begin; what a block has of a row tile that it shares with others goes
+//            through memory to a second kernel.  For contexts of unlike lengths and for long ones.
 #pragma once
 #include "cache4.cuh"
 
@@ -32,9 +36,6 @@ namespace {
 
 constexpr float A4_LOG2E = 1.4426950408889634f;
 constexpr int A4_WARPS = 4;
-#ifndef A4_BLOCKS
-#define A4_BLOCKS 4
-#endif
 
 struct Attn4Params {
     const void* q;
@@ -59,10 +60,49 @@ struct Attn4Params {
     int window;                // 0: all earlier keys
     float scale_log2;
     int row_tiles;
-    int chunk_tiles;           // tiles of 16 keys a share where shares go through memory, else 0
-    int n_chunks;
-    float* partial;            // [x][chunk][8 NT][D + 2]
+    int units;                 // row tiles of all requests (or rows with picks): requests * row_tiles
+    int stream;                // blocks that share all tiles, or 0
+    float* partial;            // stream: [blocks][2][8 NT][D + 2]
 };
+
+// A row tile: rows base .. of a request (row r: token r / n_rep, head r % n_rep of the group), and the tiles of 16 keys
+// that they see some of.
+struct A4Unit {
+    int row0, n_rows, base, first, request, tile_lo, tile_hi;
+    __device__ __forceinline__ bool live() const { return base < n_rows; }
+    // Its share of the launch's work: rows that see no key are written, too.
+    __device__ __forceinline__ int weight() const { return live() ? max(1, tile_hi - tile_lo) : 0; }
+};
+
+template <int ROWS>
+__device__ __forceinline__ A4Unit a4_unit(const Attn4Params& p, int u) {
+    A4Unit v;
+    const int x = u / p.row_tiles;
+    v.base = (u - x * p.row_tiles) * ROWS;
+    v.tile_lo = v.tile_hi = 0;
+    if (p.picks != nullptr) {
+        v.row0 = x;
+        v.request = p.row_request[x];
+        v.first = p.positions[x];
+        v.n_rows = (v.request >= 0 && v.request < p.requests && v.first >= 0) ? p.n_rep : 0;
+        v.tile_hi = p.pick_count * p.page_tiles;
+        return v;
+    }
+    v.request = x;
+    v.row0 = p.row_start[x];
+    v.n_rows = v.row0 < 0 ? 0 : (min(p.row_start[x + 1], p.rows) - v.row0) * p.n_rep;
+    v.first = p.first_pos[x];
+    if (v.live()) {
+        if (p.window > 0) v.tile_lo = max(0, v.first + v.base / p.n_rep - p.window + 1) >> 4;
+        v.tile_hi = ((v.first + (min(v.n_rows, v.base + ROWS) - 1) / p.n_rep) >> 4) + 1;
+        // (what lies beyond the table is not there)
+        if (p.page_tiles > 0) v.tile_hi = (int)min((long long)v.tile_hi, (long long)p.table_stride * p.page_tiles);
+    }
+    return v;
+}
+
+// Stream: the tiles of all units and kv heads in a row (unit 0 head 0, head 1, .., unit 1 ..), dealt out in equal shares.
+__device__ __forceinline__ long long a4_quota(long long tiles, int blocks) { return max(16LL, (tiles + blocks - 1) / blocks); }
 
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -151,8 +191,9 @@ template <int D, int NG, int NT, int PARTS>
 struct A4Layout {
     static constexpr int SIDE = 16 * D / 2;                    // codes of a tile's keys, or values
     static constexpr int SCALES = 16 * NG * 4;
-    static constexpr int STAGE = 2 * SIDE + 2 * SCALES;
-    static constexpr int STAGES = D <= 64 ? 6 : D <= 128 ? 4 : 3;
+    static constexpr int TILE = 2 * SIDE + 2 * SCALES;
+    static constexpr int STAGE = 2 * TILE;                     // a pair of tiles
+    static constexpr int STAGES = D <= 64 ? 3 : 2;
     static constexpr int PITCH = D + 4;                        // floats of a row of results (lanes of four rows meet other banks)
     static constexpr int RESULT = 8 * NT * PITCH * 4;          // a warp's result takes its ring's place
     static constexpr int RING = STAGE * STAGES > RESULT ? STAGE * STAGES : RESULT;
@@ -182,8 +223,12 @@ __device__ __forceinline__ int a4_place(int r, int unit) {
     }
 }
 
+// Blocks to an SM, by the registers that a form needs.
 template <int D, int NG, int NT, bool F32>
-__global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOCKS : 2) attention4_kernel(const Attn4Params p) {
+constexpr int A4_BLOCKS = D > 128 || NT > 1 ? 2 : NG * (F32 ? 2 : 1) <= 2 ? 4 : 3;
+
+template <int D, int NG, int NT, bool F32>
+__global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) attention4_kernel(const Attn4Params p) {
     cb_pdl_trigger();
     cb_pdl_wait();
     constexpr int PARTS = F32 ? 2 : 1;
@@ -192,153 +237,198 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
     constexpr float CODE = F32 ? 1.f : 16777216.f;      // 1 over the unit of the codes
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long scan[A4_WARPS], found[3];
     // (the warp's number by way of a shuffle: known to be the same in all lanes, what follows from it lives in uniform registers)
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
-    // which rows, which keys
-    int x = blockIdx.x;
-    const int row_tile = x % p.row_tiles;
-    x /= p.row_tiles;
-    const int kv = x % p.kv_heads;
-    x /= p.kv_heads;
-    int row0, n_rows, first, request;
-    if (p.picks != nullptr) {
-        row0 = x;
-        request = p.row_request[x];
-        first = p.positions[x];
-        n_rows = (request >= 0 && request < p.requests && first >= 0) ? p.n_rep : 0;
+    // ---- which rows, which keys ------------------------------------------------
+    int index, kv;                      // the unit and its kv head
+    long long left = 0;                 // stream: tiles that the block has still to take
+    int skip = 0, slot = 0;             // ... tiles of the unit that another block takes, and which partial result comes next
+    if (p.stream > 0) {
+        long long tiles = 0;
+        for (int u = threadIdx.x; u < p.units; u += A4_WARPS * 32) tiles += a4_unit<L::ROWS>(p, u).weight();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        if (lane == 0) scan[warp] = tiles;
+        __syncthreads();
+        tiles = 0;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) tiles += scan[w];
+        tiles *= p.kv_heads;
+        const long long quota = a4_quota(tiles, p.stream), begin = quota * blockIdx.x;
+        if (begin >= tiles) return;
+        left = min(quota, tiles - begin);
+        // the unit in which the share begins
+        long long before = 0;
+        for (int u0 = 0; u0 < p.units; u0 += A4_WARPS * 32) {
+            const int u = u0 + threadIdx.x;
+            const long long mine = u < p.units ? (long long)a4_unit<L::ROWS>(p, u).weight() * p.kv_heads : 0;
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            __syncthreads();
+            if (lane == 31) scan[warp] = upto;
+            __syncthreads();
+            long long all = 0;
+#pragma unroll
+            for (int w = 0; w < A4_WARPS; ++w) {
+                if (w < warp) upto += scan[w];
+                all += scan[w];
+            }
+            upto += before;
+            if (begin < upto && begin >= upto - mine) {
+                found[0] = u;
+                found[1] = (begin - (upto - mine)) / (mine / p.kv_heads);
+                found[2] = (begin - (upto - mine)) % (mine / p.kv_heads);
+            }
+            before += all;
+            if (before > begin) break;
+        }
+        __syncthreads();
+        index = (int)found[0];
+        kv = (int)found[1];
+        skip = (int)found[2];
     } else {
-        request = x;
-        row0 = p.row_start[x];
-        n_rows = min(p.row_start[x + 1], p.rows) - row0;
-        n_rows = (row0 < 0 ? 0 : n_rows) * p.n_rep;
-        first = p.first_pos[x];
-    }
-    const int base = row_tile * L::ROWS;
-    if (base >= n_rows) return;                 // (all blocks of a cluster together)
-    const int* table = p.table + (size_t)request * p.table_stride;
-    const int last_row = min(n_rows, base + L::ROWS) - 1;
-    const int min_pos = first + base / p.n_rep, max_pos = first + last_row / p.n_rep;
-    int tile_lo = 0, tile_hi;
-    const int* picks = nullptr;
-    if (p.picks != nullptr) {
-        picks = p.picks + ((size_t)row0 * p.kv_heads + kv) * p.pick_count;
-        tile_hi = p.pick_count * p.page_tiles;
-    } else {
-        if (p.window > 0) tile_lo = max(0, min_pos - p.window + 1) >> 4;
-        tile_hi = (max_pos >> 4) + 1;
-        // (what lies beyond the table is not there)
-        if (p.page_tiles > 0) tile_hi = (int)min((long long)tile_hi, (long long)p.table_stride * p.page_tiles);
-    }
-    const int lowest = p.window > 0 ? max_pos - p.window : -1;         // a tile that begins here or before needs a look
-    int n_chunks = 1;
-    if (p.chunk_tiles > 0) {
-        n_chunks = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
-        if ((int)blockIdx.z >= max(n_chunks, 1)) return;
-        tile_lo += blockIdx.z * p.chunk_tiles;
-        if ((int)blockIdx.z + 1 < n_chunks) tile_hi = tile_lo + p.chunk_tiles;       // (the last takes what is left)
-    } else if (gridDim.z > 1) {
-        const int share = (tile_hi - tile_lo + gridDim.z - 1) / gridDim.z;
-        tile_lo += blockIdx.z * share;
-        tile_hi = min(tile_hi, tile_lo + share);
+        index = blockIdx.x / p.kv_heads;
+        kv = blockIdx.x - index * p.kv_heads;
     }
 
-    // ---- the warp's ring ----------------------------------------------------
-    const uint32_t ring = a4_smem(smem) + warp * L::RING;
-    const bool whole = p.page_tiles > 0;                 // a tile lies in one page
-    const size_t side_rows = (size_t)p.n_pages * p.kv_heads * p.page_tokens;
-    const size_t head_row = (size_t)kv * p.page_tokens;
-    const uint8_t* const code_src[2] = {p.codes + head_row * (D / 2) + lane * 16,
-                                        p.codes + (side_rows + head_row) * (D / 2) + lane * 16};
-    // (scales: lanes of both sides side by side)
-    const uint8_t* const scale_src = p.scales + (head_row + (lane >= 4 * NG ? side_rows : 0)) * (NG * 4) + (lane % (4 * NG)) * 16;
-    // Where the lane's shares of a stage lie; of keys g (and g + 8), of values 2t and 2t + 1 (and 8 behind these).
+    // Where the lane's shares of a tile lie; of keys g (and g + 8), of values 2t and 2t + 1 (and 8 behind these).
     // (kept, not worked out anew for every tile: what the compiler cannot see through it does not take apart again)
     constexpr int EIGHT = 8 * D / 2;                        // eight rows further
     uint32_t k_at = a4_place<D>(g, (t * D / 8) >> 4) + ((t * D / 8) & 15), v_at[2], s_at = 2 * L::SIDE + g * (NG * 4);
     v_at[0] = L::SIDE + a4_place<D>(2 * t, (g * D / 16) >> 4) + ((g * D / 16) & 15);
     v_at[1] = L::SIDE + a4_place<D>(2 * t + 1, (g * D / 16) >> 4) + ((g * D / 16) & 15);
     asm volatile("" : "+r"(k_at), "+r"(v_at[0]), "+r"(v_at[1]), "+r"(s_at));
+    const uint32_t ring = a4_smem(smem) + warp * L::RING;
     uint32_t place[D / 64];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) place[j] = a4_place<D>((lane + 32 * j) / (D / 32), (lane + 32 * j) % (D / 32));
+    for (int j = 0; j < D / 64; ++j) place[j] = ring + a4_place<D>((lane + 32 * j) / (D / 32), (lane + 32 * j) % (D / 32));
+    const bool whole = p.page_tiles > 0;                 // a tile lies in one page
+    const size_t side_rows = (size_t)p.n_pages * p.kv_heads * p.page_tokens;
+    const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_tokens;
+
+  for (;;) {
+    const A4Unit unit = a4_unit<L::ROWS>(p, index);
+    if (p.stream == 0 && !unit.live()) return;           // (all blocks of a cluster together)
+    const int weight = unit.weight();
+    if (weight == 0) {                                   // (stream: nothing of it is anybody's)
+        kv = 0;
+        ++index;
+        continue;
+    }
+    const int row0 = unit.row0, n_rows = unit.n_rows, base = unit.base, first = unit.first;
+    const int live = min(L::ROWS, n_rows - base);
+    const int min_pos = first + base / p.n_rep, max_pos = first + (base + live - 1) / p.n_rep;
+    const int lowest = p.window > 0 ? max_pos - p.window : -1;         // a tile that begins here or before needs a look
+    const int* table = p.table + (size_t)unit.request * p.table_stride;
+    const int* picks = p.picks != nullptr ? p.picks + ((size_t)row0 * p.kv_heads + kv) * p.pick_count : nullptr;
+    int tile_lo = unit.tile_lo, tile_hi = unit.tile_hi, taken = weight;
+    if (p.stream > 0) {
+        taken = (int)min((long long)(weight - skip), left);
+        tile_lo += skip;
+        tile_hi = min(tile_hi, tile_lo + taken);
+    } else if (gridDim.z > 1) {
+        const int share = (weight + gridDim.z - 1) / gridDim.z;
+        tile_lo += blockIdx.z * share;
+        tile_hi = min(tile_hi, tile_lo + share);
+    }
+
+    // ---- the warp's ring ----------------------------------------------------
+    const size_t head_row = (size_t)kv * p.page_tokens;
+    const uint8_t* const code_src[2] = {p.codes + head_row * (D / 2) + lane * 16,
+                                        p.codes + (side_rows + head_row) * (D / 2) + lane * 16};
+    // (scales: lanes of both sides side by side)
+    const uint8_t* const scale_src = p.scales + (head_row + (lane >= 4 * NG ? side_rows : 0)) * (NG * 4) + (lane % (4 * NG)) * 16;
     // The first key of tile i, and (whole) which page that is: -1 where there is none.
     auto key_of = [&](int i, int& page) {
-        int index = whole ? (p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse)) : 0;
+        page = whole ? -1 : 0;
+        if (i >= tile_hi) return -1;
+        if (!whole) return i * 16;
+        int index = p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse);
         if (index * p.page_tiles > i) --index;           // (rounded up, the inverse is at most one too much)
         const int slot = (i - index * p.page_tiles) * 16;
         if (picks != nullptr) index = picks[index];
-        page = !whole ? 0 : (unsigned)index < (unsigned)p.table_stride ? table[index] : -1;
+        if ((unsigned)index < (unsigned)p.table_stride) page = table[index];
         if ((unsigned)page >= (unsigned)p.n_pages) page = -1;
-        return picks != nullptr ? index * p.page_tokens + slot : i * 16;
+        return page < 0 ? -1 : picks != nullptr ? index * p.page_tokens + slot : i * 16;
     };
-    // The tiles to fetch, one after the other; 32 of them are looked up at a time, a lane each: the row (for head 0) of
-    // each, and whether some row of the block may not see some key of it.  A tile whose page is none is masked whole;
-    // what is fetched for it (the pool's first rows) is of no account, as is what lies behind a request's last token.
-    int ahead = tile_lo + warp, looked = 0;
-    uint32_t rows_of = 0, edges_of = 0xffffffffu;
-    const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_tokens;
+    // The pairs of tiles to fetch, one after the other; 32 of them are looked up at a time, a lane each: the rows (for head 0)
+    // of both tiles, and whether some row of the block may not see some key of them.  A tile whose page is none is
+    // masked whole; what is fetched for it (the pool's first rows) is of no account, as is what lies behind a request's
+    // last token.
+    int ahead = tile_lo + 2 * warp, looked = 0;
+    uint32_t rows_of[2], edges_of;
     auto look = [&]() {
-        const int i = ahead + A4_WARPS * lane;
-        int page, key = 0;
-        bool there = false;
-        if (i < tile_hi && whole) {
-            key = key_of(i, page);
-            there = page >= 0;
+        bool edge = false;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            int page;
+            const int key = key_of(ahead + 2 * A4_WARPS * lane + u, page);
+            rows_of[u] = whole && key >= 0 ? (uint32_t)page * page_rows + (uint32_t)(key % p.page_tokens) : 0u;
+            edge = edge || !whole || key < 0 || key + 15 > min_pos || key <= lowest;
         }
-        rows_of = there ? (uint32_t)page * page_rows + (uint32_t)(key % p.page_tokens) : 0u;
-        edges_of = __ballot_sync(0xffffffffu, !there || key + 15 > min_pos || key <= lowest);
+        edges_of = __ballot_sync(0xffffffffu, edge);
     };
-    uint32_t edges = 0;                    // of the tiles in flight, the next to be taken in the lowest bit
-    auto fetch = [&](int stage) {
+    uint32_t edges = 0;                    // of the pairs in flight, the next to be taken in the lowest bit
+    auto fetch = [&](uint32_t stage) {     // `stage`: bytes from the ring's beginning
         if (ahead < tile_hi) {
-            const uint32_t to = ring + stage * L::STAGE;
             if (whole) {
-                const uint32_t row = __shfl_sync(0xffffffffu, rows_of, looked);
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint8_t* src = code_src[s] + (size_t)row * (D / 2);
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t row = __shfl_sync(0xffffffffu, rows_of[u], looked);
 #pragma unroll
-                    for (int j = 0; j < D / 64; ++j) a4_copy16(to + s * L::SIDE + place[j], src + j * 512);
-                }
-                if constexpr (8 * NG <= 32) {
-                    if (lane < 8 * NG) a4_copy16(to + 2 * L::SIDE + lane * 16, scale_src + (size_t)row * (NG * 4));
-                } else {
+                    for (int s = 0; s < 2; ++s) {
+                        const uint8_t* src = code_src[s] + (size_t)row * (D / 2);
 #pragma unroll
-                    for (int c = lane; c < 8 * NG; c += 32) {
-                        const int side = c / (4 * NG), u = c % (4 * NG);
-                        a4_copy16(to + 2 * L::SIDE + c * 16,
-                                  p.scales + (head_row + row + side * side_rows) * (NG * 4) + u * 16);
+                        for (int j = 0; j < D / 64; ++j) a4_copy16(place[j] + stage + (u * L::TILE + s * L::SIDE), src + j * 512);
+                    }
+                    if constexpr (8 * NG <= 32) {
+                        if (lane < 8 * NG)
+                            a4_copy16(ring + stage + lane * 16 + (u * L::TILE + 2 * L::SIDE), scale_src + (size_t)row * (NG * 4));
+                    } else {
+#pragma unroll
+                        for (int c = lane; c < 8 * NG; c += 32) {
+                            const int side = c / (4 * NG), at = c % (4 * NG);
+                            a4_copy16(ring + stage + u * L::TILE + 2 * L::SIDE + c * 16,
+                                      p.scales + (head_row + row + side * side_rows) * (NG * 4) + at * 16);
+                        }
                     }
                 }
             } else {
-                const int key = ahead * 16;
+                const uint32_t to = ring + stage;
 #pragma unroll 1
-                for (int c = lane; c < 16 * (D / 32); c += 32) {
-                    const int r = c / (D / 32), u = c % (D / 32);
-                    const long long one = key + r <= max_pos
-                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
+                for (int c = lane; c < 32 * (D / 32); c += 32) {
+                    const int r = c / (D / 32), u = c % (D / 32), key = ahead * 16 + r;
+                    const long long one = key <= max_pos
+                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) : -1;
                     const size_t row = one >= 0 ? (size_t)one + head_row : 0;
                     const uint8_t* src = p.codes + row * (D / 2) + u * 16;
-                    a4_copy16(to + a4_place<D>(r, u), src);
-                    a4_copy16(to + L::SIDE + a4_place<D>(r, u), src + side_rows * (D / 2));
+                    const uint32_t dst = to + (r >> 4) * L::TILE + a4_place<D>(r & 15, u);
+                    a4_copy16(dst, src);
+                    a4_copy16(dst + L::SIDE, src + side_rows * (D / 2));
                 }
 #pragma unroll 1
-                for (int c = lane; c < 16 * NG; c += 32) {
-                    const int r = c / NG, u = c % NG;
-                    const long long one = key + r <= max_pos
-                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key + r) : -1;
+                for (int c = lane; c < 32 * NG; c += 32) {
+                    const int r = c / NG, u = c % NG, key = ahead * 16 + r;
+                    const long long one = key <= max_pos
+                        ? c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) : -1;
                     const size_t row = one >= 0 ? (size_t)one + head_row : 0;
                     const uint8_t* src = p.scales + (row * NG + u) * 4;
-                    a4_copy4(to + 2 * L::SIDE + c * 4, src);
-                    a4_copy4(to + 2 * L::SIDE + L::SCALES + c * 4, src + side_rows * (NG * 4));
+                    const uint32_t dst = to + (r >> 4) * L::TILE + 2 * L::SIDE + ((r & 15) * NG + u) * 4;
+                    a4_copy4(dst, src);
+                    a4_copy4(dst + L::SCALES, src + side_rows * (NG * 4));
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         edges = (edges >> 1) | (edges_of & 1u) << (L::STAGES - 2);
         edges_of >>= 1;
-        ahead += A4_WARPS;
+        ahead += 2 * A4_WARPS;
         if (++looked == 32) {
             looked = 0;
             look();
@@ -346,7 +436,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
     };
     look();
 #pragma unroll 1
-    for (int s = 0; s < L::STAGES - 1; ++s) fetch(s);
+    for (int s = 0; s < L::STAGES - 1; ++s) fetch(s * L::STAGE);
 
     // ---- the queries, as columns of the first product --------------------------
     {
@@ -439,112 +529,123 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
             for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
 
     // ---- over the keys -----------------------------------------------------------
-    // One tile.  EDGE: some row may not see some key of it.
-    auto tile = [&](auto edge, const uint8_t* at, int key0) {
+    // A pair of tiles.  EDGE: some row may not see some key of it (keys: the tiles' first, -1 for none).
+    auto pair = [&](auto edge, const uint8_t* at, int key_a, int key_b) {
         constexpr bool EDGE = decltype(edge)::value;
-        // S^T = K Q^T, by groups
-        float s[NT][4];
-        uint32_t kw[2][2 * W];
+        float s[2][NT][4];
+        uint32_t vsc[2][2][NG];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if constexpr (D == 64 || D == 192) {
+        for (int u = 0; u < 2; ++u) {
+            // S^T = K Q^T, by groups
+            const uint8_t* tile = at + u * L::TILE;
+            uint32_t kw[2][2 * W], ksc[2][NG];
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at + k_at + h * EIGHT + j * 8);
-                    kw[h][2 * j] = v.x; kw[h][2 * j + 1] = v.y;
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (D == 64 || D == 192) {
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(tile + k_at + h * EIGHT + j * 8);
+                        kw[h][2 * j] = v.x; kw[h][2 * j + 1] = v.y;
+                    }
+                } else {
+                    // (256: the lane's second unit is the first's neighbour, which the places exchange but do not part)
+#pragma unroll
+                    for (int j = 0; j < D / 128; ++j) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(tile + (j == 0 ? k_at : k_at ^ 16) + h * EIGHT);
+                        kw[h][4 * j] = v.x; kw[h][4 * j + 1] = v.y; kw[h][4 * j + 2] = v.z; kw[h][4 * j + 3] = v.w;
+                    }
                 }
-            } else {
-                // (256: the lane's second unit is the first's neighbour, which the places exchange but do not part)
-#pragma unroll
-                for (int j = 0; j < D / 128; ++j) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at + (j == 0 ? k_at : k_at ^ 16) + h * EIGHT);
-                    kw[h][4 * j] = v.x; kw[h][4 * j + 1] = v.y; kw[h][4 * j + 2] = v.z; kw[h][4 * j + 3] = v.w;
-                }
+                a4_pairs<NG>(ksc[h], tile + s_at + 8 * h * (NG * 4));
+                a4_pairs<NG>(vsc[u][h], tile + s_at + L::SCALES + 8 * h * (NG * 4));
             }
-        }
-        uint32_t ksc[2][NG], vsc[2][NG];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            a4_pairs<NG>(ksc[h], at + s_at + 8 * h * (NG * 4));
-            a4_pairs<NG>(vsc[h], at + s_at + L::SCALES + 8 * h * (NG * 4));
-        }
+            for (int gr = 0; gr < NG; ++gr) {
+                float acc[NT][4];
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-            float acc[NT][4];
+                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+                for (int b = gr * (GROUP / 32); b < (gr + 1) * (GROUP / 32); ++b) {         // 32 features
 #pragma unroll
-            for (int b = gr * (GROUP / 32); b < (gr + 1) * (GROUP / 32); ++b) {         // 32 features
+                    for (int c = 0; c < 2; ++c) {
+                        const int ks = b * 2 + c, wi = c * W + (b >> 1);
+                        const uint32_t wa = (b & 1) ? kw[0][wi] >> 8 : kw[0][wi], wb = (b & 1) ? kw[1][wi] >> 8 : kw[1][wi];
+                        const uint32_t a0 = a4_codes<F32, false>(wa), a1 = a4_codes<F32, false>(wb);
+                        const uint32_t a2 = a4_codes<F32, true>(wa), a3 = a4_codes<F32, true>(wb);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int ks = b * 2 + c, wi = c * W + (b >> 1);
-                    const uint32_t wa = (b & 1) ? kw[0][wi] >> 8 : kw[0][wi], wb = (b & 1) ? kw[1][wi] >> 8 : kw[1][wi];
-                    const uint32_t a0 = a4_codes<F32, false>(wa), a1 = a4_codes<F32, false>(wb);
-                    const uint32_t a2 = a4_codes<F32, true>(wa), a3 = a4_codes<F32, true>(wb);
+                        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            uint2 q;
-                            if constexpr (Q_IN_REGS) q = qr[(ks * PARTS + part) * NT + n];
-                            else q = qf[((ks * PARTS + part) * NT + n) * 32];
-                            a4_mma(acc[n], a0, a1, a2, a3, q.x, q.y);
-                        }
+                            for (int n = 0; n < NT; ++n) {
+                                uint2 q;
+                                if constexpr (Q_IN_REGS) q = qr[(ks * PARTS + part) * NT + n];
+                                else q = qf[((ks * PARTS + part) * NT + n) * 32];
+                                a4_mma(acc[n], a0, a1, a2, a3, q.x, q.y);
+                            }
+                    }
                 }
-            }
-            const float sa = c4_step(ksc[0][gr]) * CODE, la = a4_low<F32>(ksc[0][gr]);
-            const float sb = c4_step(ksc[1][gr]) * CODE, lb = a4_low<F32>(ksc[1][gr]);
+                const float sa = c4_step(ksc[0][gr]) * CODE, la = a4_low<F32>(ksc[0][gr]);
+                const float sb = c4_step(ksc[1][gr]) * CODE, lb = a4_low<F32>(ksc[1][gr]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float wa = gr == 0 ? la * qsum[n][gr][c] : fmaf(la, qsum[n][gr][c], s[n][c]);
-                    const float wb = gr == 0 ? lb * qsum[n][gr][c] : fmaf(lb, qsum[n][gr][c], s[n][2 + c]);
-                    s[n][c] = fmaf(acc[n][c], sa, wa);
-                    s[n][2 + c] = fmaf(acc[n][2 + c], sb, wb);
+                    for (int c = 0; c < 2; ++c) {
+                        const float wa = gr == 0 ? la * qsum[n][gr][c] : fmaf(la, qsum[n][gr][c], s[u][n][c]);
+                        const float wb = gr == 0 ? lb * qsum[n][gr][c] : fmaf(lb, qsum[n][gr][c], s[u][n][2 + c]);
+                        s[u][n][c] = fmaf(acc[n][c], sa, wa);
+                        s[u][n][2 + c] = fmaf(acc[n][2 + c], sb, wb);
+                    }
                 }
             }
         }
 
-        // what a row does not see: bits 4 n + 2 h + c
+        // what a row does not see: bits 4 NT u + 4 n + 2 h + c
         uint32_t hidden = 0;
         if constexpr (EDGE) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int key = key0 + g + 8 * h;
-                        bool out = key0 < 0 || key > pos[n][c] || (p.window > 0 && key <= pos[n][c] - p.window);
-                        if (!whole && !out)
-                            out = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) < 0;
-                        if (out) {
-                            s[n][2 * h + c] = -INFINITY;
-                            hidden |= 1u << (4 * n + 2 * h + c);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int key0 = u == 0 ? key_a : key_b, key = key0 + g + 8 * h;
+                            bool out = key0 < 0 || key > pos[n][c] || (p.window > 0 && key <= pos[n][c] - p.window);
+                            if (!whole && !out)
+                                out = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) < 0;
+                            if (out) {
+                                s[u][n][2 * h + c] = -INFINITY;
+                                hidden |= 1u << (4 * NT * u + 4 * n + 2 * h + c);
+                            }
                         }
-                    }
         }
 
         // the references move only when they have to
-        float most_step[2];
+        float most_step[2][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            most_step[h] = c4_step(vsc[h][0]);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int gr = 1; gr < NG; ++gr) most_step[h] = fmaxf(most_step[h], c4_step(vsc[h][gr]));
-        }
+            for (int h = 0; h < 2; ++h) {
+                most_step[u][h] = c4_step(vsc[u][h][0]);
+#pragma unroll
+                for (int gr = 1; gr < NG; ++gr) most_step[u][h] = fmaxf(most_step[u][h], c4_step(vsc[u][h][gr]));
+            }
         bool move = false;
         float top[NT][2], step_top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                top[n][c] = fmaxf(s[n][c], s[n][2 + c]);
-                if constexpr (EDGE)
-                    step_top[n][c] = fmaxf((hidden >> (4 * n + c)) & 1 ? 0.f : most_step[0],
-                                           (hidden >> (4 * n + 2 + c)) & 1 ? 0.f : most_step[1]);
-                else step_top[n][c] = fmaxf(most_step[0], most_step[1]);
+                top[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+                step_top[n][c] = 0.f;
+                if constexpr (EDGE) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (!((hidden >> (4 * NT * u + 4 * n + 2 * h + c)) & 1)) step_top[n][c] = fmaxf(step_top[n][c], most_step[u][h]);
+                } else {
+                    step_top[n][c] = fmaxf(fmaxf(most_step[0][0], most_step[0][1]), fmaxf(most_step[1][0], most_step[1][1]));
+                }
                 move = move || fmaf(top[n][c], factor[n][c], -off[n][c]) > limit[n][c] || step_top[n][c] >= bound[n][c];
             }
         if (__any_sync(0xffffffffu, move)) {
@@ -571,105 +672,109 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
                 }
         }
 
-        // p, and P^T step as columns of the second product
-        uint32_t b[NG][PARTS][NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float pr[4];
+        for (int u = 0; u < 2; ++u) {
+            // p, and P^T step as columns of the second product
+            uint32_t b[NG][PARTS][NT][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                pr[j] = a4_exp2(fmaf(s[n][j], factor[n][j & 1], -off[n][j & 1]));
-                sum[n][j & 1] += pr[j];
-            }
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                float w[4];
+            for (int n = 0; n < NT; ++n) {
+                float pr[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    w[j] = pr[j] * c4_step(vsc[j >> 1][gr]);
-                    float low = a4_low<F32>(vsc[j >> 1][gr]);
-                    if constexpr (EDGE)
-                        if ((hidden >> (4 * n + j)) & 1) w[j] = low = 0.f;       // (what nobody wrote may be no number)
-                    lows[n][gr][j & 1] = fmaf(pr[j], low, lows[n][gr][j & 1]);
+                    pr[j] = a4_exp2(fmaf(s[u][n][j], factor[n][j & 1], -off[n][j & 1]));
+                    sum[n][j & 1] += pr[j];
                 }
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    const uint32_t h0 = a4_half2(w[0], w[1]), h1 = a4_half2(w[2], w[3]);
-                    if constexpr (PARTS == 2) {
-                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                        w[0] -= f0.x; w[1] -= f0.y; w[2] -= f1.x; w[3] -= f1.y;
+                for (int gr = 0; gr < NG; ++gr) {
+                    float w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[j] = pr[j] * c4_step(vsc[u][j >> 1][gr]);
+                        float low = a4_low<F32>(vsc[u][j >> 1][gr]);
+                        if constexpr (EDGE)
+                            if ((hidden >> (4 * NT * u + 4 * n + j)) & 1) w[j] = low = 0.f;   // (what nobody wrote may be no number)
+                        lows[n][gr][j & 1] = fmaf(pr[j], low, lows[n][gr][j & 1]);
                     }
-                    b[gr][part][n][0] = a4_turned(h0);
-                    b[gr][part][n][1] = a4_turned(h1);
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const uint32_t h0 = a4_half2(w[0], w[1]), h1 = a4_half2(w[2], w[3]);
+                        if constexpr (PARTS == 2) {
+                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                            w[0] -= f0.x; w[1] -= f0.y; w[2] -= f1.x; w[3] -= f1.y;
+                        }
+                        b[gr][part][n][0] = a4_turned(h0);
+                        b[gr][part][n][1] = a4_turned(h1);
+                    }
                 }
             }
-        }
 
-        // O^T += V^T P^T
-        uint32_t vw[4][W];
+            // O^T += V^T P^T
+            uint32_t vw[4][W];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint8_t* from = at + v_at[j & 1] + (j >> 1) * EIGHT;
-            if constexpr (D == 128) {
-                const uint2 v = *reinterpret_cast<const uint2*>(from);
-                vw[j][0] = v.x; vw[j][1] = v.y;
-            } else if constexpr (D == 256) {
-                const uint4 v = *reinterpret_cast<const uint4*>(from);
-                vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
-            } else {
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t* from = at + u * L::TILE + v_at[j & 1] + (j >> 1) * EIGHT;
+                if constexpr (D == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(from);
+                    vw[j][0] = v.x; vw[j][1] = v.y;
+                } else if constexpr (D == 256) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(from);
+                    vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
+                } else {
 #pragma unroll
-                for (int w = 0; w < W; ++w) vw[j][w] = reinterpret_cast<const uint32_t*>(from)[w];
+                    for (int w = 0; w < W; ++w) vw[j][w] = reinterpret_cast<const uint32_t*>(from)[w];
+                }
             }
-        }
 #pragma unroll
-        for (int w = 0; w < W; ++w)
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                // half words of two keys side by side: features of tiles 4w + half and 4w + 2 + half
-                uint32_t z0 = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
-                uint32_t z1 = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
+                for (int half = 0; half < 2; ++half) {
+                    // half words of two keys side by side: features of tiles 4w + half and 4w + 2 + half
+                    uint32_t z0 = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
+                    uint32_t z1 = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int m = 4 * w + 2 * u + half, gr = m * 16 / GROUP;
-                    if (u == 1) { z0 >>= 8; z1 >>= 8; }
-                    const uint32_t a0 = a4_codes<F32, false>(z0), a1 = a4_codes<F32, true>(z0);
-                    const uint32_t a2 = a4_codes<F32, false>(z1), a3 = a4_codes<F32, true>(z1);
+                    for (int v = 0; v < 2; ++v) {
+                        const int m = 4 * w + 2 * v + half, gr = m * 16 / GROUP;
+                        if (v == 1) { z0 >>= 8; z1 >>= 8; }
+                        const uint32_t a0 = a4_codes<F32, false>(z0), a1 = a4_codes<F32, true>(z0);
+                        const uint32_t a2 = a4_codes<F32, false>(z1), a3 = a4_codes<F32, true>(z1);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if constexpr (F32) {
-                            float part[4] = {0.f, 0.f, 0.f, 0.f};
-                            a4_mma(part, a0, a1, a2, a3, b[gr][1][n][0], b[gr][1][n][1]);
-                            a4_mma(part, a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (F32) {
+                                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                                a4_mma(part, a0, a1, a2, a3, b[gr][1][n][0], b[gr][1][n][1]);
+                                a4_mma(part, a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) o[m][n][j] += part[j];
-                        } else {
-                            a4_mma(o[m][n], a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
+                                for (int j = 0; j < 4; ++j) o[m][n][j] += part[j];
+                            } else {
+                                a4_mma(o[m][n], a0, a1, a2, a3, b[gr][0][n][0], b[gr][0][n][1]);
+                            }
                         }
                     }
                 }
-            }
+        }
     };
-    int into = L::STAGES - 1;              // the stage that was read last, to be filled; the next one is to be read
+    // the stage that was read last, to be filled; the next one is to be read
+    uint32_t into = (L::STAGES - 1) * L::STAGE;
     auto next = [&]() -> const uint8_t* {
         asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
         __syncwarp();
         fetch(into);
-        into = into + 1 == L::STAGES ? 0 : into + 1;
-        return smem + warp * L::RING + into * L::STAGE;
+        into = into == (L::STAGES - 1) * L::STAGE ? 0 : into + L::STAGE;
+        return smem + warp * L::RING + into;
     };
     // (two loops, so that the one over whole tiles is nothing else: one loop that chose between the two forms moved
     // registers about at every turn)
-    for (int i = tile_lo + warp; i < tile_hi; i += A4_WARPS) {
+    for (int i = tile_lo + 2 * warp; i < tile_hi; i += 2 * A4_WARPS) {
         while (!(edges & 1)) {
-            tile(std::false_type{}, next(), 0);
-            i += A4_WARPS;
+            pair(std::false_type{}, next(), 0, 0);
+            i += 2 * A4_WARPS;
             if (i >= tile_hi) break;
         }
         if (i >= tile_hi) break;
         int page;
-        const int key0 = key_of(i, page);
-        tile(std::true_type{}, next(), page < 0 ? -1 : key0);
+        const int key_a = key_of(i, page), key_b = key_of(i + 1, page);
+        pair(std::true_type{}, next(), key_a, key_b);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -716,7 +821,6 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
         block_state[r * 2 + 1] = l;
     }
     __syncthreads();
-    const int live = min(L::ROWS, n_rows - base);
     auto of_block = [&](int i) {
         const int r = i / D;
         float v = 0.f;
@@ -729,19 +833,33 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
         const int r = i / D, tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
         reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + (i - r * D)] = cb_from_float<T>(v);
     };
-    if (p.chunk_tiles > 0 && n_chunks > 1) {
-        float* to = p.partial + ((size_t)blockIdx.x * p.n_chunks + blockIdx.z) * (L::ROWS * (D + 2));
-        for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32) to[2 * L::ROWS + i] = of_block(i);
-        if (threadIdx.x < 2 * live) to[threadIdx.x] = block_state[threadIdx.x];
-        return;
+    if (p.stream > 0) {
+        if (taken < weight) {                            // the other blocks' results of it are needed, too
+            float* to = p.partial + ((size_t)blockIdx.x * 2 + slot) * (L::ROWS * (D + 2));
+            for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32) to[2 * L::ROWS + i] = of_block(i);
+            if (threadIdx.x < 2 * live) to[threadIdx.x] = block_state[threadIdx.x];
+        }
     }
-    if (p.chunk_tiles > 0 || gridDim.z == 1) {
+    if (p.stream > 0 ? taken == weight : gridDim.z == 1) {
         for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32) {
             const float l = block_state[(i / D) * 2 + 1];
             store(i, l == 0.f ? 0.f : of_block(i) / l);          // (a row that sees no key: zeros)
         }
-        return;
     }
+    if (p.stream > 0) {
+        left -= taken;
+        if (left == 0) return;
+        // the next kv head, or unit
+        skip = 0;
+        slot = 1;                                        // (what follows is shared only if it is the last)
+        if (++kv == p.kv_heads) {
+            kv = 0;
+            ++index;
+        }
+        __syncthreads();
+        continue;
+    }
+    if (gridDim.z == 1) return;
     // blocks of a cluster: each takes its share of the numbers from all
     for (int i = threadIdx.x; i < live * D; i += A4_WARPS * 32)
         reinterpret_cast<float*>(smem)[i + i / D * (L::PITCH - D)] = of_block(i);      // (over warp 0's, which this thread alone reads)
@@ -775,93 +893,99 @@ __global__ void __launch_bounds__(A4_WARPS * 32, (D <= 128 && NT == 1) ? A4_BLOC
         store(i, l == 0.f ? 0.f : v / l);
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    return;
+  }
 }
 
-// Shares that went through memory: one block a row, D / 4 threads a share side by side.
-constexpr int A4_MOST_CHUNKS = 1024;
-
+// Stream: a row whose tile several blocks had a share of, a block a row, D / 4 threads a result side by side.  The first of
+// these blocks has it as its second result (unless its share begins there), the others as their first.
 template <int D, int NT, bool F32>
 __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params p) {
     cb_pdl_trigger();
-    constexpr int ROWS = 8 * NT, LANES = D / 4, SETS = 256 / LANES;
+    constexpr int ROWS = 8 * NT, LANES = D / 4, SETS = 256 / LANES, ONE = ROWS * (D + 2);
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-    __shared__ float weights[A4_MOST_CHUNKS], part[8];
+    __shared__ float weights[256], part[8];
+    __shared__ long long counts[2][8];
     __shared__ float4 sums[SETS][LANES];
     cb_pdl_wait();
-    const int r = blockIdx.y;
-    int x = blockIdx.x;
-    const int row_tile = x % p.row_tiles;
-    x /= p.row_tiles;
-    const int kv = x % p.kv_heads;
-    x /= p.kv_heads;
-    int row0, n_rows, first, tile_lo = 0, tile_hi;
-    const int base = row_tile * ROWS;
-    if (p.picks != nullptr) {
-        row0 = x;
-        const int request = p.row_request[x];
-        first = p.positions[x];
-        n_rows = (request >= 0 && request < p.requests && first >= 0) ? p.n_rep : 0;
-        tile_hi = p.pick_count * p.page_tiles;
-    } else {
-        row0 = p.row_start[x];
-        n_rows = (row0 < 0 ? 0 : min(p.row_start[x + 1], p.rows) - row0) * p.n_rep;
-        first = p.first_pos[x];
-        if (p.window > 0) tile_lo = max(0, first + base / p.n_rep - p.window + 1) >> 4;
-        tile_hi = ((first + (min(n_rows, base + ROWS) - 1) / p.n_rep) >> 4) + 1;
-        if (p.page_tiles > 0) tile_hi = (int)min((long long)tile_hi, (long long)p.table_stride * p.page_tiles);
-    }
-    if (base + r >= n_rows) return;
-    const int n = min((tile_hi - tile_lo + p.chunk_tiles - 1) / p.chunk_tiles, p.n_chunks);
-    if (n <= 1) return;                          // (its block has written the row)
-    constexpr int ONE = ROWS * (D + 2);
-    const float* from = p.partial + (size_t)blockIdx.x * p.n_chunks * ONE;
+    const int r = blockIdx.y, index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads;
     const int tid = threadIdx.x, set = tid / LANES, lane = tid % LANES;
-    // weights of the shares
-    float top = -3.4e38f;
-    for (int z = tid; z < n; z += 256) {
-        weights[z] = from[(size_t)z * ONE + 2 * r];
-        top = fmaxf(top, weights[z]);
+    const A4Unit unit = a4_unit<ROWS>(p, index);
+    if (unit.base + r >= unit.n_rows) return;
+    long long tiles = 0, before = 0;
+    for (int u = tid; u < p.units; u += 256) {
+        const int w = a4_unit<ROWS>(p, u).weight();
+        tiles += w;
+        if (u < index) before += w;
     }
-    top = cb_warp_max(top);
-    if ((tid & 31) == 0) part[tid >> 5] = top;
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, part[i]);
-    float l = 0.f;
-    for (int z = tid; z < n; z += 256) {
-        const float w = a4_exp2(weights[z] - top);
-        weights[z] = w;
-        l = fmaf(from[(size_t)z * ONE + 2 * r + 1], w, l);
+    for (int o = 16; o > 0; o >>= 1) {
+        tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
     }
-    l = cb_warp_sum(l);
-    __syncthreads();
-    if ((tid & 31) == 0) part[tid >> 5] = l;
-    __syncthreads();
-    if (set < SETS) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float* mine = from + 2 * ROWS + r * D + lane * 4;
-#pragma unroll 4
-        for (int z = set; z < n; z += SETS) {
-            const float4 one = *reinterpret_cast<const float4*>(mine + (size_t)z * ONE);
-            const float w = weights[z];
-            v.x = fmaf(one.x, w, v.x);
-            v.y = fmaf(one.y, w, v.y);
-            v.z = fmaf(one.z, w, v.z);
-            v.w = fmaf(one.w, w, v.w);
-        }
-        sums[set][lane] = v;
+    if ((tid & 31) == 0) {
+        counts[0][tid >> 5] = tiles;
+        counts[1][tid >> 5] = before;
     }
     __syncthreads();
-    if (tid < D) {
-        float v = 0.f;
+    tiles = before = 0;
 #pragma unroll
-        for (int i = 0; i < SETS; ++i) v += reinterpret_cast<const float*>(sums[i])[tid];
-        l = 0.f;
+    for (int i = 0; i < 8; ++i) {
+        tiles += counts[0][i];
+        before += counts[1][i];
+    }
+    const long long quota = a4_quota(tiles * p.kv_heads, p.stream);
+    const long long begin = before * p.kv_heads + (long long)kv * unit.weight();
+    const int from = (int)(begin / quota), n = (int)((begin + unit.weight() - 1) / quota) - from + 1;
+    if (n <= 1) return;                          // (its block has written the row)
+    const bool second = begin != quota * from;
+    auto result = [&](int z) { return p.partial + ((size_t)(from + z) * 2 + (z == 0 && second ? 1 : 0)) * ONE; };
+    // their weights, and the sum
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -3.4e38f, l = 0.f;
+    for (int z0 = 0; z0 < n; z0 += 256) {        // (as a rule once: few blocks share a row tile)
+        const int here = min(256, n - z0);
+        float ref = -3.4e38f;
+        if (tid < here) ref = result(z0 + tid)[2 * r];
+        float most = fmaxf(top, cb_warp_max(ref));
+        __syncthreads();
+        if ((tid & 31) == 0) part[tid >> 5] = most;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, part[i]);
+        const float w = tid < here ? a4_exp2(ref - most) : 0.f, corr = a4_exp2(top - most);
+        float mine = tid < here ? result(z0 + tid)[2 * r + 1] * w : 0.f;
+        mine = cb_warp_sum(mine);
+        weights[tid] = w;
+        __syncthreads();
+        if ((tid & 31) == 0) part[tid >> 5] = mine;
+        __syncthreads();
+        l *= corr;
 #pragma unroll
         for (int i = 0; i < 8; ++i) l += part[i];
-        const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
-        reinterpret_cast<T*>(p.out)[(size_t)(row0 + tok) * p.out_stride + (size_t)head * D + tid] =
-            cb_from_float<T>(l == 0.f ? 0.f : v / l);
+        v.x *= corr; v.y *= corr; v.z *= corr; v.w *= corr;
+        if (set < SETS) {
+#pragma unroll 4
+            for (int z = set; z < here; z += SETS) {
+                const float2* one = reinterpret_cast<const float2*>(result(z0 + z) + 2 * ROWS + r * D + lane * 4);
+                const float2 a = one[0], b = one[1];
+                v.x = fmaf(a.x, weights[z], v.x);
+                v.y = fmaf(a.y, weights[z], v.y);
+                v.z = fmaf(b.x, weights[z], v.z);
+                v.w = fmaf(b.y, weights[z], v.w);
+            }
+        }
+        top = most;
+    }
+    if (set < SETS) sums[set][lane] = v;
+    __syncthreads();
+    if (tid < D) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) x += reinterpret_cast<const float*>(sums[i])[tid];
+        const int tok = (unit.base + r) / p.n_rep, head = kv * p.n_rep + (unit.base + r) - tok * p.n_rep;
+        reinterpret_cast<T*>(p.out)[(size_t)(unit.row0 + tok) * p.out_stride + (size_t)head * D + tid] =
+            cb_from_float<T>(l == 0.f ? 0.f : x / l);
     }
 }
 
@@ -877,11 +1001,10 @@ int attention4_launch(const Attn4Params& p, long long blocks, int shares, cudaSt
         if (rc != 0) return rc;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    const bool through_memory = p.chunk_tiles > 0;
-    const dim3 grid((unsigned)blocks, 1, (unsigned)(through_memory ? p.n_chunks : shares));
+    const dim3 grid((unsigned)(p.stream > 0 ? p.stream : blocks), 1, (unsigned)(p.stream > 0 ? 1 : shares));
     int rc = cb_launch_cluster(attention4_kernel<D, NG, NT, F32>, grid, dim3(A4_WARPS * 32), L::TOTAL, stream,
-                               through_memory ? 1 : shares, p);
-    if (rc == 0 && through_memory)
+                               p.stream > 0 ? 1 : shares, p);
+    if (rc == 0 && p.stream > 0)
         rc = cb_launch(attention4_merge_kernel<D, NT, F32>, dim3((unsigned)blocks, 8 * NT), dim3(256), 0, stream, p);
     return rc;
 }
@@ -902,14 +1025,16 @@ int attention4_of(const Attn4Params& p, int dtype, int column_tiles, long long b
         if (D % group != 0 || column_tiles < 1 || column_tiles > 2 || shares < 1 || shares > 8) return CB_ERR_UNSUPPORTED; \
         const int rows_a_tile = 8 * column_tiles;                                                                        \
         const int row_tiles = (most_rows * n_rep + rows_a_tile - 1) / rows_a_tile;                                       \
-        const long long blocks = (long long)(picks != nullptr ? rows : requests) * kv_heads * row_tiles;                 \
+        const long long units = (long long)(picks != nullptr ? rows : requests) * row_tiles, blocks = units * kv_heads;  \
         if (blocks <= 0) return 0;                                                                                       \
-        if (blocks >= (1LL << 31) || n_chunks > A4_MOST_CHUNKS) return CB_ERR_UNSUPPORTED;                                        \
+        if (blocks >= (1LL << 31)) return CB_ERR_UNSUPPORTED;                                                            \
+        const int page_tiles = page_tokens % 16 ? 0 : page_tokens / 16;                                                  \
         const Attn4Params p = {q, q_stride, out, out_stride, reinterpret_cast<const uint8_t*>(codes),                    \
                                reinterpret_cast<const uint8_t*>(scales), n_pages, page_tokens, kv_heads, n_rep,          \
                                row_start, first_pos, table, table_stride, requests, picks, pick_count, row_request,      \
-                               positions, rows, page_tokens % 16 ? 0 : page_tokens / 16,                                 \
-                               page_tokens % 16 || page_tokens == 16 ? 0u : (uint32_t)((1ull << 32) / (page_tokens / 16)) + 1u, window, scale * A4_LOG2E, row_tiles, chunk_tiles, n_chunks, partial};    \
+                               positions, rows, page_tiles,                                                              \
+                               page_tiles <= 1 ? 0u : (uint32_t)((1ull << 32) / page_tiles) + 1u, window,                \
+                               scale * A4_LOG2E, row_tiles, (int)units, stream_blocks, partial};                         \
         const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);                                                   \
         int rc = CB_ERR_UNSUPPORTED;                                                                                     \
         if (group == 32) rc = attention4_of<D, D / 32>(p, dtype, column_tiles, blocks, shares, s);                       \

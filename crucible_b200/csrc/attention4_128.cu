@@ -6,6 +6,6 @@ CB_EXPORT int cb_attention4(const void* q, int dtype, long long q_stride, void* 
                             const void* scales, int n_pages, int page_tokens, int kv_heads, int n_rep, int group,
                             const int* row_start, const int* first_pos, const int* table, int table_stride, int requests,
                             const int* picks, int pick_count, const int* row_request, const int* positions, int rows,
-                            int most_rows, int window, float scale, int column_tiles, int shares, int chunk_tiles,
-                            int n_chunks, float* partial, void* stream)
+                            int most_rows, int window, float scale, int column_tiles, int shares, int stream_blocks,
+                            float* partial, void* stream)
 ATTENTION4_ENTRY(128)

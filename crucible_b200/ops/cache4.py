@@ -312,17 +312,25 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         _walk(q, out, n_heads, scale, batch, pages, window, None, behind, batch.requests)
 
 
-_RESIDENT = 4 * tensor_core.N_SMS     # blocks of one column tile that the SMs hold at once
+def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
+    """Blocks of the walking kernel that the SMs hold at once."""
+    return tensor_core.N_SMS * (2 if dim > 128 or columns > 1 else 4 if dim // group * (2 if f32 else 1) <= 2 else 3)
 
 
-def _shares(blocks: int, tiles: int) -> tuple:
-    """(blocks of a cluster, tiles a share through memory or 0, shares): how the keys of a row tile are dealt, by the
-    launch's blocks and the most tiles of 16 keys that a row sees."""
-    want = max(1, min(_RESIDENT // max(1, blocks), tiles // 8))
+def _shares(blocks: int, tiles: int, total: int, resident: int) -> tuple:
+    """(blocks of a cluster, blocks of a stream or 0): how the keys are dealt, by the launch's row tiles of all kv heads
+    (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
+    hold."""
+    if blocks >= 4 * resident:
+        return 1, 0
+    fit, most = resident // blocks, tiles // 16
+    want = max(1, min(fit, most))
     if want <= 8:
-        return 1 << (want.bit_length() - 1), 0, 1
-    chunk = -(-tiles // want)
-    return 1, chunk, -(-tiles // chunk)
+        shares = 1 << (want.bit_length() - 1)
+        waves = -(-blocks * shares // resident)
+        if most <= fit or total * shares * 4 >= tiles * waves * resident * 3:
+            return shares, 0
+    return 1, max(1, min(resident, total // 16))
 
 
 def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
@@ -334,16 +342,17 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     if picks is not None:
         most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
+        total = tiles * blocks
     else:
         most_rows, blocks = max(batch.new_tokens[first:last]), last - first
         reach = batch.reach if window is None else min(batch.reach, window + most_rows)
         tiles = -(-reach // 16) + (window is not None)
+        total = sum([min(h + n, reach) for h, n in zip(batch.held_tokens[first:last], batch.new_tokens[first:last])]) // 16 + blocks
     columns = 1 if f32 or most_rows * n_rep <= 8 else 2
-    blocks *= kv * -(-most_rows * n_rep // (8 * columns))
-    shares, chunk, chunks = _shares(blocks, tiles)
-    partial = None
-    if chunk:
-        partial = torch.empty(blocks * chunks * 8 * columns * (dim + 2), dtype=_F32, device=q.device)
+    per = kv * -(-most_rows * n_rep // (8 * columns))
+    blocks, total = blocks * per, total * per
+    shares, stream = _shares(blocks, tiles, total, _resident(dim, pages.group, columns, f32))
+    partial = torch.empty(stream * 16 * columns * (dim + 2), dtype=_F32, device=q.device) if stream else None
     lib = build.load(f"attention4_{dim}")
     code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),
                pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv, n_rep, pages.group,
@@ -353,7 +362,7 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
                picks.data_ptr() if picks is not None else 0, picks.shape[2] if picks is not None else 0,
                batch.row_request.data_ptr(), batch.positions.data_ptr(),
                rows if picks is None else min(rows, picks.shape[0]), most_rows, window or 0, scale, columns,
-               shares, chunk, chunks, partial.data_ptr() if partial is not None else 0)
+               shares, stream, partial.data_ptr() if partial is not None else 0)
     if code == build.UNSUPPORTED:
         raise KernelError(f"attention4: {blocks} blocks of rows are more than a launch takes")
     _check(code, "attention4")

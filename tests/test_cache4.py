@@ -161,14 +161,14 @@ def test_calls_that_are_refused():
 
 def test_keys_are_dealt_to_as_many_blocks_as_there_is_room_for():
     cache4, _ = _ops()
-    for blocks in (1, 2, 8, 37, 148, 512, 100000):
-        for tiles in (1, 7, 8, 60, 500, 8192, 1 << 20):
-            shares, chunk, chunks = cache4._shares(blocks, tiles)
-            assert shares in (1, 2, 4, 8) and (shares == 1 or chunk == 0)
-            if chunk:
-                assert chunks > 1 and chunk * chunks >= tiles and chunk * (chunks - 1) < tiles and chunk >= 8
-            else:
-                assert chunks == 1 and (shares == 1 or tiles >= 8 * shares)
+    for resident in (296, 444, 592):
+        for blocks in (1, 2, 8, 37, 148, 512, 700, 100000):
+            for tiles in (1, 7, 8, 60, 500, 8192, 1 << 20):
+                for total in (blocks * tiles, blocks + tiles):
+                    shares, stream = cache4._shares(blocks, tiles, total, resident)
+                    assert shares in (1, 2, 4, 8) and (shares == 1 or stream == 0)
+                    assert 0 <= stream <= resident and (stream or blocks >= 4 * resident or shares * blocks <= max(blocks, resident))
+                    assert shares == 1 or tiles >= 16 * shares
 
 
 def test_pages_are_scored_by_no_more_blocks_than_a_cluster_has():
