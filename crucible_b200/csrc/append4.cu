@@ -1,8 +1,9 @@
 // Writing the cache in 4 bits, and reading it back as it stands.
 //
 //   append4   a row's q and k are rotated by its position, k and v go to the row's place in the pages.
-//             D/8 lanes a (row, head), eight neighbouring features a lane: 16 bytes a load where rows are
-//             aligned.  Lane l of eight takes the features whose codes lie at bits 4l.. 4l + 3 of their words, so that
+//             A block a row and a run of its heads, so that its position, place and angles are fetched once; D/8
+//             lanes a head, eight neighbouring features a lane: 16 bytes a load where rows are aligned, the next
+//             head's before this one's are worked on.  Lane l of eight takes the features whose codes lie at bits 4l.. 4l + 3 of their words, so that
 //             eight lanes' codes are turned into eight words by a transposition of 8 x 8 nibbles, three
 //             shuffles; a group's least and largest number take two to four shuffles each.
 //   bounds4   of every page that the step wrote: each feature's largest and least key over the tokens that
@@ -74,9 +75,15 @@ __device__ __forceinline__ Coding coding_of(float least, float largest) {
     return c;
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, const Coding& c) {
-    const float v = rintf(__fmul_rn(__fsub_rn(x, c.low), c.inverse));
-    return (uint32_t)fminf(fmaxf(v, 0.f), 15.f);
+// Eight codes of a group, the e-th in bits 4e.. 4e + 3.  (x - low) * inverse lies in 0 .. 15.06 (low is not above x, and the
+// step is off by 2^-8 of it at most), so that adding 1.5 2^23 rounds it to the nearest, ties to even, and leaves the code in
+// the lowest bits; what else these numbers' bits hold is the same for all eight and goes with one subtraction.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], const Coding& c) {
+    uint32_t m = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        m += __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(x[e], c.low), c.inverse), 12582912.f)) << (4 * e);
+    return m;
 }
 
 // Eight neighbouring numbers (VEC: aligned to 16 bytes).
@@ -115,81 +122,117 @@ __device__ __forceinline__ void store_eight(T* dst, const float (&v)[8]) {
     }
 }
 
-// VEC: rows are aligned to 16 bytes, and half of the rotated features is a multiple of eight.
-template <int D, int GROUP, typename T, bool VEC>
-__global__ void __launch_bounds__(256) append4_kernel(const AppendParams p) {
-    cb_pdl_trigger();
-    cb_pdl_wait();
-    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, W = D / 64, NG = D / GROUP;
-    const int lane = threadIdx.x & 31, within = lane % LANES;
-    const int w = within >> 3, l = within & 7;
-    const int k = (l & 1) | ((l & 2) << 1) | ((l & 4) >> 1);            // (0, 1, 4, 5, 2, 3, 6, 7)[l]
-    const int f = 64 * w + 8 * k;
-    const int heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0);
-    const long long items = (long long)p.rows * heads;
-    const long long stride = (long long)gridDim.x * 8 * PER_WARP;
-    const long long begin = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP;
-    for (long long at_item = begin; at_item < items; at_item += stride) {         // (whole warps: shuffles)
-        const long long item = at_item + lane / LANES;
-        const bool mine = item < items && lane < LANES * PER_WARP;
-        const int row = mine ? (int)(item / heads) : 0, head = mine ? (int)(item - (long long)row * heads) : 0;
-        const int request = p.row_request[row], pos = p.positions[row];
-        const bool live = mine && request >= 0 && request < p.n_requests && pos >= 0 && !(p.rotary > 0 && pos >= p.n_positions);
-        const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)row * p.qkv_stride + (size_t)head * D;
-        long long at = -1;
-        const int side = head >= p.n_heads + p.kv_heads;
-        if (live && head >= p.n_heads) {
-            at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-            if (at >= 0) at += (long long)(head - p.n_heads - side * p.kv_heads) * p.page_tokens
-                             + (long long)side * p.n_pages * p.kv_heads * p.page_tokens;
-        }
-        float x[8];
-        if (live) {
-            load_eight<T, VEC>(src + f, x);
-            if (f < p.rotary && head < p.n_heads + p.kv_heads) {
-                const int half = p.rotary >> 1;
-                const float* cs = p.cos_t + (size_t)pos * half;
-                const float* sn = p.sin_t + (size_t)pos * half;
-                if (VEC && !p.neighbours) {
-                    const bool first = f < half;
-                    float y[8], c[8], s[8];
-                    const int j = first ? f : f - half;
-                    load_eight<T, VEC>(src + (first ? f + half : j), y);
-                    load_eight<float, VEC>(cs + j, c);
-                    load_eight<float, VEC>(sn + j, s);
+// Eight numbers as they come from memory.
+template <typename T>
+struct Eight {
+    uint32_t raw[2 * sizeof(T)] = {};
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* src) {
+        if constexpr (VEC) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float own = __fmul_rn(x[e], c[e]), cross = __fmul_rn(y[e], s[e]);
-                        x[e] = first ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
-                    }
-                } else if (p.neighbours) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (f + 2 * e >= p.rotary) break;
-                        const float a = x[2 * e], b = x[2 * e + 1], c = cs[(f >> 1) + e], s = sn[(f >> 1) + e];
-                        x[2 * e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-                        x[2 * e + 1] = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (f + e >= p.rotary) break;
-                        const bool first = f + e < half;
-                        const int j = first ? f + e : f + e - half;
-                        const float y = cb_to_float(src[first ? j + half : j]);
-                        const float own = __fmul_rn(x[e], cs[j]), cross = __fmul_rn(y, sn[j]);
-                        x[e] = first ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
-                    }
-                }
-            }
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(src)[i];
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+            for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(raw)[e] = src[e];
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = sizeof(T) == 4 ? __uint_as_float(raw[e % (2 * sizeof(T))])
+                                  : __uint_as_float(e & 1 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
+    }
+};
+
+// Nibbles of eight lanes' words, transposed: nibble n of lane l becomes nibble l of lane n (lanes in runs of eight).
+__device__ __forceinline__ uint32_t transposed(uint32_t m, int l) {
+    uint32_t other = __shfl_xor_sync(0xffffffffu, m, 4);
+    m = (l & 4) ? __byte_perm(other, m, 0x7632) : __byte_perm(m, other, 0x5410);
+    other = __shfl_xor_sync(0xffffffffu, m, 2);
+    m = (l & 2) ? __byte_perm(other, m, 0x7351) : __byte_perm(m, other, 0x6240);
+    other = __shfl_xor_sync(0xffffffffu, m, 1);
+    return (l & 1) ? ((other >> 4) & 0x0f0f0f0fu) | (m & 0xf0f0f0f0u) : (m & 0x0f0f0f0fu) | ((other << 4) & 0xf0f0f0f0u);
+}
+
+// The eights of a row, D/8 lanes: lane 8 w + l has the word of g = l, and of the transposed words the codes of the
+// features from f on.
+template <int D>
+__device__ __forceinline__ int eight_of(int within) {
+    const int l = within & 7;
+    return 64 * (within >> 3) + 8 * ((l & 1) | ((l & 2) << 1) | ((l & 4) >> 1));         // (0, 1, 4, 5, 2, 3, 6, 7)[l]
+}
+
+// VEC: rows are aligned to 16 bytes, and half of the rotated features is a multiple of eight.
+template <int D, int GROUP, typename T, bool VEC>
+__global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, int heads_each) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, W = D / 64, NG = D / GROUP, STEP = 8 * PER_WARP;
+    const int lane = threadIdx.x & 31, within = lane % LANES;
+    const int w = within >> 3, l = within & 7, f = eight_of<D>(within);
+    const int row = blockIdx.x, heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0);
+    const int end = min(heads, ((int)blockIdx.y + 1) * heads_each);
+    int head = blockIdx.y * heads_each + (threadIdx.x >> 5) * PER_WARP + lane / LANES;
+    if (lane >= LANES * PER_WARP) head = end;                 // (lanes that have no head go along: shuffles)
+    const T* row_src = reinterpret_cast<const T*>(p.qkv) + (size_t)row * p.qkv_stride;
+    const int half = p.rotary >> 1;
+    const bool first = f < half, halves = VEC && !p.neighbours && f < p.rotary;
+    const int other_f = first ? f + half : f - half;
+    Eight<T> next_x, next_y;                                   // the next head's numbers, and those they turn with
+    auto load = [&](int h) {
+        if (h >= end) return;
+        next_x.template load<VEC>(row_src + (size_t)h * D + f);
+        if (halves && h < p.n_heads + p.kv_heads) next_y.template load<VEC>(row_src + (size_t)h * D + other_f);
+    };
+    load(head);
+    const int request = p.row_request[row], pos = p.positions[row];
+    if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) return;
+    const float* cs = p.cos_t + (size_t)pos * half;
+    const float* sn = p.sin_t + (size_t)pos * half;
+    float c[8], s[8];
+    if (halves) {
+        load_eight<float, VEC>(cs + (first ? f : other_f), c);
+        load_eight<float, VEC>(sn + (first ? f : other_f), s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = first ? -s[e] : s[e];           // a cos - b sin is a cos + b (-sin) to the bit
+    }
+    const long long place = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+    // (as many turns for every lane of a warp)
+    for (int turn = blockIdx.y * heads_each + (threadIdx.x >> 5) * PER_WARP; turn < end; turn += STEP, head += STEP) {
+        const bool live = head < end;
+        float x[8];
+        next_x.get(x);
+        if (live && f < p.rotary && head < p.n_heads + p.kv_heads) {
+            if (halves) {
+                float y[8];
+                next_y.get(y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+            } else if (p.neighbours) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (f + 2 * e >= p.rotary) break;
+                    const float a = x[2 * e], b = x[2 * e + 1], co = cs[(f >> 1) + e], si = sn[(f >> 1) + e];
+                    x[2 * e] = __fsub_rn(__fmul_rn(a, co), __fmul_rn(b, si));
+                    x[2 * e + 1] = __fadd_rn(__fmul_rn(a, si), __fmul_rn(b, co));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (f + e >= p.rotary) break;
+                    const bool lower = f + e < half;
+                    const int j = lower ? f + e : f + e - half;
+                    const float v = cb_to_float(row_src[(size_t)head * D + (lower ? j + half : j)]);
+                    const float own = __fmul_rn(x[e], cs[j]), cross = __fmul_rn(v, sn[j]);
+                    x[e] = lower ? __fsub_rn(own, cross) : __fadd_rn(cross, own);
+                }
+            }
         }
         __syncwarp();                     // q may take its own place: every lane has read what it turns
+        load(head + STEP);
         if (live && head < p.n_heads)
             store_eight<T, VEC>(reinterpret_cast<T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * D + f, x);
-        if (!__any_sync(0xffffffffu, at >= 0)) continue;
+        if (turn + PER_WARP <= p.n_heads) continue;              // queries alone
         // groups of 32 are the lanes of equal l & 2, of 64 all eight, of 128 two eights
         float least = x[0], largest = x[0];
 #pragma unroll
@@ -204,22 +247,16 @@ __global__ void __launch_bounds__(256) append4_kernel(const AppendParams p) {
             least = least_of(least, __shfl_xor_sync(0xffffffffu, least, o));
             largest = largest_of(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         }
-        const Coding c = coding_of(least, largest);
-        uint32_t m = 0;                   // the lane's codes, feature g at nibble g
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m |= code_of(x[e], c) << (4 * e);
-        // transposed over eight lanes: nibble n of lane g is nibble g of lane n
-        uint32_t other = __shfl_xor_sync(0xffffffffu, m, 4);
-        m = (l & 4) ? __byte_perm(other, m, 0x7632) : __byte_perm(m, other, 0x5410);
-        other = __shfl_xor_sync(0xffffffffu, m, 2);
-        m = (l & 2) ? __byte_perm(other, m, 0x7351) : __byte_perm(m, other, 0x6240);
-        other = __shfl_xor_sync(0xffffffffu, m, 1);
-        m = (l & 1) ? ((other >> 4) & 0x0f0f0f0fu) | (m & 0xf0f0f0f0u) : (m & 0x0f0f0f0fu) | ((other << 4) & 0xf0f0f0f0u);
-        if (at >= 0) {
+        const Coding coding = coding_of(least, largest);
+        const uint32_t m = transposed(codes_of(x, coding), l);
+        if (live && head >= p.n_heads && place >= 0) {
+            const int side = head >= p.n_heads + p.kv_heads;
+            const long long at = place + (long long)(head - p.n_heads - side * p.kv_heads) * p.page_tokens
+                + (long long)side * p.n_pages * p.kv_heads * p.page_tokens;
             p.codes[at * (D / 8) + l * W + w] = m;
             // (the first lane of a group)
             const bool one = GROUP == 32 ? (l & ~2) == 0 : GROUP == 64 ? l == 0 : (within & 15) == 0;
-            if (one) p.scales[at * NG + f / GROUP] = c.pair;
+            if (one) p.scales[at * NG + f / GROUP] = coding.pair;
         }
     }
 }
@@ -228,9 +265,10 @@ template <int D>
 __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, int group) {
     cb_pdl_trigger();
     cb_pdl_wait();
-    constexpr int WORDS = D / 8, W = D / 64;                 // 16 threads a word, two words a warp
+    constexpr int WORDS = D / 8, W = D / 64;                 // 16 threads a word, neighbours take neighbouring words
+    __shared__ float ends[2][8][16][WORDS];
     __shared__ float largest[2 * D / 32];
-    __shared__ __align__(16) int8_t rounded[2][D];
+    __shared__ __align__(16) int8_t rounded[2 * D];
     const int row = blockIdx.x / p.kv_heads, kv = blockIdx.x - row * p.kv_heads;
     const int request = p.row_request[row], pos = p.positions[row];
     if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) return;
@@ -241,8 +279,8 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
     const int held = pos - index * p.page_tokens + 1;
     const long long page = (at - (held - 1)) / ((long long)p.kv_heads * p.page_tokens);
     at += (long long)kv * p.page_tokens - (held - 1);
-    const int tid = threadIdx.x, lane = tid & 31, word = tid >> 4, t = tid & 15;
-    const int g = word / W, w = word - g * W, f = 64 * w + g;         // features f + 8 k
+    const int tid = threadIdx.x, lane = tid & 31, word = tid % WORDS, t = tid / WORDS;
+    const int g = word / W, f = 64 * (word - g * W) + g;              // features f + 8 k
     const uint32_t* codes = p.codes + at * WORDS + word;
     const uint32_t* scales = p.scales + at * (D / group);
     const int g0 = f / group, g1 = (f + 32) / group;                  // k < 4, k >= 4
@@ -261,31 +299,31 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
             lo[k] = fminf(lo[k], v);
         }
     }
-    float most = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            hi[k] = fmaxf(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], o));
-            lo[k] = fminf(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], o));
-        }
-        if (!(lo[k] <= hi[k])) hi[k] = lo[k] = 0.f;          // (a feature of which no token's key is a number)
-        most = fmaxf(most, fmaxf(fabsf(hi[k]), fabsf(lo[k])));
+        ends[0][k][t][word] = hi[k];
+        ends[1][k][t][word] = lo[k];
     }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+    __syncthreads();
+    // a thread a feature's end: the first D threads the largest, the others the least
+    const int side = tid / D, mine = tid - side * D, my_word = mine % WORDS, my_k = mine / WORDS;
+    float end = ends[side][my_k][0][my_word];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+        const float v = ends[side][my_k][i][my_word];
+        end = side ? fminf(end, v) : fmaxf(end, v);
+    }
+    if (fabsf(end) == INFINITY) end = 0.f;                   // (a feature of which no token's key is a number)
+    float most = cb_warp_max(fabsf(end));
     if (lane == 0) largest[tid >> 5] = most;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2 * D / 32; ++i) most = fmaxf(most, largest[i]);
     const float scale = __fmul_rn(most, 1.0f / 127.0f);
     const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        // lane t of a word writes feature t & 7, its largest or least
-        if ((t & 7) == k)
-            rounded[t >> 3][f + 8 * k] =
-                (int8_t)(int)fminf(fmaxf(rintf(__fmul_rn(t < 8 ? hi[k] : lo[k], inverse)), -127.f), 127.f);
-    }
+    const int my_g = my_word / W;
+    rounded[side * D + 64 * (my_word - my_g * W) + my_g + 8 * my_k] =
+        (int8_t)(int)fminf(fmaxf(rintf(__fmul_rn(end, inverse)), -127.f), 127.f);
     __syncthreads();
     const long long to = page * p.kv_heads + kv;
     if (tid < 2 * D / 16)
@@ -293,16 +331,16 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
     if (tid == 0) p.bound_scales[to] = scale;
 }
 
-// Eight neighbouring features of a row.
+// Eight neighbouring features of the row `at` (there: it is one; every lane of the warp takes part).
 template <int D>
-__device__ __forceinline__ void eight_values(const uint32_t* codes, const uint32_t* scales, long long at, int group, int f,
-                                             float (&v)[8]) {
-    const uint32_t* words = codes + at * (D / 8) + (f >> 6);
-    const uint32_t pair = scales[at * (D / group) + f / group];
+__device__ __forceinline__ void eight_values(const uint32_t* codes, const uint32_t* scales, long long at, bool there, int group,
+                                             int within, float (&v)[8]) {
+    const int l = within & 7, f = eight_of<D>(within);
+    const uint32_t m = transposed(there ? codes[at * (D / 8) + l * (D / 64) + (within >> 3)] : 0u, l);
+    const uint32_t pair = there ? scales[at * (D / group) + f / group] : 0u;
     const float step = c4_step(pair), low = c4_low(pair);
-    const int shift = c4_shift((f >> 3) & 7);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) v[g] = fmaf((float)((words[g * (D / 64)] >> shift) & 15u), step, low);
+    for (int g = 0; g < 8; ++g) v[g] = fmaf((float)((m >> (4 * g)) & 15u), step, low);
 }
 
 template <int D, typename T>
@@ -310,13 +348,27 @@ __global__ void __launch_bounds__(256) values4_kernel(const uint32_t* codes, con
                                                       T* out) {
     cb_pdl_trigger();
     cb_pdl_wait();
-    const long long items = rows * (D / 8);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < items; i += (long long)gridDim.x * 256) {
-        const long long at = i / (D / 8);
-        const int f = (int)(i - at * (D / 8)) * 8;
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
+    const int lane = threadIdx.x & 31, within = lane % LANES;
+    for (long long row = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP; row < rows;
+         row += (long long)gridDim.x * 8 * PER_WARP) {
+        const long long at = row + lane / LANES;
+        const bool there = at < rows && lane < LANES * PER_WARP;
         float v[8];
-        eight_values<D>(codes, scales, at, group, f, v);
-        store_eight<T, true>(out + at * D + f, v);
+        eight_values<D>(codes, scales, at, there, group, within, v);
+        if (there) store_eight<T, true>(out + at * D + eight_of<D>(within), v);
+    }
+}
+
+__global__ void __launch_bounds__(256) bound_values4_kernel(const uint32_t* bounds, const float* scales, int words_each,
+                                                            long long words, float* out) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < words; i += (long long)gridDim.x * 256) {
+        const uint32_t w = bounds[i];
+        const float a = scales[i / words_each];
+        reinterpret_cast<float4*>(out)[i] = make_float4((float)(int8_t)w * a, (float)(int8_t)(w >> 8) * a,
+                                                        (float)(int8_t)(w >> 16) * a, (float)(int8_t)(w >> 24) * a);
     }
 }
 
@@ -369,34 +421,34 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     __syncthreads();
     constexpr float MOST = sizeof(T) == 2 ? 3.3895314e38f : 3.4028235e38f;
-    constexpr int ITEMS = 64 * (D / 8) / 256;
-    float v[ITEMS][8];
-    long long at[ITEMS];
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
+    const int lane = threadIdx.x & 31, within = lane % LANES, f = eight_of<D>(within);
+    const long long side_rows = (long long)p.n_pages * p.kv_heads * p.page_tokens;
+    float v[ROUNDS][8];
+    long long at[ROUNDS];
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-        const int i = threadIdx.x + 256 * j, t = i / (D / 8), f = (i - t * (D / 8)) * 8, pos = index * 64 + t;
+    for (int j = 0; j < ROUNDS; ++j) {
+        const int t = (j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES, pos = index * 64 + t;
         at[j] = -1;
-        if (some && pos < held && pos >= lo)
+        if (some && lane < LANES * PER_WARP && pos < held && pos >= lo) {
             at[j] = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+            if (at[j] >= 0) at[j] += (long long)blockIdx.y * p.page_tokens;
+        }
+        eight_values<D>(p.codes, p.scales, at[j] + side_rows, at[j] >= 0, p.group, within, v[j]);
+        if (!(v[j][0] == v[j][0])) {                        // (a group's numbers are all none or all some)
+            bad[t] = 1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-        if (at[j] >= 0) {
-            at[j] += (long long)blockIdx.y * p.page_tokens;
-            eight_values<D>(p.codes, p.scales, at[j] + (long long)p.n_pages * p.kv_heads * p.page_tokens, p.group, f, v[j]);
-            if (!(v[j][0] == v[j][0])) {                    // (a group's numbers are all none or all some)
-                bad[t] = 1;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-            }
+            for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-        const int i = threadIdx.x + 256 * j, t = i / (D / 8), f = (i - t * (D / 8)) * 8;
+    for (int j = 0; j < ROUNDS; ++j) {
+        const int t = (j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES;
         const long long to = (((long long)block * p.kv_heads + blockIdx.y) * 64 + t) * D + f;
-        float k[8] = {0.f};
-        if (at[j] >= 0) eight_values<D>(p.codes, p.scales, at[j], p.group, f, k);
+        float k[8];
+        eight_values<D>(p.codes, p.scales, at[j], at[j] >= 0, p.group, within, k);
+        if (lane >= LANES * PER_WARP) continue;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (bad[t]) k[e] = __int_as_float(0x7fffffff);
@@ -411,16 +463,17 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
 template <int D, int GROUP>
 int append_of(const AppendParams& p, int dtype, cudaStream_t stream) {
     const int size = dtype == CB_F32 ? 4 : 2;
-    const long long per_block = 8 * (32 / (D / 8));
-    const long long items = (long long)p.rows * (p.n_heads + (p.write ? 2 * p.kv_heads : 0));
-    const dim3 grid((unsigned)min((items + per_block - 1) / per_block, 148LL * 32));
+    // heads a block: all of a row's where there are rows for every SM, else as few turns of a block's warps as fill them
+    const int step = 8 * (32 / (D / 8)), heads = p.n_heads + (p.write ? 2 * p.kv_heads : 0), turns = (heads + step - 1) / step;
+    const int runs = max(1, min(turns, 148 * 4 / p.rows)), heads_each = (turns + runs - 1) / runs * step;
+    const dim3 grid((unsigned)p.rows, (unsigned)((heads + heads_each - 1) / heads_each));
     const bool vec = ((uintptr_t)p.qkv | (uintptr_t)p.q | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16 == 0
         && p.qkv_stride * size % 16 == 0 && p.q_stride * size % 16 == 0 && (p.rotary / 2) % 8 == 0;
     int rc;
     if (dtype == CB_F32) rc = cb_launch(vec ? append4_kernel<D, GROUP, float, true> : append4_kernel<D, GROUP, float, false>,
-                                        grid, dim3(256), 0, stream, p);
+                                        grid, dim3(256), 0, stream, p, heads_each);
     else rc = cb_launch(vec ? append4_kernel<D, GROUP, __nv_bfloat16, true> : append4_kernel<D, GROUP, __nv_bfloat16, false>,
-                        grid, dim3(256), 0, stream, p);
+                        grid, dim3(256), 0, stream, p, heads_each);
     if (rc == 0 && p.write && p.bounds != nullptr)
         rc = cb_launch(bounds4_kernel<D>, dim3((unsigned)p.rows * p.kv_heads), dim3(2 * D), 0, stream, p, GROUP);
     return rc;
@@ -462,7 +515,7 @@ CB_EXPORT int cb_values4(const void* codes, const void* scales, int group, long 
     const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
     const uint32_t* sc = reinterpret_cast<const uint32_t*>(scales);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)min((rows * (head_dim / 8) + 255) / 256, 148LL * 32));
+    const dim3 grid((unsigned)min((rows * (head_dim / 8) + 255) / 256, 148LL * 64));
 #define VALUES(D)                                                                                                        \
     if (head_dim == D) {                                                                                                 \
         if (dtype == CB_F32) cb_launch(values4_kernel<D, float>, grid, dim3(256), 0, s, c, sc, group, rows, (float*)out); \
@@ -472,6 +525,13 @@ CB_EXPORT int cb_values4(const void* codes, const void* scales, int group, long 
     VALUES(64) VALUES(128) VALUES(192) VALUES(256)
 #undef VALUES
     return CB_ERR_UNSUPPORTED;
+}
+
+CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int heads, int head_dim, float* out, void* stream) {
+    const long long words = (long long)heads * head_dim / 2;
+    cb_launch(bound_values4_kernel, dim3((unsigned)min((words + 255) / 256, 148LL * 32)), dim3(256), 0,
+              reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const uint32_t*>(bounds), scales, head_dim / 2, words, out);
+    return cb_last_error();
 }
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,

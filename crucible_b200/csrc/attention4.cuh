@@ -55,8 +55,8 @@ struct Attn4Params {
     const int* row_request;
     const int* positions;
     int rows;
-    int page_tiles;            // tiles of 16 keys a page (0: a tile may lie in two) ...
-    uint32_t page_tiles_inverse;      // ... and 2^32 over them, rounded up (0: one tile a page)
+    int page_eights;           // runs of eight keys a page (0: a run may lie in two) ...
+    uint32_t page_eights_inverse;     // ... and 2^32 over them, rounded up (0: one run a page)
     int window;                // 0: all earlier keys
     float scale_log2;
     int row_tiles;
@@ -85,7 +85,7 @@ __device__ __forceinline__ A4Unit a4_unit(const Attn4Params& p, int u) {
         v.request = p.row_request[x];
         v.first = p.positions[x];
         v.n_rows = (v.request >= 0 && v.request < p.requests && v.first >= 0) ? p.n_rep : 0;
-        v.tile_hi = p.pick_count * p.page_tiles;
+        v.tile_hi = p.pick_count * (p.page_eights >> 1);
         return v;
     }
     v.request = x;
@@ -96,13 +96,14 @@ __device__ __forceinline__ A4Unit a4_unit(const Attn4Params& p, int u) {
         if (p.window > 0) v.tile_lo = max(0, v.first + v.base / p.n_rep - p.window + 1) >> 4;
         v.tile_hi = ((v.first + (min(v.n_rows, v.base + ROWS) - 1) / p.n_rep) >> 4) + 1;
         // (what lies beyond the table is not there)
-        if (p.page_tiles > 0) v.tile_hi = (int)min((long long)v.tile_hi, (long long)p.table_stride * p.page_tiles);
+        v.tile_hi = (int)min((long long)v.tile_hi, ((long long)p.table_stride * p.page_tokens + 15) >> 4);
     }
     return v;
 }
 
 // Stream: the tiles of all units and kv heads in a row (unit 0 head 0, head 1, .., unit 1 ..), dealt out in equal shares.
-__device__ __forceinline__ long long a4_quota(long long tiles, int blocks) { return max(16LL, (tiles + blocks - 1) / blocks); }
+// (Counted in 32 bits; the caller has seen to it that they suffice.)
+__device__ __forceinline__ uint32_t a4_quota(uint32_t tiles, uint32_t blocks) { return max(8u, (tiles + blocks - 1) / blocks); }
 
 __device__ __forceinline__ uint32_t a4_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -237,61 +238,72 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
     constexpr float CODE = F32 ? 1.f : 16777216.f;      // 1 over the unit of the codes
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long scan[A4_WARPS], found[3];
+    __shared__ uint32_t scan[A4_WARPS], found[3];
     // (the warp's number by way of a shuffle: known to be the same in all lanes, what follows from it lives in uniform registers)
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, t = lane & 3;
 
     // ---- which rows, which keys ------------------------------------------------
     int index, kv;                      // the unit and its kv head
-    long long left = 0;                 // stream: tiles that the block has still to take
+    uint32_t left = 0;                  // stream: tiles that the block has still to take
     int skip = 0, slot = 0;             // ... tiles of the unit that another block takes, and which partial result comes next
     if (p.stream > 0) {
-        long long tiles = 0;
-        for (int u = threadIdx.x; u < p.units; u += A4_WARPS * 32) tiles += a4_unit<L::ROWS>(p, u).weight();
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-        if (lane == 0) scan[warp] = tiles;
-        __syncthreads();
-        tiles = 0;
-#pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) tiles += scan[w];
-        tiles *= p.kv_heads;
-        const long long quota = a4_quota(tiles, p.stream), begin = quota * blockIdx.x;
-        if (begin >= tiles) return;
-        left = min(quota, tiles - begin);
-        // the unit in which the share begins
-        long long before = 0;
+        // all units' tiles (a unit a thread, and the next 128 if there are more), and before each unit
+        uint32_t tiles = 0, mine = 0, upto = 0;
         for (int u0 = 0; u0 < p.units; u0 += A4_WARPS * 32) {
             const int u = u0 + threadIdx.x;
-            const long long mine = u < p.units ? (long long)a4_unit<L::ROWS>(p, u).weight() * p.kv_heads : 0;
-            long long upto = mine;
+            mine = u < p.units ? (uint32_t)a4_unit<L::ROWS>(p, u).weight() * p.kv_heads : 0u;
+            upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+                const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += v;
             }
-            __syncthreads();
             if (lane == 31) scan[warp] = upto;
             __syncthreads();
-            long long all = 0;
+            upto += tiles;
 #pragma unroll
             for (int w = 0; w < A4_WARPS; ++w) {
                 if (w < warp) upto += scan[w];
-                all += scan[w];
+                tiles += scan[w];
             }
-            upto += before;
+            __syncthreads();
+        }
+        const uint32_t quota = a4_quota(tiles, p.stream), begin = quota * blockIdx.x;
+        if (begin >= tiles) return;
+        left = min(quota, tiles - begin);
+        // the unit in which the share begins: among the last 128 looked at, or looked for again
+        uint32_t before = 0;
+        for (int u0 = 0; u0 < p.units; u0 += A4_WARPS * 32) {
+            const int u = u0 + threadIdx.x;
+            if (p.units > A4_WARPS * 32) {
+                mine = u < p.units ? (uint32_t)a4_unit<L::ROWS>(p, u).weight() * p.kv_heads : 0u;
+                upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                if (lane == 31) scan[warp] = upto;
+                __syncthreads();
+                upto += before;
+#pragma unroll
+                for (int w = 0; w < A4_WARPS; ++w) {
+                    if (w < warp) upto += scan[w];
+                    before += scan[w];
+                }
+            }
             if (begin < upto && begin >= upto - mine) {
+                const uint32_t at = begin - (upto - mine), one = mine / p.kv_heads;
                 found[0] = u;
-                found[1] = (begin - (upto - mine)) / (mine / p.kv_heads);
-                found[2] = (begin - (upto - mine)) % (mine / p.kv_heads);
+                found[1] = at / one;
+                found[2] = at - at / one * one;
             }
-            before += all;
+            __syncthreads();
             if (before > begin) break;
         }
-        __syncthreads();
-        index = (int)found[0];
-        kv = (int)found[1];
-        skip = (int)found[2];
+        index = found[0];
+        kv = found[1];
+        skip = found[2];
     } else {
         index = blockIdx.x / p.kv_heads;
         kv = blockIdx.x - index * p.kv_heads;
@@ -308,8 +320,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
     uint32_t place[D / 64];
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) place[j] = ring + a4_place<D>((lane + 32 * j) / (D / 32), (lane + 32 * j) % (D / 32));
-    const bool whole = p.page_tiles > 0;                 // a tile lies in one page
+    const bool whole = p.page_eights > 0, sixteens = whole && (p.page_eights & 1) == 0;     // eight, sixteen keys lie in one page
     const size_t side_rows = (size_t)p.n_pages * p.kv_heads * p.page_tokens;
+    const size_t side_bytes = side_rows * (D / 2);
     const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_tokens;
 
   for (;;) {
@@ -329,7 +342,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
     const int* picks = p.picks != nullptr ? p.picks + ((size_t)row0 * p.kv_heads + kv) * p.pick_count : nullptr;
     int tile_lo = unit.tile_lo, tile_hi = unit.tile_hi, taken = weight;
     if (p.stream > 0) {
-        taken = (int)min((long long)(weight - skip), left);
+        taken = min(weight - skip, (int)left);
         tile_lo += skip;
         tile_hi = min(tile_hi, tile_lo + taken);
     } else if (gridDim.z > 1) {
@@ -340,52 +353,55 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
 
     // ---- the warp's ring ----------------------------------------------------
     const size_t head_row = (size_t)kv * p.page_tokens;
-    const uint8_t* const code_src[2] = {p.codes + head_row * (D / 2) + lane * 16,
-                                        p.codes + (side_rows + head_row) * (D / 2) + lane * 16};
+    const uint8_t* const code_src = p.codes + head_row * (D / 2);
     // (scales: lanes of both sides side by side)
     const uint8_t* const scale_src = p.scales + (head_row + (lane >= 4 * NG ? side_rows : 0)) * (NG * 4) + (lane % (4 * NG)) * 16;
-    // The first key of tile i, and (whole) which page that is: -1 where there is none.
+    // The first of eight keys, run i of them, and (whole) its page; -1 where there is none.
     auto key_of = [&](int i, int& page) {
         page = whole ? -1 : 0;
-        if (i >= tile_hi) return -1;
-        if (!whole) return i * 16;
-        int index = p.page_tiles_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_tiles_inverse);
-        if (index * p.page_tiles > i) --index;           // (rounded up, the inverse is at most one too much)
-        const int slot = (i - index * p.page_tiles) * 16;
+        if (i >= 2 * tile_hi) return -1;
+        if (!whole) return i * 8;
+        int index = p.page_eights_inverse == 0 ? i : (int)__umulhi((uint32_t)i, p.page_eights_inverse);
+        if (index * p.page_eights > i) --index;          // (rounded up, the inverse is at most one too much)
+        const int slot = (i - index * p.page_eights) * 8;
         if (picks != nullptr) index = picks[index];
         if ((unsigned)index < (unsigned)p.table_stride) page = table[index];
         if ((unsigned)page >= (unsigned)p.n_pages) page = -1;
-        return page < 0 ? -1 : picks != nullptr ? index * p.page_tokens + slot : i * 16;
+        return page < 0 ? -1 : picks != nullptr ? index * p.page_tokens + slot : i * 8;
     };
     // The pairs of tiles to fetch, one after the other; 32 of them are looked up at a time, a lane each: the rows (for head 0)
-    // of both tiles, and whether some row of the block may not see some key of them.  A tile whose page is none is
-    // masked whole; what is fetched for it (the pool's first rows) is of no account, as is what lies behind a request's
-    // last token.
+    // of the four runs of eight keys, and whether some row of the block may not see some key of them.  A run whose
+    // page is none is masked whole; what is fetched for it (the pool's first rows) is of no account, as is what lies behind
+    // a request's last token.
     int ahead = tile_lo + 2 * warp, looked = 0;
-    uint32_t rows_of[2], edges_of;
+    uint32_t rows_of[4], edges_of;
     auto look = [&]() {
-        bool edge = false;
+        bool edge = !whole;
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            int page;
-            const int key = key_of(ahead + 2 * A4_WARPS * lane + u, page);
-            rows_of[u] = whole && key >= 0 ? (uint32_t)page * page_rows + (uint32_t)(key % p.page_tokens) : 0u;
-            edge = edge || !whole || key < 0 || key + 15 > min_pos || key <= lowest;
+            for (int u = 0; u < 4; ++u) {
+                rows_of[u] = 0;
+                if (sixteens && (u & 1)) continue;       // (its first half's next rows)
+                int page;
+                const int key = key_of(2 * (ahead + 2 * A4_WARPS * lane) + u, page);
+                if (key >= 0) rows_of[u] = (uint32_t)page * page_rows + (uint32_t)(key % p.page_tokens);
+                edge = edge || key < 0 || key + (sixteens ? 15 : 7) > min_pos || key <= lowest;
+            }
         }
         edges_of = __ballot_sync(0xffffffffu, edge);
     };
     uint32_t edges = 0;                    // of the pairs in flight, the next to be taken in the lowest bit
     auto fetch = [&](uint32_t stage) {     // `stage`: bytes from the ring's beginning
         if (ahead < tile_hi) {
-            if (whole) {
+            if (sixteens) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const uint32_t row = __shfl_sync(0xffffffffu, rows_of[u], looked);
+                    const uint32_t row = __shfl_sync(0xffffffffu, rows_of[2 * u], looked);
+                    const uint8_t* src = code_src + (size_t)row * (D / 2) + lane * 16;
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const uint8_t* src = code_src[s] + (size_t)row * (D / 2);
-#pragma unroll
-                        for (int j = 0; j < D / 64; ++j) a4_copy16(place[j] + stage + (u * L::TILE + s * L::SIDE), src + j * 512);
+                    for (int j = 0; j < D / 64; ++j) {
+                        a4_copy16(place[j] + stage + u * L::TILE, src + j * 512);
+                        a4_copy16(place[j] + stage + (u * L::TILE + L::SIDE), src + j * 512 + side_bytes);
                     }
                     if constexpr (8 * NG <= 32) {
                         if (lane < 8 * NG)
@@ -399,6 +415,28 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
                         }
                     }
                 }
+            } else if (whole) {
+#pragma unroll 1
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t lower = __shfl_sync(0xffffffffu, u ? rows_of[2] : rows_of[0], looked);
+                    const uint32_t upper = __shfl_sync(0xffffffffu, u ? rows_of[3] : rows_of[1], looked);
+                    const uint32_t to = stage + u * L::TILE;
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        const int c = lane + 32 * j, r = c / (D / 32);
+                        const uint32_t row = r < 8 ? lower + r : upper + (r - 8);
+                        const uint8_t* src = code_src + (size_t)row * (D / 2) + (c % (D / 32)) * 16;
+                        a4_copy16(place[j] + to, src);
+                        a4_copy16(place[j] + to + L::SIDE, src + side_bytes);
+                    }
+#pragma unroll
+                    for (int c = lane; c < 8 * NG; c += 32) {
+                        // 2 NG units of 16 bytes are eight rows' scales
+                        const int side = c / (4 * NG), at = c % (4 * NG);
+                        const size_t row = (at < 2 * NG ? lower : upper) + head_row + side * side_rows;
+                        a4_copy16(ring + to + 2 * L::SIDE + c * 16, p.scales + row * (NG * 4) + (at < 2 * NG ? at : at - 2 * NG) * 16);
+                    }
+                }
             } else {
                 const uint32_t to = ring + stage;
 #pragma unroll 1
@@ -410,7 +448,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
                     const uint8_t* src = p.codes + row * (D / 2) + u * 16;
                     const uint32_t dst = to + (r >> 4) * L::TILE + a4_place<D>(r & 15, u);
                     a4_copy16(dst, src);
-                    a4_copy16(dst + L::SIDE, src + side_rows * (D / 2));
+                    a4_copy16(dst + L::SIDE, src + side_bytes);
                 }
 #pragma unroll 1
                 for (int c = lane; c < 32 * NG; c += 32) {
@@ -529,8 +567,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
             for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
 
     // ---- over the keys -----------------------------------------------------------
-    // A pair of tiles.  EDGE: some row may not see some key of it (keys: the tiles' first, -1 for none).
-    auto pair = [&](auto edge, const uint8_t* at, int key_a, int key_b) {
+    // A pair of tiles.  EDGE: some row may not see some key of it (the four runs' first keys, -1 for none).
+    auto pair = [&](auto edge, const uint8_t* at, int key_a, int key_b, int key_c, int key_d) {
         constexpr bool EDGE = decltype(edge)::value;
         float s[2][NT][4];
         uint32_t vsc[2][2][NG];
@@ -608,7 +646,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const int key0 = u == 0 ? key_a : key_b, key = key0 + g + 8 * h;
+                            const int key0 = u == 0 ? (h == 0 ? key_a : key_b) : (h == 0 ? key_c : key_d), key = key0 + g;
                             bool out = key0 < 0 || key > pos[n][c] || (p.window > 0 && key <= pos[n][c] - p.window);
                             if (!whole && !out)
                                 out = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, key) < 0;
@@ -767,14 +805,15 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
     // registers about at every turn)
     for (int i = tile_lo + 2 * warp; i < tile_hi; i += 2 * A4_WARPS) {
         while (!(edges & 1)) {
-            pair(std::false_type{}, next(), 0, 0);
+            pair(std::false_type{}, next(), 0, 0, 0, 0);
             i += 2 * A4_WARPS;
             if (i >= tile_hi) break;
         }
         if (i >= tile_hi) break;
         int page;
-        const int key_a = key_of(i, page), key_b = key_of(i + 1, page);
-        pair(std::true_type{}, next(), key_a, key_b);
+        const int key_a = key_of(2 * i, page), key_b = key_of(2 * i + 1, page);
+        const int key_c = key_of(2 * i + 2, page), key_d = key_of(2 * i + 3, page);
+        pair(std::true_type{}, next(), key_a, key_b, key_c, key_d);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -905,14 +944,14 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
     constexpr int ROWS = 8 * NT, LANES = D / 4, SETS = 256 / LANES, ONE = ROWS * (D + 2);
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
     __shared__ float weights[256], part[8];
-    __shared__ long long counts[2][8];
+    __shared__ uint32_t counts[2][8];
     __shared__ float4 sums[SETS][LANES];
     cb_pdl_wait();
     const int r = blockIdx.y, index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads;
     const int tid = threadIdx.x, set = tid / LANES, lane = tid % LANES;
     const A4Unit unit = a4_unit<ROWS>(p, index);
     if (unit.base + r >= unit.n_rows) return;
-    long long tiles = 0, before = 0;
+    uint32_t tiles = 0, before = 0;
     for (int u = tid; u < p.units; u += 256) {
         const int w = a4_unit<ROWS>(p, u).weight();
         tiles += w;
@@ -934,9 +973,8 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
         tiles += counts[0][i];
         before += counts[1][i];
     }
-    const long long quota = a4_quota(tiles * p.kv_heads, p.stream);
-    const long long begin = before * p.kv_heads + (long long)kv * unit.weight();
-    const int from = (int)(begin / quota), n = (int)((begin + unit.weight() - 1) / quota) - from + 1;
+    const uint32_t quota = a4_quota(tiles * p.kv_heads, p.stream), begin = before * p.kv_heads + kv * unit.weight();
+    const int from = begin / quota, n = (int)((begin + unit.weight() - 1) / quota) - from + 1;
     if (n <= 1) return;                          // (its block has written the row)
     const bool second = begin != quota * from;
     auto result = [&](int z) { return p.partial + ((size_t)(from + z) * 2 + (z == 0 && second ? 1 : 0)) * ONE; };
@@ -1028,12 +1066,12 @@ int attention4_of(const Attn4Params& p, int dtype, int column_tiles, long long b
         const long long units = (long long)(picks != nullptr ? rows : requests) * row_tiles, blocks = units * kv_heads;  \
         if (blocks <= 0) return 0;                                                                                       \
         if (blocks >= (1LL << 31)) return CB_ERR_UNSUPPORTED;                                                            \
-        const int page_tiles = page_tokens % 16 ? 0 : page_tokens / 16;                                                  \
+        const int eights = page_tokens % 8 ? 0 : page_tokens / 8;                                                        \
         const Attn4Params p = {q, q_stride, out, out_stride, reinterpret_cast<const uint8_t*>(codes),                    \
                                reinterpret_cast<const uint8_t*>(scales), n_pages, page_tokens, kv_heads, n_rep,          \
                                row_start, first_pos, table, table_stride, requests, picks, pick_count, row_request,      \
-                               positions, rows, page_tiles,                                                              \
-                               page_tiles <= 1 ? 0u : (uint32_t)((1ull << 32) / page_tiles) + 1u, window,                \
+                               positions, rows, eights,                                                                  \
+                               eights <= 1 ? 0u : (uint32_t)((1ull << 32) / eights) + 1u, window,                        \
                                scale * A4_LOG2E, row_tiles, (int)units, stream_blocks, partial};                         \
         const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);                                                   \
         int rc = CB_ERR_UNSUPPORTED;                                                                                     \

@@ -21,6 +21,7 @@ page of the pool is not seen, a row of a request that is none is left as it is.
 """
 from __future__ import annotations
 
+from operator import add as _add
 from typing import Optional, Sequence
 
 import torch
@@ -35,6 +36,7 @@ for _dim in HEAD_DIMS:
     build.register_module(f"attention4_{_dim}", ["common.cuh", "cache4.cuh", "attention4.cuh"])
 
 GROUPS = (32, 64, 128)
+_HALF_DIMS = tuple(d // 2 for d in HEAD_DIMS)
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 _FLOATS = (_F32, _BF16)
 
@@ -51,8 +53,27 @@ class Pages4:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, bounds: Optional[torch.Tensor] = None,
                  bound_scales: Optional[torch.Tensor] = None):
+        # (one expression over what a pool usually is; only where it is not that are the tensors looked over one by one)
+        cs, ss, dev = codes.shape, scales.shape, codes.get_device()
+        if not (len(cs) == 5 and len(ss) == 6 and codes.dtype is torch.uint8 and scales.dtype is _BF16 and cs[0] == 2 == ss[5]
+                and cs[4] in _HALF_DIMS and ss[:4] == cs[:4] and min(cs) > 0 < ss[4] and (2 * cs[4]) % ss[4] == 0
+                and 2 * cs[4] // ss[4] in GROUPS and codes.is_contiguous() and scales.is_contiguous()
+                and not (codes.data_ptr() | scales.data_ptr()) & 15 and scales.get_device() == dev
+                and (bounds is None) is (bound_scales is None)
+                and (bounds is None or (
+                    bounds.dtype is torch.int8 and bounds.shape == (cs[1], cs[2], 2, 2 * cs[4]) and bounds.is_contiguous()
+                    and not bounds.data_ptr() & 15 and bound_scales.dtype is _F32 and bound_scales.shape == cs[1:3]
+                    and bound_scales.is_contiguous() and bounds.get_device() == dev == bound_scales.get_device()))):
+            self._refuse(codes, scales, bounds, bound_scales)
+        self.codes, self.scales, self.bounds, self.bound_scales = codes, scales, bounds, bound_scales
+        _, self.n_pages, self.kv_heads, self.page_tokens, half = cs
+        self.head_dim = 2 * half
+        self.group, self.device = 2 * half // ss[4], dev
+
+    @staticmethod
+    def _refuse(codes, scales, bounds, bound_scales):
         cs, ss = codes.shape, scales.shape
-        if len(cs) != 5 or cs[0] != 2 or codes.dtype != torch.uint8 or 2 * cs[4] not in HEAD_DIMS or not codes.is_contiguous():
+        if len(cs) != 5 or cs[0] != 2 or codes.dtype != torch.uint8 or cs[4] not in _HALF_DIMS or not codes.is_contiguous():
             raise KernelError("a pool's codes are contiguous uint8 [2, pages, kv heads, page tokens, dim / 2] with dim in "
                               f"{HEAD_DIMS}, got {codes.dtype} {list(cs)}")
         dim = 2 * cs[4]
@@ -66,16 +87,10 @@ class Pages4:
             raise KernelError("a pool's codes and scales begin on multiples of 16 bytes")
         if (bounds is None) != (bound_scales is None):
             raise KernelError("bounds come with their scales")
-        if bounds is not None and not (
-                bounds.dtype == torch.int8 and tuple(bounds.shape) == (cs[1], cs[2], 2, dim) and bounds.is_contiguous()
-                and bounds.data_ptr() % 16 == 0 and bound_scales.dtype == _F32
-                and tuple(bound_scales.shape) == (cs[1], cs[2]) and bound_scales.is_contiguous()):
-            raise KernelError(f"bounds are contiguous int8 [{cs[1]}, {cs[2]}, 2, {dim}] with float32 scales [{cs[1]}, {cs[2]}], "
-                              f"got {bounds.dtype} {list(bounds.shape)} and {bound_scales.dtype} {list(bound_scales.shape)}")
         _one_device(codes, scales, bounds, bound_scales)
-        self.codes, self.scales, self.bounds, self.bound_scales = codes, scales, bounds, bound_scales
-        self.n_pages, self.kv_heads, self.page_tokens, self.head_dim = cs[1], cs[2], cs[3], dim
-        self.group, self.device = dim // ss[4], codes.get_device()
+        raise KernelError(f"bounds are contiguous int8 [{cs[1]}, {cs[2]}, 2, {dim}] that begin on a multiple of 16 bytes, with "
+                          f"float32 scales [{cs[1]}, {cs[2]}], got {bounds.dtype} {list(bounds.shape)} and {bound_scales.dtype} "
+                          f"{list(bound_scales.shape)}")
 
     @classmethod
     def new(cls, n_pages: int, page_tokens: int, kv_heads: int, head_dim: int, group: int = 64, bounds: bool = False,
@@ -108,7 +123,12 @@ class Pages4:
         """What the bounds stand for: float32 [pages, kv heads, 2, dim]."""
         if self.bounds is None:
             raise KernelError("these pages keep no bounds")
-        return self.bounds.float() * self.bound_scales[..., None, None]
+        _need_cuda(self.bounds)
+        out = torch.empty(self.bounds.shape, dtype=_F32, device=self.bounds.device)
+        lib = build.load("append4")
+        _check(_at(self.device, lib.cb_bound_values4, self.bounds.data_ptr(), self.bound_scales.data_ptr(),
+                   self.n_pages * self.kv_heads, self.head_dim, out.data_ptr()), "bounds in 8 bits")
+        return out
 
 
 class Batch:
@@ -124,7 +144,7 @@ class Batch:
     numbers, the results follow the device's."""
 
     __slots__ = ("positions", "row_request", "row_start", "first_pos", "table", "new_tokens", "held_tokens", "requests",
-                 "most_new", "reach", "lead", "device", "checked")
+                 "most_new", "reach", "lead", "device")
 
     def __init__(self, positions, row_request, row_start, first_pos, table, new_tokens: Sequence[int],
                  held_tokens: Sequence[int], reach: Optional[int] = None):
@@ -132,28 +152,26 @@ class Batch:
         self.first_pos, self.table = first_pos, table
         self.new_tokens, self.held_tokens = new_tokens, held_tokens
         self.requests = requests = len(new_tokens)
-        dev = positions.get_device()
-        self.device = dev
-        ts, rows = table.shape, positions.shape
-        if not (requests > 0 and len(held_tokens) == requests and len(ts) == 2 and ts[0] == requests and ts[1] > 0
-                and len(rows) == 1 and row_request.shape == rows and row_start.shape == (requests + 1,)
-                and first_pos.shape == (requests,)
+        self.device = dev = positions.get_device()
+        if not (requests > 0 and len(held_tokens) == requests and table.dim() == 2 and len(table) == requests and table.size(1) > 0
+                and positions.dim() == 1 == row_request.dim() == row_start.dim() == first_pos.dim()
+                and len(row_request) == len(positions) and len(row_start) == requests + 1 and len(first_pos) == requests
                 and positions.dtype is _I32 and row_request.dtype is _I32 and row_start.dtype is _I32
                 and first_pos.dtype is _I32 and table.dtype is _I32
                 and positions.is_contiguous() and row_request.is_contiguous() and row_start.is_contiguous()
                 and first_pos.is_contiguous() and table.is_contiguous()
                 and dev == row_request.get_device() == row_start.get_device() == first_pos.get_device() == table.get_device()):
             self._refuse()
-        self.most_new = max(new_tokens)
-        if self.most_new < 1 or min(new_tokens) < 1 or min(held_tokens) < 0:
+        self.most_new = most = max(new_tokens)
+        if requests == 1 or most == min(new_tokens):
+            self.lead = requests if most == 1 else 0
+            longest = most + max(held_tokens)
+        else:
+            self.lead = next(i for i, n in enumerate(new_tokens) if n != 1)
+            longest = max(map(_add, new_tokens, held_tokens))
+        self.reach = longest if reach is None else reach
+        if min(new_tokens) < 1 or min(held_tokens) < 0:
             raise KernelError("a batch's requests bring at least one token each, and hold none or more")
-        self.reach = max(map(int.__add__, new_tokens, held_tokens)) if reach is None else reach
-        lead = 0
-        for n in new_tokens:
-            if n != 1:
-                break
-            lead += 1
-        self.lead = lead
 
     def _refuse(self):
         t = {"positions": self.positions, "row_request": self.row_request, "row_start": self.row_start,
@@ -176,19 +194,28 @@ class Batch:
         return batch
 
 
-def _rows_of(t: torch.Tensor, what: str, width: int, dtype=None) -> None:
-    if t.dim() != 2 or t.shape[1] != width or t.dtype not in _FLOATS or (dtype is not None and t.dtype != dtype):
+def _rows_ok(t: torch.Tensor, what: str, width: int, dtype, rows: int) -> None:
+    """`rows` rows at least, of `width` numbers side by side; of `dtype`, or (None) float32 or bfloat16."""
+    if not (t.dim() == 2 and t.size(1) == width and (t.dtype is dtype if dtype is not None else t.dtype in _FLOATS)
+            and t.stride(1) == 1 and (t.stride(0) >= width or t.size(0) == 1) and t.size(0) >= rows):
         names = "float32 or bfloat16" if dtype is None else str(dtype).replace("torch.", "")
-        raise KernelError(f"{what}: {names} rows [T, {width}] are taken, got {t.dtype} {list(t.shape)}")
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
-        raise KernelError(f"{what}: rows must be contiguous and not overlap")
+        if t.dim() != 2 or t.shape[1] != width or t.dtype not in _FLOATS or (dtype is not None and t.dtype != dtype):
+            raise KernelError(f"{what}: {names} rows [T, {width}] are taken, got {t.dtype} {list(t.shape)}")
+        if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+            raise KernelError(f"{what}: rows must be contiguous and not overlap")
+        raise KernelError(f"{what}: the batch has {rows} rows, the tensor {t.shape[0]}")
 
 
-def _step_checks(what: str, rows: int, batch: Batch, pages: Pages4, *tensors) -> None:
-    if rows < batch.positions.shape[0]:
-        raise KernelError(f"{what}: the batch has {batch.positions.shape[0]} rows, the tensors {rows}")
-    _need_cuda(*tensors, batch.positions, pages.codes)
-    _one_device(pages.codes, batch.positions, *tensors)
+def _same_device(what: str, batch: "Batch", pages: Pages4, *others) -> None:
+    dev = pages.device
+    if dev >= 0 and batch.device == dev:
+        for t in others:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            return
+    _need_cuda(pages.codes, batch.positions, *others)
+    raise KernelError(f"{what}: pages, batch and the other tensors lie on different devices")
 
 
 def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
@@ -203,8 +230,9 @@ def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional
     width = (n_heads + 2 * kv) * dim
     if n_heads < 1:
         raise KernelError("rope_append4: a positive number of query heads is needed")
-    _rows_of(qkv, "rope_append4 rows", width)
-    _rows_of(q, "rope_append4 queries", n_heads * dim, qkv.dtype)
+    rows = batch.positions.size(0)
+    _rows_ok(qkv, "rope_append4 rows", width, None, rows)
+    _rows_ok(q, "rope_append4 queries", n_heads * dim, qkv.dtype, rows)
     if (cos is None) != (sin is None):
         raise KernelError("rope_append4: cos and sin come together")
     rotary = 0
@@ -214,13 +242,13 @@ def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional
                 or not sin.is_contiguous() or rotary > dim):
             raise KernelError(f"rope_append4: the tables are contiguous float32 [positions, r / 2] with r at most {dim}, got "
                               f"{cos.dtype} {list(cos.shape)} and {sin.dtype} {list(sin.shape)}")
-    _step_checks("rope_append4", min(qkv.shape[0], q.shape[0]), batch, pages, qkv, q, cos, sin)
+    _same_device("rope_append4", batch, pages, qkv, q, cos, sin)
     lib = build.load("append4")
     code = _at(pages.device, lib.cb_append4, qkv.data_ptr(), _code(qkv.dtype), qkv.stride(0), q.data_ptr(), q.stride(0),
                cos.data_ptr() if rotary else 0, sin.data_ptr() if rotary else 0, rotary, cos.shape[0] if rotary else 0,
                1 if neighbours else 0, 1 if write else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
                batch.table.shape[1], batch.requests, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
-               pages.page_tokens, n_heads, kv, dim, pages.group, batch.positions.shape[0],
+               pages.page_tokens, n_heads, kv, dim, pages.group, rows,
                pages.bounds.data_ptr() if pages.bounds is not None else 0,
                pages.bound_scales.data_ptr() if pages.bounds is not None else 0)
     _check(code, "rope_append4")
@@ -234,17 +262,18 @@ def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, pick
     [rows, kv heads, count], or [n, ..] for the first n rows alone.  A query is rounded to 8 bits for it (largest magnitude
     127), as the bounds are."""
     dim, kv = pages.head_dim, pages.kv_heads
-    _rows_of(q, "pick_pages4 queries", n_heads * dim)
+    rows = batch.positions.size(0)
+    _rows_ok(q, "pick_pages4 queries", n_heads * dim, None, rows)
     if n_heads < 1 or n_heads % kv:
         raise KernelError(f"pick_pages4: {n_heads} query heads do not share {kv} kv heads evenly")
     if pages.bounds is None:
         raise KernelError("pick_pages4: these pages keep no bounds")
     _picks_ok("pick_pages4", picks, kv)
-    rows = min(picks.shape[0], batch.positions.shape[0])
+    rows = min(picks.shape[0], rows)
     if first < 0 or last < 1 or first + last > picks.shape[2]:
         raise KernelError(f"pick_pages4: of {picks.shape[2]} pages the first {first} and the last {last} cannot always be "
                           "among them (the row's own page has to be)")
-    _step_checks("pick_pages4", q.shape[0], batch, pages, q, picks)
+    _same_device("pick_pages4", batch, pages, q, picks)
     # scores are held for as many pages as the longest context may have
     most = min(batch.table.shape[1], -(-batch.reach // pages.page_tokens))
     lib = build.load("pick4")
@@ -281,15 +310,15 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     walked by itself, so that this is for a few rows a request; page sizes are multiples of 16, and there is no window.
     Picks of the first n rows alone are for the first n requests, which bring one row each; the others attend to all."""
     dim, kv = pages.head_dim, pages.kv_heads
-    _rows_of(q, "attention4 queries", n_heads * dim)
-    _rows_of(out, "attention4 output", n_heads * dim, q.dtype)
+    rows = batch.positions.size(0)
+    _rows_ok(q, "attention4 queries", n_heads * dim, None, rows)
+    _rows_ok(out, "attention4 output", n_heads * dim, q.dtype, rows)
     if n_heads < 1 or n_heads % kv:
         raise KernelError(f"attention4: {n_heads} query heads do not share {kv} kv heads evenly")
     if window is not None and window < 1:
         raise KernelError(f"attention4: a window is positive, got {window}")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention4: the scale is a positive number, got {scale}")
-    rows = batch.positions.shape[0]
     behind = 0
     if picks is not None:
         _picks_ok("attention4", picks, kv)
@@ -298,7 +327,7 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         behind = picks.shape[0]
         if behind < rows and behind > batch.lead:
             raise KernelError(f"attention4: picks of {behind} of {rows} rows, but only the first {batch.lead} requests bring one row")
-    _step_checks("attention4", min(q.shape[0], out.shape[0]), batch, pages, q, out, picks)
+    _same_device("attention4", batch, pages, q, out, picks)
     if picks is not None:
         _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
     if behind < rows:
@@ -321,16 +350,16 @@ def _shares(blocks: int, tiles: int, total: int, resident: int) -> tuple:
     """(blocks of a cluster, blocks of a stream or 0): how the keys are dealt, by the launch's row tiles of all kv heads
     (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
     hold."""
-    if blocks >= 4 * resident:
+    if blocks >= 4 * resident or total >= 1 << 30:
         return 1, 0
-    fit, most = resident // blocks, tiles // 16
+    fit, most = resident // blocks, tiles // 8
     want = max(1, min(fit, most))
     if want <= 8:
         shares = 1 << (want.bit_length() - 1)
         waves = -(-blocks * shares // resident)
         if most <= fit or total * shares * 4 >= tiles * waves * resident * 3:
             return shares, 0
-    return 1, max(1, min(resident, total // 16))
+    return 1, max(1, min(resident, total // 8))
 
 
 def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
@@ -344,10 +373,12 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
         tiles = picks.shape[2] * pages.page_tokens // 16
         total = tiles * blocks
     else:
-        most_rows, blocks = max(batch.new_tokens[first:last]), last - first
+        blocks = last - first
+        most_rows = batch.most_new if blocks == batch.requests else max(batch.new_tokens[first:last])
         reach = batch.reach if window is None else min(batch.reach, window + most_rows)
         tiles = -(-reach // 16) + (window is not None)
-        total = sum([min(h + n, reach) for h, n in zip(batch.held_tokens[first:last], batch.new_tokens[first:last])]) // 16 + blocks
+        total = (blocks * tiles if blocks == 1 or window is not None else
+                 (sum(batch.held_tokens[first:last]) + sum(batch.new_tokens[first:last])) // 16 + blocks)
     columns = 1 if f32 or most_rows * n_rep <= 8 else 2
     per = kv * -(-most_rows * n_rep // (8 * columns))
     blocks, total = blocks * per, total * per
