@@ -230,8 +230,8 @@ constexpr int A4_BLOCKS = D > 128 || NT > 1 ? 2 : NG * (F32 ? 2 : 1) <= 2 ? 4 : 
 
 template <int D, int NG, int NT, bool F32>
 __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) attention4_kernel(const Attn4Params p) {
-    cb_pdl_trigger();
     cb_pdl_wait();
+    cb_pdl_trigger();              // (after the wait: what puts a stream's results together reads the step's numbers before its own)
     constexpr int PARTS = F32 ? 2 : 1;
     using L = A4Layout<D, NG, NT, PARTS>;
     constexpr int GROUP = D / NG, W = D / 64, KS = D / 16, MT = D / 16;
@@ -246,7 +246,15 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
     int index, kv;                      // the unit and its kv head
     uint32_t left = 0;                  // stream: tiles that the block has still to take
     int skip = 0, slot = 0;             // ... tiles of the unit that another block takes, and which partial result comes next
-    if (p.stream > 0) {
+    if (p.stream > 0 && p.units == 1) {
+        const uint32_t one = a4_unit<L::ROWS>(p, 0).weight(), tiles = one * p.kv_heads;
+        const uint32_t quota = a4_quota(tiles, p.stream), begin = quota * blockIdx.x;
+        if (begin >= tiles) return;
+        left = min(quota, tiles - begin);
+        index = 0;
+        kv = begin / one;
+        skip = begin - kv * one;
+    } else if (p.stream > 0) {
         // all units' tiles (a unit a thread, and the next 128 if there are more), and before each unit
         uint32_t tiles = 0, mine = 0, upto = 0;
         for (int u0 = 0; u0 < p.units; u0 += A4_WARPS * 32) {
@@ -937,90 +945,83 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
 }
 
 // Stream: a row whose tile several blocks had a share of, a block a row, D / 4 threads a result side by side.  The first of
-// these blocks has it as its second result (unless its share begins there), the others as their first.
+// these blocks has it as its second result (unless its share begins there), the others as their first.  Who has what
+// is worked out while the main kernel still runs; then every thread fetches its share of the results with their
+// references at once and keeps a running reference of its own.
 template <int D, int NT, bool F32>
 __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params p) {
-    cb_pdl_trigger();
     constexpr int ROWS = 8 * NT, LANES = D / 4, SETS = 256 / LANES, ONE = ROWS * (D + 2);
     using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
-    __shared__ float weights[256], part[8];
     __shared__ uint32_t counts[2][8];
+    __shared__ float refs[SETS][2];
     __shared__ float4 sums[SETS][LANES];
-    cb_pdl_wait();
     const int r = blockIdx.y, index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads;
     const int tid = threadIdx.x, set = tid / LANES, lane = tid % LANES;
     const A4Unit unit = a4_unit<ROWS>(p, index);
     if (unit.base + r >= unit.n_rows) return;
-    uint32_t tiles = 0, before = 0;
-    for (int u = tid; u < p.units; u += 256) {
-        const int w = a4_unit<ROWS>(p, u).weight();
-        tiles += w;
-        if (u < index) before += w;
-    }
+    uint32_t tiles = unit.weight(), before = 0;
+    if (p.units > 1) {
+        tiles = 0;
+        for (int u = tid; u < p.units; u += 256) {
+            const int w = a4_unit<ROWS>(p, u).weight();
+            tiles += w;
+            if (u < index) before += w;
+        }
+        tiles = __reduce_add_sync(0xffffffffu, tiles);
+        before = __reduce_add_sync(0xffffffffu, before);
+        if ((tid & 31) == 0) {
+            counts[0][tid >> 5] = tiles;
+            counts[1][tid >> 5] = before;
+        }
+        __syncthreads();
+        tiles = before = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if ((tid & 31) == 0) {
-        counts[0][tid >> 5] = tiles;
-        counts[1][tid >> 5] = before;
-    }
-    __syncthreads();
-    tiles = before = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        tiles += counts[0][i];
-        before += counts[1][i];
+        for (int i = 0; i < 8; ++i) {
+            tiles += counts[0][i];
+            before += counts[1][i];
+        }
     }
     const uint32_t quota = a4_quota(tiles * p.kv_heads, p.stream), begin = before * p.kv_heads + kv * unit.weight();
     const int from = begin / quota, n = (int)((begin + unit.weight() - 1) / quota) - from + 1;
     if (n <= 1) return;                          // (its block has written the row)
     const bool second = begin != quota * from;
-    auto result = [&](int z) { return p.partial + ((size_t)(from + z) * 2 + (z == 0 && second ? 1 : 0)) * ONE; };
-    // their weights, and the sum
+    cb_pdl_wait();
+    cb_pdl_trigger();
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -3.4e38f, l = 0.f;
-    for (int z0 = 0; z0 < n; z0 += 256) {        // (as a rule once: few blocks share a row tile)
-        const int here = min(256, n - z0);
-        float ref = -3.4e38f;
-        if (tid < here) ref = result(z0 + tid)[2 * r];
-        float most = fmaxf(top, cb_warp_max(ref));
-        __syncthreads();
-        if ((tid & 31) == 0) part[tid >> 5] = most;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, part[i]);
-        const float w = tid < here ? a4_exp2(ref - most) : 0.f, corr = a4_exp2(top - most);
-        float mine = tid < here ? result(z0 + tid)[2 * r + 1] * w : 0.f;
-        mine = cb_warp_sum(mine);
-        weights[tid] = w;
-        __syncthreads();
-        if ((tid & 31) == 0) part[tid >> 5] = mine;
-        __syncthreads();
-        l *= corr;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) l += part[i];
-        v.x *= corr; v.y *= corr; v.z *= corr; v.w *= corr;
-        if (set < SETS) {
+    if (set < SETS) {
 #pragma unroll 4
-            for (int z = set; z < here; z += SETS) {
-                const float2* one = reinterpret_cast<const float2*>(result(z0 + z) + 2 * ROWS + r * D + lane * 4);
-                const float2 a = one[0], b = one[1];
-                v.x = fmaf(a.x, weights[z], v.x);
-                v.y = fmaf(a.y, weights[z], v.y);
-                v.z = fmaf(b.x, weights[z], v.z);
-                v.w = fmaf(b.y, weights[z], v.w);
-            }
+        for (int z = set; z < n; z += SETS) {
+            const float* one = p.partial + ((size_t)(from + z) * 2 + (z == 0 && second ? 1 : 0)) * ONE;
+            const float2 head = *reinterpret_cast<const float2*>(one + 2 * r);
+            const float2 a = *reinterpret_cast<const float2*>(one + 2 * ROWS + r * D + lane * 4);
+            const float2 b = *reinterpret_cast<const float2*>(one + 2 * ROWS + r * D + lane * 4 + 2);
+            const float most = fmaxf(top, head.x), was = a4_exp2(top - most), w = a4_exp2(head.x - most);
+            v.x = fmaf(a.x, w, v.x * was);
+            v.y = fmaf(a.y, w, v.y * was);
+            v.z = fmaf(b.x, w, v.z * was);
+            v.w = fmaf(b.y, w, v.w * was);
+            l = fmaf(head.y, w, l * was);
+            top = most;
         }
-        top = most;
+        sums[set][lane] = v;
+        if (lane == 0) {
+            refs[set][0] = top;
+            refs[set][1] = l;
+        }
     }
-    if (set < SETS) sums[set][lane] = v;
     __syncthreads();
     if (tid < D) {
-        float x = 0.f;
+        float x = 0.f, most = -3.4e38f;
+        l = 0.f;
 #pragma unroll
-        for (int i = 0; i < SETS; ++i) x += reinterpret_cast<const float*>(sums[i])[tid];
+        for (int i = 0; i < SETS; ++i) most = fmaxf(most, refs[i][0]);
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) {
+            const float w = a4_exp2(refs[i][0] - most);
+            x = fmaf(reinterpret_cast<const float*>(sums[i])[tid], w, x);
+            l = fmaf(refs[i][1], w, l);
+        }
         const int tok = (unit.base + r) / p.n_rep, head = kv * p.n_rep + (unit.base + r) - tok * p.n_rep;
         reinterpret_cast<T*>(p.out)[(size_t)(unit.row0 + tok) * p.out_stride + (size_t)head * D + tid] =
             cb_from_float<T>(l == 0.f ? 0.f : x / l);
