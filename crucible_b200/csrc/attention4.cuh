@@ -359,6 +359,22 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         tile_hi = min(tile_hi, tile_lo + share);
     }
 
+    // the queries' numbers, asked for before anything else of the unit's
+    constexpr int MINE = L::ROWS / A4_WARPS;             // rows a warp prepares
+    T query[MINE][D / 32];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int r = warp + j * A4_WARPS;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) query[j][i] = cb_from_float<T>(0.f);
+        if (r < live) {
+            const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
+            const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(row0 + tok) * p.q_stride + (size_t)head * D;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) query[j][i] = src[lane + 32 * i];
+        }
+    }
+
     // ---- the warp's ring ----------------------------------------------------
     const size_t head_row = (size_t)kv * p.page_tokens;
     const uint8_t* const code_src = p.codes + head_row * (D / 2);
@@ -489,18 +505,13 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         __half* qs = reinterpret_cast<__half*>(smem + L::AT_Q);
         float* sums = reinterpret_cast<float*>(smem + L::AT_SUMS);
         float* factor = reinterpret_cast<float*>(smem + L::AT_FACTOR);
-#pragma unroll 1
-        for (int r = warp; r < L::ROWS; r += A4_WARPS) {
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            const int r = warp + j * A4_WARPS;
             float v[D / 32];
             float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) v[i] = 0.f;
-            if (base + r < n_rows) {
-                const int tok = (base + r) / p.n_rep, head = kv * p.n_rep + (base + r) - tok * p.n_rep;
-                const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(row0 + tok) * p.q_stride + (size_t)head * D;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) v[i] = cb_to_float(src[lane + 32 * i]);
-            }
+            for (int i = 0; i < D / 32; ++i) v[i] = cb_to_float(query[j][i]);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) most = fmaxf(most, fabsf(v[i]));
             most = cb_warp_max(most);
@@ -1052,7 +1063,8 @@ template <int D, int NG>
 int attention4_of(const Attn4Params& p, int dtype, int column_tiles, long long blocks, int shares, cudaStream_t stream) {
     if (dtype == CB_F32) return attention4_launch<D, NG, 1, true>(p, blocks, shares, stream);
     if (column_tiles == 1) return attention4_launch<D, NG, 1, false>(p, blocks, shares, stream);
-    return attention4_launch<D, NG, 2, false>(p, blocks, shares, stream);
+    if constexpr (D <= 128) return attention4_launch<D, NG, 2, false>(p, blocks, shares, stream);
+    return CB_ERR_UNSUPPORTED;           // (wider heads have no registers for two column tiles)
 }
 
 }  // namespace

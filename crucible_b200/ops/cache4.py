@@ -346,20 +346,32 @@ def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
     return tensor_core.N_SMS * (2 if dim > 128 or columns > 1 else 4 if dim // group * (2 if f32 else 1) <= 2 else 3)
 
 
-def _shares(blocks: int, tiles: int, total: int, resident: int) -> tuple:
+def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 1.0) -> tuple:
     """(blocks of a cluster, blocks of a stream or 0): how the keys are dealt, by the launch's row tiles of all kv heads
     (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
-    hold."""
-    if blocks >= 4 * resident or total >= 1 << 30:
-        return 1, 0
-    fit, most = resident // blocks, tiles // 8
-    want = max(1, min(fit, most))
-    if want <= 8:
-        shares = 1 << (want.bit_length() - 1)
-        waves = -(-blocks * shares // resident)
-        if most <= fit or total * shares * 4 >= tiles * waves * resident * 3:
-            return shares, 0
-    return 1, max(1, min(resident, total // 8))
+    hold.  A model of what either takes, in us.  A block takes a round of eight tiles in 0.7 alone on its SM and in 0.53 times
+    the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end; a launch takes 2.  A stream
+    takes no longer than its work, but 12 besides, and 6 for every unit that its blocks begin.  Modelled and measured, us:
+    1 token of 32 heads of 128 on 8 behind 16,000 keys, clusters of 8 18 and 17, a stream 17 and 18; behind 131,071 97 and
+    105, 41 and 40; 32 behind 16,000, clusters of 2 122 and 120, of 4 115 and 107, a stream 108 and 110; 64 of
+    unlike lengths up to 8,191, clusters of 2 105 and 107, a stream 108 and 108."""
+    per_sm, work = resident / tensor_core.N_SMS, 0.53 * weight * total / (8 * tensor_core.N_SMS)
+    best = None
+    for shares in (1, 2, 4, 8):
+        rounds = -(-tiles // (8 * shares))
+        each = weight * max(0.7, 0.53 * min(blocks * shares / tensor_core.N_SMS, per_sm))
+        mean = total / (8 * shares * blocks)
+        waves = max(1.0, blocks * shares / resident)
+        us = 2.0 + waves * (5.0 + mean * each) + max(0.0, rounds - mean) * each + 0.1 * shares
+        if best is None or us < best[0]:
+            best = us, shares
+        if rounds == 1:
+            break
+    if total < 1 << 30 and blocks < 4 * resident:
+        stream = max(1, min(resident, total // 8))
+        if 12.0 + 6.0 * blocks / resident + max(work, weight * max(0.7, 0.53 * stream / tensor_core.N_SMS)) < 0.95 * best[0]:
+            return 1, stream
+    return best[1], 0
 
 
 def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
@@ -379,10 +391,11 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
         tiles = -(-reach // 16) + (window is not None)
         total = (blocks * tiles if blocks == 1 or window is not None else
                  (sum(batch.held_tokens[first:last]) + sum(batch.new_tokens[first:last])) // 16 + blocks)
-    columns = 1 if f32 or most_rows * n_rep <= 8 else 2
+    columns = 1 if f32 or most_rows * n_rep <= 8 or dim > 128 else 2
     per = kv * -(-most_rows * n_rep // (8 * columns))
     blocks, total = blocks * per, total * per
-    shares, stream = _shares(blocks, tiles, total, _resident(dim, pages.group, columns, f32))
+    shares, stream = _shares(blocks, tiles, total, _resident(dim, pages.group, columns, f32),
+                             (dim / 128) ** 0.4 * (2.0 if f32 else 1.8 if columns == 2 else 1.0))
     partial = torch.empty(stream * 16 * columns * (dim + 2), dtype=_F32, device=q.device) if stream else None
     lib = build.load(f"attention4_{dim}")
     code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),

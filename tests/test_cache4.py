@@ -167,8 +167,8 @@ def test_keys_are_dealt_to_as_many_blocks_as_there_is_room_for():
                 for total in (blocks * tiles, blocks + tiles):
                     shares, stream = cache4._shares(blocks, tiles, total, resident)
                     assert shares in (1, 2, 4, 8) and (shares == 1 or stream == 0)
-                    assert 0 <= stream <= resident and (stream or blocks >= 4 * resident or shares * blocks <= max(blocks, resident))
-                    assert shares == 1 or tiles >= 8 * shares
+                    assert 0 <= stream <= resident and (stream == 0 or (blocks < 4 * resident and total >= 8))
+                    assert shares == 1 or tiles > 4 * shares          # no block of a cluster without a round
 
 
 def test_pages_are_scored_by_no_more_blocks_than_a_cluster_has():
