@@ -122,6 +122,19 @@ __device__ __forceinline__ void store_eight(T* dst, const float (&v)[8]) {
     }
 }
 
+// A word's eight codes, the lowest bits' first.  (A code under the exponent of 2^23 is 2^23 + code; one that lies 4 e bits
+// higher, up to bit 19, is taken down by 16^-e: no shift, no conversion.)
+__device__ __forceinline__ void codes_as_floats(uint32_t m, float (&v)[8]) {
+    const uint32_t upper = m >> 20;
+    constexpr float DOWN[5] = {1.f, 0.0625f, 0.00390625f, 0.000244140625f, 0.0000152587890625f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int at = e < 5 ? e : e - 5;
+        const uint32_t bits = ((e < 5 ? m : upper) & (15u << (4 * at))) | 0x4b000000u;
+        v[e] = (__uint_as_float(bits) - 8388608.f) * DOWN[at];
+    }
+}
+
 // Eight numbers as they come from memory.
 template <typename T>
 struct Eight {
@@ -165,8 +178,8 @@ __device__ __forceinline__ int eight_of(int within) {
 // VEC: rows are aligned to 16 bytes, and half of the rotated features is a multiple of eight.
 template <int D, int GROUP, typename T, bool VEC>
 __global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, int heads_each) {
-    cb_pdl_trigger();
     cb_pdl_wait();
+    cb_pdl_trigger();              // (after the wait: the kernel of the bounds reads the step's numbers before its own)
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, W = D / 64, NG = D / GROUP, STEP = 8 * PER_WARP;
     const int lane = threadIdx.x & 31, within = lane % LANES;
     const int w = within >> 3, l = within & 7, f = eight_of<D>(within);
@@ -178,13 +191,14 @@ __global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, i
     const int half = p.rotary >> 1;
     const bool first = f < half, halves = VEC && !p.neighbours && f < p.rotary;
     const int other_f = first ? f + half : f - half;
-    Eight<T> next_x, next_y;                                   // the next head's numbers, and those they turn with
-    auto load = [&](int h) {
+    Eight<T> ahead_x[2], ahead_y[2];                           // the next two heads' numbers, and those they turn with
+    auto load = [&](int h, Eight<T>& x, Eight<T>& y) {
         if (h >= end) return;
-        next_x.template load<VEC>(row_src + (size_t)h * D + f);
-        if (halves && h < p.n_heads + p.kv_heads) next_y.template load<VEC>(row_src + (size_t)h * D + other_f);
+        x.template load<VEC>(row_src + (size_t)h * D + f);
+        if (halves && h < p.n_heads + p.kv_heads) y.template load<VEC>(row_src + (size_t)h * D + other_f);
     };
-    load(head);
+    load(head, ahead_x[0], ahead_y[0]);
+    load(head + STEP, ahead_x[1], ahead_y[1]);
     const int request = p.row_request[row], pos = p.positions[row];
     if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) return;
     const float* cs = p.cos_t + (size_t)pos * half;
@@ -197,8 +211,7 @@ __global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, i
         for (int e = 0; e < 8; ++e) s[e] = first ? -s[e] : s[e];           // a cos - b sin is a cos + b (-sin) to the bit
     }
     const long long place = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-    // (as many turns for every lane of a warp)
-    for (int turn = blockIdx.y * heads_each + (threadIdx.x >> 5) * PER_WARP; turn < end; turn += STEP, head += STEP) {
+    auto one = [&](int turn, Eight<T>& next_x, Eight<T>& next_y) {
         const bool live = head < end;
         float x[8];
         next_x.get(x);
@@ -229,10 +242,10 @@ __global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, i
             }
         }
         __syncwarp();                     // q may take its own place: every lane has read what it turns
-        load(head + STEP);
+        load(head + 2 * STEP, next_x, next_y);
         if (live && head < p.n_heads)
             store_eight<T, VEC>(reinterpret_cast<T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * D + f, x);
-        if (turn + PER_WARP <= p.n_heads) continue;              // queries alone
+        if (turn + PER_WARP <= p.n_heads) return;                // queries alone
         // groups of 32 are the lanes of equal l & 2, of 64 all eight, of 128 two eights
         float least = x[0], largest = x[0];
 #pragma unroll
@@ -255,27 +268,36 @@ __global__ void __launch_bounds__(256, 3) append4_kernel(const AppendParams p, i
                 + (long long)side * p.n_pages * p.kv_heads * p.page_tokens;
             p.codes[at * (D / 8) + l * W + w] = m;
             // (the first lane of a group)
-            const bool one = GROUP == 32 ? (l & ~2) == 0 : GROUP == 64 ? l == 0 : (within & 15) == 0;
-            if (one) p.scales[at * NG + f / GROUP] = coding.pair;
+            const bool leads = GROUP == 32 ? (l & ~2) == 0 : GROUP == 64 ? l == 0 : (within & 15) == 0;
+            if (leads) p.scales[at * NG + f / GROUP] = coding.pair;
         }
+    };
+    // (as many turns for every lane of a warp)
+    for (int turn = blockIdx.y * heads_each + (threadIdx.x >> 5) * PER_WARP; turn < end; turn += 2 * STEP) {
+        one(turn, ahead_x[0], ahead_y[0]);
+        head += STEP;
+        if (turn + STEP >= end) break;
+        one(turn + STEP, ahead_x[1], ahead_y[1]);
+        head += STEP;
     }
 }
 
 template <int D>
 __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, int group) {
-    cb_pdl_trigger();
-    cb_pdl_wait();
     constexpr int WORDS = D / 8, W = D / 64;                 // 16 threads a word, neighbours take neighbouring words
     __shared__ float ends[2][8][16][WORDS];
     __shared__ float largest[2 * D / 32];
     __shared__ __align__(16) int8_t rounded[2 * D];
     const int row = blockIdx.x / p.kv_heads, kv = blockIdx.x - row * p.kv_heads;
-    const int request = p.row_request[row], pos = p.positions[row];
-    if (request < 0 || request >= p.n_requests || pos < 0 || (p.rotary > 0 && pos >= p.n_positions)) return;
-    const int index = pos / p.page_tokens;
-    if (row + 1 < p.rows && p.row_request[row + 1] == request && p.positions[row + 1] / p.page_tokens == index) return;
-    long long at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-    if (at < 0) return;
+    const int request = p.row_request[row], pos = p.positions[row], index = pos / p.page_tokens;
+    long long at = -1;
+    if (request >= 0 && request < p.n_requests && pos >= 0 && !(p.rotary > 0 && pos >= p.n_positions)
+        && !(row + 1 < p.rows && p.row_request[row + 1] == request && p.positions[row + 1] / p.page_tokens == index))
+        at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+    if (at < 0) {
+        cb_pdl_wait();             // (every block waits: what is launched behind this kernel waits for it alone)
+        return;
+    }
     const int held = pos - index * p.page_tokens + 1;
     const long long page = (at - (held - 1)) / ((long long)p.kv_heads * p.page_tokens);
     at += (long long)kv * p.page_tokens - (held - 1);
@@ -287,14 +309,18 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
     float hi[8], lo[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) hi[k] = -INFINITY, lo[k] = INFINITY;
+    cb_pdl_wait();                 // (what is above is the step's numbers, which were there before the rows were written)
+    cb_pdl_trigger();
 #pragma unroll 4
     for (int i = t; i < held; i += 16) {
         const uint32_t c = codes[(size_t)i * WORDS];
         const uint32_t a = scales[(size_t)i * (D / group) + g0], b = scales[(size_t)i * (D / group) + g1];
+        float code[8];
+        codes_as_floats(c, code);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const uint32_t pair = k < 4 ? a : b;
-            const float v = fmaf((float)((c >> c4_shift(k)) & 15u), c4_step(pair), c4_low(pair));
+            const float v = fmaf(code[c4_shift(k) / 4], c4_step(pair), c4_low(pair));
             hi[k] = fmaxf(hi[k], v);
             lo[k] = fminf(lo[k], v);
         }
@@ -339,8 +365,9 @@ __device__ __forceinline__ void eight_values(const uint32_t* codes, const uint32
     const uint32_t m = transposed(there ? codes[at * (D / 8) + l * (D / 64) + (within >> 3)] : 0u, l);
     const uint32_t pair = there ? scales[at * (D / group) + f / group] : 0u;
     const float step = c4_step(pair), low = c4_low(pair);
+    codes_as_floats(m, v);
 #pragma unroll
-    for (int g = 0; g < 8; ++g) v[g] = fmaf((float)((m >> (4 * g)) & 15u), step, low);
+    for (int g = 0; g < 8; ++g) v[g] = fmaf(v[g], step, low);
 }
 
 template <int D, typename T>
@@ -350,13 +377,19 @@ __global__ void __launch_bounds__(256) values4_kernel(const uint32_t* codes, con
     cb_pdl_wait();
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
     const int lane = threadIdx.x & 31, within = lane % LANES;
-    for (long long row = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP; row < rows;
-         row += (long long)gridDim.x * 8 * PER_WARP) {
-        const long long at = row + lane / LANES;
-        const bool there = at < rows && lane < LANES * PER_WARP;
-        float v[8];
-        eight_values<D>(codes, scales, at, there, group, within, v);
-        if (there) store_eight<T, true>(out + at * D + eight_of<D>(within), v);
+    const long long stride = (long long)gridDim.x * 8 * PER_WARP;
+    for (long long row = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP; row < rows; row += 2 * stride) {
+        float v[2][8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const long long at = row + j * stride + lane / LANES;
+            eight_values<D>(codes, scales, at, at < rows && lane < LANES * PER_WARP, group, within, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const long long at = row + j * stride + lane / LANES;
+            if (at < rows && lane < LANES * PER_WARP) store_eight<T, true>(out + at * D + eight_of<D>(within), v[j]);
+        }
     }
 }
 
@@ -515,7 +548,7 @@ CB_EXPORT int cb_values4(const void* codes, const void* scales, int group, long 
     const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
     const uint32_t* sc = reinterpret_cast<const uint32_t*>(scales);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)min((rows * (head_dim / 8) + 255) / 256, 148LL * 64));
+    const dim3 grid((unsigned)min((rows * (head_dim / 8) + 511) / 512, 148LL * 64));
 #define VALUES(D)                                                                                                        \
     if (head_dim == D) {                                                                                                 \
         if (dtype == CB_F32) cb_launch(values4_kernel<D, float>, grid, dim3(256), 0, s, c, sc, group, rows, (float*)out); \

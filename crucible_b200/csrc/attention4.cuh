@@ -969,7 +969,11 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
     const int r = blockIdx.y, index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads;
     const int tid = threadIdx.x, set = tid / LANES, lane = tid % LANES;
     const A4Unit unit = a4_unit<ROWS>(p, index);
-    if (unit.base + r >= unit.n_rows) return;
+    // (every block waits, one that has nothing to do, too: what is launched behind this kernel waits for it alone)
+    if (unit.base + r >= unit.n_rows) {
+        cb_pdl_wait();
+        return;
+    }
     uint32_t tiles = unit.weight(), before = 0;
     if (p.units > 1) {
         tiles = 0;
@@ -994,10 +998,10 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
     }
     const uint32_t quota = a4_quota(tiles * p.kv_heads, p.stream), begin = before * p.kv_heads + kv * unit.weight();
     const int from = begin / quota, n = (int)((begin + unit.weight() - 1) / quota) - from + 1;
-    if (n <= 1) return;                          // (its block has written the row)
     const bool second = begin != quota * from;
     cb_pdl_wait();
     cb_pdl_trigger();
+    if (n <= 1) return;                          // (its block has written the row)
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -3.4e38f, l = 0.f;
     if (set < SETS) {

@@ -62,39 +62,17 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
     }
     // (another block's shared memory may be written once that block runs: arrived here, waited for below)
     if (gridDim.z > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    // the group's queries in 8 bits: a warp a head
-    for (int h = warp; h < p.n_rep; h += PICK_THREADS / 32) {
-        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)(kv * p.n_rep + h) * D;
-        float v[D / 32], most = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            v[i] = cb_to_float(src[lane + 32 * i]);
-            most = fmaxf(most, fabsf(v[i]));
-        }
-        const float scale = __fmul_rn(cb_warp_max(most), 1.0f / 127.0f);
-        const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
-        int8_t* up = reinterpret_cast<int8_t*>(q8 + (size_t)h * 2 * (D / 16));
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int c = (int)fminf(fmaxf(rintf(__fmul_rn(v[i], inverse)), -127.f), 127.f);
-            up[lane + 32 * i] = (int8_t)max(c, 0);
-            up[D + lane + 32 * i] = (int8_t)min(c, 0);
-        }
-        if (lane == 0) q_scale[h] = scale;
-    }
-    __syncthreads();
-    if (gridDim.z > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    // scores: four lanes a page
+    // pages are scored by four lanes each; the first are asked for before the queries are worked on
     const int* table = p.table + (size_t)request * p.table_stride;
     const int quarter = lane & 3;
     const int stride = gridDim.z * (PICK_THREADS / 4);
     uint32_t there = (uint32_t)__cvta_generic_to_shared(score);
     if (gridDim.z > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(there));
     constexpr int WIDE = 2;
-    for (int at = blockIdx.z * (PICK_THREADS / 4); at < pages; at += WIDE * stride) {       // (whole warps: shuffles)
-        int4 hi[WIDE][D / 64], lo[WIDE][D / 64];
-        float a[WIDE];
-        int page[WIDE];
+    int4 hi[WIDE][D / 64], lo[WIDE][D / 64];
+    float a[WIDE];
+    int page[WIDE];
+    auto load = [&](int at) {
 #pragma unroll
         for (int n = 0; n < WIDE; ++n) {
             const int index = at + n * stride + (tid >> 2);
@@ -117,6 +95,31 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
                 for (int j = 0; j < D / 64; ++j) hi[n][j] = lo[n][j] = make_int4(0, 0, 0, 0);
             }
         }
+    };
+    load(blockIdx.z * (PICK_THREADS / 4));
+    // the group's queries in 8 bits: a warp a head
+    for (int h = warp; h < p.n_rep; h += PICK_THREADS / 32) {
+        const T* src = reinterpret_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)(kv * p.n_rep + h) * D;
+        float v[D / 32], most = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            v[i] = cb_to_float(src[lane + 32 * i]);
+            most = fmaxf(most, fabsf(v[i]));
+        }
+        const float scale = __fmul_rn(cb_warp_max(most), 1.0f / 127.0f);
+        const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
+        int8_t* up = reinterpret_cast<int8_t*>(q8 + (size_t)h * 2 * (D / 16));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int c = (int)fminf(fmaxf(rintf(__fmul_rn(v[i], inverse)), -127.f), 127.f);
+            up[lane + 32 * i] = (int8_t)max(c, 0);
+            up[D + lane + 32 * i] = (int8_t)min(c, 0);
+        }
+        if (lane == 0) q_scale[h] = scale;
+    }
+    __syncthreads();
+    if (gridDim.z > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    for (int at = blockIdx.z * (PICK_THREADS / 4); at < pages; at += WIDE * stride) {       // (whole warps: shuffles)
         float best[WIDE];
 #pragma unroll
         for (int n = 0; n < WIDE; ++n) best[n] = -INFINITY;
@@ -151,6 +154,7 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
                 else score[index] = s;
             }
         }
+        if (at + WIDE * stride < pages) load(at + WIDE * stride);
     }
     if (gridDim.z > 1) {
         __syncthreads();
