@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
     const int request = p.row_request[row], pos = p.positions[row], index = pos / p.page_tokens;
     long long at = -1;
     if (request >= 0 && request < p.n_requests && pos >= 0 && !(p.rotary > 0 && pos >= p.n_positions)
-        && !(row + 1 < p.rows && p.row_request[row + 1] == request && p.positions[row + 1] / p.page_tokens == index))
+        && !(row + 1 < p.rows && p.row_request[row + 1] == request && p.positions[row + 1] / p.page_tokens == index
+             && !(p.rotary > 0 && p.positions[row + 1] >= p.n_positions)))           // (a row that is left out is nobody's last)
         at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
     if (at < 0) {
         cb_pdl_wait();             // (every block waits: what is launched behind this kernel waits for it alone)

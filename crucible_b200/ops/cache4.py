@@ -331,8 +331,8 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     if picks is not None:
         _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
     if behind < rows:
-        n_rep, lead = n_heads // kv, max(behind, batch.lead)
-        if lead < batch.requests and _laid_out(q, out, batch, n_rep, pages, window, lead):
+        lead = max(behind, batch.lead)
+        if lead < batch.requests and _laid_out(q, out, n_heads, batch, pages, window, lead):
             if behind < lead:
                 _walk(q, out, n_heads, scale, batch, pages, window, None, behind, lead)
             if _tiles(q, out, n_heads, scale, batch, pages, window, lead):
@@ -347,7 +347,7 @@ def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
 
 
 def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 1.0) -> tuple:
-    """(blocks of a cluster, blocks of a stream or 0): how the keys are dealt, by the launch's row tiles of all kv heads
+    """(blocks of a cluster, blocks of a stream or 0, us that it may take): how the keys are dealt, by the launch's row tiles of all kv heads
     (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
     hold.  A model of what either takes, in us.  A block takes a round of eight tiles in 0.7 alone on its SM and in 0.53 times
     the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end; a launch takes 2.  A stream
@@ -369,9 +369,29 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
             break
     if total < 1 << 30 and blocks < 4 * resident:
         stream = max(1, min(resident, total // 8))
-        if 12.0 + 6.0 * blocks / resident + max(work, weight * max(0.7, 0.53 * stream / tensor_core.N_SMS)) < 0.95 * best[0]:
-            return 1, stream
-    return best[1], 0
+        us = 12.0 + 6.0 * blocks / resident + max(work, weight * max(0.7, 0.53 * stream / tensor_core.N_SMS))
+        if us < 0.95 * best[0]:
+            return 1, stream, us
+    return best[1], 0, best[0]
+
+
+def _dealt(dim, kv, n_rep, group, f32, batch, window, first, last) -> tuple:
+    """How the requests first .. last - 1 go through the walking kernel: (column tiles a block, blocks of a cluster, blocks of a
+    stream, us that it may take)."""
+    blocks = last - first
+    most_rows = batch.most_new if blocks == batch.requests else max(batch.new_tokens[first:last])
+    reach = batch.reach if window is None else min(batch.reach, window + most_rows)
+    tiles = -(-reach // 16) + (window is not None)
+    total = (blocks * tiles if blocks == 1 or window is not None else
+             (sum(batch.held_tokens[first:last]) + sum(batch.new_tokens[first:last])) // 16 + blocks)
+    return _columns(dim, kv, n_rep, group, f32, most_rows, blocks, tiles, total)
+
+
+def _columns(dim, kv, n_rep, group, f32, most_rows, blocks, tiles, total) -> tuple:
+    columns = 1 if f32 or most_rows * n_rep <= 8 or dim > 128 else 2
+    per = kv * -(-most_rows * n_rep // (8 * columns))
+    return columns, *_shares(blocks * per, tiles, total * per, _resident(dim, group, columns, f32),
+                             (dim / 128) ** 0.6 * (2.0 if f32 else 1.3 if columns == 2 else 1.0))
 
 
 def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
@@ -383,19 +403,10 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     if picks is not None:
         most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
-        total = tiles * blocks
+        columns, shares, stream, _ = _columns(dim, kv, n_rep, pages.group, f32, 1, blocks, tiles, tiles * blocks)
     else:
-        blocks = last - first
-        most_rows = batch.most_new if blocks == batch.requests else max(batch.new_tokens[first:last])
-        reach = batch.reach if window is None else min(batch.reach, window + most_rows)
-        tiles = -(-reach // 16) + (window is not None)
-        total = (blocks * tiles if blocks == 1 or window is not None else
-                 (sum(batch.held_tokens[first:last]) + sum(batch.new_tokens[first:last])) // 16 + blocks)
-    columns = 1 if f32 or most_rows * n_rep <= 8 or dim > 128 else 2
-    per = kv * -(-most_rows * n_rep // (8 * columns))
-    blocks, total = blocks * per, total * per
-    shares, stream = _shares(blocks, tiles, total, _resident(dim, pages.group, columns, f32),
-                             (dim / 128) ** 0.4 * (2.0 if f32 else 1.8 if columns == 2 else 1.0))
+        most_rows = batch.most_new if last - first == batch.requests else max(batch.new_tokens[first:last])
+        columns, shares, stream, _ = _dealt(dim, kv, n_rep, pages.group, f32, batch, window, first, last)
     partial = torch.empty(stream * 16 * columns * (dim + 2), dtype=_F32, device=q.device) if stream else None
     lib = build.load(f"attention4_{dim}")
     code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),
@@ -408,16 +419,32 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
                rows if picks is None else min(rows, picks.shape[0]), most_rows, window or 0, scale, columns,
                shares, stream, partial.data_ptr() if partial is not None else 0)
     if code == build.UNSUPPORTED:
-        raise KernelError(f"attention4: {blocks} blocks of rows are more than a launch takes")
+        raise KernelError(f"attention4: {rows} rows of {n_heads} heads are more than a launch takes")
     _check(code, "attention4")
 
 
-LAID_OUT_ROWS = 64          # rows of a kv head from which a portion's keys are laid out anew
+LAID_OUT: Optional[bool] = None       # tests fix which way portions go
 
 
-def _laid_out(q, out, batch, n_rep, pages, window, first) -> bool:
-    return (q.dtype is _BF16 and max(batch.new_tokens[first:]) * n_rep >= LAID_OUT_ROWS
-            and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16))
+def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
+    """Whether the portions of the requests from `first` on go by `_tiles`: bfloat16 rows of heads of 64 and 128, 64 of a kv head
+    and more (others have no kernel there that is quicker).  us, by what was measured: 6 and 1.7 a million features laid out, then a
+    tile of 128 rows walks its keys alone, 7.2 a thousand, or all of them at 0.75 PFLOP/s."""
+    dim, kv = pages.head_dim, pages.kv_heads
+    new, held = batch.new_tokens[first:], batch.held_tokens[first:]
+    n_rep = n_heads // kv
+    if (q.dtype is not _BF16 or dim > 128 or q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16
+            or max(new) * n_rep < 64):
+        return False
+    if LAID_OUT is not None:
+        return LAID_OUT
+    walk = _dealt(dim, kv, n_rep, pages.group, False, batch, window, first, batch.requests)[3]
+    reach = max(map(_add, new, held))
+    seen = reach if window is None else min(reach, window + 128)
+    pairs = sum([n * min(h + n / 2, seen) for n, h in zip(new, held)])
+    tiles = (6.0 + 1.7e-6 * (sum(new) + sum(held)) * kv * dim
+             + max(0.0072 * min(seen, reach), 4e-6 * dim * n_heads * pairs / 750.0))
+    return tiles < walk
 
 
 class _Step:

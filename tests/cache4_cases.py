@@ -133,12 +133,14 @@ class Case:
         """float64 [2, pages, kv heads, page tokens, D]."""
         return values(self.pages.codes, self.pages.scales)
 
-    def attention(self, q, scale, window=None, picks=None):
-        """(results, the largest magnitude of a value that a row sees [rows, heads, 1]) in float64."""
+    def attention(self, q, scale, window=None, picks=None, spread=None):
+        """(results, the largest magnitude of a value that a row sees) in float64, each [rows, heads * dim].  `spread`, a list:
+        also gets scale * max_j sum_f |q_f| |k_jf| of every row and head."""
         everything = self.contents()
         rep = self.heads // self.kv_heads
         out = torch.zeros(self.rows, self.heads, self.dim, dtype=torch.float64, device=self.device)
         most = torch.zeros(self.rows, self.heads, 1, dtype=torch.float64, device=self.device)
+        terms = torch.zeros(self.rows, self.heads, 1, dtype=torch.float64, device=self.device)
         row = 0
         table, positions = self.table.tolist(), self.positions.tolist()
         for r, (_, new) in enumerate(self.requests):
@@ -160,7 +162,10 @@ class Case:
                     weights = torch.softmax(heads @ k.t() * scale, dim=-1)
                     out[i, h * rep:(h + 1) * rep] = weights @ v
                     most[i, h * rep:(h + 1) * rep] = v.abs().amax()
+                    terms[i, h * rep:(h + 1) * rep] = (heads.abs() @ k.abs().t()).amax(dim=1, keepdim=True) * scale
             row += new
+        if spread is not None:
+            spread.append(terms.expand(-1, -1, self.dim).flatten(1))
         return out.flatten(1), most.expand(-1, -1, self.dim).flatten(1)
 
 
@@ -173,3 +178,12 @@ def assert_attention(got, want, most, dtype):
     assert torch.isfinite(got.float()).all()
     worst = ((got.double() - want).abs() - (off * want.abs() + more * most)).max()
     assert float(worst) <= 0.0, f"over by {float(worst)}"
+
+
+def assert_attention_laid_out(got, want, most, terms):
+    """bfloat16 portions whose keys and values are laid out in bfloat16: values are off by 2^-9 of themselves, p by 2^-9 in the
+    numerator and in the sum, keys by 2^-9, so that a score is off by d = 2^-9 scale sum |q| |k| at most and a weight by
+    a factor of e^(2 d); on top the result's rounding, and 2^-9 for the tensor cores' and the sum's float32."""
+    moved = torch.expm1(2 * 2.0 ** -9 * terms)
+    worst = ((got.double() - want).abs() - (2.0 ** -8 * want.abs() + (4 * 2.0 ** -9 + moved) * most)).max()
+    assert torch.isfinite(got.float()).all() and float(worst) <= 0.0, f"over by {float(worst)}"

@@ -165,7 +165,8 @@ def test_keys_are_dealt_to_as_many_blocks_as_there_is_room_for():
         for blocks in (1, 2, 8, 37, 148, 512, 700, 100000):
             for tiles in (1, 7, 8, 60, 500, 8192, 1 << 20):
                 for total in (blocks * tiles, blocks + tiles):
-                    shares, stream = cache4._shares(blocks, tiles, total, resident)
+                    shares, stream, us = cache4._shares(blocks, tiles, total, resident)
+                    assert us > 2
                     assert shares in (1, 2, 4, 8) and (shares == 1 or stream == 0)
                     assert 0 <= stream <= resident and (stream == 0 or (blocks < 4 * resident and total >= 8))
                     assert shares == 1 or tiles > 4 * shares          # no block of a cluster without a round

@@ -164,6 +164,16 @@ def test_bounds_follow_what_is_written(dim, page, dtype):
         assert torch.equal(case.pages.bounds[i].double(), want) and torch.equal(case.pages.bound_scales[i].double(), scale)
 
 
+def test_bounds_where_the_angles_end():
+    """Rows beyond the tables of angles are left out: the page's bounds are those of the rows before them."""
+    case = cc.Case([(0, 16)], dim=64, page=16, seed=31, bounds=True)
+    qkv = case.normal(16, (case.heads + 2 * case.kv_heads) * 64).to(BF16)
+    _append(case, qkv, torch.empty(16, case.heads * 64, dtype=BF16, device=DEV), 64, tables=cc.tables(11, 32, DEV))
+    place = int(case.table[0, 0])
+    want, scale = _bounds_by_definition(case, place, 11)
+    assert torch.equal(case.pages.bounds[place].double(), want) and torch.equal(case.pages.bound_scales[place].double(), scale)
+
+
 def _attend(case, q, scale, **more):
     from crucible_b200.ops import cache4
     out = torch.full((q.shape[0], case.heads * case.dim), 7.0, dtype=q.dtype, device=q.device)
@@ -184,11 +194,74 @@ def _attend(case, q, scale, **more):
     (256, 128, 16, 1, 5, [(61, 1), (3, 3)]),
     (256, 64, 33, 1, 16, [(90, 1)]),
 ])
-def test_attention_of_few_rows(dim, group, n_rep, kv_heads, page, requests, dtype):
+def test_attention_of_few_rows(dim, group, n_rep, kv_heads, page, requests, dtype, monkeypatch):
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", False)               # (the kernel that walks the pages as they lie)
     case = cc.Case(requests, dim=dim, group=group, n_rep=n_rep, kv_heads=kv_heads, page=page, dtype=dtype, seed=dim + n_rep)
     q = case.queries(1.5)
     want, most = case.attention(q, dim ** -0.5)
     cc.assert_attention(_attend(case, q, dim ** -0.5), want, most, dtype)
+
+
+@pytest.mark.parametrize("dim,group,n_rep,kv_heads,page,requests,window", [
+    (64, 64, 3, 2, 16, [(0, 70)], None), (64, 32, 1, 3, 16, [(5, 100), (0, 33)], None), (128, 64, 4, 1, 16, [(200, 40)], None),
+    (128, 128, 2, 2, 24, [(30, 65), (129, 64), (0, 130)], None), (128, 32, 7, 1, 7, [(90, 31)], None),
+    (64, 64, 4, 2, 64, [(40, 1), (17, 1), (0, 200), (300, 20)], None), (128, 64, 4, 1, 16, [(200, 1), (250, 90), (0, 64)], 100),
+    (64, 64, 2, 2, 16, [(500, 40)], 17)])
+def test_attention_of_portions_that_are_laid_out(dim, group, n_rep, kv_heads, page, requests, window, monkeypatch):
+    """Long portions, decoded tokens at the step's head walked beside them; what the window has passed is not read."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    tiled, tiles = [], cache4._tiles
+    monkeypatch.setattr(cache4, "_tiles", lambda *a: tiled.append(tiles(*a)) or tiled[-1])
+    case = cc.Case(requests, dim=dim, group=group, n_rep=n_rep, kv_heads=kv_heads, page=page, seed=dim + n_rep)
+    if window is not None:
+        for r, (held, new) in enumerate(requests):
+            case.table[r, :max(0, held - window + 1) // page] = [-1, case.free][r % 2]
+        case.pages.scales[:, case.free] = float("nan")
+    scale = dim ** -0.5
+    q, spread = case.queries(1.5), []
+    want, most = case.attention(q, scale, window=window, spread=spread)
+    got = _attend(case, q, scale, window=window)
+    assert tiled == [True]
+    cc.assert_attention_laid_out(got, want, most, spread[0])
+    single = sum(1 for _, n in requests if n == 1)
+    cc.assert_attention(got[:single], want[:single], most[:single], BF16) if single else None
+
+
+def test_numbers_that_are_none_in_portions_that_are_laid_out(monkeypatch):
+    """A value or key that is no number reaches the rows that see it, whole, and no others; nor does what nobody wrote."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    case = cc.Case([(20, 60), (0, 90)], dim=64, group=32, n_rep=4, kv_heads=2, seed=21)
+    q, spread = case.queries(), []
+    want, most = case.attention(q, 0.125, spread=spread)
+    scales = case.pages.scales
+    scales[:, case.free] = float("nan")
+    for r, last in ((0, 80), (1, 90)):
+        for j in range(last, case.stride * 16):
+            place = int(case.table[r, j // 16])
+            if place != case.free:
+                scales[:, place, :, j % 16] = float("nan")
+    scales[1, int(case.table[0, 50 // 16]), 1, 50 % 16, 1] = float("nan")       # a value of kv head 1 at position 50: row 30
+    scales[0, int(case.table[1, 70 // 16]), 0, 70 % 16, 0] = float("nan")       # a key of kv head 0 at position 70: row 60 + 70
+    got = _attend(case, q, 0.125)
+    bad = torch.zeros(150, 8, dtype=torch.bool, device=DEV)
+    bad[30:60, 4:] = True
+    bad[130:, :4] = True
+    bad = bad.repeat_interleave(64, dim=1)
+    assert got[bad].isnan().all()
+    fine = torch.where(bad, want, got.double())
+    cc.assert_attention_laid_out(fine, want, most, spread[0])
+
+
+def test_rows_at_odd_addresses_go_by_the_walking_kernel():
+    case = cc.Case([(300, 200)], dim=64, group=64, n_rep=4, kv_heads=1, seed=22)
+    wide = torch.zeros(200, 4 * 64 + 3, dtype=BF16, device=DEV)
+    q = wide[:, 3:]
+    q.copy_(case.queries())
+    want, most = case.attention(q, 0.125)
+    cc.assert_attention(_attend(case, q, 0.125), want, most, BF16)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
