@@ -10,8 +10,8 @@
 //             the page now holds, in 8 bits with one scale.  A block a (row, kv head), a thread a word of codes and
 //             every 16th token; only the last row of each page's run does anything.
 //   values4   the whole pool as float32 or bfloat16 rows.
-//   expand4   the pages of some requests as rows of float32 or bfloat16 in pages of 64 tokens, for attention
-//             over many rows.
+//   expand4   the pages of some requests as rows in pages of 64 tokens, for attention over many rows, and the requests'
+//             queries, all in float16.
 //
 // All are bound by memory in large calls and by their launch in small ones.
 #define CB_PDL_BIT 6      // with the other quantised operators
@@ -415,22 +415,102 @@ struct ExpandParams {
     const int* table;
     int table_stride, n_requests;
     int window;
-    void* keys;              // [blocks of 64 tokens][kv heads][64][D]
-    void* values;
+    __half* keys;            // [blocks of 64 tokens][kv heads][64][D]
+    __half* values;
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
+    const __nv_bfloat16* q;
+    long long q_stride;
+    const int* row_request;
+    int first_request;       // the requests' numbers in row_request begin with it
+    int rows, n_rep;
+    float scale_log2;
+    __half* q_half;          // [rows][heads][D]
+    float2* row_scale;       // [rows][heads]: of the scores, of the results
 };
 
+// Keys (side 0) and values go into float16 times 2^-e, e the exponent of the largest number that the request's first visible
+// key or value can hold in any group: float16's eleven bits then reach from 2^15 above that to 2^-14 below (what is
+// larger stays at 65,504).
+template <int D>
+__device__ __forceinline__ int exponent_of(const ExpandParams& p, int request, int kv, int lo, int side) {
+    const long long at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, lo);
+    if (at < 0) return 0;
+    const long long row = at + ((long long)side * p.n_pages * p.kv_heads + kv) * p.page_tokens;
+    float most = 0.f;
+    for (int g = 0; g < D / p.group; ++g) {
+        const uint32_t pair = p.scales[row * (D / p.group) + g];
+        most = fmaxf(most, fmaxf(fabsf(c4_low(pair)), fabsf(fmaf(15.f, c4_step(pair), c4_low(pair)))));
+    }
+    return most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100) : 0;
+}
+
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+}
+
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
-// last token.  Which request a block is of follows from how many blocks the requests before it have; tokens that no row of
-// the step sees are left out, as zeros.  A value that is no number becomes its key's: attention by tiles multiplies the
-// values of masked keys by zero, but does not take their scores.
-template <int D, typename T>
+// last token; the blocks behind it take 16 rows' queries each.  Which request a block is of follows from how many blocks the
+// requests before it have; tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
+// its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.  Queries are
+// scaled by a power of two so that a row's largest lies in [2^13, 2^14).
+template <int D>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     cb_pdl_trigger();
     cb_pdl_wait();
     __shared__ uint32_t bad[64];
-    const int block = blockIdx.x;
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
+    const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
+    if (block > p.n_blocks) {
+        __shared__ int exponents[16][2], request_of[16];
+        const int from = p.row_start[0] + (block - p.n_blocks - 1) * 16, to = min(min(p.row_start[p.n_requests], p.rows), from + 16);
+        const int heads = p.kv_heads * p.n_rep;
+        if (threadIdx.x < 32) {
+            const int row = from + (threadIdx.x >> 1), side = threadIdx.x & 1;
+            int request = row >= 0 && row < to ? p.row_request[row] - p.first_request : -1;
+            if (request >= p.n_requests) request = -1;
+            exponents[threadIdx.x >> 1][side] = request < 0 ? 0
+                : exponent_of<D>(p, request, blockIdx.y, p.window > 0 ? max(0, p.first_pos[request] - p.window + 1) : 0, side);
+            request_of[threadIdx.x >> 1] = request;
+        }
+        __syncthreads();
+        constexpr int WIDE = 4;
+        for (int i0 = (threadIdx.x >> 5) * PER_WARP; i0 < 16 * p.n_rep; i0 += WIDE * 8 * PER_WARP) {        // (whole warps: shuffles)
+            float v[WIDE][8];
+#pragma unroll
+            for (int u = 0; u < WIDE; ++u) {
+                const int j = i0 + u * 8 * PER_WARP + lane / LANES;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+                if (j < 16 * p.n_rep && lane < LANES * PER_WARP && request_of[j / p.n_rep] >= 0)
+                    load_eight<__nv_bfloat16, true>(p.q + (size_t)(from + j / p.n_rep) * p.q_stride
+                                                    + (size_t)(blockIdx.y * p.n_rep + j % p.n_rep) * D + within * 8, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < WIDE; ++u) {
+                const int j = i0 + u * 8 * PER_WARP + lane / LANES, r = j / p.n_rep;
+                float most = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[u][e]));
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int up = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+                if (j >= 16 * p.n_rep || lane >= LANES * PER_WARP || request_of[r] < 0) continue;
+                const size_t at = (size_t)(from + r) * heads + blockIdx.y * p.n_rep + j % p.n_rep;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[u][e] *= two_to(up);
+                store_halves(p.q_half + at * D + within * 8, v[u]);
+                if (within == 0)
+                    p.row_scale[at] = make_float2(p.scale_log2 * two_to(-up) * two_to(exponents[r][0]), two_to(exponents[r][1]));
+            }
+        }
+        return;
+    }
     if (block == 0 && blockIdx.y == 0) {
         int before = 0;
         for (int r = 0; r < p.n_requests; ++r) {
@@ -452,11 +532,11 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     const bool some = block < p.n_blocks && request < p.n_requests;
     const int lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
+    const float down_k = some ? two_to(-exponent_of<D>(p, request, blockIdx.y, lo, 0)) : 1.f;
+    const float down_v = some ? two_to(-exponent_of<D>(p, request, blockIdx.y, lo, 1)) : 1.f;
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     __syncthreads();
-    constexpr float MOST = sizeof(T) == 2 ? 3.3895314e38f : 3.4028235e38f;
-    constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
-    const int lane = threadIdx.x & 31, within = lane % LANES, f = eight_of<D>(within);
+    const int f = eight_of<D>(within);
     const long long side_rows = (long long)p.n_pages * p.kv_heads * p.page_tokens;
     float v[ROUNDS][8];
     long long at[ROUNDS];
@@ -486,11 +566,11 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (bad[t]) k[e] = __int_as_float(0x7fffffff);
-            else if (k[e] == k[e]) k[e] = fminf(fmaxf(k[e], -MOST), MOST);
-            v[j][e] = fminf(fmaxf(v[j][e], -MOST), MOST);
+            else if (k[e] == k[e]) k[e] = fminf(fmaxf(k[e] * down_k, -65504.f), 65504.f);
+            v[j][e] = fminf(fmaxf(v[j][e] * down_v, -65504.f), 65504.f);
         }
-        store_eight<T, true>(reinterpret_cast<T*>(p.keys) + to, k);
-        store_eight<T, true>(reinterpret_cast<T*>(p.values) + to, v[j]);
+        store_halves(p.keys + to, k);
+        store_halves(p.values + to, v[j]);
     }
 }
 
@@ -570,21 +650,19 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
-                         int n_requests, int window, void* keys, void* values, int dtype, int* blocks, int block_stride,
-                         int n_blocks, void* stream) {
-    if (n_blocks <= 0) return 0;
+                         int n_requests, int window, void* keys, void* values, int* blocks, int block_stride, int n_blocks,
+                         const void* q, long long q_stride, const int* row_request, int first_request, int rows, int most_rows,
+                         int n_rep, float scale, void* q_half, float* row_scale, void* stream) {
+    if (n_blocks <= 0 || most_rows <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
-                            keys, values, blocks, block_stride, n_blocks};
+                            reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), blocks, block_stride,
+                            n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, row_request, first_request, rows,
+                            n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), reinterpret_cast<float2*>(row_scale)};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)n_blocks + 1, (unsigned)kv_heads);
-#define EXPAND(D)                                                                              \
-    if (head_dim == D) {                                                                       \
-        if (dtype == CB_F32) cb_launch(expand4_kernel<D, float>, grid, dim3(256), 0, s, p);    \
-        else cb_launch(expand4_kernel<D, __nv_bfloat16>, grid, dim3(256), 0, s, p);            \
-        return cb_last_error();                                                                \
-    }
-    EXPAND(64) EXPAND(128) EXPAND(192) EXPAND(256)
-#undef EXPAND
-    return CB_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + 15) / 16), (unsigned)kv_heads);
+    if (head_dim == 64) cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);
+    else if (head_dim == 128) cb_launch(expand4_kernel<128>, grid, dim3(256), 0, s, p);
+    else return CB_ERR_UNSUPPORTED;
+    return cb_last_error();
 }

@@ -52,6 +52,7 @@
 // (engine/kernels/kernels.cu:2257-2275).
 #define CB_PDL_BIT 1      // this file's bit in CRUCIBLE_PDL
 #include <type_traits>
+#include <cuda_fp16.h>
 #include "common.cuh"
 #include "tc_common.cuh"
 
@@ -87,12 +88,14 @@ struct TcAttnParams {
     int n_pages;             // of the pool
     int runs;                // 1: the 4-D maps may be used for tiles whose pages are consecutive
     int* status;
+    const float2* row_scale; // GATE_SCALED: [rows][n_heads], of the scores (log2(e) among it) and of the results
 };
 
 // GATE: the results' gate, fixed when it is compiled: the epilogue runs once per block and its instructions
 // come from memory (12 heads of 64 without a gate, a 2,048-token prompt: 32 us; with the code of the gate of a
 // logit a result beside it 0.3 us more, of both gates 1.4).
-enum Gate { GATE_NONE = 0, GATE_RESULT = 1, GATE_HEAD = 2 };
+// GATE_SCALED: no gate, queries, keys, values and P in float16, factors of its own for a row's scores and results.
+enum Gate { GATE_NONE = 0, GATE_RESULT = 1, GATE_HEAD = 2, GATE_SCALED = 3 };
 
 // HD: the head size, 64, 128 or (keys and values at once) 256.  A tile's operand of 64 features a row
 // is one swizzle atom wide: [rows][128 bytes].
@@ -137,6 +140,10 @@ struct Storage {
     int abort_flag;
 };
 
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -436,8 +443,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         // product, which the tensor pipe works off in order; the softmax of the tiles between runs beside both.
         if (n_tiles > 0) {
             const bool sender = tc::elect_one();
-            constexpr uint32_t idesc_qk = tc::instr_desc_bf16(ROWS, KEYS);
-            constexpr uint32_t idesc_pv = tc::instr_desc_bf16_b_mn(ROWS, NARROW ? 192 : Store::PART);
+            constexpr uint32_t idesc_qk = GATE == GATE_SCALED ? tc::instr_desc_f16(ROWS, KEYS) : tc::instr_desc_bf16(ROWS, KEYS);
+            constexpr uint32_t idesc_pv = GATE == GATE_SCALED ? tc::instr_desc_f16_b_mn(ROWS, NARROW ? 192 : Store::PART)
+                                                              : tc::instr_desc_bf16_b_mn(ROWS, NARROW ? 192 : Store::PART);
             // Operand descriptors by addition: the low word carries the address in 16-byte
             // units, the high word is the same for every tile.
             const uint64_t q_desc0 = tc::smem_desc_sw128(tc::smem_u32(s.q[0]));
@@ -546,6 +554,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const __nv_bfloat16* gate = nullptr;
         float gate_f = 1.f;
         float sink = -INFINITY;                       // in the base-2 exponent
+        float scale_log2 = p.scale_log2, out_scale = p.out_scale;
         if (real) {
             const int tok = row_base + row / n_rep, head = kv_head * n_rep + row % n_rep;
             if (p.sinks != nullptr) sink = p.sinks[head] * LOG2E;
@@ -553,6 +562,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (GATE == GATE_RESULT) gate = p.gate + (size_t)tok * p.gate_stride + (size_t)head * HD;
             if (GATE == GATE_HEAD)
                 gate_f = sigmoid(__bfloat162float(p.gate[(size_t)tok * p.gate_stride + head]));
+            if (GATE == GATE_SCALED) {
+                const float2 both = p.row_scale[(size_t)tok * p.n_heads + head];
+                scale_log2 = both.x;
+                out_scale = both.y;
+            }
         }
         if (!p.q_boxes && n_tiles > 0) {
             // group sizes whose tiles would leave much of the 128 rows empty: the rows by hand,
@@ -578,7 +592,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (!got && !*abort_flag) tc::give_up(abort_flag, p.status, tc::ST_EPILOGUE_TIMEOUT);
             return __all_sync(0xffffffffu, got);
         };
-        const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2);
+        const uint64_t scale2 = pair_of(scale_log2, scale_log2);
         for (int j = group; j < n_tiles; j += GROUPS) {
             const int key0 = tile_key0(j);
             const int b = j % S_BUFS;
@@ -623,7 +637,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                     }
             }
             float mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
-            mx *= p.scale_log2;
+            mx *= scale_log2;
             // raise the reference maximum only when it is exceeded by far; the accumulator
             // in tensor memory is rescaled then, by the whole warp at once, after the second product
             // that was the last to add to it.  A shared accumulator's reference is the one of the tile before.
@@ -685,7 +699,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                         e1 = ex2_fast(e1);
                         uint64_t& into = sum[(i >> 1) & 3];
                         into = add2(into, pair_of(e0, e1));
-                        pk[16 * c + (i >> 1)] = pack_bf16(e0, e1);
+                        pk[16 * c + (i >> 1)] = GATE == GATE_SCALED ? pack_f16(e0, e1) : pack_bf16(e0, e1);
                     }
                 tc::tmem_st_32x32(at + 32 * h, pk);
                 tc::tmem_st_wait();
@@ -770,7 +784,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             const float f_other = other.x == -INFINITY ? 0.f : exp2f(other.x - m_all);
             float l_all = (my_tiles > 0 ? l : 0.f) * f_mine + other.y * f_other;
             if (sink != -INFINITY) l_all += exp2f(sink - m_all);
-            const float inv = l_all > 0.f ? p.out_scale / l_all : 0.f;
+            const float inv = l_all > 0.f ? out_scale / l_all : 0.f;
             // (a shared accumulator stands against the last tile's reference, the higher one)
             const float w_mine = SHARED ? fmaxf(f_mine, f_other) * inv : f_mine * inv, w_other = f_other * inv;
             // An accumulator that no MMA has written holds whatever was there and is not
@@ -825,6 +839,9 @@ int launch_as(int gate, dim3 grid, cudaStream_t st, const CUtensorMap (&maps)[6]
     switch (gate) {
         case GATE_NONE: return launch_gate<HD, GATE_NONE>(grid, st, maps, p);
         case GATE_RESULT: return launch_gate<HD, GATE_RESULT>(grid, st, maps, p);
+        case GATE_SCALED:
+            if constexpr (HD <= 128) return launch_gate<HD, GATE_SCALED>(grid, st, maps, p);
+            return CB_ERR_UNSUPPORTED;
     }
     return launch_gate<HD, GATE_HEAD>(grid, st, maps, p);
 }
@@ -840,14 +857,13 @@ int launch_as(int gate, dim3 grid, cudaStream_t st, const CUtensorMap (&maps)[6]
 // be left as they are.  lead: how many requests at the head bring a single token (as max_new_tokens is the others').
 // gate: null, or logits: results times their sigmoids; laid out like `out`, rows of 16-byte pieces, or with
 // gate_per_head [rows][n_heads].
-CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_rows, void* out, int out_stride,
-                                        const void* k_cache, const void* v_cache, int n_pages,
-                                        const int* req_row_start, const int* req_first_pos,
-                                        const int* block_table, int table_stride, int n_requests,
-                                        int max_new_tokens, int n_heads, int n_kv_heads, int head_dim,
-                                        int page_tokens, float scale, int window, int chunked, int keep_first,
-                                        float out_scale, const float* sinks, const void* gate, int gate_stride,
-                                        int gate_per_head, int lead, int value_cols, int* status, void* stream) {
+static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* out, int out_stride,
+                             const void* k_cache, const void* v_cache, int n_pages, const int* req_row_start,
+                             const int* req_first_pos, const int* block_table, int table_stride, int n_requests,
+                             int max_new_tokens, int n_heads, int n_kv_heads, int head_dim, int page_tokens, float scale,
+                             int window, int chunked, int keep_first, float out_scale, const float* sinks, const void* gate,
+                             int gate_stride, int gate_per_head, const float* row_scale, int lead, int value_cols, int* status,
+                             void* stream) {
     if (n_requests <= 0 || max_new_tokens <= 0) return 0;
     if (keep_first < 0 || !(scale > 0.f)) return CB_ERR_UNSUPPORTED;
     if ((head_dim != 64 && head_dim != 128 && !(head_dim == 256 && k_cache == v_cache)) || n_heads % n_kv_heads != 0 || page_tokens < 8 || page_tokens > KEYS ||
@@ -908,6 +924,7 @@ CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_r
     p.gate_stride = gate_stride;
     p.out_scale = out_scale;
     p.status = status;
+    p.row_scale = reinterpret_cast<const float2*>(row_scale);
     const int q_tiles = (max_new_tokens * n_rep + p.tile_rows - 1) / p.tile_rows;
     if (n_requests > 65535 || q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     // (single tokens of more than a tile of query heads keep ranks like a portion's)
@@ -916,10 +933,37 @@ CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_r
     p.lead_ranks = (p.lead + portions - 1) / portions;
     if (p.lead_ranks + q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     const dim3 grid(n_kv_heads, portions, p.lead_ranks + q_tiles);
-    const int form = gate == nullptr ? GATE_NONE : gate_per_head ? GATE_HEAD : GATE_RESULT;
+    const int form = row_scale != nullptr ? GATE_SCALED : gate == nullptr ? GATE_NONE : gate_per_head ? GATE_HEAD : GATE_RESULT;
     if (head_dim == 64) return launch_as<64>(form, grid, (cudaStream_t)stream, maps, p);
     if (head_dim == 256 && value_cols > 0 && value_cols <= 192 && form == GATE_NONE)
         return launch_gate<256, GATE_NONE, true>(grid, (cudaStream_t)stream, maps, p);
     if (head_dim == 256) return launch_as<256>(form, grid, (cudaStream_t)stream, maps, p);
     return launch_as<128>(form, grid, (cudaStream_t)stream, maps, p);
+}
+
+CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_rows, void* out, int out_stride,
+                                        const void* k_cache, const void* v_cache, int n_pages,
+                                        const int* req_row_start, const int* req_first_pos,
+                                        const int* block_table, int table_stride, int n_requests,
+                                        int max_new_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                        int page_tokens, float scale, int window, int chunked, int keep_first,
+                                        float out_scale, const float* sinks, const void* gate, int gate_stride,
+                                        int gate_per_head, int lead, int value_cols, int* status, void* stream) {
+    return attention_tcgen05(qkv, qkv_stride, n_rows, out, out_stride, k_cache, v_cache, n_pages, req_row_start, req_first_pos,
+                             block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
+                             scale, window, chunked, keep_first, out_scale, sinks, gate, gate_stride, gate_per_head, nullptr,
+                             lead, value_cols, status, stream);
+}
+
+// The same over queries, keys and values in float16 (heads of 64 and 128): row_scale [n_rows][n_heads][2], factors for the scores
+// (log2(e) among it) and for the results of each row and head.
+CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, int n_rows, void* out,
+                                        int out_stride, const void* keys, const void* values, int n_pages,
+                                        const int* req_row_start, const int* req_first_pos, const int* block_table,
+                                        int table_stride, int n_requests, int max_new_tokens, int n_heads, int n_kv_heads,
+                                        int head_dim, int page_tokens, int window, int* status, void* stream) {
+    if (head_dim > 128) return CB_ERR_UNSUPPORTED;
+    return attention_tcgen05(q, q_stride, n_rows, out, out_stride, keys, values, n_pages, req_row_start, req_first_pos,
+                             block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
+                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, 0, 0, status, stream);
 }

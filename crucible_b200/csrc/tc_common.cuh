@@ -197,10 +197,19 @@ __host__ __device__ constexpr uint32_t instr_desc_bf16(int m, int n) {
            ((uint32_t)(m >> 4) << 24);
 }
 
+// The same with float16 A and B (format 0).
+__host__ __device__ constexpr uint32_t instr_desc_f16(int m, int n) {
+    return instr_desc_bf16(m, n) & ~((1u << 7) | (1u << 10));
+}
+
 // The same with B stored MN-major (its N index contiguous in shared memory, as a
 // [keys, head_dim] tile of values is for P . V): bit 16 set.
 __host__ __device__ constexpr uint32_t instr_desc_bf16_b_mn(int m, int n) {
     return instr_desc_bf16(m, n) | (1u << 16);
+}
+
+__host__ __device__ constexpr uint32_t instr_desc_f16_b_mn(int m, int n) {
+    return instr_desc_f16(m, n) | (1u << 16);
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T; issued by one thread.

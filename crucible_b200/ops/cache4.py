@@ -447,31 +447,30 @@ def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
     return tiles < walk
 
 
-class _Step:
-    """What the attention kernels over 16-bit pages read of a step: its requests from some on, in blocks of 64 tokens."""
-
-    page_tokens = 64
-    __slots__ = ("positions", "req_row_start", "req_first_pos")
-
-    def __init__(self, batch, first):
-        self.positions = batch.positions
-        self.req_row_start, self.req_first_pos = batch.row_start[first:], batch.first_pos[first:]
-
-
 def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
-    """bfloat16 portions of many rows: the keys and values of the requests from `first` on are laid out in bfloat16 once
-    (not again for every tile of rows), and attention runs over these by the kernels of the 16-bit cache."""
+    """bfloat16 portions of many rows: the keys and values of the requests from `first` on are laid out once, in blocks of 64
+    tokens (not taken apart again for every tile of rows), and attention runs over these on tcgen05.  Queries, keys, values
+    and p are float16 there, with a power of two for each row, key head and value head: eleven bits of them (in bfloat16 the
+    results were off by 0.0033 of themselves, half of it the roundings inside, in float16 by 0.0017, which is their own)."""
     dim, kv = pages.head_dim, pages.kv_heads
-    counts = [-(-(h + n) // 64) for h, n in zip(batch.held_tokens[first:], batch.new_tokens[first:])]
-    n_blocks, stride, requests = sum(counts), max(counts), len(counts)
-    both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=_BF16, device=q.device)
+    new, held = batch.new_tokens[first:], batch.held_tokens[first:]
+    counts = [-(-(h + n) // 64) for h, n in zip(held, new)]
+    n_blocks, stride, requests, rows = sum(counts), max(counts), len(counts), batch.positions.shape[0]
+    both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
     blocks = torch.empty(requests, stride, dtype=_I32, device=q.device)
-    lib = build.load("append4")
-    step = _Step(batch, first)
-    _check(_at(pages.device, lib.cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv,
-               dim, pages.group, step.req_row_start.data_ptr(), step.req_first_pos.data_ptr(),
-               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1], requests, window or 0,
-               both[0].data_ptr(), both[1].data_ptr(), 1, blocks.data_ptr(), stride, n_blocks), "pages laid out")
-    new = batch.new_tokens[first:]
-    reqs = tensor_core._Requests(step, blocks, 0, requests, max(new), 64 * stride, batch.positions.shape[0])
-    return tensor_core._attend(q, out, both[0], both[1], reqs, n_heads, kv, dim, scale, window, step, step)
+    q_half = torch.empty(rows, n_heads * dim, dtype=torch.float16, device=q.device)
+    row_scale = torch.empty(rows, n_heads, 2, dtype=_F32, device=q.device)
+    starts, places = batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first
+    _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
+               pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.table.shape[1],
+               batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), blocks.data_ptr(), stride,
+               n_blocks, q.data_ptr(), q.stride(0), batch.row_request.data_ptr(), first, rows, sum(new), n_heads // kv, scale,
+               q_half.data_ptr(), row_scale.data_ptr()), "pages laid out")
+    code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q_half.data_ptr(), n_heads * dim,
+               row_scale.data_ptr(), rows, out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1,
+               starts, places, blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, 64, window or 0,
+               tensor_core.status_word(q.device).data_ptr())
+    if code == build.UNSUPPORTED:
+        return False
+    _check(code, "attention4 (tiles)")
+    return True

@@ -181,9 +181,9 @@ def assert_attention(got, want, most, dtype):
 
 
 def assert_attention_laid_out(got, want, most, terms):
-    """bfloat16 portions whose keys and values are laid out in bfloat16: values are off by 2^-9 of themselves, p by 2^-9 in the
-    numerator and in the sum, keys by 2^-9, so that a score is off by d = 2^-9 scale sum |q| |k| at most and a weight by
-    a factor of e^(2 d); on top the result's rounding, and 2^-9 for the tensor cores' and the sum's float32."""
-    moved = torch.expm1(2 * 2.0 ** -9 * terms)
-    worst = ((got.double() - want).abs() - (2.0 ** -8 * want.abs() + (4 * 2.0 ** -9 + moved) * most)).max()
+    """bfloat16 portions whose keys and values are laid out in float16: values are off by 2^-11 of themselves, p by 2^-11 (its sum
+    is float32's), keys and queries by 2^-11 and 2^-28, so that a score is off by d = 2^-11 scale sum |q| |k| at most
+    and a weight by a factor of e^(2 d); on top the result's rounding, and 2^-10 for the tensor cores' and the sum's float32."""
+    moved = torch.expm1(2 * 1.001 * 2.0 ** -11 * terms)
+    worst = ((got.double() - want).abs() - (2.0 ** -8 * want.abs() + (2 * 2.0 ** -11 + 2.0 ** -10 + moved) * most)).max()
     assert torch.isfinite(got.float()).all() and float(worst) <= 0.0, f"over by {float(worst)}"

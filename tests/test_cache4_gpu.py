@@ -229,6 +229,20 @@ def test_attention_of_portions_that_are_laid_out(dim, group, n_rep, kv_heads, pa
     cc.assert_attention(got[:single], want[:single], most[:single], BF16) if single else None
 
 
+@pytest.mark.parametrize("size,stretch,scale", [(1e-7, 1.0, 1.0), (1e8, 1.0, 1e-9), (1.0, 1e-15, 1e14), (1.0, 1e15, 1e-16),
+                                                (1e-20, 1e20, 0.1), (1e25, 1e-22, 1e-3)])
+def test_sizes_in_portions_that_are_laid_out(size, stretch, scale, monkeypatch):
+    """Keys and queries whose numbers float16 would not hold as they are."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    case = cc.Case([(30, 50), (0, 40)], dim=64, group=32, n_rep=4, kv_heads=1, seed=23, size=size)
+    case.pages.scales[1] *= 1e-3 / size                           # values as ever
+    q, spread = case.queries(stretch), []
+    q[0, :64] = 0
+    want, most = case.attention(q, scale, spread=spread)
+    cc.assert_attention_laid_out(_attend(case, q, scale), want, most, spread[0])
+
+
 def test_numbers_that_are_none_in_portions_that_are_laid_out(monkeypatch):
     """A value or key that is no number reaches the rows that see it, whole, and no others; nor does what nobody wrote."""
     from crucible_b200.ops import cache4
