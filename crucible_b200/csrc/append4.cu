@@ -406,6 +406,8 @@ __global__ void __launch_bounds__(256) bound_values4_kernel(const uint32_t* boun
     }
 }
 
+constexpr int C4_LEAST_SPAN = -100;      // the smallest exponent of a request's numbers that counts
+
 struct ExpandParams {
     const uint32_t* codes;
     const uint32_t* scales;
@@ -417,6 +419,7 @@ struct ExpandParams {
     int window;
     __half* keys;            // [blocks of 64 tokens][kv heads][64][D]
     __half* values;
+    int* spans;              // [blocks of 64 tokens][kv heads][keys, values]
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
     const __nv_bfloat16* q;
@@ -429,20 +432,59 @@ struct ExpandParams {
     float2* row_scale;       // [rows][heads]: of the scores, of the results
 };
 
-// Keys (side 0) and values go into float16 times 2^-e, e the exponent of the largest number that the request's first visible
-// key or value can hold in any group: float16's eleven bits then reach from 2^15 above that to 2^-14 below (what is
-// larger stays at 65,504).
-template <int D>
-__device__ __forceinline__ int exponent_of(const ExpandParams& p, int request, int kv, int lo, int side) {
-    const long long at = c4_row(p.table + (size_t)request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, lo);
-    if (at < 0) return 0;
-    const long long row = at + ((long long)side * p.n_pages * p.kv_heads + kv) * p.page_tokens;
-    float most = 0.f;
-    for (int g = 0; g < D / p.group; ++g) {
-        const uint32_t pair = p.scales[row * (D / p.group) + g];
-        most = fmaxf(most, fmaxf(fabsf(c4_low(pair)), fabsf(fmaf(15.f, c4_step(pair), c4_low(pair)))));
+// Which request a block of 64 tokens is of, from how many blocks the requests before it have.
+struct Laid {
+    int request, before, count, first, held;
+};
+
+__device__ __forceinline__ Laid laid_of(const ExpandParams& p, int block) {
+    Laid at = {0, 0, 0, 0, 0};
+    for (; at.request < p.n_requests; ++at.request) {
+        at.first = p.first_pos[at.request];
+        at.held = at.first + p.row_start[at.request + 1] - p.row_start[at.request];
+        at.count = (at.held + 63) >> 6;
+        if (block < at.before + at.count) break;
+        at.before += at.count;
     }
-    return most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 100) : 0;
+    return at;
+}
+
+// The exponents of the largest finite numbers that a block of 64 tokens' keys and values can hold, from their groups' pairs.
+template <int D>
+__global__ void __launch_bounds__(128) span4_kernel(const ExpandParams p) {
+    cb_pdl_trigger();
+    cb_pdl_wait();
+    const Laid in = laid_of(p, blockIdx.x);
+    const int side = threadIdx.x >> 6, pos = ((int)blockIdx.x - in.before) * 64 + (threadIdx.x & 63);
+    int e = C4_LEAST_SPAN;
+    if (in.request < p.n_requests && pos < in.held && pos >= (p.window > 0 ? max(0, in.first - p.window + 1) : 0)) {
+        const long long at = c4_row(p.table + (size_t)in.request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+        if (at >= 0) {
+            const long long row = at + ((long long)side * p.n_pages * p.kv_heads + blockIdx.y) * p.page_tokens;
+            for (int g = 0; g < D / p.group; ++g) {
+                const uint32_t pair = p.scales[row * (D / p.group) + g];
+                const float most = fmaxf(fabsf(c4_low(pair)), fabsf(fmaf(15.f, c4_step(pair), c4_low(pair))));
+                if (most == most) e = max(e, min((int)(__float_as_uint(most) >> 23) - 127, 127));
+            }
+        }
+    }
+    e = __reduce_max_sync(0xffffffffu, e);
+    __shared__ int of_warps[4];
+    if ((threadIdx.x & 31) == 0) of_warps[threadIdx.x >> 5] = e;
+    __syncthreads();
+    if (threadIdx.x < 2)
+        p.spans[((size_t)blockIdx.x * p.kv_heads + blockIdx.y) * 2 + threadIdx.x] = max(of_warps[2 * threadIdx.x], of_warps[2 * threadIdx.x + 1]);
+}
+
+// Keys (x) and values (y) of a request and kv head go into float16 times 2^(14 - e), e the largest of its blocks' exponents:
+// the largest lies below 2^15, and what is up to 2^28 times smaller keeps float16's eleven bits.  Whole warps.
+__device__ __forceinline__ int2 exponents_of(const ExpandParams& p, const Laid& in, int kv) {
+    int2 e = make_int2(C4_LEAST_SPAN, C4_LEAST_SPAN);
+    for (int i = threadIdx.x & 31; i < in.count && in.before + i < p.n_blocks; i += 32) {
+        const int2 of = reinterpret_cast<const int2*>(p.spans)[(size_t)(in.before + i) * p.kv_heads + kv];
+        e = make_int2(max(e.x, of.x), max(e.y, of.y));
+    }
+    return make_int2(__reduce_max_sync(0xffffffffu, e.x) - 14, __reduce_max_sync(0xffffffffu, e.y) - 14);
 }
 
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -455,10 +497,9 @@ __device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
 }
 
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
-// last token; the blocks behind it take 16 rows' queries each.  Which request a block is of follows from how many blocks the
-// requests before it have; tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
+// last token; the blocks behind it take 16 rows' queries each.  Tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
 // its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.  Queries are
-// scaled by a power of two so that a row's largest lies in [2^13, 2^14).
+// scaled by a power of two too, so that a row's largest lies in [2^13, 2^14).
 template <int D>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     cb_pdl_trigger();
@@ -467,16 +508,27 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
     const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
     if (block > p.n_blocks) {
-        __shared__ int exponents[16][2], request_of[16];
+        __shared__ int2 exponents[16];
+        __shared__ int request_of[16];
         const int from = p.row_start[0] + (block - p.n_blocks - 1) * 16, to = min(min(p.row_start[p.n_requests], p.rows), from + 16);
         const int heads = p.kv_heads * p.n_rep;
-        if (threadIdx.x < 32) {
-            const int row = from + (threadIdx.x >> 1), side = threadIdx.x & 1;
-            int request = row >= 0 && row < to ? p.row_request[row] - p.first_request : -1;
+        int2 e = make_int2(0, 0);
+        for (int i = threadIdx.x >> 5, last = -1; i < 16; i += 8) {
+            int request = from + i < to ? p.row_request[from + i] - p.first_request : -1;
             if (request >= p.n_requests) request = -1;
-            exponents[threadIdx.x >> 1][side] = request < 0 ? 0
-                : exponent_of<D>(p, request, blockIdx.y, p.window > 0 ? max(0, p.first_pos[request] - p.window + 1) : 0, side);
-            request_of[threadIdx.x >> 1] = request;
+            if (request >= 0 && request != last) {
+                Laid in = {0, 0, 0, 0, 0};
+                for (; in.request <= request; ++in.request) {
+                    in.before += in.count;
+                    in.count = (p.first_pos[in.request] + p.row_start[in.request + 1] - p.row_start[in.request] + 63) >> 6;
+                }
+                e = exponents_of(p, in, blockIdx.y);
+                last = request;
+            }
+            if (lane == 0) {
+                exponents[i] = e;
+                request_of[i] = request;
+            }
         }
         __syncthreads();
         constexpr int WIDE = 4;
@@ -506,7 +558,7 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
                 for (int e = 0; e < 8; ++e) v[u][e] *= two_to(up);
                 store_halves(p.q_half + at * D + within * 8, v[u]);
                 if (within == 0)
-                    p.row_scale[at] = make_float2(p.scale_log2 * two_to(-up) * two_to(exponents[r][0]), two_to(exponents[r][1]));
+                    p.row_scale[at] = make_float2(p.scale_log2 * two_to(-up) * two_to(exponents[r].x), two_to(exponents[r].y));
             }
         }
         return;
@@ -520,20 +572,13 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
             before += count;
         }
     }
-    int request = 0, before = 0, held = 0, first = 0;
-    for (; request < p.n_requests; ++request) {
-        first = p.first_pos[request];
-        held = first + p.row_start[request + 1] - p.row_start[request];
-        const int count = (held + 63) >> 6;
-        if (block < before + count) break;
-        before += count;
-    }
-    const int index = block - before;
+    const Laid in = laid_of(p, block);
+    const int request = in.request, held = in.held, index = block - in.before;
     const bool some = block < p.n_blocks && request < p.n_requests;
-    const int lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    const int lo = p.window > 0 ? max(0, in.first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
-    const float down_k = some ? two_to(-exponent_of<D>(p, request, blockIdx.y, lo, 0)) : 1.f;
-    const float down_v = some ? two_to(-exponent_of<D>(p, request, blockIdx.y, lo, 1)) : 1.f;
+    const int2 e = some ? exponents_of(p, in, blockIdx.y) : make_int2(0, 0);
+    const float down_k = two_to(-e.x), down_v = two_to(-e.y);
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     __syncthreads();
     const int f = eight_of<D>(within);
@@ -650,19 +695,25 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
-                         int n_requests, int window, void* keys, void* values, int* blocks, int block_stride, int n_blocks,
+                         int n_requests, int window, void* keys, void* values, int* spans, int* blocks, int block_stride, int n_blocks,
                          const void* q, long long q_stride, const int* row_request, int first_request, int rows, int most_rows,
                          int n_rep, float scale, void* q_half, float* row_scale, void* stream) {
     if (n_blocks <= 0 || most_rows <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
-                            reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), blocks, block_stride,
+                            reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans, blocks, block_stride,
                             n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, row_request, first_request, rows,
                             n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), reinterpret_cast<float2*>(row_scale)};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + 15) / 16), (unsigned)kv_heads);
-    if (head_dim == 64) cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);
-    else if (head_dim == 128) cb_launch(expand4_kernel<128>, grid, dim3(256), 0, s, p);
+    const dim3 blocks_grid((unsigned)n_blocks, (unsigned)kv_heads);
+    if (head_dim == 64) {
+        cb_launch(span4_kernel<64>, blocks_grid, dim3(128), 0, s, p);
+        cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);
+    } else if (head_dim == 128) {
+        cb_launch(span4_kernel<128>, blocks_grid, dim3(128), 0, s, p);
+        cb_launch(expand4_kernel<128>, grid, dim3(256), 0, s, p);
+    }
     else return CB_ERR_UNSUPPORTED;
     return cb_last_error();
 }

@@ -680,7 +680,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             // P = exp2(s * scale - reference) in bf16, two a column, over the scores' own columns:
             // keys 0-63 into the first 32, 64-127 into the next (their scores, columns 64-127, are
             // read after the first half's, whose columns are 0-63)
-            const float off = m_ref == -INFINITY ? 0.f : -m_ref;
+            // (in float16, 2^7 of that: at most 2^15, and what is 2^-21 of the largest still has its eleven bits)
+            const float off = (m_ref == -INFINITY ? 0.f : -m_ref) + (GATE == GATE_SCALED ? 7.f : 0.f);
             const uint64_t off2 = pair_of(off, off);
             uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll 1

@@ -457,15 +457,16 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
     counts = [-(-(h + n) // 64) for h, n in zip(held, new)]
     n_blocks, stride, requests, rows = sum(counts), max(counts), len(counts), batch.positions.shape[0]
     both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
-    blocks = torch.empty(requests, stride, dtype=_I32, device=q.device)
+    spans = torch.empty(2 * n_blocks * kv + requests * stride, dtype=_I32, device=q.device)
+    blocks = spans[2 * n_blocks * kv:]
     q_half = torch.empty(rows, n_heads * dim, dtype=torch.float16, device=q.device)
     row_scale = torch.empty(rows, n_heads, 2, dtype=_F32, device=q.device)
     starts, places = batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first
     _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.table.shape[1],
-               batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), blocks.data_ptr(), stride,
-               n_blocks, q.data_ptr(), q.stride(0), batch.row_request.data_ptr(), first, rows, sum(new), n_heads // kv, scale,
-               q_half.data_ptr(), row_scale.data_ptr()), "pages laid out")
+               batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
+               blocks.data_ptr(), stride, n_blocks, q.data_ptr(), q.stride(0), batch.row_request.data_ptr(), first, rows, sum(new),
+               n_heads // kv, scale, q_half.data_ptr(), row_scale.data_ptr()), "pages laid out")
     code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q_half.data_ptr(), n_heads * dim,
                row_scale.data_ptr(), rows, out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1,
                starts, places, blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, 64, window or 0,

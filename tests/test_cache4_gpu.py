@@ -243,6 +243,25 @@ def test_sizes_in_portions_that_are_laid_out(size, stretch, scale, monkeypatch):
     cc.assert_attention_laid_out(_attend(case, q, scale), want, most, spread[0])
 
 
+@pytest.mark.parametrize("small", [0.0, 1e-12, 1e-7, 1e-3])
+def test_spans_in_portions_that_are_laid_out(small, monkeypatch):
+    """What a request's keys and values are scaled by goes by all of them that are visible, not by one, and not by what the
+    window has passed or what lies behind the last."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    for window in (None, 150):
+        case = cc.Case([(90, 70), (200, 40), (0, 40)], dim=64, group=32, n_rep=4, kv_heads=2, seed=29)
+        place = case.table[0].long()
+        case.pages.scales[:, place[0], :, 0] *= small             # the first visible, in one request
+        case.pages.scales[:, place[3]] *= small
+        if window is not None:
+            for j in range(5):                                    # (positions up to 50 are passed in the second)
+                case.pages.scales[:, int(case.table[1, 0]), :, j] *= 1e20
+        q, spread = case.queries(), []
+        want, most = case.attention(q, 0.125, window=window, spread=spread)
+        cc.assert_attention_laid_out(_attend(case, q, 0.125, window=window), want, most, spread[0])
+
+
 def test_numbers_that_are_none_in_portions_that_are_laid_out(monkeypatch):
     """A value or key that is no number reaches the rows that see it, whole, and no others; nor does what nobody wrote."""
     from crucible_b200.ops import cache4
