@@ -358,14 +358,17 @@ __global__ void __launch_bounds__(2 * D) bounds4_kernel(const AppendParams p, in
     if (tid == 0) p.bound_scales[to] = scale;
 }
 
-// Eight neighbouring features of the row `at` (there: it is one; every lane of the warp takes part).
+// Eight neighbouring features of a row: its word and pair, then their values (every lane of the warp takes part).
 template <int D>
-__device__ __forceinline__ void eight_values(const uint32_t* codes, const uint32_t* scales, long long at, bool there, int group,
-                                             int within, float (&v)[8]) {
-    const int l = within & 7, f = eight_of<D>(within);
-    const uint32_t m = transposed(there ? codes[at * (D / 8) + l * (D / 64) + (within >> 3)] : 0u, l);
-    const uint32_t pair = there ? scales[at * (D / group) + f / group] : 0u;
-    const float step = c4_step(pair), low = c4_low(pair);
+__device__ __forceinline__ uint2 eight_fetched(const uint32_t* codes, const uint32_t* scales, long long at, bool there, int group,
+                                               int within) {
+    return there ? make_uint2(codes[at * (D / 8) + (within & 7) * (D / 64) + (within >> 3)], scales[at * (D / group) + eight_of<D>(within) / group])
+                 : make_uint2(0u, 0u);
+}
+
+__device__ __forceinline__ void eight_values(uint2 from, int within, float (&v)[8]) {
+    const uint32_t m = transposed(from.x, within & 7);
+    const float step = c4_step(from.y), low = c4_low(from.y);
     codes_as_floats(m, v);
 #pragma unroll
     for (int g = 0; g < 8; ++g) v[g] = fmaf(v[g], step, low);
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(256) values4_kernel(const uint32_t* codes, con
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const long long at = row + j * stride + lane / LANES;
-            eight_values<D>(codes, scales, at, at < rows && lane < LANES * PER_WARP, group, within, v[j]);
+            eight_values(eight_fetched<D>(codes, scales, at, at < rows && lane < LANES * PER_WARP, group, within), within, v[j]);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -420,16 +423,15 @@ struct ExpandParams {
     __half* keys;            // [blocks of 64 tokens][kv heads][64][D]
     __half* values;
     int* spans;              // [blocks of 64 tokens][kv heads][keys, values]
+    float2* factors;         // [requests][kv heads]: what keys and values were divided by
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
     const __nv_bfloat16* q;
     long long q_stride;
-    const int* row_request;
-    int first_request;       // the requests' numbers in row_request begin with it
     int rows, n_rep;
     float scale_log2;
     __half* q_half;          // [rows][heads][D]
-    float2* row_scale;       // [rows][heads]: of the scores, of the results
+    float* row_scale;        // [rows][heads]: log2(e) times the scale over what the queries were multiplied by
 };
 
 // Which request a block of 64 tokens is of, from how many blocks the requests before it have.
@@ -449,7 +451,17 @@ __device__ __forceinline__ Laid laid_of(const ExpandParams& p, int block) {
     return at;
 }
 
-// The exponents of the largest finite numbers that a block of 64 tokens' keys and values can hold, from their groups' pairs.
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
+}
+
+// A block of threads a block of 64 tokens and kv head: the exponents of the largest finite numbers that its keys and values
+// can hold, from their groups' pairs.
 template <int D>
 __global__ void __launch_bounds__(128) span4_kernel(const ExpandParams p) {
     cb_pdl_trigger();
@@ -487,19 +499,10 @@ __device__ __forceinline__ int2 exponents_of(const ExpandParams& p, const Laid& 
     return make_int2(__reduce_max_sync(0xffffffffu, e.x) - 14, __reduce_max_sync(0xffffffffu, e.y) - 14);
 }
 
-__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
-__device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
-    __half2 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
-}
-
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
-// last token; the blocks behind it take 16 rows' queries each.  Tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
-// its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.  Queries are
-// scaled by a power of two too, so that a row's largest lies in [2^13, 2^14).
+// last token; the blocks behind it take 16 rows' queries each, which go into float16 scaled by a power of two so that a row's
+// largest lies in [2^13, 2^14).  Tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
+// its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.
 template <int D>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     cb_pdl_trigger();
@@ -508,57 +511,35 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
     const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
     if (block > p.n_blocks) {
-        __shared__ int2 exponents[16];
-        __shared__ int request_of[16];
-        const int from = p.row_start[0] + (block - p.n_blocks - 1) * 16, to = min(min(p.row_start[p.n_requests], p.rows), from + 16);
-        const int heads = p.kv_heads * p.n_rep;
-        int2 e = make_int2(0, 0);
-        for (int i = threadIdx.x >> 5, last = -1; i < 16; i += 8) {
-            int request = from + i < to ? p.row_request[from + i] - p.first_request : -1;
-            if (request >= p.n_requests) request = -1;
-            if (request >= 0 && request != last) {
-                Laid in = {0, 0, 0, 0, 0};
-                for (; in.request <= request; ++in.request) {
-                    in.before += in.count;
-                    in.count = (p.first_pos[in.request] + p.row_start[in.request + 1] - p.row_start[in.request] + 63) >> 6;
-                }
-                e = exponents_of(p, in, blockIdx.y);
-                last = request;
-            }
-            if (lane == 0) {
-                exponents[i] = e;
-                request_of[i] = request;
-            }
-        }
-        __syncthreads();
         constexpr int WIDE = 4;
-        for (int i0 = (threadIdx.x >> 5) * PER_WARP; i0 < 16 * p.n_rep; i0 += WIDE * 8 * PER_WARP) {        // (whole warps: shuffles)
+        const int heads = p.kv_heads * p.n_rep;
+        const int from = p.row_start[0] + (block - p.n_blocks - 1) * 16, rows = min(min(p.row_start[p.n_requests], p.rows) - from, 16);
+        for (int i0 = (threadIdx.x >> 5) * PER_WARP; i0 < rows * p.n_rep; i0 += WIDE * 8 * PER_WARP) {      // (whole warps: shuffles)
             float v[WIDE][8];
 #pragma unroll
             for (int u = 0; u < WIDE; ++u) {
                 const int j = i0 + u * 8 * PER_WARP + lane / LANES;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-                if (j < 16 * p.n_rep && lane < LANES * PER_WARP && request_of[j / p.n_rep] >= 0)
+                if (j < rows * p.n_rep && lane < LANES * PER_WARP)
                     load_eight<__nv_bfloat16, true>(p.q + (size_t)(from + j / p.n_rep) * p.q_stride
                                                     + (size_t)(blockIdx.y * p.n_rep + j % p.n_rep) * D + within * 8, v[u]);
             }
 #pragma unroll
             for (int u = 0; u < WIDE; ++u) {
-                const int j = i0 + u * 8 * PER_WARP + lane / LANES, r = j / p.n_rep;
+                const int j = i0 + u * 8 * PER_WARP + lane / LANES;
                 float most = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[u][e]));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const int up = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
-                if (j >= 16 * p.n_rep || lane >= LANES * PER_WARP || request_of[r] < 0) continue;
-                const size_t at = (size_t)(from + r) * heads + blockIdx.y * p.n_rep + j % p.n_rep;
+                if (j >= rows * p.n_rep || lane >= LANES * PER_WARP) continue;
+                const size_t at = (size_t)(from + j / p.n_rep) * heads + blockIdx.y * p.n_rep + j % p.n_rep;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[u][e] *= two_to(up);
                 store_halves(p.q_half + at * D + within * 8, v[u]);
-                if (within == 0)
-                    p.row_scale[at] = make_float2(p.scale_log2 * two_to(-up) * two_to(exponents[r].x), two_to(exponents[r].y));
+                if (within == 0) p.row_scale[at] = p.scale_log2 * two_to(-up);
             }
         }
         return;
@@ -577,45 +558,48 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     const bool some = block < p.n_blocks && request < p.n_requests;
     const int lo = p.window > 0 ? max(0, in.first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
-    const int2 e = some ? exponents_of(p, in, blockIdx.y) : make_int2(0, 0);
-    const float down_k = two_to(-e.x), down_v = two_to(-e.y);
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
-    __syncthreads();
     const int f = eight_of<D>(within);
     const long long side_rows = (long long)p.n_pages * p.kv_heads * p.page_tokens;
-    float v[ROUNDS][8];
-    long long at[ROUNDS];
+    uint2 key[ROUNDS], value[ROUNDS];
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j) {
-        const int t = (j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES, pos = index * 64 + t;
-        at[j] = -1;
-        if (some && lane < LANES * PER_WARP && pos < held && pos >= lo) {
-            at[j] = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
-            if (at[j] >= 0) at[j] += (long long)blockIdx.y * p.page_tokens;
-        }
-        eight_values<D>(p.codes, p.scales, at[j] + side_rows, at[j] >= 0, p.group, within, v[j]);
-        if (!(v[j][0] == v[j][0])) {                        // (a group's numbers are all none or all some)
-            bad[t] = 1;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-        }
+        const int pos = index * 64 + (j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES;
+        long long at = -1;
+        if (some && lane < LANES * PER_WARP && pos < held && pos >= lo)
+            at = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+        if (at >= 0) at += (long long)blockIdx.y * p.page_tokens;
+        key[j] = eight_fetched<D>(p.codes, p.scales, at, at >= 0, p.group, within);
+        value[j] = eight_fetched<D>(p.codes, p.scales, at + side_rows, at >= 0, p.group, within);
     }
+    const int2 e = some ? exponents_of(p, in, blockIdx.y) : make_int2(0, 0);
+    const float down_k = two_to(-e.x), down_v = two_to(-e.y);
+    if (some && index == 0 && threadIdx.x == 0)
+        p.factors[(size_t)request * p.kv_heads + blockIdx.y] = make_float2(two_to(e.x), two_to(e.y));
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j)
+        if (c4_low(value[j].y) != c4_low(value[j].y)) {
+            bad[(j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES] = 1;
+            value[j] = make_uint2(0u, 0u);
+        }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j) {
         const int t = (j * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / LANES;
         const long long to = (((long long)block * p.kv_heads + blockIdx.y) * 64 + t) * D + f;
-        float k[8];
-        eight_values<D>(p.codes, p.scales, at[j], at[j] >= 0, p.group, within, k);
+        float k[8], v[8];
+        eight_values(key[j], within, k);
+        eight_values(value[j], within, v);
         if (lane >= LANES * PER_WARP) continue;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (bad[t]) k[e] = __int_as_float(0x7fffffff);
             else if (k[e] == k[e]) k[e] = fminf(fmaxf(k[e] * down_k, -65504.f), 65504.f);
-            v[j][e] = fminf(fmaxf(v[j][e] * down_v, -65504.f), 65504.f);
+            v[e] = fminf(fmaxf(v[e] * down_v, -65504.f), 65504.f);
         }
         store_halves(p.keys + to, k);
-        store_halves(p.values + to, v[j]);
+        store_halves(p.values + to, v);
     }
 }
 
@@ -695,25 +679,25 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
-                         int n_requests, int window, void* keys, void* values, int* spans, int* blocks, int block_stride, int n_blocks,
-                         const void* q, long long q_stride, const int* row_request, int first_request, int rows, int most_rows,
+                         int n_requests, int window, void* keys, void* values, int* spans, float* factors, int* blocks,
+                         int block_stride, int n_blocks, const void* q, long long q_stride, int rows, int most_rows,
                          int n_rep, float scale, void* q_half, float* row_scale, void* stream) {
     if (n_blocks <= 0 || most_rows <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
-                            reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans, blocks, block_stride,
-                            n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, row_request, first_request, rows,
-                            n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), reinterpret_cast<float2*>(row_scale)};
+                            reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans,
+                            reinterpret_cast<float2*>(factors), blocks, block_stride,
+                            n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, rows,
+                            n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), row_scale};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const dim3 spans_grid((unsigned)n_blocks, (unsigned)kv_heads);
     const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + 15) / 16), (unsigned)kv_heads);
-    const dim3 blocks_grid((unsigned)n_blocks, (unsigned)kv_heads);
     if (head_dim == 64) {
-        cb_launch(span4_kernel<64>, blocks_grid, dim3(128), 0, s, p);
+        cb_launch(span4_kernel<64>, spans_grid, dim3(128), 0, s, p);
         cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);
     } else if (head_dim == 128) {
-        cb_launch(span4_kernel<128>, blocks_grid, dim3(128), 0, s, p);
+        cb_launch(span4_kernel<128>, spans_grid, dim3(128), 0, s, p);
         cb_launch(expand4_kernel<128>, grid, dim3(256), 0, s, p);
-    }
-    else return CB_ERR_UNSUPPORTED;
+    } else return CB_ERR_UNSUPPORTED;
     return cb_last_error();
 }

@@ -88,7 +88,8 @@ struct TcAttnParams {
     int n_pages;             // of the pool
     int runs;                // 1: the 4-D maps may be used for tiles whose pages are consecutive
     int* status;
-    const float2* row_scale; // GATE_SCALED: [rows][n_heads], of the scores (log2(e) among it) and of the results
+    const float* row_scale;  // GATE_SCALED: [rows][n_heads], of the scores, log2(e) among it
+    const float2* factors;   // GATE_SCALED: [requests][n_kv_heads], of the scores and of the results
 };
 
 // GATE: the results' gate, fixed when it is compiled: the epilogue runs once per block and its instructions
@@ -563,8 +564,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (GATE == GATE_HEAD)
                 gate_f = sigmoid(__bfloat162float(p.gate[(size_t)tok * p.gate_stride + head]));
             if (GATE == GATE_SCALED) {
-                const float2 both = p.row_scale[(size_t)tok * p.n_heads + head];
-                scale_log2 = both.x;
+                const float2 both = p.factors[(size_t)req * gridDim.x + kv_head];
+                scale_log2 = p.row_scale[(size_t)tok * p.n_heads + head] * both.x;
                 out_scale = both.y;
             }
         }
@@ -863,7 +864,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
                              const int* req_first_pos, const int* block_table, int table_stride, int n_requests,
                              int max_new_tokens, int n_heads, int n_kv_heads, int head_dim, int page_tokens, float scale,
                              int window, int chunked, int keep_first, float out_scale, const float* sinks, const void* gate,
-                             int gate_stride, int gate_per_head, const float* row_scale, int lead, int value_cols, int* status,
+                             int gate_stride, int gate_per_head, const float* row_scale, const float* factors, int lead, int value_cols, int* status,
                              void* stream) {
     if (n_requests <= 0 || max_new_tokens <= 0) return 0;
     if (keep_first < 0 || !(scale > 0.f)) return CB_ERR_UNSUPPORTED;
@@ -925,7 +926,8 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     p.gate_stride = gate_stride;
     p.out_scale = out_scale;
     p.status = status;
-    p.row_scale = reinterpret_cast<const float2*>(row_scale);
+    p.row_scale = row_scale;
+    p.factors = reinterpret_cast<const float2*>(factors);
     const int q_tiles = (max_new_tokens * n_rep + p.tile_rows - 1) / p.tile_rows;
     if (n_requests > 65535 || q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     // (single tokens of more than a tile of query heads keep ranks like a portion's)
@@ -953,18 +955,19 @@ CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_r
     return attention_tcgen05(qkv, qkv_stride, n_rows, out, out_stride, k_cache, v_cache, n_pages, req_row_start, req_first_pos,
                              block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
                              scale, window, chunked, keep_first, out_scale, sinks, gate, gate_stride, gate_per_head, nullptr,
-                             lead, value_cols, status, stream);
+                             nullptr, lead, value_cols, status, stream);
 }
 
-// The same over queries, keys and values in float16 (heads of 64 and 128): row_scale [n_rows][n_heads][2], factors for the scores
-// (log2(e) among it) and for the results of each row and head.
-CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, int n_rows, void* out,
-                                        int out_stride, const void* keys, const void* values, int n_pages,
+// The same over queries, keys and values in float16 (heads of 64 and 128): factors for the scores of each row and head, log2(e)
+// among them (row_scale [n_rows][n_heads]), and for the scores and the results of each request and kv head (factors
+// [n_requests][n_kv_heads][2]).
+CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, const float* factors, int n_rows,
+                                        void* out, int out_stride, const void* keys, const void* values, int n_pages,
                                         const int* req_row_start, const int* req_first_pos, const int* block_table,
                                         int table_stride, int n_requests, int max_new_tokens, int n_heads, int n_kv_heads,
                                         int head_dim, int page_tokens, int window, int* status, void* stream) {
     if (head_dim > 128) return CB_ERR_UNSUPPORTED;
     return attention_tcgen05(q, q_stride, n_rows, out, out_stride, keys, values, n_pages, req_row_start, req_first_pos,
                              block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
-                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, 0, 0, status, stream);
+                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, factors, 0, 0, status, stream);
 }
