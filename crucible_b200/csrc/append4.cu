@@ -451,6 +451,9 @@ __device__ __forceinline__ Laid laid_of(const ExpandParams& p, int block) {
     return at;
 }
 
+// Rows whose queries a block takes: 64 of a kv head, or one row's.
+__host__ __device__ __forceinline__ int q_rows(int n_rep) { return n_rep < 64 ? 64 / n_rep : 1; }
+
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 __device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
@@ -500,7 +503,7 @@ __device__ __forceinline__ int2 exponents_of(const ExpandParams& p, const Laid& 
 }
 
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
-// last token; the blocks behind it take 16 rows' queries each, which go into float16 scaled by a power of two so that a row's
+// last token; the blocks behind it take some rows' queries each, which go into float16 scaled by a power of two so that a row's
 // largest lies in [2^13, 2^14).  Tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
 // its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.
 template <int D>
@@ -513,7 +516,8 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     if (block > p.n_blocks) {
         constexpr int WIDE = 4;
         const int heads = p.kv_heads * p.n_rep;
-        const int from = p.row_start[0] + (block - p.n_blocks - 1) * 16, rows = min(min(p.row_start[p.n_requests], p.rows) - from, 16);
+        const int each = q_rows(p.n_rep), from = p.row_start[0] + (block - p.n_blocks - 1) * each;
+        const int rows = min(min(p.row_start[p.n_requests], p.rows) - from, each);
         for (int i0 = (threadIdx.x >> 5) * PER_WARP; i0 < rows * p.n_rep; i0 += WIDE * 8 * PER_WARP) {      // (whole warps: shuffles)
             float v[WIDE][8];
 #pragma unroll
@@ -691,7 +695,7 @@ CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int
                             n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), row_scale};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const dim3 spans_grid((unsigned)n_blocks, (unsigned)kv_heads);
-    const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + 15) / 16), (unsigned)kv_heads);
+    const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + q_rows(n_rep) - 1) / q_rows(n_rep)), (unsigned)kv_heads);
     if (head_dim == 64) {
         cb_launch(span4_kernel<64>, spans_grid, dim3(128), 0, s, p);
         cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);

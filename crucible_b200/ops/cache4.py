@@ -428,7 +428,7 @@ LAID_OUT: Optional[bool] = None       # tests fix which way portions go
 
 def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
     """Whether the portions of the requests from `first` on go by `_tiles`: bfloat16 rows of heads of 64 and 128, 64 of a kv head
-    and more (others have no kernel there that is quicker).  us, by what was measured: 6 and 1.7 a million features laid out, then a
+    and more (others have no kernel there that is quicker).  us, by what was measured: 8.5 and 1.7 a million features laid out, then a
     tile of 128 rows walks its keys alone, 7.2 a thousand, or all of them at 0.75 PFLOP/s."""
     dim, kv = pages.head_dim, pages.kv_heads
     new, held = batch.new_tokens[first:], batch.held_tokens[first:]
@@ -442,7 +442,7 @@ def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
     reach = max(map(_add, new, held))
     seen = reach if window is None else min(reach, window + 128)
     pairs = sum([n * min(h + n / 2, seen) for n, h in zip(new, held)])
-    tiles = (6.0 + 1.7e-6 * (sum(new) + sum(held)) * kv * dim
+    tiles = (8.5 + 1.7e-6 * (sum(new) + sum(held)) * kv * dim
              + max(0.0072 * min(seen, reach), 4e-6 * dim * n_heads * pairs / 750.0))
     return tiles < walk
 
