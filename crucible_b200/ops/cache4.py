@@ -153,9 +153,9 @@ class Batch:
         self.new_tokens, self.held_tokens = new_tokens, held_tokens
         self.requests = requests = len(new_tokens)
         self.device = dev = positions.get_device()
-        if not (requests > 0 and len(held_tokens) == requests and table.dim() == 2 and len(table) == requests and table.size(1) > 0
+        if not (requests > 0 and len(held_tokens) == requests and table.dim() == 2 and table.size(0) == requests and table.size(1) > 0
                 and positions.dim() == 1 == row_request.dim() == row_start.dim() == first_pos.dim()
-                and len(row_request) == len(positions) and len(row_start) == requests + 1 and len(first_pos) == requests
+                and row_request.size(0) == positions.size(0) and row_start.size(0) == requests + 1 and first_pos.size(0) == requests
                 and positions.dtype is _I32 and row_request.dtype is _I32 and row_start.dtype is _I32
                 and first_pos.dtype is _I32 and table.dtype is _I32
                 and positions.is_contiguous() and row_request.is_contiguous() and row_start.is_contiguous()
@@ -332,7 +332,7 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
     if behind < rows:
         lead = max(behind, batch.lead)
-        if lead < batch.requests and _laid_out(q, out, n_heads, batch, pages, window, lead):
+        if lead < batch.requests and _laid_out(q, out, n_heads, batch, pages, window, behind, lead):
             if behind < lead:
                 _walk(q, out, n_heads, scale, batch, pages, window, None, behind, lead)
             if _tiles(q, out, n_heads, scale, batch, pages, window, lead):
@@ -378,20 +378,32 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
 def _dealt(dim, kv, n_rep, group, f32, batch, window, first, last) -> tuple:
     """How the requests first .. last - 1 go through the walking kernel: (column tiles a block, blocks of a cluster, blocks of a
     stream, us that it may take)."""
-    blocks = last - first
-    most_rows = batch.most_new if blocks == batch.requests else max(batch.new_tokens[first:last])
+    requests = last - first
+    new, held = batch.new_tokens, batch.held_tokens
+    if requests < batch.requests:
+        new, held = new[first:last], held[first:last]
+    most_rows = max(new)
     reach = batch.reach if window is None else min(batch.reach, window + most_rows)
     tiles = -(-reach // 16) + (window is not None)
-    total = (blocks * tiles if blocks == 1 or window is not None else
-             (sum(batch.held_tokens[first:last]) + sum(batch.new_tokens[first:last])) // 16 + blocks)
-    return _columns(dim, kv, n_rep, group, f32, most_rows, blocks, tiles, total)
+    columns = _columns(n_rep, f32, dim, most_rows)
+    if requests > 1 and most_rows > min(new):              # (blocks behind a request's last row end at once)
+        per = [kv * -(-n * n_rep // (8 * columns)) for n in new]
+        blocks = sum(per)
+        total = sum([p * min(tiles, (n + h) // 16 + 1) for p, n, h in zip(per, new, held)])
+    else:
+        per = kv * -(-most_rows * n_rep // (8 * columns))
+        blocks = requests * per
+        total = per * (requests * tiles if requests == 1 or window is not None else (sum(held) + sum(new)) // 16 + requests)
+    return columns, *_dealt_to(dim, group, f32, columns, blocks, tiles, total)
 
 
-def _columns(dim, kv, n_rep, group, f32, most_rows, blocks, tiles, total) -> tuple:
-    columns = 1 if f32 or most_rows * n_rep <= 8 or dim > 128 else 2
-    per = kv * -(-most_rows * n_rep // (8 * columns))
-    return columns, *_shares(blocks * per, tiles, total * per, _resident(dim, group, columns, f32),
-                             (dim / 128) ** 0.6 * (2.0 if f32 else 1.3 if columns == 2 else 1.0))
+def _columns(n_rep, f32, dim, most_rows) -> int:
+    return 1 if f32 or most_rows * n_rep <= 8 or dim > 128 else 2
+
+
+def _dealt_to(dim, group, f32, columns, blocks, tiles, total) -> tuple:
+    return _shares(blocks, tiles, total, _resident(dim, group, columns, f32),
+                   (dim / 128) ** 0.6 * (2.0 if f32 else 1.3 if columns == 2 else 1.0))
 
 
 def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> None:
@@ -403,7 +415,9 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     if picks is not None:
         most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
-        columns, shares, stream, _ = _columns(dim, kv, n_rep, pages.group, f32, 1, blocks, tiles, tiles * blocks)
+        columns = _columns(n_rep, f32, dim, 1)
+        per = blocks * kv * -(-n_rep // (8 * columns))
+        shares, stream, _ = _dealt_to(dim, pages.group, f32, columns, per, tiles, tiles * per)
     else:
         most_rows = batch.most_new if last - first == batch.requests else max(batch.new_tokens[first:last])
         columns, shares, stream, _ = _dealt(dim, kv, n_rep, pages.group, f32, batch, window, first, last)
@@ -426,10 +440,11 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
 LAID_OUT: Optional[bool] = None       # tests fix which way portions go
 
 
-def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
-    """Whether the portions of the requests from `first` on go by `_tiles`: bfloat16 rows of heads of 64 and 128, 64 of a kv head
-    and more (others have no kernel there that is quicker).  us, by what was measured: 8.5 and 1.7 a million features laid out, then a
-    tile of 128 rows walks its keys alone, 7.2 a thousand, or all of them at 0.75 PFLOP/s."""
+def _laid_out(q, out, n_heads, batch, pages, window, behind, first) -> bool:
+    """Whether the portions of the requests from `first` on go by `_tiles`, those from `behind` on before them walked by
+    themselves: bfloat16 rows of heads of 64 and 128, 64 of a kv head and more (others have no kernel there that is quicker).
+    us, by what was measured: 8.5 and 1.7 a million features laid out, then a tile of 128 rows walks its keys alone, 7.2
+    a thousand, or all of them at 0.75 PFLOP/s."""
     dim, kv = pages.head_dim, pages.kv_heads
     new, held = batch.new_tokens[first:], batch.held_tokens[first:]
     n_rep = n_heads // kv
@@ -438,12 +453,14 @@ def _laid_out(q, out, n_heads, batch, pages, window, first) -> bool:
         return False
     if LAID_OUT is not None:
         return LAID_OUT
-    walk = _dealt(dim, kv, n_rep, pages.group, False, batch, window, first, batch.requests)[3]
+    walk = _dealt(dim, kv, n_rep, pages.group, False, batch, window, behind, batch.requests)[3]
     reach = max(map(_add, new, held))
     seen = reach if window is None else min(reach, window + 128)
     pairs = sum([n * min(h + n / 2, seen) for n, h in zip(new, held)])
     tiles = (8.5 + 1.7e-6 * (sum(new) + sum(held)) * kv * dim
              + max(0.0072 * min(seen, reach), 4e-6 * dim * n_heads * pairs / 750.0))
+    if behind < first:
+        tiles += _dealt(dim, kv, n_rep, pages.group, False, batch, window, behind, first)[3]
     return tiles < walk
 
 
