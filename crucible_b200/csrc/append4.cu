@@ -3,17 +3,20 @@
 //   append4   a row's q and k are rotated by its position, k and v go to the row's place in the pages.
 //             A block a row and a run of its heads, so that its position, place and angles are fetched once; D/8
 //             lanes a head, eight neighbouring features a lane: 16 bytes a load where rows are aligned, the next
-//             head's before this one's are worked on.  Lane l of eight takes the features whose codes lie at bits 4l.. 4l + 3 of their words, so that
-//             eight lanes' codes are turned into eight words by a transposition of 8 x 8 nibbles, three
-//             shuffles; a group's least and largest number take two to four shuffles each.
+//             head's before this one's are worked on.  Lane l of eight takes the features whose codes lie at bits
+//             4l.. 4l + 3 of their words, so that eight lanes' codes are turned into eight words by a transposition
+//             of 8 x 8 nibbles, three shuffles; a group's least and largest number take two to four shuffles each.
+//             2,048 rows of 32 + 16 heads of 128 in bfloat16: 13.8 us, 3.1 TB/s of rows and words (a block's chain of
+//             position, place, angles, numbers, shuffles, with three blocks an SM to hide it); 64 rows 2.5 us, one 2.
 //   bounds4   of every page that the step wrote: each feature's largest and least key over the tokens that
 //             the page now holds, in 8 bits with one scale.  A block a (row, kv head), a thread a word of codes and
-//             every 16th token; only the last row of each page's run does anything.
+//             every 16th token; only the last row of each page's run does anything.  64 rows of 8 heads of 128,
+//             pages of 64: 5.5 us, a thread's chain through place, codes and pairs, then a block's largest.
 //   values4   the whole pool as float32 or bfloat16 rows.
+//   span4     before expand4: how large the numbers of every 64 tokens can be.
 //   expand4   the pages of some requests as rows in pages of 64 tokens, for attention over many rows, and the requests'
-//             queries, all in float16.
-//
-// All are bound by memory in large calls and by their launch in small ones.
+//             queries, all in float16.  2,048 tokens of 8 heads of 128 under 32 query heads: both 17 us (span4 3), 42 MB
+//             of which 32 are queries; everything a block needs is asked for before it works on any of it.
 #define CB_PDL_BIT 6      // with the other quantised operators
 #include "cache4.cuh"
 

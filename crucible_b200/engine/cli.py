@@ -2,6 +2,7 @@
 
     llm-engine generate MODEL --prompt-ids 1,2,3 [--max-tokens 40] [--temperature 0.8]
                               [--top-k 40] [--seed 1234] [--graph] [--dtype bfloat16]
+                              [--cache-group 64 [--attend-pages 16]]
     llm-engine inspect MODEL
     llm-engine logits MODEL --tokens 1,2,3 [--top 10]
     llm-engine random-weights --shape 120m --seed 0 OUT

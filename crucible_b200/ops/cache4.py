@@ -13,6 +13,10 @@ prompts; `pick_pages4` chooses for every row and kv head the pages whose bounds 
 `attention4(..., picks=)` to read alone.  Pages that are to be picked keep bounds (`Pages4.new(..., bounds=True)`):
 `rope_append4` brings those of every page that it writes up to date.
 
+Long bfloat16 portions of heads of 64 and 128 go to the tensor cores' tiles in float16, whose waits are bounded and tell of
+running out by the device's status word (`tensor_core.check_status`).  There a value that is no number makes the whole head's
+result none for the rows that see it; elsewhere only its group's features.
+
 Everything launches on torch's current stream of the tensors' device and may be captured into a CUDA graph; what is
 allocated on the way (partial results of very long contexts, pages laid out anew for long portions) comes from
 torch's pool.  Outputs may not overlap inputs, but where a function says so.  Sums and softmax statistics are
@@ -140,8 +144,10 @@ class Batch:
     so are their positions.  Rows behind the last request's are left alone.
 
     A call that is captured into a graph may be replayed with other numbers on the device, as long as no request brings more rows
-    than the most that the host was told of and the same leading requests bring one; the kernels are shaped by the host's
-    numbers, the results follow the device's."""
+    than the most that the host was told of, the same leading requests bring one and, where a request brings more, no request
+    then holds more tokens than at the capture; the kernels are shaped by the host's numbers, the results follow the device's.
+    `reach`: the longest context that they are shaped for (as long as the host's numbers say, if it is not given); pages
+    beyond it are not picked, only attention to all of them reads them."""
 
     __slots__ = ("positions", "row_request", "row_start", "first_pos", "table", "new_tokens", "held_tokens", "requests",
                  "most_new", "reach", "lead", "device")
@@ -225,7 +231,8 @@ def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional
     pages, in 4 bits.  `cos`, `sin`: float32 [positions, r / 2], the angles of every position; the first r
     features of a head turn, (a, b) -> (a cos - b sin, a sin + b cos), feature i with i + r / 2 or (`neighbours`)
     2 i with 2 i + 1.  None: nothing turns.  Rows whose position is beyond the tables are left out.  No two rows are of one place.
-    `write` False: q alone (the pages hold the rows already)."""
+    `write` False: q alone (the pages hold the rows already).
+    With bounds, every page that the step wrote gets its own anew, from the tokens up to the last that it wrote there."""
     dim, kv = pages.head_dim, pages.kv_heads
     width = (n_heads + 2 * kv) * dim
     if n_heads < 1:
