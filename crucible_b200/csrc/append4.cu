@@ -427,6 +427,7 @@ struct ExpandParams {
     __half* values;
     int* spans;              // [blocks of 64 tokens][kv heads][keys, values]
     float2* factors;         // [requests][kv heads]: what keys and values were divided by
+    uint32_t* seen;          // [requests][block_stride][2]: a bit a token that is there
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
     const __nv_bfloat16* q;
@@ -470,8 +471,8 @@ __device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
 // can hold, from their groups' pairs.
 template <int D>
 __global__ void __launch_bounds__(128) span4_kernel(const ExpandParams p) {
-    cb_pdl_trigger();
     cb_pdl_wait();
+    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin before its own)
     const Laid in = laid_of(p, blockIdx.x);
     const int side = threadIdx.x >> 6, pos = ((int)blockIdx.x - in.before) * 64 + (threadIdx.x & 63);
     int e = C4_LEAST_SPAN;
@@ -507,12 +508,12 @@ __device__ __forceinline__ int2 exponents_of(const ExpandParams& p, const Laid& 
 
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
 // last token; the blocks behind it take some rows' queries each, which go into float16 scaled by a power of two so that a row's
-// largest lies in [2^13, 2^14).  Tokens that no row of the step sees are left out, as zeros.  A value that is no number becomes
+// largest lies in [2^13, 2^14).  Tokens that no row of the step sees are left out, as zeros; of those whose table entry names no page `seen` has no bit.  A value that is no number becomes
 // its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.
 template <int D>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
-    cb_pdl_trigger();
     cb_pdl_wait();
+    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin before its own)
     __shared__ uint32_t bad[64];
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
     const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
@@ -555,8 +556,11 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
         int before = 0;
         for (int r = 0; r < p.n_requests; ++r) {
             const int count = (p.first_pos[r] + p.row_start[r + 1] - p.row_start[r] + 63) >> 6;
-            for (int i = threadIdx.x; i < p.block_stride; i += 256)
-                p.blocks[(size_t)r * p.block_stride + i] = i < count && before + i < p.n_blocks ? before + i : p.n_blocks;
+            for (int i = threadIdx.x; i < p.block_stride; i += 256) {
+                const bool one = i < count && before + i < p.n_blocks;
+                p.blocks[(size_t)r * p.block_stride + i] = one ? before + i : p.n_blocks;
+                if (!one) reinterpret_cast<uint2*>(p.seen)[(size_t)r * p.block_stride + i] = make_uint2(0u, 0u);
+            }
             before += count;
         }
     }
@@ -565,6 +569,7 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     const bool some = block < p.n_blocks && request < p.n_requests;
     const int lo = p.window > 0 ? max(0, in.first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
+    __shared__ int there[64];
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     const int f = eight_of<D>(within);
     const long long side_rows = (long long)p.n_pages * p.kv_heads * p.page_tokens;
@@ -575,6 +580,7 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
         long long at = -1;
         if (some && lane < LANES * PER_WARP && pos < held && pos >= lo)
             at = c4_row(table, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
+        if (within == 0 && lane < LANES * PER_WARP) there[pos - index * 64] = at >= 0;
         if (at >= 0) at += (long long)blockIdx.y * p.page_tokens;
         key[j] = eight_fetched<D>(p.codes, p.scales, at, at >= 0, p.group, within);
         value[j] = eight_fetched<D>(p.codes, p.scales, at + side_rows, at >= 0, p.group, within);
@@ -584,6 +590,10 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     if (some && index == 0 && threadIdx.x == 0)
         p.factors[(size_t)request * p.kv_heads + blockIdx.y] = make_float2(two_to(e.x), two_to(e.y));
     __syncthreads();
+    if (some && index < p.block_stride && blockIdx.y == 0 && threadIdx.x < 64) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, there[threadIdx.x] != 0);
+        if (lane == 0) p.seen[((size_t)request * p.block_stride + index) * 2 + (threadIdx.x >> 5)] = bits;
+    }
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j)
         if (c4_low(value[j].y) != c4_low(value[j].y)) {
@@ -686,14 +696,14 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
-                         int n_requests, int window, void* keys, void* values, int* spans, float* factors, int* blocks,
+                         int n_requests, int window, void* keys, void* values, int* spans, float* factors, uint32_t* seen, int* blocks,
                          int block_stride, int n_blocks, const void* q, long long q_stride, int rows, int most_rows,
                          int n_rep, float scale, void* q_half, float* row_scale, void* stream) {
     if (n_blocks <= 0 || most_rows <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
                             reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans,
-                            reinterpret_cast<float2*>(factors), blocks, block_stride,
+                            reinterpret_cast<float2*>(factors), seen, blocks, block_stride,
                             n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, rows,
                             n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), row_scale};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -90,6 +90,7 @@ struct TcAttnParams {
     int* status;
     const float* row_scale;  // GATE_SCALED: [rows][n_heads], of the scores, log2(e) among it
     const float2* factors;   // GATE_SCALED: [requests][n_kv_heads], of the scores and of the results
+    const uint2* seen;       // GATE_SCALED: [requests][table_stride], which of a page's 64 keys are there
 };
 
 // GATE: the results' gate, fixed when it is compiled: the epilogue runs once per block and its instructions
@@ -363,8 +364,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             armed = ++item;
             return true;
         };
+        if (GATE == GATE_SCALED) cb_pdl_wait();        // (this form's table is of the kernel before)
         int pg0 = lookup(0), pg1 = lookup(1), pg2 = lookup(2);
-        cb_pdl_wait();
+        if (GATE != GATE_SCALED) cb_pdl_wait();
         cb_pdl_trigger();     // the block holds its tensor memory: a successor that asks for some queues behind it
         bool ok = n_tiles > 0;
         if (ok && p.q_boxes && lane == 0) {
@@ -566,7 +568,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 gate_f = sigmoid(__bfloat162float(p.gate[(size_t)tok * p.gate_stride + head]));
             if (GATE == GATE_SCALED) {
                 const float2 both = p.factors[(size_t)req * gridDim.x + kv_head];
-                scale_log2 = p.row_scale[(size_t)tok * p.n_heads + head] * both.x;
+                // (never zero, which minus infinity may not meet: scores that small are all alike)
+                scale_log2 = fmaxf(p.row_scale[(size_t)tok * p.n_heads + head] * both.x, 1e-37f);
                 out_scale = both.y;
             }
         }
@@ -598,6 +601,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         for (int j = group; j < n_tiles; j += GROUPS) {
             const int key0 = tile_key0(j);
             const int b = j % S_BUFS;
+            uint2 there[2] = {make_uint2(~0u, ~0u), make_uint2(~0u, ~0u)};
+            if (GATE == GATE_SCALED)
+                for (int h = 0; h < 2; ++h)
+                    there[h] = p.seen[(size_t)req * p.table_stride + min((key0 >> 6) + h, p.table_stride - 1)];
             ok = wait_all(&s.s_full[b], (j / S_BUFS) & 1);
             if (!ok) break;
             tc::tc_fence_after_sync();
@@ -607,7 +614,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             // others the masked scores go back where they came from.
             const int last = pos - key0, first = lo - key0;
             const int kept = p.keep_first - key0;     // keys before this one are kept first tokens (<= 0: none here)
-            const bool inside = __all_sync(0xffffffffu, last >= KEYS - 1 && first <= 0);
+            const bool inside = __all_sync(0xffffffffu, last >= KEYS - 1 && first <= 0)
+                && (GATE != GATE_SCALED || (there[0].x & there[0].y & there[1].x & there[1].y) == ~0u);
             float mc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             // The scores are read twice, 64 at a time in a loop that is not unrolled: the code of
             // both passes over all 128 comes from memory at a block's first tile, and the registers
@@ -622,7 +630,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int k0 = 64 * h + 32 * c;
-                        const uint32_t seen = bits_below(last + 1 - k0) & (~bits_below(first - k0) | bits_below(kept - k0));
+                        uint32_t seen = bits_below(last + 1 - k0) & (~bits_below(first - k0) | bits_below(kept - k0));
+                        if (GATE == GATE_SCALED) seen &= c ? (h ? there[1].y : there[0].y) : (h ? there[1].x : there[0].x);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (!(seen >> i & 1u)) sv[c][i] = __float_as_uint(-INFINITY);
@@ -865,7 +874,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
                              const int* req_first_pos, const int* block_table, int table_stride, int n_requests,
                              int max_new_tokens, int n_heads, int n_kv_heads, int head_dim, int page_tokens, float scale,
                              int window, int chunked, int keep_first, float out_scale, const float* sinks, const void* gate,
-                             int gate_stride, int gate_per_head, const float* row_scale, const float* factors, int lead, int value_cols, int* status,
+                             int gate_stride, int gate_per_head, const float* row_scale, const float* factors, const uint32_t* seen, int lead, int value_cols, int* status,
                              void* stream) {
     if (n_requests <= 0 || max_new_tokens <= 0) return 0;
     if (keep_first < 0 || !(scale > 0.f)) return CB_ERR_UNSUPPORTED;
@@ -929,6 +938,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     p.status = status;
     p.row_scale = row_scale;
     p.factors = reinterpret_cast<const float2*>(factors);
+    p.seen = reinterpret_cast<const uint2*>(seen);
     const int q_tiles = (max_new_tokens * n_rep + p.tile_rows - 1) / p.tile_rows;
     if (n_requests > 65535 || q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     // (single tokens of more than a tile of query heads keep ranks like a portion's)
@@ -956,19 +966,19 @@ CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_r
     return attention_tcgen05(qkv, qkv_stride, n_rows, out, out_stride, k_cache, v_cache, n_pages, req_row_start, req_first_pos,
                              block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
                              scale, window, chunked, keep_first, out_scale, sinks, gate, gate_stride, gate_per_head, nullptr,
-                             nullptr, lead, value_cols, status, stream);
+                             nullptr, nullptr, lead, value_cols, status, stream);
 }
 
 // The same over queries, keys and values in float16 (heads of 64 and 128): factors for the scores of each row and head, log2(e)
 // among them (row_scale [n_rows][n_heads]), and for the scores and the results of each request and kv head (factors
-// [n_requests][n_kv_heads][2]).
-CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, const float* factors, int n_rows,
-                                        void* out, int out_stride, const void* keys, const void* values, int n_pages,
+// [n_requests][n_kv_heads][2]); pages of 64 tokens, and a bit for every one that is there (seen [n_requests][table_stride][2]).
+CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, const float* factors,
+                                        const uint32_t* seen, int n_rows, void* out, int out_stride, const void* keys, const void* values, int n_pages,
                                         const int* req_row_start, const int* req_first_pos, const int* block_table,
                                         int table_stride, int n_requests, int max_new_tokens, int n_heads, int n_kv_heads,
-                                        int head_dim, int page_tokens, int window, int* status, void* stream) {
+                                        int head_dim, int window, int* status, void* stream) {
     if (head_dim > 128) return CB_ERR_UNSUPPORTED;
     return attention_tcgen05(q, q_stride, n_rows, out, out_stride, keys, values, n_pages, req_row_start, req_first_pos,
-                             block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
-                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, factors, 0, 0, status, stream);
+                             block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, 64,
+                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, factors, seen, 0, 0, status, stream);
 }

@@ -14,7 +14,8 @@ prompts; `pick_pages4` chooses for every row and kv head the pages whose bounds 
 `rope_append4` brings those of every page that it writes up to date.
 
 Long bfloat16 portions of heads of 64 and 128 go to the tensor cores' tiles in float16, whose waits are bounded and tell of
-running out by the device's status word (`tensor_core.check_status`).  There a value that is no number makes the whole head's
+running out by the device's status word (`tensor_core.check_status`; a graph that is captured before there is one walks
+instead).  There a value that is no number makes the whole head's
 result none for the rows that see it; elsewhere only its group's features.
 
 Everything launches on torch's current stream of the tensors' device and may be captured into a CUDA graph; what is
@@ -31,7 +32,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import KernelError, _check, _code, _need_cuda, build, tensor_core
-from .quantized import _at, _one_device
+from .quantized import _at, _one_device, _status
 
 build.register_module("append4", ["common.cuh", "cache4.cuh"])
 build.register_module("pick4", ["common.cuh", "cache4.cuh"])
@@ -337,7 +338,7 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     _same_device("attention4", batch, pages, q, out, picks)
     if picks is not None:
         _walk(q, out, n_heads, scale, batch, pages, None, picks, 0, 0)
-    if behind < rows:
+    if behind < min(rows, batch.requests):
         lead = max(behind, batch.lead)
         if lead < batch.requests and _laid_out(q, out, n_heads, batch, pages, window, behind, lead):
             if behind < lead:
@@ -456,7 +457,7 @@ def _laid_out(q, out, n_heads, batch, pages, window, behind, first) -> bool:
     new, held = batch.new_tokens[first:], batch.held_tokens[first:]
     n_rep = n_heads // kv
     if (q.dtype is not _BF16 or dim > 128 or q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16
-            or max(new) * n_rep < 64):
+            or max(new) * n_rep < 64 or not _status(pages.device)):
         return False
     if LAID_OUT is not None:
         return LAID_OUT
@@ -481,8 +482,8 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
     counts = [-(-(h + n) // 64) for h, n in zip(held, new)]
     n_blocks, stride, requests, rows = sum(counts), max(counts), len(counts), batch.positions.shape[0]
     both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
-    spans = torch.empty(2 * n_blocks * kv + requests * stride, dtype=_I32, device=q.device)
-    blocks = spans[2 * n_blocks * kv:]
+    spans = torch.empty(2 * n_blocks * kv + 3 * requests * stride, dtype=_I32, device=q.device)
+    seen, blocks = spans[2 * n_blocks * kv:], spans[2 * (n_blocks * kv + requests * stride):]
     q_half = torch.empty(rows, n_heads * dim, dtype=torch.float16, device=q.device)
     factors = torch.empty(2 * requests * kv + rows * n_heads, dtype=_F32, device=q.device)
     row_scale = factors[2 * requests * kv:]
@@ -490,12 +491,12 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
     _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.table.shape[1],
                batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
-               factors.data_ptr(), blocks.data_ptr(), stride, n_blocks, q.data_ptr(), q.stride(0), rows, sum(new),
+               factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks, q.data_ptr(), q.stride(0), rows, sum(new),
                n_heads // kv, scale, q_half.data_ptr(), row_scale.data_ptr()), "pages laid out")
     code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q_half.data_ptr(), n_heads * dim,
-               row_scale.data_ptr(), factors.data_ptr(), rows, out.data_ptr(), out.stride(0), both[0].data_ptr(),
-               both[1].data_ptr(), n_blocks + 1, starts, places, blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, 64,
-               window or 0, tensor_core.status_word(q.device).data_ptr())
+               row_scale.data_ptr(), factors.data_ptr(), seen.data_ptr(), rows, out.data_ptr(), out.stride(0), both[0].data_ptr(),
+               both[1].data_ptr(), n_blocks + 1, starts, places, blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim,
+               window or 0, _status(pages.device))
     if code == build.UNSUPPORTED:
         return False
     _check(code, "attention4 (tiles)")

@@ -207,7 +207,8 @@ def test_attention_of_few_rows(dim, group, n_rep, kv_heads, page, requests, dtyp
     (64, 64, 3, 2, 16, [(0, 70)], None), (64, 32, 1, 3, 16, [(5, 100), (0, 33)], None), (128, 64, 4, 1, 16, [(200, 40)], None),
     (128, 128, 2, 2, 24, [(30, 65), (129, 64), (0, 130)], None), (128, 32, 7, 1, 7, [(90, 31)], None),
     (64, 64, 4, 2, 64, [(40, 1), (17, 1), (0, 200), (300, 20)], None), (128, 64, 4, 1, 16, [(200, 1), (250, 90), (0, 64)], 100),
-    (64, 64, 2, 2, 16, [(500, 40)], 17)])
+    (64, 64, 2, 2, 16, [(500, 40)], 17), (64, 64, 32, 1, 16, [(70, 5), (0, 9)], None), (128, 128, 5, 1, 8, [(3, 140)], None),
+    (64, 32, 1, 3, 16, [(0, 64), (1000, 70)], None), (128, 64, 130, 1, 16, [(10, 3)], None)])
 def test_attention_of_portions_that_are_laid_out(dim, group, n_rep, kv_heads, page, requests, window, monkeypatch):
     """Long portions, decoded tokens at the step's head walked beside them; what the window has passed is not read."""
     from crucible_b200.ops import cache4
@@ -230,7 +231,7 @@ def test_attention_of_portions_that_are_laid_out(dim, group, n_rep, kv_heads, pa
 
 
 @pytest.mark.parametrize("size,stretch,scale", [(1e-7, 1.0, 1.0), (1e8, 1.0, 1e-9), (1.0, 1e-15, 1e14), (1.0, 1e15, 1e-16),
-                                                (1e-20, 1e20, 0.1), (1e25, 1e-22, 1e-3)])
+                                                (1e-20, 1e20, 0.1), (1e25, 1e-22, 1e-3), (1e-20, 1e-22, 0.1)])
 def test_sizes_in_portions_that_are_laid_out(size, stretch, scale, monkeypatch):
     """Keys and queries whose numbers float16 would not hold as they are."""
     from crucible_b200.ops import cache4
@@ -241,6 +242,114 @@ def test_sizes_in_portions_that_are_laid_out(size, stretch, scale, monkeypatch):
     q[0, :64] = 0
     want, most = case.attention(q, scale, spread=spread)
     cc.assert_attention_laid_out(_attend(case, q, scale), want, most, spread[0])
+
+
+@pytest.mark.parametrize("window", [None, 70])
+def test_places_without_a_page_in_portions_that_are_laid_out(window, monkeypatch):
+    """What the table does not name is not seen, here too; a row that sees nothing is zero."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    case = cc.Case([(300, 40), (0, 150), (0, 33)], dim=64, group=64, n_rep=4, kv_heads=2, page=16, seed=31)
+    case.table[0, 3:7] = torch.tensor([-1, case.n_pages, -(1 << 31), 1 << 30], device=DEV)
+    case.table[0, 17] = -1
+    case.table[1, :2] = -1
+    case.table[1, 8] = -1
+    q, spread = case.queries(), []
+    want, most = case.attention(q, 0.125, window=window, spread=spread)
+    got = _attend(case, q, 0.125, window=window)
+    assert (got[40:72] == 0).all()
+    cc.assert_attention_laid_out(got, want, most, spread[0])
+    case.table = case.table[:, :9].contiguous()                    # (positions behind 143 are of no page then)
+    case.stride, case.batch = 9, None
+    case.batch = case.make_batch()
+    spread.clear()
+    want, most = case.attention(q, 0.125, window=window, spread=spread)
+    cc.assert_attention_laid_out(_attend(case, q, 0.125, window=window), want, most, spread[0])
+
+
+def test_portions_laid_out_of_a_captured_step(monkeypatch):
+    """Replayed with other queries, other places and fewer tokens; and captured where no wait that runs out could be told."""
+    from crucible_b200.ops import cache4, tensor_core
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    case = cc.Case([(5, 1), (120, 40), (0, 90)], dim=128, group=64, n_rep=3, kv_heads=1, seed=33)
+    q = case.queries()
+    outs = [torch.empty_like(q) for _ in range(3)]
+
+    def step(out):
+        cache4.attention4(q, out, case.heads, 0.1, case.batch, case.pages)
+    step(outs[0])
+    graphs = [torch.cuda.CUDAGraph() for _ in range(3)]
+    for i, (graph, out) in enumerate(zip(graphs, outs)):
+        if i == 2:
+            monkeypatch.setattr(tensor_core, "_status", {})
+        with torch.cuda.graph(graph):
+            step(out)
+    for requests in ([(5, 1), (120, 40), (0, 90)], [(4, 1), (60, 30), (3, 80)], [(0, 1), (0, 1), (1, 1)]):
+        case.requests = requests
+        starts = [0]
+        for _, n in requests:
+            starts.append(starts[-1] + n)
+        positions = [h + i for h, n in requests for i in range(n)]
+        case.rows = len(positions)
+        case.positions[:case.rows] = torch.tensor(positions, device=DEV, dtype=torch.int32)
+        case.row_request.fill_(-1)
+        case.row_request[:case.rows] = torch.tensor([r for r, (_, n) in enumerate(requests) for _ in range(n)], device=DEV)
+        case.row_start.copy_(torch.tensor(starts))
+        case.first_pos.copy_(torch.tensor([h for h, _ in requests]))
+        q.copy_(torch.randn_like(q))
+        for out in outs:
+            out.fill_(7)
+        for graph in graphs:                                       # (two that share nothing, one behind the other)
+            graph.replay()
+        spread = []
+        want, most = case.attention(q, 0.1, spread=spread)
+        for out in outs:
+            cc.assert_attention_laid_out(out[:case.rows], want, most, spread[0]) if out is not outs[2] else \
+                cc.assert_attention(out[:case.rows], want, most, BF16)
+            assert (out[case.rows:] == 7).all()
+
+
+def test_portions_laid_out_on_two_streams_at_once(monkeypatch):
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    cases = [cc.Case([(100 * i, 200)], dim=64, group=32, n_rep=2, kv_heads=4, seed=35 + i) for i in range(2)]
+    qs = [c.queries() for c in cases]
+    outs = [[torch.empty_like(q) for _ in range(10)] for q in qs]
+    streams = [torch.cuda.Stream(DEV) for _ in cases]
+    torch.cuda.synchronize()
+    for n in range(10):
+        for c, q, out, stream in zip(cases, qs, outs, streams):
+            with torch.cuda.stream(stream):
+                cache4.attention4(q, out[n], c.heads, 0.125, c.batch, c.pages)
+    torch.cuda.synchronize()
+    for c, q, out in zip(cases, qs, outs):
+        spread = []
+        want, most = c.attention(q, 0.125, spread=spread)
+        cc.assert_attention_laid_out(out[0], want, most, spread[0])
+        assert all(torch.equal(o, out[0]) for o in out[1:])
+
+
+def test_picks_of_a_padded_step():
+    """Rows behind the last request's, whether there are picks of these or not: left as they are."""
+    from crucible_b200.ops import cache4
+    case = cc.Case([(200, 1), (90, 1), (140, 1)], dim=64, group=64, page=16, bounds=True, seed=37)
+    _true_bounds(case)
+    rows = case.rows
+    q = case.queries()
+    by_definition = _picks_by_definition(case, q, 5, 1, 2)
+    case.positions = torch.cat((case.positions, torch.zeros(3, dtype=torch.int32, device=DEV)))
+    case.row_request = torch.cat((case.row_request, torch.full((3,), -1, dtype=torch.int32, device=DEV)))
+    case.batch = case.make_batch()
+    q = torch.cat((q, torch.full_like(q, float("nan"))))
+    for n in (rows, rows + 3):
+        picks = torch.full((n, case.kv_heads, 5), 99, dtype=torch.int32, device=DEV)
+        cache4.pick_pages4(q, case.heads, case.batch, case.pages, picks)
+        assert torch.equal(picks[:rows], by_definition) and (picks[rows:] == 99).all()
+        want, most = case.attention(q, 0.125, picks=picks.cpu())
+        out = torch.full_like(q, 7)
+        cache4.attention4(q, out, case.heads, 0.125, case.batch, case.pages, picks=picks)
+        cc.assert_attention(out[:rows], want[:rows], most[:rows], BF16)
+        assert (out[rows:] == 7).all()
 
 
 @pytest.mark.parametrize("small", [0.0, 1e-12, 1e-7, 1e-3])
