@@ -625,3 +625,41 @@ def test_one_captured_step_replayed_behind_longer_contexts():
             for got, chosen in ((dense, None), (sparse, picks.cpu())):
                 want, most = case.attention(q, 0.125, picks=chosen)
                 cc.assert_attention(got, want, most, BF16)
+
+
+def test_a_pool_whose_offsets_pass_32_bits(monkeypatch):
+    """The same pages at the end of a pool of more than 2^32 bytes a side give the same, to the bit."""
+    from crucible_b200.ops import cache4
+    dim, kv, page = 128, 8, 64
+    requests = [(200, 1), (70, 1), (100, 90)]
+    far = (1 << 32) // (kv * page * dim // 2) + 50
+    cos, sin = cc.tables(300, dim // 2, DEV)
+    got = []
+    for offset in (0, far):
+        case = cc.Case(requests, dim=dim, group=64, n_rep=2, kv_heads=kv, page=page, bounds=True, seed=41)
+        if offset:
+            small = case.pages
+            n = offset + small.n_pages
+            case.pages = cache4.Pages4(*(torch.empty(2, n, *t.shape[2:], dtype=t.dtype, device=DEV) for t in (small.codes, small.scales)),
+                                       *(torch.empty(n, *t.shape[1:], dtype=t.dtype, device=DEV) for t in (small.bounds, small.bound_scales)))
+            case.pages.codes[:, offset:], case.pages.scales[:, offset:] = small.codes, small.scales
+            case.pages.bounds[offset:], case.pages.bound_scales[offset:] = small.bounds, small.bound_scales
+            case.table += offset
+            case.batch = case.make_batch()
+        qkv = case.normal(case.rows, (case.heads + 2 * kv) * dim).to(BF16)
+        q = torch.empty(case.rows, case.heads * dim, dtype=BF16, device=DEV)
+        cache4.rope_append4(qkv, q, case.heads, cos, sin, case.batch, case.pages)
+        picks = torch.empty(case.rows, kv, 3, dtype=torch.int32, device=DEV)
+        cache4.pick_pages4(q, case.heads, case.batch, case.pages, picks)
+        outs = [torch.empty_like(q) for _ in range(3)]
+        cache4.attention4(q, outs[0], case.heads, 0.09, case.batch, case.pages, picks=picks)
+        for laid_out, out in zip((False, True), outs[1:]):
+            monkeypatch.setattr(cache4, "LAID_OUT", laid_out)
+            cache4.attention4(q, out, case.heads, 0.09, case.batch, case.pages)
+        p = case.pages
+        got.append((q, picks, *outs, p.codes[:, offset:].clone(), p.scales[:, offset:].clone(), p.bounds[offset:].clone(),
+                    p.bound_scales[offset:].clone()))
+        del p
+        case.pages = None
+    for small, large in zip(*got):
+        assert torch.equal(small, large)
