@@ -14,8 +14,7 @@
 //             pages of 64: 5.5 us, a thread's chain through place, codes and pairs, then a block's largest.
 //   values4   the whole pool as float32 or bfloat16 rows.
 //   span4     before expand4: how large the numbers of every 64 tokens can be.
-//   expand4   the pages of some requests as rows in pages of 64 tokens, for attention over many rows, and the requests'
-//             queries, all in float16.  2,048 tokens of 8 heads of 128 under 32 query heads: both 17 us (span4 3), 42 MB
+//   expand4   the pages of some requests as float16 rows in pages of 64 tokens, for attention over many rows.  2,048 tokens of 8 heads of 128 under 32 query heads: both 17 us (span4 3), 42 MB
 //             of which 32 are queries; everything a block needs is asked for before it works on any of it.
 #define CB_PDL_BIT 6      // with the other quantised operators
 #include "cache4.cuh"
@@ -430,12 +429,6 @@ struct ExpandParams {
     uint32_t* seen;          // [requests][block_stride][2]: a bit a token that is there
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
-    const __nv_bfloat16* q;
-    long long q_stride;
-    int rows, n_rep;
-    float scale_log2;
-    __half* q_half;          // [rows][heads][D]
-    float* row_scale;        // [rows][heads]: log2(e) times the scale over what the queries were multiplied by
 };
 
 // Which request a block of 64 tokens is of, from how many blocks the requests before it have.
@@ -455,9 +448,6 @@ __device__ __forceinline__ Laid laid_of(const ExpandParams& p, int block) {
     return at;
 }
 
-// Rows whose queries a block takes: 64 of a kv head, or one row's.
-__host__ __device__ __forceinline__ int q_rows(int n_rep) { return n_rep < 64 ? 64 / n_rep : 1; }
-
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 __device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
@@ -472,7 +462,7 @@ __device__ __forceinline__ void store_halves(__half* dst, const float (&v)[8]) {
 template <int D>
 __global__ void __launch_bounds__(128) span4_kernel(const ExpandParams p) {
     cb_pdl_wait();
-    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin before its own)
+    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin, and queries, before its own)
     const Laid in = laid_of(p, blockIdx.x);
     const int side = threadIdx.x >> 6, pos = ((int)blockIdx.x - in.before) * 64 + (threadIdx.x & 63);
     int e = C4_LEAST_SPAN;
@@ -507,51 +497,16 @@ __device__ __forceinline__ int2 exponents_of(const ExpandParams& p, const Laid& 
 }
 
 // A block of threads a block of 64 tokens and kv head; block n_blocks is of zeros, for what the table has behind a request's
-// last token; the blocks behind it take some rows' queries each, which go into float16 scaled by a power of two so that a row's
-// largest lies in [2^13, 2^14).  Tokens that no row of the step sees are left out, as zeros; of those whose table entry names no page `seen` has no bit.  A value that is no number becomes
-// its key's: attention by tiles multiplies the values of masked keys by zero, but does not take their scores.
+// last token.  Tokens that no row of the step sees are left out, as zeros; of those whose table entry names no page `seen`
+// has no bit.  A value that is no number becomes its key's: attention by tiles multiplies the values of masked keys by
+// zero, but does not take their scores.
 template <int D>
 __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     cb_pdl_wait();
-    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin before its own)
+    cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin, and queries, before its own)
     __shared__ uint32_t bad[64];
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
     const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
-    if (block > p.n_blocks) {
-        constexpr int WIDE = 4;
-        const int heads = p.kv_heads * p.n_rep;
-        const int each = q_rows(p.n_rep), from = p.row_start[0] + (block - p.n_blocks - 1) * each;
-        const int rows = min(min(p.row_start[p.n_requests], p.rows) - from, each);
-        for (int i0 = (threadIdx.x >> 5) * PER_WARP; i0 < rows * p.n_rep; i0 += WIDE * 8 * PER_WARP) {      // (whole warps: shuffles)
-            float v[WIDE][8];
-#pragma unroll
-            for (int u = 0; u < WIDE; ++u) {
-                const int j = i0 + u * 8 * PER_WARP + lane / LANES;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-                if (j < rows * p.n_rep && lane < LANES * PER_WARP)
-                    load_eight<__nv_bfloat16, true>(p.q + (size_t)(from + j / p.n_rep) * p.q_stride
-                                                    + (size_t)(blockIdx.y * p.n_rep + j % p.n_rep) * D + within * 8, v[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < WIDE; ++u) {
-                const int j = i0 + u * 8 * PER_WARP + lane / LANES;
-                float most = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[u][e]));
-#pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int up = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
-                if (j >= rows * p.n_rep || lane >= LANES * PER_WARP) continue;
-                const size_t at = (size_t)(from + j / p.n_rep) * heads + blockIdx.y * p.n_rep + j % p.n_rep;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u][e] *= two_to(up);
-                store_halves(p.q_half + at * D + within * 8, v[u]);
-                if (within == 0) p.row_scale[at] = p.scale_log2 * two_to(-up);
-            }
-        }
-        return;
-    }
     if (block == 0 && blockIdx.y == 0) {
         int before = 0;
         for (int r = 0; r < p.n_requests; ++r) {
@@ -696,19 +651,16 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
-                         int n_requests, int window, void* keys, void* values, int* spans, float* factors, uint32_t* seen, int* blocks,
-                         int block_stride, int n_blocks, const void* q, long long q_stride, int rows, int most_rows,
-                         int n_rep, float scale, void* q_half, float* row_scale, void* stream) {
-    if (n_blocks <= 0 || most_rows <= 0) return 0;
+                         int n_requests, int window, void* keys, void* values, int* spans, float* factors, uint32_t* seen,
+                         int* blocks, int block_stride, int n_blocks, void* stream) {
+    if (n_blocks <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
                             reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans,
-                            reinterpret_cast<float2*>(factors), seen, blocks, block_stride,
-                            n_blocks, reinterpret_cast<const __nv_bfloat16*>(q), q_stride, rows,
-                            n_rep, scale * 1.4426950408889634f, reinterpret_cast<__half*>(q_half), row_scale};
+                            reinterpret_cast<float2*>(factors), seen, blocks, block_stride, n_blocks};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const dim3 spans_grid((unsigned)n_blocks, (unsigned)kv_heads);
-    const dim3 grid((unsigned)(n_blocks + 1 + (most_rows + q_rows(n_rep) - 1) / q_rows(n_rep)), (unsigned)kv_heads);
+    const dim3 grid((unsigned)n_blocks + 1, (unsigned)kv_heads);
     if (head_dim == 64) {
         cb_launch(span4_kernel<64>, spans_grid, dim3(128), 0, s, p);
         cb_launch(expand4_kernel<64>, grid, dim3(256), 0, s, p);

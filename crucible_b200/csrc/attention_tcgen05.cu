@@ -88,7 +88,6 @@ struct TcAttnParams {
     int n_pages;             // of the pool
     int runs;                // 1: the 4-D maps may be used for tiles whose pages are consecutive
     int* status;
-    const float* row_scale;  // GATE_SCALED: [rows][n_heads], of the scores, log2(e) among it
     const float2* factors;   // GATE_SCALED: [requests][n_kv_heads], of the scores and of the results
     const uint2* seen;       // GATE_SCALED: [requests][table_stride], which of a page's 64 keys are there
 };
@@ -96,7 +95,7 @@ struct TcAttnParams {
 // GATE: the results' gate, fixed when it is compiled: the epilogue runs once per block and its instructions
 // come from memory (12 heads of 64 without a gate, a 2,048-token prompt: 32 us; with the code of the gate of a
 // logit a result beside it 0.3 us more, of both gates 1.4).
-// GATE_SCALED: no gate, queries, keys, values and P in float16, factors of its own for a row's scores and results
+// GATE_SCALED: no gate, keys, values and P in float16, queries put into it here, factors of its own for a row's scores and results
 // (a 2,048-token prompt, 32 heads of 128 on 8: 44.5 us, 0.77 PFLOP/s, as in bfloat16).
 enum Gate { GATE_NONE = 0, GATE_RESULT = 1, GATE_HEAD = 2, GATE_SCALED = 3 };
 
@@ -138,6 +137,7 @@ struct Storage {
     uint64_t empty[RELEASES];
     uint64_t q_full, gate_full, o_done;
     uint64_t s_full[S_BUFS], p_half[S_BUFS], p_full[S_BUFS], pv_done[2], m_full[2];
+    float row_scale[ROWS];                                  // GATE_SCALED: a row's factor of its scores, log2(e) among it
     float m_row[2][ROWS];                                   // shared: a row's reference as of a tile (tile j: j & 1)
     uint32_t tmem_base;
     int abort_flag;
@@ -552,6 +552,43 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const int pos = real ? first_pos + row / n_rep : (1 << 30);
         const int lo = real ? first_key(p, pos) : 0;
         const uint32_t lane_bits = (uint32_t)(quarter * 32) << 16;
+        if constexpr (GATE == GATE_SCALED) {
+            // The queries by hand, into float16 times 2^(13 - e), e the exponent of a row's largest; 8 NH lanes a row.
+            // (Before the wait: the kernels that lay keys and values out start this one once what was before them has
+            // ended, and they do not write queries.  Past L1, which may hold an earlier step's.)
+            constexpr int PIECES = ROWS * 8 * NH / (128 * GROUPS);
+            uint4 raw[PIECES];
+#pragma unroll
+            for (int u = 0; u < PIECES; ++u) {
+                const int i = threadIdx.x - 64 + u * 128 * GROUPS, at = first_row + i / (8 * NH);
+                raw[u] = make_uint4(0, 0, 0, 0);
+                if (n_tiles > 0 && at < n_rows) {
+                    const int tok = row_base + at / n_rep, head = kv_head * n_rep + at % n_rep;
+                    raw[u] = __ldcg(reinterpret_cast<const uint4*>(p.qkv + (size_t)tok * p.qkv_stride + (size_t)head * HD + i % (8 * NH) * 8));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < PIECES; ++u) {
+                const int i = threadIdx.x - 64 + u * 128 * GROUPS, rr = i / (8 * NH), c = i % (8 * NH);
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                float most = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+#pragma unroll
+                for (int o = 1; o < 8 * NH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int up = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+                const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+                uint32_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = pack_f16(__uint_as_float(w[e] << 16) * by, __uint_as_float(w[e] & 0xffff0000u) * by);
+                *reinterpret_cast<uint4*>(s.q[c >> 3] + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                if (c == 0) s.row_scale[rr] = p.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s.q_full);
+        }
         cb_pdl_wait();
         // what the row needs at its end, asked for now
         __nv_bfloat16* dst = nullptr;
@@ -568,12 +605,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 gate_f = sigmoid(__bfloat162float(p.gate[(size_t)tok * p.gate_stride + head]));
             if (GATE == GATE_SCALED) {
                 const float2 both = p.factors[(size_t)req * gridDim.x + kv_head];
-                // (never zero, which minus infinity may not meet: scores that small are all alike)
-                scale_log2 = fmaxf(p.row_scale[(size_t)tok * p.n_heads + head] * both.x, 1e-37f);
+                scale_log2 = both.x;
                 out_scale = both.y;
             }
         }
-        if (!p.q_boxes && n_tiles > 0) {
+        if (GATE != GATE_SCALED && !p.q_boxes && n_tiles > 0) {
             // group sizes whose tiles would leave much of the 128 rows empty: the rows by hand,
             // 16-byte pieces into the 128-byte swizzle
             for (int i = threadIdx.x - 64; i < ROWS * 8 * NH; i += 128 * GROUPS) {
@@ -597,8 +633,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (!got && !*abort_flag) tc::give_up(abort_flag, p.status, tc::ST_EPILOGUE_TIMEOUT);
             return __all_sync(0xffffffffu, got);
         };
+        if (GATE == GATE_SCALED && n_tiles > 0) {
+            ok = wait_all(&s.q_full, 0);
+            // (never zero, which minus infinity may not meet: scores that small are all alike)
+            scale_log2 = fmaxf(s.row_scale[r] * scale_log2, 1e-37f);
+        }
         const uint64_t scale2 = pair_of(scale_log2, scale_log2);
-        for (int j = group; j < n_tiles; j += GROUPS) {
+        for (int j = ok ? group : n_tiles; j < n_tiles; j += GROUPS) {
             const int key0 = tile_key0(j);
             const int b = j % S_BUFS;
             uint2 there[2] = {make_uint2(~0u, ~0u), make_uint2(~0u, ~0u)};
@@ -874,7 +915,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
                              const int* req_first_pos, const int* block_table, int table_stride, int n_requests,
                              int max_new_tokens, int n_heads, int n_kv_heads, int head_dim, int page_tokens, float scale,
                              int window, int chunked, int keep_first, float out_scale, const float* sinks, const void* gate,
-                             int gate_stride, int gate_per_head, const float* row_scale, const float* factors, const uint32_t* seen, int lead, int value_cols, int* status,
+                             int gate_stride, int gate_per_head, const float* factors, const uint32_t* seen, int lead, int value_cols, int* status,
                              void* stream) {
     if (n_requests <= 0 || max_new_tokens <= 0) return 0;
     if (keep_first < 0 || !(scale > 0.f)) return CB_ERR_UNSUPPORTED;
@@ -901,7 +942,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     const int n_rep = n_heads / n_kv_heads;
     TcAttnParams p;
     p.tile_rows = n_rep <= ROWS ? ROWS / n_rep * n_rep : 0;
-    p.q_boxes = p.tile_rows >= ROWS - ROWS / 8;
+    p.q_boxes = factors == nullptr && p.tile_rows >= ROWS - ROWS / 8;
     if (!p.q_boxes) p.tile_rows = ROWS;
     maps[4] = maps[5] = mk;
     if (p.q_boxes) {
@@ -936,7 +977,6 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     p.gate_stride = gate_stride;
     p.out_scale = out_scale;
     p.status = status;
-    p.row_scale = row_scale;
     p.factors = reinterpret_cast<const float2*>(factors);
     p.seen = reinterpret_cast<const uint2*>(seen);
     const int q_tiles = (max_new_tokens * n_rep + p.tile_rows - 1) / p.tile_rows;
@@ -947,7 +987,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     p.lead_ranks = (p.lead + portions - 1) / portions;
     if (p.lead_ranks + q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     const dim3 grid(n_kv_heads, portions, p.lead_ranks + q_tiles);
-    const int form = row_scale != nullptr ? GATE_SCALED : gate == nullptr ? GATE_NONE : gate_per_head ? GATE_HEAD : GATE_RESULT;
+    const int form = factors != nullptr ? GATE_SCALED : gate == nullptr ? GATE_NONE : gate_per_head ? GATE_HEAD : GATE_RESULT;
     if (head_dim == 64) return launch_as<64>(form, grid, (cudaStream_t)stream, maps, p);
     if (head_dim == 256 && value_cols > 0 && value_cols <= 192 && form == GATE_NONE)
         return launch_gate<256, GATE_NONE, true>(grid, (cudaStream_t)stream, maps, p);
@@ -966,19 +1006,19 @@ CB_EXPORT int cb_attention_tcgen05_kept(const void* qkv, int qkv_stride, int n_r
     return attention_tcgen05(qkv, qkv_stride, n_rows, out, out_stride, k_cache, v_cache, n_pages, req_row_start, req_first_pos,
                              block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, page_tokens,
                              scale, window, chunked, keep_first, out_scale, sinks, gate, gate_stride, gate_per_head, nullptr,
-                             nullptr, nullptr, lead, value_cols, status, stream);
+                             nullptr, lead, value_cols, status, stream);
 }
 
-// The same over queries, keys and values in float16 (heads of 64 and 128): factors for the scores of each row and head, log2(e)
-// among them (row_scale [n_rows][n_heads]), and for the scores and the results of each request and kv head (factors
-// [n_requests][n_kv_heads][2]); pages of 64 tokens, and a bit for every one that is there (seen [n_requests][table_stride][2]).
-CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, const float* row_scale, const float* factors,
-                                        const uint32_t* seen, int n_rows, void* out, int out_stride, const void* keys, const void* values, int n_pages,
-                                        const int* req_row_start, const int* req_first_pos, const int* block_table,
-                                        int table_stride, int n_requests, int max_new_tokens, int n_heads, int n_kv_heads,
-                                        int head_dim, int window, int* status, void* stream) {
-    if (head_dim > 128) return CB_ERR_UNSUPPORTED;
+// The same over keys and values in float16 (heads of 64 and 128, pages of 64 tokens): factors for the scores and the results of
+// each request and kv head (factors [n_requests][n_kv_heads][2]), and a bit for every token of a page that is there
+// (seen [n_requests][table_stride][2]).
+CB_EXPORT int cb_attention_tcgen05_half(const void* q, int q_stride, int n_rows, void* out, int out_stride, const void* keys,
+                                        const void* values, int n_pages, const int* req_row_start, const int* req_first_pos,
+                                        const int* block_table, int table_stride, int n_requests, int max_new_tokens,
+                                        int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                        const float* factors, const uint32_t* seen, int* status, void* stream) {
+    if (head_dim > 128 || factors == nullptr) return CB_ERR_UNSUPPORTED;
     return attention_tcgen05(q, q_stride, n_rows, out, out_stride, keys, values, n_pages, req_row_start, req_first_pos,
                              block_table, table_stride, n_requests, max_new_tokens, n_heads, n_kv_heads, head_dim, 64,
-                             1.f, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, row_scale, factors, seen, 0, 0, status, stream);
+                             scale, window, 0, 0, 1.f, nullptr, nullptr, 0, 0, factors, seen, 0, 0, status, stream);
 }

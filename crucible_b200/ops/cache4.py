@@ -484,19 +484,16 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
     both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
     spans = torch.empty(2 * n_blocks * kv + 3 * requests * stride, dtype=_I32, device=q.device)
     seen, blocks = spans[2 * n_blocks * kv:], spans[2 * (n_blocks * kv + requests * stride):]
-    q_half = torch.empty(rows, n_heads * dim, dtype=torch.float16, device=q.device)
-    factors = torch.empty(2 * requests * kv + rows * n_heads, dtype=_F32, device=q.device)
-    row_scale = factors[2 * requests * kv:]
+    factors = torch.empty(2 * requests * kv, dtype=_F32, device=q.device)
     starts, places = batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first
     _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.table.shape[1],
                batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
-               factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks, q.data_ptr(), q.stride(0), rows, sum(new),
-               n_heads // kv, scale, q_half.data_ptr(), row_scale.data_ptr()), "pages laid out")
-    code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q_half.data_ptr(), n_heads * dim,
-               row_scale.data_ptr(), factors.data_ptr(), seen.data_ptr(), rows, out.data_ptr(), out.stride(0), both[0].data_ptr(),
-               both[1].data_ptr(), n_blocks + 1, starts, places, blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim,
-               window or 0, _status(pages.device))
+               factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks), "pages laid out")
+    code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q.data_ptr(), q.stride(0), rows,
+               out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1, starts, places,
+               blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, scale, window or 0, factors.data_ptr(),
+               seen.data_ptr(), _status(pages.device))
     if code == build.UNSUPPORTED:
         return False
     _check(code, "attention4 (tiles)")
