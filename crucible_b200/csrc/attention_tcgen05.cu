@@ -556,28 +556,33 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             // The queries by hand, into float16 times 2^(13 - e), e the exponent of a row's largest; 8 NH lanes a row.
             // (Before the wait: the kernels that lay keys and values out start this one once what was before them has
             // ended, and they do not write queries.  Past L1, which may hold an earlier step's.)
-            constexpr int PIECES = ROWS * 8 * NH / (128 * GROUPS);
+            constexpr int STEP = 128 * GROUPS / (8 * NH), PIECES = ROWS / STEP;       // rows at once, times
+            const int r0 = (threadIdx.x - 64) / (8 * NH), c = (threadIdx.x - 64) % (8 * NH);
+            int tok = (first_row + r0) / n_rep, head = first_row + r0 - tok * n_rep;
+            const int step_tok = STEP / n_rep, step_head = STEP - step_tok * n_rep;
+            const __nv_bfloat16* from = p.qkv + (size_t)row_base * p.qkv_stride + (size_t)kv_head * n_rep * HD + c * 8;
             uint4 raw[PIECES];
 #pragma unroll
             for (int u = 0; u < PIECES; ++u) {
-                const int i = threadIdx.x - 64 + u * 128 * GROUPS, at = first_row + i / (8 * NH);
                 raw[u] = make_uint4(0, 0, 0, 0);
-                if (n_tiles > 0 && at < n_rows) {
-                    const int tok = row_base + at / n_rep, head = kv_head * n_rep + at % n_rep;
-                    raw[u] = __ldcg(reinterpret_cast<const uint4*>(p.qkv + (size_t)tok * p.qkv_stride + (size_t)head * HD + i % (8 * NH) * 8));
-                }
+                if (n_tiles > 0 && first_row + r0 + u * STEP < n_rows)
+                    raw[u] = __ldcg(reinterpret_cast<const uint4*>(from + (size_t)tok * p.qkv_stride + head * HD));
+                tok += step_tok;
+                head += step_head;
+                if (head >= n_rep) head -= n_rep, ++tok;
             }
 #pragma unroll
             for (int u = 0; u < PIECES; ++u) {
-                const int i = threadIdx.x - 64 + u * 128 * GROUPS, rr = i / (8 * NH), c = i % (8 * NH);
+                const int rr = r0 + u * STEP;
                 const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-                float most = 0.f;
+                // (magnitudes of bfloat16 compare like whole numbers)
+                uint32_t most = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+                for (int e = 0; e < 4; ++e) most = __vmaxu2(most, w[e] & 0x7fff7fffu);
 #pragma unroll
-                for (int o = 1; o < 8 * NH; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int up = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+                for (int o = 1; o < 8 * NH; o <<= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+                most = max(most >> 16, most & 0xffffu);
+                const int up = most > 0 ? min(13 - ((int)(most >> 7) - 127), 100) : 0;
                 const float by = __uint_as_float((uint32_t)(up + 127) << 23);
                 uint32_t h[4];
 #pragma unroll
