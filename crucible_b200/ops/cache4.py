@@ -358,7 +358,8 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
     """(blocks of a cluster, blocks of a stream or 0, us that it may take): how the keys are dealt, by the launch's row tiles of all kv heads
     (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
     hold.  A model of what either takes, in us.  A block takes a round of eight tiles in 0.7 alone on its SM and in 0.53 times
-    the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end; a launch takes 2.  A stream
+    the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end, a cluster half more; a launch
+    takes 2.  A stream
     takes no longer than its work, but 12 besides, and 6 for every unit that its blocks begin.  Modelled and measured, us:
     1 token of 32 heads of 128 on 8 behind 16,000 keys, clusters of 8 18 and 17, a stream 17 and 18; behind 131,071 97 and
     105, 41 and 40; 32 behind 16,000, clusters of 2 122 and 120, of 4 115 and 107, a stream 108 and 110; 64 of
@@ -369,8 +370,10 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
         rounds = -(-tiles // (8 * shares))
         each = weight * max(0.7, 0.53 * min(blocks * shares / tensor_core.N_SMS, per_sm))
         mean = total / (8 * shares * blocks)
-        waves = max(1.0, blocks * shares / resident)
-        us = 2.0 + waves * (5.0 + mean * each) + max(0.0, rounds - mean) * each + 0.1 * shares
+        waves = blocks * shares / resident
+        if waves < 2.0:
+            waves = -(-blocks * shares // resident)
+        us = 2.0 + waves * (5.0 + mean * each) + max(0.0, rounds - mean) * each + 0.1 * shares + (0.4 if shares > 1 else 0.0)
         if best is None or us < best[0]:
             best = us, shares
         if rounds == 1:
