@@ -355,16 +355,16 @@ def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
 
 
 def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 1.0) -> tuple:
-    """(blocks of a cluster, blocks of a stream or 0, us that it may take): how the keys are dealt, by the launch's row tiles of all kv heads
-    (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that the SMs
-    hold.  A model of what either takes, in us.  A block takes a round of eight tiles in 0.7 alone on its SM and in 0.53 times
-    the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end, a cluster half more; a launch
-    takes 2.  A stream
-    takes no longer than its work, but 12 besides, and 6 for every unit that its blocks begin.  Modelled and measured, us:
-    1 token of 32 heads of 128 on 8 behind 16,000 keys, clusters of 8 18 and 17, a stream 17 and 18; behind 131,071 97 and
-    105, 41 and 40; 32 behind 16,000, clusters of 2 122 and 120, of 4 115 and 107, a stream 108 and 110; 64 of
-    unlike lengths up to 8,191, clusters of 2 105 and 107, a stream 108 and 108."""
-    per_sm, work = resident / tensor_core.N_SMS, 0.53 * weight * total / (8 * tensor_core.N_SMS)
+    """(blocks of a cluster, blocks of a stream or 0, us that it may take): how the keys are dealt, by the launch's row tiles of
+    all kv heads (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that
+    the SMs hold.  A model of what either takes, in us.  A block takes a round of eight tiles in 0.7 alone on its SM and in
+    0.53 times the blocks beside it (heads of 128, bfloat16; `weight` for others), and 5 to begin and to end, a cluster half
+    more; a launch takes 2.  A stream's blocks take 1.1 and 0.24 times their number on the SM for a round (theirs are not
+    alike), and it 10.5 besides, 0.8 more for every 100 blocks, whose results are put together.  Modelled and measured, us:
+    1 token of 32 heads of 128 on 8 behind 16,000 keys, clusters of 8 19 and 17, a stream of three blocks an SM 18 and 18;
+    behind 131,071 clusters 97 and 105, a stream 44 and 41; 8 behind up to 16,000, clusters of 8 37 and 35, a stream 38
+    and 38; 32 clusters of 8 116 and 105, a stream 103 and 100."""
+    per_sm = resident / tensor_core.N_SMS
     best = None
     for shares in (1, 2, 4, 8):
         rounds = -(-tiles // (8 * shares))
@@ -379,9 +379,10 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
         if rounds == 1:
             break
     if total < 1 << 30 and blocks < 4 * resident:
-        stream = max(1, min(resident, total // 8))
-        us = 12.0 + 6.0 * blocks / resident + max(work, weight * max(0.7, 0.53 * stream / tensor_core.N_SMS))
-        if us < 0.95 * best[0]:
+        us, stream = min((max(1.0, weight) * (10.5 + 0.008 * each) + weight * (1.1 + 0.24 * n) * max(1.0, total / (8 * each)), each)
+                         for n in range(1, int(per_sm) + 1) for each in (max(1, min(n * tensor_core.N_SMS, total // 8)),))
+        us += 3.0 * blocks / resident
+        if us < best[0]:
             return 1, stream, us
     return best[1], 0, best[0]
 
