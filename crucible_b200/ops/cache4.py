@@ -26,6 +26,7 @@ page of the pool is not seen, a row of a request that is none is left as it is.
 """
 from __future__ import annotations
 
+import functools
 from operator import add as _add
 from typing import Optional, Sequence
 
@@ -122,14 +123,14 @@ class Pages4:
         _check(_at(self.device, lib.cb_values4, self.codes.data_ptr(), self.scales.data_ptr(), self.group,
                    2 * self.n_pages * self.kv_heads * self.page_tokens, self.head_dim, out.data_ptr(), _code(dtype)),
                "values in 4 bits")
-        return out[0], out[1]
+        return out.unbind()
 
     def bound_values(self) -> torch.Tensor:
         """What the bounds stand for: float32 [pages, kv heads, 2, dim]."""
         if self.bounds is None:
             raise KernelError("these pages keep no bounds")
         _need_cuda(self.bounds)
-        out = torch.empty(self.bounds.shape, dtype=_F32, device=self.bounds.device)
+        out = torch.empty_like(self.bounds, dtype=_F32)
         lib = build.load("append4")
         _check(_at(self.device, lib.cb_bound_values4, self.bounds.data_ptr(), self.bound_scales.data_ptr(),
                    self.n_pages * self.kv_heads, self.head_dim, out.data_ptr()), "bounds in 8 bits")
@@ -151,7 +152,7 @@ class Batch:
     beyond it are not picked, only attention to all of them reads them."""
 
     __slots__ = ("positions", "row_request", "row_start", "first_pos", "table", "new_tokens", "held_tokens", "requests",
-                 "most_new", "reach", "lead", "device")
+                 "most_new", "alike", "reach", "lead", "device")
 
     def __init__(self, positions, row_request, row_start, first_pos, table, new_tokens: Sequence[int],
                  held_tokens: Sequence[int], reach: Optional[int] = None):
@@ -170,7 +171,8 @@ class Batch:
                 and dev == row_request.get_device() == row_start.get_device() == first_pos.get_device() == table.get_device()):
             self._refuse()
         self.most_new = most = max(new_tokens)
-        if requests == 1 or most == min(new_tokens):
+        self.alike = alike = requests == 1 or most == min(new_tokens)      # as many rows of every request
+        if alike:
             self.lead = requests if most == 1 else 0
             longest = most + max(held_tokens)
         else:
@@ -354,6 +356,7 @@ def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
     return tensor_core.N_SMS * (2 if dim > 128 or columns > 1 else 4 if dim // group * (2 if f32 else 1) <= 2 else 3)
 
 
+@functools.lru_cache(maxsize=4096)
 def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 1.0) -> tuple:
     """(blocks of a cluster, blocks of a stream or 0, us that it may take): how the keys are dealt, by the launch's row tiles of
     all kv heads (`blocks`), the most tiles of 16 keys that one of them sees, how many they see in all, and the blocks that
@@ -378,7 +381,7 @@ def _shares(blocks: int, tiles: int, total: int, resident: int, weight: float = 
             best = us, shares
         if rounds == 1:
             break
-    if total < 1 << 30 and blocks < 4 * resident:
+    if best[0] > 10.5 and total < 1 << 30 and blocks < 4 * resident:
         us, stream = min((max(1.0, weight) * (10.5 + 0.008 * each) + weight * (1.1 + 0.24 * n) * max(1.0, total / (8 * each)), each)
                          for n in range(1, int(per_sm) + 1) for each in (max(1, min(n * tensor_core.N_SMS, total // 8)),))
         us += 3.0 * blocks / resident
@@ -394,18 +397,20 @@ def _dealt(dim, kv, n_rep, group, f32, batch, window, first, last) -> tuple:
     new, held = batch.new_tokens, batch.held_tokens
     if requests < batch.requests:
         new, held = new[first:last], held[first:last]
-    most_rows = max(new)
+        most_rows, alike = max(new), max(new) == min(new)
+    else:
+        most_rows, alike = batch.most_new, batch.alike
     reach = batch.reach if window is None else min(batch.reach, window + most_rows)
     tiles = -(-reach // 16) + (window is not None)
     columns = _columns(n_rep, f32, dim, most_rows)
-    if requests > 1 and most_rows > min(new):              # (blocks behind a request's last row end at once)
-        per = [kv * -(-n * n_rep // (8 * columns)) for n in new]
-        blocks = sum(per)
-        total = sum([p * min(tiles, (n + h) // 16 + 1) for p, n, h in zip(per, new, held)])
-    else:
+    if alike:
         per = kv * -(-most_rows * n_rep // (8 * columns))
         blocks = requests * per
         total = per * (requests * tiles if requests == 1 or window is not None else (sum(held) + sum(new)) // 16 + requests)
+    else:                                                  # (blocks behind a request's last row end at once)
+        per = [kv * -(-n * n_rep // (8 * columns)) for n in new]
+        blocks = sum(per)
+        total = sum([p * min(tiles, (n + h) // 16 + 1) for p, n, h in zip(per, new, held)])
     return columns, *_dealt_to(dim, group, f32, columns, blocks, tiles, total)
 
 
@@ -423,7 +428,7 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     have picks."""
     dim, kv = pages.head_dim, pages.kv_heads
     n_rep, f32 = n_heads // kv, q.dtype is _F32
-    rows = batch.positions.shape[0]
+    rows = batch.positions.size(0)
     if picks is not None:
         most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
