@@ -431,20 +431,29 @@ struct ExpandParams {
     int block_stride, n_blocks;
 };
 
-// Which request a block of 64 tokens is of, from how many blocks the requests before it have.
+// Which request a block of 64 tokens is of, from how many blocks the requests before it have: from the one that holds the
+// first token that a row sees to the one that holds the last.
 struct Laid {
-    int request, before, count, first, held;
+    int request, before, count, first, held, lo;
+    __device__ __forceinline__ int index_of(int block) const { return block - before + (lo >> 6); }
 };
 
+__device__ __forceinline__ Laid laid_at(const ExpandParams& p, int request, int before) {
+    Laid at = {request, before, 0, 0, 0, 0};
+    at.first = p.first_pos[request];
+    at.held = at.first + p.row_start[request + 1] - p.row_start[request];
+    at.lo = p.window > 0 ? max(0, at.first - p.window + 1) : 0;
+    at.count = max(0, ((at.held + 63) >> 6) - (at.lo >> 6));
+    return at;
+}
+
 __device__ __forceinline__ Laid laid_of(const ExpandParams& p, int block) {
-    Laid at = {0, 0, 0, 0, 0};
-    for (; at.request < p.n_requests; ++at.request) {
-        at.first = p.first_pos[at.request];
-        at.held = at.first + p.row_start[at.request + 1] - p.row_start[at.request];
-        at.count = (at.held + 63) >> 6;
-        if (block < at.before + at.count) break;
-        at.before += at.count;
+    Laid at = {0, 0, 0, 0, 0, 0};
+    for (int r = 0; r < p.n_requests; ++r) {
+        at = laid_at(p, r, at.before + at.count);
+        if (block < at.before + at.count) return at;
     }
+    at.request = p.n_requests;
     return at;
 }
 
@@ -464,9 +473,9 @@ __global__ void __launch_bounds__(128) span4_kernel(const ExpandParams p) {
     cb_pdl_wait();
     cb_pdl_trigger();              // (after the wait: the tiles' kernel reads where rows begin, and queries, before its own)
     const Laid in = laid_of(p, blockIdx.x);
-    const int side = threadIdx.x >> 6, pos = ((int)blockIdx.x - in.before) * 64 + (threadIdx.x & 63);
+    const int side = threadIdx.x >> 6, pos = in.index_of(blockIdx.x) * 64 + (threadIdx.x & 63);
     int e = C4_LEAST_SPAN;
-    if (in.request < p.n_requests && pos < in.held && pos >= (p.window > 0 ? max(0, in.first - p.window + 1) : 0)) {
+    if (in.request < p.n_requests && pos < in.held && pos >= in.lo) {
         const long long at = c4_row(p.table + (size_t)in.request * p.table_stride, p.table_stride, p.page_tokens, p.n_pages, p.kv_heads, pos);
         if (at >= 0) {
             const long long row = at + ((long long)side * p.n_pages * p.kv_heads + blockIdx.y) * p.page_tokens;
@@ -508,21 +517,20 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     constexpr int LANES = D / 8, PER_WARP = 32 / LANES, ROUNDS = 64 / (8 * PER_WARP);
     const int block = blockIdx.x, lane = threadIdx.x & 31, within = lane % LANES;
     if (block == 0 && blockIdx.y == 0) {
-        int before = 0;
+        Laid at = {0, 0, 0, 0, 0, 0};
         for (int r = 0; r < p.n_requests; ++r) {
-            const int count = (p.first_pos[r] + p.row_start[r + 1] - p.row_start[r] + 63) >> 6;
+            at = laid_at(p, r, at.before + at.count);
             for (int i = threadIdx.x; i < p.block_stride; i += 256) {
-                const bool one = i < count && before + i < p.n_blocks;
-                p.blocks[(size_t)r * p.block_stride + i] = one ? before + i : p.n_blocks;
-                if (!one) reinterpret_cast<uint2*>(p.seen)[(size_t)r * p.block_stride + i] = make_uint2(0u, 0u);
+                const int one = at.before + i - (at.lo >> 6);
+                const bool some = one >= at.before && one < min(at.before + at.count, p.n_blocks);
+                p.blocks[(size_t)r * p.block_stride + i] = some ? one : p.n_blocks;
+                if (!some) reinterpret_cast<uint2*>(p.seen)[(size_t)r * p.block_stride + i] = make_uint2(0u, 0u);
             }
-            before += count;
         }
     }
     const Laid in = laid_of(p, block);
-    const int request = in.request, held = in.held, index = block - in.before;
+    const int request = in.request, held = in.held, lo = in.lo, index = in.index_of(block);
     const bool some = block < p.n_blocks && request < p.n_requests;
-    const int lo = p.window > 0 ? max(0, in.first - p.window + 1) : 0;
     const int* table = p.table + (size_t)request * p.table_stride;
     __shared__ int there[64];
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
@@ -542,7 +550,7 @@ __global__ void __launch_bounds__(256) expand4_kernel(const ExpandParams p) {
     }
     const int2 e = some ? exponents_of(p, in, blockIdx.y) : make_int2(0, 0);
     const float down_k = two_to(-e.x), down_v = two_to(-e.y);
-    if (some && index == 0 && threadIdx.x == 0)
+    if (some && block == in.before && threadIdx.x == 0)
         p.factors[(size_t)request * p.kv_heads + blockIdx.y] = make_float2(two_to(e.x), two_to(e.y));
     __syncthreads();
     if (some && index < p.block_stride && blockIdx.y == 0 && threadIdx.x < 64) {

@@ -19,8 +19,8 @@ instead).  There a value that is no number makes the whole head's
 result none for the rows that see it; elsewhere only its group's features.
 
 Everything launches on torch's current stream of the tensors' device and may be captured into a CUDA graph; what is
-allocated on the way (partial results of very long contexts, pages laid out anew for long portions) comes from
-torch's pool.  Outputs may not overlap inputs, but where a function says so.  Sums and softmax statistics are
+allocated on the way (partial results of very long contexts, pages laid out anew for long portions, 2 GB at a time at most)
+comes from torch's pool.  Outputs may not overlap inputs, but where a function says so.  Sums and softmax statistics are
 float32.  Page ids, positions and row numbers on the device are looked over by the kernels: a key whose table entry names no
 page of the pool is not seen, a row of a request that is none is left as it is.
 """
@@ -345,9 +345,10 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         if lead < batch.requests and _laid_out(q, out, n_heads, batch, pages, window, behind, lead):
             if behind < lead:
                 _walk(q, out, n_heads, scale, batch, pages, window, None, behind, lead)
-            if _tiles(q, out, n_heads, scale, batch, pages, window, lead):
-                return
-            behind = lead
+            for first, last, counts in _slabs(batch, window, lead, _MOST_BLOCKS // (kv * dim)):
+                if counts is None or not _tiles(q, out, n_heads, scale, batch, pages, window, first, last, counts):
+                    _walk(q, out, n_heads, scale, batch, pages, window, None, first, last)
+            return
         _walk(q, out, n_heads, scale, batch, pages, window, None, behind, batch.requests)
 
 
@@ -474,22 +475,47 @@ def _laid_out(q, out, n_heads, batch, pages, window, behind, first) -> bool:
     reach = max(map(_add, new, held))
     seen = reach if window is None else min(reach, window + 128)
     pairs = sum([n * min(h + n / 2, seen) for n, h in zip(new, held)])
-    tiles = (8.5 + 1.7e-6 * (sum(new) + sum(held)) * kv * dim
-             + max(0.0072 * min(seen, reach), 4e-6 * dim * n_heads * pairs / 750.0))
+    laid = sum(new) + sum(held) if window is None else sum([n + min(h, window) for n, h in zip(new, held)])
+    tiles = 8.5 + 1.7e-6 * laid * kv * dim + max(0.0072 * min(seen, reach), 4e-6 * dim * n_heads * pairs / 750.0)
     if behind < first:
         tiles += _dealt(dim, kv, n_rep, pages.group, False, batch, window, behind, first)[3]
     return tiles < walk
 
 
-def _tiles(q, out, n_heads, scale, batch, pages, window, first) -> bool:
-    """bfloat16 portions of many rows: the keys and values of the requests from `first` on are laid out once, in blocks of 64
-    tokens (not taken apart again for every tile of rows), and attention runs over these on tcgen05.  Queries, keys, values
+_MOST_BLOCKS = (2 << 30) // (64 * 4)  # of 64 tokens and a feature that are laid out at a time: 2 GB of keys and values
+
+
+def _slabs(batch, window, first, most):
+    """The requests from `first` on, as many at a time as `most` blocks of 64 tokens hold: (first, last, the blocks of each, or
+    None where one request alone has more).  With a window, as many blocks as the step's rows can reach wherever they begin."""
+    new, held = batch.new_tokens, batch.held_tokens
+    counts, total = [], 0
+    for r in range(first, batch.requests):
+        n = -(-(new[r] + held[r]) // 64)
+        if window is not None:
+            n = min(n, (window + new[r] + 62) // 64 + 1)
+        if total + n > most:
+            if counts:
+                yield first, r, counts
+            first, counts, total = r, [], 0
+            if n > most:
+                yield r, r + 1, None
+                first = r + 1
+                continue
+        counts.append(n)
+        total += n
+    if counts:
+        yield first, batch.requests, counts
+
+
+def _tiles(q, out, n_heads, scale, batch, pages, window, first, last, counts) -> bool:
+    """bfloat16 portions of many rows: the keys and values of the requests first .. last - 1 are laid out once, in blocks of
+    64 tokens (not taken apart again for every tile of rows), and attention runs over these on tcgen05.  Queries, keys, values
     and p are float16 there, with a power of two for each row, key head and value head: eleven bits of them (in bfloat16 the
     results were off by 0.0033 of themselves, half of it the roundings inside, in float16 by 0.0017, which is their own)."""
     dim, kv = pages.head_dim, pages.kv_heads
-    new, held = batch.new_tokens[first:], batch.held_tokens[first:]
-    counts = [-(-(h + n) // 64) for h, n in zip(held, new)]
-    n_blocks, stride, requests, rows = sum(counts), max(counts), len(counts), batch.positions.shape[0]
+    new, held = batch.new_tokens[first:last], batch.held_tokens[first:last]
+    n_blocks, stride, requests, rows = sum(counts), -(-max(map(_add, new, held)) // 64), len(counts), batch.positions.size(0)
     both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
     spans = torch.empty(2 * n_blocks * kv + 3 * requests * stride, dtype=_I32, device=q.device)
     seen, blocks = spans[2 * n_blocks * kv:], spans[2 * (n_blocks * kv + requests * stride):]

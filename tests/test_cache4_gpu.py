@@ -208,7 +208,7 @@ def test_attention_of_few_rows(dim, group, n_rep, kv_heads, page, requests, dtyp
     (128, 128, 2, 2, 24, [(30, 65), (129, 64), (0, 130)], None), (128, 32, 7, 1, 7, [(90, 31)], None),
     (64, 64, 4, 2, 64, [(40, 1), (17, 1), (0, 200), (300, 20)], None), (128, 64, 4, 1, 16, [(200, 1), (250, 90), (0, 64)], 100),
     (64, 64, 2, 2, 16, [(500, 40)], 17), (64, 64, 32, 1, 16, [(70, 5), (0, 9)], None), (128, 128, 5, 1, 8, [(3, 140)], None),
-    (64, 32, 1, 3, 16, [(0, 64), (1000, 70)], None), (128, 64, 130, 1, 16, [(10, 3)], None)])
+    (64, 32, 1, 3, 16, [(0, 64), (1000, 70)], None), (128, 128, 4, 1, 24, [(3000, 70), (5, 1), (64, 66), (0, 60)], 130), (128, 64, 130, 1, 16, [(10, 3)], None)])
 def test_attention_of_portions_that_are_laid_out(dim, group, n_rep, kv_heads, page, requests, window, monkeypatch):
     """Long portions, decoded tokens at the step's head walked beside them; what the window has passed is not read."""
     from crucible_b200.ops import cache4
@@ -307,6 +307,48 @@ def test_portions_laid_out_of_a_captured_step(monkeypatch):
             cc.assert_attention_laid_out(out[:case.rows], want, most, spread[0]) if out is not outs[2] else \
                 cc.assert_attention(out[:case.rows], want, most, BF16)
             assert (out[case.rows:] == 7).all()
+
+
+def test_portions_laid_out_in_a_window_wherever_they_begin(monkeypatch):
+    """A captured step replayed at other places: as many blocks of 64 tokens as the rows may reach, not one more or less."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    case = cc.Case([(700, 50), (640, 33)], dim=64, group=64, n_rep=2, kv_heads=1, page=16, seed=43)
+    q, window = case.queries(), 79
+    out = torch.empty_like(q)
+
+    def step():
+        cache4.attention4(q, out, case.heads, 0.125, case.batch, case.pages, window=window)
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for first in ((700, 640), (0, 1), (63, 64), (127, 128), (141, 142), (143, 78), (560, 593)):
+        case.requests = [(first[0], 50), (first[1], 33)]
+        case.first_pos.copy_(torch.tensor(first))
+        case.positions.copy_(torch.cat([f + torch.arange(n) for f, n in case.requests]))
+        out.fill_(7)
+        graph.replay()
+        spread = []
+        want, most = case.attention(q, 0.125, window=window, spread=spread)
+        cc.assert_attention_laid_out(out, want, most, spread[0])
+
+
+@pytest.mark.parametrize("blocks,tiled", [(11, 3), (9, 3), (6, 3), (4, 2), (3, 2), (2, 1), (1, 0)])
+def test_portions_that_are_laid_out_a_few_requests_at_a_time(blocks, tiled, monkeypatch):
+    """No more at a time than scratch memory is for; a request that alone has more is walked."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    monkeypatch.setattr(cache4, "_MOST_BLOCKS", blocks * 2 * 64)
+    calls, tiles = [], cache4._tiles
+    monkeypatch.setattr(cache4, "_tiles", lambda *a: calls.append(a[-3:]) or tiles(*a))
+    case = cc.Case([(7, 1), (100, 70), (0, 90), (300, 40)], dim=64, group=32, n_rep=4, kv_heads=2, seed=45)   # blocks of 3, 2, 6
+    q, spread = case.queries(), []
+    want, most = case.attention(q, 0.125, spread=spread)
+    got = _attend(case, q, 0.125)
+    assert sum(last - first for first, last, _ in calls) == tiled and all(sum(counts) <= blocks for _, _, counts in calls)
+    cc.assert_attention(got[:1], want[:1], most[:1], BF16)
+    cc.assert_attention_laid_out(got, want, most, spread[0])
 
 
 def test_portions_laid_out_on_two_streams_at_once(monkeypatch):
