@@ -192,6 +192,12 @@ class Engine:
         if o.attend_pages is not None and (o.attend_pages < 3 or o.page_tokens % 16 or need.window is not None):
             raise ValueError("attend_pages takes 3 pages or more, of a multiple of 16 tokens, and attention without a window; got "
                              f"{o.attend_pages} pages of {o.page_tokens} and a window of {need.window}")
+        if o.attend_pages is not None:
+            from ..ops import cache4
+            most = min(cache4.most_pages(m.spec.n_heads // need.kv_heads, need.head_dim) for m in mixers)
+            if -(-self.context_limit // o.page_tokens) > most:
+                raise ValueError(f"attend_pages picks among {most} pages of a request at most; contexts of {self.context_limit} "
+                                 f"tokens take longer pages than {o.page_tokens}, or a max_context")
         for mixer in mixers:
             # (long portions are attended to over pages laid out anew, whose size follows the contexts)
             mixer.graph_safe_prompt_steps = False

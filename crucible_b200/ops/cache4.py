@@ -292,9 +292,14 @@ def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, pick
                pages.bounds.data_ptr(), pages.bound_scales.data_ptr(), pages.n_pages, pages.page_tokens, n_heads // kv, kv,
                dim, rows, picks.data_ptr(), picks.shape[2], first, last, most, _pick_shares(rows * kv, most))
     if code == build.UNSUPPORTED:
-        raise KernelError(f"pick_pages4 takes tables of up to {(lib.cb_pick4_room() - n_heads // kv * (2 * dim + 4)) // 4} pages "
-                          f"a request here, got {most}; longer pages make shorter tables")
+        raise KernelError(f"pick_pages4 takes tables of up to {most_pages(n_heads // kv, dim)} pages a request here, got {most}; "
+                          "longer pages make shorter tables")
     _check(code, "pick_pages4")
+
+
+def most_pages(n_rep: int, head_dim: int) -> int:
+    """Pages that a request may have for `pick_pages4`, `n_rep` query heads on a kv head."""
+    return (build.load("pick4").cb_pick4_room() - n_rep * (2 * head_dim + 4)) // 16 * 4
 
 
 def _pick_shares(blocks: int, pages: int) -> int:

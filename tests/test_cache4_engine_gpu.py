@@ -196,3 +196,21 @@ def test_what_the_engine_refuses(tmp_path):
     other = vuvosun_cases.make_folder(tmp_path, sorted(vuvosun_cases.CASES)[0])
     with pytest.raises(ValueError, match="cache"):
         _engine(other, "bfloat16", cache_group=32)
+
+
+def test_contexts_of_more_pages_than_are_picked_among(tmp_path):
+    """Refused when the engine is made, not by a step of some later token; longer pages or shorter contexts are taken."""
+    from crucible_b200.ops import cache4
+    from crucible_b200.weights import write_random_model
+    folder = os.path.join(str(tmp_path), "long")
+    write_random_model(dict(CONFIGS["heads of 64"], n_layer=1, block_size=1_000_000), folder, 0)
+    more = dict(cache_group=64, attend_pages=8, n_pages=100)
+    with pytest.raises(ValueError, match="picks among"):
+        _engine(folder, "bfloat16", **more)
+    for options in (dict(page_tokens=32), dict(max_context=cache4.most_pages(3, 64) * 16)):
+        from crucible_b200.engine.engine import StepEntry
+        engine = _engine(folder, "bfloat16", **more, **options)
+        engine.step([StepEntry("a", list(range(200)), [])])
+        assert torch.isfinite(engine.step([StepEntry("a", [7], [0])])).all()
+    with pytest.raises(ValueError, match="picks among"):
+        _engine(folder, "bfloat16", **more, max_context=cache4.most_pages(3, 64) * 16 + 1)
