@@ -152,7 +152,7 @@ class Batch:
     beyond it are not picked, only attention to all of them reads them."""
 
     __slots__ = ("positions", "row_request", "row_start", "first_pos", "table", "new_tokens", "held_tokens", "requests",
-                 "most_new", "alike", "reach", "lead", "device")
+                 "rows", "stride", "most_new", "alike", "reach", "lead", "device")
 
     def __init__(self, positions, row_request, row_start, first_pos, table, new_tokens: Sequence[int],
                  held_tokens: Sequence[int], reach: Optional[int] = None):
@@ -161,15 +161,18 @@ class Batch:
         self.new_tokens, self.held_tokens = new_tokens, held_tokens
         self.requests = requests = len(new_tokens)
         self.device = dev = positions.get_device()
-        if not (requests > 0 and len(held_tokens) == requests and table.dim() == 2 and table.size(0) == requests and table.size(1) > 0
-                and positions.dim() == 1 == row_request.dim() == row_start.dim() == first_pos.dim()
-                and row_request.size(0) == positions.size(0) and row_start.size(0) == requests + 1 and first_pos.size(0) == requests
+        # (shapes whole: asked for one size at a time they take twice as long)
+        shape, pages = positions.shape, table.shape
+        if not (requests > 0 and len(held_tokens) == requests and len(pages) == 2 and pages[0] == requests and pages[1] > 0
+                and len(shape) == 1 and row_request.shape == shape and row_start.shape == (requests + 1,)
+                and first_pos.shape == (requests,)
                 and positions.dtype is _I32 and row_request.dtype is _I32 and row_start.dtype is _I32
                 and first_pos.dtype is _I32 and table.dtype is _I32
                 and positions.is_contiguous() and row_request.is_contiguous() and row_start.is_contiguous()
                 and first_pos.is_contiguous() and table.is_contiguous()
                 and dev == row_request.get_device() == row_start.get_device() == first_pos.get_device() == table.get_device()):
             self._refuse()
+        self.rows, self.stride = shape[0], pages[1]
         self.most_new = most = max(new_tokens)
         self.alike = alike = requests == 1 or most == min(new_tokens)      # as many rows of every request
         if alike:
@@ -203,16 +206,18 @@ class Batch:
         return batch
 
 
-def _rows_ok(t: torch.Tensor, what: str, width: int, dtype, rows: int) -> None:
-    """`rows` rows at least, of `width` numbers side by side; of `dtype`, or (None) float32 or bfloat16."""
-    if not (t.dim() == 2 and t.size(1) == width and (t.dtype is dtype if dtype is not None else t.dtype in _FLOATS)
-            and t.stride(1) == 1 and (t.stride(0) >= width or t.size(0) == 1) and t.size(0) >= rows):
+def _rows_ok(t: torch.Tensor, what: str, width: int, dtype, rows: int) -> int:
+    """`rows` rows at least, of `width` numbers side by side; of `dtype`, or (None) float32 or bfloat16.  How far apart they are."""
+    shape, strides = t.shape, t.stride()
+    if not (len(shape) == 2 and shape[1] == width and (t.dtype is dtype if dtype is not None else t.dtype in _FLOATS)
+            and strides[1] == 1 and (strides[0] >= width or shape[0] == 1) and shape[0] >= rows):
         names = "float32 or bfloat16" if dtype is None else str(dtype).replace("torch.", "")
         if t.dim() != 2 or t.shape[1] != width or t.dtype not in _FLOATS or (dtype is not None and t.dtype != dtype):
             raise KernelError(f"{what}: {names} rows [T, {width}] are taken, got {t.dtype} {list(t.shape)}")
         if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
             raise KernelError(f"{what}: rows must be contiguous and not overlap")
         raise KernelError(f"{what}: the batch has {rows} rows, the tensor {t.shape[0]}")
+    return strides[0]
 
 
 def _same_device(what: str, batch: "Batch", pages: Pages4, *others) -> None:
@@ -240,24 +245,26 @@ def rope_append4(qkv: torch.Tensor, q: torch.Tensor, n_heads: int, cos: Optional
     width = (n_heads + 2 * kv) * dim
     if n_heads < 1:
         raise KernelError("rope_append4: a positive number of query heads is needed")
-    rows = batch.positions.size(0)
-    _rows_ok(qkv, "rope_append4 rows", width, None, rows)
-    _rows_ok(q, "rope_append4 queries", n_heads * dim, qkv.dtype, rows)
+    rows = batch.rows
+    qkv_stride = _rows_ok(qkv, "rope_append4 rows", width, None, rows)
+    q_stride = _rows_ok(q, "rope_append4 queries", n_heads * dim, qkv.dtype, rows)
     if (cos is None) != (sin is None):
         raise KernelError("rope_append4: cos and sin come together")
-    rotary = 0
+    rotary = positions = 0
     if cos is not None:
-        rotary = 2 * cos.shape[-1]
-        if (cos.dim() != 2 or cos.dtype != _F32 or sin.dtype != _F32 or sin.shape != cos.shape or not cos.is_contiguous()
+        shape = cos.shape
+        rotary = 2 * shape[-1] if shape else 0
+        if (len(shape) != 2 or cos.dtype is not _F32 or sin.dtype is not _F32 or sin.shape != shape or not cos.is_contiguous()
                 or not sin.is_contiguous() or rotary > dim):
             raise KernelError(f"rope_append4: the tables are contiguous float32 [positions, r / 2] with r at most {dim}, got "
                               f"{cos.dtype} {list(cos.shape)} and {sin.dtype} {list(sin.shape)}")
+        positions = shape[0]
     _same_device("rope_append4", batch, pages, qkv, q, cos, sin)
     lib = build.load("append4")
-    code = _at(pages.device, lib.cb_append4, qkv.data_ptr(), _code(qkv.dtype), qkv.stride(0), q.data_ptr(), q.stride(0),
-               cos.data_ptr() if rotary else 0, sin.data_ptr() if rotary else 0, rotary, cos.shape[0] if rotary else 0,
-               1 if neighbours else 0, 1 if write else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
-               batch.table.shape[1], batch.requests, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
+    code = _at(pages.device, lib.cb_append4, qkv.data_ptr(), _code(qkv.dtype), qkv_stride, q.data_ptr(), q_stride,
+               cos.data_ptr() if rotary else 0, sin.data_ptr() if rotary else 0, rotary, positions, 1 if neighbours else 0,
+               1 if write else 0, batch.positions.data_ptr(), batch.row_request.data_ptr(), batch.table.data_ptr(),
+               batch.stride, batch.requests, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, n_heads, kv, dim, pages.group, rows,
                pages.bounds.data_ptr() if pages.bounds is not None else 0,
                pages.bound_scales.data_ptr() if pages.bounds is not None else 0)
@@ -272,7 +279,7 @@ def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, pick
     [rows, kv heads, count], or [n, ..] for the first n rows alone.  A query is rounded to 8 bits for it (largest magnitude
     127), as the bounds are."""
     dim, kv = pages.head_dim, pages.kv_heads
-    rows = batch.positions.size(0)
+    rows = batch.rows
     _rows_ok(q, "pick_pages4 queries", n_heads * dim, None, rows)
     if n_heads < 1 or n_heads % kv:
         raise KernelError(f"pick_pages4: {n_heads} query heads do not share {kv} kv heads evenly")
@@ -285,10 +292,10 @@ def pick_pages4(q: torch.Tensor, n_heads: int, batch: Batch, pages: Pages4, pick
                           "among them (the row's own page has to be)")
     _same_device("pick_pages4", batch, pages, q, picks)
     # scores are held for as many pages as the longest context may have
-    most = min(batch.table.shape[1], -(-batch.reach // pages.page_tokens))
+    most = min(batch.stride, -(-batch.reach // pages.page_tokens))
     lib = build.load("pick4")
     code = _at(pages.device, lib.cb_pick4, q.data_ptr(), _code(q.dtype), q.stride(0), batch.positions.data_ptr(),
-               batch.row_request.data_ptr(), batch.table.data_ptr(), batch.table.shape[1], batch.requests,
+               batch.row_request.data_ptr(), batch.table.data_ptr(), batch.stride, batch.requests,
                pages.bounds.data_ptr(), pages.bound_scales.data_ptr(), pages.n_pages, pages.page_tokens, n_heads // kv, kv,
                dim, rows, picks.data_ptr(), picks.shape[2], first, last, most, _pick_shares(rows * kv, most))
     if code == build.UNSUPPORTED:
@@ -325,7 +332,7 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
     walked by itself, so that this is for a few rows a request; page sizes are multiples of 16, and there is no window.
     Picks of the first n rows alone are for the first n requests, which bring one row each; the others attend to all."""
     dim, kv = pages.head_dim, pages.kv_heads
-    rows = batch.positions.size(0)
+    rows = batch.rows
     _rows_ok(q, "attention4 queries", n_heads * dim, None, rows)
     _rows_ok(out, "attention4 output", n_heads * dim, q.dtype, rows)
     if n_heads < 1 or n_heads % kv:
@@ -434,7 +441,7 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
     have picks."""
     dim, kv = pages.head_dim, pages.kv_heads
     n_rep, f32 = n_heads // kv, q.dtype is _F32
-    rows = batch.positions.size(0)
+    rows = batch.rows
     if picks is not None:
         most_rows, blocks = 1, min(rows, picks.shape[0])
         tiles = picks.shape[2] * pages.page_tokens // 16
@@ -446,10 +453,10 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
         columns, shares, stream, _ = _dealt(dim, kv, n_rep, pages.group, f32, batch, window, first, last)
     partial = torch.empty(stream * 16 * columns * (dim + 2), dtype=_F32, device=q.device) if stream else None
     lib = build.load(f"attention4_{dim}")
-    code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0),
+    code = _at(pages.device, lib.cb_attention4, q.data_ptr(), _code(q.dtype), q.stride()[0], out.data_ptr(), out.stride()[0],
                pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages, pages.page_tokens, kv, n_rep, pages.group,
                batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first,
-               batch.table.data_ptr() + 4 * first * batch.table.shape[1], batch.table.shape[1],
+               batch.table.data_ptr() + 4 * first * batch.stride, batch.stride,
                batch.requests if picks is not None else last - first,
                picks.data_ptr() if picks is not None else 0, picks.shape[2] if picks is not None else 0,
                batch.row_request.data_ptr(), batch.positions.data_ptr(),
@@ -520,15 +527,15 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first, last, counts) ->
     results were off by 0.0033 of themselves, half of it the roundings inside, in float16 by 0.0017, which is their own)."""
     dim, kv = pages.head_dim, pages.kv_heads
     new, held = batch.new_tokens[first:last], batch.held_tokens[first:last]
-    n_blocks, stride, requests, rows = sum(counts), -(-max(map(_add, new, held)) // 64), len(counts), batch.positions.size(0)
+    n_blocks, stride, requests, rows = sum(counts), -(-max(map(_add, new, held)) // 64), len(counts), batch.rows
     both = torch.empty(2, n_blocks + 1, kv, 64, dim, dtype=torch.float16, device=q.device)
     spans = torch.empty(2 * n_blocks * kv + 3 * requests * stride, dtype=_I32, device=q.device)
     seen, blocks = spans[2 * n_blocks * kv:], spans[2 * (n_blocks * kv + requests * stride):]
     factors = torch.empty(2 * requests * kv, dtype=_F32, device=q.device)
     starts, places = batch.row_start.data_ptr() + 4 * first, batch.first_pos.data_ptr() + 4 * first
     _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
-               pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.table.shape[1],
-               batch.table.shape[1], requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
+               pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.stride,
+               batch.stride, requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
                factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks), "pages laid out")
     code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q.data_ptr(), q.stride(0), rows,
                out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1, starts, places,
