@@ -429,6 +429,7 @@ struct ExpandParams {
     uint32_t* seen;          // [requests][block_stride][2]: a bit a token that is there
     int* blocks;             // [requests][block_stride]: which blocks of 64 tokens are a request's
     int block_stride, n_blocks;
+    int rows;                // of the step's tensors: what requests have beyond them is not there
 };
 
 // Which request a block of 64 tokens is of, from how many blocks the requests before it have: from the one that holds the
@@ -441,9 +442,10 @@ struct Laid {
 __device__ __forceinline__ Laid laid_at(const ExpandParams& p, int request, int before) {
     Laid at = {request, before, 0, 0, 0, 0};
     at.first = p.first_pos[request];
-    at.held = at.first + p.row_start[request + 1] - p.row_start[request];
+    const int row = p.row_start[request];
+    at.held = row < 0 ? 0 : at.first + max(0, min(p.row_start[request + 1], p.rows) - row);
     at.lo = p.window > 0 ? max(0, at.first - p.window + 1) : 0;
-    at.count = max(0, ((at.held + 63) >> 6) - (at.lo >> 6));
+    at.count = max(0, min((at.held + 63) >> 6, p.block_stride) - (at.lo >> 6));
     return at;
 }
 
@@ -660,12 +662,12 @@ CB_EXPORT int cb_bound_values4(const void* bounds, const float* scales, int head
 CB_EXPORT int cb_expand4(const void* codes, const void* scales, int n_pages, int page_tokens, int kv_heads, int head_dim,
                          int group, const int* row_start, const int* first_pos, const int* table, int table_stride,
                          int n_requests, int window, void* keys, void* values, int* spans, float* factors, uint32_t* seen,
-                         int* blocks, int block_stride, int n_blocks, void* stream) {
+                         int* blocks, int block_stride, int n_blocks, int rows, void* stream) {
     if (n_blocks <= 0) return 0;
     const ExpandParams p = {reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint32_t*>(scales), n_pages,
                             page_tokens, kv_heads, group, row_start, first_pos, table, table_stride, n_requests, window,
                             reinterpret_cast<__half*>(keys), reinterpret_cast<__half*>(values), spans,
-                            reinterpret_cast<float2*>(factors), seen, blocks, block_stride, n_blocks};
+                            reinterpret_cast<float2*>(factors), seen, blocks, block_stride, n_blocks, rows};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const dim3 spans_grid((unsigned)n_blocks, (unsigned)kv_heads);
     const dim3 grid((unsigned)n_blocks + 1, (unsigned)kv_heads);

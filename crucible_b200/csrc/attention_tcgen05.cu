@@ -90,6 +90,7 @@ struct TcAttnParams {
     int* status;
     const float2* factors;   // GATE_SCALED: [requests][n_kv_heads], of the scores and of the results
     const uint2* seen;       // GATE_SCALED: [requests][table_stride], which of a page's 64 keys are there
+    int n_rows;              // GATE_SCALED: of the queries and results; what requests have beyond them is left alone
 };
 
 // GATE: the results' gate, fixed when it is compiled: the epilogue runs once per block and its instructions
@@ -278,7 +279,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     // table entries looked up, before the wait for them.
     const int n_rep = p.n_rep, tile_rows = p.tile_rows;
     const int row_base = p.req_row_start[req];
-    const int n_new = p.req_row_start[req + 1] - row_base;
+    int n_new = p.req_row_start[req + 1] - row_base;
+    // (this form's step comes from a caller's device numbers, which need not be those that the host was told of)
+    if (GATE == GATE_SCALED) n_new = row_base < 0 ? 0 : max(0, min(n_new, p.n_rows - row_base));
     const int n_rows = n_new * n_rep;
     const int q_tiles = (n_rows + tile_rows - 1) / tile_rows;
     const bool active = rank < q_tiles;
@@ -294,7 +297,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const int min_pos = first_pos + first_tok;
     int key_lo = first_key(p, min_pos);
     key_lo = key_lo / KEYS * KEYS;
-    const int key_end = max_pos + 1;
+    int key_end = max_pos + 1;
+    if (GATE == GATE_SCALED) key_end = min(key_end, max(key_lo + 1, p.table_stride << p.page_shift));
     // kept first tokens: their tiles that lie wholly before the window's first tile come first
     // (those inside it are part of the window's own tiles and only change the mask)
     const int kept_tiles = (active && p.window > 0 && p.keep_first > 0)
@@ -650,7 +654,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             uint2 there[2] = {make_uint2(~0u, ~0u), make_uint2(~0u, ~0u)};
             if (GATE == GATE_SCALED)
                 for (int h = 0; h < 2; ++h)
-                    there[h] = p.seen[(size_t)req * p.table_stride + min((key0 >> 6) + h, p.table_stride - 1)];
+                    there[h] = (key0 >> 6) + h < p.table_stride ? p.seen[(size_t)req * p.table_stride + (key0 >> 6) + h] : make_uint2(0u, 0u);
             ok = wait_all(&s.s_full[b], (j / S_BUFS) & 1);
             if (!ok) break;
             tc::tc_fence_after_sync();
@@ -984,6 +988,7 @@ static int attention_tcgen05(const void* qkv, int qkv_stride, int n_rows, void* 
     p.status = status;
     p.factors = reinterpret_cast<const float2*>(factors);
     p.seen = reinterpret_cast<const uint2*>(seen);
+    p.n_rows = n_rows;
     const int q_tiles = (max_new_tokens * n_rep + p.tile_rows - 1) / p.tile_rows;
     if (n_requests > 65535 || q_tiles > 65535) return CB_ERR_UNSUPPORTED;
     // (single tokens of more than a tile of query heads keep ranks like a portion's)

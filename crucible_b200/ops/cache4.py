@@ -536,7 +536,7 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first, last, counts) ->
     _check(_at(pages.device, build.load("append4").cb_expand4, pages.codes.data_ptr(), pages.scales.data_ptr(), pages.n_pages,
                pages.page_tokens, kv, dim, pages.group, starts, places, batch.table.data_ptr() + 4 * first * batch.stride,
                batch.stride, requests, window or 0, both[0].data_ptr(), both[1].data_ptr(), spans.data_ptr(),
-               factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks), "pages laid out")
+               factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks, rows), "pages laid out")
     code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q.data_ptr(), q.stride(0), rows,
                out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1, starts, places,
                blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, scale, window or 0, factors.data_ptr(),
