@@ -184,6 +184,8 @@ class Batch:
         self.reach = longest if reach is None else reach
         if min(new_tokens) < 1 or min(held_tokens) < 0:
             raise KernelError("a batch's requests bring at least one token each, and hold none or more")
+        if (most * requests if alike else sum(new_tokens)) > self.rows:
+            raise KernelError(f"a batch's requests bring {sum(new_tokens)} tokens, but it has {self.rows} rows")
 
     def _refuse(self):
         t = {"positions": self.positions, "row_request": self.row_request, "row_start": self.row_start,
