@@ -143,7 +143,7 @@ class Batch:
     rows begin, and the position of the first), `table` [requests, pages] (which page of the pool holds a
     request's tokens i * page_tokens onwards).  On the host: how many tokens of every request are
     `new_tokens`, its rows in this step, and `held_tokens`, before them.  A request's rows are consecutive and
-    so are their positions.  Rows behind the last request's are left alone.
+    so are their positions; there are at least as many rows as they bring tokens.  Rows behind the last request's are left alone.
 
     A call that is captured into a graph may be replayed with other numbers on the device, as long as no request brings more rows
     than the most that the host was told of, the same leading requests bring one and, where a request brings more, no request
@@ -507,7 +507,7 @@ def _slabs(batch, window, first, most):
     for r in range(first, batch.requests):
         n = -(-(new[r] + held[r]) // 64)
         if window is not None:
-            n = min(n, (window + new[r] + 62) // 64 + 1)
+            n = min(n, (window + batch.most_new + 62) // 64 + 1)     # (a replayed request may bring as many rows as any)
         if total + n > most:
             if counts:
                 yield first, r, counts
