@@ -366,6 +366,11 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         _walk(q, out, n_heads, scale, batch, pages, window, None, behind, batch.requests)
 
 
+def _most_rows(batch, first, last) -> int:
+    """Rows that a launch over the requests first .. last - 1 takes of each: as many as a replay may bring there."""
+    return 1 if last <= batch.lead else batch.most_new
+
+
 def _resident(dim: int, group: int, columns: int, f32: bool) -> int:
     """Blocks of the walking kernel that the SMs hold at once."""
     return tensor_core.N_SMS * (2 if dim > 128 or columns > 1 else 4 if dim // group * (2 if f32 else 1) <= 2 else 3)
@@ -451,7 +456,7 @@ def _walk(q, out, n_heads, scale, batch, pages, window, picks, first, last) -> N
         per = blocks * kv * -(-n_rep // (8 * columns))
         shares, stream, _ = _dealt_to(dim, pages.group, f32, columns, per, tiles, tiles * per)
     else:
-        most_rows = batch.most_new if last - first == batch.requests else max(batch.new_tokens[first:last])
+        most_rows = _most_rows(batch, first, last)
         columns, shares, stream, _ = _dealt(dim, kv, n_rep, pages.group, f32, batch, window, first, last)
     partial = torch.empty(stream * 16 * columns * (dim + 2), dtype=_F32, device=q.device) if stream else None
     lib = build.load(f"attention4_{dim}")
@@ -541,7 +546,7 @@ def _tiles(q, out, n_heads, scale, batch, pages, window, first, last, counts) ->
                factors.data_ptr(), seen.data_ptr(), blocks.data_ptr(), stride, n_blocks, rows), "pages laid out")
     code = _at(pages.device, build.load("attention_tcgen05").cb_attention_tcgen05_half, q.data_ptr(), q.stride(0), rows,
                out.data_ptr(), out.stride(0), both[0].data_ptr(), both[1].data_ptr(), n_blocks + 1, starts, places,
-               blocks.data_ptr(), stride, requests, max(new), n_heads, kv, dim, scale, window or 0, factors.data_ptr(),
+               blocks.data_ptr(), stride, requests, _most_rows(batch, first, last), n_heads, kv, dim, scale, window or 0, factors.data_ptr(),
                seen.data_ptr(), _status(pages.device))
     if code == build.UNSUPPORTED:
         return False

@@ -58,3 +58,16 @@ def test_rows_that_move_between_requests_in_a_window(monkeypatch):
     graph, q, out = _captured(case, 79)
     for requests in ([(461, 52), (560, 112)], [(600, 114), (640, 50)], [(63, 100), (1, 64)], [(636, 114), (703, 50)], [(0, 1), (0, 1)]):
         _check(case, graph, q, out, requests, 79)
+
+
+@pytest.mark.parametrize("blocks", [3, 1])
+def test_rows_that_move_between_requests_laid_out_one_at_a_time(blocks, monkeypatch):
+    """Requests that are laid out, or (one alone has more blocks than that) walked, by themselves: one that brought few rows at the
+    capture brings as many as the most now."""
+    from crucible_b200.ops import cache4
+    monkeypatch.setattr(cache4, "LAID_OUT", True)
+    monkeypatch.setattr(cache4, "_MOST_BLOCKS", blocks * 64)
+    case = cc.Case([(70, 40), (0, 110)], dim=64, group=64, n_rep=2, kv_heads=1, page=16, seed=49)
+    graph, q, out = _captured(case, None)
+    for requests in ([(0, 110), (70, 40)], [(5, 75), (20, 75)], [(30, 64), (0, 80)]):
+        _check(case, graph, q, out, requests, None)
