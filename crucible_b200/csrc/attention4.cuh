@@ -383,6 +383,50 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         }
     }
 
+    // Sums of a column are kept relative to 2^off, off = m - eps: m the reference of its scores (log2), at most 8 below the
+    // largest, and 2^eps the scale of p step in float16 (`limit` is eps + 8); `bound` is the step from which eps is too much.
+    float off[NT][2], limit[NT][2], bound[NT][2], sum[NT][2], lows[NT][NG][2], o[MT][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            off[n][c] = -3.0e38f;
+            limit[n][c] = 109.f;
+            bound[n][c] = a4_power(-95);
+            sum[n][c] = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) lows[n][gr][c] = 0.f;
+        }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
+
+    // Codes are 0..15, so that sums over them grow with the keys while results do not: they are differences of these sums and of
+    // the lows'.  The tensor cores cut off what they add below a sum's last bit, 0.3 of it a tile on the mean; over 2,048 tiles
+    // (equal weights, 131,000 keys by one block) results were off by 0.02 of themselves.  So every 64 tiles the part that the
+    // features of a group have in common, taken from the first of them, goes over to the lows, which it nearly cancels: under 0.0005.
+    auto settle = [&]() {
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int gr = 0; gr < NG; ++gr) {
+                        const float x = __shfl_sync(0xffffffffu, o[gr * GROUP / 16][n][c], t);
+                        lows[n][gr][c] = fmaf(x, CODE / 8.f, lows[n][gr][c]);      // (eight lanes' are added at the end)
+#pragma unroll
+                        for (int m = gr * GROUP / 16; m < (gr + 1) * GROUP / 16; ++m) {
+                            o[m][n][c] -= x;
+                            o[m][n][2 + c] = fmaf(x, -16.f, o[m][n][2 + c]);
+                        }
+                    }
+        }
+    };
+
     // ---- the warp's ring ----------------------------------------------------
     const size_t head_row = (size_t)kv * p.page_tokens;
     const uint8_t* const code_src = p.codes + head_row * (D / 2);
@@ -502,6 +546,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         if (++looked == 32) {
             looked = 0;
             look();
+            settle();
         }
     };
     look();
@@ -571,27 +616,6 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) qsum[n][gr][c] = reinterpret_cast<const float*>(smem + L::AT_SUMS)[r * NG + gr];
         }
-
-    // Sums of a column are kept relative to 2^off, off = m - eps: m the reference of its scores (log2), at most 8 below the
-    // largest, and 2^eps the scale of p step in float16 (`limit` is eps + 8); `bound` is the step from which eps is too much.
-    float off[NT][2], limit[NT][2], bound[NT][2], sum[NT][2], lows[NT][NG][2], o[MT][NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            off[n][c] = -3.0e38f;
-            limit[n][c] = 109.f;
-            bound[n][c] = a4_power(-95);
-            sum[n][c] = 0.f;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) lows[n][gr][c] = 0.f;
-        }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[m][n][i] = 0.f;
 
     // ---- over the keys -----------------------------------------------------------
     // A pair of tiles.  EDGE: some row may not see some key of it (the four runs' first keys, -1 for none).
