@@ -98,7 +98,7 @@ class CacheStorage:
 
 class CacheStorage4:
     """Device pages of one cache group in 4 bits (`ops.cache4`): a pool a slot, keys and values of one size.
-    `attend_pages`: how many pages a request that brings a single token attends to (None: all)."""
+    `attend_pages`: how many pages a decoded token attends to (None: all)."""
 
     in_4_bits = True
 
@@ -259,6 +259,7 @@ class HostStep:
     first_pos: List[int]             # per request: position of its first new token
     context_len: List[int]           # per request: tokens held after this step
     state_slots: List[int]
+    picking: Optional[int] = None    # how many requests at the step's head attend to picked pages (None: nobody picks)
 
     @cached_property
     def all_single_token(self) -> bool:
@@ -322,8 +323,9 @@ class HostStep:
         shape may depend on: the most new tokens of a request, the number of leading
         single-token requests, and the context buckets (`context_reach`) of the requests that may run
         split over their keys (all of them when every request brings few tokens; the
-        leading single-token ones otherwise).  Steps with equal keys launch the same
+        leading single-token ones otherwise), and how many requests pick pages.  Steps with equal keys launch the same
         kernels with the same grids."""
         small = self.max_new_tokens <= self.SMALL_STEP_TOKENS
         return (self.max_new_tokens, self.lead_single,
-                self.context_reach if small else 0, self.lead_context_reach)
+                self.context_reach if small else 0, self.lead_context_reach) + (
+                    () if self.picking is None else (self.picking,))

@@ -62,6 +62,12 @@ class StepEntry:
     request: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=tuple)   # places among `tokens`
+    prompt: bool = False      # a portion of a prompt: with `attend_pages`, one that is a single token
+                              # attends to all it sees, too (so that how a prompt is cut changes nothing)
+
+    @property
+    def decoded(self) -> bool:
+        return not self.prompt and len(self.tokens) == 1
 
 
 class _Choice:
@@ -79,6 +85,17 @@ class _Choice:
 
 class StepError(ValueError):
     pass
+
+
+class _InOrder:
+    """Ids on their way to the host, of entries that ran in another order."""
+
+    def __init__(self, ids, places):
+        self._ids, self._places = ids, places
+
+    def get(self) -> List[int]:
+        ids = self._ids.get()
+        return [ids[i] for i in self._places]
 
 
 # As the only token of an entry: "the token the engine last chose for this request",
@@ -99,8 +116,8 @@ class EngineOptions:
                                           # for a design that names none, what the page pool holds
     cache_group: Optional[int] = None     # keys and values in 4 bits, by groups of so many features (32, 64
                                           # or 128); None: in the engine's dtype
-    attend_pages: Optional[int] = None    # with cache_group: a request that brings one token attends to so
-                                          # many of its pages, the first, the last two and the others by a bound on their logits
+    attend_pages: Optional[int] = None    # with cache_group: a decoded token (one that is no portion of a prompt) attends to
+                                          # so many of its pages, the first, the last two and the others by a bound on their logits
 
 
 class Engine:
@@ -331,6 +348,11 @@ class Engine:
         the previous step need not visit the host; the entries' own ids are
         then placeholders and are not validated against it)."""
         entries = list(entries)
+        if self.options.attend_pages is not None:
+            # (pages are picked for the step's first rows: decoded tokens go ahead, wherever their entries stand)
+            order = sorted(range(len(entries)), key=lambda i: not entries[i].decoded)
+            if order != list(range(len(entries))):
+                return self._step_in_order(entries, order, token_source, _choose)
         self._validate(entries)
         cache = self.cache
         n_req = len(entries)
@@ -391,6 +413,26 @@ class Engine:
         if choice is None:
             return logits
         return logits, self._get_sampler().collect(choice.ids, len(choice.slots_key), choice)
+
+    def _step_in_order(self, entries, order, token_source, choose):
+        """`step` with the entries in this order; the results are in the entries' own."""
+        def parts(counts):
+            # (of each entry's items, one behind the other: where they stand in that order, and the other way round)
+            at, places = 0, [None] * len(counts)
+            for i in order:
+                places[i] = range(at, at + counts[i])
+                at += counts[i]
+            return [k for p in places for k in p]
+        if token_source is not None:
+            rows = parts([len(e.tokens) for e in entries])
+            source = torch.empty(len(rows), dtype=token_source.dtype, device=token_source.device)
+            source[torch.tensor(rows, device=source.device)] = token_source[:len(rows)]
+            token_source = source
+        result = self.step([entries[i] for i in order], token_source, choose)
+        logits = result[0] if choose else result
+        wanted = torch.tensor(parts([len(e.want) for e in entries]), dtype=torch.int64, device=logits.device)
+        logits = logits.index_select(0, wanted)
+        return (logits, _InOrder(result[1], parts([1] * len(entries)))) if choose else logits
 
     def _choose(self, logits: torch.Tensor, choice: "_Choice") -> None:
         """The argmax of a choosing step, into the choice's own buffers (a captured step keeps
@@ -556,7 +598,8 @@ class Engine:
         if code != 0:
             who = entries[bad.value].request if 0 <= bad.value < n_req else None
             raise StepError(f"request {who!r}: {pack.err.value.decode()}")
-        hs = HostStep([e.request for e in entries], counts, starts, held_after, slots)
+        picking = None if self.options.attend_pages is None else sum(e.decoded for e in entries)
+        hs = HostStep([e.request for e in entries], counts, starts, held_after, slots, picking)
         self._upload_meta(host_t, total)
         return StepContext(layout=layout, meta=dev_t, caches=self.storages, state=self.state,
                            scratch=self.scratch, dtype=self.dtype, host=hs,

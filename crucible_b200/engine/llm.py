@@ -5,8 +5,8 @@ contract).  Option names and meanings follow the reference's command line where
 it has them (`engine/src/main.rs:130-160`, `:476-497`): `max_batch`, `kv_pages`,
 `prefill_chunk_tokens`, `prefill_token_budget`, `max_prefill_requests`, `graph`;
 `profile=True` attributes device time to the model's parts (`engine/profile.py`).
-`cache_group=64` keeps keys and values in 4 bits, `attend_pages=N` with it lets a request that brings one token attend
-to N of its pages (`engine/engine.py`).
+`cache_group=64` keeps keys and values in 4 bits, `attend_pages=N` with it lets a decoded token attend to N of its
+request's pages (`engine/engine.py`).
 """
 from __future__ import annotations
 

@@ -179,7 +179,7 @@ class Scheduler:
         for live, n in plan:
             tokens = live.request.prompt[live.done:live.done + n]
             final = live.done + n == len(live.request.prompt)
-            entries.append(StepEntry(live.request.id, list(tokens), [n - 1] if final else []))
+            entries.append(StepEntry(live.request.id, list(tokens), [n - 1] if final else [], prompt=True))
             if final:
                 sample_rows.append((live, True))
             info.prefill_tokens += n

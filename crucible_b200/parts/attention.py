@@ -101,7 +101,7 @@ class PagedAttention(Mixer):
                 f"not {s.head_dim} in groups of {group}")
 
     def _forward4(self, ctx, h, qkv, cache, binding):
-        """The same over pages in 4 bits; requests that bring one token may attend to some of their pages alone."""
+        """The same over pages in 4 bits; decoded tokens may attend to some of their pages alone."""
         s = self.spec
         t = qkv.shape[0]
         pages, batch = cache.pages(binding.slot), cache4.Batch.of(ctx, binding.group)
@@ -118,8 +118,8 @@ class PagedAttention(Mixer):
         cache4.rope_append4(qkv, q, s.n_heads, cos, sin, batch, pages, write=binding.write)
         out = ctx.scratch("attn.out", (t, self.q_width), self.dtype)
         picks = None
-        if cache.attend_pages is not None and batch.lead:
-            picks = ctx.scratch("attn.picks", (batch.lead, s.n_kv_heads, cache.attend_pages), torch.int32)
+        if cache.attend_pages is not None and ctx.host.picking:
+            picks = ctx.scratch("attn.picks", (ctx.host.picking, s.n_kv_heads, cache.attend_pages), torch.int32)
             cache4.pick_pages4(q, s.n_heads, batch, pages, picks)
         cache4.attention4(q, out, s.n_heads, s.softmax_scale, batch, pages, window=s.window, picks=picks)
         return out

@@ -17,3 +17,32 @@ def test_requests_of_more_tokens_than_there_are_rows():
             _batch(rows, new, [0] * len(new))
     for rows, new in ((3, [1, 2]), (8, [1, 2]), (4, [4]), (3, [1, 1, 1])):
         assert _batch(rows, new, [7] * len(new)).rows == rows
+
+
+def test_portions_of_prompts_are_told_from_decoded_tokens():
+    """However few tokens a portion has left to it, and whatever stands before it in the step."""
+    from crucible_b200.engine.scheduler import Request, Scheduler, SchedulerOptions
+    from test_scheduler import FakeExecutor, greedy
+
+    class Seen(FakeExecutor):
+        def step(self, entries):
+            seen.append([(e.request, len(e.tokens), e.prompt, e.decoded) for e in entries])
+            return super().step(entries)
+    seen = []
+    s = Scheduler(Seen(n_pages=64), SchedulerOptions(max_batch=4, prefill_token_budget=11))
+    s.submit(Request("a", list(range(10)), greedy(4)))
+    s.submit(Request("b", list(range(3)), greedy(4)))
+    s.submit(Request("c", [5], greedy(2)))
+    s.run_to_completion()
+    assert seen[0] == [("a", 10, True, False), ("b", 1, True, False)]
+    assert seen[1] == [("a", 1, False, True), ("c", 1, True, False), ("b", 2, True, False)]
+    assert all(decoded == (not prompt) for step in seen for _, _, prompt, decoded in step)
+    assert sum(n for step in seen for _, n, prompt, _ in step if prompt) == 14
+    assert sum(decoded for step in seen for *_, decoded in step) == 3 + 3 + 1
+
+
+def test_steps_of_unlike_picks_are_captured_apart():
+    from crucible_b200.engine.context import HostStep
+    keys = {HostStep(list("ab"), [1, 1], [20, 9], [21, 10], [0, 1], picking).shape_key() for picking in (None, 0, 1, 2)}
+    assert len(keys) == 4
+    assert HostStep(list("ab"), [1, 1], [20, 9], [21, 10], [0, 1]).shape_key() in keys
