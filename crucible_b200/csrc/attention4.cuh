@@ -709,14 +709,20 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         }
 
         // the references move only when they have to
-        float most_step[2][2];
+        constexpr float LOW = 9.5367431640625e-7f;           // 2^-20
+        float most_step[2][2], most_low[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                // (a low that is 2^20 steps and more counts, too: 2^eps times it has to be far from float32's end)
                 most_step[u][h] = c4_step(vsc[u][h][0]);
+                most_low[u][h] = fabsf(__uint_as_float(vsc[u][h][0]));         // (with the step behind it: next to nothing)
 #pragma unroll
-                for (int gr = 1; gr < NG; ++gr) most_step[u][h] = fmaxf(most_step[u][h], c4_step(vsc[u][h][gr]));
+                for (int gr = 1; gr < NG; ++gr) {
+                    most_step[u][h] = fmaxf(most_step[u][h], c4_step(vsc[u][h][gr]));
+                    most_low[u][h] = fmaxf(most_low[u][h], fabsf(__uint_as_float(vsc[u][h][gr])));
+                }
             }
         bool move = false;
         float top[NT][2], step_top[NT][2];
@@ -731,9 +737,11 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
-                            if (!((hidden >> (4 * NT * u + 4 * n + 2 * h + c)) & 1)) step_top[n][c] = fmaxf(step_top[n][c], most_step[u][h]);
+                            if (!((hidden >> (4 * NT * u + 4 * n + 2 * h + c)) & 1))
+                                step_top[n][c] = fmaxf(step_top[n][c], fmaxf(most_step[u][h], LOW * most_low[u][h]));
                 } else {
                     step_top[n][c] = fmaxf(fmaxf(most_step[0][0], most_step[0][1]), fmaxf(most_step[1][0], most_step[1][1]));
+                    step_top[n][c] = fmaxf(step_top[n][c], LOW * fmaxf(fmaxf(most_low[0][0], most_low[0][1]), fmaxf(most_low[1][0], most_low[1][1])));
                 }
                 move = move || fmaf(top[n][c], factor[n][c], -off[n][c]) > limit[n][c] || step_top[n][c] >= bound[n][c];
             }

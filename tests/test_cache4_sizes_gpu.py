@@ -1,0 +1,31 @@
+"""Attention over the cache in 4 bits: numbers at the ends of what the types hold, and arguments at the ends of theirs."""
+import pytest
+import torch
+
+import cache4_cases as cc
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _attend(case, q, scale, **more):
+    from crucible_b200.ops import cache4
+    out = torch.full((q.shape[0], case.heads * case.dim), 7.0, dtype=q.dtype, device=q.device)
+    cache4.attention4(q, out, case.heads, scale, case.batch, case.pages, **more)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e9, 1e20, 1e30])
+def test_values_without_a_step(size, dtype):
+    """Groups whose numbers are all alike (a step of zero), whatever their size; among them one that is not."""
+    for held, uneven in ((0, False), (700, False), (700, True)):
+        case = cc.Case([(held, 1), (held // 2, 2)], dim=64, group=32, dtype=dtype, seed=61)
+        scales = case.pages.scales[1]
+        scales[..., 0] = 0
+        scales[..., 1] = (size * case.normal(*scales.shape[:-1])).to(BF16)
+        if uneven:
+            scales[int(case.table[0, 30]), :, 5, 1, 0] = 0.25
+        q = case.queries()
+        want, most = case.attention(q, 0.125)
+        cc.assert_attention(_attend(case, q, 0.125), want, most, dtype)
