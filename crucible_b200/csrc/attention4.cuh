@@ -142,6 +142,15 @@ __device__ __forceinline__ float a4_exp2(float x) {
     return r;
 }
 
+// 2^d, d <= 0, as two factors.  Where the scale 2^eps of p step (below) falls from that of values of nothing to that of vast ones,
+// 2^d alone is none that float32 holds, but a sum of weights times both is what it was.
+struct A4Fall {
+    float down, rest;
+    __device__ __forceinline__ explicit A4Fall(float d) : down(a4_exp2(fmaxf(d, -100.f))), rest(a4_exp2(fminf(d + 100.f, 0.f))) {}
+    __device__ __forceinline__ float whole() const { return down * rest; }
+    __device__ __forceinline__ float of(float sum) const { return sum * down * rest; }
+};
+
 __device__ __forceinline__ uint32_t a4_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -754,11 +763,12 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
                     const float st = a4_over_keys_max(step_top[n][c]);
                     const int e = min(max((int)(__float_as_uint(fmaxf(st, bound[n][c] * 0.5f)) >> 23) - 127, -96), 126);
                     const float e5 = 5.f - (float)e, to = m - e5;
-                    const float r = a4_exp2(off[n][c] - to);
+                    const A4Fall fall(off[n][c] - to);
+                    const float r = fall.whole();
                     off[n][c] = to;
                     limit[n][c] = e5 + 8.f;
                     bound[n][c] = a4_power(e + 1);
-                    sum[n][c] *= r;
+                    sum[n][c] = fall.of(sum[n][c]);
 #pragma unroll
                     for (int gr = 0; gr < NG; ++gr) lows[n][gr][c] *= r;
 #pragma unroll
@@ -911,9 +921,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         for (int w = 0; w < A4_WARPS; ++w) top = fmaxf(top, state[(w * L::ROWS + r) * 2]);
 #pragma unroll
         for (int w = 0; w < A4_WARPS; ++w) {
-            const float weight = a4_exp2(state[(w * L::ROWS + r) * 2] - top);
-            l = fmaf(state[(w * L::ROWS + r) * 2 + 1], weight, l);
-            state[(w * L::ROWS + r) * 2] = weight;
+            const A4Fall fall(state[(w * L::ROWS + r) * 2] - top);
+            l += fall.of(state[(w * L::ROWS + r) * 2 + 1]);
+            state[(w * L::ROWS + r) * 2] = fall.whole();
         }
         block_state[r * 2] = top;
         block_state[r * 2 + 1] = l;
@@ -984,9 +994,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
         float v = 0.f, l = 0.f;
 #pragma unroll
         for (int z = 0; z < 8; ++z) {
-            const float weight = a4_exp2(refs[z] - top);
-            v = fmaf(vals[z], weight, v);
-            l = fmaf(ls[z], weight, l);
+            const A4Fall fall(refs[z] - top);
+            v = fmaf(vals[z], fall.whole(), v);
+            l += fall.of(ls[z]);
         }
         store(i, l == 0.f ? 0.f : v / l);
     }
@@ -1051,12 +1061,14 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
             const float2 head = *reinterpret_cast<const float2*>(one + 2 * r);
             const float2 a = *reinterpret_cast<const float2*>(one + 2 * ROWS + r * D + lane * 4);
             const float2 b = *reinterpret_cast<const float2*>(one + 2 * ROWS + r * D + lane * 4 + 2);
-            const float most = fmaxf(top, head.x), was = a4_exp2(top - most), w = a4_exp2(head.x - most);
+            const float most = fmaxf(top, head.x);
+            const A4Fall before(top - most), now(head.x - most);
+            const float was = before.whole(), w = now.whole();
             v.x = fmaf(a.x, w, v.x * was);
             v.y = fmaf(a.y, w, v.y * was);
             v.z = fmaf(b.x, w, v.z * was);
             v.w = fmaf(b.y, w, v.w * was);
-            l = fmaf(head.y, w, l * was);
+            l = now.of(head.y) + before.of(l);
             top = most;
         }
         sums[set][lane] = v;
@@ -1073,9 +1085,9 @@ __global__ void __launch_bounds__(256) attention4_merge_kernel(const Attn4Params
         for (int i = 0; i < SETS; ++i) most = fmaxf(most, refs[i][0]);
 #pragma unroll
         for (int i = 0; i < SETS; ++i) {
-            const float w = a4_exp2(refs[i][0] - most);
-            x = fmaf(reinterpret_cast<const float*>(sums[i])[tid], w, x);
-            l = fmaf(refs[i][1], w, l);
+            const A4Fall fall(refs[i][0] - most);
+            x = fmaf(reinterpret_cast<const float*>(sums[i])[tid], fall.whole(), x);
+            l += fall.of(refs[i][1]);
         }
         const int tok = (unit.base + r) / p.n_rep, head = kv * p.n_rep + (unit.base + r) - tok * p.n_rep;
         reinterpret_cast<T*>(p.out)[(size_t)(unit.row0 + tok) * p.out_stride + (size_t)head * D + tid] =

@@ -29,3 +29,21 @@ def test_values_without_a_step(size, dtype):
         q = case.queries()
         want, most = case.attention(q, 0.125)
         cc.assert_attention(_attend(case, q, 0.125), want, most, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", [1.0, 1e6, 1e12, 1e20, 1e30])
+def test_values_of_nothing_beside_vast_ones(size, dtype, monkeypatch):
+    """Keys whose values are all zero count in the weights, before, between and behind others, in one block or in many."""
+    from crucible_b200.ops import cache4
+    deal = cache4._shares
+    for held, zeros in ((40, (0, 32)), (40, (8, 41)), (300, (0, 128)), (300, (100, 301)), (3000, (0, 1500)), (3000, (1000, 2500))):
+        for dealt in (deal, lambda *a: (1, 0, 1.0), lambda *a: (2, 0, 1.0), lambda *a: (1, 8, 1.0)):
+            monkeypatch.setattr(cache4, "_shares", dealt)
+            case = cc.Case([(held, 1)], dim=64, group=32, dtype=dtype, seed=67)
+            case.pages.scales[1] *= size
+            for j in range(*zeros):
+                case.pages.scales[1, int(case.table[0, j // 16]), :, j % 16] = 0
+            q = case.queries(0.3)
+            want, most = case.attention(q, 0.125)
+            cc.assert_attention(_attend(case, q, 0.125), want, most, dtype)
