@@ -580,7 +580,8 @@ __global__ void __launch_bounds__(A4_WARPS * 32, A4_BLOCKS<D, NG, NT, F32>) atte
             // (100: the factor 2^-e stays far from float32's ends)
             const int e = most > 0.f ? min(13 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
             const float up = a4_power(e);
-            if (lane == 0) factor[r] = p.scale_log2 * a4_power(-e);
+            // (never zero, which a masked score, minus infinity, may not meet)
+            if (lane == 0) factor[r] = fmaxf(p.scale_log2 * a4_power(-e), __int_as_float(1));
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
                 v[i] *= up;

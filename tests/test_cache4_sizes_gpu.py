@@ -47,3 +47,15 @@ def test_values_of_nothing_beside_vast_ones(size, dtype, monkeypatch):
             q = case.queries(0.3)
             want, most = case.attention(q, 0.125)
             cc.assert_attention(_attend(case, q, 0.125), want, most, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("stretch,scale", [(1e-30, 1e-16), (1e-36, 1e-5), (1e-30, 1e-37), (1.0, 1e-37)])
+def test_scores_of_next_to_nothing(stretch, scale, dtype):
+    """Queries times the scale under float32's least number: all keys count alike, masked ones not at all."""
+    case = cc.Case([(200, 1), (90, 2)], dim=64, group=32, dtype=dtype, seed=63)
+    q = case.queries(stretch)
+    want, most = case.attention(q, scale)
+    cc.assert_attention(_attend(case, q, scale), want, most, dtype)
+    want, most = case.attention(q, scale, window=37)
+    cc.assert_attention(_attend(case, q, scale, window=37), want, most, dtype)
