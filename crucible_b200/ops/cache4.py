@@ -45,6 +45,7 @@ GROUPS = (32, 64, 128)
 _HALF_DIMS = tuple(d // 2 for d in HEAD_DIMS)
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 _FLOATS = (_F32, _BF16)
+_LEAST_SCALE = 2.0 ** -126        # (one that float32 holds as a normal number, as it does one over it and either times log2 e)
 
 
 class Pages4:
@@ -327,7 +328,7 @@ def _picks_ok(what: str, picks: torch.Tensor, kv_heads: int) -> None:
 
 def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, batch: Batch, pages: Pages4,
                window: Optional[int] = None, picks: Optional[torch.Tensor] = None) -> None:
-    """out = softmax(scale q . k) v: every row over the keys of its request up to its own position (the last `window` of
+    """out = softmax(scale q . k) v (`scale` from 2^-126 to 2^126): every row over the keys of its request up to its own position (the last `window` of
     them), heads of a group over the same kv head (head h over h // (n_heads / kv heads)).  `q`, `out`: rows [T,
     n_heads * dim] of one type.  A row that sees no key is zero.  `picks` (int32 [rows, kv heads, count], as
     `pick_pages4` leaves them): the pages of the table that a row attends to, each named once, -1 for none; every row is then
@@ -341,8 +342,8 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         raise KernelError(f"attention4: {n_heads} query heads do not share {kv} kv heads evenly")
     if window is not None and window < 1:
         raise KernelError(f"attention4: a window is positive, got {window}")
-    if not 0.0 < scale < float("inf"):
-        raise KernelError(f"attention4: the scale is a positive number, got {scale}")
+    if not _LEAST_SCALE <= scale <= 1.0 / _LEAST_SCALE:
+        raise KernelError(f"attention4: the scale is a positive number from {_LEAST_SCALE:.3g} to {1.0 / _LEAST_SCALE:.3g}, got {scale}")
     behind = 0
     if picks is not None:
         _picks_ok("attention4", picks, kv)

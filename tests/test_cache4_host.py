@@ -46,3 +46,16 @@ def test_steps_of_unlike_picks_are_captured_apart():
     keys = {HostStep(list("ab"), [1, 1], [20, 9], [21, 10], [0, 1], picking).shape_key() for picking in (None, 0, 1, 2)}
     assert len(keys) == 4
     assert HostStep(list("ab"), [1, 1], [20, 9], [21, 10], [0, 1]).shape_key() in keys
+
+
+def test_scales_that_float32_does_not_hold():
+    """Nothing, or infinity, in float32: refused (and before anything is asked of a GPU)."""
+    from crucible_b200.ops import KernelError, cache4
+    pages = cache4.Pages4.new(2, 16, 1, 64, 32, device="cpu")
+    q = torch.zeros(3, 64)
+    for scale in (1e-50, 1e-46, 1e-39, 1e39, 1e300, 3e38):
+        with pytest.raises(KernelError, match="scale"):
+            cache4.attention4(q, q.clone(), 1, scale, _batch(3, [1, 2], [0, 4]), pages)
+    for scale in (2e-38, 1e-20, 1.0, 1e37):
+        with pytest.raises(KernelError, match="CUDA"):
+            cache4.attention4(q, q.clone(), 1, scale, _batch(3, [1, 2], [0, 4]), pages)
