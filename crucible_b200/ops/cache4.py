@@ -45,6 +45,7 @@ GROUPS = (32, 64, 128)
 _HALF_DIMS = tuple(d // 2 for d in HEAD_DIMS)
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 _FLOATS = (_F32, _BF16)
+_MOST_INT = (1 << 31) - 1
 _LEAST_SCALE = 2.0 ** -126        # (one that float32 holds as a normal number, as it does one over it and either times log2 e)
 
 
@@ -342,6 +343,8 @@ def attention4(q: torch.Tensor, out: torch.Tensor, n_heads: int, scale: float, b
         raise KernelError(f"attention4: {n_heads} query heads do not share {kv} kv heads evenly")
     if window is not None and window < 1:
         raise KernelError(f"attention4: a window is positive, got {window}")
+    if window is not None and window > _MOST_INT:          # (more than any position; kernels take 32 bits of it)
+        window = _MOST_INT
     if not _LEAST_SCALE <= scale <= 1.0 / _LEAST_SCALE:
         raise KernelError(f"attention4: the scale is a positive number from {_LEAST_SCALE:.3g} to {1.0 / _LEAST_SCALE:.3g}, got {scale}")
     behind = 0

@@ -59,3 +59,13 @@ def test_scores_of_next_to_nothing(stretch, scale, dtype):
     cc.assert_attention(_attend(case, q, scale), want, most, dtype)
     want, most = case.attention(q, scale, window=37)
     cc.assert_attention(_attend(case, q, scale, window=37), want, most, dtype)
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 62])
+def test_windows_beyond_every_context(window, monkeypatch):
+    from crucible_b200.ops import cache4
+    for laid_out in (False, True):
+        monkeypatch.setattr(cache4, "LAID_OUT", laid_out)
+        case = cc.Case([(100, 40), (0, 30)], dim=64, group=64, n_rep=4, kv_heads=1, seed=65)
+        q = case.queries()
+        assert torch.equal(_attend(case, q, 0.125, window=window), _attend(case, q, 0.125))
