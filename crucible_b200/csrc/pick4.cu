@@ -21,6 +21,7 @@
 namespace {
 
 constexpr int PICK_THREADS = 512;
+constexpr int PICK_ROOM = 220 * 1024;      // bytes of shared memory that scores and queries may take
 
 struct PickParams {
     const void* q;
@@ -257,16 +258,22 @@ __global__ void __launch_bounds__(PICK_THREADS) pick4_kernel(const PickParams p)
 template <int D, typename T>
 int pick_launch(const PickParams& p, int shares, cudaStream_t stream) {
     const size_t bytes = (size_t)p.most_pages * 4 + (size_t)p.n_rep * (2 * D + 4);
-    const int rc = (int)cudaFuncSetAttribute(pick4_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (rc != 0) return rc;
+    // (the limit is the most that any call takes, not this one's: another thread may be between its own and its launch)
+    static bool ready[64] = {};          // per device; setting it twice does no harm
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        const int rc = (int)cudaFuncSetAttribute(pick4_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, PICK_ROOM);
+        if (rc != 0) return rc;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
     return cb_launch_cluster(pick4_kernel<D, T>, dim3((unsigned)p.rows * p.kv_heads, 1, shares), dim3(PICK_THREADS), bytes,
                              stream, shares, p);
 }
 
 }  // namespace
 
-// Bytes of shared memory that scores and queries may take.
-CB_EXPORT int cb_pick4_room() { return 220 * 1024; }
+CB_EXPORT int cb_pick4_room() { return PICK_ROOM; }
 
 CB_EXPORT int cb_pick4(const void* q, int dtype, long long q_stride, const int* positions, const int* row_request,
                        const int* table, int table_stride, int n_requests, const void* bounds, const float* bound_scales,
@@ -274,7 +281,7 @@ CB_EXPORT int cb_pick4(const void* q, int dtype, long long q_stride, const int* 
                        int first, int last, int most_pages, int shares, void* stream) {
     if (rows <= 0) return 0;
     const int padded = (most_pages + 3) / 4 * 4;
-    if ((long long)padded * 4 + (long long)n_rep * (2 * head_dim + 4) > cb_pick4_room() || shares < 1 || shares > 8
+    if ((long long)padded * 4 + (long long)n_rep * (2 * head_dim + 4) > PICK_ROOM || shares < 1 || shares > 8
         || (long long)rows * kv_heads >= (1LL << 31))
         return CB_ERR_UNSUPPORTED;
     const PickParams p = {q, q_stride, positions, row_request, table, table_stride, n_requests,
