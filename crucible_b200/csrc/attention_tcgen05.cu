@@ -884,12 +884,14 @@ template <int HD, int GATE, bool NARROW = false>
 int launch_gate(dim3 grid, cudaStream_t st, const CUtensorMap (&maps)[6], const TcAttnParams& p) {
     constexpr int smem = (int)sizeof(Storage<HD, NARROW>);
     static_assert(smem <= 227 * 1024, "a block's shared memory");
-    static bool configured = false;
-    if (!configured) {
+    static bool configured[64] = {};          // per device; setting it twice does no harm
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
         cudaError_t e = cudaFuncSetAttribute(attention_tcgen05_kernel<HD, GATE, NARROW>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     cb_launch(attention_tcgen05_kernel<HD, GATE, NARROW>, grid, dim3(Storage<HD, NARROW>::THREADS), smem, st, maps[0],
               maps[1], maps[2], maps[3], maps[4], maps[5], p);
