@@ -5,7 +5,7 @@ pair (step, low) and stands for code * step + low.  low is the group's least num
 is (largest - low) * (1 / 15) rounded to bfloat16 (0 if it is under 1e-30), the code is (x - low) * (1 / step)
 rounded to the nearest, ties to even, and held within 0..15; every operation is float32's, rounded once.  A group
 that holds a number that is not finite, or numbers further apart than float32 reaches, stands for NaN.  A number is off by at most half a
-step (and 3 % of one where the rounding of the step cuts the largest off).
+step, as it is rounded (a group's largest number lies up to 15.06 of these above the low).
 
 `rope_append4` rotates q and k of packed rows by their positions and writes k and v to the rows' places;
 `attention4` is causal grouped-query attention over what the pages hold, for single tokens, portions and whole

@@ -59,3 +59,18 @@ def test_scales_that_float32_does_not_hold():
     for scale in (2e-38, 1e-20, 1.0, 1e37):
         with pytest.raises(KernelError, match="CUDA"):
             cache4.attention4(q, q.clone(), 1, scale, _batch(3, [1, 2], [0, 4]), pages)
+
+
+def test_a_number_is_off_by_half_a_step_and_no_more():
+    """Of the step as it is rounded: the largest number of a group, which its rounding may leave 15.06 steps above the low, is
+    within the half, too.  (On top float32's rounding of x - low and of its product with the inverse: 16 steps of 3 * 2^-24.)"""
+    import cache4_cases as cc
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(20000, 128, generator=gen).float().double() * torch.logspace(-6, 6, 20000)[:, None].float().double()
+    x[::3] += 100 * torch.randn(len(x[::3]), 1, generator=gen).float().double() * x[::3].abs().amax(dim=1, keepdim=True)
+    x = x.float().double()
+    for group in (32, 64, 128):
+        code, step, low = cc.coded(x, group)
+        step = step.double().repeat_interleave(group, 1)
+        got = code.double() * step + low.double().repeat_interleave(group, 1)
+        assert bool(((got - x).abs() <= step * (0.5 + 1e-5)).all()), float(((got - x).abs() / step).max())
