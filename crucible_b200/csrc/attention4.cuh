@@ -28,8 +28,8 @@
 //            end and the next one's begin; what a block has of a row tile that it shares with others goes
 //            through memory to a second kernel.  For contexts of unlike lengths and for long ones.
 //
-// 64 tokens of 32 heads of 128 on 8 behind 8,191 keys or fewer, groups of 64: 108 us for 473 MB, 4.4 TB/s (a copy's rate: 72);
-// one behind 131,071 41 us (22), one of 12 heads of 64 behind 700 6.8 (a launch 2).  No unit is full: shifts and masks
+// 64 tokens of 32 heads of 128 on 8 behind 8,191 keys or fewer, groups of 64: 110 us for 473 MB, 4.3 TB/s (a copy's rate: 72);
+// one behind 131,071 41.5 us (22), one of 12 heads of 64 behind 700 6.9 (a launch 2).  No unit is full: shifts and masks
 // 56 %, tensor cores 26 %, memory 54 %, but a scheduler has three to four warps, whose every tile is a chain of copy,
 // product, maximum, product: without the copies 95 us, without the products 90, without any tiles 24 (beginnings,
 // looking for what is whose, putting together).  Without gain: e4m3 codes with k of 32 for the first product (half the
