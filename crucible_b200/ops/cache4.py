@@ -15,8 +15,9 @@ prompts; `pick_pages4` chooses for every row and kv head the pages whose bounds 
 
 Long bfloat16 portions of heads of 64 and 128 go to the tensor cores' tiles in float16, whose waits are bounded and tell of
 running out by the device's status word (`tensor_core.check_status`; a graph that is captured before there is one walks
-instead).  There a value that is no number makes the whole head's
-result none for the rows that see it; elsewhere only its group's features.
+instead).  There a value that is no number makes the whole head's result none for the rows that see it; elsewhere only its
+group's features.  And there the keys of a request and kv head go into float16 by one power of two, as do the values: what is
+more than 2^28 smaller than the largest of them that some row of the step sees loses bits, for the rows before that one, too.
 
 Everything launches on torch's current stream of the tensors' device and may be captured into a CUDA graph; what is
 allocated on the way (partial results of very long contexts, pages laid out anew for long portions, 2 GB at a time at most)

@@ -52,3 +52,21 @@ def test_a_key_that_stands_out_at_every_border(dim, page, window, requests, laid
             # (a result's rounding, 2^-8 of it at most, and p and v at eleven bits)
             error, size = (((t ** 2).view(case.rows, case.heads, dim).mean(dim=2)).sqrt() for t in (got.double() - want, want))
             assert bool((error <= (2.0 ** -8 + 2.0 ** -10) * size).all()), (r, place, float((error / size).max()))
+
+
+@pytest.mark.parametrize("larger", [2.0 ** 10, 2.0 ** 24])
+def test_vast_numbers_at_a_later_position_are_not_noticed_before_it(larger, monkeypatch):
+    """Keys and values go into float16 by a power of two that follows the largest: exactly, within the range that is said."""
+    from crucible_b200.ops import cache4
+    for laid_out in (True, False):
+        monkeypatch.setattr(cache4, "LAID_OUT", laid_out)
+        case = cc.Case([(30, 90), (0, 70)], dim=64, group=32, n_rep=4, kv_heads=2, seed=87)
+        q = case.queries()
+        before = _attend(case, q, 0.125)
+        for place, first in ((100, 70), (119, 89), (75, 45)):           # (the row from which on it is seen)
+            kept = case.pages.scales.clone()
+            case.pages.scales[:, int(case.table[0, place // 16]), :, place % 16] *= larger
+            got = _attend(case, q, 0.125)
+            case.pages.scales.copy_(kept)
+            assert torch.equal(got[:first], before[:first]) and torch.equal(got[90:], before[90:])
+            assert torch.isfinite(got).all() and not torch.equal(got[first:90], before[first:90])
